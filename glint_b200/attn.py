@@ -1,0 +1,297 @@
+"""Serving attention on torch CUDA tensors, through the C ABI of include/glint_attn.h:
+what runs between a decoder's q|k|v and o linears (device.htile).
+
+  attn_prompt   causal attention over packed prompts, grouped heads
+  KV4Cache      a paged key/value cache held in 4 bits (4.5 bits a value in all)
+  kv4_append    new key/value rows into their slots;  kv4_read  slots back to BF16
+  kv4_attn      the newest tokens of each sequence attend to its slots
+  kv4_evict     sequences cut down to a budget of slots, by accumulated weight
+
+As in device.py torch only owns the memory and the stream, there is no CPU fallback,
+bad arguments raise ValueError and a failed call RuntimeError("... rc=N").  Calls are
+stream ordered and may be captured in CUDA graphs.  Tensors live on the current device.
+"""
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+from typing import Optional, Tuple
+
+import torch
+
+from .device import _check, _stream, lib
+
+BLOCK = 64
+_vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+
+
+class _Prompt(ctypes.Structure):
+    """struct GlintAttnPrompt"""
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "o", "lse", "cu_q", "cu_k")] + \
+               [(n, _i64) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "o_tok", "o_head")] + \
+               [(n, _i32) for n in ("seqs", "q_tokens", "k_tokens", "heads", "kv_heads", "head_dim", "causal")] + \
+               [("scale", _f32)]
+
+
+class _Cache(ctypes.Structure):
+    """struct GlintKv4Cache"""
+    _fields_ = [(n, _vp) for n in ("k_code", "k_meta", "v_code", "v_meta")] + \
+               [(n, _i32) for n in ("pages", "kv_heads", "page_size", "head_dim")]
+
+
+class _Attn(ctypes.Structure):
+    """struct GlintKv4Attn"""
+    _fields_ = [(n, _vp) for n in ("q", "o", "lse", "table", "lens", "weight", "weight_out", "work")] + \
+               [(n, _i64) for n in ("q_seq", "q_row", "q_head", "weight_stride")] + \
+               [(n, _i32) for n in ("seqs", "rows", "heads", "max_pages")] + [("scale", _f32)]
+
+
+class _Evict(ctypes.Structure):
+    """struct GlintKv4Evict"""
+    _fields_ = [(n, _vp) for n in ("table", "lens", "weight", "pos", "seen", "kept", "new_lens", "weight_out",
+                                   "pos_out")] + \
+               [("stride", _i64)] + [(n, _i32) for n in ("seqs", "max_pages", "budget", "recent")]
+
+
+def bind(L: ctypes.CDLL) -> ctypes.CDLL:
+    P = ctypes.POINTER
+    L.glint_attn_prompt_stream.argtypes = [P(_Prompt), _vp]
+    L.glint_kv4_append_stream.argtypes = [P(_Cache), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp]
+    L.glint_kv4_read_stream.argtypes = [P(_Cache), _vp, _i32, _vp, _vp, _vp]
+    L.glint_kv4_attn_work_bytes.argtypes = [P(_Cache), P(_Attn)]
+    L.glint_kv4_attn_stream.argtypes = [P(_Cache), P(_Attn), _vp]
+    L.glint_kv4_evict_stream.argtypes = [P(_Cache), P(_Evict), _vp]
+    for f in (L.glint_attn_prompt_stream, L.glint_kv4_append_stream, L.glint_kv4_read_stream,
+              L.glint_kv4_attn_stream, L.glint_kv4_evict_stream):
+        f.restype = _i32
+    L.glint_kv4_attn_work_bytes.restype = _i64
+    return L
+
+
+def _lib() -> ctypes.CDLL:
+    L = lib()
+    if not getattr(L, "_attn_bound", False):
+        bind(L)
+        L._attn_bound = True
+    return L
+
+
+def _on(stream):
+    """Outputs are allocated for the stream that writes them."""
+    return nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[int], ...], dense: bool = True):
+    """A CUDA tensor of this type and shape (None: any size); dense: contiguous,
+    otherwise its last dimension contiguous."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.dim() != len(shape) or any(w is not None and s != w for s, w in zip(t.shape, shape)):
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if dense and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if not dense and t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _head_dim(d: int) -> None:
+    if d not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, not {d}")
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                cu_k: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None):
+    """o [q_tokens, heads, head_dim] BF16 and lse [heads, q_tokens] f32 of packed sequences.
+
+    q [q_tokens, heads, head_dim], k and v [k_tokens, kv_heads, head_dim] BF16, any strides with
+    a contiguous last dimension (views of a fused q|k|v output, for example); cu_q and
+    cu_k [seqs + 1] int32: where each sequence's tokens begin and end (cu_k = cu_q when
+    left out).  Query i of Lq sees keys j <= i + Lk - Lq when causal (the last queries
+    line up with the last keys, so earlier tokens' keys go first), every key otherwise.
+    scale defaults to head_dim ** -0.5.  A row that sees no key gets 0 and -inf."""
+    _want(q, "q", torch.bfloat16, (None, None, None), dense=False)
+    T, H, D = q.shape
+    _head_dim(D)
+    _want(k, "k", torch.bfloat16, (None, None, D), dense=False)
+    Tk, Hk = k.shape[0], k.shape[1]
+    _want(v, "v", torch.bfloat16, (Tk, Hk, D), dense=False)
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({Hk})")
+    _want(cu_q, "cu_q", torch.int32, (None,))
+    if cu_k is None:
+        if Tk != T:
+            raise ValueError("cu_k may be left out only where k has q's tokens")
+        cu_k = cu_q
+    _want(cu_k, "cu_k", torch.int32, (cu_q.shape[0],))
+    if cu_q.shape[0] < 1:
+        raise ValueError("cu_q must have one entry more than there are sequences")
+    with _on(stream):
+        if out is None:
+            out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+        if lse is None:
+            lse = torch.empty((H, T), dtype=torch.float32, device=q.device)
+    _want(out, "out", torch.bfloat16, (T, H, D), dense=False)
+    _want(lse, "lse", torch.float32, (H, T))
+    a = _Prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
+                cu_k.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                out.stride(0), out.stride(1), cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0,
+                D ** -0.5 if scale is None else scale)
+    _check(_lib().glint_attn_prompt_stream(a, _stream(stream)), "glint_attn_prompt_stream")
+    return out, lse
+
+
+class KV4Cache:
+    """One layer's key/value cache in 4 bits, in pages of page_size slots.
+
+    k_code, v_code [pages, kv_heads, page_size, head_dim / 2] uint8 and k_meta, v_meta
+    [pages, kv_heads, page_size, head_dim / 64, 2] BF16 (step, lo): include/glint_attn.h
+    has the layout.  The tensors are the caller's to keep; slots are filled by
+    kv4_append and need no initial value."""
+
+    def __init__(self, k_code: torch.Tensor, k_meta: torch.Tensor, v_code: torch.Tensor, v_meta: torch.Tensor):
+        _want(k_code, "k_code", torch.uint8, (None, None, None, None))
+        pages, kv_heads, page_size, half = k_code.shape
+        _head_dim(2 * half)
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError(f"page_size must be 16, 32, 64 or 128, not {page_size}")
+        if pages < 1 or kv_heads < 1 or pages * page_size > 2 ** 31 - 1:
+            raise ValueError(f"a cache has between 1 and 2**31 - 1 slots, not {pages} pages of {page_size}")
+        _want(v_code, "v_code", torch.uint8, k_code.shape)
+        for t, name in ((k_meta, "k_meta"), (v_meta, "v_meta")):
+            _want(t, name, torch.bfloat16, (pages, kv_heads, page_size, half // 32, 2))
+        if any(t.data_ptr() % 16 for t in (k_code, k_meta, v_code, v_meta)):
+            raise ValueError("the cache's tensors must be 16-byte aligned")
+        self.k_code, self.k_meta, self.v_code, self.v_meta = k_code, k_meta, v_code, v_meta
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, 2 * half
+        self._c = _Cache(k_code.data_ptr(), k_meta.data_ptr(), v_code.data_ptr(), v_meta.data_ptr(), pages, kv_heads,
+                         page_size, 2 * half)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "KV4Cache":
+        _head_dim(head_dim)
+
+        def code():
+            return torch.empty((pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=device)
+
+        def meta():
+            return torch.empty((pages, kv_heads, page_size, head_dim // BLOCK, 2), dtype=torch.bfloat16, device=device)
+        return cls(code(), meta(), code(), meta())
+
+
+def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
+    """k, v [tokens, kv_heads, head_dim] BF16 (any strides, last dimension contiguous), quantised
+    into slots[t] = page * page_size + place in the page (int32; negative: skipped)."""
+    _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
+    _want(v, "v", torch.bfloat16, tuple(k.shape), dense=False)
+    _want(slots, "slots", torch.int32, (k.shape[0],))
+    _check(_lib().glint_kv4_append_stream(cache._c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+                                          v.stride(0), v.stride(1), slots.data_ptr(), k.shape[0], _stream(stream)),
+           "glint_kv4_append_stream")
+
+
+def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
+             v_out: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [tokens, kv_heads, head_dim] BF16: the values of slots[t] (zeros for a slot outside
+    the cache), for example as attn_prompt's keys of an earlier part of a prompt."""
+    _want(slots, "slots", torch.int32, (None,))
+    shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
+    with _on(stream):
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+    _want(k_out, "k_out", torch.bfloat16, shape)
+    _want(v_out, "v_out", torch.bfloat16, shape)
+    _check(_lib().glint_kv4_read_stream(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
+                                        _stream(stream)), "glint_kv4_read_stream")
+    return k_out, v_out
+
+
+def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor,
+             scale: Optional[float] = None, weight: Optional[torch.Tensor] = None,
+             weight_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+             lse: Optional[torch.Tensor] = None, stream=None):
+    """o (as q, contiguous) and lse [seqs, heads, rows] f32 of each sequence's newest `rows`
+    tokens over its lens[b] cached slots, which end with those tokens' own.
+
+    q [seqs, rows, heads, head_dim] BF16 (any strides, last dimension contiguous); table
+    [seqs, max_pages] int32: the pages of a sequence in order; lens [seqs] int32.  With
+    weight_out [seqs, kv_heads, >= max_pages * page_size] f32 each slot's softmax weights,
+    summed over the head's query heads and rows, are added to weight (zero when left
+    out, and in the newest `rows` slots) and written there; weight_out may be weight."""
+    _want(q, "q", torch.bfloat16, (None, None, None, cache.head_dim), dense=False)
+    B, R, H, D = q.shape
+    if H < 1 or H % cache.kv_heads:
+        raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({cache.kv_heads})")
+    if R < 1 or H // cache.kv_heads * R > 256:
+        raise ValueError(f"rows ({R}) times query heads a kv head must be 1 to 256")
+    _want(table, "table", torch.int32, (B, None))
+    _want(lens, "lens", torch.int32, (B,))
+    wide = 0
+    if weight_out is not None:
+        _want(weight_out, "weight_out", torch.float32, (B, cache.kv_heads, None))
+        wide = weight_out.shape[2]
+        if wide < table.shape[1] * cache.page_size:
+            raise ValueError(f"weight_out must have {table.shape[1] * cache.page_size} slots or more, not {wide}")
+        if weight is not None:
+            _want(weight, "weight", torch.float32, (B, cache.kv_heads, wide))
+    elif weight is not None:
+        raise ValueError("weight needs weight_out")
+    L = _lib()
+    a = _Attn(q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(),
+              None if weight is None else weight.data_ptr(), None if weight_out is None else weight_out.data_ptr(),
+              None, q.stride(0), q.stride(1), q.stride(2), wide, B, R, H, table.shape[1],
+              D ** -0.5 if scale is None else scale)
+    with _on(stream):
+        if out is None:
+            out = torch.empty((B, R, H, D), dtype=torch.bfloat16, device=q.device)
+        if lse is None:
+            lse = torch.empty((B, H, R), dtype=torch.float32, device=q.device)
+        if weight_out is not None:
+            work = torch.empty(max(0, L.glint_kv4_attn_work_bytes(cache._c, a)), dtype=torch.uint8, device=q.device)
+            a.work = work.data_ptr()
+    _want(out, "out", torch.bfloat16, (B, R, H, D))
+    _want(lse, "lse", torch.float32, (B, H, R))
+    a.o, a.lse = out.data_ptr(), lse.data_ptr()
+    _check(L.glint_kv4_attn_stream(cache._c, a, _stream(stream)), "glint_kv4_attn_stream")
+    return out, lse
+
+
+def kv4_evict(cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, weight: torch.Tensor, pos: torch.Tensor,
+              seen: torch.Tensor, budget: int, recent: int = 0, *, weight_out: torch.Tensor, pos_out: torch.Tensor,
+              stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence down to n = min(lens[b], budget) slots, each kv head on its own:
+    kept are the slots with pos >= seen[b] - recent, then the largest weights, ties to
+    the lowest slot; kept slots from n on move into the freed slots below n.
+
+    weight f32 and pos int32 [seqs, kv_heads, >= max_pages * page_size] belong to the
+    slots (pos: the token's position); seen [seqs] int32: tokens seen so far.  weight_out
+    and pos_out get the kept slots' entries and may not be weight and pos themselves
+    (two pairs of tensors that take turns).  Returns
+    (kept [seqs, kv_heads, budget] int32: the slot each one came from, -1 from n on;
+    new_lens [seqs] int32)."""
+    B, P = table.shape if table.dim() == 2 else (None, 0)
+    _want(table, "table", torch.int32, (None, None))
+    _want(lens, "lens", torch.int32, (B,))
+    _want(seen, "seen", torch.int32, (B,))
+    _want(weight, "weight", torch.float32, (B, cache.kv_heads, None))
+    wide = weight.shape[2]
+    _want(pos, "pos", torch.int32, (B, cache.kv_heads, wide))
+    if budget < 1 or recent < 0 or recent > budget:
+        raise ValueError("budget must be 1 or more and recent between 0 and budget")
+    if P < 1 or P * cache.page_size > min(wide, 524288):
+        raise ValueError(f"table has room for {P * cache.page_size} slots: weight must cover them, 524288 at most")
+    with _on(stream):
+        kept = torch.empty((B, cache.kv_heads, budget), dtype=torch.int32, device=table.device)
+        new_lens = torch.empty((B,), dtype=torch.int32, device=table.device)
+    _want(weight_out, "weight_out", torch.float32, tuple(weight.shape))
+    _want(pos_out, "pos_out", torch.int32, tuple(pos.shape))
+    if weight_out.data_ptr() == weight.data_ptr() or pos_out.data_ptr() == pos.data_ptr():
+        raise ValueError("weight_out and pos_out must not be weight and pos")
+    e = _Evict(table.data_ptr(), lens.data_ptr(), weight.data_ptr(), pos.data_ptr(), seen.data_ptr(), kept.data_ptr(),
+               new_lens.data_ptr(), weight_out.data_ptr(), pos_out.data_ptr(), wide, B, P, budget, recent)
+    _check(_lib().glint_kv4_evict_stream(cache._c, e, _stream(stream)), "glint_kv4_evict_stream")
+    return kept, new_lens
