@@ -250,12 +250,10 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
             out = torch.empty((B, R, H, D), dtype=torch.bfloat16, device=q.device)
         if lse is None:
             lse = torch.empty((B, H, R), dtype=torch.float32, device=q.device)
-        if weight_out is not None:
-            work = torch.empty(max(0, L.glint_kv4_attn_work_bytes(cache._c, a)), dtype=torch.uint8, device=q.device)
-            a.work = work.data_ptr()
+        work = torch.empty(max(0, L.glint_kv4_attn_work_bytes(cache._c, a)), dtype=torch.uint8, device=q.device)
     _want(out, "out", torch.bfloat16, (B, R, H, D))
     _want(lse, "lse", torch.float32, (B, H, R))
-    a.o, a.lse = out.data_ptr(), lse.data_ptr()
+    a.o, a.lse, a.work = out.data_ptr(), lse.data_ptr(), work.data_ptr()
     _check(L.glint_kv4_attn_stream(cache._c, a, _stream(stream)), "glint_kv4_attn_stream")
     return out, lse
 

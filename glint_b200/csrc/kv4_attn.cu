@@ -1,9 +1,23 @@
 /* Attention of a sequence's newest tokens over its 4-bit cache.
  *
- * One warp per query row: a lane holds D / 32 neighbouring values of q and of the
- * output, each slot's score is a shuffle sum, and the running maximum and sum of the
- * softmax rescale the output as they change.  Simple and right for every case; the
- * cache is read once per query head.
+ * The rows of one kv head (its query heads times the new tokens, 8 or 16 at a time: the
+ * columns of a tensor-core tile) share every byte of the cache that is read.  With
+ * x = lo + step * code for K and V, per 64-value block b of a slot t:
+ *
+ *   s[t, n] = sum_b step (sum_d (code - 8) q[n, d]) + (lo + 8 step) (sum_d q[n, d])
+ *   o[d, n] = sum_t (code - 8) (p[t, n] step)       + sum_t p[t, n] (lo + 8 step)
+ *
+ * so the products are mma.sync tiles whose A operand is the codes themselves: (w &
+ * 0x000F000F) | 0x43004300 is the BF16 pair 128 + code, less 136 it is code - 8, exact.
+ * The tile's inner index may be any order that both operands share, so a 32-bit word's
+ * nibbles j and j + 4 make a pair as they lie.  For K (rows = slots, inner = d) q is
+ * permuted to match once; for V (rows = d, inner = slots) a pair is the same nibble of
+ * two slots, two byte permutes for eight pairs.  p * step is rounded to BF16 (2^-9 of
+ * each weight, the rounding any BF16 tensor-core attention makes); scores, maximum,
+ * sums and the lo terms stay in f32.
+ *
+ * Bound: HBM (D + D / 8 bytes a slot and head at 4.5 bits a value) as long as the
+ * unpacking keeps up: about 2.2 ALU operations a byte.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -11,141 +25,691 @@
 #include <algorithm>
 
 #include "kv4.cuh"
+#include "ptx.cuh"
 
 namespace glint {
+static __device__ int g_kv4_error = 0, g_kv4_error_taken = 0;
+int kv4_error_word(bool clear) { return read_error_word(g_kv4_error, g_kv4_error_taken, clear); }
+
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kTile = 32;        /* slots a warp takes at a time */
+constexpr float kLazy = 8.f;     /* the running maximum may lag by 2^8 */
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+/* Two columns sets at most: 8 columns take 16 warps of 128 registers, 16 take 8 warps
+ * of up to 255 (their accumulators are twice as many). */
+template <int D, int NT>
+struct Cfg {
+    static constexpr int kWarps = NT == 1 ? 16 : 8;
+    static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kNb = D / 64;
+    static constexpr int kCode = kTile * D / 2, kMeta = kTile * kNb * 4;
+    static constexpr int kStage = 2 * (kCode + kMeta);
+    static constexpr int kState = kCols * D + 2 * kCols; /* floats: O, m, l */
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kSmem = kRing + kWarps * kState * 4 + kWarps * kStages * 16 + kWarps * 4 + 16;
+};
 
 struct Args {
     GlintKv4Cache c;
     GlintKv4Attn a;
+    int group, cols;      /* query heads a kv head; group * rows */
+    int chunks, segs;     /* column chunks a kv head; segments a sequence = kv_heads * chunks */
+    int parts;            /* grid of the attention kernel */
+    int min_units;        /* tiles a CTA takes at least */
+    float *part;          /* [parts][2][kState] unfinished segments */
+    float *score;         /* [seqs][kv_heads][max slots][cols] log2-scaled scores, or NULL */
+    float *lse2;          /* [seqs][kv_heads][cols] log2 sums, with score */
 };
 
-/* lane's D / 32 values of one row */
-template <int D>
-__device__ __forceinline__ void row_values(const uint8_t *code, const uint16_t *meta, int64_t at, int t, int lane,
-                                           float (&x)[D / 32])
+__device__ __forceinline__ float ex2(float x)
 {
-    const int e = lane * (D / 32);
-    const int64_t byte = at * (D / 2) + kv4_unit<D>(e / 64, t) + (e % 64) / 2;
-    uint32_t w = D == 128 ? *reinterpret_cast<const uint16_t *>(code + byte) : code[byte];
-    const uint32_t m = reinterpret_cast<const uint32_t *>(meta)[at * (D / 64) + e / 64];
-    const float step = __uint_as_float(m << 16), lo = __uint_as_float(m & 0xFFFF0000u);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        x[i] = fmaf(step, (float)((w >> (4 * i)) & 15u), lo);
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-
-/* index of slot t's row (head h of sequence b), -1 where its page is outside the cache */
-__device__ __forceinline__ int64_t row_of(const Args &g, int b, int h, int t)
-{
-    const int p = g.a.table[(int64_t)b * g.a.max_pages + t / g.c.page_size];
-    if (p < 0 || p >= g.c.pages)
-        return -1;
-    return ((int64_t)p * g.c.kv_heads + h) * g.c.page_size + t % g.c.page_size;
-}
-
 __device__ __forceinline__ int length_of(const Args &g, int b)
 {
     return min(max(g.a.lens[b], 0), g.a.max_pages * g.c.page_size);
 }
+__device__ __forceinline__ int tiles_of(const Args &g, int b) { return (length_of(g, b) + kTile - 1) / kTile; }
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32) kv4_attn_kernel(const Args g)
+/* The tiles of all segments in one row (sequence, then segment, then tile), cut into
+ * equal ranges over the CTAs: sequences of any mix of lengths keep every SM busy. */
+struct Plan {
+    int64_t units;
+    int parts;
+    __device__ __forceinline__ int64_t begin(int i) const { return units * i / parts; }
+    __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * parts - 1) / units); }
+};
+__device__ __forceinline__ Plan plan_of(const Args &g)
 {
     const int lane = threadIdx.x & 31;
-    const int64_t wq = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-    const int heads = g.a.heads, rows = g.a.rows;
-    if (wq >= (int64_t)g.a.seqs * rows * heads)
-        return;
-    const int b = (int)(wq / (rows * heads)), r = (int)(wq / heads % rows), hq = (int)(wq % heads);
-    const int h = hq / (heads / g.c.kv_heads);
-    const int seen = length_of(g, b) - rows + r + 1;
-    float q[D / 32], o[D / 32] = {}, m = -INFINITY, l = 0.f;
+    int64_t n = 0;
+    for (int b = lane; b < g.a.seqs; b += 32)
+        n += tiles_of(g, b);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        q[i] = __bfloat162float(g.a.q[b * g.a.q_seq + r * g.a.q_row + hq * g.a.q_head + lane * (D / 32) + i]);
-    for (int t = 0; t < seen; ++t) {
-        const int64_t at = row_of(g, b, h, t);
-        if (at < 0)
-            continue;
-        float x[D / 32], s = 0.f;
-        row_values<D>(g.c.k_code, g.c.k_meta, at, t, lane, x);
+    for (int off = 16; off > 0; off >>= 1)
+        n += __shfl_xor_sync(0xFFFFFFFFu, n, off);
+    Plan p;
+    p.units = n * g.segs;
+    p.parts = (int)max((int64_t)1, min((int64_t)g.parts, p.units / g.min_units));
+    return p;
+}
+/* a place in that row */
+struct At {
+    int b, seg, tile, tiles;
+    int64_t seg_begin; /* unit of the segment's first tile */
+};
+__device__ __forceinline__ At locate(const Args &g, int64_t u) /* u < units; whole warp */
+{
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 32) {
+        const int b = b0 + lane;
+        const int t = b < g.a.seqs ? tiles_of(g, b) : 0;
+        int64_t s = t;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-            s = fmaf(q[i], x[i], s);
-        s = warp_sum(s) * g.a.scale;
-        const float top = fmaxf(m, s);
-        const float keep = m == -INFINITY ? 0.f : expf(m - top), p = s == -INFINITY ? 0.f : expf(s - top);
-        row_values<D>(g.c.v_code, g.c.v_meta, at, t, lane, x);
-        l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-            o[i] = fmaf(p, x[i], o[i] * keep);
-        m = top;
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        g.a.o[wq * D + lane * (D / 32) + i] = __float2bfloat16_rn(o[i] * inv);
-    const int64_t li = ((int64_t)b * heads + hq) * rows + r;
-    float *lse = reinterpret_cast<float *>(g.a.work);
-    if (lane == 0) {
-        const float v = l == 0.f ? -INFINITY : m + logf(l);
-        if (g.a.lse)
-            g.a.lse[li] = v;
-        if (lse)
-            lse[li] = v;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t o = __shfl_up_sync(0xFFFFFFFFu, s, off);
+            if (lane >= off)
+                s += o;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, (before + s) * g.segs > u);
+        if (past || b0 + 32 >= g.a.seqs) {
+            const int l = past ? __ffs(past) - 1 : 31;
+            At at;
+            at.b = b0 + l;
+            at.tiles = __shfl_sync(0xFFFFFFFFu, t, l);
+            const int64_t first = (before + __shfl_sync(0xFFFFFFFFu, s, l) - at.tiles) * g.segs;
+            at.seg = at.tiles ? (int)((u - first) / at.tiles) : 0;
+            at.seg_begin = first + (int64_t)at.seg * at.tiles;
+            at.tile = (int)(u - at.seg_begin);
+            return at;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
 }
 
-/* weight_out: a thread per slot, the rows and heads of its group in order */
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32) kv4_weight_kernel(const Args g)
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    const int h = blockIdx.y, b = blockIdx.z, t = blockIdx.x * kWarps * 32 + threadIdx.x;
-    const int len = length_of(g, b), group = g.a.heads / g.c.kv_heads;
-    if (t >= len)
-        return;
-    const int64_t at = row_of(g, b, h, t);
-    const float *lse = reinterpret_cast<const float *>(g.a.work);
-    float sum = 0.f;
-    if (at >= 0) {
-        for (int j = 0; j < group; ++j) {
-            const int hq = h * group + j;
-            for (int r = 0; r < g.a.rows; ++r) {
-                const float z = lse[((int64_t)b * g.a.heads + hq) * g.a.rows + r];
-                if (t >= len - g.a.rows + r + 1 || z == -INFINITY)
-                    continue;
-                const __nv_bfloat16 *q = g.a.q + b * g.a.q_seq + r * g.a.q_row + hq * g.a.q_head;
-                float s = 0.f;
-                for (int e = 0; e < D; ++e) {
-                    const uint32_t w = g.c.k_code[at * (D / 2) + kv4_unit<D>(e / 64, t) + (e % 64) / 2];
-                    const uint32_t m = reinterpret_cast<const uint32_t *>(g.c.k_meta)[at * (D / 64) + e / 64];
-                    const float x = fmaf(__uint_as_float(m << 16), (float)((w >> (4 * (e & 1))) & 15u),
-                                         __uint_as_float(m & 0xFFFF0000u));
-                    s = fmaf(__bfloat162float(q[e]), x, s);
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+/* nibbles j and j + 4 of w as the BF16 pair (code - 8, code - 8) */
+__device__ __forceinline__ uint32_t codes(uint32_t w, int j)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w >> (4 * j)), "r"(0x43004300u));
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&r), __floats2bfloat162_rn(136.f, 136.f));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+/* slot (of 8) that row r of a tile stands for: with the swapped halves, the four slots
+ * of any fragment load (rows 0-3, rows 4-7, even rows, odd rows) differ mod 4 */
+__device__ __forceinline__ int slot_of(int r) { return (r & 4) | (((r ^ (r >> 2)) & 1) << 1) | ((r >> 1) & 1); }
+
+/* A warp's running softmax over the slots it has seen, as tile fragments: lane (g, c) =
+ * (lane / 4, lane % 4) holds columns 2c, 2c + 1 of m, l and, per 64-block b and j < 4,
+ * o at d = 64 b + 8 g + j (values 0, 1) and + 4 (values 2, 3). */
+template <int D, int NT>
+struct State {
+    float o[NT][D / 64][4][4];
+    float m[NT][2], l[NT][2], lo[NT][D / 64][2];
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[n][b][j][i] = 0.f;
+                lo[n][b][0] = lo[n][b][1] = 0.f;
+            }
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
+    }
+};
+
+/* q of one segment's columns as B fragments, and its sums per block */
+template <int D, int NT>
+struct Query {
+    uint32_t b[NT][D / 64][4][2];
+    float sum[NT][D / 64][2];
+    int see[NT][2]; /* slots that columns 2c, 2c + 1 see */
+};
+
+template <int D, int NT>
+__device__ __forceinline__ void load_query(const Args &g, int b, int seg, Query<D, NT> &q, int lane)
+{
+    const int h = seg / g.chunks, ch = seg - h * g.chunks;
+    const int gr = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int col = ch * 8 * NT + n * 8 + gr;
+        const bool live = col < g.cols;
+        const int r = live ? col / g.group : 0, hq = h * g.group + (live ? col - r * g.group : 0);
+        const __nv_bfloat16 *p = g.a.q + b * g.a.q_seq + r * g.a.q_row + hq * g.a.q_head + 16 * c;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            uint32_t v[16];
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] = live ? (uint32_t)__bfloat16_as_ushort(p[64 * k + i]) : 0u;
+                s += __uint_as_float(v[i] << 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                q.b[n][k][j][0] = v[j] | (v[j + 4] << 16);
+                q.b[n][k][j][1] = v[j + 8] | (v[j + 12] << 16);
+            }
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+            q.sum[n][k][0] = __shfl_sync(0xFFFFFFFFu, s, 8 * c);
+            q.sum[n][k][1] = __shfl_sync(0xFFFFFFFFu, s, 8 * c + 4);
+        }
+        const int len = length_of(g, b);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int cc = ch * 8 * NT + n * 8 + 2 * c + i;
+            q.see[n][i] = cc < g.cols ? len - g.a.rows + cc / g.group + 1 : len;
+        }
+    }
+}
+
+/* One tile of 32 slots (from slot t0) in shared memory. */
+template <int D, int NT, bool SCORE>
+__device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, State<D, NT> &st, uint32_t stage,
+                                          int t0, uint32_t valid, bool whole, float scale2, float *score, int chunk,
+                                          int lane)
+{
+    using C = Cfg<D, NT>;
+    constexpr int NB = D / 64, RB = D / 2;
+    const int gr = lane >> 2, c = lane & 3;
+    const int tg = slot_of(gr);
+    const uint32_t kcode = stage, kmeta = stage + C::kCode, vcode = kmeta + C::kMeta, vmeta = vcode + C::kCode;
+    float s[2][NT][4];
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl) {
+        const int ta = sl * 16 + tg, tb = ta + 8; /* slots of fragment rows g and g + 8 */
+        float acc[NB][NT][4];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[k][n][i] = 0.f;
+            const uint2 wa = lds64(kcode + ta * RB + kv4_unit<D>(k, ta) + 8 * c);
+            const uint2 wb = lds64(kcode + tb * RB + kv4_unit<D>(k, tb) + 8 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t a[4] = {codes(wa.x, j), codes(wb.x, j), codes(wa.y, j), codes(wb.y, j)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    mma(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[sl][n][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const uint32_t ma = lds32(kmeta + (ta * NB + k) * 4), mb = lds32(kmeta + (tb * NB + k) * 4);
+            const float sa = __uint_as_float(ma << 16), sb = __uint_as_float(mb << 16);
+            const float la = fmaf(8.f, sa, __uint_as_float(ma & 0xFFFF0000u));
+            const float lb = fmaf(8.f, sb, __uint_as_float(mb & 0xFFFF0000u));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[sl][n][0] = fmaf(sa, acc[k][n][0], fmaf(la, q.sum[n][k][0], s[sl][n][0]));
+                s[sl][n][1] = fmaf(sa, acc[k][n][1], fmaf(la, q.sum[n][k][1], s[sl][n][1]));
+                s[sl][n][2] = fmaf(sb, acc[k][n][2], fmaf(lb, q.sum[n][k][0], s[sl][n][2]));
+                s[sl][n][3] = fmaf(sb, acc[k][n][3], fmaf(lb, q.sum[n][k][1], s[sl][n][3]));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = i < 2 ? ta : tb;
+                s[sl][n][i] *= scale2;
+                if (!whole && (!((valid >> t) & 1u) || t0 + t >= q.see[n][i & 1]))
+                    s[sl][n][i] = -INFINITY;
+            }
+        if constexpr (SCORE) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int col = chunk * 8 * NT + n * 8 + 2 * c;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float *p = score + (int64_t)(t0 + (i ? tb : ta)) * g.cols + col;
+                    if ((valid >> (i ? tb : ta)) & 1u) {
+                        if (col < g.cols)
+                            p[0] = s[sl][n][2 * i];
+                        if (col + 1 < g.cols)
+                            p[1] = s[sl][n][2 * i + 1];
+                    }
                 }
-                sum += expf(s * g.a.scale - z);
             }
         }
     }
-    const int64_t i = ((int64_t)b * g.c.kv_heads + h) * g.a.weight_stride + t;
-    const float old = g.a.weight && t < len - g.a.rows ? g.a.weight[i] : 0.f;
-    g.a.weight_out[i] = old + sum;
+    /* running maximum per column, over the 8 lanes that share it */
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float top[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(fmaxf(s[0][n][i], s[0][n][i + 2]), fmaxf(s[1][n][i], s[1][n][i + 2]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1)
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], off));
+        }
+        const bool grow = top[0] > st.m[n][0] + kLazy || top[1] > st.m[n][1] + kLazy ||
+                          (st.m[n][0] == -INFINITY && top[0] != -INFINITY) ||
+                          (st.m[n][1] == -INFINITY && top[1] != -INFINITY);
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float m = fmaxf(st.m[n][i], top[i]);
+                const float f = st.m[n][i] == -INFINITY ? 0.f : ex2(st.m[n][i] - m);
+                st.m[n][i] = m;
+                st.l[n][i] *= f;
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    st.lo[n][k][i] *= f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        st.o[n][k][j][i] *= f, st.o[n][k][j][i + 2] *= f;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl) {
+        const int ta = sl * 16 + tg, tb = ta + 8;
+        uint32_t pb[NT][NB][2];
+        float steps[NB][2], mids[NB][2];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const uint32_t ma = lds32(vmeta + (ta * NB + k) * 4), mb = lds32(vmeta + (tb * NB + k) * 4);
+            steps[k][0] = __uint_as_float(ma << 16), steps[k][1] = __uint_as_float(mb << 16);
+            mids[k][0] = fmaf(8.f, steps[k][0], __uint_as_float(ma & 0xFFFF0000u));
+            mids[k][1] = fmaf(8.f, steps[k][1], __uint_as_float(mb & 0xFFFF0000u));
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float m = st.m[n][i & 1];
+                p[i] = ex2(s[sl][n][i] - (m == -INFINITY ? 0.f : m));
+                st.l[n][i & 1] += p[i];
+            }
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                float w[4], x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = p[i] * steps[k][i >> 1], x[i] = p[i] * mids[k][i >> 1];
+                    /* a masked slot's step and lo may be anything, NaN too */
+                    if (!whole && s[sl][n][i] == -INFINITY)
+                        w[i] = x[i] = 0.f;
+                }
+                st.lo[n][k][0] += x[0] + x[2];
+                st.lo[n][k][1] += x[1] + x[3];
+                pb[n][k][0] = transpose8x8(pack2(w[0], w[1]));
+                pb[n][k][1] = transpose8x8(pack2(w[2], w[3]));
+            }
+        }
+        const int te = sl * 16 + slot_of(2 * c), to = sl * 16 + slot_of(2 * c + 1); /* inner 2c, 2c + 1; + 8 */
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const uint32_t w0 = lds32(vcode + te * RB + kv4_unit<D>(k, te) + 4 * gr);
+            const uint32_t w1 = lds32(vcode + to * RB + kv4_unit<D>(k, to) + 4 * gr);
+            const uint32_t w2 = lds32(vcode + (te + 8) * RB + kv4_unit<D>(k, te + 8) + 4 * gr);
+            const uint32_t w3 = lds32(vcode + (to + 8) * RB + kv4_unit<D>(k, to + 8) + 4 * gr);
+            const uint32_t x0 = __byte_perm(w0, w1, 0x5410), y0 = __byte_perm(w0, w1, 0x7632);
+            const uint32_t x1 = __byte_perm(w2, w3, 0x5410), y1 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t a[4] = {codes(x0, j), codes(y0, j), codes(x1, j), codes(y1, j)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    mma(st.o[n][k][j], a, pb[n][k][0], pb[n][k][1]);
+            }
+        }
+    }
 }
 
-template <int D>
-int launch(const Args &g, cudaStream_t st)
+/* where a warp's next tile to fetch lies, and the pages that hold it */
+struct Fetch {
+    int b, seg, tile, tiles;
+    int page; /* lanes 0 and 1: the page of the tile's slots 0-15 and 16-31, -1 for none */
+};
+__device__ __forceinline__ void fetch_page(const Args &g, Fetch &f, int lane)
 {
-    const int64_t n = (int64_t)g.a.seqs * g.a.rows * g.a.heads;
-    kv4_attn_kernel<D><<<(unsigned)((n + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(g);
-    if (g.a.weight_out) {
-        const int cap = g.a.max_pages * g.c.page_size;
-        kv4_weight_kernel<D><<<dim3((cap + kWarps * 32 - 1) / (kWarps * 32), g.c.kv_heads, g.a.seqs), kWarps * 32, 0, st>>>(g);
+    const int t = f.tile * kTile + 16 * lane;
+    f.page = -1;
+    if (lane < 2 && f.tiles > 0 && t < length_of(g, f.b))
+        f.page = g.a.table[(int64_t)f.b * g.a.max_pages + t / g.c.page_size];
+}
+__device__ __forceinline__ void fetch_advance(const Args &g, Fetch &f, int by)
+{
+    f.tile += by;
+    while (f.b < g.a.seqs && f.tile >= f.tiles) {
+        f.tile -= f.tiles;
+        if (++f.seg == g.segs || f.tiles == 0) {
+            f.seg = 0;
+            ++f.b;
+            f.tiles = f.b < g.a.seqs ? tiles_of(g, f.b) : 0;
+        }
     }
-    return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
+}
+/* copy the tile into a stage; its valid slots go to *valid */
+template <int D, int NT>
+__device__ __forceinline__ void fetch_issue(const Args &g, const Fetch &f, uint8_t *stage, uint64_t *bar,
+                                            uint32_t *valid, int lane)
+{
+    using C = Cfg<D, NT>;
+    const int len = length_of(g, f.b), t0 = f.tile * kTile;
+    const bool ok = f.page >= 0 && f.page < g.c.pages;
+    const uint32_t half = __ballot_sync(0xFFFFFFFFu, ok) & 3u;
+    const int p0 = __shfl_sync(0xFFFFFFFFu, f.page, 0), p1 = __shfl_sync(0xFFFFFFFFu, f.page, 1);
+    const bool split = g.c.page_size == 16; /* two pages a tile, else one */
+    const int h = f.seg / g.chunks;
+    if (lane == 0) {
+        uint32_t v = ((half & 1u) ? 0xFFFFu : 0u) | ((half & 2u) ? 0xFFFF0000u : 0u);
+        if (t0 + kTile > len)
+            v &= (1u << (len - t0)) - 1u; /* len > t0 */
+        *valid = v;
+        const uint32_t n = split ? __popc(half) * (C::kStage / 2) : (half ? C::kStage : 0);
+        mbar_expect_tx(bar, n);
+    }
+    __syncwarp();
+    if (lane < 4) {
+        const bool code = !(lane & 1), key = lane < 2;
+        const uint8_t *src = key ? (code ? g.c.k_code : reinterpret_cast<const uint8_t *>(g.c.k_meta))
+                                 : (code ? g.c.v_code : reinterpret_cast<const uint8_t *>(g.c.v_meta));
+        const int row = code ? D / 2 : D / 16; /* bytes a slot */
+        uint8_t *dst = stage + (key ? 0 : C::kCode + C::kMeta) + (code ? 0 : C::kCode);
+        const int64_t slot = t0 % g.c.page_size;
+        if (!split) {
+            if (half)
+                bulk_g2s(dst, src + (((int64_t)p0 * g.c.kv_heads + h) * g.c.page_size + slot) * row, kTile * row, bar);
+        } else {
+            if (half & 1u)
+                bulk_g2s(dst, src + ((int64_t)p0 * g.c.kv_heads + h) * 16 * row, 16 * row, bar);
+            if (half & 2u)
+                bulk_g2s(dst + 16 * row, src + ((int64_t)p1 * g.c.kv_heads + h) * 16 * row, 16 * row, bar);
+        }
+    }
+}
+
+/* columns [0, cols) of one segment from its joined state: thread i of n */
+template <int D>
+__device__ __forceinline__ void write_column4(const Args &g, int b, int seg, int kcols, int n, int d, float4 o, float m,
+                                              float l)
+{
+    const int h = seg / g.chunks, col = (seg - h * g.chunks) * kcols + n;
+    if (col >= g.cols)
+        return;
+    const int r = col / g.group, hq = h * g.group + col - r * g.group;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); /* no slot seen: 0; NaN stays */
+    uint2 w;
+    w.x = pack2(o.x * inv, o.y * inv), w.y = pack2(o.z * inv, o.w * inv);
+    __nv_bfloat16 *out = g.a.o + (((int64_t)b * g.a.rows + r) * g.a.heads + hq) * D + d;
+    *reinterpret_cast<uint2 *>(out) = w;
+    if (d == 0) {
+        const float z = l == 0.f ? -INFINITY : m + log2f(l);
+        if (g.a.lse)
+            g.a.lse[((int64_t)b * g.a.heads + hq) * g.a.rows + r] = z == -INFINITY ? z : z * kLn2;
+        if (g.lse2)
+            g.lse2[((int64_t)b * g.c.kv_heads + h) * g.cols + col] = z;
+    }
+}
+
+template <int D, int NT, bool SCORE>
+__global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(const Args g)
+{
+    using C = Cfg<D, NT>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float *state = reinterpret_cast<float *>(smem + C::kRing);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kWarps * C::kState * 4);
+    uint32_t *valids = reinterpret_cast<uint32_t *>(bars + C::kWarps * C::kStages);
+    int *used = reinterpret_cast<int *>(valids + C::kWarps * C::kStages);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Plan plan = plan_of(g);
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    /* sequences without a slot: no tile reaches them */
+    for (int b = blockIdx.x; b < g.a.seqs; b += gridDim.x)
+        if (length_of(g, b) == 0)
+            for (int i = threadIdx.x; i < g.segs * C::kCols * (D / 4); i += C::kWarps * 32) {
+                const int seg = i / (C::kCols * (D / 4)), e = i % (C::kCols * (D / 4));
+                write_column4<D>(g, b, seg, C::kCols, e / (D / 4), e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f),
+                                 -INFINITY, 0.f);
+            }
+    if (blockIdx.x >= plan.parts || plan.units == 0)
+        return;
+    const int64_t begin = plan.begin(blockIdx.x), end = plan.begin(blockIdx.x + 1);
+    if (begin == end)
+        return;
+
+    uint8_t *ring = smem + warp * C::kStages * C::kStage;
+    uint64_t *bar = bars + warp * C::kStages;
+    uint32_t *valid = valids + warp * C::kStages;
+    if (lane == 0) {
+        for (int i = 0; i < C::kStages; ++i)
+            mbar_init(bar + i, 1);
+        mbar_init_fence();
+    }
+    __syncwarp();
+
+    At at = locate(g, begin);
+    Fetch f{at.b, at.seg, at.tile, at.tiles, -1};
+    fetch_advance(g, f, warp);
+    int64_t fetched = begin + warp; /* unit that f stands at */
+    fetch_page(g, f, lane);
+    int issued = 0; /* copies this warp has started, a stage each */
+    for (int i = 0; i < C::kStages && fetched < end; ++i, ++issued, fetched += C::kWarps) {
+        fetch_issue<D, NT>(g, f, ring + i * C::kStage, bar + i, valid + i, lane);
+        fetch_advance(g, f, C::kWarps);
+        fetch_page(g, f, lane);
+    }
+
+    const float scale2 = g.a.scale * kLog2e;
+    bool alive = true;
+    int slot = 0;
+    uint32_t phase = 0;
+    int64_t unit = begin + warp;
+    Query<D, NT> q;
+    State<D, NT> st;
+    for (int64_t pos = begin; pos < end;) {
+        const int64_t seg_end = at.seg_begin + at.tiles, stop = min(end, seg_end);
+        const bool mine = unit < stop;
+        if (mine) {
+            load_query<D, NT>(g, at.b, at.seg, q, lane);
+            st.clear();
+        }
+        const int h = at.seg / g.chunks, chunk = at.seg - h * g.chunks;
+        const int len = length_of(g, at.b);
+        float *score = SCORE ? g.score + ((int64_t)at.b * g.c.kv_heads + h) * g.a.max_pages * g.c.page_size * g.cols
+                             : nullptr;
+        for (; unit < stop; unit += C::kWarps) {
+            if (alive)
+                alive = mbar_wait_suspend_bounded(bar + slot, phase, &g_kv4_error);
+            const int t0 = (int)(unit - at.seg_begin) * kTile;
+            const uint32_t v = valid[slot];
+            const bool whole = v == 0xFFFFFFFFu && t0 + kTile <= len - g.a.rows + 1;
+            tile_step<D, NT, SCORE>(g, q, st, saddr(ring + slot * C::kStage), t0, v, whole, scale2, score, chunk, lane);
+            __syncwarp();
+            if (fetched < end) {
+                if (alive) {
+                    fetch_issue<D, NT>(g, f, ring + slot * C::kStage, bar + slot, valid + slot, lane);
+                    ++issued;
+                }
+                fetched += C::kWarps;
+                fetch_advance(g, f, C::kWarps);
+                fetch_page(g, f, lane);
+            }
+            if (++slot == C::kStages)
+                slot = 0, phase ^= 1u;
+        }
+        /* this warp's state to shared memory, the lo terms added in */
+        float *mem = state + warp * C::kState;
+        if (lane == 0)
+            used[warp] = mine ? 1 : 0;
+        if (mine) {
+            const int gr = lane >> 2, c = lane & 3;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float l = st.l[n][i], lo[D / 64];
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k)
+                        lo[k] = st.lo[n][k][i];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) {
+                        l += __shfl_xor_sync(0xFFFFFFFFu, l, off);
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k)
+                            lo[k] += __shfl_xor_sync(0xFFFFFFFFu, lo[k], off);
+                    }
+                    const int col = n * 8 + 2 * c + i;
+                    if (gr == 0)
+                        mem[C::kCols * D + col] = st.m[n][i], mem[C::kCols * D + C::kCols + col] = l;
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+                        for (int up = 0; up < 2; ++up)
+                            *reinterpret_cast<float4 *>(mem + col * D + 64 * k + 8 * gr + 4 * up) =
+                                make_float4(st.o[n][k][0][2 * up + i] + lo[k], st.o[n][k][1][2 * up + i] + lo[k],
+                                            st.o[n][k][2][2 * up + i] + lo[k], st.o[n][k][3][2 * up + i] + lo[k]);
+                }
+        }
+        __syncthreads();
+        /* joined over the warps in their order; the whole segment, or a part of it for the join kernel */
+        const bool first = at.seg_begin >= begin, whole_seg = first && seg_end <= end;
+        float *part = g.part + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * C::kState;
+        for (int i = threadIdx.x; i < C::kCols * (D / 4); i += C::kWarps * 32) {
+            const int n = i / (D / 4), d = i % (D / 4) * 4;
+            float m = -INFINITY, l = 0.f;
+            for (int w = 0; w < C::kWarps; ++w)
+                if (used[w])
+                    m = fmaxf(m, state[w * C::kState + C::kCols * D + n]);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < C::kWarps; ++w) {
+                if (!used[w])
+                    continue;
+                const float *s = state + w * C::kState;
+                const float mw = s[C::kCols * D + n], fw = mw == -INFINITY ? 0.f : ex2(mw - m);
+                const float4 v = *reinterpret_cast<const float4 *>(s + n * D + d);
+                l = fmaf(fw, s[C::kCols * D + C::kCols + n], l);
+                o.x = fmaf(fw, v.x, o.x), o.y = fmaf(fw, v.y, o.y), o.z = fmaf(fw, v.z, o.z), o.w = fmaf(fw, v.w, o.w);
+            }
+            if (whole_seg) {
+                write_column4<D>(g, at.b, at.seg, C::kCols, n, d, o, m, l);
+            } else {
+                *reinterpret_cast<float4 *>(part + n * D + d) = o;
+                if (d == 0)
+                    part[C::kCols * D + n] = m, part[C::kCols * D + C::kCols + n] = l;
+            }
+        }
+        __syncthreads();
+        pos = stop;
+        if (pos < end) { /* the next segment that has tiles */
+            at.seg_begin = seg_end;
+            at.tile = 0;
+            if (++at.seg == g.segs) {
+                at.seg = 0;
+                do
+                    ++at.b;
+                while (at.b < g.a.seqs - 1 && tiles_of(g, at.b) == 0);
+                at.tiles = tiles_of(g, at.b);
+            }
+        }
+    }
+    if (!alive) /* a wait ran out: the copies still in flight, before the memory goes */
+        for (int i = 0; i < C::kStages; ++i)
+            if (const int n = (issued + C::kStages - 1 - i) / C::kStages)
+                mbar_wait_suspend_bounded(bar + i, (n - 1) & 1, &g_kv4_error);
+}
+
+/* Joins the parts of the segment that begins in range blockIdx.x and runs on past it. */
+template <int D, int NT>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const Args g)
+{
+    using C = Cfg<D, NT>;
+    const Plan plan = plan_of(g);
+    const int i = blockIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory"); /* in every CTA: this kernel ends after the one before */
+    if (i + 1 >= plan.parts || plan.units == 0)
+        return;
+    const int64_t end = plan.begin(i + 1);
+    if (plan.begin(i) == end)
+        return;
+    const At at = locate(g, end - 1);
+    const int64_t seg_end = at.seg_begin + at.tiles;
+    if (seg_end <= end || at.seg_begin < plan.begin(i))
+        return;
+    const int last = plan.owner(seg_end - 1);
+    for (int e = threadIdx.x; e < C::kCols * (D / 4); e += 256) {
+        const int n = e / (D / 4), d = e % (D / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+        for (int p = i; p <= last; ++p)
+            m = fmaxf(m, g.part[((int64_t)p * 2 + (p == i)) * C::kState + C::kCols * D + n]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = i; p <= last; ++p) {
+            const float *s = g.part + ((int64_t)p * 2 + (p == i)) * C::kState;
+            const float mp = s[C::kCols * D + n], fp = mp == -INFINITY ? 0.f : ex2(mp - m);
+            const float4 v = *reinterpret_cast<const float4 *>(s + n * D + d);
+            l = fmaf(fp, s[C::kCols * D + C::kCols + n], l);
+            o.x = fmaf(fp, v.x, o.x), o.y = fmaf(fp, v.y, o.y), o.z = fmaf(fp, v.z, o.z), o.w = fmaf(fp, v.w, o.w);
+        }
+        write_column4<D>(g, at.b, at.seg, C::kCols, n, d, o, m, l);
+    }
+}
+
+/* weight_out from the scores: a thread per slot, the columns in order */
+__global__ void __launch_bounds__(256) kv4_weight_kernel(const Args g)
+{
+    const int bh = blockIdx.y, b = bh / g.c.kv_heads;
+    const int len = length_of(g, b), t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= len)
+        return;
+    const int cap = g.a.max_pages * g.c.page_size;
+    const int page = g.a.table[(int64_t)b * g.a.max_pages + t / g.c.page_size];
+    const float *s = g.score + ((int64_t)bh * cap + t) * g.cols, *z = g.lse2 + (int64_t)bh * g.cols;
+    float sum = 0.f;
+    if (page >= 0 && page < g.c.pages)
+        for (int n = 0; n < g.cols; ++n)
+            if (s[n] != -INFINITY)
+                sum += ex2(s[n] - z[n]);
+    const int64_t i = (int64_t)bh * g.a.weight_stride + t;
+    const float old = g.a.weight && t < len - g.a.rows ? g.a.weight[i] : 0.f;
+    g.a.weight_out[i] = old + sum;
 }
 
 int check(const GlintKv4Cache *c, const GlintKv4Attn *a)
@@ -155,8 +719,64 @@ int check(const GlintKv4Cache *c, const GlintKv4Attn *a)
         return rc;
     if (!a || a->seqs < 0 || a->rows < 1 || a->heads < 1 || a->heads % c->kv_heads || a->max_pages < 1 ||
         (int64_t)a->heads / c->kv_heads * a->rows > 256 || (int64_t)a->max_pages * c->page_size > INT32_MAX ||
-        a->seqs > 65535 || c->kv_heads > 65535)
+        (int64_t)a->seqs * c->kv_heads > 65535)
         return kBadArg;
+    return kOk;
+}
+
+/* bytes of the parts, rounded up; of the log2 sums; of the scores */
+struct Work {
+    int64_t part, lse2, score;
+};
+Work work_of(const GlintKv4Cache &c, const GlintKv4Attn &a)
+{
+    const int64_t cols = (int64_t)a.heads / c.kv_heads * a.rows, kcols = cols <= 8 ? 8 : 16;
+    Work w;
+    w.part = (int64_t)sm_count() * 2 * (kcols * c.head_dim + 2 * kcols) * 4;
+    w.lse2 = a.weight_out ? ((int64_t)a.seqs * c.kv_heads * cols * 4 + 15) / 16 * 16 : 0;
+    w.score = a.weight_out ? (int64_t)a.seqs * c.kv_heads * a.max_pages * c.page_size * cols * 4 : 0;
+    return w;
+}
+
+/* the next kernel's launch may overlap the end of the one before; it waits itself
+ * (griddepcontrol.wait) before it touches that one's results */
+template <class... P>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, const Args &g)
+{
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, g);
+}
+
+template <int D, int NT>
+int launch(Args &g, cudaStream_t st)
+{
+    using C = Cfg<D, NT>;
+    const void *kernel = g.score ? (const void *)kv4_attn_kernel<D, NT, true> : (const void *)kv4_attn_kernel<D, NT, false>;
+    if (!ensure_smem(kernel, C::kSmem))
+        return kLaunch;
+    g.chunks = (g.cols + C::kCols - 1) / C::kCols;
+    g.segs = g.c.kv_heads * g.chunks;
+    g.min_units = C::kWarps / 2;
+    if (g.score)
+        kv4_attn_kernel<D, NT, true><<<g.parts, C::kWarps * 32, C::kSmem, st>>>(g);
+    else
+        kv4_attn_kernel<D, NT, false><<<g.parts, C::kWarps * 32, C::kSmem, st>>>(g);
+    if (cudaGetLastError() != cudaSuccess)
+        return kLaunch;
+    if (launch_after(kv4_join_kernel<D, NT>, dim3(g.parts), 256, st, g) != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunch;
+    }
+    if (g.score) {
+        const int cap = g.a.max_pages * g.c.page_size;
+        kv4_weight_kernel<<<dim3((cap + 255) / 256, g.a.seqs * g.c.kv_heads), 256, 0, st>>>(g);
+        if (cudaGetLastError() != cudaSuccess)
+            return kLaunch;
+    }
     return kOk;
 }
 
@@ -172,7 +792,8 @@ int64_t glint_kv4_attn_work_bytes(const GlintKv4Cache *c, const GlintKv4Attn *a)
     const int rc = check(c, a);
     if (rc != kOk)
         return rc;
-    return a->weight_out ? (int64_t)a->seqs * a->heads * a->rows * 4 : 0;
+    const Work w = work_of(*c, *a);
+    return w.part + w.lse2 + w.score;
 }
 
 int glint_kv4_attn_stream(const GlintKv4Cache *c, const GlintKv4Attn *a, cudaStream_t stream)
@@ -182,13 +803,23 @@ int glint_kv4_attn_stream(const GlintKv4Cache *c, const GlintKv4Attn *a, cudaStr
         return rc;
     if (a->seqs == 0)
         return kOk;
-    if (!a->q || !a->o || !a->table || !a->lens || (a->weight_out && !a->work) ||
+    if (!a->q || !a->o || !a->table || !a->lens || !a->work || !aligned_to(a->work, 16) || !aligned_to(a->o, 16) ||
         (a->weight_out && a->weight_stride < (int64_t)a->max_pages * c->page_size))
         return kBadArg;
-    Args g{*c, *a};
-    if (!a->weight_out)
-        g.a.work = nullptr;
-    return c->head_dim == 128 ? launch<128>(g, stream) : launch<64>(g, stream);
+    Args g{};
+    g.c = *c, g.a = *a;
+    g.group = a->heads / c->kv_heads, g.cols = g.group * a->rows;
+    g.parts = sm_count();
+    const Work w = work_of(*c, *a);
+    uint8_t *work = static_cast<uint8_t *>(a->work);
+    g.part = reinterpret_cast<float *>(work);
+    if (a->weight_out) {
+        g.lse2 = reinterpret_cast<float *>(work + w.part);
+        g.score = reinterpret_cast<float *>(work + w.part + w.lse2);
+    }
+    if (c->head_dim == 128)
+        return g.cols <= 8 ? launch<128, 1>(g, stream) : launch<128, 2>(g, stream);
+    return g.cols <= 8 ? launch<64, 1>(g, stream) : launch<64, 2>(g, stream);
 }
 
 } /* extern "C" */

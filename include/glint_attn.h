@@ -83,8 +83,8 @@ int glint_kv4_read_stream(const GlintKv4Cache *c, const int *slots, int tokens, 
  * weight_out (NULL: none) [seqs, kv_heads, weight_stride] f32: weight + the slot's
  * softmax weights summed over the head's query heads and rows; weight counts as zero
  * when NULL and in the newest `rows` slots; slots >= lens[b] are not written; weight
- * may be weight_out.  With weight_out, work is glint_kv4_attn_work_bytes() of device
- * memory for the call; NULL otherwise.
+ * may be weight_out.  work: glint_kv4_attn_work_bytes() of 16-byte aligned device
+ * memory, the call's own until it completes, of any content.
  * Limits: rows >= 1, heads / kv_heads * rows <= 256. */
 typedef struct GlintKv4Attn {
     const glint_bf16_t *q;

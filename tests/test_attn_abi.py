@@ -20,7 +20,7 @@ def structs():
     p = (ctypes.addressof(buf) + 15) & ~15
     cache = attn._Cache(p, p, p, p, 4, 2, 64, 128)
     prompt = attn._Prompt(*[p] * 7, *[8] * 8, 1, 4, 4, 4, 2, 128, 1, 1.0)
-    at = attn._Attn(p, p, p, p, p, None, None, None, 8, 8, 8, 256, 1, 1, 4, 4, 1.0)
+    at = attn._Attn(p, p, p, p, p, None, None, p, 8, 8, 8, 256, 1, 1, 4, 4, 1.0)
     ev = attn._Evict(p, p, p, p, p, p, p, p + 16, p + 16, 256, 1, 4, 8, 2)
     return buf, p, cache, prompt, at, ev
 
@@ -65,15 +65,16 @@ def test_cache_arguments(lib):
 def test_attn_arguments(lib):
     f = lib.glint_kv4_attn_stream
     for kw, rc in ((dict(q=None), -1), (dict(o=None), -1), (dict(table=None), -1), (dict(lens=None), -1),
-                   (dict(rows=0), -1), (dict(rows=129), -1), (dict(heads=3), -1), (dict(max_pages=0), -1),
+                   (dict(work=None), -1), (dict(rows=0), -1), (dict(rows=129), -1), (dict(heads=3), -1), (dict(max_pages=0), -1),
                    (dict(seqs=-1), -1), (dict(seqs=0), 0)):
         buf, p, cache, _, at, _ = structs()
         assert f(cache, put(at, **kw), None) == rc, kw
     buf, p, cache, _, at, _ = structs()
-    assert f(cache, put(at, weight_out=p), None) == -1                               # no workspace
-    assert f(cache, put(at, work=p, weight_stride=255), None) == -1                  # weights too short
-    assert lib.glint_kv4_attn_work_bytes(cache, at) > 0
-    assert lib.glint_kv4_attn_work_bytes(cache, put(at, weight_out=None)) == 0
+    assert f(cache, put(at, weight_out=p, weight_stride=255), None) == -1            # weights too short
+    more = lib.glint_kv4_attn_work_bytes(cache, at)
+    assert more > lib.glint_kv4_attn_work_bytes(cache, put(at, weight_out=None)) > 0
+    assert f(cache, put(at, work=p + 8), None) == -1
+    assert f(cache, put(at, work=p, o=p + 8), None) == -1
     assert f(cache, None, None) == -1
 
 
