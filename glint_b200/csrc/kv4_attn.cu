@@ -34,6 +34,9 @@ int kv4_error_word(bool clear) { return read_error_word(g_kv4_error, g_kv4_error
 namespace {
 
 constexpr int kTile = 32;        /* slots a warp takes at a time */
+constexpr int kGroup = 4;        /* warps of a worker */
+constexpr int kJoin = 2;         /* what a segment costs beside its tiles, in tiles */
+constexpr int kWorker = 4;       /* a worker's range, at least */
 constexpr float kLazy = 8.f;     /* the running maximum may lag by 2^8 */
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -57,8 +60,8 @@ struct Args {
     GlintKv4Attn a;
     int group, cols;      /* query heads a kv head; group * rows */
     int chunks, segs;     /* column chunks a kv head; segments a sequence = kv_heads * chunks */
-    int parts;            /* grid of the attention kernel */
-    int min_units;        /* tiles a CTA takes at least */
+    int parts;            /* workers at most: warps of the grid / kGroup */
+    int page_log2;
     float *part;          /* [parts][2][kState] unfinished segments */
     float *score;         /* [seqs][kv_heads][max slots][cols] log2-scaled scores, or NULL */
     float *lse2;          /* [seqs][kv_heads][cols] log2 sums, with score */
@@ -76,41 +79,57 @@ __device__ __forceinline__ int length_of(const Args &g, int b)
 }
 __device__ __forceinline__ int tiles_of(const Args &g, int b) { return (length_of(g, b) + kTile - 1) / kTile; }
 
-/* The tiles of all segments in one row (sequence, then segment, then tile), cut into
- * equal ranges over the CTAs: sequences of any mix of lengths keep every SM busy. */
+/* All segments in one row (sequence after sequence), each as long as kJoin plus its
+ * tiles, cut into equal ranges over the workers (four warps each): sequences of any mix
+ * of lengths keep every SM busy, and a range of many short segments, each with a query
+ * to load and a result to write, is not taken for as little work as one long one. */
 struct Plan {
     int64_t units;
-    int parts;
+    int parts; /* workers with a range */
     __device__ __forceinline__ int64_t begin(int i) const { return units * i / parts; }
     __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * parts - 1) / units); }
 };
+__device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + kJoin : 0; }
 __device__ __forceinline__ Plan plan_of(const Args &g)
 {
-    const int lane = threadIdx.x & 31;
     int64_t n = 0;
-    for (int b = lane; b < g.a.seqs; b += 32)
-        n += tiles_of(g, b);
+    for (int b = threadIdx.x & 31; b < g.a.seqs; b += 32)
+        n += cost_of(tiles_of(g, b));
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1)
         n += __shfl_xor_sync(0xFFFFFFFFu, n, off);
     Plan p;
     p.units = n * g.segs;
-    p.parts = (int)max((int64_t)1, min((int64_t)g.parts, p.units / g.min_units));
+    p.parts = (int)max((int64_t)1, min((int64_t)g.parts, p.units / kWorker));
     return p;
 }
-/* a place in that row */
-struct At {
-    int b, seg, tile, tiles;
-    int64_t seg_begin; /* unit of the segment's first tile */
+/* A segment on a walk along a range: `first` is its first tile's place, counted from
+ * the range's begin (negative where the range begins inside the segment). */
+struct Walk {
+    int b, seg, tiles, first;
+    __device__ __forceinline__ int lo() const { return max(0, -first); }
+    __device__ __forceinline__ int hi(int range) const { return min(tiles, range - first); }
+    __device__ __forceinline__ bool next(const Args &g, int range) /* false at the range's end */
+    {
+        first += tiles + kJoin;
+        if (first >= range)
+            return false;
+        if (++seg == g.segs) {
+            seg = 0;
+            do
+                tiles = ++b < g.a.seqs ? tiles_of(g, b) : 0;
+            while (tiles == 0 && b < g.a.seqs);
+        }
+        return b < g.a.seqs;
+    }
 };
-__device__ __forceinline__ At locate(const Args &g, int64_t u) /* u < units; whole warp */
+__device__ __forceinline__ Walk locate(const Args &g, int64_t u) /* u < units; whole warp */
 {
     const int lane = threadIdx.x & 31;
     int64_t before = 0;
     for (int b0 = 0;; b0 += 32) {
-        const int b = b0 + lane;
-        const int t = b < g.a.seqs ? tiles_of(g, b) : 0;
-        int64_t s = t;
+        const int t = b0 + lane < g.a.seqs ? tiles_of(g, b0 + lane) : 0;
+        int64_t s = cost_of(t);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const int64_t o = __shfl_up_sync(0xFFFFFFFFu, s, off);
@@ -120,14 +139,14 @@ __device__ __forceinline__ At locate(const Args &g, int64_t u) /* u < units; who
         const uint32_t past = __ballot_sync(0xFFFFFFFFu, (before + s) * g.segs > u);
         if (past || b0 + 32 >= g.a.seqs) {
             const int l = past ? __ffs(past) - 1 : 31;
-            At at;
-            at.b = b0 + l;
-            at.tiles = __shfl_sync(0xFFFFFFFFu, t, l);
-            const int64_t first = (before + __shfl_sync(0xFFFFFFFFu, s, l) - at.tiles) * g.segs;
-            at.seg = at.tiles ? (int)((u - first) / at.tiles) : 0;
-            at.seg_begin = first + (int64_t)at.seg * at.tiles;
-            at.tile = (int)(u - at.seg_begin);
-            return at;
+            Walk w;
+            w.b = b0 + l;
+            w.tiles = __shfl_sync(0xFFFFFFFFu, t, l);
+            const int cost = max(1, cost_of(w.tiles));
+            const int64_t off = u - (before + __shfl_sync(0xFFFFFFFFu, s, l) - cost) * g.segs;
+            w.seg = (int)(off / cost);
+            w.first = (int)((int64_t)w.seg * cost - off) + kJoin;
+            return w;
         }
         before += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
@@ -140,11 +159,17 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-/* nibbles j and j + 4 of w as the BF16 pair (code - 8, code - 8) */
-__device__ __forceinline__ uint32_t codes(uint32_t w, int j)
+/* nibbles j and j + 4 of w as the BF16 pair (128 + code, 128 + code) */
+__device__ __forceinline__ uint32_t codes128(uint32_t w, int j)
 {
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w >> (4 * j)), "r"(0x43004300u));
+    return r;
+}
+/* the same as (code - 8, code - 8), exact */
+__device__ __forceinline__ uint32_t codes(uint32_t w, int j)
+{
+    const uint32_t r = codes128(w, j);
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&r), __floats2bfloat162_rn(136.f, 136.f));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
@@ -237,9 +262,9 @@ __device__ __forceinline__ void load_query(const Args &g, int b, int seg, Query<
 }
 
 /* One tile of 32 slots (from slot t0) in shared memory. */
-template <int D, int NT, bool SCORE>
+template <int D, int NT, bool SCORE, bool WHOLE>
 __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, State<D, NT> &st, uint32_t stage,
-                                          int t0, uint32_t valid, bool whole, float scale2, float *score, int chunk,
+                                          int t0, uint32_t valid, float scale2, float *score, int chunk,
                                           int lane)
 {
     using C = Cfg<D, NT>;
@@ -258,12 +283,12 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    acc[k][n][i] = 0.f;
+                    acc[k][n][i] = -136.f * q.sum[n][k][i & 1]; /* 128 + code, less 136 */
             const uint2 wa = lds64(kcode + ta * RB + kv4_unit<D>(k, ta) + 8 * c);
             const uint2 wb = lds64(kcode + tb * RB + kv4_unit<D>(k, tb) + 8 * c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t a[4] = {codes(wa.x, j), codes(wb.x, j), codes(wa.y, j), codes(wb.y, j)};
+                const uint32_t a[4] = {codes128(wa.x, j), codes128(wb.x, j), codes128(wa.y, j), codes128(wb.y, j)};
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     mma(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1]);
@@ -294,7 +319,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             for (int i = 0; i < 4; ++i) {
                 const int t = i < 2 ? ta : tb;
                 s[sl][n][i] *= scale2;
-                if (!whole && (!((valid >> t) & 1u) || t0 + t >= q.see[n][i & 1]))
+                if (!WHOLE && (!((valid >> t) & 1u) || t0 + t >= q.see[n][i & 1]))
                     s[sl][n][i] = -INFINITY;
             }
         if constexpr (SCORE) {
@@ -304,7 +329,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float *p = score + (int64_t)(t0 + (i ? tb : ta)) * g.cols + col;
-                    if ((valid >> (i ? tb : ta)) & 1u) {
+                    if (WHOLE || ((valid >> (i ? tb : ta)) & 1u)) {
                         if (col < g.cols)
                             p[0] = s[sl][n][2 * i];
                         if (col + 1 < g.cols)
@@ -373,7 +398,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
                 for (int i = 0; i < 4; ++i) {
                     w[i] = p[i] * steps[k][i >> 1], x[i] = p[i] * mids[k][i >> 1];
                     /* a masked slot's step and lo may be anything, NaN too */
-                    if (!whole && s[sl][n][i] == -INFINITY)
+                    if (!WHOLE && s[sl][n][i] == -INFINITY)
                         w[i] = x[i] = 0.f;
                 }
                 st.lo[n][k][0] += x[0] + x[2];
@@ -402,29 +427,25 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
     }
 }
 
-/* where a warp's next tile to fetch lies, and the pages that hold it */
+/* a warp's next tile to fetch, and the pages that hold it */
 struct Fetch {
-    int b, seg, tile, tiles;
+    Walk w;
+    int tile; /* -1: none left */
     int page; /* lanes 0 and 1: the page of the tile's slots 0-15 and 16-31, -1 for none */
 };
-__device__ __forceinline__ void fetch_page(const Args &g, Fetch &f, int lane)
+__device__ __forceinline__ void fetch_seek(const Args &g, Fetch &f, int range, int lane)
 {
-    const int t = f.tile * kTile + 16 * lane;
-    f.page = -1;
-    if (lane < 2 && f.tiles > 0 && t < length_of(g, f.b))
-        f.page = g.a.table[(int64_t)f.b * g.a.max_pages + t / g.c.page_size];
-}
-__device__ __forceinline__ void fetch_advance(const Args &g, Fetch &f, int by)
-{
-    f.tile += by;
-    while (f.b < g.a.seqs && f.tile >= f.tiles) {
-        f.tile -= f.tiles;
-        if (++f.seg == g.segs || f.tiles == 0) {
-            f.seg = 0;
-            ++f.b;
-            f.tiles = f.b < g.a.seqs ? tiles_of(g, f.b) : 0;
+    while (f.tile >= f.w.hi(range)) {
+        f.tile -= max(f.w.hi(range), f.w.lo());
+        if (!f.w.next(g, range)) {
+            f.tile = -1;
+            return;
         }
     }
+    const int t = f.tile * kTile + 16 * lane;
+    f.page = -1;
+    if (lane < 2 && t < length_of(g, f.w.b))
+        f.page = g.a.table[(int64_t)f.w.b * g.a.max_pages + (t >> g.page_log2)];
 }
 /* copy the tile into a stage; its valid slots go to *valid */
 template <int D, int NT>
@@ -432,12 +453,12 @@ __device__ __forceinline__ void fetch_issue(const Args &g, const Fetch &f, uint8
                                             uint32_t *valid, int lane)
 {
     using C = Cfg<D, NT>;
-    const int len = length_of(g, f.b), t0 = f.tile * kTile;
+    const int len = length_of(g, f.w.b), t0 = f.tile * kTile;
     const bool ok = f.page >= 0 && f.page < g.c.pages;
     const uint32_t half = __ballot_sync(0xFFFFFFFFu, ok) & 3u;
     const int p0 = __shfl_sync(0xFFFFFFFFu, f.page, 0), p1 = __shfl_sync(0xFFFFFFFFu, f.page, 1);
     const bool split = g.c.page_size == 16; /* two pages a tile, else one */
-    const int h = f.seg / g.chunks;
+    const int h = f.w.seg / g.chunks;
     if (lane == 0) {
         uint32_t v = ((half & 1u) ? 0xFFFFu : 0u) | ((half & 2u) ? 0xFFFF0000u : 0u);
         if (t0 + kTile > len)
@@ -453,10 +474,10 @@ __device__ __forceinline__ void fetch_issue(const Args &g, const Fetch &f, uint8
                                  : (code ? g.c.v_code : reinterpret_cast<const uint8_t *>(g.c.v_meta));
         const int row = code ? D / 2 : D / 16; /* bytes a slot */
         uint8_t *dst = stage + (key ? 0 : C::kCode + C::kMeta) + (code ? 0 : C::kCode);
-        const int64_t slot = t0 % g.c.page_size;
+        const int slot = t0 & (g.c.page_size - 1);
         if (!split) {
             if (half)
-                bulk_g2s(dst, src + (((int64_t)p0 * g.c.kv_heads + h) * g.c.page_size + slot) * row, kTile * row, bar);
+                bulk_g2s(dst, src + ((((int64_t)p0 * g.c.kv_heads + h) << g.page_log2) + slot) * row, kTile * row, bar);
         } else {
             if (half & 1u)
                 bulk_g2s(dst, src + ((int64_t)p0 * g.c.kv_heads + h) * 16 * row, 16 * row, bar);
@@ -489,6 +510,46 @@ __device__ __forceinline__ void write_column4(const Args &g, int b, int seg, int
     }
 }
 
+/* barrier of one worker's warps */
+__device__ __forceinline__ void worker_sync(int i)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(i + 1), "n"(kGroup * 32) : "memory");
+}
+
+/* a warp's state to shared memory (O by column, m, l), the lo terms added in */
+template <int D, int NT>
+__device__ __forceinline__ void store_state(const State<D, NT> &st, float *mem, int lane)
+{
+    using C = Cfg<D, NT>;
+    const int gr = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float l = st.l[n][i], lo[D / 64];
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k)
+                lo[k] = st.lo[n][k][i];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, off);
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k)
+                    lo[k] += __shfl_xor_sync(0xFFFFFFFFu, lo[k], off);
+            }
+            const int col = n * 8 + 2 * c + i;
+            if (gr == 0)
+                mem[C::kCols * D + col] = st.m[n][i], mem[C::kCols * D + C::kCols + col] = l;
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+                for (int up = 0; up < 2; ++up)
+                    *reinterpret_cast<float4 *>(mem + col * D + 64 * k + 8 * gr + 4 * up) =
+                        make_float4(st.o[n][k][0][2 * up + i] + lo[k], st.o[n][k][1][2 * up + i] + lo[k],
+                                    st.o[n][k][2][2 * up + i] + lo[k], st.o[n][k][3][2 * up + i] + lo[k]);
+        }
+}
+
 template <int D, int NT, bool SCORE>
 __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(const Args g)
 {
@@ -510,11 +571,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
                 write_column4<D>(g, b, seg, C::kCols, e / (D / 4), e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f),
                                  -INFINITY, 0.f);
             }
-    if (blockIdx.x >= plan.parts || plan.units == 0)
+    /* workers go round the SMs first, so a few of them spread out */
+    const int worker = (warp / kGroup) * gridDim.x + blockIdx.x, w = warp % kGroup;
+    if (worker >= plan.parts || plan.units == 0)
         return;
-    const int64_t begin = plan.begin(blockIdx.x), end = plan.begin(blockIdx.x + 1);
-    if (begin == end)
-        return;
+    const int64_t begin = plan.begin(worker);
+    const int range = (int)(plan.begin(worker + 1) - begin);
 
     uint8_t *ring = smem + warp * C::kStages * C::kStage;
     uint64_t *bar = bars + warp * C::kStages;
@@ -526,110 +588,85 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
     }
     __syncwarp();
 
-    At at = locate(g, begin);
-    Fetch f{at.b, at.seg, at.tile, at.tiles, -1};
-    fetch_advance(g, f, warp);
-    int64_t fetched = begin + warp; /* unit that f stands at */
-    fetch_page(g, f, lane);
-    int issued = 0; /* copies this warp has started, a stage each */
-    for (int i = 0; i < C::kStages && fetched < end; ++i, ++issued, fetched += C::kWarps) {
-        fetch_issue<D, NT>(g, f, ring + i * C::kStage, bar + i, valid + i, lane);
-        fetch_advance(g, f, C::kWarps);
-        fetch_page(g, f, lane);
-    }
-
     const float scale2 = g.a.scale * kLog2e;
-    bool alive = true;
-    int slot = 0;
+    Walk at = locate(g, begin);
+    Fetch f{at, at.lo() + w, -1};
+    fetch_seek(g, f, range, lane);
+    int issued = 0; /* copies this warp has started, a stage each */
+    int slot = 0;   /* the stage it reads next, and the parity of its phase */
     uint32_t phase = 0;
-    int64_t unit = begin + warp;
+    bool alive = true;
+    auto fetch = [&](int stage) {
+        if (f.tile < 0 || !alive)
+            return;
+        fetch_issue<D, NT>(g, f, ring + stage * C::kStage, bar + stage, valid + stage, lane);
+        ++issued;
+        f.tile += kGroup;
+        fetch_seek(g, f, range, lane);
+    };
+    for (int i = 0; i < C::kStages; ++i)
+        fetch(i);
+
     Query<D, NT> q;
     State<D, NT> st;
-    for (int64_t pos = begin; pos < end;) {
-        const int64_t seg_end = at.seg_begin + at.tiles, stop = min(end, seg_end);
-        const bool mine = unit < stop;
+    float *mem = state + warp * C::kState;
+    int turn = w; /* how far the worker's next tile is from this warp's */
+    do {
+        const int lo = at.lo(), hi = at.hi(range);
+        if (lo >= hi)
+            continue;
+        const int h = at.seg / g.chunks, chunk = at.seg - h * g.chunks, len = length_of(g, at.b);
+        int tile = lo + turn;
+        const bool mine = tile < hi;
         if (mine) {
             load_query<D, NT>(g, at.b, at.seg, q, lane);
             st.clear();
         }
-        const int h = at.seg / g.chunks, chunk = at.seg - h * g.chunks;
-        const int len = length_of(g, at.b);
         float *score = SCORE ? g.score + ((int64_t)at.b * g.c.kv_heads + h) * g.a.max_pages * g.c.page_size * g.cols
                              : nullptr;
-        for (; unit < stop; unit += C::kWarps) {
+        for (; tile < hi; tile += kGroup) {
             if (alive)
                 alive = mbar_wait_suspend_bounded(bar + slot, phase, &g_kv4_error);
-            const int t0 = (int)(unit - at.seg_begin) * kTile;
-            const uint32_t v = valid[slot];
-            const bool whole = v == 0xFFFFFFFFu && t0 + kTile <= len - g.a.rows + 1;
-            tile_step<D, NT, SCORE>(g, q, st, saddr(ring + slot * C::kStage), t0, v, whole, scale2, score, chunk, lane);
+            const uint32_t v = valid[slot], stage = saddr(ring + slot * C::kStage);
+            if (v == 0xFFFFFFFFu && tile * kTile + kTile <= len - g.a.rows + 1)
+                tile_step<D, NT, SCORE, true>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);
+            else
+                tile_step<D, NT, SCORE, false>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);
             __syncwarp();
-            if (fetched < end) {
-                if (alive) {
-                    fetch_issue<D, NT>(g, f, ring + slot * C::kStage, bar + slot, valid + slot, lane);
-                    ++issued;
-                }
-                fetched += C::kWarps;
-                fetch_advance(g, f, C::kWarps);
-                fetch_page(g, f, lane);
-            }
+            fetch(slot);
             if (++slot == C::kStages)
                 slot = 0, phase ^= 1u;
         }
-        /* this warp's state to shared memory, the lo terms added in */
-        float *mem = state + warp * C::kState;
+        turn = tile - hi;
+        if (mine)
+            store_state<D, NT>(st, mem, lane);
         if (lane == 0)
             used[warp] = mine ? 1 : 0;
-        if (mine) {
-            const int gr = lane >> 2, c = lane & 3;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float l = st.l[n][i], lo[D / 64];
-#pragma unroll
-                    for (int k = 0; k < D / 64; ++k)
-                        lo[k] = st.lo[n][k][i];
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        l += __shfl_xor_sync(0xFFFFFFFFu, l, off);
-#pragma unroll
-                        for (int k = 0; k < D / 64; ++k)
-                            lo[k] += __shfl_xor_sync(0xFFFFFFFFu, lo[k], off);
-                    }
-                    const int col = n * 8 + 2 * c + i;
-                    if (gr == 0)
-                        mem[C::kCols * D + col] = st.m[n][i], mem[C::kCols * D + C::kCols + col] = l;
-#pragma unroll
-                    for (int k = 0; k < D / 64; ++k)
-#pragma unroll
-                        for (int up = 0; up < 2; ++up)
-                            *reinterpret_cast<float4 *>(mem + col * D + 64 * k + 8 * gr + 4 * up) =
-                                make_float4(st.o[n][k][0][2 * up + i] + lo[k], st.o[n][k][1][2 * up + i] + lo[k],
-                                            st.o[n][k][2][2 * up + i] + lo[k], st.o[n][k][3][2 * up + i] + lo[k]);
-                }
-        }
-        __syncthreads();
+        worker_sync(warp / kGroup);
         /* joined over the warps in their order; the whole segment, or a part of it for the join kernel */
-        const bool first = at.seg_begin >= begin, whole_seg = first && seg_end <= end;
-        float *part = g.part + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * C::kState;
-        for (int i = threadIdx.x; i < C::kCols * (D / 4); i += C::kWarps * 32) {
+        const bool first = at.first >= 0, whole = first && at.first + at.tiles <= range;
+        float *part = g.part + ((int64_t)worker * 2 + (first ? 1 : 0)) * C::kState;
+        const float *states = state + (warp - w) * C::kState;
+        const int *mask = used + (warp - w);
+        for (int i = w * 32 + lane; i < C::kCols * (D / 4); i += kGroup * 32) {
             const int n = i / (D / 4), d = i % (D / 4) * 4;
             float m = -INFINITY, l = 0.f;
-            for (int w = 0; w < C::kWarps; ++w)
-                if (used[w])
-                    m = fmaxf(m, state[w * C::kState + C::kCols * D + n]);
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+                if (mask[k])
+                    m = fmaxf(m, states[k * C::kState + C::kCols * D + n]);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < C::kWarps; ++w) {
-                if (!used[w])
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                if (!mask[k])
                     continue;
-                const float *s = state + w * C::kState;
-                const float mw = s[C::kCols * D + n], fw = mw == -INFINITY ? 0.f : ex2(mw - m);
+                const float *s = states + k * C::kState;
+                const float mk = s[C::kCols * D + n], fk = mk == -INFINITY ? 0.f : ex2(mk - m);
                 const float4 v = *reinterpret_cast<const float4 *>(s + n * D + d);
-                l = fmaf(fw, s[C::kCols * D + C::kCols + n], l);
-                o.x = fmaf(fw, v.x, o.x), o.y = fmaf(fw, v.y, o.y), o.z = fmaf(fw, v.z, o.z), o.w = fmaf(fw, v.w, o.w);
+                l = fmaf(fk, s[C::kCols * D + C::kCols + n], l);
+                o.x = fmaf(fk, v.x, o.x), o.y = fmaf(fk, v.y, o.y), o.z = fmaf(fk, v.z, o.z), o.w = fmaf(fk, v.w, o.w);
             }
-            if (whole_seg) {
+            if (whole) {
                 write_column4<D>(g, at.b, at.seg, C::kCols, n, d, o, m, l);
             } else {
                 *reinterpret_cast<float4 *>(part + n * D + d) = o;
@@ -637,27 +674,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
                     part[C::kCols * D + n] = m, part[C::kCols * D + C::kCols + n] = l;
             }
         }
-        __syncthreads();
-        pos = stop;
-        if (pos < end) { /* the next segment that has tiles */
-            at.seg_begin = seg_end;
-            at.tile = 0;
-            if (++at.seg == g.segs) {
-                at.seg = 0;
-                do
-                    ++at.b;
-                while (at.b < g.a.seqs - 1 && tiles_of(g, at.b) == 0);
-                at.tiles = tiles_of(g, at.b);
-            }
-        }
-    }
+        worker_sync(warp / kGroup);
+    } while (at.next(g, range));
     if (!alive) /* a wait ran out: the copies still in flight, before the memory goes */
         for (int i = 0; i < C::kStages; ++i)
             if (const int n = (issued + C::kStages - 1 - i) / C::kStages)
                 mbar_wait_suspend_bounded(bar + i, (n - 1) & 1, &g_kv4_error);
 }
 
-/* Joins the parts of the segment that begins in range blockIdx.x and runs on past it. */
+/* Joins the parts of the segment that begins in worker blockIdx.x's range and runs on
+ * past it. */
 template <int D, int NT>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const Args g)
 {
@@ -667,14 +693,12 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Args g)
     asm volatile("griddepcontrol.wait;" ::: "memory"); /* in every CTA: this kernel ends after the one before */
     if (i + 1 >= plan.parts || plan.units == 0)
         return;
-    const int64_t end = plan.begin(i + 1);
-    if (plan.begin(i) == end)
+    const int64_t begin = plan.begin(i), end = plan.begin(i + 1);
+    const Walk at = locate(g, end - 1);
+    const int64_t first = end - 1 + at.first; /* the segment's first tile in the row */
+    if (first < begin || first >= end || first + at.tiles <= end)
         return;
-    const At at = locate(g, end - 1);
-    const int64_t seg_end = at.seg_begin + at.tiles;
-    if (seg_end <= end || at.seg_begin < plan.begin(i))
-        return;
-    const int last = plan.owner(seg_end - 1);
+    const int last = plan.owner(first + at.tiles - 1);
     for (int e = threadIdx.x; e < C::kCols * (D / 4); e += 256) {
         const int n = e / (D / 4), d = e % (D / 4) * 4;
         float m = -INFINITY, l = 0.f;
@@ -700,7 +724,7 @@ __global__ void __launch_bounds__(256) kv4_weight_kernel(const Args g)
     if (t >= len)
         return;
     const int cap = g.a.max_pages * g.c.page_size;
-    const int page = g.a.table[(int64_t)b * g.a.max_pages + t / g.c.page_size];
+    const int page = g.a.table[(int64_t)b * g.a.max_pages + (t >> g.page_log2)];
     const float *s = g.score + ((int64_t)bh * cap + t) * g.cols, *z = g.lse2 + (int64_t)bh * g.cols;
     float sum = 0.f;
     if (page >= 0 && page < g.c.pages)
@@ -732,7 +756,8 @@ Work work_of(const GlintKv4Cache &c, const GlintKv4Attn &a)
 {
     const int64_t cols = (int64_t)a.heads / c.kv_heads * a.rows, kcols = cols <= 8 ? 8 : 16;
     Work w;
-    w.part = (int64_t)sm_count() * 2 * (kcols * c.head_dim + 2 * kcols) * 4;
+    /* 16 warps a CTA for 8 columns, 8 for 16: the same bytes */
+    w.part = (int64_t)sm_count() * (kcols == 8 ? 4 : 2) * 2 * (kcols * c.head_dim + 2 * kcols) * 4;
     w.lse2 = a.weight_out ? ((int64_t)a.seqs * c.kv_heads * cols * 4 + 15) / 16 * 16 : 0;
     w.score = a.weight_out ? (int64_t)a.seqs * c.kv_heads * a.max_pages * c.page_size * cols * 4 : 0;
     return w;
@@ -760,11 +785,12 @@ int launch(Args &g, cudaStream_t st)
         return kLaunch;
     g.chunks = (g.cols + C::kCols - 1) / C::kCols;
     g.segs = g.c.kv_heads * g.chunks;
-    g.min_units = C::kWarps / 2;
+    const int grid = sm_count();
+    g.parts = grid * (C::kWarps / kGroup);
     if (g.score)
-        kv4_attn_kernel<D, NT, true><<<g.parts, C::kWarps * 32, C::kSmem, st>>>(g);
+        kv4_attn_kernel<D, NT, true><<<grid, C::kWarps * 32, C::kSmem, st>>>(g);
     else
-        kv4_attn_kernel<D, NT, false><<<g.parts, C::kWarps * 32, C::kSmem, st>>>(g);
+        kv4_attn_kernel<D, NT, false><<<grid, C::kWarps * 32, C::kSmem, st>>>(g);
     if (cudaGetLastError() != cudaSuccess)
         return kLaunch;
     if (launch_after(kv4_join_kernel<D, NT>, dim3(g.parts), 256, st, g) != cudaSuccess) {
@@ -809,7 +835,8 @@ int glint_kv4_attn_stream(const GlintKv4Cache *c, const GlintKv4Attn *a, cudaStr
     Args g{};
     g.c = *c, g.a = *a;
     g.group = a->heads / c->kv_heads, g.cols = g.group * a->rows;
-    g.parts = sm_count();
+    while ((1 << g.page_log2) < c->page_size)
+        ++g.page_log2;
     const Work w = work_of(*c, *a);
     uint8_t *work = static_cast<uint8_t *>(a->work);
     g.part = reinterpret_cast<float *>(work);
