@@ -28,31 +28,30 @@
 #include "ptx.cuh"
 
 namespace glint {
-static __device__ int g_kv4_error = 0, g_kv4_error_taken = 0;
-int kv4_error_word(bool clear) { return read_error_word(g_kv4_error, g_kv4_error_taken, clear); }
-
 namespace {
 
 constexpr int kTile = 32;        /* slots a warp takes at a time */
-constexpr int kGroup = 4;        /* warps of a worker */
 constexpr int kJoin = 2;         /* what a segment costs beside its tiles, in tiles */
 constexpr int kWorker = 4;       /* a worker's range, at least */
 constexpr float kLazy = 8.f;     /* the running maximum may lag by 2^8 */
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-/* Two columns sets at most: 8 columns take 16 warps of 128 registers, 16 take 8 warps
- * of up to 255 (their accumulators are twice as many). */
+/* Workers of four warps.  An SM quarter shares 512 registers a lane among its warps:
+ * four of 128 for 8 columns; for 16 (twice the accumulators) three of 168 at head_dim 64,
+ * two of 255 at 128. */
+constexpr int kGroup = 4;
 template <int D, int NT>
 struct Cfg {
-    static constexpr int kWarps = NT == 1 ? 16 : 8;
-    static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);
+    static constexpr int kWarps = NT == 1 ? 16 : D == 64 ? 12 : 8;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kStages = NT == 1 && D == 128 ? 2 : 4;
     static constexpr int kCols = 8 * NT;
     static constexpr int kNb = D / 64;
     static constexpr int kCode = kTile * D / 2, kMeta = kTile * kNb * 4;
     static constexpr int kStage = 2 * (kCode + kMeta);
     static constexpr int kState = kCols * D + 2 * kCols; /* floats: O, m, l */
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + kWarps * kState * 4 + kWarps * kStages * 16 + kWarps * 4 + 16;
+    static constexpr int kSmem = kRing + kWarps * kState * 4 + kWarps * 4;
 };
 
 struct Args {
@@ -60,7 +59,7 @@ struct Args {
     GlintKv4Attn a;
     int group, cols;      /* query heads a kv head; group * rows */
     int chunks, segs;     /* column chunks a kv head; segments a sequence = kv_heads * chunks */
-    int parts;            /* workers at most: warps of the grid / kGroup */
+    int parts;            /* workers at most: workers of a CTA times CTAs */
     int page_log2;
     float *part;          /* [parts][2][kState] unfinished segments */
     float *score;         /* [seqs][kv_heads][max slots][cols] log2-scaled scores, or NULL */
@@ -80,7 +79,7 @@ __device__ __forceinline__ int length_of(const Args &g, int b)
 __device__ __forceinline__ int tiles_of(const Args &g, int b) { return (length_of(g, b) + kTile - 1) / kTile; }
 
 /* All segments in one row (sequence after sequence), each as long as kJoin plus its
- * tiles, cut into equal ranges over the workers (four warps each): sequences of any mix
+ * tiles, cut into equal ranges over the workers (kGroup warps each): sequences of any mix
  * of lengths keep every SM busy, and a range of many short segments, each with a query
  * to load and a result to write, is not taken for as little work as one long one. */
 struct Plan {
@@ -227,6 +226,7 @@ __device__ __forceinline__ void load_query(const Args &g, int b, int seg, Query<
 {
     const int h = seg / g.chunks, ch = seg - h * g.chunks;
     const int gr = lane >> 2, c = lane & 3;
+    const uint32_t sign = g.a.scale < 0.f ? 0x8000u : 0u; /* the kernel scales by |scale| */
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int col = ch * 8 * NT + n * 8 + gr;
@@ -239,7 +239,7 @@ __device__ __forceinline__ void load_query(const Args &g, int b, int seg, Query<
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                v[i] = live ? (uint32_t)__bfloat16_as_ushort(p[64 * k + i]) : 0u;
+                v[i] = live ? (uint32_t)__bfloat16_as_ushort(p[64 * k + i]) ^ sign : 0u;
                 s += __uint_as_float(v[i] << 16);
             }
 #pragma unroll
@@ -283,7 +283,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    acc[k][n][i] = -136.f * q.sum[n][k][i & 1]; /* 128 + code, less 136 */
+                    acc[k][n][i] = 0.f;
             const uint2 wa = lds64(kcode + ta * RB + kv4_unit<D>(k, ta) + 8 * c);
             const uint2 wb = lds64(kcode + tb * RB + kv4_unit<D>(k, tb) + 8 * c);
 #pragma unroll
@@ -303,8 +303,8 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
         for (int k = 0; k < NB; ++k) {
             const uint32_t ma = lds32(kmeta + (ta * NB + k) * 4), mb = lds32(kmeta + (tb * NB + k) * 4);
             const float sa = __uint_as_float(ma << 16), sb = __uint_as_float(mb << 16);
-            const float la = fmaf(8.f, sa, __uint_as_float(ma & 0xFFFF0000u));
-            const float lb = fmaf(8.f, sb, __uint_as_float(mb & 0xFFFF0000u));
+            const float la = fmaf(-128.f, sa, __uint_as_float(ma & 0xFFFF0000u));
+            const float lb = fmaf(-128.f, sb, __uint_as_float(mb & 0xFFFF0000u));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 s[sl][n][0] = fmaf(sa, acc[k][n][0], fmaf(la, q.sum[n][k][0], s[sl][n][0]));
@@ -318,7 +318,6 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = i < 2 ? ta : tb;
-                s[sl][n][i] *= scale2;
                 if (!WHOLE && (!((valid >> t) & 1u) || t0 + t >= q.see[n][i & 1]))
                     s[sl][n][i] = -INFINITY;
             }
@@ -331,9 +330,9 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
                     float *p = score + (int64_t)(t0 + (i ? tb : ta)) * g.cols + col;
                     if (WHOLE || ((valid >> (i ? tb : ta)) & 1u)) {
                         if (col < g.cols)
-                            p[0] = s[sl][n][2 * i];
+                            p[0] = s[sl][n][2 * i] * scale2;
                         if (col + 1 < g.cols)
-                            p[1] = s[sl][n][2 * i + 1];
+                            p[1] = s[sl][n][2 * i + 1] * scale2;
                     }
                 }
             }
@@ -349,6 +348,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1)
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], off));
+            top[i] *= scale2;
         }
         const bool grow = top[0] > st.m[n][0] + kLazy || top[1] > st.m[n][1] + kLazy ||
                           (st.m[n][0] == -INFINITY && top[0] != -INFINITY) ||
@@ -370,6 +370,12 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             }
         }
     }
+    float less[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            less[n][i] = st.m[n][i] == -INFINITY ? 0.f : -st.m[n][i];
 #pragma unroll
     for (int sl = 0; sl < 2; ++sl) {
         const int ta = sl * 16 + tg, tb = ta + 8;
@@ -387,22 +393,19 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float m = st.m[n][i & 1];
-                p[i] = ex2(s[sl][n][i] - (m == -INFINITY ? 0.f : m));
+                p[i] = ex2(fmaf(s[sl][n][i], scale2, less[n][i & 1]));
                 st.l[n][i & 1] += p[i];
             }
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                float w[4], x[4];
+                float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    w[i] = p[i] * steps[k][i >> 1], x[i] = p[i] * mids[k][i >> 1];
                     /* a masked slot's step and lo may be anything, NaN too */
-                    if (!WHOLE && s[sl][n][i] == -INFINITY)
-                        w[i] = x[i] = 0.f;
+                    const bool out = !WHOLE && s[sl][n][i] == -INFINITY;
+                    w[i] = out ? 0.f : p[i] * steps[k][i >> 1];
+                    st.lo[n][k][i & 1] = out ? st.lo[n][k][i & 1] : fmaf(p[i], mids[k][i >> 1], st.lo[n][k][i & 1]);
                 }
-                st.lo[n][k][0] += x[0] + x[2];
-                st.lo[n][k][1] += x[1] + x[3];
                 pb[n][k][0] = transpose8x8(pack2(w[0], w[1]));
                 pb[n][k][1] = transpose8x8(pack2(w[2], w[3]));
             }
@@ -427,64 +430,74 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
     }
 }
 
-/* a warp's next tile to fetch, and the pages that hold it */
+/* A warp's walk over the tiles it fetches. */
 struct Fetch {
     Walk w;
-    int tile; /* -1: none left */
-    int page; /* lanes 0 and 1: the page of the tile's slots 0-15 and 16-31, -1 for none */
+    int tile; /* the next one, -1: none left */
+    int len;  /* its sequence's length */
+    int page; /* lanes 0 and 1: the page of its slots 0-15 and 16-31, -1 for none */
 };
 __device__ __forceinline__ void fetch_seek(const Args &g, Fetch &f, int range, int lane)
 {
     while (f.tile >= f.w.hi(range)) {
         f.tile -= max(f.w.hi(range), f.w.lo());
+        const int b = f.w.b;
         if (!f.w.next(g, range)) {
             f.tile = -1;
             return;
         }
+        if (f.w.b != b)
+            f.len = length_of(g, f.w.b);
     }
     const int t = f.tile * kTile + 16 * lane;
     f.page = -1;
-    if (lane < 2 && t < length_of(g, f.w.b))
+    if (lane < 2 && t < f.len)
         f.page = g.a.table[(int64_t)f.w.b * g.a.max_pages + (t >> g.page_log2)];
 }
-/* copy the tile into a stage; its valid slots go to *valid */
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+/* start copying the tile into a stage (16 bytes a lane and copy); returns its valid slots */
 template <int D, int NT>
-__device__ __forceinline__ void fetch_issue(const Args &g, const Fetch &f, uint8_t *stage, uint64_t *bar,
-                                            uint32_t *valid, int lane)
+__device__ __forceinline__ uint32_t fetch_issue(const Args &g, const Fetch &f, uint32_t stage, int lane)
 {
     using C = Cfg<D, NT>;
-    const int len = length_of(g, f.w.b), t0 = f.tile * kTile;
-    const bool ok = f.page >= 0 && f.page < g.c.pages;
-    const uint32_t half = __ballot_sync(0xFFFFFFFFu, ok) & 3u;
+    constexpr int N = C::kCode / 512, M = C::kMeta / 16;
+    const int t0 = f.tile * kTile, h = f.w.seg / g.chunks;
+    const uint32_t half = __ballot_sync(0xFFFFFFFFu, f.page >= 0 && f.page < g.c.pages);
     const int p0 = __shfl_sync(0xFFFFFFFFu, f.page, 0), p1 = __shfl_sync(0xFFFFFFFFu, f.page, 1);
-    const bool split = g.c.page_size == 16; /* two pages a tile, else one */
-    const int h = f.w.seg / g.chunks;
-    if (lane == 0) {
-        uint32_t v = ((half & 1u) ? 0xFFFFu : 0u) | ((half & 2u) ? 0xFFFF0000u : 0u);
-        if (t0 + kTile > len)
-            v &= (1u << (len - t0)) - 1u; /* len > t0 */
-        *valid = v;
-        const uint32_t n = split ? __popc(half) * (C::kStage / 2) : (half ? C::kStage : 0);
-        mbar_expect_tx(bar, n);
-    }
-    __syncwarp();
-    if (lane < 4) {
-        const bool code = !(lane & 1), key = lane < 2;
-        const uint8_t *src = key ? (code ? g.c.k_code : reinterpret_cast<const uint8_t *>(g.c.k_meta))
-                                 : (code ? g.c.v_code : reinterpret_cast<const uint8_t *>(g.c.v_meta));
-        const int row = code ? D / 2 : D / 16; /* bytes a slot */
-        uint8_t *dst = stage + (key ? 0 : C::kCode + C::kMeta) + (code ? 0 : C::kCode);
-        const int slot = t0 & (g.c.page_size - 1);
-        if (!split) {
-            if (half)
-                bulk_g2s(dst, src + ((((int64_t)p0 * g.c.kv_heads + h) << g.page_log2) + slot) * row, kTile * row, bar);
-        } else {
-            if (half & 1u)
-                bulk_g2s(dst, src + ((int64_t)p0 * g.c.kv_heads + h) * 16 * row, 16 * row, bar);
-            if (half & 2u)
-                bulk_g2s(dst + 16 * row, src + ((int64_t)p1 * g.c.kv_heads + h) * 16 * row, 16 * row, bar);
+    /* rows of slots 0 and 16: the halves are in two pages or 16 rows apart in one */
+    const int in = t0 & (g.c.page_size - 1);
+    const int64_t r0 = (((int64_t)p0 * g.c.kv_heads + h) << g.page_log2) + in;
+    const int64_t r1 = g.page_log2 == 4 ? ((int64_t)p1 * g.c.kv_heads + h) << 4 : r0 + 16;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int u = i >= N / 2;
+        if ((half >> u) & 1u) {
+            const int at = (lane + 32 * i) * 16;
+            const int64_t src = (u ? r1 : r0) * (D / 2) + at - u * (C::kCode / 2);
+            copy16(stage + at, g.c.k_code + src);
+            copy16(stage + C::kCode + C::kMeta + at, g.c.v_code + src);
         }
     }
+    const int m = lane & (M - 1), u = m >= M / 2;
+    if (lane < 2 * M && ((half >> u) & 1u)) {
+        const bool key = lane < M;
+        const uint16_t *meta = key ? g.c.k_meta : g.c.v_meta;
+        copy16(stage + (key ? 0 : C::kCode + C::kMeta) + C::kCode + m * 16,
+               reinterpret_cast<const uint8_t *>(meta) + (u ? r1 : r0) * (D / 16) + m * 16 - u * (C::kMeta / 2));
+    }
+    uint32_t v = ((half & 1u) ? 0xFFFFu : 0u) | ((half & 2u) ? 0xFFFF0000u : 0u);
+    if (t0 + kTile > f.len)
+        v &= (1u << (f.len - t0)) - 1u; /* len > t0 */
+    return v;
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() /* all but the newest N groups have landed */
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 /* columns [0, cols) of one segment from its joined state: thread i of n */
@@ -511,9 +524,10 @@ __device__ __forceinline__ void write_column4(const Args &g, int b, int seg, int
 }
 
 /* barrier of one worker's warps */
+template <int WARPS>
 __device__ __forceinline__ void worker_sync(int i)
 {
-    asm volatile("bar.sync %0, %1;" ::"r"(i + 1), "n"(kGroup * 32) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(i + 1), "n"(WARPS * 32) : "memory");
 }
 
 /* a warp's state to shared memory (O by column, m, l), the lo terms added in */
@@ -551,14 +565,12 @@ __device__ __forceinline__ void store_state(const State<D, NT> &st, float *mem, 
 }
 
 template <int D, int NT, bool SCORE>
-__global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(const Args g)
+__global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) kv4_attn_kernel(const Args g)
 {
     using C = Cfg<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     float *state = reinterpret_cast<float *>(smem + C::kRing);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kWarps * C::kState * 4);
-    uint32_t *valids = reinterpret_cast<uint32_t *>(bars + C::kWarps * C::kStages);
-    int *used = reinterpret_cast<int *>(valids + C::kWarps * C::kStages);
+    int *used = reinterpret_cast<int *>(state + C::kWarps * C::kState);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Plan plan = plan_of(g);
     asm volatile("griddepcontrol.launch_dependents;");
@@ -566,7 +578,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
     /* sequences without a slot: no tile reaches them */
     for (int b = blockIdx.x; b < g.a.seqs; b += gridDim.x)
         if (length_of(g, b) == 0)
-            for (int i = threadIdx.x; i < g.segs * C::kCols * (D / 4); i += C::kWarps * 32) {
+            for (int i = threadIdx.x; i < g.segs * C::kCols * (D / 4); i += C::kThreads) {
                 const int seg = i / (C::kCols * (D / 4)), e = i % (C::kCols * (D / 4));
                 write_column4<D>(g, b, seg, C::kCols, e / (D / 4), e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f),
                                  -INFINITY, 0.f);
@@ -577,35 +589,27 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
         return;
     const int64_t begin = plan.begin(worker);
     const int range = (int)(plan.begin(worker + 1) - begin);
-
-    uint8_t *ring = smem + warp * C::kStages * C::kStage;
-    uint64_t *bar = bars + warp * C::kStages;
-    uint32_t *valid = valids + warp * C::kStages;
-    if (lane == 0) {
-        for (int i = 0; i < C::kStages; ++i)
-            mbar_init(bar + i, 1);
-        mbar_init_fence();
-    }
-    __syncwarp();
-
-    const float scale2 = g.a.scale * kLog2e;
     Walk at = locate(g, begin);
-    Fetch f{at, at.lo() + w, -1};
+
+    const uint32_t ring = saddr(smem + warp * C::kStages * C::kStage);
+    const float scale2 = fabsf(g.a.scale) * kLog2e;
+    uint32_t valid[C::kStages]; /* of the tiles on their way, in order */
+    Fetch f{at, at.lo() + w, length_of(g, at.b), -1};
     fetch_seek(g, f, range, lane);
-    int issued = 0; /* copies this warp has started, a stage each */
-    int slot = 0;   /* the stage it reads next, and the parity of its phase */
-    uint32_t phase = 0;
-    bool alive = true;
     auto fetch = [&](int stage) {
-        if (f.tile < 0 || !alive)
-            return;
-        fetch_issue<D, NT>(g, f, ring + stage * C::kStage, bar + stage, valid + stage, lane);
-        ++issued;
-        f.tile += kGroup;
-        fetch_seek(g, f, range, lane);
+        uint32_t v = 0;
+        if (f.tile >= 0) {
+            v = fetch_issue<D, NT>(g, f, ring + stage * C::kStage, lane);
+            f.tile += kGroup;
+            fetch_seek(g, f, range, lane);
+        }
+        copies_commit();
+        return v;
     };
+#pragma unroll
     for (int i = 0; i < C::kStages; ++i)
-        fetch(i);
+        valid[i] = fetch(i);
+    int slot = 0; /* the stage to read next */
 
     Query<D, NT> q;
     State<D, NT> st;
@@ -625,24 +629,26 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
         float *score = SCORE ? g.score + ((int64_t)at.b * g.c.kv_heads + h) * g.a.max_pages * g.c.page_size * g.cols
                              : nullptr;
         for (; tile < hi; tile += kGroup) {
-            if (alive)
-                alive = mbar_wait_suspend_bounded(bar + slot, phase, &g_kv4_error);
-            const uint32_t v = valid[slot], stage = saddr(ring + slot * C::kStage);
+            copies_wait<C::kStages - 1>();
+            __syncwarp();
+            const uint32_t v = valid[0], stage = ring + slot * C::kStage;
             if (v == 0xFFFFFFFFu && tile * kTile + kTile <= len - g.a.rows + 1)
                 tile_step<D, NT, SCORE, true>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);
             else
                 tile_step<D, NT, SCORE, false>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);
             __syncwarp();
-            fetch(slot);
-            if (++slot == C::kStages)
-                slot = 0, phase ^= 1u;
+#pragma unroll
+            for (int i = 1; i < C::kStages; ++i)
+                valid[i - 1] = valid[i];
+            valid[C::kStages - 1] = fetch(slot);
+            slot = slot + 1 == C::kStages ? 0 : slot + 1;
         }
         turn = tile - hi;
         if (mine)
             store_state<D, NT>(st, mem, lane);
         if (lane == 0)
             used[warp] = mine ? 1 : 0;
-        worker_sync(warp / kGroup);
+        worker_sync<kGroup>(warp / kGroup);
         /* joined over the warps in their order; the whole segment, or a part of it for the join kernel */
         const bool first = at.first >= 0, whole = first && at.first + at.tiles <= range;
         float *part = g.part + ((int64_t)worker * 2 + (first ? 1 : 0)) * C::kState;
@@ -674,12 +680,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kWarps * 32, 1) kv4_attn_kernel(co
                     part[C::kCols * D + n] = m, part[C::kCols * D + C::kCols + n] = l;
             }
         }
-        worker_sync(warp / kGroup);
+        worker_sync<kGroup>(warp / kGroup);
     } while (at.next(g, range));
-    if (!alive) /* a wait ran out: the copies still in flight, before the memory goes */
-        for (int i = 0; i < C::kStages; ++i)
-            if (const int n = (issued + C::kStages - 1 - i) / C::kStages)
-                mbar_wait_suspend_bounded(bar + i, (n - 1) & 1, &g_kv4_error);
 }
 
 /* Joins the parts of the segment that begins in worker blockIdx.x's range and runs on
@@ -748,7 +750,7 @@ int check(const GlintKv4Cache *c, const GlintKv4Attn *a)
     return kOk;
 }
 
-/* bytes of the parts, rounded up; of the log2 sums; of the scores */
+/* bytes of the parts; of the log2 sums, rounded up; of the scores */
 struct Work {
     int64_t part, lse2, score;
 };
@@ -756,8 +758,7 @@ Work work_of(const GlintKv4Cache &c, const GlintKv4Attn &a)
 {
     const int64_t cols = (int64_t)a.heads / c.kv_heads * a.rows, kcols = cols <= 8 ? 8 : 16;
     Work w;
-    /* 16 warps a CTA for 8 columns, 8 for 16: the same bytes */
-    w.part = (int64_t)sm_count() * (kcols == 8 ? 4 : 2) * 2 * (kcols * c.head_dim + 2 * kcols) * 4;
+    w.part = 2 * (int64_t)sm_count() * (kcols == 8 ? Cfg<64, 1>::kWarps : Cfg<64, 2>::kWarps) / kGroup * (kcols * c.head_dim + 2 * kcols) * 4; /* workers an SM, at most */
     w.lse2 = a.weight_out ? ((int64_t)a.seqs * c.kv_heads * cols * 4 + 15) / 16 * 16 : 0;
     w.score = a.weight_out ? (int64_t)a.seqs * c.kv_heads * a.max_pages * c.page_size * cols * 4 : 0;
     return w;
@@ -788,9 +789,9 @@ int launch(Args &g, cudaStream_t st)
     const int grid = sm_count();
     g.parts = grid * (C::kWarps / kGroup);
     if (g.score)
-        kv4_attn_kernel<D, NT, true><<<grid, C::kWarps * 32, C::kSmem, st>>>(g);
+        kv4_attn_kernel<D, NT, true><<<grid, C::kThreads, C::kSmem, st>>>(g);
     else
-        kv4_attn_kernel<D, NT, false><<<grid, C::kWarps * 32, C::kSmem, st>>>(g);
+        kv4_attn_kernel<D, NT, false><<<grid, C::kThreads, C::kSmem, st>>>(g);
     if (cudaGetLastError() != cudaSuccess)
         return kLaunch;
     if (launch_after(kv4_join_kernel<D, NT>, dim3(g.parts), 256, st, g) != cudaSuccess) {
