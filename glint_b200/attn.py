@@ -27,7 +27,7 @@ _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_
 
 class _Prompt(ctypes.Structure):
     """struct GlintAttnPrompt"""
-    _fields_ = [(n, _vp) for n in ("q", "k", "v", "o", "lse", "cu_q", "cu_k")] + \
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "o", "lse", "cu_q", "cu_k", "work")] + \
                [(n, _i64) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "o_tok", "o_head")] + \
                [(n, _i32) for n in ("seqs", "q_tokens", "k_tokens", "heads", "kv_heads", "head_dim", "causal")] + \
                [("scale", _f32)]
@@ -55,6 +55,7 @@ class _Evict(ctypes.Structure):
 
 def bind(L: ctypes.CDLL) -> ctypes.CDLL:
     P = ctypes.POINTER
+    L.glint_attn_prompt_work_bytes.argtypes = [P(_Prompt)]
     L.glint_attn_prompt_stream.argtypes = [P(_Prompt), _vp]
     L.glint_kv4_append_stream.argtypes = [P(_Cache), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp]
     L.glint_kv4_read_stream.argtypes = [P(_Cache), _vp, _i32, _vp, _vp, _vp]
@@ -64,7 +65,7 @@ def bind(L: ctypes.CDLL) -> ctypes.CDLL:
     for f in (L.glint_attn_prompt_stream, L.glint_kv4_append_stream, L.glint_kv4_read_stream,
               L.glint_kv4_attn_stream, L.glint_kv4_evict_stream):
         f.restype = _i32
-    L.glint_kv4_attn_work_bytes.restype = _i64
+    L.glint_attn_prompt_work_bytes.restype = L.glint_kv4_attn_work_bytes.restype = _i64
     return L
 
 
@@ -136,10 +137,16 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     _want(out, "out", torch.bfloat16, (T, H, D), dense=False)
     _want(lse, "lse", torch.float32, (H, T))
     a = _Prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
-                cu_k.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                cu_k.data_ptr(), None, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                 out.stride(0), out.stride(1), cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0,
                 D ** -0.5 if scale is None else scale)
-    _check(_lib().glint_attn_prompt_stream(a, _stream(stream)), "glint_attn_prompt_stream")
+    L = _lib()
+    n = L.glint_attn_prompt_work_bytes(a)
+    if n > 0:
+        with _on(stream):
+            work = torch.empty(n, dtype=torch.uint8, device=q.device)
+        a.work = work.data_ptr()
+    _check(L.glint_attn_prompt_stream(a, _stream(stream)), "glint_attn_prompt_stream")
     return out, lse
 
 

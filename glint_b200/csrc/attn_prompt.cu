@@ -1,9 +1,30 @@
-/* Causal attention over packed prompts with grouped heads.
+/* Causal attention over packed prompts with grouped heads, on tcgen05.
  *
- * One warp per query row: a lane holds D / 32 values of q and of the output (element
- * lane + 32 i, so loads are coalesced at any alignment), each key's score is a shuffle
- * sum, and the running maximum and sum of the softmax rescale the output as they
- * change.  Simple and right for every case.
+ * A CTA takes two tiles of up to 128 query rows of one sequence and one kv head: rows
+ * are (token, query head of the group) pairs, group * (128 / group) of them, so the
+ * group's heads share every K and V tile that is loaded.  Per tile of 128 keys
+ *
+ *   S = Q K^T          UMMA 128 x 128 x D, Q and K in shared memory (TMA, 128-byte swizzle)
+ *   P = 2^(S c - m)    a thread per row: S from TMEM, running maximum m and sum l in f32,
+ *                      P as BF16 back into S's columns (2^-8 of each weight at most, the
+ *                      rounding that the tensor cores' operand asks for)
+ *   O += P V           UMMA 128 x D x 128, P from TMEM, V as it lies (inner index = key rows)
+ *
+ * Where the weights are many, their roundings cancel; a row of few keys, or of a few that
+ * carry most of it, would show them.  So a tile of keys in which some row has a weight
+ * above 1/16 of its running sum also gets what the rounding dropped, as a second BF16
+ * operand (a sequence's first tile nearly always, later ones as peaked as they are).
+ *
+ * The two tiles take turns: while one's softmax runs, the tensor cores work on the
+ * other.  m may lag behind the true maximum by 2^8, so O is rescaled rarely.  Few blocks
+ * with many keys are cut along the keys and joined by a second kernel.
+ *
+ * Masked scores are replaced, never added to, and a masked weight is 0; a NaN or an
+ * infinity in V would still reach other rows as 0 * NaN, so tiles with masked places
+ * are looked through, and where one is found the rows are done one by one instead.
+ *
+ * Bound: exponentials (16 a clock and SM) and the tensor cores take the same time at
+ * D = 128, 2048 clocks for two tiles.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -13,11 +34,15 @@
 #include "../../include/glint_attn.h"
 #include "common.cuh"
 #include "glint_internal.h"
+#include "ptx.cuh"
 
 namespace glint {
+static __device__ int g_attn_error = 0, g_attn_error_taken = 0;
+int attn_error_word(bool clear) { return read_error_word(g_attn_error, g_attn_error_taken, clear); }
+
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4; /* of the plain kernel */
 
 /* sequence of query token t and its bounds; false for a token outside every sequence */
 struct Span {
@@ -41,8 +66,9 @@ __device__ __forceinline__ bool span_of(const GlintAttnPrompt &a, int t, Span &s
     return true;
 }
 
+/* one query row by one warp, in f32: right for any stride, alignment and value */
 template <int D>
-__device__ void plain_row(const GlintAttnPrompt &a, const Span &s, int t, int hq, int lane)
+__device__ __forceinline__ void plain_row(const GlintAttnPrompt &a, const Span &s, int t, int hq, int lane)
 {
     const int h = hq / (a.heads / a.kv_heads);
     const int seen = a.causal ? min(s.k1 - s.k0, t - s.q0 + 1 + (s.k1 - s.k0) - (s.q1 - s.q0)) : s.k1 - s.k0;
@@ -99,21 +125,760 @@ int plain_launch(const GlintAttnPrompt &a, cudaStream_t st)
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
+
+/* ---- tensor-core kernel ------------------------------------------------------------ */
+constexpr int kRows = 128, kKeys = 128;
+constexpr float kLazy = 8.f;   /* the running maximum may lag by 2^8 */
+constexpr float kHeavy = 15.f; /* a weight above 1 / (1 + kHeavy) of the running sum keeps its low half */
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int D>
+struct Cfg {
+    static constexpr int kTileBytes = kKeys * D * 2;
+    static constexpr int kStages = D == 128 ? 2 : 4; /* of K, and of V */
+    static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + 256;
+    /* TMEM columns: S of tile i at 128 i, O at 256 + D i.  In S's place, for 32 keys a
+     * time, 16 columns of P and 16 of what P's rounding dropped. */
+    static constexpr uint32_t kS = 0, kO = 256;
+};
+constexpr int kThreads = 384; /* warps 0-3, 4-7: softmax of the two tiles; 8: loads; 9: UMMA; 10, 11 idle */
+constexpr int kSlotRows = 2 * kRows;
+
+struct Args {
+    GlintAttnPrompt a;
+    int group, tok;    /* query heads a kv head; tokens a tile */
+    int sms;
+    bool vec;          /* o takes 16-byte stores */
+    bool split;        /* there is a workspace for parts */
+    float *part;       /* [slot][256][D], then m, l [slot][256] each, then bad [slot] */
+};
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r)
+{
+    tmem_st16(taddr, r);
+    tmem_st16(taddr + 16, r + 16);
+}
+/* the loads into r have arrived: its values are this statement's, so no use moves ahead of it */
+__device__ __forceinline__ void tmem_ld_wait(uint32_t *r)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+/* UMMA shared-memory descriptors, 128-byte swizzle, version 1.  Inner index contiguous
+ * (Q, K): 8-row atoms of 1024 B.  Outer index contiguous (V: 64 of D by 8 keys an atom):
+ * the next 64 of D lie a box of 128 keys further, the next 8 keys 1024 B further. */
+__device__ __forceinline__ uint64_t desc_base(uint32_t sa)
+{
+    return (uint64_t)((sa >> 4) & 0x3FFF) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_inner(uint32_t sa) { return desc_base(sa) | ((uint64_t)1 << 16); }
+__device__ __forceinline__ uint64_t desc_outer(uint32_t sa)
+{
+    return desc_base(sa) | ((uint64_t)(kKeys * 128 >> 4) << 16);
+}
+/* f32 accumulate, BF16 A and B, M = 128; bit 16: B has its outer index contiguous */
+constexpr uint32_t idesc_of(int n, bool outer_b)
+{
+    return (1u << 4) | (1u << 7) | (1u << 10) | (outer_b ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ uint64_t pack2f(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2f(uint64_t v, float &lo, float &hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+/* The blocks (two tiles of one sequence) of all sequences in one row, each with every kv
+ * head; the last blocks of a sequence see the most keys and go first.  Where there are
+ * at most half as many as SMs, the keys of each are cut into parts of kCut tiles or more
+ * (a part costs its block's rows in f32, written and read: 130 KB each way). */
+constexpr int kCut = 4;
+struct Item {
+    Span s;
+    int block, head, cut, cuts, slot;
+};
+__device__ __forceinline__ int blocks_of(const Args &g, int seq)
+{
+    const int n = bound(g.a.cu_q, seq + 1, g.a.q_tokens) - bound(g.a.cu_q, seq, g.a.q_tokens);
+    return max(0, (n + 2 * g.tok - 1) / (2 * g.tok));
+}
+__device__ __forceinline__ int seen_of(const Args &g, const Span &s, int t);
+/* tiles of keys that an item's two query tiles see */
+__device__ __forceinline__ void tiles_of(const Args &g, const Item &it, int (&n)[2])
+{
+    const int t0 = it.s.q0 + it.block * 2 * g.tok;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int end = min(it.s.q1, t0 + (i + 1) * g.tok); /* one past the tile's last token */
+        n[i] = end > t0 + i * g.tok ? (seen_of(g, it.s, end - 1) + kKeys - 1) / kKeys : 0;
+    }
+}
+/* the whole warp; false past the last item */
+__device__ __forceinline__ bool item_of(const Args &g, int index, Item &it)
+{
+    const int lane = threadIdx.x & 31;
+    int64_t blocks = 0;
+    for (int b = lane; b < g.a.seqs; b += 32)
+        blocks += blocks_of(g, b);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+        blocks += __shfl_xor_sync(0xFFFFFFFFu, blocks, off);
+    const int64_t items = blocks * g.a.kv_heads;
+    const int cuts = g.split && items > 0 ? (int)max((int64_t)1, g.sms / items) : 1;
+    if (index >= items * cuts)
+        return false;
+    it.slot = index, it.cut = index % cuts, it.cuts = cuts;
+    const int rest = index / cuts;
+    it.head = rest % g.a.kv_heads;
+    const int64_t want = blocks - 1 - rest / g.a.kv_heads;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < g.a.seqs; b0 += 32) {
+        const int n = b0 + lane < g.a.seqs ? blocks_of(g, b0 + lane) : 0;
+        int64_t sum = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t o = __shfl_up_sync(0xFFFFFFFFu, sum, off);
+            if (lane >= off)
+                sum += o;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > want);
+        if (past) {
+            const int l = __ffs(past) - 1, seq = b0 + l;
+            it.block = (int)(want - (before + __shfl_sync(0xFFFFFFFFu, sum - n, l)));
+            it.s.q0 = bound(g.a.cu_q, seq, g.a.q_tokens), it.s.q1 = bound(g.a.cu_q, seq + 1, g.a.q_tokens);
+            it.s.k0 = bound(g.a.cu_k, seq, g.a.k_tokens);
+            it.s.k1 = max(it.s.k0, bound(g.a.cu_k, seq + 1, g.a.k_tokens));
+            int tiles[2];
+            tiles_of(g, it, tiles);
+            it.cuts = min(cuts, max(1, max(tiles[0], tiles[1]) / kCut));
+            return true;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    }
+    return false;
+}
+/* keys that query token t of the item's sequence sees */
+__device__ __forceinline__ int seen_of(const Args &g, const Span &s, int t)
+{
+    const int keys = s.k1 - s.k0;
+    return g.a.causal ? min(keys, max(0, t - s.q0 + 1 + keys - (s.q1 - s.q0))) : keys;
+}
+/* first tile of a cut, of n tiles */
+__device__ __forceinline__ int cut_begin(int n, int cut, int cuts) { return (int)((int64_t)n * cut / cuts); }
+
+/* D values of one row: 16-byte stores where o allows */
+template <int D>
+__device__ __forceinline__ void store_row32(const Args &g, __nv_bfloat16 *o, const float (&v)[32])
+{
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&p);
+    }
+    if (g.vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<uint4 *>(o)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            o[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+/* any NaN or infinity among two BF16 */
+__device__ __forceinline__ uint32_t odd2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+
+/* whether any of a tile's 128 softmax threads has `p` */
+__device__ __forceinline__ bool any_of_tile(int i, bool p)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                 : "=r"(r)
+                 : "r"((uint32_t)p), "r"(1 + i)
+                 : "memory");
+    return r != 0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant__ Args g, const __grid_constant__ Maps maps)
+{
+    using C = Cfg<D>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = raw + ((1024 - (saddr(raw) & 1023)) & 1023);
+    uint8_t *sq = smem, *sk = sq + 2 * C::kTileBytes, *sv = sk + C::kStages * C::kTileBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sv + C::kStages * C::kTileBytes);
+    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages,
+             *v_empty = v_full + C::kStages, *s_full = v_empty + C::kStages, *p_full = s_full + 2, *o_done = p_full + 4;
+    __shared__ uint32_t tmem_slot;
+    __shared__ Item s_item;
+    __shared__ int s_ok;
+    __shared__ int s_bad[2], s_low[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (warp == 0) {
+        Item it;
+        const bool ok = item_of(g, blockIdx.x, it) && it.cut < it.cuts;
+        if (lane == 0) {
+            s_item = it, s_ok = ok, s_bad[0] = s_bad[1] = 0;
+        }
+    } else if (warp == 8 && lane == 0) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < C::kStages; ++i)
+            mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + 2 * i, 4), mbar_init(p_full + 2 * i + 1, 4);
+        mbar_init_fence();
+    }
+    __syncthreads();
+    if (!s_ok)
+        return;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_slot;
+    const Item it = s_item;
+    const Span s = it.s;
+    /* tiles of keys that each query tile goes through: [first, last[i]) */
+    const int t0 = s.q0 + it.block * 2 * g.tok;
+    int n[2];
+    tiles_of(g, it, n);
+    const int most = max(n[0], n[1]);
+    const int first = cut_begin(most, it.cut, it.cuts), stop = cut_begin(most, it.cut + 1, it.cuts);
+    const int last[2] = {max(first, min(n[0], stop)), max(first, min(n[1], stop))};
+    bool alive = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (alive)
+            alive = mbar_wait_suspend_bounded(bar, parity, &g_attn_error);
+        return alive;
+    };
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity) {
+        wait(bar, parity);
+        __syncwarp();
+    };
+
+    if (warp == 8) {
+        /* ---- loads */
+        if (lane == 0 && first < stop) {
+            const int rows = g.group * g.tok;
+            mbar_expect_tx(q_full, 2 * (D / 64) * rows * 128);
+            for (int i = 0; i < 2; ++i)
+                for (int d = 0; d < D / 64; ++d)
+                    tma_load_3d(sq + i * C::kTileBytes + d * kRows * 128, &maps.q, q_full, d * 64, it.head * g.group,
+                                t0 + i * g.tok);
+            int issued = 0;
+            for (int j = first; j < stop && alive; ++j, ++issued) {
+                const int st = issued % C::kStages;
+                const uint32_t ph = (issued / C::kStages + 1) & 1; /* first use: returns at once */
+                const int key = s.k0 + j * kKeys;
+                if (!wait(k_empty + st, ph))
+                    break;
+                mbar_expect_tx(k_full + st, C::kTileBytes);
+                for (int d = 0; d < D / 64; ++d)
+                    tma_load_3d(sk + st * C::kTileBytes + d * kKeys * 128, &maps.k, k_full + st, d * 64, it.head, key);
+                if (!wait(v_empty + st, ph)) {
+                    ++issued; /* K of this one is in flight */
+                    break;
+                }
+                mbar_expect_tx(v_full + st, C::kTileBytes);
+                for (int d = 0; d < D / 64; ++d)
+                    tma_load_3d(sv + st * C::kTileBytes + d * kKeys * 128, &maps.v, v_full + st, d * 64, it.head, key);
+            }
+            if (!alive) { /* let the copies already started land before the CTA exits */
+                mbar_wait_bounded(q_full, 0, &g_attn_error);
+                for (int j = max(0, issued - C::kStages); j < issued; ++j) {
+                    mbar_wait_bounded(k_full + j % C::kStages, (j / C::kStages) & 1, &g_attn_error);
+                    mbar_wait_bounded(v_full + j % C::kStages, (j / C::kStages) & 1, &g_attn_error);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        /* ---- UMMA */
+        if (lane == 0 && first < stop) {
+            constexpr uint32_t kQk = idesc_of(kKeys, false), kPv = idesc_of(D, true);
+            auto scores = [&](int i, int st) { /* S_i = Q_i K^T */
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const uint32_t off = (d / 4) * kKeys * 128 + (d % 4) * 32;
+                    umma_ss(tmem + C::kS + 128 * i, desc_inner(saddr(sq) + i * C::kTileBytes + off),
+                            desc_inner(saddr(sk) + st * C::kTileBytes + off), kQk, d > 0);
+                }
+                umma_commit(s_full + i);
+            };
+            /* operands of 16 keys: P_i in TMEM, V in shared memory */
+            auto p_at = [&](int i, int k) { return tmem + C::kS + 128 * i + (k / 2) * 32 + (k % 2) * 8; };
+            auto v_at = [&](int st, int k) { return desc_outer(saddr(sv) + st * C::kTileBytes + k * 16 * 128); };
+            wait(q_full, 0);
+            wait(k_full, 0);
+            tc_after();
+            if (alive) {
+                for (int i = 0; i < 2; ++i)
+                    if (first < last[i])
+                        scores(i, 0);
+                umma_commit(k_empty);
+            }
+            for (int j = first; j < stop && alive; ++j) {
+                const int c = j - first, st = c % C::kStages, nst = (c + 1) % C::kStages;
+                const bool more = j + 1 < stop;
+                if (more && !wait(k_full + nst, ((c + 1) / C::kStages) & 1))
+                    break;
+                if (!wait(v_full + st, (c / C::kStages) & 1))
+                    break;
+                for (int i = 0; i < 2; ++i) {
+                    if (j >= last[i])
+                        continue;
+                    for (int half = 0; half < 2; ++half) {
+                        if (!wait(p_full + 2 * i + half, c & 1))
+                            break;
+                        tc_after();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_ts(tmem + C::kO + D * i, p_at(i, half * 4 + k), v_at(st, half * 4 + k), kPv,
+                                    c > 0 || half > 0 || k > 0);
+                    }
+                    if (!alive)
+                        break;
+                    if (s_low[i]) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
+                    }
+                    umma_commit(o_done + i);
+                    if (j + 1 < last[i])
+                        scores(i, nst);
+                }
+                if (!alive)
+                    break;
+                if (more)
+                    umma_commit(k_empty + nst);
+                umma_commit(v_empty + st);
+            }
+            /* the last commit has arrived before this CTA's memory can go */
+            wait(v_empty + (stop - 1 - first) % C::kStages, ((stop - 1 - first) / C::kStages) & 1);
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        /* ---- softmax of tile i, a row a thread */
+        const int i = warp >> 2, wl = warp & 3, r = wl * 32 + lane;
+        const uint32_t lanes = (uint32_t)(wl * 32) << 16;
+        const uint32_t ts = tmem + C::kS + 128 * i + lanes, to = tmem + C::kO + D * i + lanes;
+        const int tile0 = t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
+        const bool live = r < g.group * g.tok && t < s.q1;
+        const int seen = live ? seen_of(g, s, t) : 0;
+        const int all = tile0 < s.q1 ? seen_of(g, s, tile0) : 0; /* keys that every row sees */
+        const float scale2 = g.a.scale * kLog2e;
+        float m = -INFINITY, l = 0.f;
+        bool odd = false;
+        for (int j = first; j < last[i]; ++j) {
+            const int c = j - first;
+            warp_wait(s_full + i, c & 1);
+            tc_after();
+            const bool masked = (j + 1) * kKeys > all;
+            const int lim = masked ? seen - j * kKeys : kKeys;
+            /* S twice, 32 columns at a time and 32 more on their way: for the maximum, and
+             * for the weights (all 128 in registers at once would not fit beside the rest) */
+            uint32_t x[2][32];
+            tmem_ld32(ts, x[0]);
+            if (masked) { /* V's odd values would reach rows that do not see them */
+                warp_wait(v_full + c % C::kStages, (c / C::kStages) & 1);
+                const uint4 *v = reinterpret_cast<const uint4 *>(sv + (c % C::kStages) * C::kTileBytes);
+                uint32_t any = 0;
+#pragma unroll 4
+                for (int e = r; e < C::kTileBytes / 16; e += kRows) {
+                    const uint4 w = v[e];
+                    any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
+                }
+                odd |= any != 0;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                tmem_ld_wait(x[q & 1]);
+                tmem_ld32(ts + 32 * ((q + 1) & 3), x[(q + 1) & 1]);
+                float a = -INFINITY, b = -INFINITY;
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        a = fmaxf(a, 32 * q + e < lim ? __uint_as_float(x[q & 1][e]) : -INFINITY);
+                        b = fmaxf(b, 32 * q + e + 1 < lim ? __uint_as_float(x[q & 1][e + 1]) : -INFINITY);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        a = fmaxf(a, __uint_as_float(x[q & 1][e])), b = fmaxf(b, __uint_as_float(x[q & 1][e + 1]));
+                }
+                top = fmaxf(top, fmaxf(a, b));
+            }
+            /* rows that are no query's (of whatever lies there) take no part in what the warp decides */
+            top = live ? top * scale2 : -INFINITY;
+            const bool grow = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+                const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - nm);
+                m = nm, l *= f;
+                if (c > 0) { /* O of the tiles before, once they are in */
+                    warp_wait(o_done + i, (c - 1) & 1);
+                    tc_after();
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        uint32_t o[32];
+                        tmem_ld32(to + 32 * q, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(to + 32 * q, o);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            const float less = m == -INFINITY ? 0.f : -m;
+            const bool low = any_of_tile(i, ex2(top + less) * kHeavy > l);
+            if (r == 0)
+                s_low[i] = low;
+            const uint64_t sc = pack2f(scale2, scale2), ls = pack2f(less, less);
+            uint64_t sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t p[16];
+                tmem_ld_wait(x[q & 1]);
+                if (q < 3)
+                    tmem_ld32(ts + 32 * (q + 1), x[(q + 1) & 1]);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        x[q & 1][e] = 32 * q + e < lim ? x[q & 1][e] : 0xFF800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float a, b;
+                    unpack2f(fma2(pack2f(__uint_as_float(x[q & 1][2 * e]), __uint_as_float(x[q & 1][2 * e + 1])), sc, ls), a, b);
+                    a = ex2(a), b = ex2(b);
+                    x[q & 1][2 * e] = __float_as_uint(a), x[q & 1][2 * e + 1] = __float_as_uint(b);
+                    sum = add2(sum, pack2f(a, b));
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                    p[e] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+                tmem_st16(ts + 32 * q, p);
+                if (low) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = __uint_as_float(x[q & 1][2 * e]) - __uint_as_float(p[e] << 16);
+                        const float b = __uint_as_float(x[q & 1][2 * e + 1]) - __uint_as_float(p[e] & 0xFFFF0000u);
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                        p[e] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    tmem_st16(ts + 32 * q + 16, p);
+                }
+                if (q & 1) {
+                    tmem_st_wait();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(p_full + 2 * i + (q >> 1));
+                }
+            }
+            float a, b;
+            unpack2f(sum, a, b);
+            l += a + b;
+        }
+        if (odd)
+            s_bad[i] = 1;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory"); /* the tile's four warps */
+        const int done = last[i] - first;
+        if (done > 0) {
+            warp_wait(o_done + i, (done - 1) & 1);
+            tc_after();
+        }
+        const bool bad = s_bad[i] != 0;
+        if (it.cuts > 1) {
+            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
+            float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32] = {};
+                if (done > 0) {
+                    tmem_ld32(to + 32 * q, o);
+                    tmem_ld_wait(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
+            if (r == 0)
+                reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
+        } else if (!bad) {
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32] = {};
+                if (done > 0) {
+                    tmem_ld32(to + 32 * q, o);
+                    tmem_ld_wait(o);
+                }
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+                if (live)
+                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
+            }
+            if (live && g.a.lse)
+                g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        } else {
+            for (int k = wl; k < g.group * g.tok; k += 4) {
+                const int tk = tile0 + k / g.group;
+                if (tk < s.q1)
+                    plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
+            }
+        }
+        tc_before();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+/* Joins the parts of blocks whose keys were cut: a warp a row. */
+template <int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args g)
+{
+    const int lane = threadIdx.x & 31;
+    Item it;
+    /* a block for each part of 32 of its rows; the item's first part does the work */
+    if (!item_of(g, blockIdx.x, it) || it.cut != 0 || it.cuts == 1)
+        return;
+    const float *ml = g.part + (int64_t)g.sms * kSlotRows * D;
+    const int *bads = reinterpret_cast<const int *>(ml + (int64_t)2 * g.sms * kSlotRows);
+    for (int k = 0; k < 4; ++k) {
+        const int row = blockIdx.y * 32 + (threadIdx.x >> 5) * 4 + k, i = row / kRows, r = row % kRows;
+        const int t = it.s.q0 + it.block * 2 * g.tok + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
+        if (r >= g.group * g.tok || t >= it.s.q1)
+            continue;
+        float m = -INFINITY, l = 0.f;
+        int bad = 0;
+        for (int c = 0; c < it.cuts; ++c) {
+            m = fmaxf(m, ml[(int64_t)(it.slot + c) * kSlotRows + row]);
+            bad |= bads[2 * (it.slot + c) + i];
+        }
+        if (bad) {
+            plain_row<D>(g.a, it.s, t, hq, lane);
+            continue;
+        }
+        float o[D / 32] = {};
+        for (int c = 0; c < it.cuts; ++c) {
+            const int64_t at = (int64_t)(it.slot + c) * kSlotRows + row;
+            const float mc = ml[at], f = mc == -INFINITY ? 0.f : ex2(mc - m);
+            l = fmaf(f, ml[(int64_t)g.sms * kSlotRows + at], l);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e)
+                o[e] = fmaf(f, g.part[at * D + lane + 32 * e], o[e]);
+        }
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+            g.a.o[t * g.a.o_tok + hq * g.a.o_head + lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
+        if (lane == 0 && g.a.lse)
+            g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+}
+
+/* [tokens][heads][D] as (D, heads, tokens); boxes of 64 x heads x tokens */
+bool encode(CUtensorMap *m, const void *p, int D, int heads, int tokens, int64_t head_stride, int64_t tok_stride,
+            int box_heads, int box_tokens)
+{
+    auto enc = tensor_map_encoder();
+    if (!enc)
+        return false;
+    /* the stride of a dimension of one is never used */
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head_stride : D) * 2, (cuuint64_t)(tokens > 1 ? tok_stride : D) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, one[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims, strides, box, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool strides_ok(const void *p, int heads, int tokens, int64_t head, int64_t tok)
+{
+    auto ok = [](int64_t s) { return s > 0 && s % 8 == 0 && s < ((int64_t)1 << 38); };
+    return aligned_to(p, 16) && (heads == 1 || ok(head)) && (tokens == 1 || ok(tok));
+}
+/* the tensor-core kernel's calls: what TMA can address, rows that fit a tile, a scale
+ * whose order the running maximum keeps */
+bool tc_supported(const GlintAttnPrompt &a)
+{
+    const int group = a.heads / a.kv_heads;
+    return group <= kRows && a.scale > 0.f && a.k_tokens > 0 && strides_ok(a.q, a.heads, a.q_tokens, a.q_head, a.q_tok) &&
+           strides_ok(a.k, a.kv_heads, a.k_tokens, a.k_head, a.k_tok) &&
+           strides_ok(a.v, a.kv_heads, a.k_tokens, a.v_head, a.v_tok);
+}
+int64_t part_bytes(const GlintAttnPrompt &a)
+{
+    return (int64_t)sm_count() * (kSlotRows * (a.head_dim + 2) + 2) * 4;
+}
+/* whether some lengths of the sequences could make cuts worth while */
+bool may_split(const GlintAttnPrompt &a)
+{
+    const int tok = kRows / (a.heads / a.kv_heads);
+    const int64_t least = ((int64_t)a.q_tokens + 2 * tok - 1) / (2 * tok) * a.kv_heads;
+    return a.k_tokens > kKeys && 2 * least <= sm_count();
+}
+
+template <int D>
+int tc_launch(const GlintAttnPrompt &a, cudaStream_t st)
+{
+    Args g{};
+    g.a = a;
+    g.group = a.heads / a.kv_heads, g.tok = kRows / g.group, g.sms = sm_count();
+    g.vec = aligned_to(a.o, 16) && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
+    g.split = a.work && may_split(a);
+    g.part = static_cast<float *>(a.work);
+    Maps maps;
+    if (!encode(&maps.q, a.q, D, a.heads, a.q_tokens, a.q_head, a.q_tok, g.group, g.tok) ||
+        !encode(&maps.k, a.k, D, a.kv_heads, a.k_tokens, a.k_head, a.k_tok, 1, kKeys) ||
+        !encode(&maps.v, a.v, D, a.kv_heads, a.k_tokens, a.v_head, a.v_tok, 1, kKeys))
+        return kUnsupported;
+    if (!ensure_smem((const void *)attn_kernel<D>, Cfg<D>::kSmem))
+        return kLaunch;
+    /* every sequence may end in a block of its own */
+    const int64_t items = ((int64_t)a.q_tokens / (2 * g.tok) + a.seqs) * a.kv_heads;
+    const int64_t grid = std::max(items, (int64_t)(g.split ? g.sms : 0));
+    if (grid > INT32_MAX)
+        return kUnsupported;
+    attn_kernel<D><<<(unsigned)grid, kThreads, Cfg<D>::kSmem, st>>>(g, maps);
+    if (cudaGetLastError() != cudaSuccess)
+        return kLaunch;
+    if (g.split) {
+        attn_join_kernel<D><<<dim3((unsigned)g.sms, kSlotRows / 32), 256, 0, st>>>(g);
+        if (cudaGetLastError() != cudaSuccess)
+            return kLaunch;
+    }
+    return kOk;
+}
+
 } // namespace
 } // namespace glint
 
 using namespace glint;
 
-extern "C" int glint_attn_prompt_stream(const GlintAttnPrompt *a, cudaStream_t stream)
+namespace {
+int check(const GlintAttnPrompt *a)
 {
     if (!a || a->seqs < 0 || a->q_tokens < 0 || a->k_tokens < 0 || a->heads < 1 || a->kv_heads < 1 ||
         a->heads % a->kv_heads)
         return kBadArg;
-    if (a->head_dim != 64 && a->head_dim != 128)
-        return kUnsupported;
+    return a->head_dim == 64 || a->head_dim == 128 ? kOk : kUnsupported;
+}
+} // namespace
+
+extern "C" {
+
+int64_t glint_attn_prompt_work_bytes(const GlintAttnPrompt *a)
+{
+    const int rc = check(a);
+    if (rc != kOk)
+        return rc;
+    return may_split(*a) && a->q_tokens > 0 ? part_bytes(*a) : 0;
+}
+
+int glint_attn_prompt_stream(const GlintAttnPrompt *a, cudaStream_t stream)
+{
+    const int rc = check(a);
+    if (rc != kOk)
+        return rc;
     if (a->seqs == 0 || a->q_tokens == 0)
         return kOk;
-    if (!a->q || !a->o || !a->cu_q || !a->cu_k || (a->k_tokens > 0 && (!a->k || !a->v)))
+    if (!a->q || !a->o || !a->cu_q || !a->cu_k || (a->k_tokens > 0 && (!a->k || !a->v)) || !aligned_to(a->work, 16))
         return kBadArg;
+    if (tc_supported(*a)) {
+        const int r = a->head_dim == 128 ? tc_launch<128>(*a, stream) : tc_launch<64>(*a, stream);
+        if (r != kUnsupported)
+            return r;
+    }
     return plain_launch(*a, stream);
 }
+
+} /* extern "C" */

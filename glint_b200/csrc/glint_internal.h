@@ -87,6 +87,7 @@ int encode_error_word(bool clear);
 int expand_error_word(bool clear);
 int decode_error_word(bool clear);
 int km_error_word(bool clear);
+int attn_error_word(bool clear);
 /* Decode-shaped path streamed through TMA (bs == 64, K % 256 == 0, M <= 32). */
 bool htile_decode_supported(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
                             int M, int N, int K, int blocksize);

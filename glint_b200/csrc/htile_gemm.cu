@@ -1676,10 +1676,10 @@ int read_kernel_error(bool clear)
     if (v < 0)
         return -1;
     const int e = encode_error_word(clear), x = expand_error_word(clear), d = decode_error_word(clear),
-              k = km_error_word(clear);
-    if (e < 0 || x < 0 || d < 0 || k < 0)
+              k = km_error_word(clear), a = attn_error_word(clear);
+    if (e < 0 || x < 0 || d < 0 || k < 0 || a < 0)
         return -1;
-    return v | e | x | d | k;
+    return v | e | x | d | k | a;
 }
 
 } // namespace glint

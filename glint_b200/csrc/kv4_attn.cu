@@ -322,6 +322,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
                     s[sl][n][i] = -INFINITY;
             }
         if constexpr (SCORE) {
+            auto scaled = [&](float v) { return !WHOLE && v == -INFINITY ? v : v * scale2; };
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int col = chunk * 8 * NT + n * 8 + 2 * c;
@@ -330,9 +331,9 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
                     float *p = score + (int64_t)(t0 + (i ? tb : ta)) * g.cols + col;
                     if (WHOLE || ((valid >> (i ? tb : ta)) & 1u)) {
                         if (col < g.cols)
-                            p[0] = s[sl][n][2 * i] * scale2;
+                            p[0] = scaled(s[sl][n][2 * i]);
                         if (col + 1 < g.cols)
-                            p[1] = s[sl][n][2 * i + 1] * scale2;
+                            p[1] = scaled(s[sl][n][2 * i + 1]);
                     }
                 }
             }
@@ -393,7 +394,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[i] = ex2(fmaf(s[sl][n][i], scale2, less[n][i & 1]));
+                p[i] = !WHOLE && s[sl][n][i] == -INFINITY ? 0.f : ex2(fmaf(s[sl][n][i], scale2, less[n][i & 1]));
                 st.l[n][i & 1] += p[i];
             }
 #pragma unroll

@@ -33,17 +33,22 @@ extern "C" {
  * j <= i + Lk - Lq when causal, all Lk keys otherwise; where Lk < Lq the first
  * Lq - Lk rows see none.  o [q_tokens, heads, head_dim] with strides o_tok, o_head;
  * lse [heads, q_tokens] f32 or NULL.  Tokens outside every sequence are not written.
- * o may not overlap q, k or v.  16-byte aligned q, k and v with strides that are
- * multiples of 8 take the tensor-core kernel, anything else a plain one. */
+ * o may not overlap q, k or v.  work: glint_attn_prompt_work_bytes() of 16-byte
+ * aligned device memory, the call's own until it completes, of any content; it lets few
+ * queries with many keys share the GPU, and may be NULL.  16-byte aligned q, k and v
+ * with positive strides that are multiples of 8, and scale > 0, take the tensor-core
+ * kernel, anything else a plain one. */
 typedef struct GlintAttnPrompt {
     const glint_bf16_t *q, *k, *v;
     glint_bf16_t *o;
     float *lse;
     const int *cu_q, *cu_k;
+    void *work;
     int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;
     int seqs, q_tokens, k_tokens, heads, kv_heads, head_dim, causal;
     float scale;
 } GlintAttnPrompt;
+int64_t glint_attn_prompt_work_bytes(const GlintAttnPrompt *a);
 int glint_attn_prompt_stream(const GlintAttnPrompt *a, cudaStream_t stream);
 
 /* The 4-bit cache.  Slots lie in pages of page_size (16, 32, 64 or 128) per head:

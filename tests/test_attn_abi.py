@@ -19,7 +19,7 @@ def structs():
     buf = (ctypes.c_uint8 * 256)()
     p = (ctypes.addressof(buf) + 15) & ~15
     cache = attn._Cache(p, p, p, p, 4, 2, 64, 128)
-    prompt = attn._Prompt(*[p] * 7, *[8] * 8, 1, 4, 4, 4, 2, 128, 1, 1.0)
+    prompt = attn._Prompt(*[p] * 7, None, *[8] * 8, 1, 4, 4, 4, 2, 128, 1, 1.0)
     at = attn._Attn(p, p, p, p, p, None, None, p, 8, 8, 8, 256, 1, 1, 4, 4, 1.0)
     ev = attn._Evict(p, p, p, p, p, p, p, p + 16, p + 16, 256, 1, 4, 8, 2)
     return buf, p, cache, prompt, at, ev
@@ -39,6 +39,11 @@ def test_prompt_arguments(lib):
         buf, p, _, prompt, _, _ = structs()
         assert f(put(prompt, **kw), None) == rc, kw
     assert f(None, None) == -1
+    buf, p, _, prompt, _, _ = structs()
+    assert f(put(prompt, work=p + 8), None) == -1
+    assert lib.glint_attn_prompt_work_bytes(put(prompt, head_dim=96)) == -6
+    assert lib.glint_attn_prompt_work_bytes(None) == -1
+    assert lib.glint_attn_prompt_work_bytes(put(prompt, head_dim=128, q_tokens=10 ** 6)) == 0
 
 
 def test_cache_arguments(lib):
