@@ -62,12 +62,26 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t &met
     }
     /* lo is one of the BF16 inputs, so its upper half is all of it */
     meta = (__float_as_uint(lo) & 0xFFFF0000u) | (uint32_t)__bfloat16_as_ushort(sb);
+    /* (x - lo) * (1 / step) is within 2^-18 of the quotient (at most 15.06 here), so it
+     * rounds to the same integer unless it lies that near to a half; those, and steps so
+     * small or large that 1 / step is not a normal number, divide */
     uint32_t w = 0;
-    if (step > 0.f) {
+    bool near = !(step > 1e-30f && step < 1e30f);
+    const float inv = __frcp_rn(step);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, step)), 0.f), 15.f);
-            w |= (uint32_t)c << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+        const float t = (x[i] - lo) * inv, u = t + 12582912.f; /* 1.5 * 2^23: rounds to an integer in u's low bits */
+        near |= !(fabsf(t - (u - 12582912.f)) < 0.49999f);
+        w |= (__float_as_uint(u) & 15u) << (4 * i);
+    }
+    if (near) {
+        w = 0;
+        if (step > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, step)), 0.f), 15.f);
+                w |= (uint32_t)c << (4 * i);
+            }
         }
     }
     return w;
@@ -78,19 +92,28 @@ struct AppendArgs {
     const __nv_bfloat16 *k, *v;
     int64_t k_tok, k_head, v_tok, v_head;
     const int *slots;
-    int64_t chunks; /* tokens * kv_heads * D / 8 */
+    uint32_t chunks; /* tokens * kv_heads * D / 8 */
+    int page_log2;
 };
+/* 32-bit chunk numbers: longer calls go in slices of this many tokens */
+inline int slice_tokens(const GlintKv4Cache &c) { return (int)std::max((int64_t)1, (int64_t)0x7FFFFFFF / ((int64_t)c.kv_heads * (c.head_dim / 8))); }
+inline int log2_of(int n)
+{
+    int l = 0;
+    while ((1 << l) < n)
+        ++l;
+    return l;
+}
 
 template <int D, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const AppendArgs a)
 {
     constexpr int CH = D / 8; /* chunks a row: a power of two, so a block's 8 lanes stay in one row */
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
     const bool live = i < a.chunks;
     const int ch = (int)(i % CH);
-    const int64_t row = i / CH;
-    const int h = live ? (int)(row % a.c.kv_heads) : 0;
-    const int64_t t = live ? row / a.c.kv_heads : 0;
+    const uint32_t row = live ? i / CH : 0, t = row / (uint32_t)a.c.kv_heads;
+    const int h = (int)(row - t * (uint32_t)a.c.kv_heads);
     float x[8] = {}, y[8] = {};
     const int slot = live ? a.slots[t] : -1;
     if (live) {
@@ -101,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const AppendArgs a
     const uint32_t kw = quantise8(x, km), vw = quantise8(y, vm);
     if (slot < 0 || slot >= a.c.pages * a.c.page_size)
         return;
-    const int page = slot / a.c.page_size, r = slot - page * a.c.page_size;
-    const int64_t at = ((int64_t)page * a.c.kv_heads + h) * a.c.page_size + r;
+    const int page = slot >> a.page_log2, r = slot & (a.c.page_size - 1);
+    const int64_t at = (((int64_t)page * a.c.kv_heads + h) << a.page_log2) + r;
     const int64_t byte = at * (D / 2) + kv4_unit<D>(ch / 8, r) + (ch % 8) * 4;
     *reinterpret_cast<uint32_t *>(a.c.k_code + byte) = kw;
     *reinterpret_cast<uint32_t *>(a.c.v_code + byte) = vw;
@@ -128,21 +151,21 @@ __device__ __forceinline__ uint4 values8(uint32_t w, uint32_t meta)
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache c, const int *slots, int64_t chunks,
-                                                            uint4 *ko, uint4 *vo)
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache c, const int *slots, uint32_t chunks,
+                                                            int page_log2, uint4 *ko, uint4 *vo)
 {
     constexpr int CH = D / 8;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
     if (i >= chunks)
         return;
     const int ch = (int)(i % CH);
-    const int64_t row = i / CH;
-    const int h = (int)(row % c.kv_heads);
-    const int slot = slots[row / c.kv_heads];
+    const uint32_t row = i / CH, t = row / (uint32_t)c.kv_heads;
+    const int h = (int)(row - t * (uint32_t)c.kv_heads);
+    const int slot = slots[t];
     uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
     if (slot >= 0 && slot < c.pages * c.page_size) {
-        const int page = slot / c.page_size, r = slot - page * c.page_size;
-        const int64_t at = ((int64_t)page * c.kv_heads + h) * c.page_size + r;
+        const int page = slot >> page_log2, r = slot & (c.page_size - 1);
+        const int64_t at = (((int64_t)page * c.kv_heads + h) << page_log2) + r;
         const int64_t byte = at * (D / 2) + kv4_unit<D>(ch / 8, r) + (ch % 8) * 4;
         const int64_t m = at * (D / 64) + ch / 8;
         const uint32_t kw = *reinterpret_cast<const uint32_t *>(c.k_code + byte);
@@ -154,17 +177,27 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache 
 }
 
 /* ---- eviction --------------------------------------------------------------------
- * One CTA per (sequence, kv head).  The n-th largest key is found by four passes over
- * 8-bit digits (a histogram each); a bit per slot and the running count of kept bits
- * then give, for the k-th free slot below n, the k-th kept slot from n on by a binary
- * search, so no list is built and the moves are independent of one another (sources
- * lie at n and above, destinations below). */
-constexpr int kEvThreads = 1024;
+ * A cluster of 1 to 8 CTAs per (sequence, kv head), each with an equal stretch of the
+ * slots.  The n-th largest key is found by four passes over 8-bit digits: a histogram in
+ * every CTA, summed through the others' shared memory.  A bit per slot (kept) and the
+ * running count of bits then number the free slots below n and the kept ones from n on;
+ * the free ones are listed across the cluster's shared memory, and the k-th kept one is
+ * moved into the k-th of the list.  Sources lie at n and above, destinations below, so
+ * the moves do not depend on one another.
+ *
+ * Bound: 8 bytes a slot and head read (weight and position), and the latency of nine
+ * cluster barriers.
+ */
+constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32;
+constexpr int kEvSlots = 4; /* slots a thread that another CTA is taken for */
 constexpr int kEvMaxSlots = 524288;
+constexpr int kEvKeys = 40960; /* keys a CTA holds in shared memory; with more it reads weights again */
 
 struct EvictArgs {
     GlintKv4Cache c;
     GlintKv4Evict e;
+    int cluster, stretch; /* CTAs a head; slots a CTA at most, a multiple of kEvThreads */
+    int page_log2;
 };
 
 /* larger key = kept first: protected, then by weight, NaN last */
@@ -177,132 +210,236 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int64_t guard)
     const uint32_t u = __float_as_uint(w + 0.f); /* -0 and +0 tie */
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-
-__device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total)
+__device__ __forceinline__ void cluster_barrier()
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t there(const void *p, uint32_t cta) /* the same place in another CTA */
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(cta));
+    return r;
+}
+__device__ __forceinline__ int load_there(uint32_t a)
+{
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_there(uint32_t a, int v)
+{
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+/* sum over the lanes below this one */
+__device__ __forceinline__ int warp_before(int v)
+{
     int s = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
         const int o = __shfl_up_sync(0xFFFFFFFFu, s, off);
-        if (lane >= off)
+        if ((int)lane_id() >= off)
             s += o;
     }
-    if (lane == 31)
-        warp_sums[warp] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kEvThreads / 32; ++w) {
-        before += w < warp ? warp_sums[w] : 0;
-        total += warp_sums[w];
-    }
-    __syncthreads();
-    return before + s - v; /* exclusive */
+    return s - v;
+}
+/* count one key into bin d: the bin of the warp's first lane (often most of them: equal
+ * weights, zeros) by one addition, the others by theirs.  Integer counts: any order. */
+__device__ __forceinline__ void count(int *hist, bool in, uint32_t d)
+{
+    const uint32_t some = __ballot_sync(0xFFFFFFFFu, in);
+    if (!some)
+        return;
+    const int lead = __ffs(some) - 1;
+    const uint32_t first = __shfl_sync(0xFFFFFFFFu, d, lead);
+    const uint32_t same = __ballot_sync(0xFFFFFFFFu, in && d == first);
+    if ((int)lane_id() == lead)
+        atomicAdd(&hist[d], __popc(same));
+    else if (in && !((same >> lane_id()) & 1u))
+        atomicAdd(&hist[d], 1);
 }
 
 template <int D>
-__global__ void __launch_bounds__(kEvThreads) kv4_evict_kernel(const EvictArgs a)
+__global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArgs a)
 {
     extern __shared__ uint32_t ev_smem[];
-    __shared__ int hist[256];
-    __shared__ int warp_sums[kEvThreads / 32];
+    __shared__ int hist[2][256], tot[256];
+    __shared__ int near_of[kEvWarps], far_of[kEvWarps], eq_of[kEvWarps]; /* per warp: free below n, kept from n on, keys equal to the n-th */
+    __shared__ int s_free, s_far, s_need;
     __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
     const GlintKv4Cache &c = a.c;
     const GlintKv4Evict &e = a.e;
-    const int b = blockIdx.x / c.kv_heads, h = blockIdx.x - b * c.kv_heads;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int cap = e.max_pages * c.page_size;
-    const int L = min(max(e.lens[b], 0), cap), n = min(L, e.budget);
-    const int words = (cap + 31) / 32;
-    uint32_t *bits = ev_smem;                             /* one bit per slot: kept */
-    int *rank = reinterpret_cast<int *>(ev_smem + words); /* kept bits before each word */
-    const int64_t row = ((int64_t)b * c.kv_heads + h) * e.stride;
+    const int rank = blockIdx.x % a.cluster, bh = blockIdx.x / a.cluster;
+    const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int L = min(max(e.lens[b], 0), e.max_pages << a.page_log2), n = min(L, e.budget);
+    /* an equal stretch of the slots for each CTA, a multiple of kEvThreads (no more than a.stretch) */
+    const int stretch = max(1, (L + a.cluster * kEvThreads - 1) / (a.cluster * kEvThreads)) * kEvThreads;
+    const int begin = rank * stretch, end = min(L, begin + stretch); /* this CTA's; none where end <= begin */
+    const int words = stretch / 32, per_warp = words / kEvWarps;
+    uint32_t *bits = ev_smem;                                      /* kept, a bit a slot */
+    int *free_at = reinterpret_cast<int *>(bits + a.stretch / 32); /* this warp's free slots below n before a word */
+    int *far_at = free_at + a.stretch / 32;                        /* its kept slots from n on before a word */
+    uint32_t *keys = reinterpret_cast<uint32_t *>(far_at + a.stretch / 32); /* later this CTA's part of the list of free slots */
+    int *list = reinterpret_cast<int *>(keys);
+    const bool held = a.stretch <= kEvKeys;
+    const int64_t row = (int64_t)bh * e.stride;
     const float *w = e.weight + row;
     const int *pos = e.pos + row;
     const int64_t guard = (int64_t)e.seen[b] - e.recent;
-    if (h == 0 && tid == 0)
+    auto key = [&](int t) { return held ? keys[t - begin] : evict_key(w[t], pos[t], guard); };
+    if (h == 0 && rank == 0 && tid == 0)
         e.new_lens[b] = n;
+    if (held) {
+#pragma unroll 8
+        for (int t = begin + tid; t < end; t += kEvThreads)
+            keys[t - begin] = evict_key(w[t], pos[t], guard);
+    }
+    if (tid < 256)
+        hist[0][tid] = 0;
+    __syncthreads();
 
     /* the n-th largest key, a digit at a time */
     uint32_t prefix = 0;
-    int need = n;
-    for (int shift = 24; shift >= 0 && L > n; shift -= 8) {
-        if (tid < 256)
-            hist[tid] = 0;
-        __syncthreads();
-        const uint32_t high = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        for (int t = tid; t < L; t += kEvThreads) {
-            const uint32_t k = evict_key(w[t], pos[t], guard);
-            if ((k & high) == prefix)
-                atomicAdd(&hist[(k >> shift) & 255u], 1); /* integer counts: the order does not matter */
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int d = 255, left = need;
-            while (d > 0 && hist[d] < left)
-                left -= hist[d--];
-            s_prefix = prefix | ((uint32_t)d << shift);
-            s_need = left;
-        }
-        __syncthreads();
-        prefix = s_prefix, need = s_need;
-        __syncthreads();
-    }
-    /* kept: above the n-th key, and of those equal to it the `need` lowest slots */
-    int eq_before = 0, kept_before = 0;
-    for (int t0 = 0; t0 < L; t0 += kEvThreads) {
-        const int t = t0 + tid;
-        const uint32_t k = t < L ? evict_key(w[t], pos[t], guard) : 0u;
-        const bool eq = t < L && L > n && k == prefix;
-        int total;
-        const int r = block_scan(eq ? 1 : 0, warp_sums, total);
-        const bool keep = t < L && (L <= n || k > prefix || (eq && eq_before + r < need));
-        eq_before += total;
-        const uint32_t m = __ballot_sync(0xFFFFFFFFu, keep);
-        int all;
-        const int kr = block_scan(keep ? 1 : 0, warp_sums, all);
-        if (lane == 0 && t / 32 < words)
-            bits[t / 32] = m, rank[t / 32] = kept_before + kr;
-        kept_before += all;
-    }
-    __syncthreads();
-    /* result slot i: itself where kept, else the matching kept slot from n on */
-    int *kept = e.kept + ((int64_t)b * c.kv_heads + h) * e.budget;
-    const int below = n > 0 ? rank[(n - 1) / 32] + __popc(bits[(n - 1) / 32] & (0xFFFFFFFFu >> (31 - (n - 1) % 32))) : 0;
-    for (int i = tid; i < e.budget; i += kEvThreads) {
-        if (i >= n) {
-            kept[i] = -1;
-            continue;
-        }
-        int src = i;
-        if (!((bits[i / 32] >> (i % 32)) & 1u)) {
-            /* i is free slot number i - (kept before i); its row is kept slot `want` of all */
-            const int want = below + i - (rank[i / 32] + __popc(bits[i / 32] & ((1u << (i % 32)) - 1u)));
-            int lo = 0, hi = (L - 1) / 32; /* last word with rank <= want */
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (rank[mid] <= want)
-                    lo = mid;
-                else
-                    hi = mid - 1;
+    int need = n, eq_before = 0;
+    if (L > n) {
+        for (int p = 0; p < 4; ++p) {
+            const int shift = 24 - 8 * p;
+            const uint32_t high = p ? 0xFFFFFFFFu << (shift + 8) : 0u;
+#pragma unroll 4
+            for (int t0 = begin; t0 < end; t0 += kEvThreads) {
+                const int t = t0 + tid;
+                const uint32_t k = t < end ? key(t) : 0u;
+                count(hist[p & 1], t < end && (k & high) == prefix, (k >> shift) & 255u);
             }
-            src = lo * 32 + __fns(bits[lo], 0, want - rank[lo] + 1);
+            cluster_barrier();
+            if (tid < 256) {
+                int sum = 0;
+                for (int r = 0; r < a.cluster; ++r)
+                    sum += load_there(there(&hist[p & 1][tid], r));
+                tot[tid] = sum;
+                hist[(p + 1) & 1][tid] = 0; /* read by the others before the barrier above */
+            }
+            __syncthreads();
+            if (warp == 0) { /* lane i: bins 255 - 8 i down to 248 - 8 i */
+                int sum = 0;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    sum += tot[255 - 8 * lane - q];
+                int left = need - warp_before(sum); /* still wanted from this lane's bins on */
+                if (left > 0 && left <= sum) {
+                    int d = 255 - 8 * lane;
+                    while (tot[d] < left)
+                        left -= tot[d--];
+                    s_prefix = prefix | ((uint32_t)d << shift), s_need = left;
+                }
+            }
+            __syncthreads();
+            prefix = s_prefix, need = s_need;
         }
-        kept[i] = src;
-        e.weight_out[row + i] = w[src];
-        e.pos_out[row + i] = pos[src];
-        if (src == i)
-            continue;
-        const int *table = e.table + (int64_t)b * e.max_pages;
-        const int pf = table[src / c.page_size], pt = table[i / c.page_size];
+        /* the last histogram counts, for its digit, the keys equal to the n-th */
+        for (int r = 0; r < rank; ++r)
+            eq_before += load_there(there(&hist[1][prefix & 255u], r));
+    }
+    /* kept: above the n-th key, and of those equal to it the `need` lowest slots.  A warp
+     * has per_warp words of 32 slots. */
+    const int w0 = warp * per_warp;
+    int eqs = 0;
+#pragma unroll 4
+    for (int q = 0; q < per_warp; ++q) {
+        const int t = begin + (w0 + q) * 32 + lane;
+        eqs += __popc(__ballot_sync(0xFFFFFFFFu, t < end && L > n && key(t) == prefix));
+    }
+    if (lane == 0)
+        eq_of[warp] = eqs;
+    __syncthreads();
+    for (int k = 0; k < warp; ++k)
+        eq_before += eq_of[k];
+    int frees = 0, fars = 0;
+#pragma unroll 4
+    for (int q = 0; q < per_warp; ++q) {
+        const int t0 = begin + (w0 + q) * 32, t = t0 + lane;
+        const uint32_t k = t < end ? key(t) : 0u;
+        const bool eq = t < end && L > n && k == prefix;
+        const uint32_t me = __ballot_sync(0xFFFFFFFFu, eq);
+        const bool keep = t < end && (L <= n || k > prefix ||
+                                      (eq && eq_before + __popc(me & ((1u << lane) - 1u)) < need));
+        eq_before += __popc(me);
+        const uint32_t m = __ballot_sync(0xFFFFFFFFu, keep), below = __ballot_sync(0xFFFFFFFFu, t < n);
+        if (lane == 0)
+            bits[w0 + q] = m, free_at[w0 + q] = frees, far_at[w0 + q] = fars;
+        frees += __popc(below & ~m), fars += __popc(m & ~below);
+    }
+    if (lane == 0)
+        near_of[warp] = frees, far_of[warp] = fars;
+    __syncthreads(); /* also: the keys are not needed any more */
+    if (warp == 0) {
+        const int f = lane < kEvWarps ? near_of[lane] : 0, g = lane < kEvWarps ? far_of[lane] : 0;
+        const int fb = warp_before(f), gb = warp_before(g);
+        if (lane < kEvWarps)
+            near_of[lane] = fb, far_of[lane] = gb;
+        if (lane == 31)
+            s_free = fb + f, s_far = gb + g;
+    }
+    cluster_barrier(); /* counts and the keys' memory, of every CTA */
+    int free_base = 0, far_base = 0, moved = 0;
+    for (int r = 0; r < a.cluster; ++r) {
+        const int f = load_there(there(&s_free, r)), g = load_there(there(&s_far, r));
+        free_base += r < rank ? f : 0, far_base += r < rank ? g : 0, moved += f;
+    }
+    const int part = max(1, (moved + a.cluster - 1) / a.cluster); /* entries of the list a CTA holds */
+    int *kept = e.kept + (int64_t)bh * e.budget;
+#pragma unroll 2
+    for (int q = 0; q < per_warp; ++q) { /* the free slots of this CTA's into the list */
+        const int t0 = begin + (w0 + q) * 32, t = t0 + lane;
+        const uint32_t out = t0 >= n ? 0u : ~bits[w0 + q] & (n - t0 >= 32 ? 0xFFFFFFFFu : (1u << (n - t0)) - 1u);
+        if ((out >> lane) & 1u) {
+            const int k = free_base + near_of[warp] + free_at[w0 + q] + __popc(out & ((1u << lane) - 1u));
+            store_there(there(&list[k % part], k / part), t);
+        }
+    }
+    /* the kept ones below n, shared out evenly: most of them lie in the first CTAs */
+#pragma unroll 4
+    for (int t = rank * kEvThreads + tid; t < n; t += a.cluster * kEvThreads) {
+        const int r = t / stretch, at = t - r * stretch;
+        if ((load_there(there(&bits[at / 32], r)) >> (at % 32)) & 1)
+            kept[t] = t, e.weight_out[row + t] = w[t], e.pos_out[row + t] = pos[t];
+    }
+    for (int i = n + rank * kEvThreads + tid; i < e.budget; i += a.cluster * kEvThreads)
+        kept[i] = -1;
+    cluster_barrier();
+    /* the kept slots from n on, a thread each: number j of this CTA's by two searches */
+    const int *table = e.table + (int64_t)b * e.max_pages;
+    for (int j = tid; j < s_far; j += kEvThreads) {
+        int wp = 0;
+#pragma unroll
+        for (int step = kEvWarps / 2; step > 0; step /= 2)
+            if (far_of[wp + step] <= j)
+                wp += step;
+        const int in = j - far_of[wp];
+        int lo = wp * per_warp, hi = lo + per_warp - 1; /* its last word with far_at <= in */
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (far_at[mid] <= in)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        uint32_t m = bits[lo];
+        const int t0 = begin + lo * 32;
+        if (t0 < n)
+            m &= 0xFFFFFFFFu << (n - t0); /* n - t0 < 32: the word has a slot from n on */
+        for (int k = in - far_at[lo]; k > 0; --k)
+            m &= m - 1;
+        const int src = t0 + __ffs(m) - 1, k = far_base + j;
+        const int dst = load_there(there(&list[k % part], k / part));
+        kept[dst] = src, e.weight_out[row + dst] = w[src], e.pos_out[row + dst] = pos[src];
+        const int pf = table[src >> a.page_log2], pt = table[dst >> a.page_log2];
         if (pf < 0 || pf >= c.pages || pt < 0 || pt >= c.pages)
             continue;
-        const int rf = src % c.page_size, rt = i % c.page_size;
-        const int64_t from = ((int64_t)pf * c.kv_heads + h) * c.page_size + rf;
-        const int64_t to = ((int64_t)pt * c.kv_heads + h) * c.page_size + rt;
+        const int rf = src & (c.page_size - 1), rt = dst & (c.page_size - 1);
+        const int64_t from = (((int64_t)pf * c.kv_heads + h) << a.page_log2) + rf;
+        const int64_t to = (((int64_t)pt * c.kv_heads + h) << a.page_log2) + rt;
         uint4 kc[D / 32], vc[D / 32];
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
@@ -326,6 +463,7 @@ __global__ void __launch_bounds__(kEvThreads) kv4_evict_kernel(const EvictArgs a
             reinterpret_cast<uint32_t *>(c.v_meta)[to * (D / 64) + q] = vm[q];
         }
     }
+    cluster_barrier(); /* no CTA leaves while another may read its list */
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kLaunch; }
@@ -348,15 +486,15 @@ int glint_kv4_append_stream(const GlintKv4Cache *c, const glint_bf16_t *k, const
         return kBadArg;
     if (tokens == 0)
         return kOk;
-    const AppendArgs a{*c, k, v, k_tok, k_head, v_tok, v_head, slots, (int64_t)tokens * c->kv_heads * (c->head_dim / 8)};
     const bool al = aligned_to(k, 16) && aligned_to(v, 16) && (k_tok | k_head | v_tok | v_head) % 8 == 0;
-    const unsigned grid = (unsigned)((a.chunks + kThreads - 1) / kThreads);
-    if (c->head_dim == 128)
-        al ? kv4_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(a)
-           : kv4_append_kernel<128, false><<<grid, kThreads, 0, stream>>>(a);
-    else
-        al ? kv4_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(a)
-           : kv4_append_kernel<64, false><<<grid, kThreads, 0, stream>>>(a);
+    const auto kernel = c->head_dim == 128 ? (al ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
+                                           : (al ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
+    const int most = slice_tokens(*c);
+    for (int t = 0; t < tokens; t += std::min(most, tokens - t)) {
+        const uint32_t n = (uint32_t)std::min(most, tokens - t) * c->kv_heads * (c->head_dim / 8);
+        const AppendArgs a{*c, k + t * k_tok, v + t * v_tok, k_tok, k_head, v_tok, v_head, slots + t, n, log2_of(c->page_size)};
+        kernel<<<(n + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
+    }
     return launched();
 }
 
@@ -370,13 +508,14 @@ int glint_kv4_read_stream(const GlintKv4Cache *c, const int *slots, int tokens, 
         return kBadArg;
     if (tokens == 0)
         return kOk;
-    const int64_t chunks = (int64_t)tokens * c->kv_heads * (c->head_dim / 8);
-    const unsigned grid = (unsigned)((chunks + kThreads - 1) / kThreads);
+    const auto kernel = c->head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>;
+    const int most = slice_tokens(*c);
     uint4 *ko = reinterpret_cast<uint4 *>(k_out), *vo = reinterpret_cast<uint4 *>(v_out);
-    if (c->head_dim == 128)
-        kv4_read_kernel<128><<<grid, kThreads, 0, stream>>>(*c, slots, chunks, ko, vo);
-    else
-        kv4_read_kernel<64><<<grid, kThreads, 0, stream>>>(*c, slots, chunks, ko, vo);
+    for (int t = 0; t < tokens; t += std::min(most, tokens - t)) {
+        const uint32_t n = (uint32_t)std::min(most, tokens - t) * c->kv_heads * (c->head_dim / 8);
+        const int64_t at = (int64_t)t * c->kv_heads * (c->head_dim / 8);
+        kernel<<<(n + kThreads - 1) / kThreads, kThreads, 0, stream>>>(*c, slots + t, n, log2_of(c->page_size), ko + at, vo + at);
+    }
     return launched();
 }
 
@@ -394,17 +533,29 @@ int glint_kv4_evict_stream(const GlintKv4Cache *c, const GlintKv4Evict *e, cudaS
         !e->pos_out || e->weight == e->weight_out || e->pos == e->pos_out ||
         (int64_t)e->seqs * c->kv_heads > INT32_MAX)
         return kBadArg;
-    const EvictArgs a{*c, *e};
-    const int words = (e->max_pages * c->page_size + 31) / 32;
-    const int smem = words * 8;
-    const void *kern = c->head_dim == 128 ? (const void *)kv4_evict_kernel<128> : (const void *)kv4_evict_kernel<64>;
-    if (smem > 40 * 1024 && !ensure_smem(kern, kEvMaxSlots / 32 * 8))
+    EvictArgs a{*c, *e, 1, 0, log2_of(c->page_size)};
+    /* up to eight CTAs (a portable cluster) while each thread has kEvSlots or more */
+    const int cap = e->max_pages * c->page_size;
+    while (a.cluster < 8 && cap > kEvSlots * kEvThreads * a.cluster)
+        a.cluster *= 2;
+    a.stretch = (cap + a.cluster * kEvThreads - 1) / (a.cluster * kEvThreads) * kEvThreads;
+    if ((int64_t)e->seqs * c->kv_heads * a.cluster > INT32_MAX)
+        return kBadArg;
+    /* keys, or at least this CTA's part of the list: at most half of the slots are free ones below n */
+    const int smem = a.stretch / 32 * 12 + (a.stretch <= kEvKeys ? a.stretch * 4 : a.stretch / 2 * 4 + 16);
+    const auto kernel = c->head_dim == 128 ? kv4_evict_kernel<128> : kv4_evict_kernel<64>;
+    if (!ensure_smem((const void *)kernel, kEvKeys / 32 * 12 + kEvKeys * 4))
         return kLaunch;
-    const unsigned grid = (unsigned)(e->seqs * c->kv_heads);
-    if (c->head_dim == 128)
-        kv4_evict_kernel<128><<<grid, kEvThreads, smem, stream>>>(a);
-    else
-        kv4_evict_kernel<64><<<grid, kEvThreads, smem, stream>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(e->seqs * c->kv_heads * a.cluster)), cfg.blockDim = dim3(kEvThreads);
+    cfg.dynamicSmemBytes = smem, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunch;
+    }
     return launched();
 }
 
