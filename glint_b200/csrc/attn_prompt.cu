@@ -5,7 +5,7 @@
  * group's heads share every K and V tile that is loaded.  Per tile of 128 keys
  *
  *   S = Q K^T          UMMA 128 x 128 x D, Q and K in shared memory (TMA, 128-byte swizzle)
- *   P = 2^(S c - m)    a thread per row: S from TMEM, running maximum m and sum l in f32,
+ *   P = 2^(S c - m)    two threads a row: S from TMEM, running maximum m and sum l in f32,
  *                      P as BF16 back into S's columns (2^-8 of each weight at most, the
  *                      rounding that the tensor cores' operand asks for)
  *   O += P V           UMMA 128 x D x 128, P from TMEM, V as it lies (inner index = key rows)
@@ -135,13 +135,17 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int D>
 struct Cfg {
     static constexpr int kTileBytes = kKeys * D * 2;
-    static constexpr int kStages = D == 128 ? 2 : 4; /* of K, and of V */
+    static constexpr int kStages = D == 128 ? 2 : 4; /* of V and the K after it */
     static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + 256;
     /* TMEM columns: S of tile i at 128 i, O at 256 + D i.  In S's place, for 32 keys a
      * time, 16 columns of P and 16 of what P's rounding dropped. */
     static constexpr uint32_t kS = 0, kO = 256;
 };
-constexpr int kThreads = 384; /* warps 0-3, 4-7: softmax of the two tiles; 8: loads; 9: UMMA; 10, 11 idle */
+/* warps 0-15: softmax, eight for each tile (four for keys 0-63 of a tile of keys, four for
+ * 64-127; two threads share a row); 16: loads; 17: UMMA, the two tiles in turn (one
+ * thread each let them fall into step, both in softmax and then both in UMMA: 1.3 times
+ * the time) */
+constexpr int kLoadWarp = 16, kMmaWarp = 17, kThreads = 576;
 constexpr int kSlotRows = 2 * kRows;
 
 struct Args {
@@ -203,10 +207,23 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r)
+__device__ __forceinline__ void tmem_zero16(uint32_t taddr)
 {
-    tmem_st16(taddr, r);
-    tmem_st16(taddr + 16, r + 16);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 /* the loads into r have arrived: its values are this statement's, so no use moves ahead of it */
 __device__ __forceinline__ void tmem_ld_wait(uint32_t *r)
@@ -364,16 +381,10 @@ __device__ __forceinline__ void store_row32(const Args &g, __nv_bfloat16 *o, con
 /* any NaN or infinity among two BF16 */
 __device__ __forceinline__ uint32_t odd2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
-/* whether any of a tile's 128 softmax threads has `p` */
-__device__ __forceinline__ bool any_of_tile(int i, bool p)
+/* barrier `id` of n threads */
+__device__ __forceinline__ void some_sync(int id, int n)
 {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                 "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
-                 : "=r"(r)
-                 : "r"((uint32_t)p), "r"(1 + i)
-                 : "memory");
-    return r != 0;
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
 }
 
 template <int D>
@@ -384,12 +395,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     uint8_t *smem = raw + ((1024 - (saddr(raw) & 1023)) & 1023);
     uint8_t *sq = smem, *sk = sq + 2 * C::kTileBytes, *sv = sk + C::kStages * C::kTileBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sv + C::kStages * C::kTileBytes);
-    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages,
-             *v_empty = v_full + C::kStages, *s_full = v_empty + C::kStages, *p_full = s_full + 2, *o_done = p_full + 4;
+    /* full[c]: V of tile c and K of tile c + 1; q_full: Q and the first K, used once */
+    uint64_t *q_full = bars, *k_done = bars + 1, *full = bars + 2, *empty = full + C::kStages, *s_full = empty + C::kStages,
+             *p_full = s_full + 2, *o_done = p_full + 2;
     __shared__ uint32_t tmem_slot;
     __shared__ Item s_item;
     __shared__ int s_ok;
-    __shared__ int s_bad[2], s_low[2];
+    __shared__ int s_bad[2];
+    __shared__ __align__(8) uint8_t s_low[2][8]; /* per tile and softmax warp: the low half of P is not all zero */
+    __shared__ float s_top[2][2][kRows], s_sum[2][2][kRows], s_end[2][2][kRows]; /* a row's two threads tell each other */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == 0) {
@@ -398,18 +412,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         if (lane == 0) {
             s_item = it, s_ok = ok, s_bad[0] = s_bad[1] = 0;
         }
-    } else if (warp == 8 && lane == 0) {
-        mbar_init(q_full, 1);
+    } else if (warp == kLoadWarp && lane == 0) {
+        mbar_init(q_full, 1), mbar_init(k_done, 1);
         for (int i = 0; i < C::kStages; ++i)
-            mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+            mbar_init(full + i, 1), mbar_init(empty + i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + 2 * i, 4), mbar_init(p_full + 2 * i + 1, 4);
+            mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + i, 8);
         mbar_init_fence();
     }
     __syncthreads();
     if (!s_ok)
         return;
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -437,43 +451,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         __syncwarp();
     };
 
-    if (warp == 8) {
+    if (warp == kLoadWarp) {
         /* ---- loads */
         if (lane == 0 && first < stop) {
-            const int rows = g.group * g.tok;
-            mbar_expect_tx(q_full, 2 * (D / 64) * rows * 128);
+            const int rows = g.group * g.tok, total = stop - first;
+            auto load = [&](uint8_t *to, const CUtensorMap *map, uint64_t *bar, int j) {
+                for (int d = 0; d < D / 64; ++d)
+                    tma_load_3d(to + d * kKeys * 128, map, bar, d * 64, it.head, s.k0 + j * kKeys);
+            };
+            mbar_expect_tx(q_full, 2 * (D / 64) * rows * 128 + C::kTileBytes);
             for (int i = 0; i < 2; ++i)
                 for (int d = 0; d < D / 64; ++d)
                     tma_load_3d(sq + i * C::kTileBytes + d * kRows * 128, &maps.q, q_full, d * 64, it.head * g.group,
                                 t0 + i * g.tok);
+            load(sk, &maps.k, q_full, first);
             int issued = 0;
-            for (int j = first; j < stop && alive; ++j, ++issued) {
-                const int st = issued % C::kStages;
-                const uint32_t ph = (issued / C::kStages + 1) & 1; /* first use: returns at once */
-                const int key = s.k0 + j * kKeys;
-                if (!wait(k_empty + st, ph))
+            for (int c = 0; c < total; ++c, ++issued) {
+                const int st = c % C::kStages;
+                const bool more = c + 1 < total;
+                /* the first use of a stage returns at once; the first K's place is free after its products */
+                if (!wait(empty + st, (c / C::kStages + 1) & 1) || (c == C::kStages - 1 && more && !wait(k_done, 0)))
                     break;
-                mbar_expect_tx(k_full + st, C::kTileBytes);
-                for (int d = 0; d < D / 64; ++d)
-                    tma_load_3d(sk + st * C::kTileBytes + d * kKeys * 128, &maps.k, k_full + st, d * 64, it.head, key);
-                if (!wait(v_empty + st, ph)) {
-                    ++issued; /* K of this one is in flight */
-                    break;
-                }
-                mbar_expect_tx(v_full + st, C::kTileBytes);
-                for (int d = 0; d < D / 64; ++d)
-                    tma_load_3d(sv + st * C::kTileBytes + d * kKeys * 128, &maps.v, v_full + st, d * 64, it.head, key);
+                mbar_expect_tx(full + st, (more ? 2 : 1) * C::kTileBytes);
+                load(sv + st * C::kTileBytes, &maps.v, full + st, first + c);
+                if (more)
+                    load(sk + (c + 1) % C::kStages * C::kTileBytes, &maps.k, full + st, first + c + 1);
             }
             if (!alive) { /* let the copies already started land before the CTA exits */
                 mbar_wait_bounded(q_full, 0, &g_attn_error);
-                for (int j = max(0, issued - C::kStages); j < issued; ++j) {
-                    mbar_wait_bounded(k_full + j % C::kStages, (j / C::kStages) & 1, &g_attn_error);
-                    mbar_wait_bounded(v_full + j % C::kStages, (j / C::kStages) & 1, &g_attn_error);
-                }
+                for (int c = max(0, issued - C::kStages); c < issued; ++c)
+                    mbar_wait_bounded(full + c % C::kStages, (c / C::kStages) & 1, &g_attn_error);
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == kMmaWarp) {
         /* ---- UMMA */
         if (lane == 0 && first < stop) {
             constexpr uint32_t kQk = idesc_of(kKeys, false), kPv = idesc_of(D, true);
@@ -489,212 +500,194 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             /* operands of 16 keys: P_i in TMEM, V in shared memory */
             auto p_at = [&](int i, int k) { return tmem + C::kS + 128 * i + (k / 2) * 32 + (k % 2) * 8; };
             auto v_at = [&](int st, int k) { return desc_outer(saddr(sv) + st * C::kTileBytes + k * 16 * 128); };
-            wait(q_full, 0);
-            wait(k_full, 0);
-            tc_after();
-            if (alive) {
+            const int total = stop - first;
+            if (wait(q_full, 0)) {
+                tc_after();
                 for (int i = 0; i < 2; ++i)
                     if (first < last[i])
                         scores(i, 0);
-                umma_commit(k_empty);
+                umma_commit(k_done);
             }
-            for (int j = first; j < stop && alive; ++j) {
-                const int c = j - first, st = c % C::kStages, nst = (c + 1) % C::kStages;
-                const bool more = j + 1 < stop;
-                if (more && !wait(k_full + nst, ((c + 1) / C::kStages) & 1))
-                    break;
-                if (!wait(v_full + st, (c / C::kStages) & 1))
-                    break;
-                for (int i = 0; i < 2; ++i) {
-                    if (j >= last[i])
+            for (int c = 0; c < total && alive; ++c) {
+                const int st = c % C::kStages, nst = (c + 1) % C::kStages;
+                wait(full + st, (c / C::kStages) & 1);
+                for (int i = 0; i < 2 && alive; ++i) {
+                    if (first + c >= last[i] || !wait(p_full + i, c & 1))
                         continue;
-                    for (int half = 0; half < 2; ++half) {
-                        if (!wait(p_full + 2 * i + half, c & 1))
-                            break;
-                        tc_after();
+                    tc_after();
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_ts(tmem + C::kO + D * i, p_at(i, half * 4 + k), v_at(st, half * 4 + k), kPv,
-                                    c > 0 || half > 0 || k > 0);
-                    }
-                    if (!alive)
-                        break;
-                    if (s_low[i]) {
+                    for (int k = 0; k < 8; ++k)
+                        umma_ts(tmem + C::kO + D * i, p_at(i, k), v_at(st, k), kPv, c > 0 || k > 0);
+                    if (*reinterpret_cast<const volatile uint64_t *>(s_low[i])) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
                     }
                     umma_commit(o_done + i);
-                    if (j + 1 < last[i])
+                    if (first + c + 1 < last[i])
                         scores(i, nst);
                 }
-                if (!alive)
-                    break;
-                if (more)
-                    umma_commit(k_empty + nst);
-                umma_commit(v_empty + st);
+                if (alive)
+                    umma_commit(empty + st);
             }
             /* the last commit has arrived before this CTA's memory can go */
-            wait(v_empty + (stop - 1 - first) % C::kStages, ((stop - 1 - first) / C::kStages) & 1);
+            wait(empty + (total - 1) % C::kStages, ((total - 1) / C::kStages) & 1);
         }
         __syncwarp();
-    } else if (warp < 8) {
-        /* ---- softmax of tile i, a row a thread */
-        const int i = warp >> 2, wl = warp & 3, r = wl * 32 + lane;
+    } else {
+        /* ---- softmax of tile i: row r, keys 64 hf to 64 hf + 63 of each tile of keys */
+        const int i = warp >> 3, hf = (warp >> 2) & 1, wl = warp & 3, r = wl * 32 + lane;
         const uint32_t lanes = (uint32_t)(wl * 32) << 16;
-        const uint32_t ts = tmem + C::kS + 128 * i + lanes, to = tmem + C::kO + D * i + lanes;
+        const uint32_t ts = tmem + C::kS + 128 * i + 64 * hf + lanes, to = tmem + C::kO + D * i + lanes;
         const int tile0 = t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
         const bool live = r < g.group * g.tok && t < s.q1;
         const int seen = live ? seen_of(g, s, t) : 0;
         const int all = tile0 < s.q1 ? seen_of(g, s, tile0) : 0; /* keys that every row sees */
         const float scale2 = g.a.scale * kLog2e;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f; /* of the row; of this thread's keys */
         bool odd = false;
         for (int j = first; j < last[i]; ++j) {
             const int c = j - first;
             warp_wait(s_full + i, c & 1);
             tc_after();
             const bool masked = (j + 1) * kKeys > all;
-            const int lim = masked ? seen - j * kKeys : kKeys;
-            /* S twice, 32 columns at a time and 32 more on their way: for the maximum, and
-             * for the weights (all 128 in registers at once would not fit beside the rest) */
-            uint32_t x[2][32];
-            tmem_ld32(ts, x[0]);
+            uint32_t x[64];
+            tmem_ld32(ts, x);
+            tmem_ld32(ts + 32, x + 32);
             if (masked) { /* V's odd values would reach rows that do not see them */
-                warp_wait(v_full + c % C::kStages, (c / C::kStages) & 1);
+                warp_wait(full + c % C::kStages, (c / C::kStages) & 1);
                 const uint4 *v = reinterpret_cast<const uint4 *>(sv + (c % C::kStages) * C::kTileBytes);
                 uint32_t any = 0;
 #pragma unroll 4
-                for (int e = r; e < C::kTileBytes / 16; e += kRows) {
+                for (int e = r + kRows * hf; e < C::kTileBytes / 16; e += 2 * kRows) {
                     const uint4 w = v[e];
                     any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
                 }
                 odd |= any != 0;
             }
-            float top = -INFINITY;
+            tmem_ld_wait(x);
+            tmem_ld_wait(x + 32);
+            if (masked) {
+                const int lim = seen - j * kKeys - 64 * hf;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                tmem_ld_wait(x[q & 1]);
-                tmem_ld32(ts + 32 * ((q + 1) & 3), x[(q + 1) & 1]);
-                float a = -INFINITY, b = -INFINITY;
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        a = fmaxf(a, 32 * q + e < lim ? __uint_as_float(x[q & 1][e]) : -INFINITY);
-                        b = fmaxf(b, 32 * q + e + 1 < lim ? __uint_as_float(x[q & 1][e + 1]) : -INFINITY);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        a = fmaxf(a, __uint_as_float(x[q & 1][e])), b = fmaxf(b, __uint_as_float(x[q & 1][e + 1]));
-                }
-                top = fmaxf(top, fmaxf(a, b));
+                for (int e = 0; e < 64; ++e)
+                    x[e] = e < lim ? x[e] : 0xFF800000u;
             }
-            /* rows that are no query's (of whatever lies there) take no part in what the warp decides */
+            float top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])), other = fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]));
+#pragma unroll
+            for (int e = 4; e < 64; e += 4) {
+                top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+                other = fmaxf(other, fmaxf(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])));
+            }
+            top = fmaxf(top, other);
+            /* the row's maximum and sum so far, from both of its threads */
+            s_top[i][hf][r] = top, s_sum[i][hf][r] = l;
+            some_sync(1 + 4 * i + wl, 64);
+            top = fmaxf(top, s_top[i][hf ^ 1][r]);
+            float sum_old = l + s_sum[i][hf ^ 1][r];
+            /* rows that are no query's (of whatever lies there) take no part in what the warps decide */
             top = live ? top * scale2 : -INFINITY;
             const bool grow = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
             if (__any_sync(0xFFFFFFFFu, grow)) {
                 const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - nm);
-                m = nm, l *= f;
-                if (c > 0) { /* O of the tiles before, once they are in */
+                m = nm, l *= f, sum_old *= f;
+                if (c > 0) { /* O of the tiles before, once they are in: half of the row's columns each */
                     warp_wait(o_done + i, (c - 1) & 1);
                     tc_after();
+#pragma unroll 1
+                    for (int q = hf * (D / 2); q < (hf + 1) * (D / 2); q += 8) {
+                        uint32_t o[8];
+                        tmem_ld8(to + q, o);
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {
-                        uint32_t o[32];
-                        tmem_ld32(to + 32 * q, o);
-                        tmem_ld_wait(o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
+                        for (int e = 0; e < 8; ++e)
                             o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(to + 32 * q, o);
+                        tmem_st8(to + q, o);
                     }
                     tmem_st_wait();
                 }
             }
             const float less = m == -INFINITY ? 0.f : -m;
-            const bool low = any_of_tile(i, ex2(top + less) * kHeavy > l);
-            if (r == 0)
-                s_low[i] = low;
+            const bool low = __any_sync(0xFFFFFFFFu, ex2(top + less) * kHeavy > sum_old);
+            if (lane == 0)
+                s_low[i][4 * hf + wl] = low;
             const uint64_t sc = pack2f(scale2, scale2), ls = pack2f(less, less);
             uint64_t sum = 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
                 uint32_t p[16];
-                tmem_ld_wait(x[q & 1]);
-                if (q < 3)
-                    tmem_ld32(ts + 32 * (q + 1), x[(q + 1) & 1]);
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        x[q & 1][e] = 32 * q + e < lim ? x[q & 1][e] : 0xFF800000u;
-                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
+                    uint32_t *v = x + 32 * q + 2 * e;
                     float a, b;
-                    unpack2f(fma2(pack2f(__uint_as_float(x[q & 1][2 * e]), __uint_as_float(x[q & 1][2 * e + 1])), sc, ls), a, b);
+                    unpack2f(fma2(pack2f(__uint_as_float(v[0]), __uint_as_float(v[1])), sc, ls), a, b);
                     a = ex2(a), b = ex2(b);
-                    x[q & 1][2 * e] = __float_as_uint(a), x[q & 1][2 * e + 1] = __float_as_uint(b);
                     sum = add2(sum, pack2f(a, b));
                     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
                     p[e] = *reinterpret_cast<const uint32_t *>(&h);
+                    v[0] = __float_as_uint(a), v[1] = __float_as_uint(b);
                 }
                 tmem_st16(ts + 32 * q, p);
+                /* what the rounding dropped; zeros where no row of the warp needs it, since
+                 * another warp's rows may, and one product serves them all */
                 if (low) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float a = __uint_as_float(x[q & 1][2 * e]) - __uint_as_float(p[e] << 16);
-                        const float b = __uint_as_float(x[q & 1][2 * e + 1]) - __uint_as_float(p[e] & 0xFFFF0000u);
+                        const float a = __uint_as_float(x[32 * q + 2 * e]) - __uint_as_float(p[e] << 16);
+                        const float b = __uint_as_float(x[32 * q + 2 * e + 1]) - __uint_as_float(p[e] & 0xFFFF0000u);
                         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
                         p[e] = *reinterpret_cast<const uint32_t *>(&h);
                     }
                     tmem_st16(ts + 32 * q + 16, p);
-                }
-                if (q & 1) {
-                    tmem_st_wait();
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0)
-                        mbar_arrive(p_full + 2 * i + (q >> 1));
+                } else {
+                    tmem_zero16(ts + 32 * q + 16);
                 }
             }
+            tmem_st_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(p_full + i);
             float a, b;
             unpack2f(sum, a, b);
             l += a + b;
         }
         if (odd)
             s_bad[i] = 1;
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory"); /* the tile's four warps */
+        s_end[i][hf][r] = l;
+        some_sync(9 + i, 256); /* the tile's eight warps */
+        l = s_end[i][0][r] + s_end[i][1][r];
         const int done = last[i] - first;
         if (done > 0) {
             warp_wait(o_done + i, (done - 1) & 1);
             tc_after();
         }
         const bool bad = s_bad[i] != 0;
+        const int d0 = hf * (D / 2); /* each thread finishes half of its row */
         if (it.cuts > 1) {
-            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
+            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D + d0;
             float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
+            for (int q = 0; q < D / 64; ++q) {
                 uint32_t o[32] = {};
                 if (done > 0) {
-                    tmem_ld32(to + 32 * q, o);
+                    tmem_ld32(to + d0 + 32 * q, o);
                     tmem_ld_wait(o);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
-            if (r == 0)
+            if (hf == 0)
+                ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
+            if (r == 0 && hf == 0)
                 reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
         } else if (!bad) {
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
+            for (int q = 0; q < D / 64; ++q) {
                 uint32_t o[32] = {};
                 if (done > 0) {
-                    tmem_ld32(to + 32 * q, o);
+                    tmem_ld32(to + d0 + 32 * q, o);
                     tmem_ld_wait(o);
                 }
                 float v[32];
@@ -702,12 +695,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 for (int e = 0; e < 32; ++e)
                     v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
                 if (live)
-                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
+                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + d0 + 32 * q, v);
             }
-            if (live && g.a.lse)
+            if (live && hf == 0 && g.a.lse)
                 g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         } else {
-            for (int k = wl; k < g.group * g.tok; k += 4) {
+            for (int k = warp & 7; k < g.group * g.tok; k += 8) {
                 const int tk = tile0 + k / g.group;
                 if (tk < s.q1)
                     plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
@@ -716,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         tc_before();
     }
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
