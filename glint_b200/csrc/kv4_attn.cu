@@ -31,7 +31,9 @@ namespace glint {
 namespace {
 
 constexpr int kTile = 32;        /* slots a warp takes at a time */
-constexpr int kJoin = 2;         /* what a segment costs beside its tiles, in tiles */
+/* What a segment costs beside its tiles, in tiles: with 2, 4, 6, 8, 12 thirty-two sequences
+ * of 3 to 8191 slots (8 heads of 128) took 49, 37, 32, 30, 30 us. */
+constexpr int kJoin = 8;
 constexpr int kWorker = 4;       /* a worker's range, at least */
 constexpr float kLazy = 8.f;     /* the running maximum may lag by 2^8 */
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -47,6 +49,7 @@ struct Cfg {
     static constexpr int kStages = NT == 1 && D == 128 ? 2 : 4;
     static constexpr int kCols = 8 * NT;
     static constexpr int kNb = D / 64;
+    static constexpr int kJoinThreads = kCols * (D / 4) < 256 ? kCols * (D / 4) : 256;
     static constexpr int kCode = kTile * D / 2, kMeta = kTile * kNb * 4;
     static constexpr int kStage = 2 * (kCode + kMeta);
     static constexpr int kState = kCols * D + 2 * kCols; /* floats: O, m, l */
@@ -61,6 +64,7 @@ struct Args {
     int chunks, segs;     /* column chunks a kv head; segments a sequence = kv_heads * chunks */
     int parts;            /* workers at most: workers of a CTA times CTAs */
     int page_log2;
+    bool vec;             /* q takes 16-byte loads */
     float *part;          /* [parts][2][kState] unfinished segments */
     float *score;         /* [seqs][kv_heads][max slots][cols] log2-scaled scores, or NULL */
     float *lse2;          /* [seqs][kv_heads][cols] log2 sums, with score */
@@ -83,15 +87,20 @@ __device__ __forceinline__ int tiles_of(const Args &g, int b) { return (length_o
  * of lengths keep every SM busy, and a range of many short segments, each with a query
  * to load and a result to write, is not taken for as little work as one long one. */
 struct Plan {
-    int64_t units;
-    int parts; /* workers with a range */
-    __device__ __forceinline__ int64_t begin(int i) const { return units * i / parts; }
-    __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * parts - 1) / units); }
+    int units;    /* the host has seen to it that they fit */
+    int parts;    /* workers with a range */
+    int each, more; /* units of a range; ranges with one more */
+    __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
+    __device__ __forceinline__ int owner(int u) const
+    {
+        const int big = more * (each + 1);
+        return u < big ? u / (each + 1) : more + (u - big) / each;
+    }
 };
 __device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + kJoin : 0; }
 __device__ __forceinline__ Plan plan_of(const Args &g)
 {
-    int64_t n = 0;
+    int n = 0;
     for (int b = threadIdx.x & 31; b < g.a.seqs; b += 32)
         n += cost_of(tiles_of(g, b));
 #pragma unroll
@@ -99,7 +108,8 @@ __device__ __forceinline__ Plan plan_of(const Args &g)
         n += __shfl_xor_sync(0xFFFFFFFFu, n, off);
     Plan p;
     p.units = n * g.segs;
-    p.parts = (int)max((int64_t)1, min((int64_t)g.parts, p.units / kWorker));
+    p.parts = max(1, min(g.parts, p.units / kWorker));
+    p.each = p.units / p.parts, p.more = p.units - p.each * p.parts;
     return p;
 }
 /* A segment on a walk along a range: `first` is its first tile's place, counted from
@@ -122,16 +132,16 @@ struct Walk {
         return b < g.a.seqs;
     }
 };
-__device__ __forceinline__ Walk locate(const Args &g, int64_t u) /* u < units; whole warp */
+__device__ __forceinline__ Walk locate(const Args &g, int u) /* u < units; whole warp */
 {
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;
+    int before = 0;
     for (int b0 = 0;; b0 += 32) {
         const int t = b0 + lane < g.a.seqs ? tiles_of(g, b0 + lane) : 0;
-        int64_t s = cost_of(t);
+        int s = cost_of(t);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int64_t o = __shfl_up_sync(0xFFFFFFFFu, s, off);
+            const int o = __shfl_up_sync(0xFFFFFFFFu, s, off);
             if (lane >= off)
                 s += o;
         }
@@ -142,9 +152,9 @@ __device__ __forceinline__ Walk locate(const Args &g, int64_t u) /* u < units; w
             w.b = b0 + l;
             w.tiles = __shfl_sync(0xFFFFFFFFu, t, l);
             const int cost = max(1, cost_of(w.tiles));
-            const int64_t off = u - (before + __shfl_sync(0xFFFFFFFFu, s, l) - cost) * g.segs;
-            w.seg = (int)(off / cost);
-            w.first = (int)((int64_t)w.seg * cost - off) + kJoin;
+            const int off = u - (before + __shfl_sync(0xFFFFFFFFu, s, l) - cost) * g.segs;
+            w.seg = off / cost;
+            w.first = w.seg * cost - off + kJoin;
             return w;
         }
         before += __shfl_sync(0xFFFFFFFFu, s, 31);
@@ -157,6 +167,25 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  "{%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+/* the same onto zero */
+__device__ __forceinline__ void mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+/* (step, lo) of a row's blocks */
+template <int NB>
+__device__ __forceinline__ void load_meta(uint32_t at, uint32_t (&m)[NB])
+{
+    if constexpr (NB == 2) {
+        const uint2 v = lds64(at);
+        m[0] = v.x, m[1] = v.y;
+    } else {
+        m[0] = lds32(at);
+    }
 }
 /* nibbles j and j + 4 of w as the BF16 pair (128 + code, 128 + code) */
 __device__ __forceinline__ uint32_t codes128(uint32_t w, int j)
@@ -237,9 +266,22 @@ __device__ __forceinline__ void load_query(const Args &g, int b, int seg, Query<
         for (int k = 0; k < D / 64; ++k) {
             uint32_t v[16];
             float s = 0.f;
+            if (g.vec) {
+                const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+                const uint4 a = live ? *reinterpret_cast<const uint4 *>(p + 64 * k) : z;
+                const uint4 c = live ? *reinterpret_cast<const uint4 *>(p + 64 * k + 8) : z;
+                const uint32_t w[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[2 * i] = w[i] & 0xFFFFu, v[2 * i + 1] = w[i] >> 16;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    v[i] = live ? (uint32_t)__bfloat16_as_ushort(p[64 * k + i]) : 0u;
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                v[i] = live ? (uint32_t)__bfloat16_as_ushort(p[64 * k + i]) ^ sign : 0u;
+                v[i] ^= live ? sign : 0u;
                 s += __uint_as_float(v[i] << 16);
             }
 #pragma unroll
@@ -279,11 +321,6 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
         float acc[NB][NT][4];
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[k][n][i] = 0.f;
             const uint2 wa = lds64(kcode + ta * RB + kv4_unit<D>(k, ta) + 8 * c);
             const uint2 wb = lds64(kcode + tb * RB + kv4_unit<D>(k, tb) + 8 * c);
 #pragma unroll
@@ -291,7 +328,8 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
                 const uint32_t a[4] = {codes128(wa.x, j), codes128(wb.x, j), codes128(wa.y, j), codes128(wb.y, j)};
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    mma(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1]);
+                    j ? mma(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1])
+                      : mma0(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1]);
             }
         }
 #pragma unroll
@@ -299,9 +337,12 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 s[sl][n][i] = 0.f;
+        uint32_t mas[NB], mbs[NB];
+        load_meta(kmeta + ta * NB * 4, mas);
+        load_meta(kmeta + tb * NB * 4, mbs);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const uint32_t ma = lds32(kmeta + (ta * NB + k) * 4), mb = lds32(kmeta + (tb * NB + k) * 4);
+            const uint32_t ma = mas[k], mb = mbs[k];
             const float sa = __uint_as_float(ma << 16), sb = __uint_as_float(mb << 16);
             const float la = fmaf(-128.f, sa, __uint_as_float(ma & 0xFFFF0000u));
             const float lb = fmaf(-128.f, sb, __uint_as_float(mb & 0xFFFF0000u));
@@ -382,9 +423,12 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
         const int ta = sl * 16 + tg, tb = ta + 8;
         uint32_t pb[NT][NB][2];
         float steps[NB][2], mids[NB][2];
+        uint32_t mas[NB], mbs[NB];
+        load_meta(vmeta + ta * NB * 4, mas);
+        load_meta(vmeta + tb * NB * 4, mbs);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const uint32_t ma = lds32(vmeta + (ta * NB + k) * 4), mb = lds32(vmeta + (tb * NB + k) * 4);
+            const uint32_t ma = mas[k], mb = mbs[k];
             steps[k][0] = __uint_as_float(ma << 16), steps[k][1] = __uint_as_float(mb << 16);
             mids[k][0] = fmaf(8.f, steps[k][0], __uint_as_float(ma & 0xFFFF0000u));
             mids[k][1] = fmaf(8.f, steps[k][1], __uint_as_float(mb & 0xFFFF0000u));
@@ -588,8 +632,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) kv4_attn_kernel(const
     const int worker = (warp / kGroup) * gridDim.x + blockIdx.x, w = warp % kGroup;
     if (worker >= plan.parts || plan.units == 0)
         return;
-    const int64_t begin = plan.begin(worker);
-    const int range = (int)(plan.begin(worker + 1) - begin);
+    const int begin = plan.begin(worker), range = plan.begin(worker + 1) - begin;
     Walk at = locate(g, begin);
 
     const uint32_t ring = saddr(smem + warp * C::kStages * C::kStage);
@@ -685,57 +728,97 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) kv4_attn_kernel(const
     } while (at.next(g, range));
 }
 
+constexpr int kJoinParts = 32;
 /* Joins the parts of the segment that begins in worker blockIdx.x's range and runs on
  * past it. */
 template <int D, int NT>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const Args g)
+__global__ void __launch_bounds__(Cfg<D, NT>::kJoinThreads) kv4_join_kernel(const Args g)
 {
     using C = Cfg<D, NT>;
+    __shared__ float ms[C::kCols][kJoinParts + 1], ls[C::kCols][kJoinParts + 1];
     const Plan plan = plan_of(g);
     const int i = blockIdx.x;
+    Walk at{};
+    int last = i;
+    if (i + 1 < plan.parts && plan.units > 0) {
+        const int begin = plan.begin(i), end = plan.begin(i + 1);
+        at = locate(g, end - 1);
+        const int first = end - 1 + at.first; /* the segment's first tile in the row */
+        if (first >= begin && first < end && first + at.tiles > end)
+            last = plan.owner(first + at.tiles - 1);
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory"); /* in every CTA: this kernel ends after the one before */
-    if (i + 1 >= plan.parts || plan.units == 0)
+    if (last == i)
         return;
-    const int64_t begin = plan.begin(i), end = plan.begin(i + 1);
-    const Walk at = locate(g, end - 1);
-    const int64_t first = end - 1 + at.first; /* the segment's first tile in the row */
-    if (first < begin || first >= end || first + at.tiles <= end)
-        return;
-    const int last = plan.owner(first + at.tiles - 1);
-    for (int e = threadIdx.x; e < C::kCols * (D / 4); e += 256) {
-        const int n = e / (D / 4), d = e % (D / 4) * 4;
-        float m = -INFINITY, l = 0.f;
-        for (int p = i; p <= last; ++p)
-            m = fmaxf(m, g.part[((int64_t)p * 2 + (p == i)) * C::kState + C::kCols * D + n]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = i; p <= last; ++p) {
-            const float *s = g.part + ((int64_t)p * 2 + (p == i)) * C::kState;
-            const float mp = s[C::kCols * D + n], fp = mp == -INFINITY ? 0.f : ex2(mp - m);
-            const float4 v = *reinterpret_cast<const float4 *>(s + n * D + d);
-            l = fmaf(fp, s[C::kCols * D + C::kCols + n], l);
-            o.x = fmaf(fp, v.x, o.x), o.y = fmaf(fp, v.y, o.y), o.z = fmaf(fp, v.z, o.z), o.w = fmaf(fp, v.w, o.w);
+    /* kJoinParts parts a time: their maxima and sums side by side, then their rows */
+    constexpr int T = C::kJoinThreads, N = C::kCols * (D / 4) / T;
+    float m[N], l[N];
+    float4 o[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        m[k] = -INFINITY, l[k] = 0.f, o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = i; p0 <= last; p0 += kJoinParts) {
+        const int np = min(kJoinParts, last + 1 - p0);
+        for (int e = threadIdx.x; e < np * C::kCols; e += T) {
+            const int p = p0 + e / C::kCols, n = e % C::kCols;
+            const float *s = g.part + ((int64_t)p * 2 + (p == i)) * C::kState + C::kCols * D;
+            ms[n][p - p0] = s[n], ls[n][p - p0] = s[C::kCols + n];
         }
-        write_column4<D>(g, at.b, at.seg, C::kCols, n, d, o, m, l);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int e = threadIdx.x + T * k, n = e / (D / 4), d = e % (D / 4) * 4;
+            float top = m[k];
+            for (int p = 0; p < np; ++p)
+                top = fmaxf(top, ms[n][p]);
+            const float f0 = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
+            l[k] *= f0;
+            o[k].x *= f0, o[k].y *= f0, o[k].z *= f0, o[k].w *= f0;
+            m[k] = top;
+#pragma unroll 8
+            for (int p = 0; p < np; ++p) {
+                const float4 v = *reinterpret_cast<const float4 *>(
+                    g.part + ((int64_t)(p0 + p) * 2 + (p0 + p == i)) * C::kState + n * D + d);
+                const float f = ms[n][p] == -INFINITY ? 0.f : ex2(ms[n][p] - top);
+                l[k] = fmaf(f, ls[n][p], l[k]);
+                o[k].x = fmaf(f, v.x, o[k].x), o[k].y = fmaf(f, v.y, o[k].y);
+                o[k].z = fmaf(f, v.z, o[k].z), o[k].w = fmaf(f, v.w, o[k].w);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int e = threadIdx.x + T * k, n = e / (D / 4), d = e % (D / 4) * 4;
+        write_column4<D>(g, at.b, at.seg, C::kCols, n, d, o[k], m[k], l[k]);
     }
 }
 
-/* weight_out from the scores: a thread per slot, the columns in order */
+/* weight_out from the scores: a thread per slot, the columns in order (four a load where
+ * they are a multiple of four) */
 __global__ void __launch_bounds__(256) kv4_weight_kernel(const Args g)
 {
     const int bh = blockIdx.y, b = bh / g.c.kv_heads;
     const int len = length_of(g, b), t = blockIdx.x * 256 + threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory"); /* scores and sums are the kernels' before */
     if (t >= len)
         return;
-    const int cap = g.a.max_pages * g.c.page_size;
-    const int page = g.a.table[(int64_t)b * g.a.max_pages + (t >> g.page_log2)];
-    const float *s = g.score + ((int64_t)bh * cap + t) * g.cols, *z = g.lse2 + (int64_t)bh * g.cols;
-    float sum = 0.f;
-    if (page >= 0 && page < g.c.pages)
-        for (int n = 0; n < g.cols; ++n)
-            if (s[n] != -INFINITY)
-                sum += ex2(s[n] - z[n]);
     const int64_t i = (int64_t)bh * g.a.weight_stride + t;
     const float old = g.a.weight && t < len - g.a.rows ? g.a.weight[i] : 0.f;
+    const int page = g.a.table[(int64_t)b * g.a.max_pages + (t >> g.page_log2)];
+    const float *s = g.score + ((int64_t)bh * (g.a.max_pages << g.page_log2) + t) * g.cols, *z = g.lse2 + (int64_t)bh * g.cols;
+    float sum = 0.f;
+    auto add = [&](float v, float zn) { sum += v == -INFINITY ? 0.f : ex2(v - zn); };
+    if (page >= 0 && page < g.c.pages) {
+        int n = 0;
+        if (g.cols % 4 == 0)
+            for (; n < g.cols; n += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(s + n), y = *reinterpret_cast<const float4 *>(z + n);
+                add(v.x, y.x), add(v.y, y.y), add(v.z, y.z), add(v.w, y.w);
+            }
+        for (; n < g.cols; ++n)
+            add(s[n], z[n]);
+    }
     g.a.weight_out[i] = old + sum;
 }
 
@@ -747,6 +830,10 @@ int check(const GlintKv4Cache *c, const GlintKv4Attn *a)
     if (!a || a->seqs < 0 || a->rows < 1 || a->heads < 1 || a->heads % c->kv_heads || a->max_pages < 1 ||
         (int64_t)a->heads / c->kv_heads * a->rows > 256 || (int64_t)a->max_pages * c->page_size > INT32_MAX ||
         (int64_t)a->seqs * c->kv_heads > 65535)
+        return kBadArg;
+    /* the row of segments is counted in 32 bits */
+    const int64_t cols = (int64_t)a->heads / c->kv_heads * a->rows, chunks = cols <= 8 ? 1 : (cols + 15) / 16;
+    if ((((int64_t)a->max_pages * c->page_size + kTile - 1) / kTile + kJoin) * a->seqs * c->kv_heads * chunks > INT32_MAX)
         return kBadArg;
     return kOk;
 }
@@ -795,15 +882,16 @@ int launch(Args &g, cudaStream_t st)
         kv4_attn_kernel<D, NT, false><<<grid, C::kThreads, C::kSmem, st>>>(g);
     if (cudaGetLastError() != cudaSuccess)
         return kLaunch;
-    if (launch_after(kv4_join_kernel<D, NT>, dim3(g.parts), 256, st, g) != cudaSuccess) {
+    if (launch_after(kv4_join_kernel<D, NT>, dim3(g.parts), C::kJoinThreads, st, g) != cudaSuccess) {
         cudaGetLastError();
         return kLaunch;
     }
     if (g.score) {
-        const int cap = g.a.max_pages * g.c.page_size;
-        kv4_weight_kernel<<<dim3((cap + 255) / 256, g.a.seqs * g.c.kv_heads), 256, 0, st>>>(g);
-        if (cudaGetLastError() != cudaSuccess)
+        const dim3 grid((g.a.max_pages * g.c.page_size + 255) / 256, g.a.seqs * g.c.kv_heads);
+        if (launch_after(kv4_weight_kernel, grid, 256, st, g) != cudaSuccess) {
+            cudaGetLastError();
             return kLaunch;
+        }
     }
     return kOk;
 }
@@ -839,6 +927,7 @@ int glint_kv4_attn_stream(const GlintKv4Cache *c, const GlintKv4Attn *a, cudaStr
     g.group = a->heads / c->kv_heads, g.cols = g.group * a->rows;
     while ((1 << g.page_log2) < c->page_size)
         ++g.page_log2;
+    g.vec = aligned_to(a->q, 16) && (a->q_seq | a->q_row | a->q_head) % 8 == 0;
     const Work w = work_of(*c, *a);
     uint8_t *work = static_cast<uint8_t *>(a->work);
     g.part = reinterpret_cast<float *>(work);

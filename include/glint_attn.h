@@ -90,7 +90,9 @@ int glint_kv4_read_stream(const GlintKv4Cache *c, const int *slots, int tokens, 
  * when NULL and in the newest `rows` slots; slots >= lens[b] are not written; weight
  * may be weight_out.  work: glint_kv4_attn_work_bytes() of 16-byte aligned device
  * memory, the call's own until it completes, of any content.
- * Limits: rows >= 1, heads / kv_heads * rows <= 256. */
+ * Limits: rows >= 1, heads / kv_heads * rows <= 256, seqs * kv_heads <= 65535, and
+ * max_pages * page_size / 32 tiles times seqs * kv_heads (times a 16th of heads /
+ * kv_heads * rows where that is above 16) in 31 bits. */
 typedef struct GlintKv4Attn {
     const glint_bf16_t *q;
     glint_bf16_t *o;
