@@ -5,7 +5,7 @@
  * group's heads share every K and V tile that is loaded.  Per tile of 128 keys
  *
  *   S = Q K^T          UMMA 128 x 128 x D, Q and K in shared memory (TMA, 128-byte swizzle)
- *   P = 2^(S c - m)    two threads a row: S from TMEM, running maximum m and sum l in f32,
+ *   P = 2^(S c - m)    a thread per row: S from TMEM, running maximum m and sum l in f32,
  *                      P as BF16 back into S's columns (2^-8 of each weight at most, the
  *                      rounding that the tensor cores' operand asks for)
  *   O += P V           UMMA 128 x D x 128, P from TMEM, V as it lies (inner index = key rows)
@@ -141,11 +141,10 @@ struct Cfg {
      * time, 16 columns of P and 16 of what P's rounding dropped. */
     static constexpr uint32_t kS = 0, kO = 256;
 };
-/* warps 0-15: softmax, eight for each tile (four for keys 0-63 of a tile of keys, four for
- * 64-127; two threads share a row); 16: loads; 17: UMMA, the two tiles in turn (one
+/* warps 0-3, 4-7: softmax of the two tiles; 8: loads; 9: UMMA, the two tiles in turn (one
  * thread each let them fall into step, both in softmax and then both in UMMA: 1.3 times
- * the time) */
-constexpr int kLoadWarp = 16, kMmaWarp = 17, kThreads = 576;
+ * the time; two threads a row of softmax: as fast over 16384 keys, 4 % slower over fewer) */
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kThreads = 320;
 constexpr int kSlotRows = 2 * kRows;
 
 struct Args {
@@ -381,6 +380,13 @@ __device__ __forceinline__ void store_row32(const Args &g, __nv_bfloat16 *o, con
 /* any NaN or infinity among two BF16 */
 __device__ __forceinline__ uint32_t odd2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(uint32_t a, uint32_t b) { return max_nan(__uint_as_float(a), __uint_as_float(b)); }
 /* barrier `id` of n threads */
 __device__ __forceinline__ void some_sync(int id, int n)
 {
@@ -402,8 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __shared__ Item s_item;
     __shared__ int s_ok;
     __shared__ int s_bad[2];
-    __shared__ __align__(8) uint8_t s_low[2][8]; /* per tile and softmax warp: the low half of P is not all zero */
-    __shared__ float s_top[2][2][kRows], s_sum[2][2][kRows], s_end[2][2][kRows]; /* a row's two threads tell each other */
+    __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: the low half of P is not all zero */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == 0) {
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         for (int i = 0; i < C::kStages; ++i)
             mbar_init(full + i, 1), mbar_init(empty + i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + i, 8);
+            mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + i, 4);
         mbar_init_fence();
     }
     __syncthreads();
@@ -433,13 +438,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     const uint32_t tmem = tmem_slot;
     const Item it = s_item;
     const Span s = it.s;
-    /* tiles of keys that each query tile goes through: [first, last[i]) */
+    /* tiles of keys that each query tile goes through: [first, last_of(i)) */
     const int t0 = s.q0 + it.block * 2 * g.tok;
     int n[2];
     tiles_of(g, it, n);
     const int most = max(n[0], n[1]);
     const int first = cut_begin(most, it.cut, it.cuts), stop = cut_begin(most, it.cut + 1, it.cuts);
-    const int last[2] = {max(first, min(n[0], stop)), max(first, min(n[1], stop))};
+    /* of query tile i: up to last_of(i) (no array: its index is not a constant) */
+    const int last0 = max(first, min(n[0], stop)), last1 = max(first, min(n[1], stop));
+    auto last_of = [&](int i) { return i ? last1 : last0; };
     bool alive = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (alive)
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             if (wait(q_full, 0)) {
                 tc_after();
                 for (int i = 0; i < 2; ++i)
-                    if (first < last[i])
+                    if (first < last_of(i))
                         scores(i, 0);
                 umma_commit(k_done);
             }
@@ -512,19 +519,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const int st = c % C::kStages, nst = (c + 1) % C::kStages;
                 wait(full + st, (c / C::kStages) & 1);
                 for (int i = 0; i < 2 && alive; ++i) {
-                    if (first + c >= last[i] || !wait(p_full + i, c & 1))
+                    if (first + c >= last_of(i) || !wait(p_full + i, c & 1))
                         continue;
                     tc_after();
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         umma_ts(tmem + C::kO + D * i, p_at(i, k), v_at(st, k), kPv, c > 0 || k > 0);
-                    if (*reinterpret_cast<const volatile uint64_t *>(s_low[i])) {
+                    if (*reinterpret_cast<const volatile uint32_t *>(s_low[i])) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
                     }
                     umma_commit(o_done + i);
-                    if (first + c + 1 < last[i])
+                    if (first + c + 1 < last_of(i))
                         scores(i, nst);
                 }
                 if (alive)
@@ -535,67 +542,70 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         }
         __syncwarp();
     } else {
-        /* ---- softmax of tile i: row r, keys 64 hf to 64 hf + 63 of each tile of keys */
-        const int i = warp >> 3, hf = (warp >> 2) & 1, wl = warp & 3, r = wl * 32 + lane;
+        /* ---- softmax of tile i, row r */
+        const int i = warp >> 2, wl = warp & 3, r = wl * 32 + lane;
         const uint32_t lanes = (uint32_t)(wl * 32) << 16;
-        const uint32_t ts = tmem + C::kS + 128 * i + 64 * hf + lanes, to = tmem + C::kO + D * i + lanes;
-        const int tile0 = t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
-        const bool live = r < g.group * g.tok && t < s.q1;
-        const int seen = live ? seen_of(g, s, t) : 0;
-        const int all = tile0 < s.q1 ? seen_of(g, s, tile0) : 0; /* keys that every row sees */
+        const uint32_t ts = tmem + C::kS + 128 * i + lanes, to = tmem + C::kO + D * i + lanes;
+        /* Few registers live through this loop: 128 hold scores, and a spilled one would come
+         * back from L2 (the tiles leave next to no L1). */
+        int seen; /* keys this row sees; 0 where it is no query's */
+        {
+            const int t = t0 + i * g.tok + r / g.group;
+            seen = r < g.group * g.tok && t < s.q1 ? seen_of(g, s, t) : 0;
+        }
+        /* tiles of keys from `plain` on have a place that some row does not see */
+        const int plain = t0 + i * g.tok < s.q1 ? seen_of(g, s, t0 + i * g.tok) / kKeys - first : 0;
         const float scale2 = g.a.scale * kLog2e;
         float m = -INFINITY, l = 0.f; /* of the row; of this thread's keys */
-        bool odd = false;
-        for (int j = first; j < last[i]; ++j) {
-            const int c = j - first;
+        const int done = last_of(i) - first;
+#pragma unroll 1
+        for (int c = 0; c < done; ++c) {
             warp_wait(s_full + i, c & 1);
             tc_after();
-            const bool masked = (j + 1) * kKeys > all;
-            uint32_t x[64];
-            tmem_ld32(ts, x);
-            tmem_ld32(ts + 32, x + 32);
+            const bool masked = c >= plain;
+            uint32_t x[kKeys];
+#pragma unroll
+            for (int q = 0; q < kKeys; q += 32)
+                tmem_ld32(ts + q, x + q);
             if (masked) { /* V's odd values would reach rows that do not see them */
                 warp_wait(full + c % C::kStages, (c / C::kStages) & 1);
                 const uint4 *v = reinterpret_cast<const uint4 *>(sv + (c % C::kStages) * C::kTileBytes);
                 uint32_t any = 0;
 #pragma unroll 4
-                for (int e = r + kRows * hf; e < C::kTileBytes / 16; e += 2 * kRows) {
+                for (int e = r; e < C::kTileBytes / 16; e += kRows) {
                     const uint4 w = v[e];
                     any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
                 }
-                odd |= any != 0;
+                if (any)
+                    s_bad[i] = 1;
             }
-            tmem_ld_wait(x);
-            tmem_ld_wait(x + 32);
-            if (masked) {
-                const int lim = seen - j * kKeys - 64 * hf;
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
+            for (int q = 0; q < kKeys; q += 32)
+                tmem_ld_wait(x + q);
+            if (masked) {
+                const int lim = seen - (first + c) * kKeys;
+#pragma unroll
+                for (int e = 0; e < kKeys; ++e)
                     x[e] = e < lim ? x[e] : 0xFF800000u;
             }
-            float top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])), other = fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]));
+            float top = max_nan(x[0], x[1]), other = max_nan(x[2], x[3]);
 #pragma unroll
-            for (int e = 4; e < 64; e += 4) {
-                top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-                other = fmaxf(other, fmaxf(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])));
+            for (int e = 4; e < kKeys; e += 4) {
+                top = max_nan(top, max_nan(x[e], x[e + 1]));
+                other = max_nan(other, max_nan(x[e + 2], x[e + 3]));
             }
-            top = fmaxf(top, other);
-            /* the row's maximum and sum so far, from both of its threads */
-            s_top[i][hf][r] = top, s_sum[i][hf][r] = l;
-            some_sync(1 + 4 * i + wl, 64);
-            top = fmaxf(top, s_top[i][hf ^ 1][r]);
-            float sum_old = l + s_sum[i][hf ^ 1][r];
             /* rows that are no query's (of whatever lies there) take no part in what the warps decide */
-            top = live ? top * scale2 : -INFINITY;
-            const bool grow = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
-            if (__any_sync(0xFFFFFFFFu, grow)) {
-                const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - nm);
-                m = nm, l *= f, sum_old *= f;
-                if (c > 0) { /* O of the tiles before, once they are in: half of the row's columns each */
+            top = seen > 0 ? max_nan(top, other) * scale2 : -INFINITY;
+            if (__any_sync(0xFFFFFFFFu, !(top <= m + kLazy))) { /* NaN too */
+                /* a NaN or an infinite score: every weight of the row is NaN from here on */
+                const float nm = top < INFINITY ? fmaxf(m, top) : __int_as_float(0x7FFFFFFF);
+                const float f = m == -INFINITY && nm == nm ? 0.f : ex2(m - nm);
+                m = m == m ? nm : m, l *= f;
+                if (c > 0) { /* O of the tiles before, once they are in */
                     warp_wait(o_done + i, (c - 1) & 1);
                     tc_after();
 #pragma unroll 1
-                    for (int q = hf * (D / 2); q < (hf + 1) * (D / 2); q += 8) {
+                    for (int q = 0; q < D; q += 8) {
                         uint32_t o[8];
                         tmem_ld8(to + q, o);
 #pragma unroll
@@ -607,13 +617,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
             }
             const float less = m == -INFINITY ? 0.f : -m;
-            const bool low = __any_sync(0xFFFFFFFFu, ex2(top + less) * kHeavy > sum_old);
+            const bool low = __any_sync(0xFFFFFFFFu, ex2(top + less) * kHeavy > l);
             if (lane == 0)
-                s_low[i][4 * hf + wl] = low;
+                s_low[i][wl] = low;
             const uint64_t sc = pack2f(scale2, scale2), ls = pack2f(less, less);
             uint64_t sum = 0;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int q = 0; q < kKeys / 32; ++q) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -651,43 +661,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             unpack2f(sum, a, b);
             l += a + b;
         }
-        if (odd)
-            s_bad[i] = 1;
-        s_end[i][hf][r] = l;
-        some_sync(9 + i, 256); /* the tile's eight warps */
-        l = s_end[i][0][r] + s_end[i][1][r];
-        const int done = last[i] - first;
+        some_sync(1 + i, 128); /* the tile's warps: what they found in V */
+        const int tile0 = t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
+        const bool live = r < g.group * g.tok && t < s.q1;
         if (done > 0) {
             warp_wait(o_done + i, (done - 1) & 1);
             tc_after();
         }
         const bool bad = s_bad[i] != 0;
-        const int d0 = hf * (D / 2); /* each thread finishes half of its row */
         if (it.cuts > 1) {
-            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D + d0;
+            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
             float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
 #pragma unroll 1
-            for (int q = 0; q < D / 64; ++q) {
+            for (int q = 0; q < D / 32; ++q) {
                 uint32_t o[32] = {};
                 if (done > 0) {
-                    tmem_ld32(to + d0 + 32 * q, o);
+                    tmem_ld32(to + 32 * q, o);
                     tmem_ld_wait(o);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            if (hf == 0)
-                ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
-            if (r == 0 && hf == 0)
+            ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
+            if (r == 0)
                 reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
         } else if (!bad) {
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll 1
-            for (int q = 0; q < D / 64; ++q) {
+            for (int q = 0; q < D / 32; ++q) {
                 uint32_t o[32] = {};
                 if (done > 0) {
-                    tmem_ld32(to + d0 + 32 * q, o);
+                    tmem_ld32(to + 32 * q, o);
                     tmem_ld_wait(o);
                 }
                 float v[32];
@@ -695,12 +700,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 for (int e = 0; e < 32; ++e)
                     v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
                 if (live)
-                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + d0 + 32 * q, v);
+                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
             }
-            if (live && hf == 0 && g.a.lse)
+            if (live && g.a.lse)
                 g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         } else {
-            for (int k = warp & 7; k < g.group * g.tok; k += 8) {
+            for (int k = wl; k < g.group * g.tok; k += 4) {
                 const int tk = tile0 + k / g.group;
                 if (tk < s.q1)
                     plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
