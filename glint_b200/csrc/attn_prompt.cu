@@ -287,6 +287,7 @@ constexpr int kCut = 4;
 struct Item {
     Span s;
     int block, head, cut, cuts, slot;
+    int t0, first, last0, last1; /* first token; query tile i goes through the tiles of keys [first, lasti) */
 };
 __device__ __forceinline__ int blocks_of(const Args &g, int seq)
 {
@@ -387,12 +388,21 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return r;
 }
 __device__ __forceinline__ float max_nan(uint32_t a, uint32_t b) { return max_nan(__uint_as_float(a), __uint_as_float(b)); }
-/* barrier `id` of n threads */
-__device__ __forceinline__ void some_sync(int id, int n)
+/* whether any of a tile's 128 softmax threads has `p` */
+__device__ __forceinline__ bool any_of_tile(int i, bool p)
 {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                 : "=r"(r)
+                 : "r"((uint32_t)p), "r"(1 + i)
+                 : "memory");
+    return r != 0;
 }
 
+/* One CTA an SM for all items: barriers and TMEM are set up once, and while a tile's
+ * softmax warps write one item's rows, the next item's loads and first products run.
+ * K of the tiles of keys, and V of them, stand in rings that run on from item to item. */
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant__ Args g, const __grid_constant__ Maps maps)
 {
@@ -401,33 +411,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     uint8_t *smem = raw + ((1024 - (saddr(raw) & 1023)) & 1023);
     uint8_t *sq = smem, *sk = sq + 2 * C::kTileBytes, *sv = sk + C::kStages * C::kTileBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sv + C::kStages * C::kTileBytes);
-    /* full[c]: V of tile c and K of tile c + 1; q_full: Q and the first K, used once */
-    uint64_t *q_full = bars, *k_done = bars + 1, *full = bars + 2, *empty = full + C::kStages, *s_full = empty + C::kStages,
-             *p_full = s_full + 2, *o_done = p_full + 2;
+    /* q_full: an item's Q and first K; kv_full[p]: V of the tile at ring place p and K of the next one */
+    uint64_t *q_full = bars, *q_empty = bars + 1, *item_full = bars + 2, *item_empty = bars + 4, *s_full = bars + 6,
+             *p_full = bars + 8, *o_done = bars + 10, *kv_full = bars + 12, *k_empty = kv_full + C::kStages,
+             *v_empty = k_empty + C::kStages;
     __shared__ uint32_t tmem_slot;
-    __shared__ Item s_item;
-    __shared__ int s_ok;
-    __shared__ int s_bad[2];
+    __shared__ Item s_item[2];
+    __shared__ int s_more[2];
     __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: the low half of P is not all zero */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (warp == 0) {
-        Item it;
-        const bool ok = item_of(g, blockIdx.x, it) && it.cut < it.cuts;
-        if (lane == 0) {
-            s_item = it, s_ok = ok, s_bad[0] = s_bad[1] = 0;
-        }
-    } else if (warp == kLoadWarp && lane == 0) {
-        mbar_init(q_full, 1), mbar_init(k_done, 1);
+    if (warp == kLoadWarp && lane == 0) {
+        mbar_init(q_full, 1), mbar_init(q_empty, 1);
         for (int i = 0; i < C::kStages; ++i)
-            mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; ++i)
+            mbar_init(kv_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_empty + i, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(item_full + i, 1), mbar_init(item_empty + i, 9); /* eight softmax warps and the UMMA one */
             mbar_init(s_full + i, 1), mbar_init(o_done + i, 1), mbar_init(p_full + i, 4);
+        }
         mbar_init_fence();
     }
-    __syncthreads();
-    if (!s_ok)
-        return;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -436,17 +439,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
-    const Item it = s_item;
-    const Span s = it.s;
-    /* tiles of keys that each query tile goes through: [first, last_of(i)) */
-    const int t0 = s.q0 + it.block * 2 * g.tok;
-    int n[2];
-    tiles_of(g, it, n);
-    const int most = max(n[0], n[1]);
-    const int first = cut_begin(most, it.cut, it.cuts), stop = cut_begin(most, it.cut + 1, it.cuts);
-    /* of query tile i: up to last_of(i) (no array: its index is not a constant) */
-    const int last0 = max(first, min(n[0], stop)), last1 = max(first, min(n[1], stop));
-    auto last_of = [&](int i) { return i ? last1 : last0; };
     bool alive = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (alive)
@@ -459,41 +451,71 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     };
 
     if (warp == kLoadWarp) {
-        /* ---- loads */
-        if (lane == 0 && first < stop) {
-            const int rows = g.group * g.tok, total = stop - first;
-            auto load = [&](uint8_t *to, const CUtensorMap *map, uint64_t *bar, int j) {
-                for (int d = 0; d < D / 64; ++d)
-                    tma_load_3d(to + d * kKeys * 128, map, bar, d * 64, it.head, s.k0 + j * kKeys);
-            };
-            mbar_expect_tx(q_full, 2 * (D / 64) * rows * 128 + C::kTileBytes);
-            for (int i = 0; i < 2; ++i)
-                for (int d = 0; d < D / 64; ++d)
-                    tma_load_3d(sq + i * C::kTileBytes + d * kRows * 128, &maps.q, q_full, d * 64, it.head * g.group,
-                                t0 + i * g.tok);
-            load(sk, &maps.k, q_full, first);
-            int issued = 0;
-            for (int c = 0; c < total; ++c, ++issued) {
-                const int st = c % C::kStages;
-                const bool more = c + 1 < total;
-                /* the first use of a stage returns at once; the first K's place is free after its products */
-                if (!wait(empty + st, (c / C::kStages + 1) & 1) || (c == C::kStages - 1 && more && !wait(k_done, 0)))
-                    break;
-                mbar_expect_tx(full + st, (more ? 2 : 1) * C::kTileBytes);
-                load(sv + st * C::kTileBytes, &maps.v, full + st, first + c);
-                if (more)
-                    load(sk + (c + 1) % C::kStages * C::kTileBytes, &maps.k, full + st, first + c + 1);
+        /* ---- items and loads */
+        int place = 0, items = 0, queries = 0; /* ring place; items published; of them with tiles */
+        for (int round = 0;; ++round) {
+            /* every other round in reverse: the items fall in cost, and the CTAs take turns at the dear end */
+            Item it;
+            const int index = round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+            const bool more = item_of(g, index, it);
+            if (more && it.cut >= it.cuts)
+                continue;
+            if (lane == 0) {
+                if (more) {
+                    it.t0 = it.s.q0 + it.block * 2 * g.tok;
+                    int n[2];
+                    tiles_of(g, it, n);
+                    const int most = max(n[0], n[1]), stop = cut_begin(most, it.cut + 1, it.cuts);
+                    it.first = cut_begin(most, it.cut, it.cuts);
+                    it.last0 = max(it.first, min(n[0], stop)), it.last1 = max(it.first, min(n[1], stop));
+                }
+                wait(item_empty + (items & 1), (items / 2 + 1) & 1); /* first uses return at once */
+                s_more[items & 1] = more && alive, s_item[items & 1] = it;
+                mbar_arrive(item_full + (items & 1));
+                const int total = more ? max(it.last0, it.last1) - it.first : 0;
+                if (total > 0 && wait(q_empty, (queries + 1) & 1)) {
+                    auto load = [&](uint8_t *to, const CUtensorMap *map, uint64_t *bar, int j) {
+                        for (int d = 0; d < D / 64; ++d)
+                            tma_load_3d(to + d * kKeys * 128, map, bar, d * 64, it.head, it.s.k0 + j * kKeys);
+                    };
+                    /* K at ring place p: free once K at p - kStages has been used */
+                    auto k_free = [&](int p) { return wait(k_empty + p % C::kStages, (p / C::kStages + 1) & 1); };
+                    if (k_free(place)) {
+                        mbar_expect_tx(q_full, 2 * (D / 64) * g.group * g.tok * 128 + C::kTileBytes);
+                        for (int i = 0; i < 2; ++i)
+                            for (int d = 0; d < D / 64; ++d)
+                                tma_load_3d(sq + i * C::kTileBytes + d * kRows * 128, &maps.q, q_full, d * 64,
+                                            it.head * g.group, it.t0 + i * g.tok);
+                        load(sk + place % C::kStages * C::kTileBytes, &maps.k, q_full, it.first);
+                        ++queries;
+                        for (int c = 0; c < total; ++c, ++place) {
+                            const int st = place % C::kStages;
+                            const bool next = c + 1 < total;
+                            if (!wait(v_empty + st, (place / C::kStages + 1) & 1) || (next && !k_free(place + 1)))
+                                break;
+                            mbar_expect_tx(kv_full + st, (next ? 2 : 1) * C::kTileBytes);
+                            load(sv + st * C::kTileBytes, &maps.v, kv_full + st, it.first + c);
+                            if (next)
+                                load(sk + (place + 1) % C::kStages * C::kTileBytes, &maps.k, kv_full + st, it.first + c + 1);
+                        }
+                    }
+                }
             }
-            if (!alive) { /* let the copies already started land before the CTA exits */
-                mbar_wait_bounded(q_full, 0, &g_attn_error);
-                for (int c = max(0, issued - C::kStages); c < issued; ++c)
-                    mbar_wait_bounded(full + c % C::kStages, (c / C::kStages) & 1, &g_attn_error);
-            }
+            ++items;
+            alive = __shfl_sync(0xFFFFFFFFu, alive, 0);
+            if (!more || !alive)
+                break;
+        }
+        if (lane == 0 && !alive) { /* let the copies already started land before the CTA exits */
+            if (queries)
+                mbar_wait_bounded(q_full, (queries - 1) & 1, &g_attn_error);
+            for (int p = max(0, place - C::kStages); p < place; ++p)
+                mbar_wait_bounded(kv_full + p % C::kStages, (p / C::kStages) & 1, &g_attn_error);
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
         /* ---- UMMA */
-        if (lane == 0 && first < stop) {
+        if (lane == 0) {
             constexpr uint32_t kQk = idesc_of(kKeys, false), kPv = idesc_of(D, true);
             auto scores = [&](int i, int st) { /* S_i = Q_i K^T */
 #pragma unroll
@@ -507,38 +529,61 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             /* operands of 16 keys: P_i in TMEM, V in shared memory */
             auto p_at = [&](int i, int k) { return tmem + C::kS + 128 * i + (k / 2) * 32 + (k % 2) * 8; };
             auto v_at = [&](int st, int k) { return desc_outer(saddr(sv) + st * C::kTileBytes + k * 16 * 128); };
-            const int total = stop - first;
-            if (wait(q_full, 0)) {
+            int place = 0, queries = 0;
+            uint32_t done = 0; /* bit i: parity of the tiles of keys that query tile i is through */
+            for (int items = 0; wait(item_full + (items & 1), (items / 2) & 1); ++items) {
+                const bool more = s_more[items & 1];
+                const int first = s_item[items & 1].first;
+                const int n0 = s_item[items & 1].last0 - first, n1 = s_item[items & 1].last1 - first;
+                mbar_arrive(item_empty + (items & 1));
+                if (!more)
+                    break;
+                const int total = max(n0, n1);
+                if (total == 0)
+                    continue;
+                if (!wait(q_full, queries & 1))
+                    break;
+                ++queries;
                 tc_after();
                 for (int i = 0; i < 2; ++i)
-                    if (first < last_of(i))
-                        scores(i, 0);
-                umma_commit(k_done);
-            }
-            for (int c = 0; c < total && alive; ++c) {
-                const int st = c % C::kStages, nst = (c + 1) % C::kStages;
-                wait(full + st, (c / C::kStages) & 1);
-                for (int i = 0; i < 2 && alive; ++i) {
-                    if (first + c >= last_of(i) || !wait(p_full + i, c & 1))
-                        continue;
-                    tc_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        umma_ts(tmem + C::kO + D * i, p_at(i, k), v_at(st, k), kPv, c > 0 || k > 0);
-                    if (*reinterpret_cast<const volatile uint32_t *>(s_low[i])) {
+                    if ((i ? n1 : n0) > 0)
+                        scores(i, place % C::kStages);
+                umma_commit(k_empty + place % C::kStages);
+                if (total == 1)
+                    umma_commit(q_empty);
+                for (int c = 0; c < total && alive; ++c, ++place) {
+                    const int st = place % C::kStages, nst = (place + 1) % C::kStages;
+                    wait(kv_full + st, (place / C::kStages) & 1);
+                    for (int i = 0; i < 2 && alive; ++i) {
+                        const int n = i ? n1 : n0;
+                        if (c >= n || !wait(p_full + i, (done >> i) & 1u))
+                            continue;
+                        done ^= 1u << i;
+                        tc_after();
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
+                            umma_ts(tmem + C::kO + D * i, p_at(i, k), v_at(st, k), kPv, c > 0 || k > 0);
+                        if (*reinterpret_cast<const volatile uint32_t *>(s_low[i])) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
+                        }
+                        umma_commit(o_done + i);
+                        if (c + 1 < n)
+                            scores(i, nst);
                     }
-                    umma_commit(o_done + i);
-                    if (first + c + 1 < last_of(i))
-                        scores(i, nst);
+                    if (!alive)
+                        break;
+                    if (c + 1 < total)
+                        umma_commit(k_empty + nst);
+                    if (c + 2 == total)
+                        umma_commit(q_empty);
+                    umma_commit(v_empty + st);
                 }
-                if (alive)
-                    umma_commit(empty + st);
             }
             /* the last commit has arrived before this CTA's memory can go */
-            wait(empty + (total - 1) % C::kStages, ((total - 1) / C::kStages) & 1);
+            if (place > 0)
+                wait(v_empty + (place - 1) % C::kStages, ((place - 1) / C::kStages) & 1);
         }
         __syncwarp();
     } else {
@@ -546,172 +591,185 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         const int i = warp >> 2, wl = warp & 3, r = wl * 32 + lane;
         const uint32_t lanes = (uint32_t)(wl * 32) << 16;
         const uint32_t ts = tmem + C::kS + 128 * i + lanes, to = tmem + C::kO + D * i + lanes;
-        /* Few registers live through this loop: 128 hold scores, and a spilled one would come
-         * back from L2 (the tiles leave next to no L1). */
-        int seen; /* keys this row sees; 0 where it is no query's */
-        {
-            const int t = t0 + i * g.tok + r / g.group;
-            seen = r < g.group * g.tok && t < s.q1 ? seen_of(g, s, t) : 0;
-        }
-        /* tiles of keys from `plain` on have a place that some row does not see */
-        const int plain = t0 + i * g.tok < s.q1 ? seen_of(g, s, t0 + i * g.tok) / kKeys - first : 0;
         const float scale2 = g.a.scale * kLog2e;
-        float m = -INFINITY, l = 0.f; /* of the row; of this thread's keys */
-        const int done = last_of(i) - first;
-#pragma unroll 1
-        for (int c = 0; c < done; ++c) {
-            warp_wait(s_full + i, c & 1);
-            tc_after();
-            const bool masked = c >= plain;
-            uint32_t x[kKeys];
-#pragma unroll
-            for (int q = 0; q < kKeys; q += 32)
-                tmem_ld32(ts + q, x + q);
-            if (masked) { /* V's odd values would reach rows that do not see them */
-                warp_wait(full + c % C::kStages, (c / C::kStages) & 1);
-                const uint4 *v = reinterpret_cast<const uint4 *>(sv + (c % C::kStages) * C::kTileBytes);
-                uint32_t any = 0;
-#pragma unroll 4
-                for (int e = r; e < C::kTileBytes / 16; e += kRows) {
-                    const uint4 w = v[e];
-                    any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
-                }
-                if (any)
-                    s_bad[i] = 1;
-            }
-#pragma unroll
-            for (int q = 0; q < kKeys; q += 32)
-                tmem_ld_wait(x + q);
-            if (masked) {
-                const int lim = seen - (first + c) * kKeys;
-#pragma unroll
-                for (int e = 0; e < kKeys; ++e)
-                    x[e] = e < lim ? x[e] : 0xFF800000u;
-            }
-            float top = max_nan(x[0], x[1]), other = max_nan(x[2], x[3]);
-#pragma unroll
-            for (int e = 4; e < kKeys; e += 4) {
-                top = max_nan(top, max_nan(x[e], x[e + 1]));
-                other = max_nan(other, max_nan(x[e + 2], x[e + 3]));
-            }
-            /* rows that are no query's (of whatever lies there) take no part in what the warps decide */
-            top = seen > 0 ? max_nan(top, other) * scale2 : -INFINITY;
-            if (__any_sync(0xFFFFFFFFu, !(top <= m + kLazy))) { /* NaN too */
-                /* a NaN or an infinite score: every weight of the row is NaN from here on */
-                const float nm = top < INFINITY ? fmaxf(m, top) : __int_as_float(0x7FFFFFFF);
-                const float f = m == -INFINITY && nm == nm ? 0.f : ex2(m - nm);
-                m = m == m ? nm : m, l *= f;
-                if (c > 0) { /* O of the tiles before, once they are in */
-                    warp_wait(o_done + i, (c - 1) & 1);
-                    tc_after();
-#pragma unroll 1
-                    for (int q = 0; q < D; q += 8) {
-                        uint32_t o[8];
-                        tmem_ld8(to + q, o);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st8(to + q, o);
-                    }
-                    tmem_st_wait();
-                }
-            }
-            const float less = m == -INFINITY ? 0.f : -m;
-            const bool low = __any_sync(0xFFFFFFFFu, ex2(top + less) * kHeavy > l);
-            if (lane == 0)
-                s_low[i][wl] = low;
-            const uint64_t sc = pack2f(scale2, scale2), ls = pack2f(less, less);
-            uint64_t sum = 0;
-#pragma unroll
-            for (int q = 0; q < kKeys / 32; ++q) {
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    uint32_t *v = x + 32 * q + 2 * e;
-                    float a, b;
-                    unpack2f(fma2(pack2f(__uint_as_float(v[0]), __uint_as_float(v[1])), sc, ls), a, b);
-                    a = ex2(a), b = ex2(b);
-                    sum = add2(sum, pack2f(a, b));
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                    p[e] = *reinterpret_cast<const uint32_t *>(&h);
-                    v[0] = __float_as_uint(a), v[1] = __float_as_uint(b);
-                }
-                tmem_st16(ts + 32 * q, p);
-                /* what the rounding dropped; zeros where no row of the warp needs it, since
-                 * another warp's rows may, and one product serves them all */
-                if (low) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float a = __uint_as_float(x[32 * q + 2 * e]) - __uint_as_float(p[e] << 16);
-                        const float b = __uint_as_float(x[32 * q + 2 * e + 1]) - __uint_as_float(p[e] & 0xFFFF0000u);
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                        p[e] = *reinterpret_cast<const uint32_t *>(&h);
-                    }
-                    tmem_st16(ts + 32 * q + 16, p);
-                } else {
-                    tmem_zero16(ts + 32 * q + 16);
-                }
-            }
-            tmem_st_wait();
-            tc_before();
+        uint32_t turns = 0; /* tiles of keys gone through, of all items */
+        int place0 = 0;     /* ring place of the item's first */
+        for (int items = 0;; ++items) {
+            warp_wait(item_full + (items & 1), (items / 2) & 1);
+            if (!alive || !s_more[items & 1])
+                break;
+            const Item it = s_item[items & 1];
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(p_full + i);
-            float a, b;
-            unpack2f(sum, a, b);
-            l += a + b;
-        }
-        some_sync(1 + i, 128); /* the tile's warps: what they found in V */
-        const int tile0 = t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
-        const bool live = r < g.group * g.tok && t < s.q1;
-        if (done > 0) {
-            warp_wait(o_done + i, (done - 1) & 1);
-            tc_after();
-        }
-        const bool bad = s_bad[i] != 0;
-        if (it.cuts > 1) {
-            float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
-            float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
+                mbar_arrive(item_empty + (items & 1));
+            const Span s = it.s;
+            const int done = (i ? it.last1 : it.last0) - it.first;
+            /* Few registers live through this loop: 128 hold scores, and a spilled one would come
+             * back from L2 (the tiles leave next to no L1). */
+            int seen; /* keys this row sees, from the item's first on; 0 or less where it is no query's */
+            {
+                const int t = it.t0 + i * g.tok + r / g.group;
+                seen = (r < g.group * g.tok && t < s.q1 ? seen_of(g, s, t) : 0) - it.first * kKeys;
+            }
+            /* tiles of keys from `plain` on have a place that some row does not see */
+            const int plain = it.t0 + i * g.tok < s.q1 ? seen_of(g, s, it.t0 + i * g.tok) / kKeys - it.first : 0;
+            float m = -INFINITY, l = 0.f; /* of the row */
+            bool odd = false;
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-                uint32_t o[32] = {};
-                if (done > 0) {
-                    tmem_ld32(to + 32 * q, o);
-                    tmem_ld_wait(o);
+            for (int c = 0; c < done; ++c, ++turns) {
+                warp_wait(s_full + i, turns & 1);
+                tc_after();
+                const bool masked = c >= plain;
+                uint32_t x[kKeys];
+#pragma unroll
+                for (int q = 0; q < kKeys; q += 32)
+                    tmem_ld32(ts + q, x + q);
+                if (masked) { /* V's odd values would reach rows that do not see them */
+                    const int p = place0 + c;
+                    warp_wait(kv_full + p % C::kStages, (p / C::kStages) & 1);
+                    const uint4 *v = reinterpret_cast<const uint4 *>(sv + p % C::kStages * C::kTileBytes);
+                    uint32_t any = 0;
+#pragma unroll 4
+                    for (int e = r; e < C::kTileBytes / 16; e += kRows) {
+                        const uint4 w = v[e];
+                        any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
+                    }
+                    odd |= any != 0;
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
-            ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
-            if (r == 0)
-                reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
-        } else if (!bad) {
-            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-                uint32_t o[32] = {};
-                if (done > 0) {
-                    tmem_ld32(to + 32 * q, o);
-                    tmem_ld_wait(o);
-                }
-                float v[32];
+                for (int q = 0; q < kKeys; q += 32)
+                    tmem_ld_wait(x + q);
+                if (masked) {
+                    const int lim = seen - c * kKeys;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
-                if (live)
-                    store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
+                    for (int e = 0; e < kKeys; ++e)
+                        x[e] = e < lim ? x[e] : 0xFF800000u;
+                }
+                float top = max_nan(x[0], x[1]), other = max_nan(x[2], x[3]);
+#pragma unroll
+                for (int e = 4; e < kKeys; e += 4) {
+                    top = max_nan(top, max_nan(x[e], x[e + 1]));
+                    other = max_nan(other, max_nan(x[e + 2], x[e + 3]));
+                }
+                /* rows that are no query's (of whatever lies there) take no part in what the warps decide */
+                top = seen > 0 ? max_nan(top, other) * scale2 : -INFINITY;
+                if (__any_sync(0xFFFFFFFFu, !(top <= m + kLazy))) { /* NaN too */
+                    /* a NaN or an infinite score: every weight of the row is NaN from here on */
+                    const float nm = top < INFINITY ? fmaxf(m, top) : __int_as_float(0x7FFFFFFF);
+                    const float f = m == -INFINITY && nm == nm ? 0.f : ex2(m - nm);
+                    m = m == m ? nm : m, l *= f;
+                    if (c > 0) { /* O of the tiles before, once they are in */
+                        warp_wait(o_done + i, (turns + 1) & 1);
+                        tc_after();
+#pragma unroll 1
+                        for (int q = 0; q < D; q += 8) {
+                            uint32_t o[8];
+                            tmem_ld8(to + q, o);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st8(to + q, o);
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                const float less = m == -INFINITY ? 0.f : -m;
+                const bool low = __any_sync(0xFFFFFFFFu, ex2(top + less) * kHeavy > l);
+                if (lane == 0)
+                    s_low[i][wl] = low;
+                const uint64_t sc = pack2f(scale2, scale2), ls = pack2f(less, less);
+                uint64_t sum = 0;
+#pragma unroll
+                for (int q = 0; q < kKeys / 32; ++q) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint32_t *v = x + 32 * q + 2 * e;
+                        float a, b;
+                        unpack2f(fma2(pack2f(__uint_as_float(v[0]), __uint_as_float(v[1])), sc, ls), a, b);
+                        a = ex2(a), b = ex2(b);
+                        sum = add2(sum, pack2f(a, b));
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                        p[e] = *reinterpret_cast<const uint32_t *>(&h);
+                        v[0] = __float_as_uint(a), v[1] = __float_as_uint(b);
+                    }
+                    tmem_st16(ts + 32 * q, p);
+                    /* what the rounding dropped; zeros where no row of the warp needs it, since
+                     * another warp's rows may, and one product serves them all */
+                    if (low) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float a = __uint_as_float(x[32 * q + 2 * e]) - __uint_as_float(p[e] << 16);
+                            const float b = __uint_as_float(x[32 * q + 2 * e + 1]) - __uint_as_float(p[e] & 0xFFFF0000u);
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                            p[e] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                        tmem_st16(ts + 32 * q + 16, p);
+                    } else {
+                        tmem_zero16(ts + 32 * q + 16);
+                    }
+                }
+                tmem_st_wait();
+                tc_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(p_full + i);
+                float a, b;
+                unpack2f(sum, a, b);
+                l += a + b;
             }
-            if (live && g.a.lse)
-                g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-        } else {
-            for (int k = wl; k < g.group * g.tok; k += 4) {
-                const int tk = tile0 + k / g.group;
-                if (tk < s.q1)
-                    plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
+            place0 += max(it.last0, it.last1) - it.first;
+            const bool bad = any_of_tile(i, odd);
+            const int tile0 = it.t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
+            const bool live = r < g.group * g.tok && t < s.q1;
+            if (done > 0) {
+                warp_wait(o_done + i, (turns + 1) & 1);
+                tc_after();
             }
+            if (it.cuts > 1) {
+                float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
+                float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
+#pragma unroll 1
+                for (int q = 0; q < D / 32; ++q) {
+                    uint32_t o[32] = {};
+                    if (done > 0) {
+                        tmem_ld32(to + 32 * q, o);
+                        tmem_ld_wait(o);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+                ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
+                if (r == 0)
+                    reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
+            } else if (!bad) {
+                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll 1
+                for (int q = 0; q < D / 32; ++q) {
+                    uint32_t o[32] = {};
+                    if (done > 0) {
+                        tmem_ld32(to + 32 * q, o);
+                        tmem_ld_wait(o);
+                    }
+                    float v[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+                    if (live)
+                        store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
+                }
+                if (live && g.a.lse)
+                    g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+            } else {
+                for (int k = wl; k < g.group * g.tok; k += 4) {
+                    const int tk = tile0 + k / g.group;
+                    if (tk < s.q1)
+                        plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
+                }
+            }
+            tc_before(); /* O is read: the next item's products may write it once this warp's weights are in */
         }
-        tc_before();
     }
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -823,9 +881,9 @@ int tc_launch(const GlintAttnPrompt &a, cudaStream_t st)
         return kLaunch;
     /* every sequence may end in a block of its own */
     const int64_t items = ((int64_t)a.q_tokens / (2 * g.tok) + a.seqs) * a.kv_heads;
-    const int64_t grid = std::max(items, (int64_t)(g.split ? g.sms : 0));
-    if (grid > INT32_MAX)
+    if (items > INT32_MAX / 2)
         return kUnsupported;
+    const int64_t grid = g.split ? g.sms : std::min(items, (int64_t)g.sms);
     attn_kernel<D><<<(unsigned)grid, kThreads, Cfg<D>::kSmem, st>>>(g, maps);
     if (cudaGetLastError() != cudaSuccess)
         return kLaunch;
