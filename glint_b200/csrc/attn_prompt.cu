@@ -280,19 +280,27 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
 }
 
 /* The blocks (two tiles of one sequence) of all sequences in one row, each with every kv
- * head; the last blocks of a sequence see the most keys and go first.  Where there are
- * at most half as many as SMs, the keys of each are cut into parts of kCut tiles or more
- * (a part costs its block's rows in f32, written and read: 130 KB each way). */
+ * head, those that see the most keys first, so that the CTAs, which take them in turn,
+ * end together (12 prompts of 1 to 2011 tokens in their own order: 133 us).  A block's
+ * cost is its level: its number in the sequence, plus the blocks of keys before it.
+ * Where there are at most half as many items as SMs, the keys of each are cut into parts
+ * of kCut tiles or more (a part costs its block's rows in f32, written and read: 130 KB
+ * each way). */
 constexpr int kCut = 4;
+constexpr int kSeqsHeld = 1024; /* sequences whose blocks and levels a CTA keeps in shared memory */
+struct Seq {
+    int blocks, level; /* level of the first block; of every block where all keys are seen */
+};
 struct Item {
     Span s;
     int block, head, cut, cuts, slot;
     int t0, first, last0, last1; /* first token; query tile i goes through the tiles of keys [first, lasti) */
 };
-__device__ __forceinline__ int blocks_of(const Args &g, int seq)
+__device__ __forceinline__ Seq seq_of(const Args &g, int seq)
 {
-    const int n = bound(g.a.cu_q, seq + 1, g.a.q_tokens) - bound(g.a.cu_q, seq, g.a.q_tokens);
-    return max(0, (n + 2 * g.tok - 1) / (2 * g.tok));
+    const int n = max(0, bound(g.a.cu_q, seq + 1, g.a.q_tokens) - bound(g.a.cu_q, seq, g.a.q_tokens));
+    const int keys = max(0, bound(g.a.cu_k, seq + 1, g.a.k_tokens) - bound(g.a.cu_k, seq, g.a.k_tokens));
+    return Seq{(n + 2 * g.tok - 1) / (2 * g.tok), (g.a.causal ? max(0, keys - n) : keys) / (2 * g.tok)};
 }
 __device__ __forceinline__ int seen_of(const Args &g, const Span &s, int t);
 /* tiles of keys that an item's two query tiles see */
@@ -305,47 +313,70 @@ __device__ __forceinline__ void tiles_of(const Args &g, const Item &it, int (&n)
         n[i] = end > t0 + i * g.tok ? (seen_of(g, it.s, end - 1) + kKeys - 1) / kKeys : 0;
     }
 }
-/* the whole warp; false past the last item */
-__device__ __forceinline__ bool item_of(const Args &g, int index, Item &it)
+/* item `index` (or, with `whole`, the first part of the index-th item before its keys are
+ * cut), by the whole warp; false past the last one.  held: the first kSeqsHeld sequences' seq_of */
+__device__ __forceinline__ bool item_of(const Args &g, const Seq *held, int index, bool whole, Item &it)
 {
     const int lane = threadIdx.x & 31;
-    int64_t blocks = 0;
-    for (int b = lane; b < g.a.seqs; b += 32)
-        blocks += blocks_of(g, b);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-        blocks += __shfl_xor_sync(0xFFFFFFFFu, blocks, off);
-    const int64_t items = blocks * g.a.kv_heads;
+    auto seq = [&](int b) { return b >= g.a.seqs ? Seq{0, 0} : b < kSeqsHeld ? held[b] : seq_of(g, b); };
+    /* of a sequence's blocks, those of this level or above */
+    auto above = [&](Seq q, int level) {
+        return g.a.causal ? min(q.blocks, max(0, q.blocks + q.level - level)) : q.level >= level ? q.blocks : 0;
+    };
+    int blocks = 0, top = 0;
+    for (int b = lane; b < g.a.seqs; b += 32) {
+        const Seq q = seq(b);
+        blocks += q.blocks, top = max(top, q.blocks + q.level);
+    }
+    blocks = __reduce_add_sync(0xFFFFFFFFu, blocks), top = __reduce_max_sync(0xFFFFFFFFu, top);
+    const int64_t items = (int64_t)blocks * g.a.kv_heads;
     const int cuts = g.split && items > 0 ? (int)max((int64_t)1, g.sms / items) : 1;
-    if (index >= items * cuts)
+    if (whole ? index >= items : index >= items * cuts)
         return false;
+    index *= whole ? cuts : 1;
     it.slot = index, it.cut = index % cuts, it.cuts = cuts;
-    const int rest = index / cuts;
-    it.head = rest % g.a.kv_heads;
-    const int64_t want = blocks - 1 - rest / g.a.kv_heads;
-    int64_t before = 0;
+    const int rest = index / cuts, want = rest / g.a.kv_heads;
+    it.head = rest - want * g.a.kv_heads;
+    /* the level it is in: the highest with more than `want` blocks at or above it */
+    int lo = 0, hi = top;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        int n = 0;
+        for (int b = lane; b < g.a.seqs; b += 32)
+            n += above(seq(b), mid);
+        if (__reduce_add_sync(0xFFFFFFFFu, n) > want)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    int n = 0;
+    for (int b = lane; b < g.a.seqs; b += 32)
+        n += above(seq(b), lo + 1);
+    int left = want - __reduce_add_sync(0xFFFFFFFFu, n); /* its number among the blocks of this level */
     for (int b0 = 0; b0 < g.a.seqs; b0 += 32) {
-        const int n = b0 + lane < g.a.seqs ? blocks_of(g, b0 + lane) : 0;
-        int64_t sum = n;
+        const Seq q = seq(b0 + lane);
+        const int here = above(q, lo) - above(q, lo + 1);
+        int sum = here;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int64_t o = __shfl_up_sync(0xFFFFFFFFu, sum, off);
+            const int o = __shfl_up_sync(0xFFFFFFFFu, sum, off);
             if (lane >= off)
                 sum += o;
         }
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > want);
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, sum > left);
         if (past) {
-            const int l = __ffs(past) - 1, seq = b0 + l;
-            it.block = (int)(want - (before + __shfl_sync(0xFFFFFFFFu, sum - n, l)));
-            it.s.q0 = bound(g.a.cu_q, seq, g.a.q_tokens), it.s.q1 = bound(g.a.cu_q, seq + 1, g.a.q_tokens);
-            it.s.k0 = bound(g.a.cu_k, seq, g.a.k_tokens);
-            it.s.k1 = max(it.s.k0, bound(g.a.cu_k, seq + 1, g.a.k_tokens));
+            const int l = __ffs(past) - 1, b = b0 + l;
+            const int first = __shfl_sync(0xFFFFFFFFu, sum - here, l), level = __shfl_sync(0xFFFFFFFFu, q.level, l);
+            it.block = g.a.causal ? lo - level : left - first;
+            it.s.q0 = bound(g.a.cu_q, b, g.a.q_tokens), it.s.q1 = bound(g.a.cu_q, b + 1, g.a.q_tokens);
+            it.s.k0 = bound(g.a.cu_k, b, g.a.k_tokens);
+            it.s.k1 = max(it.s.k0, bound(g.a.cu_k, b + 1, g.a.k_tokens));
             int tiles[2];
             tiles_of(g, it, tiles);
             it.cuts = min(cuts, max(1, max(tiles[0], tiles[1]) / kCut));
             return true;
         }
-        before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+        left -= __shfl_sync(0xFFFFFFFFu, sum, 31);
     }
     return false;
 }
@@ -418,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __shared__ uint32_t tmem_slot;
     __shared__ Item s_item[2];
     __shared__ int s_more[2];
+    __shared__ Seq s_seqs[kSeqsHeld];
     __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: the low half of P is not all zero */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -439,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
+    asm volatile("griddepcontrol.launch_dependents;");
     bool alive = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (alive)
@@ -452,12 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 
     if (warp == kLoadWarp) {
         /* ---- items and loads */
+        for (int b = lane; b < min(kSeqsHeld, g.a.seqs); b += 32)
+            s_seqs[b] = seq_of(g, b);
+        __syncwarp();
         int place = 0, items = 0, queries = 0; /* ring place; items published; of them with tiles */
         for (int round = 0;; ++round) {
             /* every other round in reverse: the items fall in cost, and the CTAs take turns at the dear end */
             Item it;
             const int index = round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-            const bool more = item_of(g, index, it);
+            const bool more = item_of(g, s_seqs, index, false, it);
             if (more && it.cut >= it.cuts)
                 continue;
             if (lane == 0) {
@@ -778,24 +814,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     }
 }
 
+constexpr int kJoinRows = 32;
 /* Joins the parts of blocks whose keys were cut: a warp a row. */
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args g)
 {
+    __shared__ Seq s_seqs[kSeqsHeld];
+    __shared__ Item s_item;
+    __shared__ int s_ok;
     const int lane = threadIdx.x & 31;
-    Item it;
-    /* a block for each part of 32 of its rows; the item's first part does the work */
-    if (!item_of(g, blockIdx.x, it) || it.cut != 0 || it.cuts == 1)
+    for (int b = threadIdx.x; b < min(kSeqsHeld, g.a.seqs); b += 256)
+        s_seqs[b] = seq_of(g, b);
+    __syncthreads();
+    /* blockIdx.x: an item; blockIdx.y: kJoinRows of its rows */
+    if (threadIdx.x < 32) {
+        Item first;
+        const bool ok = item_of(g, s_seqs, blockIdx.x, true, first);
+        if (lane == 0)
+            s_item = first, s_ok = ok && first.cuts > 1;
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory"); /* the parts are the kernel's before */
+    if (!s_ok)
         return;
+    const Item it = s_item;
     const float *ml = g.part + (int64_t)g.sms * kSlotRows * D;
     const int *bads = reinterpret_cast<const int *>(ml + (int64_t)2 * g.sms * kSlotRows);
-    for (int k = 0; k < 4; ++k) {
-        const int row = blockIdx.y * 32 + (threadIdx.x >> 5) * 4 + k, i = row / kRows, r = row % kRows;
+    for (int k = 0; k < kJoinRows / 8; ++k) {
+        const int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * (kJoinRows / 8) + k, i = row / kRows, r = row % kRows;
         const int t = it.s.q0 + it.block * 2 * g.tok + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
         if (r >= g.group * g.tok || t >= it.s.q1)
             continue;
         float m = -INFINITY, l = 0.f;
         int bad = 0;
+#pragma unroll 4
         for (int c = 0; c < it.cuts; ++c) {
             m = fmaxf(m, ml[(int64_t)(it.slot + c) * kSlotRows + row]);
             bad |= bads[2 * (it.slot + c) + i];
@@ -805,6 +857,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
             continue;
         }
         float o[D / 32] = {};
+#pragma unroll 4
         for (int c = 0; c < it.cuts; ++c) {
             const int64_t at = (int64_t)(it.slot + c) * kSlotRows + row;
             const float mc = ml[at], f = mc == -INFINITY ? 0.f : ex2(mc - m);
@@ -888,9 +941,17 @@ int tc_launch(const GlintAttnPrompt &a, cudaStream_t st)
     if (cudaGetLastError() != cudaSuccess)
         return kLaunch;
     if (g.split) {
-        attn_join_kernel<D><<<dim3((unsigned)g.sms, kSlotRows / 32), 256, 0, st>>>(g);
-        if (cudaGetLastError() != cudaSuccess)
+        /* launched beside the other; it waits for that one's end itself */
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3((unsigned)std::min(items, (int64_t)g.sms / 2), kSlotRows / kJoinRows);
+        cfg.blockDim = dim3(256), cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, attn_join_kernel<D>, g) != cudaSuccess) {
+            cudaGetLastError();
             return kLaunch;
+        }
     }
     return kOk;
 }
