@@ -286,7 +286,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
  * Where there are at most half as many items as SMs, the keys of each are cut into parts
  * of kCut tiles or more (a part costs its block's rows in f32, written and read: 130 KB
  * each way). */
-constexpr int kCut = 4;
+constexpr int kCut = 4, kMostCuts = 32; /* a warp's lanes join them */
 constexpr int kSeqsHeld = 1024; /* sequences whose blocks and levels a CTA keeps in shared memory */
 struct Seq {
     int blocks, level; /* level of the first block; of every block where all keys are seen */
@@ -330,7 +330,7 @@ __device__ __forceinline__ bool item_of(const Args &g, const Seq *held, int inde
     }
     blocks = __reduce_add_sync(0xFFFFFFFFu, blocks), top = __reduce_max_sync(0xFFFFFFFFu, top);
     const int64_t items = (int64_t)blocks * g.a.kv_heads;
-    const int cuts = g.split && items > 0 ? (int)max((int64_t)1, g.sms / items) : 1;
+    const int cuts = g.split && items > 0 ? (int)min((int64_t)kMostCuts, max((int64_t)1, g.sms / items)) : 1;
     if (whole ? index >= items : index >= items * cuts)
         return false;
     index *= whole ? cuts : 1;
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     }
 }
 
-constexpr int kJoinRows = 32;
+constexpr int kJoinRows = 32; /* divides a tile's 128 */
 /* Joins the parts of blocks whose keys were cut: a warp a row. */
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args g)
@@ -830,6 +830,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     if (threadIdx.x < 32) {
         Item first;
         const bool ok = item_of(g, s_seqs, blockIdx.x, true, first);
+        first.t0 = first.s.q0 + first.block * 2 * g.tok;
         if (lane == 0)
             s_item = first, s_ok = ok && first.cuts > 1;
     }
@@ -840,38 +841,57 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     const Item it = s_item;
     const float *ml = g.part + (int64_t)g.sms * kSlotRows * D;
     const int *bads = reinterpret_cast<const int *>(ml + (int64_t)2 * g.sms * kSlotRows);
-    for (int k = 0; k < kJoinRows / 8; ++k) {
-        const int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * (kJoinRows / 8) + k, i = row / kRows, r = row % kRows;
-        const int t = it.s.q0 + it.block * 2 * g.tok + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
+    /* lane c: part c's maximum and sum, for all the warp's rows at once; then the rows themselves */
+    constexpr int R = kJoinRows / 8;
+    const int row0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * R, i = row0 / kRows;
+    float m[R], l[R];
+    const bool part = lane < it.cuts;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int64_t at = (int64_t)(it.slot + lane) * kSlotRows + row0 + k;
+        m[k] = part ? ml[at] : -INFINITY, l[k] = part ? ml[(int64_t)g.sms * kSlotRows + at] : 0.f;
+    }
+    const bool bad = __any_sync(0xFFFFFFFFu, part && bads[2 * (it.slot + lane) + i]);
+    float f[R], o[R][D / 32] = {};
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        float top = m[k];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1)
+            top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+        f[k] = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
+        l[k] = warp_sum(f[k] * l[k]);
+        m[k] = top;
+    }
+    if (!bad) {
+#pragma unroll 2
+        for (int c = 0; c < it.cuts; ++c) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float *p = g.part + ((int64_t)(it.slot + c) * kSlotRows + row0 + k) * D + lane;
+                const float fc = __shfl_sync(0xFFFFFFFFu, f[k], c);
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e)
+                    o[k][e] = fmaf(fc, p[32 * e], o[k][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int r = row0 + k - i * kRows;
+        const int t = it.t0 + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
         if (r >= g.group * g.tok || t >= it.s.q1)
             continue;
-        float m = -INFINITY, l = 0.f;
-        int bad = 0;
-#pragma unroll 4
-        for (int c = 0; c < it.cuts; ++c) {
-            m = fmaxf(m, ml[(int64_t)(it.slot + c) * kSlotRows + row]);
-            bad |= bads[2 * (it.slot + c) + i];
-        }
         if (bad) {
             plain_row<D>(g.a, it.s, t, hq, lane);
             continue;
         }
-        float o[D / 32] = {};
-#pragma unroll 4
-        for (int c = 0; c < it.cuts; ++c) {
-            const int64_t at = (int64_t)(it.slot + c) * kSlotRows + row;
-            const float mc = ml[at], f = mc == -INFINITY ? 0.f : ex2(mc - m);
-            l = fmaf(f, ml[(int64_t)g.sms * kSlotRows + at], l);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
-                o[e] = fmaf(f, g.part[at * D + lane + 32 * e], o[e]);
-        }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const float inv = l[k] > 0.f ? 1.f / l[k] : (l[k] == 0.f ? 0.f : l[k]);
 #pragma unroll
         for (int e = 0; e < D / 32; ++e)
-            g.a.o[t * g.a.o_tok + hq * g.a.o_head + lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
+            g.a.o[t * g.a.o_tok + hq * g.a.o_head + lane + 32 * e] = __float2bfloat16_rn(o[k][e] * inv);
         if (lane == 0 && g.a.lse)
-            g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+            g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l[k] == 0.f ? -INFINITY : (m[k] + log2f(l[k])) * kLn2;
     }
 }
 
