@@ -14,12 +14,13 @@ stream ordered and may be captured in CUDA graphs.  Tensors live on the current 
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+import struct
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
 
-from .device import _check, _stream, lib
+from .device import _check, lib
 
 BLOCK = 64
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
@@ -77,9 +78,66 @@ def _lib() -> ctypes.CDLL:
     return L
 
 
-def _on(stream):
-    """Outputs are allocated for the stream that writes them."""
-    return nullcontext() if stream is None else torch.cuda.stream(stream)
+class _Calls:
+    """The entry points taking their structs as packed bytes (a third of the time that
+    filling a ctypes.Structure takes), looked up once."""
+
+    def __init__(self):
+        L = _lib()
+        cp = ctypes.c_char_p
+
+        def get(name, *args, res=_i32):
+            return ctypes.CFUNCTYPE(res, *args)((name, L))
+        self.prompt = get("glint_attn_prompt_stream", cp, _vp)
+        self.append = get("glint_kv4_append_stream", cp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp)
+        self.read = get("glint_kv4_read_stream", cp, _vp, _i32, _vp, _vp, _vp)
+        self.attn = get("glint_kv4_attn_stream", cp, cp, _vp)
+        self.evict = get("glint_kv4_evict_stream", cp, cp, _vp)
+        self.prompt_work = get("glint_attn_prompt_work_bytes", cp, res=_i64)
+        self.attn_work = get("glint_kv4_attn_work_bytes", cp, cp, res=_i64)
+
+
+_calls: Optional[_Calls] = None
+
+
+def _c() -> _Calls:
+    global _calls
+    if _calls is None:
+        _calls = _Calls()
+    return _calls
+
+
+# the layouts of the structs above, pointers and strides in 64 bits
+_pack_prompt = struct.Struct("8P8q7if").pack
+_pack_cache = struct.Struct("4P4i").pack
+_pack_attn = struct.Struct("8P4q4if4x").pack
+_pack_evict = struct.Struct("9Pq4i").pack
+
+
+@lru_cache(maxsize=256)
+def _prompt_work(q_tokens: int, k_tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return max(0, _c().prompt_work(_pack_prompt(*[0] * 16, 1, q_tokens, k_tokens, heads, kv_heads, head_dim, 1, 1.0)))
+
+
+@lru_cache(maxsize=256)
+def _attn_work(kv_heads: int, page_size: int, head_dim: int, seqs: int, rows: int, heads: int, max_pages: int,
+               weights: bool) -> int:
+    cache = _pack_cache(16, 16, 16, 16, 1, kv_heads, page_size, head_dim)  # sizes are all that counts here
+    return max(0, _c().attn_work(cache, _pack_attn(*[0] * 6, 1 if weights else 0, 0, *[0] * 4, seqs, rows, heads,
+                                                   max_pages, 1.0)))
+
+
+def _raw(like: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> int:
+    """The stream's handle; torch.cuda.current_stream() itself takes 5 us of a 15 us call."""
+    return torch._C._cuda_getCurrentRawStream(like.get_device()) if stream is None else stream.cuda_stream
+
+
+def _empty(like: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
+    """Memory for the stream that writes it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[int], ...], dense: bool = True):
@@ -87,13 +145,16 @@ def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[
     otherwise its last dimension contiguous."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.dim() != len(shape) or any(w is not None and s != w for s, w in zip(t.shape, shape)):
-        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
-    if dense and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    if not dense and t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.shape != shape:
+        if None not in shape or len(t.shape) != len(shape) or \
+                any(w is not None and s != w for s, w in zip(t.shape, shape)):
+            raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if dense:
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    elif t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
@@ -126,27 +187,25 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
         if Tk != T:
             raise ValueError("cu_k may be left out only where k has q's tokens")
         cu_k = cu_q
-    _want(cu_k, "cu_k", torch.int32, (cu_q.shape[0],))
+    else:
+        _want(cu_k, "cu_k", torch.int32, cu_q.shape)
     if cu_q.shape[0] < 1:
         raise ValueError("cu_q must have one entry more than there are sequences")
-    with _on(stream):
-        if out is None:
-            out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-        if lse is None:
-            lse = torch.empty((H, T), dtype=torch.float32, device=q.device)
-    _want(out, "out", torch.bfloat16, (T, H, D), dense=False)
-    _want(lse, "lse", torch.float32, (H, T))
-    a = _Prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
-                cu_k.data_ptr(), None, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                out.stride(0), out.stride(1), cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0,
-                D ** -0.5 if scale is None else scale)
-    L = _lib()
-    n = L.glint_attn_prompt_work_bytes(a)
-    if n > 0:
-        with _on(stream):
-            work = torch.empty(n, dtype=torch.uint8, device=q.device)
-        a.work = work.data_ptr()
-    _check(L.glint_attn_prompt_stream(a, _stream(stream)), "glint_attn_prompt_stream")
+    if out is None:
+        out = _empty(q, (T, H, D), torch.bfloat16, stream)
+    else:
+        _want(out, "out", torch.bfloat16, (T, H, D), dense=False)
+    if lse is None:
+        lse = _empty(q, (H, T), torch.float32, stream)
+    else:
+        _want(lse, "lse", torch.float32, (H, T))
+    n = _prompt_work(T, Tk, H, Hk, D)
+    work = _empty(q, (n,), torch.uint8, stream) if n else None
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    a = _pack_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
+                     cu_k.data_ptr(), work.data_ptr() if n else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                     cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0, D ** -0.5 if scale is None else scale)
+    _check(_c().prompt(a, _raw(q, stream)), "glint_attn_prompt_stream")
     return out, lse
 
 
@@ -173,8 +232,8 @@ class KV4Cache:
             raise ValueError("the cache's tensors must be 16-byte aligned")
         self.k_code, self.k_meta, self.v_code, self.v_meta = k_code, k_meta, v_code, v_meta
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, 2 * half
-        self._c = _Cache(k_code.data_ptr(), k_meta.data_ptr(), v_code.data_ptr(), v_meta.data_ptr(), pages, kv_heads,
-                         page_size, 2 * half)
+        self._c = _pack_cache(k_code.data_ptr(), k_meta.data_ptr(), v_code.data_ptr(), v_meta.data_ptr(), pages,
+                              kv_heads, page_size, 2 * half)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "KV4Cache":
@@ -192,11 +251,11 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     """k, v [tokens, kv_heads, head_dim] BF16 (any strides, last dimension contiguous), quantised
     into slots[t] = page * page_size + place in the page (int32; negative: skipped)."""
     _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
-    _want(v, "v", torch.bfloat16, tuple(k.shape), dense=False)
-    _want(slots, "slots", torch.int32, (k.shape[0],))
-    _check(_lib().glint_kv4_append_stream(cache._c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
-                                          v.stride(0), v.stride(1), slots.data_ptr(), k.shape[0], _stream(stream)),
-           "glint_kv4_append_stream")
+    _want(v, "v", torch.bfloat16, k.shape, dense=False)
+    _want(slots, "slots", torch.int32, k.shape[:1])
+    ks, vs = k.stride(), v.stride()
+    _check(_c().append(cache._c, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), k.shape[0],
+                       _raw(k, stream)), "glint_kv4_append_stream")
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
@@ -205,15 +264,16 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor]
     the cache), for example as attn_prompt's keys of an earlier part of a prompt."""
     _want(slots, "slots", torch.int32, (None,))
     shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
-    with _on(stream):
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-        if v_out is None:
-            v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-    _want(k_out, "k_out", torch.bfloat16, shape)
-    _want(v_out, "v_out", torch.bfloat16, shape)
-    _check(_lib().glint_kv4_read_stream(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
-                                        _stream(stream)), "glint_kv4_read_stream")
+    if k_out is None:
+        k_out = _empty(slots, shape, torch.bfloat16, stream)
+    else:
+        _want(k_out, "k_out", torch.bfloat16, shape)
+    if v_out is None:
+        v_out = _empty(slots, shape, torch.bfloat16, stream)
+    else:
+        _want(v_out, "v_out", torch.bfloat16, shape)
+    _check(_c().read(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(), _raw(slots, stream)),
+           "glint_kv4_read_stream")
     return k_out, v_out
 
 
@@ -247,21 +307,22 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
             _want(weight, "weight", torch.float32, (B, cache.kv_heads, wide))
     elif weight is not None:
         raise ValueError("weight needs weight_out")
-    L = _lib()
-    a = _Attn(q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(),
-              None if weight is None else weight.data_ptr(), None if weight_out is None else weight_out.data_ptr(),
-              None, q.stride(0), q.stride(1), q.stride(2), wide, B, R, H, table.shape[1],
-              D ** -0.5 if scale is None else scale)
-    with _on(stream):
-        if out is None:
-            out = torch.empty((B, R, H, D), dtype=torch.bfloat16, device=q.device)
-        if lse is None:
-            lse = torch.empty((B, H, R), dtype=torch.float32, device=q.device)
-        work = torch.empty(max(0, L.glint_kv4_attn_work_bytes(cache._c, a)), dtype=torch.uint8, device=q.device)
-    _want(out, "out", torch.bfloat16, (B, R, H, D))
-    _want(lse, "lse", torch.float32, (B, H, R))
-    a.o, a.lse, a.work = out.data_ptr(), lse.data_ptr(), work.data_ptr()
-    _check(L.glint_kv4_attn_stream(cache._c, a, _stream(stream)), "glint_kv4_attn_stream")
+    if out is None:
+        out = _empty(q, (B, R, H, D), torch.bfloat16, stream)
+    else:
+        _want(out, "out", torch.bfloat16, (B, R, H, D))
+    if lse is None:
+        lse = _empty(q, (B, H, R), torch.float32, stream)
+    else:
+        _want(lse, "lse", torch.float32, (B, H, R))
+    work = _empty(q, (_attn_work(cache.kv_heads, cache.page_size, D, B, R, H, table.shape[1],
+                                 weight_out is not None),), torch.uint8, stream)
+    qs = q.stride()
+    a = _pack_attn(q.data_ptr(), out.data_ptr(), lse.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                   0 if weight is None else weight.data_ptr(), 0 if weight_out is None else weight_out.data_ptr(),
+                   work.data_ptr(), qs[0], qs[1], qs[2], wide, B, R, H, table.shape[1],
+                   D ** -0.5 if scale is None else scale)
+    _check(_c().attn(cache._c, a, _raw(q, stream)), "glint_kv4_attn_stream")
     return out, lse
 
 
@@ -289,14 +350,13 @@ def kv4_evict(cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, weight: 
         raise ValueError("budget must be 1 or more and recent between 0 and budget")
     if P < 1 or P * cache.page_size > min(wide, 524288):
         raise ValueError(f"table has room for {P * cache.page_size} slots: weight must cover them, 524288 at most")
-    with _on(stream):
-        kept = torch.empty((B, cache.kv_heads, budget), dtype=torch.int32, device=table.device)
-        new_lens = torch.empty((B,), dtype=torch.int32, device=table.device)
-    _want(weight_out, "weight_out", torch.float32, tuple(weight.shape))
-    _want(pos_out, "pos_out", torch.int32, tuple(pos.shape))
+    kept = _empty(table, (B, cache.kv_heads, budget), torch.int32, stream)
+    new_lens = _empty(table, (B,), torch.int32, stream)
+    _want(weight_out, "weight_out", torch.float32, weight.shape)
+    _want(pos_out, "pos_out", torch.int32, pos.shape)
     if weight_out.data_ptr() == weight.data_ptr() or pos_out.data_ptr() == pos.data_ptr():
         raise ValueError("weight_out and pos_out must not be weight and pos")
-    e = _Evict(table.data_ptr(), lens.data_ptr(), weight.data_ptr(), pos.data_ptr(), seen.data_ptr(), kept.data_ptr(),
+    e = _pack_evict(table.data_ptr(), lens.data_ptr(), weight.data_ptr(), pos.data_ptr(), seen.data_ptr(), kept.data_ptr(),
                new_lens.data_ptr(), weight_out.data_ptr(), pos_out.data_ptr(), wide, B, P, budget, recent)
-    _check(_lib().glint_kv4_evict_stream(cache._c, e, _stream(stream)), "glint_kv4_evict_stream")
+    _check(_c().evict(cache._c, e, _raw(table, stream)), "glint_kv4_evict_stream")
     return kept, new_lens
