@@ -19,72 +19,113 @@ namespace {
 
 constexpr int kThreads = 256;
 
-/* 8 values of a row, BF16 -> f32; ALIGNED: one 16-byte load */
+/* 8 values of a row as BF16 pairs; ALIGNED: one 16-byte load */
 template <bool ALIGNED>
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8])
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, uint32_t (&x)[4])
 {
     if constexpr (ALIGNED) {
         const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = __bfloat162float(p[i]);
+        for (int i = 0; i < 4; ++i)
+            x[i] = (uint32_t)__bfloat16_as_ushort(p[2 * i]) | ((uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16);
     }
 }
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b)
+{
+    asm("min.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return a;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b)
+{
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return a;
+}
+__device__ __forceinline__ uint64_t pack2f(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2f(uint64_t v, float &lo, float &hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
 /* One block's 8 values of this lane -> 8 nibbles; (step, lo) of the block the same in
  * all 8 lanes of the aligned group. */
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t &meta)
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t &meta)
 {
-    float lo = x[0], hi = x[0];
-    /* any NaN or infinity: its exponent is all ones, and stays so in this difference */
-    float odd = 0.f;
+    uint32_t mn = min2(min2(x[0], x[1]), min2(x[2], x[3])), mx = max2(max2(x[0], x[1]), max2(x[2], x[3]));
+    /* any NaN or infinity: an exponent of ones carries into bit 15 or 31 */
+    uint32_t odd = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
-        odd += x[i] - x[i];
-    }
+    for (int i = 0; i < 4; ++i)
+        odd |= (x[i] & 0x7F807F80u) + 0x00800080u;
+    odd &= 0x80008000u;
 #pragma unroll
     for (int off = 4; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, off));
-        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, off);
+        mn = min2(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, off));
+        mx = max2(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
     }
+    const uint32_t group = 0xFFu << (lane_id() & 24u);
+    const bool any = (__ballot_sync(0xFFFFFFFFu, odd != 0) & group) != 0;
+    const float lo = fminf(low_half(mn), high_half(mn)), hi = fmaxf(low_half(mx), high_half(mx));
     const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f));
     const float step = __bfloat162float(sb);
-    if (odd != 0.f || step - step != 0.f) { /* not finite: the block reads as NaN */
+    if (any || step - step != 0.f) { /* not finite: the block reads as NaN */
         meta = 0x7FC00000u;
         return 0u;
     }
     /* lo is one of the BF16 inputs, so its upper half is all of it */
     meta = (__float_as_uint(lo) & 0xFFFF0000u) | (uint32_t)__bfloat16_as_ushort(sb);
-    /* (x - lo) * (1 / step) is within 2^-18 of the quotient (at most 15.06 here), so it
-     * rounds to the same integer unless it lies that near to a half; those, and steps so
-     * small or large that 1 / step is not a normal number, divide */
-    uint32_t w = 0;
-    bool near = !(step > 1e-30f && step < 1e30f);
-    const float inv = __frcp_rn(step);
+    /* The quotient d / step, d = x - lo, as f32 division gives it, from the correctly rounded
+     * reciprocal y: q = d y, then q + (d - q step) y (P. Markstein, IBM J. Res. Dev. 34(1),
+     * 1990); exact where y and step are normal numbers with room to spare.  Adding 1.5 * 2^23
+     * rounds it to an integer, ties to even.  It is at most 15.06, so the code needs no
+     * clamp.  Four codes at a time are added up as c0 + 16 c1 + 256 c2 + 4096 c3, exact in f32. */
+    float c[8];
+    if (step > 1e-30f && step < 1e30f) {
+        const float y = __frcp_rn(step);
+        const uint64_t y2 = pack2f(y, y), lo2 = pack2f(-lo, -lo), less = pack2f(-step, -step);
+        const uint64_t magic = pack2f(12582912.f, 12582912.f), minus = pack2f(-12582912.f, -12582912.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float t = (x[i] - lo) * inv, u = t + 12582912.f; /* 1.5 * 2^23: rounds to an integer in u's low bits */
-        near |= !(fabsf(t - (u - 12582912.f)) < 0.49999f);
-        w |= (__float_as_uint(u) & 15u) << (4 * i);
-    }
-    if (near) {
-        w = 0;
-        if (step > 0.f) {
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t d = add2(pack2f(low_half(x[i]), high_half(x[i])), lo2), q = mul2(d, y2);
+            unpack2f(add2(add2(fma2(fma2(q, less, d), y2, q), magic), minus), c[2 * i], c[2 * i + 1]);
+        }
+    } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, step)), 0.f), 15.f);
-                w |= (uint32_t)c << (4 * i);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const float v = i & 1 ? high_half(x[i / 2]) : low_half(x[i / 2]);
+            c[i] = step > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(v - lo, step)), 0.f), 15.f) : 0.f;
         }
     }
-    return w;
+    const float a = fmaf(4096.f, c[3], fmaf(256.f, c[2], fmaf(16.f, c[1], c[0])));
+    const float b = fmaf(4096.f, c[7], fmaf(256.f, c[6], fmaf(16.f, c[5], c[4])));
+    /* 2^23 + a has a in its low bits */
+    return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
 }
 
 struct AppendArgs {
@@ -114,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const AppendArgs a
     const int ch = (int)(i % CH);
     const uint32_t row = live ? i / CH : 0, t = row / (uint32_t)a.c.kv_heads;
     const int h = (int)(row - t * (uint32_t)a.c.kv_heads);
-    float x[8] = {}, y[8] = {};
+    uint32_t x[4] = {}, y[4] = {};
     const int slot = live ? a.slots[t] : -1;
     if (live) {
         load8<ALIGNED>(a.k + t * a.k_tok + h * a.k_head + ch * 8, x);
