@@ -181,6 +181,14 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
                  "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
                  : "memory");
 }
+/* the same, added to D, but to none of the lanes whose bit in `off` is set */
+__device__ __forceinline__ void umma_ts_lanes(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, const uint32_t (&off)[4])
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %5, %6, %7}, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+                 : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar))
@@ -205,10 +213,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
-}
-__device__ __forceinline__ void tmem_zero16(uint32_t taddr)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr), "r"(0u) : "memory");
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r)
 {
@@ -418,7 +422,12 @@ __device__ __forceinline__ float max_nan(float a, float b)
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(uint32_t a, uint32_t b) { return max_nan(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float max3_nan(float a, uint32_t b, uint32_t c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return r;
+}
 /* whether any of a tile's 128 softmax threads has `p` */
 __device__ __forceinline__ bool any_of_tile(int i, bool p)
 {
@@ -450,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __shared__ Item s_item[2];
     __shared__ int s_more[2];
     __shared__ Seq s_seqs[kSeqsHeld];
-    __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: the low half of P is not all zero */
+    __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: P has a low half */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == kLoadWarp && lane == 0) {
@@ -553,18 +562,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         /* ---- UMMA */
         if (lane == 0) {
             constexpr uint32_t kQk = idesc_of(kKeys, false), kPv = idesc_of(D, true);
+            /* descriptors of one operand differ in their addresses alone (in 16 bytes, with no
+             * carry out of the field), so each is a base and a constant: the thread has about
+             * 60 clocks to make the next product's */
+            const uint64_t dq = desc_inner(saddr(sq)), dk = desc_inner(saddr(sk)), dv = desc_outer(saddr(sv));
             auto scores = [&](int i, int st) { /* S_i = Q_i K^T */
+                const uint64_t a = dq + (uint32_t)(i * (C::kTileBytes >> 4)), b = dk + (uint32_t)(st * (C::kTileBytes >> 4));
+                const uint32_t to = tmem + C::kS + 128 * i;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    const uint32_t off = (d / 4) * kKeys * 128 + (d % 4) * 32;
-                    umma_ss(tmem + C::kS + 128 * i, desc_inner(saddr(sq) + i * C::kTileBytes + off),
-                            desc_inner(saddr(sk) + st * C::kTileBytes + off), kQk, d > 0);
+                    const uint32_t off = ((d / 4) * kKeys * 128 + (d % 4) * 32) >> 4;
+                    umma_ss(to, a + off, b + off, kQk, d > 0);
                 }
                 umma_commit(s_full + i);
             };
-            /* operands of 16 keys: P_i in TMEM, V in shared memory */
-            auto p_at = [&](int i, int k) { return tmem + C::kS + 128 * i + (k / 2) * 32 + (k % 2) * 8; };
-            auto v_at = [&](int st, int k) { return desc_outer(saddr(sv) + st * C::kTileBytes + k * 16 * 128); };
             int place = 0, queries = 0;
             uint32_t done = 0; /* bit i: parity of the tiles of keys that query tile i is through */
             for (int items = 0; wait(item_full + (items & 1), (items / 2) & 1); ++items) {
@@ -596,13 +607,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                             continue;
                         done ^= 1u << i;
                         tc_after();
+                        /* 16 keys a product: P_i in TMEM, V in shared memory */
+                        const uint32_t to = tmem + C::kO + D * i, from = tmem + C::kS + 128 * i;
+                        const uint64_t v = dv + (uint32_t)(st * (C::kTileBytes >> 4));
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            umma_ts(tmem + C::kO + D * i, p_at(i, k), v_at(st, k), kPv, c > 0 || k > 0);
-                        if (*reinterpret_cast<const volatile uint32_t *>(s_low[i])) {
+                            umma_ts(to, from + (k / 2) * 32 + (k % 2) * 8, v + k * 128, kPv, c > 0 || k > 0);
+                        if (const uint32_t low = *reinterpret_cast<const volatile uint32_t *>(s_low[i])) {
+                            /* the warps without one have left scores in its place */
+                            const uint32_t off[4] = {low & 0xFFu ? 0u : ~0u, low & 0xFF00u ? 0u : ~0u,
+                                                     low & 0xFF0000u ? 0u : ~0u, low & 0xFF000000u ? 0u : ~0u};
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
-                                umma_ts(tmem + C::kO + D * i, p_at(i, k) + 16, v_at(st, k), kPv, true);
+                                umma_ts_lanes(to, from + (k / 2) * 32 + (k % 2) * 8 + 16, v + k * 128, kPv, off);
                         }
                         umma_commit(o_done + i);
                         if (c + 1 < n)
@@ -681,12 +698,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     for (int e = 0; e < kKeys; ++e)
                         x[e] = e < lim ? x[e] : 0xFF800000u;
                 }
-                float top = max_nan(x[0], x[1]), other = max_nan(x[2], x[3]);
+                float top = max3_nan(__uint_as_float(x[0]), x[1], x[2]), other = max3_nan(__uint_as_float(x[3]), x[4], x[5]);
 #pragma unroll
-                for (int e = 4; e < kKeys; e += 4) {
-                    top = max_nan(top, max_nan(x[e], x[e + 1]));
-                    other = max_nan(other, max_nan(x[e + 2], x[e + 3]));
+                for (int e = 6; e < kKeys - 2; e += 4) {
+                    top = max3_nan(top, x[e], x[e + 1]);
+                    other = max3_nan(other, x[e + 2], x[e + 3]);
                 }
+                top = max3_nan(top, x[kKeys - 2], x[kKeys - 1]);
                 /* rows that are no query's (of whatever lies there) take no part in what the warps decide */
                 top = seen > 0 ? max_nan(top, other) * scale2 : -INFINITY;
                 if (__any_sync(0xFFFFFFFFu, !(top <= m + kLazy))) { /* NaN too */
@@ -730,9 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         v[0] = __float_as_uint(a), v[1] = __float_as_uint(b);
                     }
                     tmem_st16(ts + 32 * q, p);
-                    /* what the rounding dropped; zeros where no row of the warp needs it, since
-                     * another warp's rows may, and one product serves them all */
-                    if (low) {
+                    if (low) { /* what the rounding dropped */
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float a = __uint_as_float(x[32 * q + 2 * e]) - __uint_as_float(p[e] << 16);
@@ -741,8 +757,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                             p[e] = *reinterpret_cast<const uint32_t *>(&h);
                         }
                         tmem_st16(ts + 32 * q + 16, p);
-                    } else {
-                        tmem_zero16(ts + 32 * q + 16);
                     }
                 }
                 tmem_st_wait();
