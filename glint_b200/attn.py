@@ -127,9 +127,16 @@ def _attn_work(kv_heads: int, page_size: int, head_dim: int, seqs: int, rows: in
                                                    max_pages, 1.0)))
 
 
-def _raw(like: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> int:
-    """The stream's handle; torch.cuda.current_stream() itself takes 5 us of a 15 us call."""
-    return torch._C._cuda_getCurrentRawStream(like.get_device()) if stream is None else stream.cuda_stream
+def _raw(like: torch.Tensor, stream: Optional[torch.cuda.Stream], *others) -> int:
+    """The stream's handle (torch.cuda.current_stream() itself takes 5 us of a 15 us call),
+    once all tensors are seen to live on the current device."""
+    dev = like.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"all tensors must be on one device, not on cuda:{dev} and {t.device}")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{dev}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
 def _empty(like: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
@@ -205,7 +212,7 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     a = _pack_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
                      cu_k.data_ptr(), work.data_ptr() if n else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                      cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0, D ** -0.5 if scale is None else scale)
-    _check(_c().prompt(a, _raw(q, stream)), "glint_attn_prompt_stream")
+    _check(_c().prompt(a, _raw(q, stream, k, v, cu_q, cu_k, out, lse)), "glint_attn_prompt_stream")
     return out, lse
 
 
@@ -230,6 +237,8 @@ class KV4Cache:
             _want(t, name, torch.bfloat16, (pages, kv_heads, page_size, half // 32, 2))
         if any(t.data_ptr() % 16 for t in (k_code, k_meta, v_code, v_meta)):
             raise ValueError("the cache's tensors must be 16-byte aligned")
+        if any(t.device != k_code.device for t in (k_meta, v_code, v_meta)):
+            raise ValueError("the cache's tensors must be on one device")
         self.k_code, self.k_meta, self.v_code, self.v_meta = k_code, k_meta, v_code, v_meta
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, 2 * half
         self._c = _pack_cache(k_code.data_ptr(), k_meta.data_ptr(), v_code.data_ptr(), v_meta.data_ptr(), pages,
@@ -255,7 +264,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     _want(slots, "slots", torch.int32, k.shape[:1])
     ks, vs = k.stride(), v.stride()
     _check(_c().append(cache._c, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), k.shape[0],
-                       _raw(k, stream)), "glint_kv4_append_stream")
+                       _raw(k, stream, v, slots, cache.k_code)), "glint_kv4_append_stream")
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
@@ -272,8 +281,8 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor]
         v_out = _empty(slots, shape, torch.bfloat16, stream)
     else:
         _want(v_out, "v_out", torch.bfloat16, shape)
-    _check(_c().read(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(), _raw(slots, stream)),
-           "glint_kv4_read_stream")
+    _check(_c().read(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
+                     _raw(slots, stream, k_out, v_out, cache.k_code)), "glint_kv4_read_stream")
     return k_out, v_out
 
 
@@ -322,7 +331,8 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
                    0 if weight is None else weight.data_ptr(), 0 if weight_out is None else weight_out.data_ptr(),
                    work.data_ptr(), qs[0], qs[1], qs[2], wide, B, R, H, table.shape[1],
                    D ** -0.5 if scale is None else scale)
-    _check(_c().attn(cache._c, a, _raw(q, stream)), "glint_kv4_attn_stream")
+    _check(_c().attn(cache._c, a, _raw(q, stream, cache.k_code, table, lens, weight, weight_out, out, lse)),
+           "glint_kv4_attn_stream")
     return out, lse
 
 
@@ -358,5 +368,6 @@ def kv4_evict(cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, weight: 
         raise ValueError("weight_out and pos_out must not be weight and pos")
     e = _pack_evict(table.data_ptr(), lens.data_ptr(), weight.data_ptr(), pos.data_ptr(), seen.data_ptr(), kept.data_ptr(),
                new_lens.data_ptr(), weight_out.data_ptr(), pos_out.data_ptr(), wide, B, P, budget, recent)
-    _check(_c().evict(cache._c, e, _raw(table, stream)), "glint_kv4_evict_stream")
+    _check(_c().evict(cache._c, e, _raw(table, stream, cache.k_code, lens, weight, pos, seen, weight_out, pos_out)),
+           "glint_kv4_evict_stream")
     return kept, new_lens

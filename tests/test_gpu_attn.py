@@ -190,6 +190,27 @@ def test_prompt_tokens_outside_sequences_are_not_written():
     assert bool((lse[:, :5] == 7).all()) and bool((lse[:, 33:] == 7).all())
 
 
+def test_prompt_past_32_bits():
+    """Rows of q, k, v and o more than 2^32 elements apart."""
+    g = gen(17)
+    step, T = 2 ** 26, 70
+    flat = torch.empty(step * T, dtype=torch.bfloat16, device="cuda")
+    y = flat.view(T, step)[:, :8 * 128].view(T, 8, 128)
+    y.copy_(randn(T, 8, 128, g=g))
+    out = flat.view(T, step)[:, 2048:2048 + 4 * 128].view(T, 4, 128)
+    A().attn_prompt(y[:, :4], y[:, 4:6], y[:, 6:], cu([T]), out=out)
+    want = prompt_reference(y[:, :4], y[:, 4:6], y[:, 6:], [T], [T], True, 128 ** -0.5)
+    within(out, want[0], want[1], "o")
+
+
+def test_prompt_many_sequences():
+    """More sequences than a block keeps the sizes of."""
+    g = gen(18)
+    lens = [1 + i % 5 for i in range(1500)] + [70]
+    T = sum(lens)
+    check_prompt(randn(T, 2, 64, g=g), randn(T, 1, 64, g=g), randn(T, 1, 64, g=g), lens, lens)
+
+
 def test_prompt_other_stream_and_graph():
     g = gen(5)
     q, k, v = randn(200, 8, 128, g=g), randn(200, 2, 128, g=g), randn(200, 2, 128, g=g)
@@ -520,6 +541,34 @@ def test_cache_attention_other_stream_and_graph():
         assert torch.equal(got, want) and torch.equal(w0, w2)
 
 
+def test_cache_past_32_bits():
+    """Pages whose bytes lie past 4 GiB of a cache's codes: append, read, attention, eviction."""
+    g = gen(16)
+    kv, dim, page, n = 8, 128, 64, 150
+    pages = (2 ** 32 + 2 ** 24) // (kv * page * dim // 2)
+    cache = A().KV4Cache.empty(pages, kv, dim, page)
+    table = torch.tensor([[pages - 1, 1, pages - 2]], dtype=torch.int32, device="cuda")
+    t = torch.arange(n, device="cuda")
+    slots = (table[0, t // page] * page + t % page).int()
+    k, v = randn(n, kv, dim, g=g), randn(n, kv, dim, g=g)
+    A().kv4_append(cache, k, v, slots)
+    for x, got in zip((k, v), A().kv4_read(cache, slots)):
+        assert torch.equal(bits(got), bits(values(*quantise(x)).bfloat16()))
+    kd, vd = (values(*quantise(x), dtype=torch.float64) for x in (k, v))
+    q = randn(1, 1, 16, dim, g=g)
+    o, lse = A().kv4_attn(q, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    want = attn_reference(q, [n], kd, vd, quantise(v)[1].double().repeat_interleave(64, -1), dim ** -0.5)
+    within(o, want[0], want[1], "o")
+    within(lse, want[2], want[3], "lse")
+    w = torch.arange(3 * page, device="cuda").float().expand(1, kv, -1).contiguous()
+    pos = torch.zeros_like(w, dtype=torch.int32)
+    one = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kept, _ = A().kv4_evict(cache, table, one, w, pos, one, 20, weight_out=torch.empty_like(w),
+                            pos_out=torch.empty_like(pos))
+    assert kept[0, 0].tolist() == list(range(130, 150))
+    assert torch.equal(bits(A().kv4_read(cache, slots[:20])[0]), bits(values(*quantise(k[130:])).bfloat16()))
+
+
 # ---- eviction ------------------------------------------------------------------------------
 
 def evict_reference(w, pos, seen, L, budget, recent):
@@ -615,6 +664,8 @@ def test_refusals():
                 dict(out=q.float()), dict(lse=torch.empty(4, 5, device="cuda")), dict(q=randn(4, 4, 96, g=g))):
         with pytest.raises(ValueError):
             attn.attn_prompt(**{**dict(q=q, k=k, v=k, cu_q=ends), **bad})
+    empty = attn.attn_prompt(q[:0], k[:0], k[:0], cu([]))
+    assert empty[0].shape == (0, 4, 128) and empty[1].shape == (4, 0)
     with pytest.raises(ValueError):
         attn.KV4Cache.empty(2, 2, 96)
     with pytest.raises(ValueError):
