@@ -314,8 +314,13 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int L = min(max(e.lens[b], 0), e.max_pages << a.page_log2), n = min(L, e.budget);
-    /* an equal stretch of the slots for each CTA, a multiple of kEvThreads (no more than a.stretch) */
-    const int stretch = max(1, (L + a.cluster * kEvThreads - 1) / (a.cluster * kEvThreads)) * kEvThreads;
+    /* as many CTAs as the length is worth, with an equal stretch of the slots each (a multiple
+     * of kEvThreads, no more than a.stretch); the others make room at once, and a cluster's
+     * barriers do not wait for them */
+    const int ctas = min(a.cluster, max(1, (L + kEvSlots * kEvThreads - 1) / (kEvSlots * kEvThreads)));
+    if (rank >= ctas)
+        return;
+    const int stretch = max(1, (L + ctas * kEvThreads - 1) / (ctas * kEvThreads)) * kEvThreads;
     const int begin = rank * stretch, end = min(L, begin + stretch); /* this CTA's; none where end <= begin */
     const int words = stretch / 32, per_warp = words / kEvWarps;
     uint32_t *bits = ev_smem;                                      /* kept, a bit a slot */
@@ -355,9 +360,13 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
             }
             cluster_barrier();
             if (tid < 256) {
-                int sum = 0;
-                for (int r = 0; r < a.cluster; ++r)
-                    sum += load_there(there(&hist[p & 1][tid], r));
+                int n[8], sum = 0;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    n[r] = r < ctas ? load_there(there(&hist[p & 1][tid], r)) : 0;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    sum += n[r];
                 tot[tid] = sum;
                 hist[(p + 1) & 1][tid] = 0; /* read by the others before the barrier above */
             }
@@ -379,8 +388,9 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
             prefix = s_prefix, need = s_need;
         }
         /* the last histogram counts, for its digit, the keys equal to the n-th */
-        for (int r = 0; r < rank; ++r)
-            eq_before += load_there(there(&hist[1][prefix & 255u], r));
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            eq_before += r < rank ? load_there(there(&hist[1][prefix & 255u], r)) : 0;
     }
     /* kept: above the n-th key, and of those equal to it the `need` lowest slots.  A warp
      * has per_warp words of 32 slots. */
@@ -424,11 +434,12 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     }
     cluster_barrier(); /* counts and the keys' memory, of every CTA */
     int free_base = 0, far_base = 0, moved = 0;
-    for (int r = 0; r < a.cluster; ++r) {
-        const int f = load_there(there(&s_free, r)), g = load_there(there(&s_far, r));
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int f = r < ctas ? load_there(there(&s_free, r)) : 0, g = r < ctas ? load_there(there(&s_far, r)) : 0;
         free_base += r < rank ? f : 0, far_base += r < rank ? g : 0, moved += f;
     }
-    const int part = max(1, (moved + a.cluster - 1) / a.cluster); /* entries of the list a CTA holds */
+    const int part = max(1, (moved + ctas - 1) / ctas); /* entries of the list a CTA holds */
     int *kept = e.kept + (int64_t)bh * e.budget;
 #pragma unroll 2
     for (int q = 0; q < per_warp; ++q) { /* the free slots of this CTA's into the list */
@@ -441,12 +452,12 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     }
     /* the kept ones below n, shared out evenly: most of them lie in the first CTAs */
 #pragma unroll 4
-    for (int t = rank * kEvThreads + tid; t < n; t += a.cluster * kEvThreads) {
+    for (int t = rank * kEvThreads + tid; t < n; t += ctas * kEvThreads) {
         const int r = t / stretch, at = t - r * stretch;
         if ((load_there(there(&bits[at / 32], r)) >> (at % 32)) & 1)
             kept[t] = t, e.weight_out[row + t] = w[t], e.pos_out[row + t] = pos[t];
     }
-    for (int i = n + rank * kEvThreads + tid; i < e.budget; i += a.cluster * kEvThreads)
+    for (int i = n + rank * kEvThreads + tid; i < e.budget; i += ctas * kEvThreads)
         kept[i] = -1;
     cluster_barrier();
     /* the kept slots from n on, a thread each: number j of this CTA's by two searches */
@@ -579,7 +590,8 @@ int glint_kv4_evict_stream(const GlintKv4Cache *c, const GlintKv4Evict *e, cudaS
     const int cap = e->max_pages * c->page_size;
     while (a.cluster < 8 && cap > kEvSlots * kEvThreads * a.cluster)
         a.cluster *= 2;
-    a.stretch = (cap + a.cluster * kEvThreads - 1) / (a.cluster * kEvThreads) * kEvThreads;
+    /* a CTA's memory: its share of the longest sequence, or what fewer CTAs have of a shorter one */
+    a.stretch = std::max((cap + a.cluster * kEvThreads - 1) / (a.cluster * kEvThreads), kEvSlots) * kEvThreads;
     if ((int64_t)e->seqs * c->kv_heads * a.cluster > INT32_MAX)
         return kBadArg;
     /* keys, or at least this CTA's part of the list: at most half of the slots are free ones below n */
