@@ -153,7 +153,7 @@ struct Args {
     int sms;
     bool vec;          /* o takes 16-byte stores */
     bool split;        /* there is a workspace for parts */
-    float *part;       /* [slot][256][D], then m, l [slot][256] each, then bad [slot] */
+    float *part;       /* [slot][2 tiles][D / 4][128 rows] of 4, then m, l [slot][256] each, then bad [slot][2] */
 };
 struct Maps {
     CUtensorMap q, k, v;
@@ -393,26 +393,6 @@ __device__ __forceinline__ int seen_of(const Args &g, const Span &s, int t)
 /* first tile of a cut, of n tiles */
 __device__ __forceinline__ int cut_begin(int n, int cut, int cuts) { return (int)((int64_t)n * cut / cuts); }
 
-/* D values of one row: 16-byte stores where o allows */
-template <int D>
-__device__ __forceinline__ void store_row32(const Args &g, __nv_bfloat16 *o, const float (&v)[32])
-{
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&p);
-    }
-    if (g.vec) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            reinterpret_cast<uint4 *>(o)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            o[i] = __float2bfloat16_rn(v[i]);
-    }
-}
 /* any NaN or infinity among two BF16 */
 __device__ __forceinline__ uint32_t odd2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
@@ -460,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __shared__ int s_more[2];
     __shared__ Seq s_seqs[kSeqsHeld];
     __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: P has a low half */
+    __shared__ uint4 s_stage[8][32 * 4]; /* per softmax warp: 32 rows of 32 BF16 */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == kLoadWarp && lane == 0) {
@@ -777,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 tc_after();
             }
             if (it.cuts > 1) {
-                float *part = g.part + ((int64_t)it.slot * kSlotRows + i * kRows + r) * D;
+                uint4 *part = reinterpret_cast<uint4 *>(g.part) + ((int64_t)it.slot * 2 + i) * (D / 4) * kRows + r;
                 float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
 #pragma unroll 1
                 for (int q = 0; q < D / 32; ++q) {
@@ -788,26 +769,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        reinterpret_cast<uint4 *>(part + 32 * q)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        part[(8 * q + e) * kRows] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
                 ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
                 if (r == 0)
                     reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
             } else if (!bad) {
                 const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+                /* 32 columns a time through shared memory: a thread's own row would be a line of its
+                 * own in every store, four threads a row make whole sectors (3.5 -> 2 us a block) */
+                uint4 *stage = s_stage[warp];
+                int64_t at[4]; /* of rows lane / 4 + 8 k, 16 bytes at lane % 4 */
+                uint32_t mine = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = wl * 32 + lane / 4 + 8 * k, tk = tile0 + row / g.group;
+                    mine |= row < g.group * g.tok && tk < s.q1 ? 1u << k : 0u;
+                    at[k] = tk * g.a.o_tok + (it.head * g.group + row % g.group) * g.a.o_head + lane % 4 * 8;
+                }
 #pragma unroll 1
                 for (int q = 0; q < D / 32; ++q) {
-                    uint32_t o[32] = {};
+                    uint32_t o[32] = {}, w[16];
                     if (done > 0) {
                         tmem_ld32(to + 32 * q, o);
                         tmem_ld_wait(o);
                     }
-                    float v[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        v[e] = done > 0 ? __uint_as_float(o[e]) * inv : 0.f;
-                    if (live)
-                        store_row32<D>(g, g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q, v);
+                    for (int e = 0; e < 16; ++e) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(done > 0 ? __uint_as_float(o[2 * e]) * inv : 0.f,
+                                                                       done > 0 ? __uint_as_float(o[2 * e + 1]) * inv : 0.f);
+                        w[e] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    if (g.vec) {
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            stage[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int row = lane / 4 + 8 * k;
+                            const uint4 v = stage[row * 4 + (lane % 4 ^ ((row >> 1) & 3))];
+                            if ((mine >> k) & 1u)
+                                *reinterpret_cast<uint4 *>(g.a.o + at[k] + 32 * q) = v;
+                        }
+                    } else if (live) {
+                        __nv_bfloat16 *out = g.a.o + t * g.a.o_tok + hq * g.a.o_head + 32 * q;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            out[2 * e] = __ushort_as_bfloat16((unsigned short)(w[e] & 0xFFFFu));
+                            out[2 * e + 1] = __ushort_as_bfloat16((unsigned short)(w[e] >> 16));
+                        }
+                    }
                 }
                 if (live && g.a.lse)
                     g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -829,19 +842,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 }
 
 constexpr int kJoinRows = 32; /* divides a tile's 128 */
-/* Joins the parts of blocks whose keys were cut: a warp a row. */
+/* Joins the parts of blocks whose keys were cut: 32 rows a block, a row a lane, an eighth of
+ * its columns a warp (the parts lie by row within four columns, so loads are whole lines). */
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args g)
 {
     __shared__ Seq s_seqs[kSeqsHeld];
     __shared__ Item s_item;
     __shared__ int s_ok;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int b = threadIdx.x; b < min(kSeqsHeld, g.a.seqs); b += 256)
         s_seqs[b] = seq_of(g, b);
     __syncthreads();
     /* blockIdx.x: an item; blockIdx.y: kJoinRows of its rows */
-    if (threadIdx.x < 32) {
+    if (warp == 0) {
         Item first;
         const bool ok = item_of(g, s_seqs, blockIdx.x, true, first);
         first.t0 = first.s.q0 + first.block * 2 * g.tok;
@@ -853,60 +867,57 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     if (!s_ok)
         return;
     const Item it = s_item;
-    const float *ml = g.part + (int64_t)g.sms * kSlotRows * D;
-    const int *bads = reinterpret_cast<const int *>(ml + (int64_t)2 * g.sms * kSlotRows);
-    /* lane c: part c's maximum and sum, for all the warp's rows at once; then the rows themselves */
-    constexpr int R = kJoinRows / 8;
-    const int row0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * R, i = row0 / kRows;
-    float m[R], l[R];
-    const bool part = lane < it.cuts;
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-        const int64_t at = (int64_t)(it.slot + lane) * kSlotRows + row0 + k;
-        m[k] = part ? ml[at] : -INFINITY, l[k] = part ? ml[(int64_t)g.sms * kSlotRows + at] : 0.f;
+    constexpr int C4 = D / 32; /* fours of columns a thread */
+    const int row0 = blockIdx.y * kJoinRows, i = row0 / kRows, r = row0 % kRows + lane;
+    const float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + row0 + lane;
+    const int *bads = reinterpret_cast<const int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2)) + 2 * it.slot + i;
+    const float4 *part = reinterpret_cast<const float4 *>(g.part) + (((int64_t)it.slot * 2 + i) * (D / 4) + warp * C4) * kRows + r;
+    const bool bad = __any_sync(0xFFFFFFFFu, lane < it.cuts && bads[2 * lane]);
+    if (bad) {
+        for (int k = warp; k < kJoinRows; k += 8) {
+            const int row = row0 % kRows + k, t = it.t0 + i * g.tok + row / g.group;
+            if (row < g.group * g.tok && t < it.s.q1)
+                plain_row<D>(g.a, it.s, t, it.head * g.group + row % g.group, lane);
+        }
+        return;
     }
-    const bool bad = __any_sync(0xFFFFFFFFu, part && bads[2 * (it.slot + lane) + i]);
-    float f[R], o[R][D / 32] = {};
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 8
+    for (int c = 0; c < it.cuts; ++c)
+        m = max_nan(m, ml[(int64_t)c * kSlotRows]);
+    float4 o[C4];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        float top = m[k];
+    for (int e = 0; e < C4; ++e)
+        o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < it.cuts; ++c) {
+        const float mc = ml[(int64_t)c * kSlotRows], f = mc == -INFINITY ? 0.f : ex2(mc - m);
+        l = fmaf(f, ml[((int64_t)g.sms + c) * kSlotRows], l);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1)
-            top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-        f[k] = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
-        l[k] = warp_sum(f[k] * l[k]);
-        m[k] = top;
-    }
-    if (!bad) {
-#pragma unroll 2
-        for (int c = 0; c < it.cuts; ++c) {
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-                const float *p = g.part + ((int64_t)(it.slot + c) * kSlotRows + row0 + k) * D + lane;
-                const float fc = __shfl_sync(0xFFFFFFFFu, f[k], c);
-#pragma unroll
-                for (int e = 0; e < D / 32; ++e)
-                    o[k][e] = fmaf(fc, p[32 * e], o[k][e]);
-            }
+        for (int e = 0; e < C4; ++e) {
+            const float4 v = part[((int64_t)c * 2 * (D / 4) + e) * kRows];
+            o[e].x = fmaf(f, v.x, o[e].x), o[e].y = fmaf(f, v.y, o[e].y);
+            o[e].z = fmaf(f, v.z, o[e].z), o[e].w = fmaf(f, v.w, o[e].w);
         }
     }
+    const int t = it.t0 + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
+    if (r >= g.group * g.tok || t >= it.s.q1)
+        return;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    __nv_bfloat16 *out = g.a.o + t * g.a.o_tok + hq * g.a.o_head + warp * C4 * 4;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        const int r = row0 + k - i * kRows;
-        const int t = it.t0 + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
-        if (r >= g.group * g.tok || t >= it.s.q1)
-            continue;
-        if (bad) {
-            plain_row<D>(g.a, it.s, t, hq, lane);
-            continue;
+    for (int e = 0; e < C4; ++e) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(o[e].x * inv, o[e].y * inv);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(o[e].z * inv, o[e].w * inv);
+        if (g.vec) {
+            *reinterpret_cast<uint2 *>(out + 4 * e) =
+                make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+        } else {
+            out[4 * e] = a.x, out[4 * e + 1] = a.y, out[4 * e + 2] = b.x, out[4 * e + 3] = b.y;
         }
-        const float inv = l[k] > 0.f ? 1.f / l[k] : (l[k] == 0.f ? 0.f : l[k]);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e)
-            g.a.o[t * g.a.o_tok + hq * g.a.o_head + lane + 32 * e] = __float2bfloat16_rn(o[k][e] * inv);
-        if (lane == 0 && g.a.lse)
-            g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l[k] == 0.f ? -INFINITY : (m[k] + log2f(l[k])) * kLn2;
     }
+    if (warp == 0 && g.a.lse)
+        g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 /* [tokens][heads][D] as (D, heads, tokens); boxes of 64 x heads x tokens */
