@@ -1108,6 +1108,38 @@ def bench_reference(args):
     print(json.dumps(line), flush=True)
 
 
+def profile_attention(case: str, g):
+    """(call, values) of one serving attention kernel: attention over a prompt of 8192
+    tokens (32 query, 8 kv heads of 128), over a 4-bit cache of 16 x 16384 slots (64
+    query, 8 kv heads of 128), the append of 16384 tokens, eviction of 16 x 32768 slots
+    down to 4096."""
+    import torch
+    from glint_b200 import attn as A
+    i32 = dict(dtype=torch.int32, device="cuda")
+    T, H, KV, Dh = (8192, 32, 8, 128) if case == "attn" else (16384, 64, 8, 128)
+    y = torch.randn((T, H + 2 * KV, Dh), generator=g, device="cuda").to(torch.bfloat16)
+    q, k, v = y[:, :H], y[:, H:H + KV], y[:, H + KV:]
+    if case == "attn":
+        ends = torch.tensor([0, T], **i32)
+        return (lambda: A.attn_prompt(q, k, v, ends)), T * (H + 2 * KV) * Dh
+    seqs, slots = 16, 32768 if case == "kv4evict" else 16384
+    cache = A.KV4Cache.empty(seqs * slots // 64, KV, Dh, 64)
+    table = torch.arange(seqs * slots // 64, **i32).view(seqs, -1)
+    for c in range(0, seqs * slots, T):
+        A.kv4_append(cache, k, v, torch.arange(c, c + T, **i32))
+    lens = torch.full((seqs,), slots, **i32)
+    if case == "kv4append":
+        at = torch.arange(T, **i32)
+        return (lambda: A.kv4_append(cache, k, v, at)), 2 * T * KV * Dh
+    if case == "kv4attn":
+        q1 = q[:seqs, None]
+        return (lambda: A.kv4_attn(q1, cache, table, lens)), 2 * seqs * slots * KV * Dh
+    w = torch.rand((seqs, KV, slots), generator=g, device="cuda")
+    pos = torch.arange(slots, **i32).expand(seqs, KV, -1).contiguous()
+    wo, po = torch.empty_like(w), torch.empty_like(pos)
+    return (lambda: A.kv4_evict(cache, table, lens, w, pos, lens, 4096, 256, weight_out=wo, pos_out=po)), w.numel()
+
+
 def profile_case(case: str, iters: int = 5):
     """A small, fixed workload of one kernel family for ncu captures (a few
     launches, a few hundred MB on the device, inputs larger than L2)."""
@@ -1181,6 +1213,8 @@ def profile_case(case: str, iters: int = 5):
             fn = lambda: D.gemv_km(x, hk, sk, N, out=y)  # noqa: E731
         else:
             fn = lambda: D.gemv_select(x, hk, pk_, sk, N, K // 10, out=y)  # noqa: E731
+    elif case in ("attn", "kv4attn", "kv4append", "kv4evict"):
+        fn, n = profile_attention(case, g)
     else:
         raise SystemExit(f"unknown case {case}")
     for _ in range(2):
@@ -1203,8 +1237,8 @@ def main():
     ap.add_argument("--impl", default="glint_b200", choices=["glint_b200", "reference"])
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--profile", default=None,
-                    help="run one small kernel case (encode|expand|gemv<M>|gemvt<M>|gemm<M>|gemmp<M>|km|kmstep|int8|int8d) "
-                         "for ncu")
+                    help="run one small kernel case (encode|expand|gemv<M>|gemvt<M>|gemm<M>|gemmp<M>|km|kmstep|int8|int8d|"
+                         "attn|kv4attn|kv4append|kv4evict) for ncu")
     args = ap.parse_args()
     if args.profile:
         profile_case(args.profile)

@@ -10,6 +10,8 @@ include/glint_htile.h, cuda/p7_abi.c).  Python front ends:
                          stream ordered), used by the tests and bench.py
   glint_b200.shard       multi-GPU placement: per-tensor LPT and column-parallel
                          linears
+  glint_b200.attn        attention between the q|k|v and o linears: packed prompts, the
+                         paged 4-bit key/value cache, attention over it, eviction
   glint_b200.pin         the pin tool (glint_pin.py's interface) as a GPU pipeline
   glint_b200.unpin       the unpin tool (glint_unpin.py's interface) on the GPU
 """

@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             } else if (!bad) {
                 const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
                 /* 32 columns a time through shared memory: a thread's own row would be a line of its
-                 * own in every store, four threads a row make whole sectors (3.5 -> 2 us a block) */
+                 * own in every store, four threads a row make whole sectors (12 prompts 114 -> 112 us) */
                 uint4 *stage = s_stage[warp];
                 int64_t at[4]; /* of rows lane / 4 + 8 k, 16 bytes at lane % 4 */
                 uint32_t mine = 0;
