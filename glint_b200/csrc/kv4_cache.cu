@@ -1,11 +1,11 @@
 /* The 4-bit key/value cache: append (quantise rows into their slots), read (slots back
  * to BF16) and eviction by accumulated attention weight.
  *
- * Append and read move each byte once: a thread takes 8 neighbouring values of a row
- * (16 bytes of BF16, 4 bytes of codes), the 8 threads of a 64-value block find its
- * minimum and maximum with three shuffles, and K and V go through one thread so that
- * two loads are in flight.  HBM-bound in principle: 2 * (2 D + D / 2 + D / 16) bytes a
- * token and head.
+ * Append and read move each byte once.  Append: a thread takes 16 neighbouring values of a
+ * row (32 bytes of BF16, 8 bytes of codes), the 4 threads of a 64-value block find its
+ * minimum and maximum with two shuffles, and K and V go through one thread so that four
+ * loads are in flight.  Read: 8 values a thread.  HBM's bound is 2 * (2 D + D / 2 + D / 16)
+ * bytes a token and head; append is bound by its instructions, about 20 a value.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -19,16 +19,19 @@ namespace {
 
 constexpr int kThreads = 256;
 
-/* 8 values of a row as BF16 pairs; ALIGNED: one 16-byte load */
+/* 16 values of a row as BF16 pairs; ALIGNED: two 16-byte loads */
 template <bool ALIGNED>
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, uint32_t (&x)[4])
+__device__ __forceinline__ void load16(const __nv_bfloat16 *p, uint32_t (&x)[8])
 {
     if constexpr (ALIGNED) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
-        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             x[i] = (uint32_t)__bfloat16_as_ushort(p[2 * i]) | ((uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16);
     }
 }
@@ -73,59 +76,68 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
-/* One block's 8 values of this lane -> 8 nibbles; (step, lo) of the block the same in
- * all 8 lanes of the aligned group. */
-__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t &meta)
+/* One block's 16 values of this lane -> 16 nibbles; (step, lo) of the block the same in
+ * all 4 lanes of the aligned group. */
+__device__ __forceinline__ uint2 quantise16(const uint32_t (&x)[8], uint32_t &meta)
 {
-    uint32_t mn = min2(min2(x[0], x[1]), min2(x[2], x[3])), mx = max2(max2(x[0], x[1]), max2(x[2], x[3]));
-    /* any NaN or infinity: an exponent of ones carries into bit 15 or 31 */
-    uint32_t odd = 0;
+    uint32_t mn = x[0], mx = x[0], odd = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        odd |= (x[i] & 0x7F807F80u) + 0x00800080u;
-    odd &= 0x80008000u;
+    for (int i = 0; i < 8; ++i) {
+        mn = min2(mn, x[i]), mx = max2(mx, x[i]);
+        odd |= (x[i] & 0x7F807F80u) + 0x00800080u; /* NaN, infinity: an exponent of ones carries into bit 15 or 31 */
+    }
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) {
+    for (int off = 2; off > 0; off >>= 1) {
         mn = min2(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, off));
         mx = max2(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
     }
-    const uint32_t group = 0xFFu << (lane_id() & 24u);
-    const bool any = (__ballot_sync(0xFFFFFFFFu, odd != 0) & group) != 0;
+    const bool any = (__ballot_sync(0xFFFFFFFFu, (odd & 0x80008000u) != 0) >> (lane_id() & 28u) & 15u) != 0;
     const float lo = fminf(low_half(mn), high_half(mn)), hi = fmaxf(low_half(mx), high_half(mx));
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f));
+    /* Quotients as f32 division gives them, from the correctly rounded reciprocal y of the
+     * divisor s: q = n y, then q + (n - q s) y (P. Markstein, IBM J. Res. Dev. 34(1), 1990);
+     * exact where y, s and n are normal numbers with room to spare. */
+    const float range = hi - lo;
+    float fifteenth;
+    if (range > 1e-28f && range < 1e30f) {
+        const float y = 1.f / 15.f, q = range * y;
+        fifteenth = fmaf(fmaf(-q, 15.f, range), y, q);
+    } else {
+        fifteenth = __fdiv_rn(range, 15.f);
+    }
+    const __nv_bfloat16 sb = __float2bfloat16_rn(fifteenth);
     const float step = __bfloat162float(sb);
     if (any || step - step != 0.f) { /* not finite: the block reads as NaN */
         meta = 0x7FC00000u;
-        return 0u;
+        return make_uint2(0u, 0u);
     }
     /* lo is one of the BF16 inputs, so its upper half is all of it */
     meta = (__float_as_uint(lo) & 0xFFFF0000u) | (uint32_t)__bfloat16_as_ushort(sb);
-    /* The quotient d / step, d = x - lo, as f32 division gives it, from the correctly rounded
-     * reciprocal y: q = d y, then q + (d - q step) y (P. Markstein, IBM J. Res. Dev. 34(1),
-     * 1990); exact where y and step are normal numbers with room to spare.  Adding 1.5 * 2^23
-     * rounds it to an integer, ties to even.  It is at most 15.06, so the code needs no
-     * clamp.  Four codes at a time are added up as c0 + 16 c1 + 256 c2 + 4096 c3, exact in f32. */
-    float c[8];
+    /* (x - lo) / step, at most 15.06, plus 1.5 * 2^23 is rounded to an integer, ties to even:
+     * no clamp.  Four codes at a time are added up as c0 + 16 c1 + 256 c2 + 4096 c3, exact in
+     * f32; plus 2^23 they stand in the low bits. */
+    float c[16];
     if (step > 1e-30f && step < 1e30f) {
         const float y = __frcp_rn(step);
         const uint64_t y2 = pack2f(y, y), lo2 = pack2f(-lo, -lo), less = pack2f(-step, -step);
         const uint64_t magic = pack2f(12582912.f, 12582912.f), minus = pack2f(-12582912.f, -12582912.f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const uint64_t d = add2(pack2f(low_half(x[i]), high_half(x[i])), lo2), q = mul2(d, y2);
             unpack2f(add2(add2(fma2(fma2(q, less, d), y2, q), magic), minus), c[2 * i], c[2 * i + 1]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
             const float v = i & 1 ? high_half(x[i / 2]) : low_half(x[i / 2]);
             c[i] = step > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(v - lo, step)), 0.f), 15.f) : 0.f;
         }
     }
-    const float a = fmaf(4096.f, c[3], fmaf(256.f, c[2], fmaf(16.f, c[1], c[0])));
-    const float b = fmaf(4096.f, c[7], fmaf(256.f, c[6], fmaf(16.f, c[5], c[4])));
-    /* 2^23 + a has a in its low bits */
-    return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
+    uint32_t four[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        four[i] = __float_as_uint(fmaf(4096.f, c[4 * i + 3], fmaf(256.f, c[4 * i + 2], fmaf(16.f, c[4 * i + 1], c[4 * i]))) +
+                                  8388608.f);
+    return make_uint2(__byte_perm(four[0], four[1], 0x5410), __byte_perm(four[2], four[3], 0x5410));
 }
 
 struct AppendArgs {
@@ -133,7 +145,7 @@ struct AppendArgs {
     const __nv_bfloat16 *k, *v;
     int64_t k_tok, k_head, v_tok, v_head;
     const int *slots;
-    uint32_t chunks; /* tokens * kv_heads * D / 8 */
+    uint32_t chunks; /* tokens * kv_heads * D / 16 */
     int page_log2;
 };
 /* 32-bit chunk numbers: longer calls go in slices of this many tokens */
@@ -149,30 +161,30 @@ inline int log2_of(int n)
 template <int D, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const AppendArgs a)
 {
-    constexpr int CH = D / 8; /* chunks a row: a power of two, so a block's 8 lanes stay in one row */
+    constexpr int CH = D / 16; /* chunks a row: a power of two, so a block's 4 lanes stay in one row */
     const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
     const bool live = i < a.chunks;
     const int ch = (int)(i % CH);
     const uint32_t row = live ? i / CH : 0, t = row / (uint32_t)a.c.kv_heads;
     const int h = (int)(row - t * (uint32_t)a.c.kv_heads);
-    uint32_t x[4] = {}, y[4] = {};
+    uint32_t x[8] = {}, y[8] = {};
     const int slot = live ? a.slots[t] : -1;
     if (live) {
-        load8<ALIGNED>(a.k + t * a.k_tok + h * a.k_head + ch * 8, x);
-        load8<ALIGNED>(a.v + t * a.v_tok + h * a.v_head + ch * 8, y);
+        load16<ALIGNED>(a.k + t * a.k_tok + h * a.k_head + ch * 16, x);
+        load16<ALIGNED>(a.v + t * a.v_tok + h * a.v_head + ch * 16, y);
     }
     uint32_t km, vm;
-    const uint32_t kw = quantise8(x, km), vw = quantise8(y, vm);
+    const uint2 kw = quantise16(x, km), vw = quantise16(y, vm);
     if (slot < 0 || slot >= a.c.pages * a.c.page_size)
         return;
     const int page = slot >> a.page_log2, r = slot & (a.c.page_size - 1);
     const int64_t at = (((int64_t)page * a.c.kv_heads + h) << a.page_log2) + r;
-    const int64_t byte = at * (D / 2) + kv4_unit<D>(ch / 8, r) + (ch % 8) * 4;
-    *reinterpret_cast<uint32_t *>(a.c.k_code + byte) = kw;
-    *reinterpret_cast<uint32_t *>(a.c.v_code + byte) = vw;
-    if (ch % 8 == 0) {
-        reinterpret_cast<uint32_t *>(a.c.k_meta)[at * (D / 64) + ch / 8] = km;
-        reinterpret_cast<uint32_t *>(a.c.v_meta)[at * (D / 64) + ch / 8] = vm;
+    const int64_t byte = at * (D / 2) + kv4_unit<D>(ch / 4, r) + (ch % 4) * 8;
+    *reinterpret_cast<uint2 *>(a.c.k_code + byte) = kw;
+    *reinterpret_cast<uint2 *>(a.c.v_code + byte) = vw;
+    if (ch % 4 == 0) {
+        reinterpret_cast<uint32_t *>(a.c.k_meta)[at * (D / 64) + ch / 4] = km;
+        reinterpret_cast<uint32_t *>(a.c.v_meta)[at * (D / 64) + ch / 4] = vm;
     }
 }
 
@@ -543,7 +555,7 @@ int glint_kv4_append_stream(const GlintKv4Cache *c, const glint_bf16_t *k, const
                                            : (al ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
     const int most = slice_tokens(*c);
     for (int t = 0; t < tokens; t += std::min(most, tokens - t)) {
-        const uint32_t n = (uint32_t)std::min(most, tokens - t) * c->kv_heads * (c->head_dim / 8);
+        const uint32_t n = (uint32_t)std::min(most, tokens - t) * c->kv_heads * (c->head_dim / 16);
         const AppendArgs a{*c, k + t * k_tok, v + t * v_tok, k_tok, k_head, v_tok, v_head, slots + t, n, log2_of(c->page_size)};
         kernel<<<(n + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
     }
