@@ -4,8 +4,12 @@
  * Append and read move each byte once.  Append: a thread takes 16 neighbouring values of a
  * row (32 bytes of BF16, 8 bytes of codes), the 4 threads of a 64-value block find its
  * minimum and maximum with two shuffles, and K and V go through one thread so that four
- * loads are in flight.  Read: 8 values a thread.  HBM's bound is 2 * (2 D + D / 2 + D / 16)
- * bytes a token and head; append is bound by its instructions, about 20 a value.
+ * loads are in flight.  Read: 8 values a thread, one 16-byte store each for K and V (16
+ * values and two stores: 22 us in place of 18).
+ *
+ * HBM's bound is 2 * (2 D + D / 2 + D / 16) bytes a token and head.  At 16383 tokens, 8
+ * heads of 128: append 21 us = 4.1 TB/s, bound by its instructions (8 values a thread:
+ * 28 us), read 18 us = 4.8 TB/s.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
