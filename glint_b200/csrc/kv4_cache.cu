@@ -242,8 +242,12 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache 
  * moved into the k-th of the list.  Sources lie at n and above, destinations below, so
  * the moves do not depend on one another.
  *
- * Bound: 8 bytes a slot and head read (weight and position), and the latency of nine
- * cluster barriers.
+ * Floor: 8 bytes a slot and head read (weight and position), 8 + D + D / 8 read and
+ * written a slot moved.  Bound: latency, of six cluster barriers and of what each waits
+ * for.  16 ragged sequences of up to 32768 slots to 4096, 8 heads of 128: 35 us, about 17 of
+ * them the four digits, 7 the lists, 11 the moves (a lane's 16 bytes of K and of V; with a
+ * slot a lane the moves took 18).  512 threads a CTA: 39 us there, 28 instead of 34 for two
+ * such sequences.  One of 1025 to 1024: 14 us.
  */
 constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32;
 constexpr int kEvSlots = 4; /* slots a thread that another CTA is taken for */
@@ -300,29 +304,13 @@ __device__ __forceinline__ int warp_before(int v)
     }
     return s - v;
 }
-/* count one key into bin d: the bin of the warp's first lane (often most of them: equal
- * weights, zeros) by one addition, the others by theirs.  Integer counts: any order. */
-__device__ __forceinline__ void count(int *hist, bool in, uint32_t d)
-{
-    const uint32_t some = __ballot_sync(0xFFFFFFFFu, in);
-    if (!some)
-        return;
-    const int lead = __ffs(some) - 1;
-    const uint32_t first = __shfl_sync(0xFFFFFFFFu, d, lead);
-    const uint32_t same = __ballot_sync(0xFFFFFFFFu, in && d == first);
-    if ((int)lane_id() == lead)
-        atomicAdd(&hist[d], __popc(same));
-    else if (in && !((same >> lane_id()) & 1u))
-        atomicAdd(&hist[d], 1);
-}
-
 template <int D>
 __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArgs a)
 {
     extern __shared__ uint32_t ev_smem[];
     __shared__ int hist[2][256], tot[256];
     __shared__ int near_of[kEvWarps], far_of[kEvWarps], eq_of[kEvWarps]; /* per warp: free below n, kept from n on, keys equal to the n-th */
-    __shared__ int s_free, s_far, s_need;
+    __shared__ int s_free, s_far, s_need, s_same;
     __shared__ uint32_t s_prefix;
     const GlintKv4Cache &c = a.c;
     const GlintKv4Evict &e = a.e;
@@ -349,16 +337,20 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     const float *w = e.weight + row;
     const int *pos = e.pos + row;
     const int64_t guard = (int64_t)e.seen[b] - e.recent;
-    auto key = [&](int t) { return held ? keys[t - begin] : evict_key(w[t], pos[t], guard); };
+    auto key = [&](int t) { return held ? keys[t - begin] : evict_key(__ldg(w + t), __ldg(pos + t), guard); };
     if (h == 0 && rank == 0 && tid == 0)
         e.new_lens[b] = n;
-    if (held) {
+    for (int i = tid; i < 256; i += kEvThreads)
+        hist[0][i] = 0;
+    __syncthreads();
+    if (held) { /* and the first digit's counts: integers, so any order gives the same */
 #pragma unroll 8
-        for (int t = begin + tid; t < end; t += kEvThreads)
-            keys[t - begin] = evict_key(w[t], pos[t], guard);
+        for (int t = begin + tid; t < end; t += kEvThreads) {
+            const uint32_t k = evict_key(__ldg(w + t), __ldg(pos + t), guard);
+            keys[t - begin] = k;
+            atomicAdd(&hist[0][k >> 24], 1);
+        }
     }
-    if (tid < 256)
-        hist[0][tid] = 0;
     __syncthreads();
 
     /* the n-th largest key, a digit at a time */
@@ -368,11 +360,13 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
         for (int p = 0; p < 4; ++p) {
             const int shift = 24 - 8 * p;
             const uint32_t high = p ? 0xFFFFFFFFu << (shift + 8) : 0u;
+            if (p || !held) {
 #pragma unroll 4
-            for (int t0 = begin; t0 < end; t0 += kEvThreads) {
-                const int t = t0 + tid;
-                const uint32_t k = t < end ? key(t) : 0u;
-                count(hist[p & 1], t < end && (k & high) == prefix, (k >> shift) & 255u);
+                for (int t = begin + tid; t < end; t += kEvThreads) {
+                    const uint32_t k = key(t);
+                    if ((k & high) == prefix)
+                        atomicAdd(&hist[p & 1][(k >> shift) & 255u], 1);
+                }
             }
             cluster_barrier();
             if (tid < 256) {
@@ -397,41 +391,44 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
                     int d = 255 - 8 * lane;
                     while (tot[d] < left)
                         left -= tot[d--];
-                    s_prefix = prefix | ((uint32_t)d << shift), s_need = left;
+                    s_prefix = prefix | ((uint32_t)d << shift), s_need = left, s_same = tot[d];
                 }
             }
             __syncthreads();
             prefix = s_prefix, need = s_need;
         }
-        /* the last histogram counts, for its digit, the keys equal to the n-th */
+    }
+    /* kept: above the n-th key, and of those equal to it the `need` lowest slots (or all,
+     * where there are no more).  A warp has per_warp words of 32 slots. */
+    const int w0 = warp * per_warp;
+    const bool ties = L > n && s_same > need;
+    if (ties) { /* the last histogram counts, for its digit, the keys equal to the n-th */
 #pragma unroll
         for (int r = 0; r < 8; ++r)
             eq_before += r < rank ? load_there(there(&hist[1][prefix & 255u], r)) : 0;
+        int eqs = 0;
+        for (int q = 0; q < per_warp; ++q) {
+            const int t = begin + (w0 + q) * 32 + lane;
+            eqs += __popc(__ballot_sync(0xFFFFFFFFu, t < end && key(t) == prefix));
+        }
+        if (lane == 0)
+            eq_of[warp] = eqs;
+        __syncthreads();
+        for (int k = 0; k < warp; ++k)
+            eq_before += eq_of[k];
     }
-    /* kept: above the n-th key, and of those equal to it the `need` lowest slots.  A warp
-     * has per_warp words of 32 slots. */
-    const int w0 = warp * per_warp;
-    int eqs = 0;
-#pragma unroll 4
-    for (int q = 0; q < per_warp; ++q) {
-        const int t = begin + (w0 + q) * 32 + lane;
-        eqs += __popc(__ballot_sync(0xFFFFFFFFu, t < end && L > n && key(t) == prefix));
-    }
-    if (lane == 0)
-        eq_of[warp] = eqs;
-    __syncthreads();
-    for (int k = 0; k < warp; ++k)
-        eq_before += eq_of[k];
     int frees = 0, fars = 0;
 #pragma unroll 4
     for (int q = 0; q < per_warp; ++q) {
         const int t0 = begin + (w0 + q) * 32, t = t0 + lane;
         const uint32_t k = t < end ? key(t) : 0u;
-        const bool eq = t < end && L > n && k == prefix;
-        const uint32_t me = __ballot_sync(0xFFFFFFFFu, eq);
-        const bool keep = t < end && (L <= n || k > prefix ||
-                                      (eq && eq_before + __popc(me & ((1u << lane) - 1u)) < need));
-        eq_before += __popc(me);
+        bool keep = t < end && (L <= n || k >= prefix);
+        if (ties) {
+            const uint32_t me = __ballot_sync(0xFFFFFFFFu, t < end && k == prefix);
+            if (k == prefix && eq_before + __popc(me & ((1u << lane) - 1u)) >= need)
+                keep = false;
+            eq_before += __popc(me);
+        }
         const uint32_t m = __ballot_sync(0xFFFFFFFFu, keep), below = __ballot_sync(0xFFFFFFFFu, t < n);
         if (lane == 0)
             bits[w0 + q] = m, free_at[w0 + q] = frees, far_at[w0 + q] = fars;
@@ -471,64 +468,74 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     for (int t = rank * kEvThreads + tid; t < n; t += ctas * kEvThreads) {
         const int r = t / stretch, at = t - r * stretch;
         if ((load_there(there(&bits[at / 32], r)) >> (at % 32)) & 1)
-            kept[t] = t, e.weight_out[row + t] = w[t], e.pos_out[row + t] = pos[t];
+            kept[t] = t, e.weight_out[row + t] = __ldg(w + t), e.pos_out[row + t] = __ldg(pos + t);
     }
     for (int i = n + rank * kEvThreads + tid; i < e.budget; i += ctas * kEvThreads)
         kept[i] = -1;
     cluster_barrier();
-    /* the kept slots from n on, a thread each: number j of this CTA's by two searches */
+    /* the kept slots from n on: a lane each to find number j of this CTA's by two searches, then
+     * the lanes together, 16 bytes each of K and of V */
+    constexpr int kLanes = D / 16; /* a slot's */
     const int *table = e.table + (int64_t)b * e.max_pages;
-    for (int j = tid; j < s_far; j += kEvThreads) {
-        int wp = 0;
+    for (int j0 = warp * 32; j0 < s_far; j0 += kEvThreads) {
+        const int j = j0 + lane;
+        int64_t from = -1, to = -1; /* slots' rows in the cache */
+        if (j < s_far) {
+            int wp = 0;
 #pragma unroll
-        for (int step = kEvWarps / 2; step > 0; step /= 2)
-            if (far_of[wp + step] <= j)
-                wp += step;
-        const int in = j - far_of[wp];
-        int lo = wp * per_warp, hi = lo + per_warp - 1; /* its last word with far_at <= in */
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (far_at[mid] <= in)
-                lo = mid;
-            else
-                hi = mid - 1;
+            for (int step = kEvWarps / 2; step > 0; step /= 2)
+                if (far_of[wp + step] <= j)
+                    wp += step;
+            const int in = j - far_of[wp];
+            int lo = wp * per_warp, hi = lo + per_warp - 1; /* its last word with far_at <= in */
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (far_at[mid] <= in)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            uint32_t m = bits[lo];
+            const int t0 = begin + lo * 32;
+            if (t0 < n)
+                m &= 0xFFFFFFFFu << (n - t0); /* n - t0 < 32: the word has a slot from n on */
+            for (int k = in - far_at[lo]; k > 0; --k)
+                m &= m - 1;
+            const int src = t0 + __ffs(m) - 1, k = far_base + j;
+            const int dst = load_there(there(&list[k % part], k / part));
+            const float weight = __ldg(w + src);
+            const int position = __ldg(pos + src);
+            const int pf = __ldg(table + (src >> a.page_log2)), pt = __ldg(table + (dst >> a.page_log2));
+            kept[dst] = src, e.weight_out[row + dst] = weight, e.pos_out[row + dst] = position;
+            if (pf >= 0 && pf < c.pages && pt >= 0 && pt < c.pages) {
+                from = (((int64_t)pf * c.kv_heads + h) << a.page_log2) + (src & (c.page_size - 1));
+                to = (((int64_t)pt * c.kv_heads + h) << a.page_log2) + (dst & (c.page_size - 1));
+            }
         }
-        uint32_t m = bits[lo];
-        const int t0 = begin + lo * 32;
-        if (t0 < n)
-            m &= 0xFFFFFFFFu << (n - t0); /* n - t0 < 32: the word has a slot from n on */
-        for (int k = in - far_at[lo]; k > 0; --k)
-            m &= m - 1;
-        const int src = t0 + __ffs(m) - 1, k = far_base + j;
-        const int dst = load_there(there(&list[k % part], k / part));
-        kept[dst] = src, e.weight_out[row + dst] = w[src], e.pos_out[row + dst] = pos[src];
-        const int pf = table[src >> a.page_log2], pt = table[dst >> a.page_log2];
-        if (pf < 0 || pf >= c.pages || pt < 0 || pt >= c.pages)
-            continue;
-        const int rf = src & (c.page_size - 1), rt = dst & (c.page_size - 1);
-        const int64_t from = (((int64_t)pf * c.kv_heads + h) << a.page_log2) + rf;
-        const int64_t to = (((int64_t)pt * c.kv_heads + h) << a.page_log2) + rt;
-        uint4 kc[D / 32], vc[D / 32];
+        const int part16 = lane % (kLanes / 2), block = part16 / 2; /* 16 bytes of a row */
+        const bool is_v = lane % kLanes >= kLanes / 2;
+        uint8_t *const code = is_v ? c.v_code : c.k_code;
+        uint32_t *const meta = reinterpret_cast<uint32_t *>(is_v ? c.v_meta : c.k_meta);
+        uint4 x[kLanes];
+        uint32_t y[kLanes];
 #pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-            kc[q] = *reinterpret_cast<const uint4 *>(c.k_code + from * (D / 2) + kv4_unit<D>(q / 2, rf) + (q % 2) * 16);
-            vc[q] = *reinterpret_cast<const uint4 *>(c.v_code + from * (D / 2) + kv4_unit<D>(q / 2, rf) + (q % 2) * 16);
-        }
-        uint32_t km[D / 64], vm[D / 64];
-#pragma unroll
-        for (int q = 0; q < D / 64; ++q) {
-            km[q] = reinterpret_cast<const uint32_t *>(c.k_meta)[from * (D / 64) + q];
-            vm[q] = reinterpret_cast<const uint32_t *>(c.v_meta)[from * (D / 64) + q];
+        for (int q = 0; q < kLanes; ++q) {
+            const int64_t at = __shfl_sync(0xFFFFFFFFu, from, q * (32 / kLanes) + lane / kLanes);
+            if (at >= 0) {
+                const int r = (int)at & (c.page_size - 1);
+                x[q] = *reinterpret_cast<const uint4 *>(code + at * (D / 2) + kv4_unit<D>(block, r) + (part16 % 2) * 16);
+                y[q] = part16 < D / 64 ? meta[at * (D / 64) + part16] : 0u;
+            }
         }
 #pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-            *reinterpret_cast<uint4 *>(c.k_code + to * (D / 2) + kv4_unit<D>(q / 2, rt) + (q % 2) * 16) = kc[q];
-            *reinterpret_cast<uint4 *>(c.v_code + to * (D / 2) + kv4_unit<D>(q / 2, rt) + (q % 2) * 16) = vc[q];
-        }
-#pragma unroll
-        for (int q = 0; q < D / 64; ++q) {
-            reinterpret_cast<uint32_t *>(c.k_meta)[to * (D / 64) + q] = km[q];
-            reinterpret_cast<uint32_t *>(c.v_meta)[to * (D / 64) + q] = vm[q];
+        for (int q = 0; q < kLanes; ++q) {
+            const int64_t at = __shfl_sync(0xFFFFFFFFu, to, q * (32 / kLanes) + lane / kLanes);
+            if (at >= 0) {
+                const int r = (int)at & (c.page_size - 1);
+                *reinterpret_cast<uint4 *>(code + at * (D / 2) + kv4_unit<D>(block, r) + (part16 % 2) * 16) = x[q];
+                if (part16 < D / 64)
+                    meta[at * (D / 64) + part16] = y[q];
+            }
         }
     }
     cluster_barrier(); /* no CTA leaves while another may read its list */
