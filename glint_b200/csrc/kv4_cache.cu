@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache 
  * the moves do not depend on one another.
  *
  * Floor: 8 bytes a slot and head read (weight and position), 8 + D + D / 8 read and
- * written a slot moved.  Bound: latency, of six cluster barriers and of what each waits
+ * written a slot moved.  Bound: latency, of seven cluster barriers and of what each waits
  * for.  16 ragged sequences of up to 32768 slots to 4096, 8 heads of 128: 35 us, about 17 of
  * them the four digits, 7 the lists, 11 the moves (a lane's 16 bytes of K and of V; with a
  * slot a lane the moves took 18).  512 threads a CTA: 39 us there, 28 instead of 34 for two
