@@ -142,9 +142,9 @@ def _raw(like: torch.Tensor, stream: Optional[torch.cuda.Stream], *others) -> in
 def _empty(like: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
     """Memory for the stream that writes it."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape, dtype=dtype)
 
 
 def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[int], ...], dense: bool = True):
@@ -154,10 +154,14 @@ def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.shape != shape:
-        if None not in shape or len(t.shape) != len(shape) or \
-                any(w is not None and s != w for s, w in zip(t.shape, shape)):
-            raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    got = t.shape
+    if got != shape:
+        bad = len(got) != len(shape)
+        for w, n in zip(shape, got):  # a loop: a generator's start takes as long as the rest
+            if n != w and w is not None:
+                bad = True
+        if bad:
+            raise ValueError(f"{name} must have shape {shape}, not {tuple(got)}")
     if dense:
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
