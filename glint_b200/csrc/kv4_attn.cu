@@ -19,7 +19,7 @@
  * Floor: HBM, D + D / 8 bytes a slot and head at 4.5 bits a value.  Bound: unpacking,
  * about 790 warp instructions for 32 slots of K and V at D = 128 (ALU 63 %, issue 64 % busy).
  * 16 sequences of 16384 slots, 64 / 8 heads: 80 us (loads alone 57, arithmetic alone 71);
- * 64 of 32768: 531 us, 4.55 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 39
+ * 64 of 32768: 531 us, 4.55 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 37
  * with weights.  One of 1021: 11 us, latency.
  */
 #include <cuda_runtime.h>
@@ -797,32 +797,66 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kJoinThreads) kv4_join_kernel(cons
     }
 }
 
-/* weight_out from the scores: a thread per slot, the columns in order (four a load where
- * they are a multiple of four) */
+/* weight_out from the scores: the columns of a slot in order, by one thread (four a load
+ * where they are a multiple of four). */
+/* Slots a thread, 256 apart, loaded together.  1, 2, 4: one sequence of 1021 slots, 32 / 8
+ * heads, 13.0, 13.6, 14.4 us; 32 ragged of up to 8191 38.4, 37.3, 36.8; 16 of 16384, 64 / 8
+ * heads, 102.6, 101.1, 100.1. */
+constexpr int kWeightSlots = 2;
 __global__ void __launch_bounds__(256) kv4_weight_kernel(const Args g)
 {
     const int bh = blockIdx.y, b = bh / g.c.kv_heads;
-    const int len = length_of(g, b), t = blockIdx.x * 256 + threadIdx.x;
-    asm volatile("griddepcontrol.wait;" ::: "memory"); /* scores and sums are the kernels' before */
-    if (t >= len)
+    const int len = length_of(g, b), first = blockIdx.x * 256 * kWeightSlots;
+    if (first >= len && (blockIdx.x | blockIdx.y)) /* one CTA waits in any case: this kernel ends after the one before */
         return;
-    const int64_t i = (int64_t)bh * g.a.weight_stride + t;
-    const float old = g.a.weight && t < len - g.a.rows ? g.a.weight[i] : 0.f;
-    const int page = g.a.table[(int64_t)b * g.a.max_pages + (t >> g.page_log2)];
-    const float *s = g.score + ((int64_t)bh * (g.a.max_pages << g.page_log2) + t) * g.cols, *z = g.lse2 + (int64_t)bh * g.cols;
-    float sum = 0.f;
-    auto add = [&](float v, float zn) { sum += v == -INFINITY ? 0.f : ex2(v - zn); };
-    if (page >= 0 && page < g.c.pages) {
-        int n = 0;
-        if (g.cols % 4 == 0)
-            for (; n < g.cols; n += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(s + n), y = *reinterpret_cast<const float4 *>(z + n);
-                add(v.x, y.x), add(v.y, y.y), add(v.z, y.z), add(v.w, y.w);
-            }
-        for (; n < g.cols; ++n)
-            add(s[n], z[n]);
+    /* the caller's, older than the scores' kernel */
+    float sum[kWeightSlots], old[kWeightSlots];
+    bool in[kWeightSlots];
+    const int64_t row = (int64_t)bh * g.a.weight_stride;
+#pragma unroll
+    for (int j = 0; j < kWeightSlots; ++j) {
+        const int t = first + j * 256 + threadIdx.x;
+        old[j] = g.a.weight && t < len - g.a.rows ? g.a.weight[row + t] : 0.f;
+        const int page = t < len ? g.a.table[(int64_t)b * g.a.max_pages + (t >> g.page_log2)] : -1;
+        in[j] = page >= 0 && page < g.c.pages;
+        sum[j] = 0.f;
     }
-    g.a.weight_out[i] = old + sum;
+    asm volatile("griddepcontrol.wait;" ::: "memory"); /* scores and sums are the kernels' before */
+    const float *z = g.lse2 + (int64_t)bh * g.cols;
+    const float *s = g.score + ((int64_t)bh * (g.a.max_pages << g.page_log2) + first + threadIdx.x) * g.cols;
+    auto add = [&](int j, int n, int count) {
+        if (!in[j])
+            return;
+        const float *p = s + (int64_t)j * 256 * g.cols + n;
+        auto one = [&](float v, float zn) { sum[j] += v == -INFINITY ? 0.f : ex2(v - zn); };
+        if (count == 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(p), y = *reinterpret_cast<const float4 *>(z + n);
+            one(v.x, y.x), one(v.y, y.y), one(v.z, y.z), one(v.w, y.w);
+        } else {
+            one(*p, z[n]);
+        }
+    };
+    if (g.cols == 4) { /* one load a slot: all slots' at once */
+#pragma unroll
+        for (int j = 0; j < kWeightSlots; ++j)
+            add(j, 0, 4);
+    } else { /* a slot's columns lie apart from the next thread's: slot by slot, while its sectors are at hand */
+#pragma unroll
+        for (int j = 0; j < kWeightSlots; ++j) {
+            int n = 0;
+            if (g.cols % 4 == 0)
+                for (; n < g.cols; n += 4)
+                    add(j, n, 4);
+            for (; n < g.cols; ++n)
+                add(j, n, 1);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kWeightSlots; ++j) {
+        const int t = first + j * 256 + threadIdx.x;
+        if (t < len)
+            g.a.weight_out[row + t] = old[j] + sum[j];
+    }
 }
 
 int check(const GlintKv4Cache *c, const GlintKv4Attn *a)
@@ -890,7 +924,7 @@ int launch(Args &g, cudaStream_t st)
         return kLaunch;
     }
     if (g.score) {
-        const dim3 grid((g.a.max_pages * g.c.page_size + 255) / 256, g.a.seqs * g.c.kv_heads);
+        const dim3 grid((g.a.max_pages * g.c.page_size - 1) / (256 * kWeightSlots) + 1, g.a.seqs * g.c.kv_heads);
         if (launch_after(kv4_weight_kernel, grid, 256, st, g) != cudaSuccess) {
             cudaGetLastError();
             return kLaunch;
