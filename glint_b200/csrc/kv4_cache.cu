@@ -244,10 +244,11 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache 
  *
  * Floor: 8 bytes a slot and head read (weight and position), 8 + D + D / 8 read and
  * written a slot moved.  Bound: latency, of seven cluster barriers and of what each waits
- * for.  16 ragged sequences of up to 32768 slots to 4096, 8 heads of 128: 35 us, about 17 of
- * them the four digits, 7 the lists, 11 the moves (a lane's 16 bytes of K and of V; with a
- * slot a lane the moves took 18).  512 threads a CTA: 39 us there, 28 instead of 34 for two
- * such sequences.  One of 1025 to 1024: 14 us.
+ * for: for a sequence of 32768 slots about 50000 clocks, 8400 of them for the keys and the
+ * first digit's counts, 16000 for the digits, 3000 for the bits, 6600 for the list (the
+ * first CTA's slots, mostly), 8700 for the moves (16 bytes a lane; a slot a lane: 14000).
+ * 16 ragged sequences of up to 32768 slots to 4096, 8 heads of 128: 33 us (512 threads a
+ * CTA: 37, though 27 in place of 32 for two such sequences alone).  8 of 1025 to 1024: 12.6.
  */
 constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32;
 constexpr int kEvSlots = 4; /* slots a thread that another CTA is taken for */
@@ -308,7 +309,8 @@ template <int D>
 __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArgs a)
 {
     extern __shared__ uint32_t ev_smem[];
-    __shared__ int hist[2][256], tot[256];
+    __shared__ int hist[2][256];
+    __shared__ __align__(16) int tot[256];
     __shared__ int near_of[kEvWarps], far_of[kEvWarps], eq_of[kEvWarps]; /* per warp: free below n, kept from n on, keys equal to the n-th */
     __shared__ int s_free, s_far, s_need, s_same;
     __shared__ uint32_t s_prefix;
@@ -382,16 +384,20 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
             }
             __syncthreads();
             if (warp == 0) { /* lane i: bins 255 - 8 i down to 248 - 8 i */
+                const int4 hi = reinterpret_cast<const int4 *>(tot)[63 - 2 * lane], lo = reinterpret_cast<const int4 *>(tot)[62 - 2 * lane];
+                const int in[8] = {hi.w, hi.z, hi.y, hi.x, lo.w, lo.z, lo.y, lo.x};
                 int sum = 0;
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    sum += tot[255 - 8 * lane - q];
+                    sum += in[q];
                 int left = need - warp_before(sum); /* still wanted from this lane's bins on */
                 if (left > 0 && left <= sum) {
-                    int d = 255 - 8 * lane;
-                    while (tot[d] < left)
-                        left -= tot[d--];
-                    s_prefix = prefix | ((uint32_t)d << shift), s_need = left, s_same = tot[d];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        if (left > 0 && left <= in[q])
+                            s_prefix = prefix | ((uint32_t)(255 - 8 * lane - q) << shift), s_need = left, s_same = in[q];
+                        left -= in[q];
+                    }
                 }
             }
             __syncthreads();
@@ -453,6 +459,12 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
         free_base += r < rank ? f : 0, far_base += r < rank ? g : 0, moved += f;
     }
     const int part = max(1, (moved + ctas - 1) / ctas); /* entries of the list a CTA holds */
+    const uint32_t inv = 0xFFFFFFFFu / (uint32_t)part;
+    auto entry = [&](int k) { /* entry k of the list, k < 2^19: at most one off before the step up */
+        int r = (int)__umulhi((uint32_t)k, inv);
+        r += k - r * part >= part;
+        return there(&list[k - r * part], r);
+    };
     int *kept = e.kept + (int64_t)bh * e.budget;
 #pragma unroll 2
     for (int q = 0; q < per_warp; ++q) { /* the free slots of this CTA's into the list */
@@ -460,9 +472,10 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
         const uint32_t out = t0 >= n ? 0u : ~bits[w0 + q] & (n - t0 >= 32 ? 0xFFFFFFFFu : (1u << (n - t0)) - 1u);
         if ((out >> lane) & 1u) {
             const int k = free_base + near_of[warp] + free_at[w0 + q] + __popc(out & ((1u << lane) - 1u));
-            store_there(there(&list[k % part], k / part), t);
+            store_there(entry(k), t);
         }
     }
+    cluster_barrier(); /* lists, the last words that others write here */
     /* the kept ones below n, shared out evenly: most of them lie in the first CTAs */
 #pragma unroll 4
     for (int t = rank * kEvThreads + tid; t < n; t += ctas * kEvThreads) {
@@ -472,7 +485,6 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
     }
     for (int i = n + rank * kEvThreads + tid; i < e.budget; i += ctas * kEvThreads)
         kept[i] = -1;
-    cluster_barrier();
     /* the kept slots from n on: a lane each to find number j of this CTA's by two searches, then
      * the lanes together, 16 bytes each of K and of V */
     constexpr int kLanes = D / 16; /* a slot's */
@@ -499,10 +511,15 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
             const int t0 = begin + lo * 32;
             if (t0 < n)
                 m &= 0xFFFFFFFFu << (n - t0); /* n - t0 < 32: the word has a slot from n on */
-            for (int k = in - far_at[lo]; k > 0; --k)
-                m &= m - 1;
-            const int src = t0 + __ffs(m) - 1, k = far_base + j;
-            const int dst = load_there(there(&list[k % part], k / part));
+            int skip = in - far_at[lo], at = 0; /* its bit after `skip` others, by halves */
+#pragma unroll
+            for (int half = 16; half > 0; half /= 2) {
+                const int low = __popc(m >> at & ((1u << half) - 1u));
+                if (skip >= low)
+                    skip -= low, at += half;
+            }
+            const int src = t0 + at, k = far_base + j;
+            const int dst = load_there(entry(k));
             const float weight = __ldg(w + src);
             const int position = __ldg(pos + src);
             const int pf = __ldg(table + (src >> a.page_log2)), pt = __ldg(table + (dst >> a.page_log2));
@@ -538,7 +555,9 @@ __global__ void __launch_bounds__(kEvThreads, 4) kv4_evict_kernel(const EvictArg
             }
         }
     }
-    cluster_barrier(); /* no CTA leaves while another may read its list */
+    /* no CTA leaves while another may read its bits or list; nothing is handed over */
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kLaunch; }
