@@ -4,11 +4,12 @@
  * columns of a tensor-core tile) share every byte of the cache that is read.  With
  * x = lo + step * code for K and V, per 64-value block b of a slot t:
  *
- *   s[t, n] = sum_b step (sum_d (code - 8) q[n, d]) + (lo + 8 step) (sum_d q[n, d])
+ *   s[t, n] = sum_b step (sum_d (code + 16) q[n, d]) + (lo - 16 step) (sum_d q[n, d])
  *   o[d, n] = sum_t (code - 8) (p[t, n] step)       + sum_t p[t, n] (lo + 8 step)
  *
  * so the products are mma.sync tiles whose A operand is the codes themselves: (w &
- * 0x000F000F) | 0x43004300 is the BF16 pair 128 + code, less 136 it is code - 8, exact.
+ * 0x00780078) | 0x41804180 is the BF16 pair 16 + code, as K takes it; (w & 0x000F000F) |
+ * 0x43004300 is 128 + code, less 136 it is code - 8, as V does; all exact.
  * The tile's inner index may be any order that both operands share, so a 32-bit word's
  * nibbles j and j + 4 make a pair as they lie.  For K (rows = slots, inner = d) q is
  * permuted to match once; for V (rows = d, inner = slots) a pair is the same nibble of
@@ -19,7 +20,7 @@
  * Floor: HBM, D + D / 8 bytes a slot and head at 4.5 bits a value.  Bound: unpacking,
  * about 790 warp instructions for 32 slots of K and V at D = 128 (ALU 63 %, issue 64 % busy).
  * 16 sequences of 16384 slots, 64 / 8 heads: 80 us (loads alone 57, arithmetic alone 71);
- * 64 of 32768: 531 us, 4.55 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 37
+ * 64 of 32768: 534 us, 4.53 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 38
  * with weights.  One of 1021: 11 us, latency.
  */
 #include <cuda_runtime.h>
@@ -190,7 +191,16 @@ __device__ __forceinline__ void load_meta(uint32_t at, uint32_t (&m)[NB])
         m[0] = lds32(at);
     }
 }
-/* nibbles j and j + 4 of w as the BF16 pair (128 + code, 128 + code) */
+/* nibbles j and j + 4 of w as the BF16 pair (16 + code, 16 + code), for the products whose
+ * excess is taken back in f32: 128 + code needs a shift less, but its eight times larger sums
+ * cancel to eight times the error (lse of few slots: 2e-6 of its value) */
+__device__ __forceinline__ uint32_t codes16(uint32_t w, int j)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x00780078, %2, 0xEA;" : "=r"(r) : "r"(j ? w >> (4 * j - 3) : w << 3), "r"(0x41804180u));
+    return r;
+}
+/* the same as (128 + code, 128 + code) */
 __device__ __forceinline__ uint32_t codes128(uint32_t w, int j)
 {
     uint32_t r;
@@ -328,7 +338,7 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
             const uint2 wb = lds64(kcode + tb * RB + kv4_unit<D>(k, tb) + 8 * c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t a[4] = {codes128(wa.x, j), codes128(wb.x, j), codes128(wa.y, j), codes128(wb.y, j)};
+                const uint32_t a[4] = {codes16(wa.x, j), codes16(wb.x, j), codes16(wa.y, j), codes16(wb.y, j)};
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     j ? mma(acc[k][n], a, q.b[n][k][j][0], q.b[n][k][j][1])
@@ -347,8 +357,8 @@ __device__ __forceinline__ void tile_step(const Args &g, const Query<D, NT> &q, 
         for (int k = 0; k < NB; ++k) {
             const uint32_t ma = mas[k], mb = mbs[k];
             const float sa = __uint_as_float(ma << 16), sb = __uint_as_float(mb << 16);
-            const float la = fmaf(-128.f, sa, __uint_as_float(ma & 0xFFFF0000u));
-            const float lb = fmaf(-128.f, sb, __uint_as_float(mb & 0xFFFF0000u));
+            const float la = fmaf(-16.f, sa, __uint_as_float(ma & 0xFFFF0000u));
+            const float lb = fmaf(-16.f, sb, __uint_as_float(mb & 0xFFFF0000u));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 s[sl][n][0] = fmaf(sa, acc[k][n][0], fmaf(la, q.sum[n][k][0], s[sl][n][0]));

@@ -460,6 +460,27 @@ def test_cache_attention_long(dim, lens, heads, kv, rows):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+def test_cache_attention_scores_keep_f32(dim):
+    """lse of one slot is its scaled score.  The products take codes with 16 added, so a 64-block's
+    sum is about 24 * sqrt(64) = 192 for unit q; each of its four steps may drop 2^-23 of that,
+    evenly spread: 2^-23 * 192 / sqrt(3) * 2 = 2^-23 * 222, times a step of 4.7 / 15 for 64 unit
+    normals, over a score of sqrt(64): 8.7 * 2^-23 of the scores in the mean square (two
+    blocks: sqrt(2) in both)."""
+    g = gen(dim + 5)
+    seqs, kv, heads = 256, 2, 8
+    cache = A().KV4Cache.empty(seqs, kv, dim, 16)
+    k, v = randn(seqs, kv, dim, g=g), randn(seqs, kv, dim, g=g)
+    A().kv4_append(cache, k, v, torch.arange(seqs, dtype=torch.int32, device="cuda") * 16)
+    table = torch.arange(seqs, dtype=torch.int32, device="cuda")[:, None]
+    q = randn(seqs, 1, heads, dim, g=g)
+    _, lse = A().kv4_attn(q, cache, table, torch.ones(seqs, dtype=torch.int32, device="cuda"))
+    kd = values(*quantise(k), dtype=torch.float64).repeat_interleave(heads // kv, 1)
+    want = (q[:, 0].double() * kd).sum(-1) * dim ** -0.5
+    error = float((lse[..., 0].double() - want).norm() / want.norm())
+    assert error <= 8.7 * 2.0 ** -23, f"scores are {error} off"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_cache_attention_large_scores(dim):
     g = gen(dim)
     lens = [515, 130]
