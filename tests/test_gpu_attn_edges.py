@@ -1,0 +1,91 @@
+"""GPU tests of the serving attention operators past the lengths of test_gpu_attn.py: prompts
+whose keys are cut over the SMs, values that are not finite at such lengths, eviction with more
+slots than a CTA's shared memory holds keys.  References and bounds are that file's."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_attn import (A, bits, check_prompt, cu, evict_reference, gen, gpu, kernel_error,  # noqa: E402,F401
+                           prompt_reference, randn, within)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,lq,lk", [(8, 2, [1], [1000]), (4, 4, [130], [9000]), (16, 1, [17], [897]),
+                                            (5, 1, [100, 30], [5000, 3001]), (2, 2, [5, 0, 64, 1], [1024, 2000, 4097, 7]),
+                                            (1, 1, [300], [2049])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_keys_cut_over_sms(dim, heads, kv, lq, lk, causal):
+    """Few queries with many keys: parts of the keys, joined by a second kernel."""
+    g = gen(sum(lk) + dim)
+    check_prompt(randn(sum(lq), heads, dim, g=g), randn(sum(lk), kv, dim, g=g), randn(sum(lk), kv, dim, g=g), lq, lk, causal)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_cut_large_scores(dim):
+    """Parts whose maxima lie far apart."""
+    g = gen(dim + 1)
+    k = randn(6000, 2, dim, g=g) * torch.linspace(0.1, 20, 6000, device="cuda")[:, None, None].bfloat16()
+    q, v = randn(90, 4, dim, g=g, scale=4), randn(6000, 2, dim, g=g)
+    check_prompt(q, k, v, [90], [6000])
+    check_prompt(q, k.flip(0).contiguous(), v, [90], [6000])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("heads,kv,lq,lk", [(4, 2, [200], [5000]), (4, 1, [40, 150], [3000, 1200]), (64, 32, [700], [700])])
+def test_prompt_masked_values_stay_out_of_long_rows(dim, bad, heads, kv, lq, lk):
+    """As for short sequences: with the keys cut, and with more blocks than are cut."""
+    g = gen(dim + sum(lk))
+    n, m = sum(lq), sum(lk)
+    q, k, v = randn(n, heads, dim, g=g), randn(m + 50, kv, dim, g=g), randn(m + 50, kv, dim, g=g)
+    want = prompt_reference(q, k[:m], v[:m], lq, lk, True, dim ** -0.5)
+    for tail in (1, 30, 97):  # the last keys of every sequence
+        k2, v2 = k.clone(), v.clone()
+        rows = torch.ones(n, dtype=torch.bool, device="cuda")
+        at = kat = 0
+        for a, b in zip(lq, lk):
+            at, kat = at + a, kat + b
+            rows[max(at - a, at - tail):at] = False
+            for x in (k2, v2):
+                x[kat - tail:kat] = bad
+        for x in (k2, v2):
+            x[m:] = bad
+        o, lse = A().attn_prompt(q, k2, v2, cu(lq), cu(lk))
+        assert kernel_error() == 0
+        within(o[rows], want[0][rows], want[1][rows], "o")
+        within(lse[:, rows], want[2][:, rows], want[3][:, rows], "lse")
+
+
+@pytest.mark.parametrize("length,page", [(330001, 128), (524288, 64), (5000, 128)])
+def test_evict_past_the_keys_held(length, page):
+    """A table of 524288 slots: weights are read again for every digit.  Ties run over every
+    stretch of slots; rows, weights and positions move as `kept` says."""
+    g = gen(length)
+    kv, dim, pages, budget, recent = 1, 64, 524288 // page, 4001, 100
+    cache = A().KV4Cache.empty(pages, kv, dim, page)
+    for t in (cache.k_code, cache.v_code):
+        t.copy_(torch.randint(0, 256, t.shape, device="cuda", generator=g, dtype=torch.uint8))
+    for t in (cache.k_meta, cache.v_meta):
+        t.copy_(torch.rand(t.shape, device="cuda", generator=g))
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)[None]
+    w = torch.randint(0, 40, (1, kv, pages * page), device="cuda", generator=g).float()  # the 4001st is one of thousands
+    pos = torch.rand(w.shape, device="cuda", generator=g).argsort(-1).to(torch.int32)
+    seen = torch.tensor([pages * page], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+    t = torch.arange(length, device="cuda")
+    slots = (table[0, t // page] * page + t % page).int()
+    before = A().kv4_read(cache, slots)
+    wo, po = torch.full_like(w, -1.0), torch.full_like(pos, -1)
+    kept, new = A().kv4_evict(cache, table, lens, w, pos, seen, budget, recent, weight_out=wo, pos_out=po)
+    after = A().kv4_read(cache, slots)
+    n = min(length, budget)
+    assert int(new) == n
+    want = evict_reference(w[0, 0].tolist(), pos[0, 0].tolist(), pages * page, length, budget, recent)
+    assert kept[0, 0].tolist() == want + [-1] * (budget - n)
+    src = torch.tensor(want, dtype=torch.long, device="cuda")
+    assert torch.equal(wo[0, 0, :n], w[0, 0][src]) and torch.equal(po[0, 0, :n], pos[0, 0][src])
+    assert bool((wo[0, 0, n:] == -1).all()) and bool((po[0, 0, n:] == -1).all())
+    for x, y in zip(before, after):
+        assert torch.equal(bits(y[:n]), bits(x[src])) and torch.equal(bits(y[n:]), bits(x[n:]))
