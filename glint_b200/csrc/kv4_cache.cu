@@ -627,6 +627,11 @@ int glint_kv4_evict_stream(const GlintKv4Cache *c, const GlintKv4Evict *e, cudaS
         !e->pos_out || e->weight == e->weight_out || e->pos == e->pos_out ||
         (int64_t)e->seqs * c->kv_heads > INT32_MAX)
         return kBadArg;
+    /* new_lens is written while other heads' CTAs, and others of a cluster, still read lens and seen:
+     * CTAs that disagree on a length disagree on which of them take part */
+    auto apart = [&](const int *in) { return in + e->seqs <= e->new_lens || e->new_lens + e->seqs <= in; };
+    if (!apart(e->lens) || !apart(e->seen))
+        return kBadArg;
     EvictArgs a{*c, *e, 1, 0, log2_of(c->page_size)};
     /* up to eight CTAs (a portable cluster) while each thread has kEvSlots or more */
     const int cap = e->max_pages * c->page_size;

@@ -114,9 +114,9 @@ int glint_kv4_attn_stream(const GlintKv4Cache *c, const GlintKv4Attn *a, cudaStr
  * where they are; the k-th kept slot from n on moves into the k-th free slot below n.
  * table and lens as above; weight, pos, weight_out, pos_out [seqs, kv_heads, stride].
  * kept [seqs, kv_heads, budget] int32: the slot each of the n now comes from (-1 from
- * n on); new_lens [seqs]; weight_out and pos_out get the kept slots' entries below n
- * and may not overlap weight and pos.  Sequences do not share the pages they move
- * rows in.  Limits: 0 <= recent <= budget, budget >= 1, max_pages * page_size <=
+ * n on); new_lens [seqs], which may not overlap lens or seen; weight_out and pos_out
+ * get the kept slots' entries below n and may not overlap weight and pos.  Sequences do
+ * not share the pages they move rows in.  Limits: 0 <= recent <= budget, budget >= 1, max_pages * page_size <=
  * 524288 and <= stride. */
 typedef struct GlintKv4Evict {
     const int *table, *lens;

@@ -1,0 +1,29 @@
+"""What the serving attention operators decide on the host: refusals before any device work,
+workspace sizes, and the control flow that a kernel file shares with the CPU."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from glint_b200 import attn, build
+    build.build()
+    return attn._lib()
+
+
+@pytest.mark.parametrize("field", ["lens", "seen"])
+@pytest.mark.parametrize("by", [0, 1, -1, 2, -2])
+def test_evict_refuses_new_lens_in_place(lib, field, by):
+    """Other heads read a sequence's lens and seen after one of them has written new_lens."""
+    from glint_b200 import attn
+    buf = (ctypes.c_uint8 * 4096)()
+    p = (ctypes.addressof(buf) + 15) & ~15
+    cache = attn._Cache(p, p, p, p, 4, 2, 64, 128)
+    at = {n: p + 256 * i for i, n in enumerate(("table", "lens", "weight", "pos", "seen", "kept", "new_lens",
+                                                "weight_out", "pos_out"))}
+    at["new_lens"] = at[field] + 4 * by
+    ev = attn._Evict(*at.values(), 256, 3, 4, 8, 2)
+    assert lib.glint_kv4_evict_stream(cache, ev, None) == -1
