@@ -114,14 +114,15 @@ _pack_attn = struct.Struct("8P4q4if4x").pack
 _pack_evict = struct.Struct("9Pq4i").pack
 
 
+# sizes grow with the current device's SMs: `dev` is part of what they are kept by
 @lru_cache(maxsize=256)
-def _prompt_work(q_tokens: int, k_tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
+def _prompt_work(dev: int, q_tokens: int, k_tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
     return max(0, _c().prompt_work(_pack_prompt(*[0] * 16, 1, q_tokens, k_tokens, heads, kv_heads, head_dim, 1, 1.0)))
 
 
 @lru_cache(maxsize=256)
-def _attn_work(kv_heads: int, page_size: int, head_dim: int, seqs: int, rows: int, heads: int, max_pages: int,
-               weights: bool) -> int:
+def _attn_work(dev: int, kv_heads: int, page_size: int, head_dim: int, seqs: int, rows: int, heads: int,
+               max_pages: int, weights: bool) -> int:
     cache = _pack_cache(16, 16, 16, 16, 1, kv_heads, page_size, head_dim)  # sizes are all that counts here
     return max(0, _c().attn_work(cache, _pack_attn(*[0] * 6, 1 if weights else 0, 0, *[0] * 4, seqs, rows, heads,
                                                    max_pages, 1.0)))
@@ -210,13 +211,14 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
         lse = _empty(q, (H, T), torch.float32, stream)
     else:
         _want(lse, "lse", torch.float32, (H, T))
-    n = _prompt_work(T, Tk, H, Hk, D)
+    raw = _raw(q, stream, k, v, cu_q, cu_k, out, lse)
+    n = _prompt_work(q.get_device(), T, Tk, H, Hk, D)
     work = _empty(q, (n,), torch.uint8, stream) if n else None
     qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
     a = _pack_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(),
                      cu_k.data_ptr(), work.data_ptr() if n else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                      cu_q.shape[0] - 1, T, Tk, H, Hk, D, 1 if causal else 0, D ** -0.5 if scale is None else scale)
-    _check(_c().prompt(a, _raw(q, stream, k, v, cu_q, cu_k, out, lse)), "glint_attn_prompt_stream")
+    _check(_c().prompt(a, raw), "glint_attn_prompt_stream")
     return out, lse
 
 
@@ -328,15 +330,15 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
         lse = _empty(q, (B, H, R), torch.float32, stream)
     else:
         _want(lse, "lse", torch.float32, (B, H, R))
-    work = _empty(q, (_attn_work(cache.kv_heads, cache.page_size, D, B, R, H, table.shape[1],
+    raw = _raw(q, stream, cache.k_code, table, lens, weight, weight_out, out, lse)
+    work = _empty(q, (_attn_work(q.get_device(), cache.kv_heads, cache.page_size, D, B, R, H, table.shape[1],
                                  weight_out is not None),), torch.uint8, stream)
     qs = q.stride()
     a = _pack_attn(q.data_ptr(), out.data_ptr(), lse.data_ptr(), table.data_ptr(), lens.data_ptr(),
                    0 if weight is None else weight.data_ptr(), 0 if weight_out is None else weight_out.data_ptr(),
                    work.data_ptr(), qs[0], qs[1], qs[2], wide, B, R, H, table.shape[1],
                    D ** -0.5 if scale is None else scale)
-    _check(_c().attn(cache._c, a, _raw(q, stream, cache.k_code, table, lens, weight, weight_out, out, lse)),
-           "glint_kv4_attn_stream")
+    _check(_c().attn(cache._c, a, raw), "glint_kv4_attn_stream")
     return out, lse
 
 

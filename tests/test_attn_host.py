@@ -27,3 +27,26 @@ def test_evict_refuses_new_lens_in_place(lib, field, by):
     at["new_lens"] = at[field] + 4 * by
     ev = attn._Evict(*at.values(), 256, 3, 4, 8, 2)
     assert lib.glint_kv4_evict_stream(cache, ev, None) == -1
+
+
+def test_workspaces_are_sized_for_their_device(monkeypatch):
+    """Devices of different SM counts in one process: no size kept for one is used for another."""
+    from glint_b200 import attn
+    device = 0
+
+    class Calls:
+        def prompt_work(self, a):
+            return 1000 * (device + 1)
+
+        def attn_work(self, c, a):
+            return 2000 * (device + 1)
+    monkeypatch.setattr(attn, "_c", lambda: Calls())
+    for f in (attn._prompt_work, attn._attn_work):
+        f.cache_clear()
+    try:
+        for device in (0, 1, 0, 1):
+            assert attn._prompt_work(device, 4, 5000, 4, 2, 128) == 1000 * (device + 1)
+            assert attn._attn_work(device, 2, 64, 128, 1, 1, 4, 8, False) == 2000 * (device + 1)
+    finally:
+        for f in (attn._prompt_work, attn._attn_work):
+            f.cache_clear()
