@@ -39,6 +39,7 @@
 #include "../../include/glint_attn.h"
 #include "common.cuh"
 #include "glint_internal.h"
+#include "item_loop.h"
 #include "ptx.cuh"
 
 namespace glint {
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     /* q_full: an item's Q and first K; kv_full[p]: V of the tile at ring place p and K of the next one */
     uint64_t *q_full = bars, *q_empty = bars + 1, *item_full = bars + 2, *item_empty = bars + 4, *s_full = bars + 6,
              *p_full = bars + 8, *o_done = bars + 10, *kv_full = bars + 12, *k_empty = kv_full + C::kStages,
-             *v_empty = k_empty + C::kStages;
+             *v_empty = k_empty + C::kStages, *drained = v_empty + C::kStages;
     __shared__ uint32_t tmem_slot;
     __shared__ Item s_item[2];
     __shared__ int s_more[2];
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == kLoadWarp && lane == 0) {
-        mbar_init(q_full, 1), mbar_init(q_empty, 1);
+        mbar_init(q_full, 1), mbar_init(q_empty, 1), mbar_init(drained, 1);
         for (int i = 0; i < C::kStages; ++i)
             mbar_init(kv_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_empty + i, 1);
         for (int i = 0; i < 2; ++i) {
@@ -473,9 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             alive = mbar_wait_suspend_bounded(bar, parity, &g_attn_error);
         return alive;
     };
-    auto warp_wait = [&](uint64_t *bar, uint32_t parity) {
-        wait(bar, parity);
-        __syncwarp();
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity) { /* a warp goes on, or gives up, as one */
+        alive = __all_sync(0xFFFFFFFFu, wait(bar, parity));
     };
 
     if (warp == kLoadWarp) {
@@ -620,9 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     umma_commit(v_empty + st);
                 }
             }
-            /* the last commit has arrived before this CTA's memory can go */
-            if (place > 0)
-                wait(v_empty + (place - 1) % C::kStages, ((place - 1) / C::kStages) & 1);
+            /* every product is done before this CTA's memory can go, after a wait that ran out too */
+            umma_commit(drained);
+            mbar_wait_bounded(drained, 0, &g_attn_error);
         }
         __syncwarp();
     } else {
@@ -633,10 +633,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         const float scale2 = g.a.scale * kLog2e;
         uint32_t turns = 0; /* tiles of keys gone through, of all items */
         int place0 = 0;     /* ring place of the item's first */
-        for (int items = 0;; ++items) {
+        auto next = [&](int items) {
             warp_wait(item_full + (items & 1), (items / 2) & 1);
-            if (!alive || !s_more[items & 1])
-                break;
+            return alive && s_more[items & 1];
+        };
+        auto any = [&](bool p) { return any_of_tile(i, p); };
+        item_loop(next, any, [&](int items) {
             const Item it = s_item[items & 1];
             __syncwarp();
             if (lane == 0)
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 l += a + b;
             }
             place0 += max(it.last0, it.last1) - it.first;
-            const bool bad = any_of_tile(i, odd);
+            const bool bad = any(odd);
             const int tile0 = it.t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
             const bool live = r < g.group * g.tok && t < s.q1;
             if (done > 0) {
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
             }
             tc_before(); /* O is read: the next item's products may write it once this warp's weights are in */
-        }
+        });
     }
     __syncthreads();
     if (warp == kMmaWarp) {

@@ -1,10 +1,14 @@
 """What the serving attention operators decide on the host: refusals before any device work,
 workspace sizes, and the control flow that a kernel file shares with the CPU."""
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 
 torch = pytest.importorskip("torch")
+
+NATIVE = Path(__file__).resolve().parent / "native"
 
 
 @pytest.fixture(scope="module")
@@ -50,3 +54,13 @@ def test_workspaces_are_sized_for_their_device(monkeypatch):
     finally:
         for f in (attn._prompt_work, attn._attn_work):
             f.cache_clear()
+
+
+@pytest.mark.parametrize("mode", ["loop", "alone"])
+def test_no_warp_is_left_at_a_barrier(tmp_path, mode):
+    """The prompt kernel's item loop where bounded waits run out in some warps of a tile and not in
+    others; and that the harness sees the hang of warps that leave by themselves."""
+    exe = tmp_path / "check_item_loop"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-pthread", "-o", str(exe), str(NATIVE / "check_item_loop.cpp")], check=True)
+    r = subprocess.run([str(exe), mode], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.startswith(f"OK {mode}"), r.stdout + r.stderr
