@@ -21,7 +21,8 @@
  *
  * Masked scores are replaced, never added to, and a masked weight is 0; a NaN or an
  * infinity in V would still reach other rows as 0 * NaN, so tiles with masked places
- * are looked through, and where one is found the rows are done one by one instead.
+ * are looked through and such values taken out of shared memory.  Rows that do see one
+ * get it afterwards: o of a column is then known without a product.
  *
  * Floor: exponentials (16 a clock and SM) and the tensor cores take the same time at
  * D = 128, 2048 clocks for two tiles of queries by one of keys.  Bound: a tile's softmax
@@ -401,6 +402,56 @@ __device__ __forceinline__ int cut_begin(int n, int cut, int cuts) { return (int
 
 /* any NaN or infinity among two BF16 */
 __device__ __forceinline__ uint32_t odd2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+/* acc + 0 * w, BF16 pairs: NaN from the first of them on */
+__device__ __forceinline__ uint32_t add_times0(uint32_t w, uint32_t acc)
+{
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w), "r"(0u));
+    return acc;
+}
+/* two BF16, 0 in place of such a one */
+__device__ __forceinline__ uint32_t without_odd2(uint32_t w) { return w & ~((odd2(w) >> 15) * 0xFFFFu); }
+
+/* V's first keys of a column with a NaN, +infinity and -infinity, of the first n keys of a
+ * sequence: at[kind * D + column], n and more for none.  By `threads` threads, with `sync` their
+ * barrier; V as the tensor-core kernel takes it (16-byte loads). */
+template <int D, class Sync>
+__device__ __noinline__ void first_odd(const GlintAttnPrompt &a, const Span &s, int head, int n, int *at, int tid,
+                                       int threads, Sync sync)
+{
+    for (int e = tid; e < 3 * D; e += threads)
+        at[e] = INT32_MAX;
+    sync();
+    constexpr int C = D / 8; /* 16 bytes of a row */
+    const __nv_bfloat16 *v = a.v + (int64_t)s.k0 * a.v_tok + head * a.v_head + tid % C * 8;
+    const int step = threads / C;
+    constexpr int N = 8; /* loads under way */
+    for (int j0 = tid / C; j0 < n; j0 += N * step) {
+        uint4 w[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) /* of the last key again, past it */
+            w[q] = __ldg(reinterpret_cast<const uint4 *>(v + min(j0 + q * step, n - 1) * a.v_tok));
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            if (odd2(w[q].x) | odd2(w[q].y) | odd2(w[q].z) | odd2(w[q].w)) {
+                const uint32_t x[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t b = x[e / 2] >> (16 * (e % 2)) & 0xFFFFu;
+                    if ((b & 0x7F80u) == 0x7F80u)
+                        atomicMin(at + (b & 0x7Fu ? 0 : b & 0x8000u ? 2 * D : D) + tid % C * 8 + e, min(j0 + q * step, n - 1));
+                }
+            }
+        }
+    }
+    sync();
+}
+/* what column d of a row that sees `seen` keys is by them: NaN, an infinity, or (0) its sum */
+template <int D>
+__device__ __forceinline__ float odd_value(const int *at, int d, int seen)
+{
+    const bool up = at[D + d] < seen, down = at[2 * D + d] < seen;
+    return at[d] < seen || (up && down) ? __int_as_float(0x7FFFFFFF) : up ? INFINITY : down ? -INFINITY : 0.f;
+}
 
 __device__ __forceinline__ float max_nan(float a, float b)
 {
@@ -442,10 +493,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
              *p_full = bars + 8, *o_done = bars + 10, *kv_full = bars + 12, *k_empty = kv_full + C::kStages,
              *v_empty = k_empty + C::kStages, *drained = v_empty + C::kStages;
     __shared__ uint32_t tmem_slot;
-    __shared__ Item s_item[2];
-    __shared__ int s_more[2];
+    /* Of four items: item k is published once all warps have begun item k - 2, so a place is filled
+     * again after both tiles are done with its item, however far one is ahead of the other; an
+     * item's fields are read again where they are needed, not held in registers. */
+    __shared__ Item s_item[4];
+    __shared__ int s_more[4];
     __shared__ Seq s_seqs[kSeqsHeld];
     __shared__ __align__(4) uint8_t s_low[2][4]; /* per tile and softmax warp: P has a low half */
+    __shared__ int s_odd[4][2]; /* and per tile: odd values that a row of it sees were taken out of V */
     __shared__ uint4 s_stage[8][32 * 4]; /* per softmax warp: 32 rows of 32 BF16 */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -501,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     it.last0 = max(it.first, min(n[0], stop)), it.last1 = max(it.first, min(n[1], stop));
                 }
                 wait(item_empty + (items & 1), (items / 2 + 1) & 1); /* first uses return at once */
-                s_more[items & 1] = more && alive, s_item[items & 1] = it;
+                s_more[items & 3] = more && alive, s_item[items & 3] = it;
+                s_odd[items & 3][0] = s_odd[items & 3][1] = 0;
                 mbar_arrive(item_full + (items & 1));
                 const int total = more ? max(it.last0, it.last1) - it.first : 0;
                 if (total > 0 && wait(q_empty, (queries + 1) & 1)) {
@@ -565,9 +621,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             int place = 0, queries = 0;
             uint32_t done = 0; /* bit i: parity of the tiles of keys that query tile i is through */
             for (int items = 0; wait(item_full + (items & 1), (items / 2) & 1); ++items) {
-                const bool more = s_more[items & 1];
-                const int first = s_item[items & 1].first;
-                const int n0 = s_item[items & 1].last0 - first, n1 = s_item[items & 1].last1 - first;
+                const bool more = s_more[items & 3];
+                const int first = s_item[items & 3].first;
+                const int n0 = s_item[items & 3].last0 - first, n1 = s_item[items & 3].last1 - first;
                 mbar_arrive(item_empty + (items & 1));
                 if (!more)
                     break;
@@ -635,15 +691,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         int place0 = 0;     /* ring place of the item's first */
         auto next = [&](int items) {
             warp_wait(item_full + (items & 1), (items / 2) & 1);
-            return alive && s_more[items & 1];
+            return alive && s_more[items & 3];
         };
         auto any = [&](bool p) { return any_of_tile(i, p); };
         item_loop(next, any, [&](int items) {
-            const Item it = s_item[items & 1];
+            const Item &it = s_item[items & 3];
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(item_empty + (items & 1));
-            const Span s = it.s;
+            const Span &s = it.s;
             const int done = (i ? it.last1 : it.last0) - it.first;
             /* Few registers live through this loop: 128 hold scores, and a spilled one would come
              * back from L2 (the tiles leave next to no L1). */
@@ -655,28 +711,45 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             /* tiles of keys from `plain` on have a place that some row does not see */
             const int plain = it.t0 + i * g.tok < s.q1 ? seen_of(g, s, it.t0 + i * g.tok) / kKeys - it.first : 0;
             float m = -INFINITY, l = 0.f; /* of the row */
-            bool odd = false;
 #pragma unroll 1
             for (int c = 0; c < done; ++c, ++turns) {
+                const bool masked = c >= plain;
+                /* V's odd values would reach rows that do not see them.  The first tile that multiplies
+                 * by this V takes them out for both: its weights are waited for before either product
+                 * (and tile 1 has masked places in no tile of keys where tile 0 has none). */
+                if (masked && (i == 0 || c >= it.last0 - it.first)) {
+                    const int p = place0 + c;
+                    warp_wait(kv_full + p % C::kStages, (p / C::kStages) & 1);
+                    uint4 *v = reinterpret_cast<uint4 *>(sv + p % C::kStages * C::kTileBytes);
+                    uint32_t zero = 0; /* 0 times every value, added up */
+#pragma unroll 8
+                    for (int e = r; e < C::kTileBytes / 16; e += kRows) {
+                        const uint4 w = v[e];
+                        zero = add_times0(w.x, add_times0(w.y, add_times0(w.z, add_times0(w.w, zero))));
+                    }
+                    if (odd2(zero)) {
+                        int key = kKeys; /* the first that has one */
+#pragma unroll 1
+                        for (int e = r; e < C::kTileBytes / 16; e += kRows) {
+                            const uint4 w = v[e];
+                            if (odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w)) {
+                                v[e] = make_uint4(without_odd2(w.x), without_odd2(w.y), without_odd2(w.z), without_odd2(w.w));
+                                key = min(key, e / 8 % kKeys);
+                            }
+                        }
+                        fence_proxy_async_smem(); /* the products read through the asynchronous proxy */
+                        for (int j = i; j < 2; ++j) /* the tiles that have a row that sees it */
+                            if (c < (j ? it.last1 : it.last0) - it.first &&
+                                (it.first + c) * kKeys + key < seen_of(g, s, min(s.q1, it.t0 + (j + 1) * g.tok) - 1))
+                                s_odd[items & 3][j] = 1;
+                    }
+                }
                 warp_wait(s_full + i, turns & 1);
                 tc_after();
-                const bool masked = c >= plain;
                 uint32_t x[kKeys];
 #pragma unroll
                 for (int q = 0; q < kKeys; q += 32)
                     tmem_ld32(ts + q, x + q);
-                if (masked) { /* V's odd values would reach rows that do not see them */
-                    const int p = place0 + c;
-                    warp_wait(kv_full + p % C::kStages, (p / C::kStages) & 1);
-                    const uint4 *v = reinterpret_cast<const uint4 *>(sv + p % C::kStages * C::kTileBytes);
-                    uint32_t any = 0;
-#pragma unroll 4
-                    for (int e = r; e < C::kTileBytes / 16; e += kRows) {
-                        const uint4 w = v[e];
-                        any |= odd2(w.x) | odd2(w.y) | odd2(w.z) | odd2(w.w);
-                    }
-                    odd |= any != 0;
-                }
 #pragma unroll
                 for (int q = 0; q < kKeys; q += 32)
                     tmem_ld_wait(x + q);
@@ -757,13 +830,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 l += a + b;
             }
             place0 += max(it.last0, it.last1) - it.first;
-            const bool bad = any(odd);
             const int tile0 = it.t0 + i * g.tok, t = tile0 + r / g.group, hq = it.head * g.group + r % g.group;
             const bool live = r < g.group * g.tok && t < s.q1;
             if (done > 0) {
                 warp_wait(o_done + i, (turns + 1) & 1);
                 tc_after();
             }
+            const bool odd = done > 0 && s_odd[items & 3][i];
             if (it.cuts > 1) {
                 uint4 *part = reinterpret_cast<uint4 *>(g.part) + ((int64_t)it.slot * 2 + i) * (D / 4) * kRows + r;
                 float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + i * kRows + r;
@@ -780,8 +853,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
                 ml[0] = m, ml[(int64_t)g.sms * kSlotRows] = l;
                 if (r == 0)
-                    reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = bad;
-            } else if (!bad) {
+                    reinterpret_cast<int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2))[2 * it.slot + i] = odd;
+            } else {
                 const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
                 /* 32 columns a time through shared memory: a thread's own row would be a line of its
                  * own in every store, four threads a row make whole sectors (12 prompts 114 -> 112 us) */
@@ -831,11 +904,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
                 if (live && g.a.lse)
                     g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-            } else {
-                for (int k = wl; k < g.group * g.tok; k += 4) {
-                    const int tk = tile0 + k / g.group;
-                    if (tk < s.q1)
-                        plain_row<D>(g.a, s, tk, it.head * g.group + k % g.group, lane);
+                if (any(odd)) {
+                    int *at_key = reinterpret_cast<int *>(s_stage[4 * i]); /* of the tile's four warps; 3 D ints */
+                    first_odd<D>(g.a, s, it.head, seen_of(g, s, min(s.q1, tile0 + g.tok) - 1), at_key, r, kRows,
+                                 [&] { any(false); });
+                    if (live && l > 0.f && l < INFINITY)
+                        for (int d = 0; d < D; ++d) {
+                            const float x = odd_value<D>(at_key, d, seen_of(g, s, t));
+                            if (x != 0.f)
+                                g.a.o[t * g.a.o_tok + hq * g.a.o_head + d] = __float2bfloat16_rn(x);
+                        }
                 }
             }
             tc_before(); /* O is read: the next item's products may write it once this warp's weights are in */
@@ -852,11 +930,11 @@ constexpr int kJoinRows = 32; /* divides a tile's 128 */
 /* Joins the parts of blocks whose keys were cut: 32 rows a block, a row a lane, an eighth of
  * its columns a warp (the parts lie by row within four columns, so loads are whole lines). */
 template <int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args g)
+__global__ void __launch_bounds__(256, 4) attn_join_kernel(const __grid_constant__ Args g)
 {
     __shared__ Seq s_seqs[kSeqsHeld];
     __shared__ Item s_item;
-    __shared__ int s_ok;
+    __shared__ int s_ok, s_first[3 * D];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int b = threadIdx.x; b < min(kSeqsHeld, g.a.seqs); b += 256)
         s_seqs[b] = seq_of(g, b);
@@ -877,17 +955,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     constexpr int C4 = D / 32; /* fours of columns a thread */
     const int row0 = blockIdx.y * kJoinRows, i = row0 / kRows, r = row0 % kRows + lane;
     const float *ml = g.part + (int64_t)g.sms * kSlotRows * D + (int64_t)it.slot * kSlotRows + row0 + lane;
-    const int *bads = reinterpret_cast<const int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2)) + 2 * it.slot + i;
+    const int *odds = reinterpret_cast<const int *>(g.part + (int64_t)g.sms * kSlotRows * (D + 2)) + 2 * it.slot + i;
     const float4 *part = reinterpret_cast<const float4 *>(g.part) + (((int64_t)it.slot * 2 + i) * (D / 4) + warp * C4) * kRows + r;
-    const bool bad = __any_sync(0xFFFFFFFFu, lane < it.cuts && bads[2 * lane]);
-    if (bad) {
-        for (int k = warp; k < kJoinRows; k += 8) {
-            const int row = row0 % kRows + k, t = it.t0 + i * g.tok + row / g.group;
-            if (row < g.group * g.tok && t < it.s.q1)
-                plain_row<D>(g.a, it.s, t, it.head * g.group + row % g.group, lane);
-        }
-        return;
-    }
+    const bool odd = __any_sync(0xFFFFFFFFu, lane < it.cuts && odds[2 * lane]);
     float m = -INFINITY, l = 0.f;
 #pragma unroll 8
     for (int c = 0; c < it.cuts; ++c)
@@ -908,7 +978,23 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
         }
     }
     const int t = it.t0 + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
-    if (r >= g.group * g.tok || t >= it.s.q1)
+    const bool live = r < g.group * g.tok && t < it.s.q1;
+    if (__syncthreads_or(odd)) {
+        first_odd<D>(g.a, it.s, it.head, seen_of(g, it.s, min(it.s.q1, it.t0 + (i + 1) * g.tok) - 1), s_first, threadIdx.x,
+                     256, [] { __syncthreads(); });
+        if (live && l > 0.f && l < INFINITY) {
+            const int seen = seen_of(g, it.s, t), d = warp * C4 * 4;
+#pragma unroll
+            for (int e = 0; e < C4; ++e) {
+                auto set = [&](float &x, int at) {
+                    const float z = odd_value<D>(s_first, d + at, seen);
+                    x = z != 0.f ? z : x;
+                };
+                set(o[e].x, 4 * e), set(o[e].y, 4 * e + 1), set(o[e].z, 4 * e + 2), set(o[e].w, 4 * e + 3);
+            }
+        }
+    }
+    if (!live)
         return;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     __nv_bfloat16 *out = g.a.o + t * g.a.o_tok + hq * g.a.o_head + warp * C4 * 4;

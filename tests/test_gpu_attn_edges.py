@@ -89,3 +89,52 @@ def test_evict_past_the_keys_held(length, page):
     assert bool((wo[0, 0, n:] == -1).all()) and bool((po[0, 0, n:] == -1).all())
     for x, y in zip(before, after):
         assert torch.equal(bits(y[:n]), bits(x[src])) and torch.equal(bits(y[n:]), bits(x[n:]))
+
+
+def gpu_ms(f, n=3):
+    f()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    for _ in range(n):
+        f()
+    end.record()
+    end.synchronize()
+    return begin.elapsed_time(end) / n
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(4096, 4096), (100, 20000)])
+def test_prompt_masked_values_cost_little(dim, lq, lk):
+    """Values that are not finite past the last sequence, and at its last key: a look at V (its
+    bytes are a small part of the call) for the blocks that meet them, and no more."""
+    g = gen(dim + lq)
+    q, k, v = randn(lq, 8, dim, g=g), randn(lk + 64, 8, dim, g=g), randn(lk + 64, 8, dim, g=g)
+    a = (cu([lq]), cu([lk]))
+    clean = gpu_ms(lambda: A().attn_prompt(q, k, v, *a))
+    want = A().attn_prompt(q, k, v, *a)[0]
+    v[lk - 1:] = float("nan")
+    bad = gpu_ms(lambda: A().attn_prompt(q, k, v, *a))
+    got = A().attn_prompt(q, k, v, *a)[0]
+    assert kernel_error() == 0
+    assert bool(got[-1].isnan().all()) and torch.equal(got[:-1], want[:-1])
+    assert bad <= 4 * clean + 0.2, f"{bad:.3f} ms against {clean:.3f}"
+
+
+def test_prompt_masked_values_stay_out_of_very_long_rows():
+    """300000 keys, more blocks than are cut: nothing a block does for odd values may outlast the
+    bounded waits of its other warps."""
+    g = gen(77)
+    n, m, heads, dim = 600, 300000, 32, 64
+    q = randn(n, heads, dim, g=g)
+    k, v = (randn(m + 100, heads, dim, g=g) for _ in range(2))
+    v[m - 1], v[m:] = float("nan"), float("inf")
+    o, lse = A().attn_prompt(q, k, v, cu([n]), cu([m]))
+    torch.cuda.synchronize()
+    assert kernel_error() == 0
+    assert bool(o[-1].isnan().all())
+    for h in (0, heads - 1):
+        rows = slice(0, n, 13)
+        want, bound, z, bz = prompt_reference(q[:, h:h + 1], k[:m, h:h + 1], v[:m, h:h + 1].nan_to_num(), [n], [m], True,
+                                              dim ** -0.5)
+        within(o[:-1, h:h + 1][rows], want[:-1][rows], bound[:-1][rows], "o")
+        within(lse[h:h + 1, :-1], z[:, :-1], bz[:, :-1], "lse")
