@@ -22,7 +22,9 @@
  * Masked scores are replaced, never added to, and a masked weight is 0; a NaN or an
  * infinity in V would still reach other rows as 0 * NaN, so tiles with masked places
  * are looked through and such values taken out of shared memory.  Rows that do see one
- * get it afterwards: o of a column is then known without a product.
+ * get it afterwards: o of a column is then known without a product.  So it is with an
+ * infinity among other tiles' values, whose products make a NaN of it wherever a weight
+ * or the half that BF16 drops is 0 or negative: rows that come out not finite are looked at.
  *
  * Floor: exponentials (16 a clock and SM) and the tensor cores take the same time at
  * D = 128, 2048 clocks for two tiles of queries by one of keys.  Bound: a tile's softmax
@@ -80,6 +82,7 @@ __device__ __forceinline__ void plain_row(const GlintAttnPrompt &a, const Span &
     const int h = hq / (a.heads / a.kv_heads);
     const int seen = a.causal ? min(s.k1 - s.k0, t - s.q0 + 1 + (s.k1 - s.k0) - (s.q1 - s.q0)) : s.k1 - s.k0;
     float q[D / 32], o[D / 32] = {}, m = -INFINITY, l = 0.f;
+    float odd[D / 32] = {}; /* infinities and NaN among the values seen, added up: a weight may be 0 in f32 */
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
         q[i] = __bfloat162float(a.q[t * a.q_tok + hq * a.q_head + lane + 32 * i]);
@@ -95,14 +98,18 @@ __device__ __forceinline__ void plain_row(const GlintAttnPrompt &a, const Span &
         const float keep = m == -INFINITY ? 0.f : expf(m - top), p = x == -INFINITY ? 0.f : expf(x - top);
         l = l * keep + p;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-            o[i] = fmaf(p, __bfloat162float(v[32 * i]), o[i] * keep);
+        for (int i = 0; i < D / 32; ++i) {
+            const float y = __bfloat162float(v[32 * i]);
+            const bool finite = fabsf(y) < INFINITY;
+            o[i] = fmaf(p, finite ? y : 0.f, o[i] * keep);
+            odd[i] += finite ? 0.f : y;
+        }
         m = top;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
-        a.o[t * a.o_tok + hq * a.o_head + lane + 32 * i] = __float2bfloat16_rn(o[i] * inv);
+        a.o[t * a.o_tok + hq * a.o_head + lane + 32 * i] = __float2bfloat16_rn(l > 0.f && !(odd[i] == 0.f) ? odd[i] : o[i] * inv);
     if (a.lse && lane == 0)
         a.lse[(int64_t)hq * a.q_tokens + t] = l == 0.f ? -INFINITY : m + logf(l);
 }
@@ -721,13 +728,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     const int p = place0 + c;
                     warp_wait(kv_full + p % C::kStages, (p / C::kStages) & 1);
                     uint4 *v = reinterpret_cast<uint4 *>(sv + p % C::kStages * C::kTileBytes);
-                    uint32_t zero = 0; /* 0 times every value, added up */
+                    uint32_t zero[4] = {}; /* 0 times every value, added up */
 #pragma unroll 8
                     for (int e = r; e < C::kTileBytes / 16; e += kRows) {
                         const uint4 w = v[e];
-                        zero = add_times0(w.x, add_times0(w.y, add_times0(w.z, add_times0(w.w, zero))));
+                        zero[0] = add_times0(w.x, zero[0]), zero[1] = add_times0(w.y, zero[1]);
+                        zero[2] = add_times0(w.z, zero[2]), zero[3] = add_times0(w.w, zero[3]);
                     }
-                    if (odd2(zero)) {
+                    if (odd2(zero[0]) | odd2(zero[1]) | odd2(zero[2]) | odd2(zero[3])) {
                         int key = kKeys; /* the first that has one */
 #pragma unroll 1
                         for (int e = r; e < C::kTileBytes / 16; e += kRows) {
@@ -859,6 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 /* 32 columns a time through shared memory: a thread's own row would be a line of its
                  * own in every store, four threads a row make whole sectors (12 prompts 114 -> 112 us) */
                 uint4 *stage = s_stage[warp];
+                uint32_t zero[4] = {}; /* 0 times the row's values, added up */
                 int64_t at[4]; /* of rows lane / 4 + 8 k, 16 bytes at lane % 4 */
                 uint32_t mine = 0;
 #pragma unroll
@@ -879,6 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         const __nv_bfloat162 h = __floats2bfloat162_rn(done > 0 ? __uint_as_float(o[2 * e]) * inv : 0.f,
                                                                        done > 0 ? __uint_as_float(o[2 * e + 1]) * inv : 0.f);
                         w[e] = *reinterpret_cast<const uint32_t *>(&h);
+                        zero[e % 4] = add_times0(w[e], zero[e % 4]);
                     }
                     if (g.vec) {
                         __syncwarp();
@@ -904,11 +914,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
                 if (live && g.a.lse)
                     g.a.lse[(int64_t)hq * g.a.q_tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-                if (any(odd)) {
+                const bool seen_odd = live && l > 0.f && l < INFINITY; /* a NaN score is the whole row's */
+                if (any(odd || (seen_odd && (odd2(zero[0]) | odd2(zero[1]) | odd2(zero[2]) | odd2(zero[3]))))) {
                     int *at_key = reinterpret_cast<int *>(s_stage[4 * i]); /* of the tile's four warps; 3 D ints */
                     first_odd<D>(g.a, s, it.head, seen_of(g, s, min(s.q1, tile0 + g.tok) - 1), at_key, r, kRows,
                                  [&] { any(false); });
-                    if (live && l > 0.f && l < INFINITY)
+                    if (seen_odd)
                         for (int d = 0; d < D; ++d) {
                             const float x = odd_value<D>(at_key, d, seen_of(g, s, t));
                             if (x != 0.f)
@@ -978,11 +989,15 @@ __global__ void __launch_bounds__(256, 4) attn_join_kernel(const __grid_constant
         }
     }
     const int t = it.t0 + i * g.tok + r / g.group, hq = it.head * g.group + r % g.group;
-    const bool live = r < g.group * g.tok && t < it.s.q1;
-    if (__syncthreads_or(odd)) {
+    const bool live = r < g.group * g.tok && t < it.s.q1, seen_odd = live && l > 0.f && l < INFINITY;
+    float zero = 0.f; /* 0 times the thread's values, added up */
+#pragma unroll
+    for (int e = 0; e < C4; ++e)
+        zero = fmaf(0.f, o[e].x, fmaf(0.f, o[e].y, fmaf(0.f, o[e].z, fmaf(0.f, o[e].w, zero))));
+    if (__syncthreads_or(odd || (seen_odd && zero != zero))) {
         first_odd<D>(g.a, it.s, it.head, seen_of(g, it.s, min(it.s.q1, it.t0 + (i + 1) * g.tok) - 1), s_first, threadIdx.x,
                      256, [] { __syncthreads(); });
-        if (live && l > 0.f && l < INFINITY) {
+        if (seen_odd) {
             const int seen = seen_of(g, it.s, t), d = warp * C4 * 4;
 #pragma unroll
             for (int e = 0; e < C4; ++e) {

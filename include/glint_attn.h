@@ -12,7 +12,8 @@
  * query head h reads key/value head h / (heads / kv_heads).  Strides are in elements,
  * a head's head_dim values are contiguous.  A row whose mask leaves no key gives o = 0
  * and lse = -inf.  Values in masked places (NaN and infinities included) never reach
- * a result.  lse is the natural log of the sum of exponentials of the scaled scores.
+ * a result; an infinity in v that a row sees is that column of its o, NaN where it sees
+ * a NaN or infinities of both signs.  lse is the natural log of the sum of exponentials of the scaled scores.
  *
  * Return codes: 0 ok, -1 bad argument, -3 launch failure, -6 (GLINT_ERR_UNSUPPORTED)
  * a head_dim or page_size outside the lists here.  All calls are asynchronous on

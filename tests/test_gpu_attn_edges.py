@@ -138,3 +138,42 @@ def test_prompt_masked_values_stay_out_of_very_long_rows():
                                               dim ** -0.5)
         within(o[:-1, h:h + 1][rows], want[:-1][rows], bound[:-1][rows], "o")
         within(lse[h:h + 1, :-1], z[:, :-1], bz[:, :-1], "lse")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,lq,lk", [(64, 32, [700, 90], [700, 90]), (4, 2, [150], [2500]), (5, 1, [33], [33]),
+                                            (16, 16, [1500], [1700])])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("plain", [False, True])
+def test_prompt_infinities_that_rows_see(dim, heads, kv, lq, lk, causal, plain):
+    """In tiles of keys without a masked place and with one, where a weight is large, small and 0 in
+    f32; the other columns are as they are without."""
+    g = gen(dim + sum(lk))
+    n, m = sum(lq), sum(lk)
+    q, k, v = randn(n, heads, dim, g=g, scale=6), randn(m, kv, dim, g=g), randn(m, kv, dim, g=g)
+    if plain:
+        v = torch.cat([v, v[..., :1]], -1)[..., :dim]  # rows that are not 16-byte aligned
+    want = prompt_reference(q, k, v, lq, lk, causal, dim ** -0.5)
+    marks = torch.zeros(3, m, dim, dtype=torch.bool, device="cuda")  # NaN, +inf, -inf by key and column
+    for key, column, kind in ((3, 5, 1), (20, 5, 2), (7, 7, 2), (30, 9, 0), (m - 1, 0, 1), (m - 40 if m > 80 else 31, 33, 2),
+                              (0, 63, 1), (m // 2, dim - 2, 1), (m // 2 + 1, dim - 2, 1)):
+        marks[kind, key, column] = True
+    for kind, value in enumerate((float("nan"), float("inf"), -float("inf"))):
+        v[marks[kind][:, None].expand(-1, kv, -1)] = value
+    o, lse = A().attn_prompt(q, k, v, cu(lq), cu(lk), causal=causal)
+    assert kernel_error() == 0
+    expect = want[0].clone()
+    at = kat = 0
+    for a, b in zip(lq, lk):
+        seen = torch.arange(a, device="cuda") + 1 + b - a if causal else torch.full((a,), b, device="cuda")
+        counts = torch.cat([torch.zeros(3, 1, dim, device="cuda"), marks[:, kat:kat + b].float().cumsum(1)], 1)
+        some = counts[:, seen.clamp(0, b)] > 0
+        x = torch.where(some[0] | (some[1] & some[2]), float("nan"),
+                        torch.where(some[1], float("inf"), torch.where(some[2], -float("inf"), 0.0)))[:, None]
+        expect[at:at + a] = torch.where(x == 0, expect[at:at + a], x.expand(-1, heads, -1).double())
+        at, kat = at + a, kat + b
+    odd = ~expect.isfinite()
+    assert bool(odd.any()) and torch.equal(o.isfinite(), ~odd)
+    assert bool(((o.double() == expect) | (o.isnan() & expect.isnan()))[odd].all())
+    within(torch.where(odd, 0.0, o.double()), torch.where(odd, 0.0, expect), want[1], "o")
+    within(lse, want[2], want[3], "lse")
