@@ -84,7 +84,8 @@ __device__ __forceinline__ int length_of(const Args &g, int b)
 {
     return min(max(g.a.lens[b], 0), g.a.max_pages * g.c.page_size);
 }
-__device__ __forceinline__ int tiles_of(const Args &g, int b) { return (length_of(g, b) + kTile - 1) / kTile; }
+/* a length may be 2^31 - 16: no signed sum goes past it, here and below */
+__device__ __forceinline__ int tiles_of(const Args &g, int b) { return (int)(((uint32_t)length_of(g, b) + kTile - 1) / kTile); }
 
 /* All segments in one row (sequence after sequence), each as long as kJoin plus its
  * tiles, cut into equal ranges over the workers (kGroup warps each): sequences of any mix
@@ -547,7 +548,7 @@ __device__ __forceinline__ uint32_t fetch_issue(const Args &g, const Fetch &f, u
                reinterpret_cast<const uint8_t *>(meta) + (u ? r1 : r0) * (D / 16) + m * 16 - u * (C::kMeta / 2));
     }
     uint32_t v = ((half & 1u) ? 0xFFFFu : 0u) | ((half & 2u) ? 0xFFFF0000u : 0u);
-    if (t0 + kTile > f.len)
+    if ((uint32_t)t0 + kTile > (uint32_t)f.len)
         v &= (1u << (f.len - t0)) - 1u; /* len > t0 */
     return v;
 }
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) kv4_attn_kernel(const
             copies_wait<C::kStages - 1>();
             __syncwarp();
             const uint32_t v = valid[0], stage = ring + slot * C::kStage;
-            if (v == 0xFFFFFFFFu && tile * kTile + kTile <= len - g.a.rows + 1)
+            if (v == 0xFFFFFFFFu && (uint32_t)tile * kTile + kTile <= (uint32_t)max(len - g.a.rows + 1, 0))
                 tile_step<D, NT, SCORE, true>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);
             else
                 tile_step<D, NT, SCORE, false>(g, q, st, stage, tile * kTile, v, scale2, score, chunk, lane);

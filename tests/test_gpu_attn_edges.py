@@ -2,13 +2,15 @@
 whose keys are cut over the SMs, values that are not finite at such lengths, eviction with more
 slots than a CTA's shared memory holds keys.  References and bounds are that file's."""
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_gpu_attn import (A, bits, check_prompt, cu, evict_reference, gen, gpu, kernel_error,  # noqa: E402,F401
-                           prompt_reference, randn, within)
+                           prompt_reference, quantise, randn, values, within)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
@@ -177,3 +179,33 @@ def test_prompt_infinities_that_rows_see(dim, heads, kv, lq, lk, causal, plain):
     assert bool(((o.double() == expect) | (o.isnan() & expect.isnan()))[odd].all())
     within(torch.where(odd, 0.0, o.double()), torch.where(odd, 0.0, expect), want[1], "o")
     within(lse, want[2], want[3], "lse")
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 16, 2 ** 31 - 29])
+def test_cache_attention_longest_sequence(length):
+    """As many slots as a table of 16-slot pages can name, all of them in one page: the softmax of that
+    page's 16 over again, lse the log of the pages more.  A warp of 2368 adds four weights a tile of
+    32 to its sums, each addition 2^-23 of the sum off at most: 2^28 / 2368 * 2^-23 in all."""
+    g = gen(31)
+    pages, dim = 2 ** 27 - 1, 64
+    cache = A().KV4Cache.empty(2, 1, dim, 16)
+    k, v = randn(16, 1, dim, g=g), randn(16, 1, dim, g=g)
+    slots = torch.arange(16, 32, dtype=torch.int32, device="cuda")
+    A().kv4_append(cache, k, v, slots)
+    table = torch.ones(1, pages, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+    q = randn(1, 1, 2, dim, g=g)
+    weight = torch.empty(1, 1, pages * 16, device="cuda")
+    o, lse = A().kv4_attn(q, cache, table, lens, weight_out=weight)
+    torch.cuda.synchronize()
+    kd, vd = (values(*quantise(x), dtype=torch.float64)[:, 0] for x in (k, v))
+    off = 2.0 ** 28 / 2368 * 2.0 ** -23
+    total = torch.zeros(16, dtype=torch.float64, device="cuda")
+    for h in range(2):
+        s = kd @ q[0, 0, h].double() * dim ** -0.5
+        p = torch.softmax(s, 0)
+        total += p / pages
+        assert bool(((o[0, 0, h].double() - p @ vd).abs() <= (2 * off + 2.0 ** -8) * (p @ vd.abs() + 1)).all())
+        assert abs(float(lse[0, h, 0]) - float(torch.logsumexp(s, 0)) - math.log(pages)) <= 2 * off
+    for at in (0, 2 ** 30, 2 ** 31 - 48):
+        assert bool(((weight[0, 0, at:at + 16].double() / total - 1).abs() <= 4 * off).all())
