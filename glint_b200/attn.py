@@ -124,8 +124,7 @@ def _prompt_work(dev: int, q_tokens: int, k_tokens: int, heads: int, kv_heads: i
 def _attn_work(dev: int, kv_heads: int, page_size: int, head_dim: int, seqs: int, rows: int, heads: int,
                max_pages: int, weights: bool) -> int:
     cache = _pack_cache(16, 16, 16, 16, 1, kv_heads, page_size, head_dim)  # sizes are all that counts here
-    return max(0, _c().attn_work(cache, _pack_attn(*[0] * 6, 1 if weights else 0, 0, *[0] * 4, seqs, rows, heads,
-                                                   max_pages, 1.0)))
+    return _c().attn_work(cache, _pack_attn(*[0] * 6, 1 if weights else 0, 0, *[0] * 4, seqs, rows, heads, max_pages, 1.0))
 
 
 def _raw(like: torch.Tensor, stream: Optional[torch.cuda.Stream], *others) -> int:
@@ -170,6 +169,11 @@ def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[Optional[
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
+def _want16(t: torch.Tensor, name: str) -> None:
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+
+
 def _head_dim(d: int) -> None:
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, not {d}")
@@ -192,7 +196,7 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     _want(k, "k", torch.bfloat16, (None, None, D), dense=False)
     Tk, Hk = k.shape[0], k.shape[1]
     _want(v, "v", torch.bfloat16, (Tk, Hk, D), dense=False)
-    if Hk < 1 or H % Hk:
+    if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({Hk})")
     _want(cu_q, "cu_q", torch.int32, (None,))
     if cu_k is None:
@@ -283,10 +287,12 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor]
         k_out = _empty(slots, shape, torch.bfloat16, stream)
     else:
         _want(k_out, "k_out", torch.bfloat16, shape)
+        _want16(k_out, "k_out")
     if v_out is None:
         v_out = _empty(slots, shape, torch.bfloat16, stream)
     else:
         _want(v_out, "v_out", torch.bfloat16, shape)
+        _want16(v_out, "v_out")
     _check(_c().read(cache._c, slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
                      _raw(slots, stream, k_out, v_out, cache.k_code)), "glint_kv4_read_stream")
     return k_out, v_out
@@ -312,12 +318,15 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
         raise ValueError(f"rows ({R}) times query heads a kv head must be 1 to 256")
     _want(table, "table", torch.int32, (B, None))
     _want(lens, "lens", torch.int32, (B,))
+    P = table.shape[1]
+    if P < 1 or P * cache.page_size > 2 ** 31 - 1:
+        raise ValueError(f"table must name between 1 and 2**31 - 1 slots a sequence, not {P} pages of {cache.page_size}")
     wide = 0
     if weight_out is not None:
         _want(weight_out, "weight_out", torch.float32, (B, cache.kv_heads, None))
         wide = weight_out.shape[2]
-        if wide < table.shape[1] * cache.page_size:
-            raise ValueError(f"weight_out must have {table.shape[1] * cache.page_size} slots or more, not {wide}")
+        if wide < P * cache.page_size:
+            raise ValueError(f"weight_out must have {P * cache.page_size} slots or more, not {wide}")
         if weight is not None:
             _want(weight, "weight", torch.float32, (B, cache.kv_heads, wide))
     elif weight is not None:
@@ -326,17 +335,21 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
         out = _empty(q, (B, R, H, D), torch.bfloat16, stream)
     else:
         _want(out, "out", torch.bfloat16, (B, R, H, D))
+        _want16(out, "out")
     if lse is None:
         lse = _empty(q, (B, H, R), torch.float32, stream)
     else:
         _want(lse, "lse", torch.float32, (B, H, R))
     raw = _raw(q, stream, cache.k_code, table, lens, weight, weight_out, out, lse)
-    work = _empty(q, (_attn_work(q.get_device(), cache.kv_heads, cache.page_size, D, B, R, H, table.shape[1],
-                                 weight_out is not None),), torch.uint8, stream)
+    n = _attn_work(q.get_device(), cache.kv_heads, cache.page_size, D, B, R, H, P, weight_out is not None)
+    if n < 0:
+        raise ValueError(f"{B} sequences of up to {P} pages, {cache.kv_heads} kv heads and {H // cache.kv_heads * R} rows a kv "
+                         "head are more than one call takes")
+    work = _empty(q, (n,), torch.uint8, stream)
     qs = q.stride()
     a = _pack_attn(q.data_ptr(), out.data_ptr(), lse.data_ptr(), table.data_ptr(), lens.data_ptr(),
                    0 if weight is None else weight.data_ptr(), 0 if weight_out is None else weight_out.data_ptr(),
-                   work.data_ptr(), qs[0], qs[1], qs[2], wide, B, R, H, table.shape[1],
+                   work.data_ptr(), qs[0], qs[1], qs[2], wide, B, R, H, P,
                    D ** -0.5 if scale is None else scale)
     _check(_c().attn(cache._c, a, raw), "glint_kv4_attn_stream")
     return out, lse
@@ -362,8 +375,8 @@ def kv4_evict(cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, weight: 
     _want(weight, "weight", torch.float32, (B, cache.kv_heads, None))
     wide = weight.shape[2]
     _want(pos, "pos", torch.int32, (B, cache.kv_heads, wide))
-    if budget < 1 or recent < 0 or recent > budget:
-        raise ValueError("budget must be 1 or more and recent between 0 and budget")
+    if not 1 <= budget < 2 ** 31 or recent < 0 or recent > budget:
+        raise ValueError("budget must be 1 or more (in 31 bits) and recent between 0 and budget")
     if P < 1 or P * cache.page_size > min(wide, 524288):
         raise ValueError(f"table has room for {P * cache.page_size} slots: weight must cover them, 524288 at most")
     kept = _empty(table, (B, cache.kv_heads, budget), torch.int32, stream)

@@ -209,3 +209,34 @@ def test_cache_attention_longest_sequence(length):
         assert abs(float(lse[0, h, 0]) - float(torch.logsumexp(s, 0)) - math.log(pages)) <= 2 * off
     for at in (0, 2 ** 30, 2 ** 31 - 48):
         assert bool(((weight[0, 0, at:at + 16].double() / total - 1).abs() <= 4 * off).all())
+
+
+def test_refusals_of_layouts_and_sizes():
+    """What the C entry points answer with -1 is a ValueError here, and nothing has run."""
+    attn = A()
+    g = gen(40)
+    cache = attn.KV4Cache.empty(4, 2, 128, 16)
+    q = randn(3, 1, 4, 128, g=g)
+    table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    lens = torch.ones(3, dtype=torch.int32, device="cuda")
+    shifted = torch.empty(q.numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view(q.shape)
+    for bad in (dict(out=shifted), dict(table=table[:, :0])):
+        with pytest.raises(ValueError):
+            attn.kv4_attn(**{**dict(q=q, cache=cache, table=table, lens=lens), **bad})
+    many = 40000  # sequences times kv heads past a grid's second dimension
+    with pytest.raises(ValueError):
+        attn.kv4_attn(randn(many, 1, 2, 128, g=g), cache, table[:1].expand(many, -1).contiguous(), lens[:1].expand(many).contiguous())
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    rows = torch.empty(3 * 2 * 128 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(3, 2, 128)
+    for bad in (dict(k_out=rows), dict(v_out=rows)):
+        with pytest.raises(ValueError):
+            attn.kv4_read(cache, slots, **bad)
+    pos = torch.zeros(3, 2, 32, dtype=torch.int32, device="cuda")
+    wo, po = torch.zeros(3, 2, 32, device="cuda"), torch.zeros_like(pos)
+    for bad in (dict(budget=2 ** 31),):
+        with pytest.raises(ValueError):
+            attn.kv4_evict(**{**dict(cache=cache, table=table, lens=lens, weight=wo.clone(), pos=pos, seen=lens, budget=4,
+                                     recent=0, weight_out=wo, pos_out=po), **bad})
+    k = randn(3, 2, 128, g=g)
+    with pytest.raises(ValueError):
+        attn.attn_prompt(q[:, 0, :0], k, k, cu([3]))
