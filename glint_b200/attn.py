@@ -174,6 +174,11 @@ def _want16(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be 16-byte aligned")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two contiguous tensors of one size."""
+    return abs(a.data_ptr() - b.data_ptr()) < a.numel() * a.element_size()
+
+
 def _head_dim(d: int) -> None:
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, not {d}")
@@ -329,6 +334,8 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.
             raise ValueError(f"weight_out must have {P * cache.page_size} slots or more, not {wide}")
         if weight is not None:
             _want(weight, "weight", torch.float32, (B, cache.kv_heads, wide))
+            if weight.data_ptr() != weight_out.data_ptr() and _overlap(weight, weight_out):
+                raise ValueError("weight_out must be weight or apart from it")
     elif weight is not None:
         raise ValueError("weight needs weight_out")
     if out is None:
@@ -383,8 +390,8 @@ def kv4_evict(cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, weight: 
     new_lens = _empty(table, (B,), torch.int32, stream)
     _want(weight_out, "weight_out", torch.float32, weight.shape)
     _want(pos_out, "pos_out", torch.int32, pos.shape)
-    if weight_out.data_ptr() == weight.data_ptr() or pos_out.data_ptr() == pos.data_ptr():
-        raise ValueError("weight_out and pos_out must not be weight and pos")
+    if _overlap(weight_out, weight) or _overlap(pos_out, pos):
+        raise ValueError("weight_out and pos_out must not be weight and pos, nor overlap them")
     e = _pack_evict(table.data_ptr(), lens.data_ptr(), weight.data_ptr(), pos.data_ptr(), seen.data_ptr(), kept.data_ptr(),
                new_lens.data_ptr(), weight_out.data_ptr(), pos_out.data_ptr(), wide, B, P, budget, recent)
     _check(_c().evict(cache._c, e, _raw(table, stream, cache.k_code, lens, weight, pos, seen, weight_out, pos_out)),

@@ -220,7 +220,9 @@ def test_refusals_of_layouts_and_sizes():
     table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
     lens = torch.ones(3, dtype=torch.int32, device="cuda")
     shifted = torch.empty(q.numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view(q.shape)
-    for bad in (dict(out=shifted), dict(table=table[:, :0])):
+    flat = torch.zeros(3 * 2 * 32 + 8, device="cuda")
+    near = (flat[:-8].view(3, 2, 32), flat[8:].view(3, 2, 32))
+    for bad in (dict(out=shifted), dict(table=table[:, :0]), dict(weight=near[0], weight_out=near[1])):
         with pytest.raises(ValueError):
             attn.kv4_attn(**{**dict(q=q, cache=cache, table=table, lens=lens), **bad})
     many = 40000  # sequences times kv heads past a grid's second dimension
@@ -233,10 +235,26 @@ def test_refusals_of_layouts_and_sizes():
             attn.kv4_read(cache, slots, **bad)
     pos = torch.zeros(3, 2, 32, dtype=torch.int32, device="cuda")
     wo, po = torch.zeros(3, 2, 32, device="cuda"), torch.zeros_like(pos)
-    for bad in (dict(budget=2 ** 31),):
+    for bad in (dict(budget=2 ** 31), dict(weight=near[0], weight_out=near[1])):
         with pytest.raises(ValueError):
-            attn.kv4_evict(**{**dict(cache=cache, table=table, lens=lens, weight=wo.clone(), pos=pos, seen=lens, budget=4,
+            attn.kv4_evict(**{**dict(cache=cache, table=table, lens=lens, weight=near[0], pos=pos, seen=lens, budget=4,
                                      recent=0, weight_out=wo, pos_out=po), **bad})
     k = randn(3, 2, 128, g=g)
     with pytest.raises(ValueError):
         attn.attn_prompt(q[:, 0, :0], k, k, cu([3]))
+
+
+def test_calls_without_a_sequence():
+    attn = A()
+    cache = attn.KV4Cache.empty(4, 2, 128, 16)
+    none = dict(device="cuda")
+    table = torch.zeros(0, 2, dtype=torch.int32, **none)
+    lens = torch.zeros(0, dtype=torch.int32, **none)
+    weight, pos = torch.zeros(0, 2, 32, **none), torch.zeros(0, 2, 32, dtype=torch.int32, **none)
+    o, lse = attn.kv4_attn(torch.zeros(0, 1, 4, 128, dtype=torch.bfloat16, **none), cache, table, lens, weight_out=weight)
+    assert o.shape == (0, 1, 4, 128) and lse.shape == (0, 4, 1)
+    kept, new = attn.kv4_evict(cache, table, lens, weight, pos, lens, 7, weight_out=weight.clone(), pos_out=pos.clone())
+    assert kept.shape == (0, 2, 7) and new.shape == (0,)
+    rows = torch.zeros(0, 2, 128, dtype=torch.bfloat16, **none)
+    attn.kv4_append(cache, rows, rows, lens)
+    assert attn.kv4_read(cache, lens)[0].shape == (0, 2, 128)
