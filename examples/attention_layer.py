@@ -30,7 +30,8 @@ class AttentionLayer:
     wqkv, wo: (hole, plug, absmax) planes of the [(heads + 2 kv_heads) * head_dim, hidden] and
     [hidden, heads * head_dim] weights.  Each sequence may hold `capacity` slots; beyond
     `budget` (plus `slack`, so that eviction runs once in `slack` steps) the slots of
-    least weight go, the `recent` newest tokens excepted."""
+    least weight go, the `recent` newest tokens excepted.  A call that would take a sequence
+    past its slots raises ValueError."""
 
     def __init__(self, wqkv, wo, hidden: int, heads: int, kv_heads: int, head_dim: int, seqs: int, capacity: int,
                  budget: int, recent: int, slack: int = 16, window: int = 8, page_size: int = 64,
@@ -60,12 +61,20 @@ class AttentionLayer:
         o = o.reshape(-1, self.heads * self.head_dim)
         return device.htile(o, *self.wo, self.hidden, mode="fast", out_dtype=torch.bfloat16)
 
+    def _room(self, longest: int) -> None:
+        have = self.table.shape[1] * self.cache.page_size
+        if longest > have:  # an index past the table would end the process's use of the GPU
+            raise ValueError(f"{longest} slots wanted of a sequence's {have}: a larger capacity or a smaller budget")
+
     def _slots(self, seq: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
         page = self.cache.page_size
         return self.table[seq, at // page] * page + (at % page).to(torch.int32)
 
     def prompt(self, x: torch.Tensor, lens: List[int]) -> torch.Tensor:
         """x [sum(lens), hidden]: the prompts, packed; each fills its sequence from the start."""
+        if len(lens) != self.table.shape[0] or min(lens) < 1 or sum(lens) != x.shape[0]:
+            raise ValueError(f"a prompt of a token or more for each of {self.table.shape[0]} sequences, packed")
+        self._room(max(lens))
         n = torch.tensor(lens, device="cuda")
         ends = torch.zeros(len(lens) + 1, dtype=torch.int32, device="cuda")
         ends[1:] = n.cumsum(0)
@@ -90,6 +99,9 @@ class AttentionLayer:
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """x [seqs, hidden]: one token of every sequence."""
         seqs = x.shape[0]
+        if seqs != self.table.shape[0]:
+            raise ValueError(f"a token of each of {self.table.shape[0]} sequences, not {seqs}")
+        self._room(self.longest + 1)
         q, k, v = self._qkv(x, self.seen)
         seq = torch.arange(seqs, device="cuda")
         attn.kv4_append(self.cache, k, v, self._slots(seq, self.lens))
