@@ -30,9 +30,11 @@
  * D = 128, 2048 clocks for two tiles of queries by one of keys.  Bound: a tile's softmax
  * (about 2150 clocks) and its UMMA round trip (1870) follow on one another, and only two
  * tiles alternate (TMEM holds two S and two O); tensor pipe 55 %, exponentials 52 % busy.
- * 8192 tokens, 32 / 8 heads of 128: 501 us, 1097 TFLOP/s (a tile pair per CTA launch in
- * place of persistent CTAs: 578).  16384: 2119 us, 1038.  Twelve prompts of up to 2011: 109.
+ * 8192 tokens, 32 / 8 heads of 128: 502 us, 1095 TFLOP/s (a tile pair per CTA launch in
+ * place of persistent CTAs: 578).  16384: 2116 us, 1039.  Twelve prompts of up to 2011: 112.
  * 512 after 7777, 16 / 4 heads of 64: 54.  17 tokens: 11, latency.
+ * A value that is not finite, seen or not, costs the blocks that meet it a pass over their
+ * V: 100 queries over 20000 keys 77 -> 330 to 360 us, 4096 tokens 83 -> 130 to 170.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -75,7 +77,8 @@ __device__ __forceinline__ bool span_of(const GlintAttnPrompt &a, int t, Span &s
     return true;
 }
 
-/* one query row by one warp, in f32: right for any stride, alignment and value */
+/* one query row by one warp, in f32: right for any stride, alignment and scale; some 200 clocks
+ * a key (2048 tokens, 32 / 8 heads of 128: 8.4 ms, where the tensor-core kernel takes 0.08) */
 template <int D>
 __device__ __forceinline__ void plain_row(const GlintAttnPrompt &a, const Span &s, int t, int hq, int lane)
 {
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             const Span &s = it.s;
             const int done = (i ? it.last1 : it.last0) - it.first;
             /* Few registers live through this loop: 128 hold scores, and a spilled one would come
-             * back from L2 (the tiles leave next to no L1). */
+             * back from L2 (the tiles leave next to no L1).  None is at D = 128, two at 64. */
             int seen; /* keys this row sees, from the item's first on; 0 or less where it is no query's */
             {
                 const int t = it.t0 + i * g.tok + r / g.group;

@@ -17,10 +17,11 @@
  * each weight, the rounding any BF16 tensor-core attention makes); scores, maximum,
  * sums and the lo terms stay in f32.
  *
- * Floor: HBM, D + D / 8 bytes a slot and head at 4.5 bits a value.  Bound: unpacking,
- * about 790 warp instructions for 32 slots of K and V at D = 128 (ALU 63 %, issue 64 % busy).
- * 16 sequences of 16384 slots, 64 / 8 heads: 80 us (loads alone 57, arithmetic alone 71);
- * 64 of 32768: 534 us, 4.53 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 38
+ * Floor: HBM, D + D / 8 bytes a slot and head at 4.5 bits a value.  Bound: instructions,
+ * about 790 of a warp for 32 slots of K and V at D = 128 (ALU 63 %, issue 64 % busy): 320
+ * unpack codes, the rest fetch, look up pages, find maxima, exponentiate and multiply.
+ * 16 sequences of 16384 slots, 64 / 8 heads: 81 us (loads alone 57, arithmetic alone 71);
+ * 64 of 32768: 536 us, 4.51 TB/s.  32 ragged ones of up to 8191, 32 / 8 heads: 30 us, 38
  * with weights.  One of 1021: 11 us, latency.
  */
 #include <cuda_runtime.h>

@@ -243,8 +243,8 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const GlintKv4Cache 
  * the moves do not depend on one another.
  *
  * Floor: 8 bytes a slot and head read (weight and position), 8 + D + D / 8 read and
- * written a slot moved.  Bound: latency, of seven cluster barriers and of what each waits
- * for: for a sequence of 32768 slots about 50000 clocks, 8400 of them for the keys and the
+ * written a slot moved.  Bound: latency, of the seven cluster barriers that this way of
+ * finding the n-th key takes whatever the keys, and of what each waits for: for a sequence of 32768 slots about 50000 clocks, 8400 of them for the keys and the
  * first digit's counts, 16000 for the digits, 3000 for the bits, 6600 for the list (the
  * first CTA's slots, mostly), 8700 for the moves (16 bytes a lane; a slot a lane: 14000).
  * 16 ragged sequences of up to 32768 slots to 4096, 8 heads of 128: 33 us (512 threads a
