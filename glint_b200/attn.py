@@ -1,6 +1,9 @@
 """Serving attention on torch CUDA tensors, through the C ABI of include/glint_attn.h:
 what runs between a decoder's q|k|v and o linears (device.htile).
 
+  rope          rotary positions of q and k, norms of their heads before them
+  rope_freqs    its frequencies, stretched for long contexts or not
+  rope_append   rope, and keys and values into the cache, in one pass
   attn_prompt   causal attention over packed prompts, grouped heads
   KV4Cache      a paged key/value cache held in 4 bits (4.5 bits a value in all)
   kv4_append    new key/value rows into their slots;  kv4_read  slots back to BF16
@@ -14,6 +17,7 @@ stream ordered and may be captured in CUDA graphs.  Tensors live on the current 
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from functools import lru_cache
 from typing import Optional, Tuple
@@ -24,6 +28,14 @@ from .device import _check, lib
 
 BLOCK = 64
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+
+
+class _Rope(ctypes.Structure):
+    """struct GlintRope"""
+    _fields_ = [(n, _vp) for n in ("q", "k", "q_out", "k_out", "positions", "inv_freq", "q_norm", "k_norm")] + \
+               [(n, _i64) for n in ("q_tok", "q_head", "k_tok", "k_head", "qo_tok", "qo_head", "ko_tok", "ko_head")] + \
+               [("scale", ctypes.c_double), ("eps", ctypes.c_double)] + \
+               [(n, _i32) for n in ("tokens", "heads", "kv_heads", "head_dim", "half", "interleaved")]
 
 
 class _Prompt(ctypes.Structure):
@@ -56,6 +68,8 @@ class _Evict(ctypes.Structure):
 
 def bind(L: ctypes.CDLL) -> ctypes.CDLL:
     P = ctypes.POINTER
+    L.glint_rope_stream.argtypes = [P(_Rope), _vp]
+    L.glint_kv4_rope_append_stream.argtypes = [P(_Cache), P(_Rope), _vp, _i64, _i64, _vp, _vp]
     L.glint_attn_prompt_work_bytes.argtypes = [P(_Prompt)]
     L.glint_attn_prompt_stream.argtypes = [P(_Prompt), _vp]
     L.glint_kv4_append_stream.argtypes = [P(_Cache), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp]
@@ -63,7 +77,7 @@ def bind(L: ctypes.CDLL) -> ctypes.CDLL:
     L.glint_kv4_attn_work_bytes.argtypes = [P(_Cache), P(_Attn)]
     L.glint_kv4_attn_stream.argtypes = [P(_Cache), P(_Attn), _vp]
     L.glint_kv4_evict_stream.argtypes = [P(_Cache), P(_Evict), _vp]
-    for f in (L.glint_attn_prompt_stream, L.glint_kv4_append_stream, L.glint_kv4_read_stream,
+    for f in (L.glint_rope_stream, L.glint_kv4_rope_append_stream, L.glint_attn_prompt_stream, L.glint_kv4_append_stream, L.glint_kv4_read_stream,
               L.glint_kv4_attn_stream, L.glint_kv4_evict_stream):
         f.restype = _i32
     L.glint_attn_prompt_work_bytes.restype = L.glint_kv4_attn_work_bytes.restype = _i64
@@ -88,6 +102,8 @@ class _Calls:
 
         def get(name, *args, res=_i32):
             return ctypes.CFUNCTYPE(res, *args)((name, L))
+        self.rope = get("glint_rope_stream", cp, _vp)
+        self.rope_append = get("glint_kv4_rope_append_stream", cp, cp, _vp, _i64, _i64, _vp, _vp)
         self.prompt = get("glint_attn_prompt_stream", cp, _vp)
         self.append = get("glint_kv4_append_stream", cp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp)
         self.read = get("glint_kv4_read_stream", cp, _vp, _i32, _vp, _vp, _vp)
@@ -108,6 +124,7 @@ def _c() -> _Calls:
 
 
 # the layouts of the structs above, pointers and strides in 64 bits
+_pack_rope = struct.Struct("8P8q2d6i").pack
 _pack_prompt = struct.Struct("8P8q7if").pack
 _pack_cache = struct.Struct("4P4i").pack
 _pack_attn = struct.Struct("8P4q4if4x").pack
@@ -182,6 +199,171 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _head_dim(d: int) -> None:
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, not {d}")
+
+
+def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
+               device="cuda") -> Tuple[torch.Tensor, float]:
+    """(inv_freq [rotary_dim / 2] f32, scale) for rope: base ** (-2 i / rotary_dim), stretched for contexts
+    longer than a model was trained on as `scaling` says, in the keys of a model's rope_scaling
+    (rope_type, or type):
+
+    default   not stretched
+    linear    every frequency divided by `factor`
+    llama3    wavelengths over original_max_position_embeddings / low_freq_factor divided by `factor`,
+              those under .. / high_freq_factor kept, between them a ramp over their turns
+    yarn      frequencies of fewer than beta_slow (1) turns in the original length divided by `factor`,
+              those of more than beta_fast (32) kept, between them a ramp over their numbers; scale
+              attention_factor, or 0.1 ln(factor) + 1
+    longrope  each divided by its own of `factors` (a model's short_factor or long_factor); scale
+              attention_factor, or with `factor` sqrt(1 + ln(factor) / ln(original length))"""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even, not {rotary_dim}")
+    if not base > 0:
+        raise ValueError(f"base must be above 0, not {base}")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    freq = base ** (-2 * i / max(rotary_dim, 1))
+    scaling = dict(scaling or {})
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+
+    def of(key, *default):
+        v = scaling.get(key)
+        if v is None:
+            if not default:
+                raise ValueError(f"rope_type {kind!r} needs {key!r}")
+            return default[0]
+        if key != "attention_factor" and not v > 0:
+            raise ValueError(f"{key!r} must be above 0, not {v}")
+        return float(v)
+    scale = 1.0
+    if kind == "linear":
+        freq = freq / of("factor")
+    elif kind == "llama3":
+        low, high = of("low_freq_factor"), of("high_freq_factor")
+        if not high > low:
+            raise ValueError(f"'high_freq_factor' must be above 'low_freq_factor', not {high} and {low}")
+        turns = of("original_max_position_embeddings") * freq / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        freq = freq * (keep + (1 - keep) / of("factor"))
+    elif kind == "yarn":
+        factor, length = of("factor"), of("original_max_position_embeddings")
+
+        def number(turns):  # of the frequency that makes so many turns
+            return rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low = max(math.floor(number(of("beta_fast", 32.0))), 0)
+        high = min(math.ceil(number(of("beta_slow", 1.0))), rotary_dim - 1)
+        keep = 1 - ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq * (keep + (1 - keep) / factor)
+        scale = of("attention_factor", 0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
+    elif kind == "longrope":
+        factors = torch.tensor(scaling.get("factors") or [], dtype=torch.float64)
+        if factors.shape != freq.shape or not bool((factors > 0).all()):
+            raise ValueError(f"'factors' must be {rotary_dim // 2} numbers above 0")
+        freq = freq / factors
+        by = of("factor", 1.0)
+        scale = of("attention_factor", math.sqrt(1 + math.log(by) / math.log(of("original_max_position_embeddings")))
+                   if by > 1 else 1.0)
+    elif kind != "default":
+        raise ValueError(f"rope_type must be default, linear, llama3, yarn or longrope, not {kind!r}")
+    return freq.float().to(device), scale
+
+
+def _heads_apart(t: torch.Tensor, name: str) -> None:
+    """No two heads of an output lie on one another."""
+    (T, H, D), (st, sh, _) = t.shape, t.stride()
+    if T and H and not ((sh >= D or H == 1) and (st >= (H - 1) * sh + D or T == 1) or
+                        (st >= D or T == 1) and (sh >= (T - 1) * st + D or H == 1)):
+        raise ValueError(f"the heads of {name} overlap one another")
+
+
+def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two [tokens, heads, head_dim] tensors of one type surely share no element: their spans do
+    not meet, or they are different heads of one buffer's tokens."""
+    (T, Ha, D), (sa, ha, _) = a.shape, a.stride()
+    (Tb, Hb, _), (sb, hb, _) = b.shape, b.stride()
+    if not (T and Ha and Tb and Hb):
+        return True
+    ea, eb, size = (Ha - 1) * ha + D, (Hb - 1) * hb + D, a.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + ((T - 1) * sa + ea) * size <= pb or pb + ((Tb - 1) * sb + eb) * size <= pa:
+        return True
+    if sa != sb or (pb - pa) % size:
+        return False
+    off = (pb - pa) // size % sa if sa else 0
+    return ea <= off and off + eb <= sa
+
+
+def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, others, keys):
+    """The checks that rope and rope_append share; (struct, stream, q_out, k_out).  others: further
+    inputs (name, tensor) of q's type; keys: k_out is wanted whether it was given or not."""
+    _want(q, "q", torch.bfloat16, (None, None, None), dense=False)
+    T, H, D = q.shape
+    _head_dim(D)
+    if H < 1:
+        raise ValueError("q must have a head or more")
+    Hk = 0
+    if k is not None:
+        _want(k, "k", torch.bfloat16, (T, None, D), dense=False)
+        Hk = k.shape[1]
+    elif k_norm is not None or k_out is not None:
+        raise ValueError("k_norm and k_out need k")
+    _want(positions, "positions", torch.int32, (T,))
+    _want(inv_freq, "inv_freq", torch.float32, (None,))
+    half = inv_freq.shape[0]
+    if half > D // 2:
+        raise ValueError(f"inv_freq must have {D // 2} frequencies or fewer, not {half}")
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None:
+            _want(w, name, torch.float32, (D,))
+            _want16(w, name)
+    if not (eps > 0 and math.isfinite(eps) and math.isfinite(scale)):
+        raise ValueError(f"eps must be above 0 and scale finite, not {eps} and {scale}")
+    given = q_out is not None or k_out is not None
+    if q_out is None:
+        q_out = _empty(q, (T, H, D), torch.bfloat16, stream)
+    else:
+        _want(q_out, "q_out", torch.bfloat16, (T, H, D), dense=False)
+    if k_out is None:
+        if keys and k is not None:
+            k_out = _empty(q, (T, Hk, D), torch.bfloat16, stream)
+    else:
+        _want(k_out, "k_out", torch.bfloat16, (T, Hk, D), dense=False)
+    raw = _raw(q, stream, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
+    if given:
+        outs = [(n, o) for n, o in (("q_out", q_out), ("k_out", k_out)) if o is not None]
+        for n, o in outs:
+            _heads_apart(o, n)
+            for m, x in [("q", q), ("k", k)] + others:
+                itself = m == n[0] and x is not None and x.data_ptr() == o.data_ptr() and x.stride() == o.stride()
+                if x is not None and not itself and not _rows_apart(o, x):
+                    raise ValueError(f"{n} must be {n[0]} itself or apart from q, k and v: it may overlap {m}")
+        if len(outs) == 2 and not _rows_apart(q_out, k_out):
+            raise ValueError("q_out and k_out must be apart")
+    qs, os = q.stride(), q_out.stride()
+    ks = (0, 0) if k is None else k.stride()
+    kos = (0, 0) if k_out is None else k_out.stride()
+    a = _pack_rope(q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
+                   positions.data_ptr(), inv_freq.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                   0 if k_norm is None else k_norm.data_ptr(), qs[0], qs[1], ks[0], ks[1], os[0], os[1], kos[0], kos[1],
+                   scale, eps, T, H, Hk, D, half, 1 if interleaved else 0)
+    return a, raw, q_out, k_out
+
+
+def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
+         interleaved: bool = False, scale: float = 1.0, q_norm: Optional[torch.Tensor] = None,
+         k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+         k_out: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(q_out, k_out): q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] BF16 (any strides,
+    last dimension contiguous; k may be None) rotated by positions [tokens] int32.
+
+    inv_freq [half] f32 (rope_freqs): 2 * half <= head_dim values of a head are rotated, the pairs (i, i +
+    half), or (2i, 2i + 1) with interleaved, by position * inv_freq[i]; the others stay.  scale multiplies cos
+    and sin.  q_norm, k_norm [head_dim] f32: each head is divided by sqrt(mean of squares + eps) and
+    multiplied by these first.  q_out and k_out may be q and k themselves (any other overlap is
+    refused); left out, they are new and contiguous."""
+    a, raw, q_out, k_out = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
+                                 [], True)
+    _check(_c().rope(a, raw), "glint_rope_stream")
+    return q_out, k_out
 
 
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -280,6 +462,25 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     ks, vs = k.stride(), v.stride()
     _check(_c().append(cache._c, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), k.shape[0],
                        _raw(k, stream, v, slots, cache.k_code)), "glint_kv4_append_stream")
+
+
+def rope_append(cache: KV4Cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                inv_freq: torch.Tensor, slots: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
+                q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """rope(q, k, ...), then kv4_append(cache, the rotated k, v, slots), in one pass: the same q_out (which is
+    returned) and the same bytes in the cache.  The rotated keys go to the cache alone unless k_out is given (k
+    itself, or a tensor of k's shape), as a prompt's attention wants them.  A token whose slot is
+    negative is rotated and not cached."""
+    _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
+    _want(v, "v", torch.bfloat16, k.shape, dense=False)
+    _want(slots, "slots", torch.int32, k.shape[:1])
+    a, raw, q_out, _ = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
+                             [("v", v)], False)
+    _raw(q, stream, v, slots, cache.k_code)
+    vs = v.stride()
+    _check(_c().rope_append(cache._c, a, v.data_ptr(), vs[0], vs[1], slots.data_ptr(), raw), "glint_kv4_rope_append_stream")
+    return q_out
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,

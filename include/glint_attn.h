@@ -1,7 +1,9 @@
 /* Attention between a decoder's q|k|v and o linears (libglint_encode.so; additive, no
- * counterpart in the reference's C ABI): causal attention over packed prompts, and a
+ * counterpart in the reference's C ABI): rotary positions, causal attention over packed prompts, and a
  * paged key/value cache held in 4 bits with what fills, reads and shrinks it.
  *
+ *   glint_rope_stream         rotary positions of q and k, norms of their heads before them
+ *   glint_kv4_rope_append_stream  the same, and keys and values into their slots
  *   glint_attn_prompt_stream  o = softmax(scale q k^T) v over packed sequences
  *   glint_kv4_append_stream   new key/value rows, quantised into their slots
  *   glint_kv4_read_stream     slots back to BF16 rows
@@ -27,6 +29,28 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* Rotary positions.  For each token t and head x of q (heads) and k (kv_heads; 0: no k):
+ *   y = x, or (x r) w with r = 1 / sqrt(mean(x^2) + eps) where there are weights w
+ *       (q_norm, k_norm: head_dim f32, 16-byte aligned; NULL: none)
+ *   c = scale cos(p f), s = scale sin(p f), p = positions[t], f = inv_freq[i], i < half
+ *   (o1, o2) = (y1 c - y2 s, y2 c + y1 s) on places (i, i + half), or (2i, 2i + 1) with
+ *       interleaved; places from 2 half on are y.  0 <= half <= head_dim / 2.
+ * Angles and r are computed in 64 bits and rounded to f32, products and sums of y, c and s
+ * are rounded to f32 one by one and o once to BF16.  positions device int32, inv_freq
+ * device f32; scale and eps in 64 bits, eps > 0.  q_out may be q itself (the same strides),
+ * k_out k; otherwise outputs overlap no input.  16-byte aligned tensors with
+ * strides that are multiples of 8 are read and written 16 bytes at a time. */
+typedef struct GlintRope {
+    const glint_bf16_t *q, *k;
+    glint_bf16_t *q_out, *k_out;
+    const int *positions;
+    const float *inv_freq, *q_norm, *k_norm;
+    int64_t q_tok, q_head, k_tok, k_head, qo_tok, qo_head, ko_tok, ko_head;
+    double scale, eps;
+    int tokens, heads, kv_heads, head_dim, half, interleaved;
+} GlintRope;
+int glint_rope_stream(const GlintRope *a, cudaStream_t stream);
 
 /* Packed prompts.  Sequence s has the query tokens [cu_q[s], cu_q[s + 1]) and the
  * keys [cu_k[s], cu_k[s + 1]) (device int32, seqs + 1 entries, non-decreasing; values
@@ -77,6 +101,11 @@ typedef struct GlintKv4Cache {
 int glint_kv4_append_stream(const GlintKv4Cache *c, const glint_bf16_t *k, const glint_bf16_t *v, int64_t k_tok,
                             int64_t k_head, int64_t v_tok, int64_t v_head, const int *slots, int tokens,
                             cudaStream_t stream);
+/* glint_rope_stream, and its keys with v [tokens, kv_heads, head_dim] into slots[t]: the cache
+ * gets the bytes that glint_kv4_append_stream makes of k_out.  a->k_out may be NULL: the
+ * rotated keys go to the cache alone.  Outputs do not overlap v. */
+int glint_kv4_rope_append_stream(const GlintKv4Cache *c, const GlintRope *a, const glint_bf16_t *v, int64_t v_tok,
+                                 int64_t v_head, const int *slots, cudaStream_t stream);
 /* k_out, v_out [tokens, kv_heads, head_dim] BF16, contiguous and 16-byte aligned: the
  * values of slots[t], rounded to BF16; zeros for entries outside the cache. */
 int glint_kv4_read_stream(const GlintKv4Cache *c, const int *slots, int tokens, glint_bf16_t *k_out,
