@@ -1,0 +1,22 @@
+/* The activation of a gated feed-forward projection, shared by the H-TILE kernels whose
+ * epilogue applies it (htile_gemv.cu, htile_decode.cu, htile_gemm.cu). */
+#ifndef GLINT_B200_GATED_CUH_
+#define GLINT_B200_GATED_CUH_
+
+#include "../../include/glint_htile.h"
+
+namespace glint {
+
+/* act(g) u, act(g) = g / (1 + exp(-z)): z = g (silu), or 2 sqrt(2 / pi) (g + 0.044715 g^3), which
+ * makes it g (1 + tanh(z / 2)) / 2.  The fast exponential is within 2^-17 of its value
+ * wherever act(g) is not 0 in BF16 and the division within 2^-22, far inside the result's
+ * rounding; below z = -87 act(g) is 0. */
+__device__ __forceinline__ float gated_value(float g, float u, int act)
+{
+    const float z = act == GLINT_ACT_GELU_TANH ? g * fmaf(0.0713548162726f * g, g, 1.59576912160573f) : g;
+    return __fdividef(g, 1.f + __expf(-z)) * u;
+}
+
+} // namespace glint
+
+#endif

@@ -27,7 +27,8 @@ struct ExpandJob {
     void *out;
 };
 
-enum OutKind : int { kOutF32 = 0, kOutBF16 = 1 };
+/* kOutGated: BF16 act(row 2i) * row 2i + 1, of the H-TILE kernels that know it */
+enum OutKind : int { kOutF32 = 0, kOutBF16 = 1, kOutGated = 2 };
 
 /* H-TILE arithmetic: kPrecise splits every dequantised weight into a BF16 pair
  * (hi + lo) so the tensor-core sums match an f32 dot product to ~1e-6; kFast uses
@@ -105,6 +106,17 @@ int htile_decode_gather_launch(const uint8_t *hole, const uint8_t *plug, const f
                                const __nv_bfloat16 *x, void *const *y_ranks, uint32_t *const *flag_ranks,
                                int world, int rank, OutKind y_kind, int M, int N, int K, int ldy, int n0,
                                HtileMode mode, cudaStream_t stream);
+
+/* h[M, N / 2] BF16 = act(y[:, 2i]) * y[:, 2i + 1], y as of htile_launch (N even; gated.cuh):
+ * M <= 32 and any M of the TMA kernels' shapes (bs == 64, K % 256 == 0, 16-byte alignment), and
+ * all others.  work: htile_gemm_gated_work() bytes, fast mode only. */
+int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
+                              void *h, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
+int64_t htile_gemm_gated_work(int M, int N, int K);
+int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
+                            void *h, void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
+int htile_gemv_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
+                            void *h, int M, int N, int K, int blocksize, HtileMode mode, int act, cudaStream_t stream);
 
 /* K-major layout, parent-only decode GEMV and activation-selected plug correction
  * (kmajor.cu): n % 8 == 0, K % 64 == 0, K <= kKmMaxK, blocksize 64, 16-byte

@@ -42,6 +42,7 @@
 #include <unordered_map>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "gather.cuh"
 #include "glint_internal.h"
 #include "ptx.cuh"
@@ -628,9 +629,10 @@ struct RowArgs {
     uint32_t tail_tx;
     float *tail_ws;
     int *tail_cnt;
+    int act; /* kOutGated: of the gate rows */
 };
 
-template <int MT, bool SPLIT, bool BF16OUT, int NB>
+template <int MT, bool SPLIT, int OUT, int NB>
 __global__ void __launch_bounds__(kThreads, 1)
     htile_rows_kernel(const __grid_constant__ CUtensorMap hmap, const __grid_constant__ CUtensorMap pmap,
                       const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap xmap,
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
          * in block order, publishes the unit's partial and, as the tile's last
          * unit, adds the tile's KU partials in unit order.  No waits on other CTAs:
          * a failed TMA wait still publishes (zeros), so the count stays whole. */
-        if constexpr (MT <= 2) { /* the tail's shared buffer exists for MT <= 2 only */
+        if constexpr (MT <= 2 && OUT != kOutGated) { /* the tail's shared buffer exists for MT <= 2 only */
             const int j = warp - active;
             if (!has_tail || j >= kTailWarps)
                 return;
@@ -822,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int q = 0; q < 4; ++q) {
                     const int n = n16 + pg + (q >> 1) * 8, col = mt * 8 + 2 * t + (q & 1);
                     if (n < a.N && col < a.M) {
-                        if (BF16OUT)
+                        if (OUT == kOutBF16)
                             static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * a.N + n] = __float2bfloat16_rn(sum[mt][q]);
                         else
                             static_cast<float *>(a.y)[(int64_t)col * a.N + n] = sum[mt][q];
@@ -905,6 +907,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_arrive(cmb_empty);
         }
         const int nb0 = n_begin + blk * a.RB;
+        if constexpr (OUT == kOutGated) {
+            /* Rows 2i and 2i + 1 (gate and up; nb0 is even) are with lanes g and g + 4, g < 4.  Of
+             * its two activation rows each of the pair keeps one: the lower lane takes up of
+             * the first for gate of the second, and both have what one output needs. */
+            const bool up = g >= 4;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float keep = up ? acc[mt][2 * h + 1] : acc[mt][2 * h], give = up ? acc[mt][2 * h] : acc[mt][2 * h + 1];
+                    const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 16);
+                    const int row = r0 + pg + 8 * h, col = mt * 8 + 2 * t + (up ? 1 : 0), n = nb0 + row;
+                    if (row < a.RB && n < n_end && col < a.M)
+                        static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] =
+                            __float2bfloat16_rn(up ? gated_value(got, keep, a.act) : gated_value(keep, got, a.act));
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -913,8 +934,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int n = nb0 + row;
                 if (row < a.RB && n < n_end && col < a.M) {
                     if (a.ga.world > 0) {
-                        gather_store<BF16OUT>(a.ga, col, n, acc[mt][q]);
-                    } else if (BF16OUT) {
+                        gather_store<OUT == kOutBF16>(a.ga, col, n, acc[mt][q]);
+                    } else if (OUT == kOutBF16) {
                         static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * a.N + n] = __float2bfloat16_rn(acc[mt][q]);
                     } else {
                         static_cast<float *>(a.y)[(int64_t)col * a.N + n] = acc[mt][q];
@@ -1045,10 +1066,10 @@ int launch_mt(int MT, const Maps &m, const DecodeArgs &a, int grid, cudaStream_t
     return launch_t<4, SPLIT, BF16OUT>(m, a, grid, st, pdl);
 }
 
-template <int MT, bool SPLIT, bool BF16OUT, int NB>
+template <int MT, bool SPLIT, int OUT, int NB>
 int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
-    auto kern = htile_rows_kernel<MT, SPLIT, BF16OUT, NB>;
+    auto kern = htile_rows_kernel<MT, SPLIT, OUT, NB>;
     if (!ensure_smem((const void *)kern, r_smem_bytes<MT>()))
         return kLaunch;
     cudaLaunchConfig_t cfg = {};
@@ -1067,14 +1088,14 @@ int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, b
     }
     return kOk;
 }
-template <int MT, bool SPLIT, bool BF16OUT>
+template <int MT, bool SPLIT, int OUT>
 int launch_rows_t(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
     const int nb = 4 * a.UB / a.KH;
     if (nb == 2)
-        return launch_rows_nb<MT, SPLIT, BF16OUT, 2>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, SPLIT, OUT, 2>(m, a, grid, st, pdl);
     if (nb == 1)
-        return launch_rows_nb<MT, SPLIT, BF16OUT, 1>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, SPLIT, OUT, 1>(m, a, grid, st, pdl);
     return kLaunch;
 }
 
@@ -1084,12 +1105,14 @@ constexpr int align1k(int v) { return (v + 1023) & ~1023; }
  * Units take as many 256-k slices (UB = 4, 2, 1) as keep >= 3 ring stages, the
  * consumer warps' plan valid and K whole; row blocks of more than 4 tiles take
  * one (their requests are large already, and the shared tail needs UB = 1). */
-bool plan_rows(RowArgs &a, int R, int MT)
+bool plan_rows(RowArgs &a, int R, int MT, bool pairs = false)
 {
     const int M = a.M, K = a.K;
     a.R = R;
     a.nb = (a.R + kRowBlockMax - 1) / kRowBlockMax;
     a.RB = (a.R + a.nb - 1) / a.nb;
+    if (pairs) /* rows 2i and 2i + 1 in one block */
+        a.RB += a.RB & 1;
     a.T = (a.RB + 15) / 16;
     a.xrows = std::min(M, 8 * MT);
     const int ring = MT == 1 ? r_ring<1>() : MT == 2 ? r_ring<2>() : r_ring<4>();
@@ -1132,12 +1155,13 @@ bool plan_rows(RowArgs &a, int R, int MT)
  * leave most SMs a mostly empty last tile. */
 int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
                 OutKind yk, int M, int N, int K, HtileMode mode, cudaStream_t st, bool pdl,
-                const GatherArgs *gt = nullptr, bool tail = false)
+                const GatherArgs *gt = nullptr, bool tail = false, int act = 0)
 {
     const int MT = M <= 8 ? 1 : (M <= 16 ? 2 : 4);
     const int sms = sm_count();
     RowArgs a{};
-    a.y = y, a.M = M, a.N = N, a.K = K;
+    a.y = y, a.M = M, a.N = N, a.K = K, a.act = act;
+    const bool gated = yk == kOutGated;
     if (gt)
         a.ga = *gt;
     int grid = 0;
@@ -1159,7 +1183,10 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
     }
     if (!grid) {
         const int g0 = std::max(1, std::min(sms, tiles));
-        if (!plan_rows(a, (N + g0 - 1) / g0, MT))
+        int R = (N + g0 - 1) / g0;
+        if (gated) /* whole pairs, and no less than the tile of rows that is read from shared memory */
+            R = std::max(16, R + (R & 1));
+        if (!plan_rows(a, R, MT, gated))
             return kLaunch;
         grid = (N + a.R - 1) / a.R;
     }
@@ -1188,11 +1215,14 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
     }
     const bool bf = yk == kOutBF16, pr = mode == kPrecise;
 #define GLINT_ROWS_CASE(mt)                                                                                            \
+    if (MT == mt && gated)                                                                                             \
+        return pr ? launch_rows_t<mt, true, kOutGated>(maps, a, grid, st, pdl)                                         \
+                  : launch_rows_t<mt, false, kOutGated>(maps, a, grid, st, pdl);                                       \
     if (MT == mt)                                                                                                      \
-        return pr ? (bf ? launch_rows_t<mt, true, true>(maps, a, grid, st, pdl)                                         \
-                        : launch_rows_t<mt, true, false>(maps, a, grid, st, pdl))                                       \
-                  : (bf ? launch_rows_t<mt, false, true>(maps, a, grid, st, pdl)                                        \
-                        : launch_rows_t<mt, false, false>(maps, a, grid, st, pdl));
+        return pr ? (bf ? launch_rows_t<mt, true, kOutBF16>(maps, a, grid, st, pdl)                                     \
+                        : launch_rows_t<mt, true, kOutF32>(maps, a, grid, st, pdl))                                     \
+                  : (bf ? launch_rows_t<mt, false, kOutBF16>(maps, a, grid, st, pdl)                                    \
+                        : launch_rows_t<mt, false, kOutF32>(maps, a, grid, st, pdl));
     GLINT_ROWS_CASE(1)
     GLINT_ROWS_CASE(2)
     GLINT_ROWS_CASE(4)
@@ -1357,6 +1387,14 @@ int htile_decode_launch(const uint8_t *hole, const uint8_t *plug, const float *a
                         OutKind yk, int M, int N, int K, HtileMode mode, cudaStream_t st)
 {
     return decode_launch_impl(hole, plug, am, x, y, yk, M, N, K, mode, st, nullptr);
+}
+
+/* act(gate) * up of rows 2i and 2i + 1: always the row-owned kernel, whose sums never leave their
+ * CTA (no workspace, at any N) */
+int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
+                              int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+{
+    return launch_rows(hole, plug, am, x, h, kOutGated, M, N, K, mode, st, true, nullptr, false, act);
 }
 
 bool htile_gather_supported(int M, int N) { return M >= 1 && M <= 32 && N >= 1; }

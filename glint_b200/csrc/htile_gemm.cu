@@ -49,6 +49,7 @@
 #include <unordered_map>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "gather.cuh"
 #include "glint_internal.h"
 #include "ptx.cuh"
@@ -245,6 +246,7 @@ struct GemmArgs {
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
     GatherArgs ga; /* world > 0: y[m, n] goes to every rank's y at [m, ga.n0 + n] (row stride ga.ldy) */
+    int act;       /* gated kernel: of the gate rows */
 };
 
 /* Work split (stream-K for the first S tiles, then data-parallel rounds): the
@@ -302,6 +304,23 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
                 *yp = __uint_as_float(v[j]);
     }
 }
+/* h[m, n / 2] = act(y[m, n]) y[m, n + 1], n even, of rows m0 .. m0+jl-1 from 32 accumulator values
+ * of each lane's column n (pairs of lanes hold n and n + 1; n_cols is even).  Of two rows each lane of a pair
+ * keeps one: the even lane takes up of the first for gate of the second. */
+__device__ __forceinline__ void store_gated(void *h, int n_cols, int act, const uint32_t (&v)[32], int m0, int jl, int n)
+{
+    const bool up = n & 1;
+    const size_t ld = (size_t)(n_cols / 2);
+    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(h) + (size_t)(m0 + (up ? 1 : 0)) * ld + n / 2;
+    const bool live = n < n_cols;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2, p += 2 * ld) {
+        const float keep = __uint_as_float(up ? v[j + 1] : v[j]), give = __uint_as_float(up ? v[j] : v[j + 1]);
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
+        if (live && j + (up ? 1 : 0) < jl)
+            *p = __float2bfloat16_rn(up ? gated_value(got, keep, act) : gated_value(keep, got, act));
+    }
+}
 /* y rows m0 .. m0+jl-1 at column n: this call's y; in a gathered call this
  * rank's y and, with `peers`, every other rank's (over NVLink, starting with the
  * next rank so that the ranks' stores spread over the links) */
@@ -351,6 +370,7 @@ __device__ __forceinline__ void copy_rows_to_peers(const GatherArgs &g, int m0, 
     }
 }
 
+template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     htile_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs args)
 {
@@ -591,13 +611,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     uint32_t v[32];
                     tmem_ld32(tb + c * 32, v);
                     tmem_ld_wait();
-                    store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, false);
+                    if constexpr (GATED)
+                        store_gated(args.y, args.N, args.act, v, m0 + c * 32, min(32, mlim - c * 32), n);
+                    else
+                        store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, false);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_remote(accempty0);
-                if (args.ga.world > 1 && n < args.N) {
+                if (!GATED && args.ga.world > 1 && n < args.N) {
                     if (args.y_bf16)
                         copy_rows_to_peers<__nv_bfloat16>(args.ga, m0, mlim, args.ga.n0 + n);
                     else
@@ -670,10 +693,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 16; ++j)
                         v[h * 16 + j] = __float_as_uint(acc[j]);
                 }
-                store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, true);
+                if constexpr (GATED)
+                    store_gated(args.y, args.N, args.act, v, m0 + c * 32, min(32, mlim - c * 32), n);
+                else
+                    store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, true);
             }
         }
-        if (args.ga.world > 0)
+        if (!GATED && args.ga.world > 0)
             gather_complete(args.ga, kEpiWarps, lane, cta_done, &g_glint_kernel_error);
     }
     tc_fence_before();
@@ -729,6 +755,7 @@ struct PreciseArgs {
     int M, N, K;
     int y_bf16;
     int mtiles, tiles;
+    int act; /* gated kernel: of the gate rows */
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
@@ -748,6 +775,7 @@ __device__ __forceinline__ uint32_t split_hilo(float c)
     return hi | (f32_to_bf16_bits(rest) << 16);
 }
 
+template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
     htile_gemm_precise_kernel(const __grid_constant__ Maps maps, const PreciseArgs args)
 {
@@ -991,10 +1019,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
                 if (lane == 0)
                     mbar_arrive_remote(ae0 + (uint32_t)b * 8u);
             }
-            if (!alive || !nok)
+            if (!alive)
+                continue;
+            const int jl = min(32, args.M - m0);
+            if constexpr (GATED) {
+                uint32_t v[32];
+#pragma unroll
+                for (int jj = 0; jj < 32; ++jj)
+                    v[jj] = __float_as_uint(run[jj]);
+                store_gated(args.y, args.N, args.act, v, m0, jl, n);
+                continue;
+            }
+            if (!nok)
                 continue;
             const size_t step = (size_t)args.N;
-            const int jl = min(32, args.M - m0);
             if (args.y_bf16) {
                 __nv_bfloat16 *yp = static_cast<__nv_bfloat16 *>(args.y) + (size_t)m0 * step + n;
 #pragma unroll
@@ -1533,8 +1571,8 @@ int max_pairs(int kind = 0)
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const void *kern = kind == 2   ? (const void *)int8_tc_kernel<false>
-                       : kind == 1 ? (const void *)htile_gemm_precise_kernel
-                                   : (const void *)htile_gemm_kernel;
+                       : kind == 1 ? (const void *)htile_gemm_precise_kernel<false>
+                                   : (const void *)htile_gemm_kernel<false>;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
         cudaGetLastError();
         n = std::max(1, sm_count() / 2);
@@ -1545,34 +1583,18 @@ int max_pairs(int kind = 0)
 } // namespace
 
 namespace {
-int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
-                     bool y_bf16, int M, int N, int K, cudaStream_t st, const GatherArgs *ga)
+/* How a product's tiles are shared by the pairs: whole tiles only, unless the last
+ * data-parallel round would leave more than 2% of the pairs' time idle; then the
+ * remainder is shared stream-K: with two or more rounds, (tiles mod P) + P tiles,
+ * after which whole rounds follow (their sums overlap whole tiles); between one and
+ * two rounds, the tiles beyond one round (e.g. 512 x 14336: 112 tiles on 74 pairs,
+ * 86.8 -> 76.9 us; sharing all tiles instead cost more in split-tile sums than it
+ * saved). */
+int gemm_plan(GemmArgs &a)
 {
-    Maps maps;
-    if (!encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, BMH,
-                    CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&maps.h, CU_TENSOR_MAP_DATA_TYPE_UINT8, hole, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
-                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&maps.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, plug, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
-                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&maps.am, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, am, (uint64_t)K / 64, (uint64_t)N,
-                    (uint64_t)K / 64 * 4, 4, BN, CU_TENSOR_MAP_SWIZZLE_NONE))
-        return kLaunch;
-    if (!ensure_smem((const void *)htile_gemm_kernel, kSmemBytes))
-        return kLaunch;
-    GemmArgs a{};
-    a.y = y, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0;
-    if (ga)
-        a.ga = *ga;
-    a.mtiles = (M + BMX - 1) / BMX, a.ntiles = (N + 2 * BN - 1) / (2 * BN);
-    a.G = K / (PSTEPS * BK);
+    a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
+    a.G = a.K / (PSTEPS * BK);
     const int tiles = a.mtiles * a.ntiles;
-    /* whole tiles only, unless the last data-parallel round would leave more than
-     * 2% of the pairs' time idle; then the remainder is shared stream-K: with two or
-     * more rounds, (tiles mod P) + P tiles, after which whole rounds follow (their
-     * sums overlap whole tiles); between one and two rounds, the tiles beyond one
-     * round (e.g. 512 x 14336: 112 tiles on 74 pairs, 86.8 -> 76.9 us; sharing all
-     * tiles instead cost more in split-tile sums than it saved) */
     const int maxp = max_pairs();
     const int rounds = (tiles + maxp - 1) / maxp;
     const bool idle = (double)(rounds * maxp - tiles) > 0.02 * rounds * maxp;
@@ -1583,9 +1605,61 @@ int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, 
     a.R = split ? (split1 ? 1 : tiles / pairs - 1) : (tiles + pairs - 1) / pairs;
     a.S = split ? tiles - a.R * pairs : 0;
     a.U = a.S * a.G;
-    if (!gemm_scratch(st, (size_t)pairs * 2 * 2 * 4 * kPartFloats, (size_t)tiles * 8, &a.ws, &a.counters))
+    return pairs;
+}
+size_t part_floats(int pairs) { return (size_t)pairs * 2 * 2 * 4 * kPartFloats; }
+
+bool gemm_maps(Maps &maps, const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, int M,
+               int N, int K)
+{
+    return encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, BMH,
+                      CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_map(&maps.h, CU_TENSOR_MAP_DATA_TYPE_UINT8, hole, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
+                      PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_map(&maps.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, plug, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
+                      PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_map(&maps.am, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, am, (uint64_t)K / 64, (uint64_t)N,
+                      (uint64_t)K / 64 * 4, 4, BN, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
+                     bool y_bf16, int M, int N, int K, cudaStream_t st, const GatherArgs *ga)
+{
+    Maps maps;
+    if (!gemm_maps(maps, hole, plug, am, x, M, N, K) || !ensure_smem((const void *)htile_gemm_kernel<false>, kSmemBytes))
         return kLaunch;
-    htile_gemm_kernel<<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, a);
+    GemmArgs a{};
+    a.y = y, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0;
+    if (ga)
+        a.ga = *ga;
+    const int pairs = gemm_plan(a);
+    if (!gemm_scratch(st, part_floats(pairs), (size_t)a.tiles * 8, &a.ws, &a.counters))
+        return kLaunch;
+    htile_gemm_kernel<false><<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, a);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
+}
+
+template <bool GATED>
+int precise_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
+                        bool y_bf16, int M, int N, int K, int act, cudaStream_t st)
+{
+    Maps maps;
+    if (!encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, PBMH,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_map(&maps.h, CU_TENSOR_MAP_DATA_TYPE_UINT8, hole, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
+                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_map(&maps.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, plug, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
+                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B))
+        return kLaunch;
+    maps.am = maps.h; /* not read: the epilogue loads absmax itself */
+    if (!ensure_smem((const void *)htile_gemm_precise_kernel<GATED>, PSmemBytes))
+        return kLaunch;
+    PreciseArgs a{};
+    a.y = y, a.am = am, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0, a.act = act;
+    a.mtiles = (M + PBMX - 1) / PBMX;
+    a.tiles = a.mtiles * ((N + 2 * BN - 1) / (2 * BN));
+    const int pairs = std::max(1, std::min(a.tiles, max_pairs(1)));
+    htile_gemm_precise_kernel<GATED><<<2 * pairs, PThreads, PSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 } // namespace
@@ -1612,23 +1686,36 @@ int htile_gemm_gather_launch(const uint8_t *hole, const uint8_t *plug, const flo
 int htile_gemm_precise_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x,
                               void *y, bool y_bf16, int M, int N, int K, cudaStream_t st)
 {
+    return precise_launch_impl<false>(hole, plug, am, x, y, y_bf16, M, N, K, 0, st);
+}
+
+/* act(gate) * up of rows 2i and 2i + 1 at any M.  Split tiles' sums and counters are the
+ * caller's: work of htile_gemm_gated_work() bytes, the counters zeroed here, call by call. */
+int64_t htile_gemm_gated_work(int M, int N, int K)
+{
+    GemmArgs a{};
+    a.M = M, a.N = N, a.K = K;
+    const int pairs = gemm_plan(a);
+    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 8 * sizeof(int)) : 0;
+}
+int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
+                            void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+{
+    if (mode == kPrecise)
+        return precise_launch_impl<true>(hole, plug, am, x, h, true, M, N, K, act, st);
     Maps maps;
-    if (!encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, PBMH,
-                    CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&maps.h, CU_TENSOR_MAP_DATA_TYPE_UINT8, hole, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
-                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&maps.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, plug, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
-                    PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (!gemm_maps(maps, hole, plug, am, x, M, N, K) || !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
         return kLaunch;
-    maps.am = maps.h; /* not read: the epilogue loads absmax itself */
-    if (!ensure_smem((const void *)htile_gemm_precise_kernel, PSmemBytes))
-        return kLaunch;
-    PreciseArgs a{};
-    a.y = y, a.am = am, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0;
-    a.mtiles = (M + PBMX - 1) / PBMX;
-    a.tiles = a.mtiles * ((N + 2 * BN - 1) / (2 * BN));
-    const int pairs = std::max(1, std::min(a.tiles, max_pairs(1)));
-    htile_gemm_precise_kernel<<<2 * pairs, PThreads, PSmemBytes, st>>>(maps, a);
+    GemmArgs a{};
+    a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.act = act;
+    const int pairs = gemm_plan(a);
+    if (a.S) {
+        a.ws = static_cast<float *>(work);
+        a.counters = reinterpret_cast<int *>(a.ws + part_floats(pairs));
+        if (cudaMemsetAsync(a.counters, 0, (size_t)a.S * 8 * sizeof(int), st) != cudaSuccess)
+            return kLaunch;
+    }
+    htile_gemm_kernel<true><<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 

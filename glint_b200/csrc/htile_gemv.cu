@@ -28,6 +28,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "glint_internal.h"
 
 namespace glint {
@@ -60,12 +61,12 @@ struct Operands {
     float s[2];       /* absmax of the rows' current 64-block */
 };
 
-template <int MT, bool SPLIT, bool BF16OUT>
+template <int MT, bool SPLIT, int OUT>
 __global__ void __launch_bounds__(kGemvThreads) htile_gemv_kernel(const uint8_t *__restrict__ hole,
                                                                   const uint8_t *__restrict__ plug,
                                                                   const float *__restrict__ absmax,
                                                                   const __nv_bfloat16 *__restrict__ x, void *y, int M,
-                                                                  int N, int K, int bs64, int chunks_per_warp)
+                                                                  int N, int K, int bs64, int chunks_per_warp, int act)
 {
     __shared__ uint32_t lut[256 * 32];
     __shared__ float red[kGemvWarps][16][8 * MT];
@@ -219,18 +220,31 @@ __global__ void __launch_bounds__(kGemvThreads) htile_gemv_kernel(const uint8_t 
             red[warp][g + 8][mt * 8 + 2 * t + 1] = acc[mt][3];
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * 8 * MT; i += kGemvThreads) {
-            const int row = i / (8 * MT), col = i % (8 * MT);
+        auto sum = [&](int row, int col) {
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < kGemvWarps; ++w)
                 v += red[w][row][col];
-            const int n = n0 + row;
-            if (col < M && n < N) {
-                if (BF16OUT)
-                    static_cast<__nv_bfloat16 *>(y)[(int64_t)col * N + n] = __float2bfloat16_rn(v);
-                else
-                    static_cast<float *>(y)[(int64_t)col * N + n] = v;
+            return v;
+        };
+        if constexpr (OUT == kOutGated) {
+            for (int i = threadIdx.x; i < 8 * 8 * MT; i += kGemvThreads) {
+                const int row = 2 * (i / (8 * MT)), col = i % (8 * MT), n = n0 + row;
+                if (col < M && n < N)
+                    static_cast<__nv_bfloat16 *>(y)[(int64_t)col * (N / 2) + n / 2] =
+                        __float2bfloat16_rn(gated_value(sum(row, col), sum(row + 1, col), act));
+            }
+        } else {
+            for (int i = threadIdx.x; i < 16 * 8 * MT; i += kGemvThreads) {
+                const int row = i / (8 * MT), col = i % (8 * MT);
+                const float v = sum(row, col);
+                const int n = n0 + row;
+                if (col < M && n < N) {
+                    if (OUT == kOutBF16)
+                        static_cast<__nv_bfloat16 *>(y)[(int64_t)col * N + n] = __float2bfloat16_rn(v);
+                    else
+                        static_cast<float *>(y)[(int64_t)col * N + n] = v;
+                }
             }
         }
         __syncthreads();
@@ -271,48 +285,103 @@ __global__ void htile_generic_kernel(const uint8_t *hole, const uint8_t *plug, c
     }
 }
 
-template <int MT, bool SPLIT, bool BF16OUT>
+template <int MT, bool SPLIT, int OUT>
 int launch_gemv_t(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y, int M,
-                  int N, int K, int bs, cudaStream_t st)
+                  int N, int K, int bs, int act, cudaStream_t st)
 {
     const int K64 = K / 64;
     const int cpw = (K64 + kGemvWarps - 1) / kGemvWarps;
     const int tiles = (N + 15) / 16;
     const int grid = std::max(1, std::min(tiles, sm_count() * 4));
-    htile_gemv_kernel<MT, SPLIT, BF16OUT><<<grid, kGemvThreads, 0, st>>>(hole, plug, am, x, y, M, N, K, bs / 64, cpw);
+    htile_gemv_kernel<MT, SPLIT, OUT><<<grid, kGemvThreads, 0, st>>>(hole, plug, am, x, y, M, N, K, bs / 64, cpw, act);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
-template <bool SPLIT, bool BF16OUT>
+template <bool SPLIT, int OUT>
 int launch_gemv_slices(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
-                       int M, int N, int K, int bs, cudaStream_t st)
+                       int M, int N, int K, int bs, int act, cudaStream_t st)
 {
-    const size_t ysz = BF16OUT ? 2 : 4;
+    const size_t yrow = OUT == kOutGated ? (size_t)(N / 2) * 2 : (size_t)N * (OUT == kOutBF16 ? 2 : 4);
     for (int m0 = 0; m0 < M; m0 += 32) {
         const int mm = std::min(32, M - m0);
         const __nv_bfloat16 *xs = x + (int64_t)m0 * K;
-        void *ys = static_cast<char *>(y) + (size_t)m0 * N * ysz;
+        void *ys = static_cast<char *>(y) + (size_t)m0 * yrow;
         int rc;
         if (mm <= 8)
-            rc = launch_gemv_t<1, SPLIT, BF16OUT>(hole, plug, am, xs, ys, mm, N, K, bs, st);
+            rc = launch_gemv_t<1, SPLIT, OUT>(hole, plug, am, xs, ys, mm, N, K, bs, act, st);
         else if (mm <= 16)
-            rc = launch_gemv_t<2, SPLIT, BF16OUT>(hole, plug, am, xs, ys, mm, N, K, bs, st);
+            rc = launch_gemv_t<2, SPLIT, OUT>(hole, plug, am, xs, ys, mm, N, K, bs, act, st);
         else
-            rc = launch_gemv_t<4, SPLIT, BF16OUT>(hole, plug, am, xs, ys, mm, N, K, bs, st);
+            rc = launch_gemv_t<4, SPLIT, OUT>(hole, plug, am, xs, ys, mm, N, K, bs, act, st);
         if (rc != kOk)
             return rc;
     }
     return kOk;
 }
 
+/* one output f a warp at a time, for any K, blocksize and alignment */
+__global__ void htile_generic_gated_kernel(const uint8_t *hole, const uint8_t *plug, const float *absmax,
+                                           const __nv_bfloat16 *x, __nv_bfloat16 *h, int M, int F, int K, int bs, int act)
+{
+    const int mgroups = (M + 7) / 8;
+    const int64_t items = (int64_t)F * mgroups;
+    const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
+    for (int64_t it = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); it < items; it += warps) {
+        const int f = (int)(it / mgroups), m0 = (int)(it % mgroups) * 8;
+        float acc[2][8] = {};
+        for (int k = lane_id(); k < K; k += 32) {
+            float w[2];
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                const int64_t i = (2 * (int64_t)f + part) * K + k;
+                const int sh = (int)(i & 1) * 4;
+                w[part] = g_cells[(hole[i >> 1] >> sh) & 15][(plug[i >> 1] >> sh) & 15] * absmax[i / bs];
+            }
+#pragma unroll
+            for (int mm = 0; mm < 8; ++mm)
+                if (m0 + mm < M) {
+                    const float v = __bfloat162float(x[(int64_t)(m0 + mm) * K + k]);
+                    acc[0][mm] = fmaf(w[0], v, acc[0][mm]), acc[1][mm] = fmaf(w[1], v, acc[1][mm]);
+                }
+        }
+#pragma unroll
+        for (int mm = 0; mm < 8; ++mm) {
+            const float gate = warp_sum(acc[0][mm]), up = warp_sum(acc[1][mm]);
+            if (lane_id() == 0 && m0 + mm < M)
+                h[(int64_t)(m0 + mm) * F + f] = __float2bfloat16_rn(gated_value(gate, up, act));
+        }
+    }
+}
+
+bool gemv_supported(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, int N, int K, int bs)
+{
+    return K % 64 == 0 && bs % 64 == 0 && aligned_to(hole, 8) && aligned_to(plug, 8) && aligned_to(x, 16) &&
+           aligned_to(am, 4) && (int64_t)N * (K / 64) < (int64_t)0xFFFFFFFF;
+}
+unsigned generic_grid(int64_t items)
+{
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, (int64_t)sm_count() * 16));
+}
+
 } // namespace
+
+/* act(gate) * up of rows 2i and 2i + 1 for the shapes that the TMA kernels do not take */
+int htile_gemv_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
+                            int M, int N, int K, int bs, HtileMode mode, int act, cudaStream_t st)
+{
+    if (gemv_supported(hole, plug, am, x, N, K, bs))
+        return mode == kPrecise ? launch_gemv_slices<true, kOutGated>(hole, plug, am, x, h, M, N, K, bs, act, st)
+                                : launch_gemv_slices<false, kOutGated>(hole, plug, am, x, h, M, N, K, bs, act, st);
+    htile_generic_gated_kernel<<<generic_grid((int64_t)(N / 2) * ((M + 7) / 8)), 256, 0, st>>>(
+        hole, plug, am, x, static_cast<__nv_bfloat16 *>(h), M, N / 2, K, bs, act);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
+}
 
 /* Decode-shaped H-TILE.  Exposed to htile_gemm.cu's dispatcher. */
 int htile_gemv_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
                       OutKind yk, int M, int N, int K, int bs, HtileMode mode, cudaStream_t st)
 {
-    const bool fast_shape = K % 64 == 0 && bs % 64 == 0 && aligned_to(hole, 8) && aligned_to(plug, 8) &&
-                            aligned_to(x, 16) && aligned_to(am, 4) && (int64_t)N * (K / 64) < (int64_t)0xFFFFFFFF;
+    const bool fast_shape = gemv_supported(hole, plug, am, x, N, K, bs);
     if (htile_decode_supported(hole, plug, am, x, M, N, K, bs))
         return htile_decode_launch(hole, plug, am, x, y, yk, M, N, K, mode, st);
     if (M > 32 && htile_decode_supported(hole, plug, am, x, 32, N, K, bs)) {
@@ -332,13 +401,12 @@ int htile_gemv_launch(const uint8_t *hole, const uint8_t *plug, const float *am,
     }
     if (fast_shape) {
         if (mode == kPrecise)
-            return yk == kOutBF16 ? launch_gemv_slices<true, true>(hole, plug, am, x, y, M, N, K, bs, st)
-                                  : launch_gemv_slices<true, false>(hole, plug, am, x, y, M, N, K, bs, st);
-        return yk == kOutBF16 ? launch_gemv_slices<false, true>(hole, plug, am, x, y, M, N, K, bs, st)
-                              : launch_gemv_slices<false, false>(hole, plug, am, x, y, M, N, K, bs, st);
+            return yk == kOutBF16 ? launch_gemv_slices<true, kOutBF16>(hole, plug, am, x, y, M, N, K, bs, 0, st)
+                                  : launch_gemv_slices<true, kOutF32>(hole, plug, am, x, y, M, N, K, bs, 0, st);
+        return yk == kOutBF16 ? launch_gemv_slices<false, kOutBF16>(hole, plug, am, x, y, M, N, K, bs, 0, st)
+                              : launch_gemv_slices<false, kOutF32>(hole, plug, am, x, y, M, N, K, bs, 0, st);
     }
-    const int64_t items = (int64_t)N * ((M + 7) / 8);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, (int64_t)sm_count() * 16));
+    const unsigned grid = generic_grid((int64_t)N * ((M + 7) / 8));
     if (yk == kOutBF16)
         htile_generic_kernel<true><<<grid, 256, 0, st>>>(hole, plug, am, x, y, M, N, K, bs);
     else

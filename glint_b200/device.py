@@ -155,6 +155,92 @@ def htile_reference_abi(x: torch.Tensor, hole, plug, absmax, N: int, blocksize: 
     return out
 
 
+# ---- gated feed-forward projection (include/glint_htile.h)
+
+_ACTS = {"silu": 0, "gelu_tanh": 1}
+
+
+class GlintHtileGated(ctypes.Structure):
+    """struct GlintHtileGated of include/glint_htile.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("hole", "plug", "absmax", "x", "h", "work")] + \
+               [(n, ctypes.c_int) for n in ("M", "F", "K", "blocksize", "mode", "act")]
+
+
+def _gated_lib():
+    L = lib()
+    if not getattr(L, "_gated_bound", False):
+        L.glint_htile_gated_work_bytes.argtypes = [ctypes.POINTER(GlintHtileGated)]
+        L.glint_htile_gated_work_bytes.restype = ctypes.c_int64
+        L.glint_htile_gated_stream.argtypes = [ctypes.POINTER(GlintHtileGated), ctypes.c_void_p]
+        L.glint_htile_gated_stream.restype = ctypes.c_int
+        L._gated_bound = True
+    return L
+
+
+def pack_gated(gate: Sequence[torch.Tensor], up: Sequence[torch.Tensor], F: int, K: int, blocksize: int = 64):
+    """(hole, plug, absmax) of the [2 F, K] weight that htile_gated takes, from those of the gate and up
+    weights [F, K]: their rows in turn.  Done once, when a model is loaded; a row must be whole
+    bytes and blocks (K even and a multiple of blocksize)."""
+    if F < 0 or K < 0 or blocksize < 1 or K % 2 or K % blocksize:
+        raise ValueError(f"rows of {K} weights are not whole bytes and blocks of {blocksize}")
+    out = []
+    for g, u, per, dtype, nm in zip(gate, up, (K // 2, K // 2, K // blocksize), (torch.uint8, torch.uint8, torch.float32),
+                                    ("hole", "plug", "absmax")):
+        for t in (g, u):
+            if t.dtype != dtype or t.numel() != F * per:
+                raise ValueError(f"{nm} must be {F * per} of {dtype}, not {t.numel()} of {t.dtype}")
+        if g.device != u.device:
+            raise ValueError(f"gate and up must be on one device, not on {g.device} and {u.device}")
+        out.append(torch.stack([g.reshape(F, per), u.reshape(F, per)], 1).reshape(-1))
+    return tuple(out)
+
+
+def htile_gated(x: torch.Tensor, hole: torch.Tensor, plug: torch.Tensor, absmax: torch.Tensor, F: int,
+                blocksize: int = 64, mode="precise", act: str = "silu", out=None, stream=None) -> torch.Tensor:
+    """h[M, F] = act(x @ Wg^T) * (x @ Wu^T) in BF16, the planes those of the [2 F, K] weight with Wg's and
+    Wu's rows in turn (pack_gated).  act: "silu" or "gelu_tanh"; mode as htile's, both products
+    in f32 up to the activation."""
+    for t, nm in ((x, "x"), (hole, "hole"), (plug, "plug"), (absmax, "absmax")):
+        _cuda(t, nm)
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise ValueError("x must be a 2-D bfloat16 tensor [M, K]")
+    if mode not in _MODES or act not in _ACTS:
+        raise ValueError(f"mode must be 'precise' or 'fast' and act 'silu' or 'gelu_tanh', not {mode!r} and {act!r}")
+    M, K = x.shape
+    if F < 0 or blocksize < 1:
+        raise ValueError("F must be 0 or more and blocksize 1 or more")
+    n = 2 * F * K
+    if hole.dtype != torch.uint8 or plug.dtype != torch.uint8 or absmax.dtype != torch.float32 or \
+            hole.numel() < n_packed(n) or plug.numel() < n_packed(n) or absmax.numel() < n_absmax(n, blocksize):
+        raise ValueError(f"hole and plug must be uint8 planes and absmax the float32 scales of a [{2 * F}, {K}] weight")
+    dev = x.get_device()
+    if out is not None:
+        _cuda(out, "out")
+        if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, F):
+            raise ValueError(f"out must be a bfloat16 tensor of shape {(M, F)}")
+        for t in (x, hole, plug, absmax):
+            if out.data_ptr() < t.data_ptr() + t.numel() * t.element_size() and t.data_ptr() < out.data_ptr() + 2 * M * F:
+                raise ValueError("out overlaps an input")
+    if dev != torch.cuda.current_device() or any(t.get_device() != dev for t in (hole, plug, absmax, out) if t is not None):
+        raise ValueError("all tensors must be on the current device")
+    L, s = _gated_lib(), stream if stream is not None else torch.cuda.current_stream()
+
+    def memory(shape, dtype):  # of the stream that writes it
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=x.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=x.device)
+    out = out if out is not None else memory((M, F), torch.bfloat16)
+    a = GlintHtileGated(hole.data_ptr(), plug.data_ptr(), absmax.data_ptr(), x.data_ptr(), out.data_ptr(), None, M, F, K,
+                        blocksize, _MODES[mode], _ACTS[act])
+    need = L.glint_htile_gated_work_bytes(ctypes.byref(a))
+    work = memory((need,), torch.uint8) if need > 0 else None
+    if work is not None:
+        a.work = work.data_ptr()
+    _check(L.glint_htile_gated_stream(ctypes.byref(a), s.cuda_stream), "glint_htile_gated_stream")
+    return out
+
+
 # ---- K-major decode: parent-only GEMV + activation-selected plug correction ----
 # (include/glint_km.h; the reference's Mojo decoders' glint_gemv_km, select_topk,
 # apply_corr_k, transpose_plug / transpose_scales)

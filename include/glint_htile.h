@@ -55,6 +55,31 @@ int glint_htile_stream(
     const glint_bf16_t *d_x, void *d_y, int y_dtype,
     int M, int N, int K, int blocksize, int mode, cudaStream_t stream);
 
+/* The gated feed-forward projection: both products, the activation and its product in one call.
+ * W [2 F, K] holds the gate and up rows in turn (row 2f: gate f, row 2f + 1: up f), packed as
+ * any GLINT weight of 2 F rows:
+ *   h[m, f] = act(g) u, g = W[2f] . x[m], u = W[2f + 1] . x[m]   (both in f32)
+ *   GLINT_ACT_SILU       act(g) = g / (1 + exp(-g))
+ *   GLINT_ACT_GELU_TANH  act(g) = g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2
+ * x BF16 [M, K], h BF16 [M, F], row-major; h overlaps nothing else.  mode as above.  Any M, F,
+ * K, blocksize and pointer alignment is accepted; blocksize 64, K % 256 == 0 and 16-byte
+ * aligned pointers take the streaming and tensor-core kernels.  work:
+ * glint_htile_gated_work_bytes() of 16-byte aligned device memory (by sizes, mode and
+ * alignment only; 0: NULL will do), the call's own until it completes, of any content; -1
+ * for arguments that the call itself refuses. */
+#define GLINT_ACT_SILU 0
+#define GLINT_ACT_GELU_TANH 1
+typedef struct GlintHtileGated {
+    const uint8_t *hole, *plug;
+    const float *absmax;
+    const glint_bf16_t *x;
+    glint_bf16_t *h;
+    void *work;
+    int M, F, K, blocksize, mode, act;
+} GlintHtileGated;
+int64_t glint_htile_gated_work_bytes(const GlintHtileGated *a);
+int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream);
+
 /* Same contract as glint_htile_stream for decode shapes, for callers that cannot
  * let a library allocate device memory (for example a serving process whose own
  * allocator already owns all free HBM, or an integration whose memory budget is
