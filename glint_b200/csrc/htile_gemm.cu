@@ -69,11 +69,20 @@ constexpr int XSTAGES = 5; /* shared-memory ring of activation tiles (freed by t
 constexpr int PSTAGES = 2; /* shared-memory ring of plane tiles, 4 K steps each (freed by the dequantisers) */
 constexpr int PSTEPS = 4;  /* K steps per plane stage: 128-byte plane rows, one absmax box */
 constexpr int WSLOTS = 8;  /* TMEM weight ring */
-constexpr int kDeqWarps = 8, kEpiWarps = 4;
-constexpr int kDeq0 = 2, kEpi0 = kDeq0 + kDeqWarps; /* first warp of each role */
-constexpr int kPlaneWarp = kEpi0 + kEpiWarps;       /* plane producer */
-constexpr int kThreads = (kPlaneWarp + 1) * 32;
-constexpr int kWpt = BK * 4 / kDeqWarps;            /* 32 weights per dequantiser thread and K step */
+constexpr int kDeq0 = 2;                 /* first dequantiser warp */
+constexpr int kDeqWarps = 8;
+constexpr int kWpt = BK * 4 / kDeqWarps; /* 32 weights per dequantiser thread and K step */
+/* Warps of the product alone and with a gated epilogue, whose accumulator is busy longer
+ * (an exchange, an exponential and a division for each output): two warps a quadrant there. */
+template <bool GATED>
+struct GemmCfg {
+    static constexpr int kEpiWarps = GATED ? 8 : 4;
+    static constexpr int kEpi0 = kDeq0 + kDeqWarps;
+    static constexpr int kPlaneWarp = kEpi0 + kEpiWarps; /* plane producer */
+    static constexpr int kThreads = (kPlaneWarp + 1) * 32;
+    static constexpr int kChunks = BMX / 32 / (kEpiWarps / 4); /* of 32 columns, an epilogue warp's */
+    static constexpr int kAtOnce = GATED ? 2 : 4; /* contributors of a split tile loaded before they are added */
+};
 constexpr int kPartFloats = 8 * 32 * 32;            /* one epilogue warp's share of a partial tile */
 constexpr int kStageX = BMH * BK * 2;               /* 16 KB */
 constexpr int kPlaneBox = BN * PSTEPS * BK / 2;     /* 16 KB: 128 rows x 128 B */
@@ -187,6 +196,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                    "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -206,6 +224,16 @@ struct Ring {
     }
 };
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+/* the loads into r have arrived: its values are this statement's, so no use moves ahead of it */
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 /* UMMA shared-memory descriptor, K-major, 128-byte swizzle: 8-row atoms of
@@ -304,22 +332,36 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
                 *yp = __uint_as_float(v[j]);
     }
 }
-/* h[m, n / 2] = act(y[m, n]) y[m, n + 1], n even, of rows m0 .. m0+jl-1 from 32 accumulator values
- * of each lane's column n (pairs of lanes hold n and n + 1; n_cols is even).  Of two rows each lane of a pair
- * keeps one: the even lane takes up of the first for gate of the second. */
-__device__ __forceinline__ void store_gated(void *h, int n_cols, int act, const uint32_t (&v)[32], int m0, int jl, int n)
+/* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of 16
+ * rows.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
+ * second.  o: 8 outputs, of rows 2i + (n & 1), as BF16 pairs. */
+__device__ __forceinline__ void gated16(const uint32_t (&v)[16], bool up, int act, uint32_t (&o)[4])
 {
-    const bool up = n & 1;
-    const size_t ld = (size_t)(n_cols / 2);
-    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(h) + (size_t)(m0 + (up ? 1 : 0)) * ld + n / 2;
-    const bool live = n < n_cols;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2, p += 2 * ld) {
-        const float keep = __uint_as_float(up ? v[j + 1] : v[j]), give = __uint_as_float(up ? v[j] : v[j + 1]);
-        const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
-        if (live && j + (up ? 1 : 0) < jl)
-            *p = __float2bfloat16_rn(up ? gated_value(got, keep, act) : gated_value(keep, got, act));
+    for (int i = 0; i < 4; ++i) {
+        float h[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t a = v[4 * i + 2 * j], b = v[4 * i + 2 * j + 1];
+            const float keep = __uint_as_float(up ? b : a), give = __uint_as_float(up ? a : b);
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
+            h[j] = gated_value(up ? got : keep, up ? keep : got, act);
+        }
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(h[0], h[1]);
+        o[i] = *reinterpret_cast<const uint32_t *>(&b2);
     }
+}
+/* them into column n / 2 of h [.., n_cols / 2], rows m0 .. m0+jl-1 */
+__device__ __forceinline__ void store_gated(void *h, int n_cols, const uint32_t (&o)[4], int m0, int jl, int n)
+{
+    if (n >= n_cols)
+        return;
+    const size_t ld = (size_t)(n_cols / 2);
+    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(h) + (size_t)(m0 + (n & 1)) * ld + n / 2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j, p += 2 * ld)
+        if (2 * j + (n & 1) < jl)
+            *p = __ushort_as_bfloat16((unsigned short)(o[j / 2] >> (16 * (j & 1))));
 }
 /* y rows m0 .. m0+jl-1 at column n: this call's y; in a gathered call this
  * rank's y and, with `peers`, every other rank's (over NVLink, starting with the
@@ -371,9 +413,10 @@ __device__ __forceinline__ void copy_rows_to_peers(const GatherArgs &g, int m0, 
 }
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThreads, 1)
     htile_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs args)
 {
+    using C = GemmCfg<GATED>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     float *lut = reinterpret_cast<float *>(smem_raw); /* at the start: its address folds into the loads */
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw + kLutBytes) + 1023) &
@@ -401,7 +444,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const Segments seg0{0, ub, ue};
     int T, ga, gb;
 
-    for (int i = threadIdx.x; i < 256 * 32; i += kThreads)
+    for (int i = threadIdx.x; i < 256 * 32; i += C::kThreads)
         lut[(i >> 5) * 64 + (i & 31)] = (&g_cells[0][0])[i >> 5];
     if (threadIdx.x == 0) {
         for (int s = 0; s < XSTAGES; ++s) {
@@ -417,7 +460,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(&w_empty[a], 1);
         }
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 2 * kEpiWarps);
+        mbar_init(acc_empty, 2 * C::kEpiWarps);
         mbar_init(mma_done, 1);
         *cta_done = 0;
         mbar_init_fence();
@@ -459,7 +502,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                               &g_glint_kernel_error);
             }
         }
-    } else if (warp == kPlaneWarp) {
+    } else if (warp == C::kPlaneWarp) {
         /* ---- plane producer (both CTAs): hole, plug and absmax of this CTA's weight rows */
         if (lane == 0) {
             Ring st;
@@ -521,7 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_wait_bounded(mma_done, 0, &g_glint_kernel_error);
         }
         __syncwarp();
-    } else if (warp < kEpi0) {
+    } else if (warp < C::kEpi0) {
         /* ---- dequantisers: thread -> weight row r (TMEM lane), kWpt weights (K part kq) */
         const int q = warp & 3, kq = (warp - kDeq0) >> 2;
         const int r = q * 32 + (int)lane;
@@ -593,7 +636,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
          * contributor stores its f32 partial (L2 only) and counts itself in; the
          * last one adds all partials in K order, so y does not depend on which
          * pair finished last. */
-        const int q = warp & 3;
+        const int q = warp & 3, c0 = GATED ? (warp - C::kEpi0) / 4 * C::kChunks : 0, c1 = c0 + C::kChunks;
         const uint32_t accempty0 = peer_addr(saddr(acc_empty), 0);
         const uint32_t tb = tmem + ((uint32_t)(q * 32) << 16) + kAccCol;
         int t = 0;
@@ -606,20 +649,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int mlim = min(BMX, args.M - m0);
             const bool whole = ga == 0 && gb == G;
             if (whole) {
+                [[maybe_unused]] uint32_t o[2 * C::kChunks][4];
+                if constexpr (GATED) {
+                    /* the outputs stay in registers until the accumulator is released: their stores
+                     * run beside the next tile's products */
+#pragma unroll
+                    for (int c = 0; c < 2 * C::kChunks; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(tb + c0 * 32 + c * 16, v);
+                        tmem_ld_wait(v);
+                        gated16(v, n & 1, args.act, o[c]);
+                    }
+                } else {
 #pragma unroll 1
-                for (int c = 0; c < BMX / 32 && c * 32 < mlim; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(tb + c * 32, v);
-                    tmem_ld_wait();
-                    if constexpr (GATED)
-                        store_gated(args.y, args.N, args.act, v, m0 + c * 32, min(32, mlim - c * 32), n);
-                    else
+                    for (int c = 0; c < BMX / 32 && c * 32 < mlim; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(tb + c * 32, v);
+                        tmem_ld_wait();
                         store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, false);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_remote(accempty0);
+                if constexpr (GATED) {
+#pragma unroll
+                    for (int c = 0; c < 2 * C::kChunks; ++c)
+                        store_gated(args.y, args.N, o[c], m0 + c0 * 32 + c * 16, mlim - c0 * 32 - c * 16, n);
+                }
                 if (!GATED && args.ga.world > 1 && n < args.N) {
                     if (args.y_bf16)
                         copy_rows_to_peers<__nv_bfloat16>(args.ga, m0, mlim, args.ga.n0 + n);
@@ -632,7 +690,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int slot = ub >= T * G ? 0 : 1;
             float *mine = args.ws + ((((size_t)pair * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats;
 #pragma unroll 1
-            for (int c = 0; c < BMX / 32; ++c) {
+            for (int c = c0; c < c1; ++c) {
                 uint32_t v[32];
                 tmem_ld32(tb + c * 32, v);
                 tmem_ld_wait();
@@ -646,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 mbar_arrive_remote(accempty0); /* accumulator free: the rest works from memory */
             __threadfence();
             __syncwarp();
-            int *cnt = args.counters + ((size_t)T * 2 + rank) * 4 + q;
+            int *cnt = args.counters + ((size_t)T * 2 + rank) * C::kEpiWarps + c0 / C::kChunks * 4 + q;
             const int pf = pair_of(args, T * G, npairs), pl = pair_of(args, (T + 1) * G - 1, npairs);
             int prev = 0;
             if (lane == 0)
@@ -660,7 +718,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (lane == 0)
                 *cnt = 0;
 #pragma unroll 1
-            for (int c = 0; c < BMX / 32 && c * 32 < mlim; ++c) {
+            for (int c = c0; c < c1 && c * 32 < mlim; ++c) {
                 uint32_t v[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -669,10 +727,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 16; ++j)
                         acc[j] = 0.f;
 #pragma unroll 1
-                    for (int p0 = pf; p0 <= pl; p0 += 4) {
-                        float part[4][16];
+                    for (int p0 = pf; p0 <= pl; p0 += C::kAtOnce) {
+                        float part[C::kAtOnce][16];
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
+                        for (int b = 0; b < C::kAtOnce; ++b) {
                             const int pq = min(p0 + b, pl);
                             const int sq = unit_begin(args, pq, npairs) >= T * G ? 0 : 1;
                             const float *src = args.ws + ((((size_t)pq * 2 + sq) * 2 + rank) * 4 + q) * kPartFloats +
@@ -682,25 +740,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 part[b][j] = __ldcg(src + j * 32);
                         }
 #pragma unroll
-                        for (int b = 0; b < 4; ++b)
+                        for (int b = 0; b < C::kAtOnce; ++b)
                             if (p0 + b <= pl) {
 #pragma unroll
                                 for (int j = 0; j < 16; ++j)
                                     acc[j] += part[b][j];
                             }
                     }
+                    if constexpr (GATED) {
+                        uint32_t u[16], o[4];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        v[h * 16 + j] = __float_as_uint(acc[j]);
+                        for (int j = 0; j < 16; ++j)
+                            u[j] = __float_as_uint(acc[j]);
+                        gated16(u, n & 1, args.act, o);
+                        store_gated(args.y, args.N, o, m0 + c * 32 + h * 16, mlim - c * 32 - h * 16, n);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            v[h * 16 + j] = __float_as_uint(acc[j]);
+                    }
                 }
-                if constexpr (GATED)
-                    store_gated(args.y, args.N, args.act, v, m0 + c * 32, min(32, mlim - c * 32), n);
-                else
+                if constexpr (!GATED)
                     store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, true);
             }
         }
         if (!GATED && args.ga.world > 0)
-            gather_complete(args.ga, kEpiWarps, lane, cta_done, &g_glint_kernel_error);
+            gather_complete(args.ga, C::kEpiWarps, lane, cta_done, &g_glint_kernel_error);
     }
     tc_fence_before();
     __syncthreads();
@@ -757,16 +822,6 @@ struct PreciseArgs {
     int mtiles, tiles;
     int act; /* gated kernel: of the gate rows */
 };
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15])
-                 : "r"(taddr));
-}
 
 __device__ __forceinline__ uint32_t split_hilo(float c)
 {
@@ -1023,11 +1078,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
                 continue;
             const int jl = min(32, args.M - m0);
             if constexpr (GATED) {
-                uint32_t v[32];
 #pragma unroll
-                for (int jj = 0; jj < 32; ++jj)
-                    v[jj] = __float_as_uint(run[jj]);
-                store_gated(args.y, args.N, args.act, v, m0, jl, n);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[16], o[4];
+#pragma unroll
+                    for (int jj = 0; jj < 16; ++jj)
+                        v[jj] = __float_as_uint(run[h * 16 + jj]);
+                    gated16(v, n & 1, args.act, o);
+                    store_gated(args.y, args.N, o, m0 + h * 16, jl - h * 16, n);
+                }
                 continue;
             }
             if (!nok)
@@ -1566,7 +1625,7 @@ int max_pairs(int kind = 0)
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2 * std::max(1, sm_count() / 2));
-    cfg.blockDim = dim3(kind == 2 ? I8Cfg<false>::kThreads : kind ? PThreads : kThreads);
+    cfg.blockDim = dim3(kind == 2 ? I8Cfg<false>::kThreads : kind ? PThreads : GemmCfg<false>::kThreads);
     cfg.dynamicSmemBytes = kind == 2 ? I8Cfg<false>::kSmem : kind ? PSmemBytes : kSmemBytes;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -1635,7 +1694,7 @@ int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, 
     const int pairs = gemm_plan(a);
     if (!gemm_scratch(st, part_floats(pairs), (size_t)a.tiles * 8, &a.ws, &a.counters))
         return kLaunch;
-    htile_gemm_kernel<false><<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, a);
+    htile_gemm_kernel<false><<<2 * pairs, GemmCfg<false>::kThreads, kSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
@@ -1696,7 +1755,7 @@ int64_t htile_gemm_gated_work(int M, int N, int K)
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
     const int pairs = gemm_plan(a);
-    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 8 * sizeof(int)) : 0;
+    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int)) : 0;
 }
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
                             void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
@@ -1712,10 +1771,10 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     if (a.S) {
         a.ws = static_cast<float *>(work);
         a.counters = reinterpret_cast<int *>(a.ws + part_floats(pairs));
-        if (cudaMemsetAsync(a.counters, 0, (size_t)a.S * 8 * sizeof(int), st) != cudaSuccess)
+        if (cudaMemsetAsync(a.counters, 0, (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int), st) != cudaSuccess)
             return kLaunch;
     }
-    htile_gemm_kernel<true><<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, a);
+    htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
