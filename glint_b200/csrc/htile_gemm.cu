@@ -70,13 +70,14 @@ constexpr int PSTAGES = 2; /* shared-memory ring of plane tiles, 4 K steps each 
 constexpr int PSTEPS = 4;  /* K steps per plane stage: 128-byte plane rows, one absmax box */
 constexpr int WSLOTS = 8;  /* TMEM weight ring */
 constexpr int kDeq0 = 2;                 /* first dequantiser warp */
-constexpr int kDeqWarps = 8;
-constexpr int kWpt = BK * 4 / kDeqWarps; /* 32 weights per dequantiser thread and K step */
+constexpr int kStepWarps = 8;             /* dequantisers of a K step */
+constexpr int kWpt = BK * 4 / kStepWarps; /* 32 weights per dequantiser thread and K step */
 /* Warps of the product alone and with a gated epilogue, whose accumulator is busy longer
  * (an exchange, an exponential and a division for each output): two warps a quadrant there. */
 template <bool GATED>
 struct GemmCfg {
-    static constexpr int kEpiWarps = GATED ? 8 : 4;
+    static constexpr int kGroups = GATED ? 2 : 1; /* of dequantisers, that take K steps in turn */
+    static constexpr int kDeqWarps = kStepWarps * kGroups, kEpiWarps = GATED ? 8 : 4;
     static constexpr int kEpi0 = kDeq0 + kDeqWarps;
     static constexpr int kPlaneWarp = kEpi0 + kEpiWarps; /* plane producer */
     static constexpr int kThreads = (kPlaneWarp + 1) * 32;
@@ -95,6 +96,7 @@ constexpr int kLutBytes = 256 * 256;
 constexpr int kSmemBytes = kLutBytes + 1024 + XSTAGES * kStageX + PSTAGES * kPStage + 512;
 constexpr uint32_t kAccCol = 0, kWCol = 256; /* TMEM column bases: accumulator, weight ring */
 static_assert(kWCol + WSLOTS * (BK / 2) <= 512, "TMEM columns");
+static_assert(WSLOTS >= XSTAGES, "a step's barrier also frees its x tile");
 constexpr uint32_t kTmemCols = 512;
 
 /* ---- cluster / pair primitives ------------------------------------------------ */
@@ -182,6 +184,15 @@ __device__ __forceinline__ void umma_pair_ts_bf16(uint32_t d, uint32_t a, uint64
 __device__ __forceinline__ void umma_commit_to(uint32_t cluster_addr)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
+/* the same on the barrier at one place in both CTAs of the pair.  One instruction for the two: a
+ * commit takes the issuing thread some 150 cycles, and four of them a K step held the UMMAs up. */
+__device__ __forceinline__ void umma_commit_pair(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     saddr(bar)),
+                 "h"((uint16_t)3)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
@@ -423,12 +434,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                                                 ~uintptr_t(1023));
     uint8_t *xring = smem, *pring = smem + XSTAGES * kStageX;
     uint64_t *x_full = reinterpret_cast<uint64_t *>(pring + PSTAGES * kPStage); /* leader: both x halves */
-    uint64_t *x_empty = x_full + XSTAGES; /* x tile read by the pair UMMAs */
-    uint64_t *p_full = x_empty + XSTAGES; /* this CTA's planes landed */
+    uint64_t *p_full = x_full + XSTAGES;  /* this CTA's planes landed */
     uint64_t *p_empty = p_full + PSTAGES; /* planes read by this CTA's dequantisers */
     uint64_t *w_full = p_empty + PSTAGES; /* leader: both CTAs' weight slots written */
-    uint64_t *w_empty = w_full + WSLOTS; /* weight slot read by the pair UMMAs */
-    uint64_t *acc_full = w_empty + WSLOTS;
+    /* K step read by the pair's UMMAs: its weight slot is free, and so is its x tile */
+    uint64_t *step_done = w_full + WSLOTS;
+    uint64_t *acc_full = step_done + WSLOTS;
     uint64_t *acc_empty = acc_full + 1;  /* leader: both CTAs' epilogues drained */
     uint64_t *mma_done = acc_empty + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
@@ -447,17 +458,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
     for (int i = threadIdx.x; i < 256 * 32; i += C::kThreads)
         lut[(i >> 5) * 64 + (i & 31)] = (&g_cells[0][0])[i >> 5];
     if (threadIdx.x == 0) {
-        for (int s = 0; s < XSTAGES; ++s) {
+        for (int s = 0; s < XSTAGES; ++s)
             mbar_init(&x_full[s], 1);
-            mbar_init(&x_empty[s], 1);
-        }
         for (int s = 0; s < PSTAGES; ++s) {
             mbar_init(&p_full[s], 1);
-            mbar_init(&p_empty[s], kDeqWarps);
+            mbar_init(&p_empty[s], C::kDeqWarps);
         }
         for (int a = 0; a < WSLOTS; ++a) {
-            mbar_init(&w_full[a], 2 * kDeqWarps);
-            mbar_init(&w_empty[a], 1);
+            mbar_init(&w_full[a], 2 * kStepWarps);
+            mbar_init(&step_done[a], 1);
         }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 2 * C::kEpiWarps);
@@ -480,14 +489,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
     if (warp == 0) {
         /* ---- activation producer (both CTAs): this CTA's half of the x tile */
         if (lane == 0) {
-            Ring st;
+            Ring st, back; /* back: the step XSTAGES before, whose tile the next one replaces */
             int64_t issued = 0;
             for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
                 const int mr = (T % args.mtiles) * BMX + (int)rank * BMH;
                 for (int ks = ga * PSTEPS; ks < gb * PSTEPS && alive; ++ks, st.next<XSTAGES>()) {
-                    /* the first use of a stage waits on parity 1: returns at once */
-                    if (!wait_or_fail(&x_empty[st.i], st.ph ^ 1u, alive))
-                        break;
+                    if (issued >= XSTAGES) {
+                        if (!wait_or_fail(&step_done[back.i], back.ph, alive))
+                            break;
+                        back.next<WSLOTS>();
+                    }
                     if (leader)
                         mbar_expect_tx(&x_full[st.i], 2 * kStageX);
                     tma_load_2d_pair(xring + st.i * kStageX, &maps.x, peer_addr(saddr(&x_full[st.i]), 0), ks * BK, mr);
@@ -532,8 +543,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         if (leader && lane == 0) {
             Ring st, ws;
             int t = 0;
-            const uint32_t empty0 = peer_addr(saddr(&x_empty[0]), 0), empty1 = peer_addr(saddr(&x_empty[0]), 1);
-            const uint32_t wempty0 = peer_addr(saddr(&w_empty[0]), 0), wempty1 = peer_addr(saddr(&w_empty[0]), 1);
             for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb); ++t) {
                 if (t >= 1 && !wait_or_fail(acc_empty, (uint32_t)(t - 1) & 1u, alive))
                     break;
@@ -549,15 +558,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                     for (int kk = 0; kk < BK / 16; ++kk)
                         umma_pair_ts_bf16(tmem + kAccCol, wa + kk * 8, sw128_desc(xs + kk * 32), kIdesc,
                                           (ks > k0 || kk > 0) ? 1u : 0u);
-                    umma_commit_to(empty0 + (uint32_t)st.i * 8u);
-                    umma_commit_to(empty1 + (uint32_t)st.i * 8u);
-                    umma_commit_to(wempty0 + (uint32_t)ws.i * 8u);
-                    umma_commit_to(wempty1 + (uint32_t)ws.i * 8u);
+                    umma_commit_pair(&step_done[ws.i]);
                 }
-                if (alive) {
-                    umma_commit_to(peer_addr(saddr(acc_full), 0));
-                    umma_commit_to(peer_addr(saddr(acc_full), 1));
-                }
+                if (alive)
+                    umma_commit_pair(acc_full);
             }
             /* all UMMAs issued by this thread have completed before TMEM is released */
             umma_commit_to(peer_addr(saddr(mma_done), 0));
@@ -566,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         __syncwarp();
     } else if (warp < C::kEpi0) {
         /* ---- dequantisers: thread -> weight row r (TMEM lane), kWpt weights (K part kq) */
-        const int q = warp & 3, kq = (warp - kDeq0) >> 2;
+        const int q = warp & 3, kq = ((warp - kDeq0) >> 2) & 1, group = C::kGroups > 1 ? (warp - kDeq0) / kStepWarps : 0;
         const int r = q * 32 + (int)lane;
         const uint32_t lutb = saddr(lut), lane4 = lane * 4u;
         /* this thread's kWpt/2 plane bytes of K step j sit at byte j*32 + kq*kWpt/2 of
@@ -576,31 +580,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         const uint32_t tw = tmem + ((uint32_t)(q * 32) << 16) + kWCol + (uint32_t)kq * (kWpt / 2);
         const uint32_t wfull0 = peer_addr(saddr(&w_full[0]), 0);
         float4 sc4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        Ring st, ws;
+        Ring st, ws{group, 0};
+        auto onward = [&] {
+            if ((ws.i += C::kGroups) >= WSLOTS)
+                ws.i -= WSLOTS, ws.ph ^= 1u;
+        };
         for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
-            for (int ks = ga * PSTEPS; ks < gb * PSTEPS && alive; ++ks, ws.next<WSLOTS>()) {
+            for (int ks = ga * PSTEPS + group; ks < gb * PSTEPS && alive; ks += C::kGroups, onward()) {
                 const int j = ks & (PSTEPS - 1);
-                if (j == 0 && !warp_wait(&p_full[st.i], st.ph, alive))
+                if (j == group && !warp_wait(&p_full[st.i], st.ph, alive))
                     break;
                 const uint32_t ps = saddr(pring + st.i * kPStage);
                 const uint32_t kbj = (uint32_t)j * (BK / 2) + kb;
                 const uint32_t pofs = prow + ((((kbj >> 4) ^ pswz) << 4) | (kbj & 15u));
                 const uint4 H = lds128(ps + pofs), P = lds128(ps + kPlaneBox + pofs);
                 const uint32_t hw[4] = {H.x, H.y, H.z, H.w}, pw[4] = {P.x, P.y, P.z, P.w};
-                if (j == 0) {
+                if (j == group) {
                     const uint4 a4 = lds128(ps + 2 * kPlaneBox + (uint32_t)r * 16u);
                     sc4 = make_float4(__uint_as_float(a4.x), __uint_as_float(a4.y), __uint_as_float(a4.z),
                                       __uint_as_float(a4.w));
                 }
                 const float sc = j == 0 ? sc4.x : j == 1 ? sc4.y : j == 2 ? sc4.z : sc4.w;
-                if (j == PSTEPS - 1) {
+                if (j == PSTEPS - C::kGroups + group) {
                     __syncwarp();
                     if (lane == 0)
                         mbar_arrive(&p_empty[st.i]);
                     st.next<PSTAGES>();
                 }
                 /* the first use of a slot waits on parity 1: returns at once */
-                if (!warp_wait(&w_empty[ws.i], ws.ph ^ 1u, alive))
+                if (!warp_wait(&step_done[ws.i], ws.ph ^ 1u, alive))
                     break;
                 tc_fence_after();
                 const uint64_t sc2 = pack2f(sc, sc);
