@@ -7,11 +7,12 @@
  *   (o1, o2) = (y1 c - y2 s, y2 c + y1 s)   on the pairs (i, i + R / 2) or (2i, 2i + 1)
  *
  * A warp takes a token, or a part of its heads where tokens are few: 16 values a lane, so
- * 4 (D = 128) or 8 heads at a time, the next ones' loads under way.  Its angles are the
+ * 4 (D = 128) or 8 heads a step, the next step's loads under way.  Its angles are the
  * same for every head, so each is computed once, in 64 bits (a far position times a frequency
- * is hundreds of thousands of radians, of which f32 would keep two digits), and stays in
- * registers as (c, +-s) of the lane's 16 places.  A value's partner is in the same lane
- * (2i, 2i + 1), comes by shuffles (R / 2 a multiple of 16) or through shared memory.
+ * is hundreds of thousands of radians, of which f32 would keep two digits), and (c, s) of the
+ * lane's 8 pairs stay in registers.  A lane's 16 values are two runs of 8 that are partners of
+ * one another (i, i + R / 2; R / 2 a multiple of 8) or 16 neighbours (2i, 2i + 1), so no value
+ * leaves its lane; other R exchange through shared memory.
  *
  * The mean is summed in 64 bits and products and sums are rounded one by one, as they stand
  * above: the result depends on no order, and what is then rounded to BF16 and to 4 bits is
@@ -21,6 +22,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -28,6 +30,8 @@ namespace glint {
 namespace {
 
 constexpr int kWarps = 8;
+/* where a value's partner is: R / 2 places on, in whole runs of 8 or not; beside it */
+enum Pairing : int { kRuns, kAny, kBeside };
 
 struct Args {
     GlintRope a;
@@ -36,65 +40,85 @@ struct Args {
     const int *slots;
     int64_t v_tok, v_head;
     int page_log2;
-    int rows;           /* heads of a token: q, k and, with the cache, v */
-    int chunk, chunks;  /* of them a warp takes; such parts a token */
-    int64_t warps;      /* tokens * chunks */
+    int q_steps, k_steps;     /* of a token's heads; v, with the cache, takes as many as k */
+    int steps, chunk, chunks; /* in all; of them a warp takes; such parts a token */
+    int64_t warps;            /* tokens * chunks */
 };
 
-/* 16 values as BF16 pairs, by loads that may follow a store to the same place */
+/* 8 values as BF16 pairs, by loads that may follow a store to the same place */
 template <bool VEC>
-__device__ __forceinline__ void get16(const __nv_bfloat16 *p, uint32_t (&x)[8])
+__device__ __forceinline__ void get8(const __nv_bfloat16 *p, uint32_t *x)
 {
     if constexpr (VEC) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 w = reinterpret_cast<const uint4 *>(p)[i];
-            x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
-        }
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 4; ++i)
             x[i] = (uint32_t)__bfloat16_as_ushort(p[2 * i]) | ((uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16);
     }
 }
 template <bool VEC>
-__device__ __forceinline__ void put16(__nv_bfloat16 *p, const uint32_t (&x)[8])
+__device__ __forceinline__ void put8(__nv_bfloat16 *p, const uint32_t *x)
 {
     if constexpr (VEC) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            reinterpret_cast<uint4 *>(p)[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        *reinterpret_cast<uint4 *>(p) = make_uint4(x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             p[2 * i] = __ushort_as_bfloat16((unsigned short)(x[i] & 0xFFFFu));
             p[2 * i + 1] = __ushort_as_bfloat16((unsigned short)(x[i] >> 16));
         }
     }
 }
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t round2(float lo, float hi)
+{
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&b);
+}
+__device__ __forceinline__ uint32_t round2(uint64_t v)
+{
+    float lo, hi;
+    unpack2f(v, lo, hi);
+    return round2(lo, hi);
+}
 
-template <int D, bool VEC, bool APPEND>
+template <int D, Pairing P, bool VEC, bool APPEND>
 __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
 {
     constexpr int L = D / 16, N = 32 / L; /* lanes a head, heads a step */
+    constexpr bool kMoves = APPEND && P == kRuns; /* values go to the lanes that quantise them */
     __shared__ float2 turns[kWarps][D / 2];
-    __shared__ float4 mixed[kWarps][N * D / 4];
+    /* a step's heads, f32 values for partners to read or BF16 ones; 16 bytes keep rows off one another's banks */
+    constexpr int kRow = (P == kAny ? 4 : 2) * D + 16;
+    __shared__ __align__(16) uint8_t mixed[P == kAny || kMoves ? kWarps : 1][N * kRow];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
     if (w >= g.warps)
         return; /* no barrier of the block follows */
     const GlintRope &a = g.a;
-    const int t = (int)(w / g.chunks), r0 = (int)(w - (int64_t)t * g.chunks) * g.chunk, r1 = min(g.rows, r0 + g.chunk);
-    const int e0 = lane % L * 16; /* the lane's first place in its head */
-    const int keys = a.heads, values = a.heads + a.kv_heads;
+    const int t = (int)(w / g.chunks), s0 = (int)(w - (int64_t)t * g.chunks) * g.chunk, s1 = min(g.steps, s0 + g.chunk);
+    const int l = lane % L, in = lane / L, half = a.half;
+    /* the lane's runs of 8 values: partners while there are any (then the lane turns them), else neighbours */
+    const bool partners = P == kRuns && l < half / 8;
+    const int ea = P != kRuns ? 16 * l : partners ? 8 * l : 2 * half + 16 * (l - half / 8);
+    const int eb = partners ? ea + half : ea + 8;
 
-    auto load = [&](int r, uint32_t (&x)[8]) {
-        r += lane / L;
-        const __nv_bfloat16 *p = r < keys ? a.q + t * a.q_tok + r * a.q_head
-                                 : !APPEND || r < values ? a.k + t * a.k_tok + (r - keys) * a.k_head
-                                                         : g.v + t * g.v_tok + (r - values) * g.v_head;
-        if (r < r1) {
-            get16<VEC>(p + e0, x);
+    const __nv_bfloat16 *const q = a.q + t * a.q_tok, *const k = a.k + t * a.k_tok, *const v = APPEND ? g.v + t * g.v_tok : nullptr;
+    const int k0 = g.q_steps, v0 = g.q_steps + g.k_steps; /* first steps of k and v */
+    auto load = [&](int s, uint32_t (&x)[8]) {
+        const bool query = s < k0, value = APPEND && s >= v0;
+        const int row = (s - (query ? 0 : value ? v0 : k0)) * N + in;
+        const __nv_bfloat16 *p = (query ? q : value ? v : k) + row * (query ? a.q_head : value ? g.v_head : a.k_head);
+        if (s < s1 && row < (query ? a.heads : a.kv_heads)) {
+            get8<VEC>(p + (value ? 16 * l : ea), x);
+            get8<VEC>(p + (value ? 16 * l + 8 : eb), x + 4);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -102,41 +126,42 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
         }
     };
     uint32_t x[8];
-    load(r0, x);
+    load(s0, x);
 
-    const double pos = (double)a.positions[t];
-    for (int i = lane; i < a.half; i += 32) {
-        double s, c;
-        sincos(pos * (double)a.inv_freq[i], &s, &c);
-        turns[warp][i] = make_float2((float)(c * a.scale), (float)(s * a.scale));
-    }
-    __syncwarp();
-    /* o = y c + partner s; behind the rotated part c = 1, the partner 0 and s = -0: -0 is what
-     * may be added to any y */
-    uint64_t c2[8], s2[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float c[2], s[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int e = e0 + 2 * i + j;
-            const bool second = a.interleaved ? j : e >= a.half;
-            const float2 v = turns[warp][e < 2 * a.half ? (a.interleaved ? e / 2 : second ? e - a.half : e) : 0];
-            c[j] = e < 2 * a.half ? v.x : 1.f;
-            s[j] = e < 2 * a.half ? (second ? v.y : -v.y) : -0.f;
+    if (s0 < v0) {
+        const double pos = (double)a.positions[t];
+        for (int i = lane; i < half; i += 32) {
+            double s, c;
+            sincos(pos * (double)a.inv_freq[i], &s, &c);
+            turns[warp][i] = make_float2((float)(c * a.scale), (float)(s * a.scale));
         }
-        c2[i] = pack2f(c[0], c[1]), s2[i] = pack2f(s[0], s[1]);
+        __syncwarp();
     }
-    const bool shuffled = a.half % 16 == 0;
-    const int away = a.half / 16, from = e0 < a.half ? lane + away : e0 < 2 * a.half ? lane - away : lane;
-
-    /* 16 values of a head, normed with its weights (NULL: not) and rotated, as BF16 pairs */
-    auto turned = [&](const uint32_t (&x)[8], const float *weight, uint32_t (&o)[8]) {
-        uint64_t y[8], p[8];
+    uint64_t c2[4], s2[4]; /* of pairs 8 l .. 8 l + 7 */
+    if constexpr (P != kAny) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            y[i] = pack2f(low_half(x[i]), high_half(x[i]));
-        if (a.q_norm || a.k_norm) {
+        for (int i = 0; i < 4; ++i) {
+            const int f = 8 * l + 2 * i;
+            const float2 e = turns[warp][f < half ? f : 0], o = turns[warp][f + 1 < half ? f + 1 : 0];
+            c2[i] = pack2f(e.x, o.x), s2[i] = pack2f(e.y, o.y);
+        }
+    }
+
+    /* the lane's values of a head, normed with its weights (NULL: not) and turned, as BF16 pairs */
+    auto turned = [&](const uint32_t (&x)[8], const float *weight, uint32_t (&o)[8]) {
+        /* first and second values of pairs 2 i, 2 i + 1 */
+        uint64_t y1[4], y2[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (P == kBeside) {
+                y1[i] = pack2f(low_half(x[2 * i]), low_half(x[2 * i + 1]));
+                y2[i] = pack2f(high_half(x[2 * i]), high_half(x[2 * i + 1]));
+            } else {
+                y1[i] = pack2f(low_half(x[i]), high_half(x[i]));
+                y2[i] = pack2f(low_half(x[4 + i]), high_half(x[4 + i]));
+            }
+        }
+        if (weight) {
             double sum = 0.;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -147,92 +172,121 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
             for (int off = 1; off < L; off *= 2)
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
             const float r = (float)(1. / sqrt(sum * (1. / D) + a.eps));
-            if (weight) {
+            const uint64_t r2 = pack2f(r, r);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 w4 = reinterpret_cast<const float4 *>(weight + e0)[i];
-                    y[2 * i] = mul2(mul2(y[2 * i], pack2f(r, r)), pack2f(w4.x, w4.y));
-                    y[2 * i + 1] = mul2(mul2(y[2 * i + 1], pack2f(r, r)), pack2f(w4.z, w4.w));
+            for (int i = 0; i < 2; ++i) {
+                const float4 u = __ldg(reinterpret_cast<const float4 *>(weight + ea) + i);
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(weight + eb) + i);
+                if constexpr (P == kBeside) { /* u is pairs 2 i, 2 i + 1 of the first run, v of the second */
+                    y1[i] = mul2(mul2(y1[i], r2), pack2f(u.x, u.z)), y2[i] = mul2(mul2(y2[i], r2), pack2f(u.y, u.w));
+                    y1[2 + i] = mul2(mul2(y1[2 + i], r2), pack2f(v.x, v.z));
+                    y2[2 + i] = mul2(mul2(y2[2 + i], r2), pack2f(v.y, v.w));
+                } else {
+                    y1[2 * i] = mul2(mul2(y1[2 * i], r2), pack2f(u.x, u.y));
+                    y1[2 * i + 1] = mul2(mul2(y1[2 * i + 1], r2), pack2f(u.z, u.w));
+                    y2[2 * i] = mul2(mul2(y2[2 * i], r2), pack2f(v.x, v.y));
+                    y2[2 * i + 1] = mul2(mul2(y2[2 * i + 1], r2), pack2f(v.z, v.w));
                 }
             }
         }
-        if (a.interleaved) {
+        if constexpr (P == kAny) { /* 16 neighbours a lane, whose partners may be anywhere */
+            float *head = reinterpret_cast<float *>(mixed[warp] + in * kRow);
+            float y[16];
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float u, v;
-                unpack2f(y[i], u, v);
-                p[i] = pack2f(v, u);
+            for (int i = 0; i < 4; ++i)
+                unpack2f(y1[i], y[2 * i], y[2 * i + 1]), unpack2f(y2[i], y[8 + 2 * i], y[9 + 2 * i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                reinterpret_cast<float4 *>(head + ea)[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = ea + i;
+                if (e < 2 * half) {
+                    const float2 cs = turns[warp][e < half ? e : e - half];
+                    /* roundings one by one, as everywhere here: no fma */
+                    y[i] = e < half ? __fsub_rn(__fmul_rn(y[i], cs.x), __fmul_rn(head[e + half], cs.y))
+                                    : __fadd_rn(__fmul_rn(y[i], cs.x), __fmul_rn(head[e - half], cs.y));
+                }
             }
-        } else if (shuffled) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                p[i] = __shfl_sync(0xFFFFFFFFu, y[i], from);
-        } else {
-            float4 *mine = mixed[warp] + (lane * 16) / 4;
-            __syncwarp();
+                o[i] = round2(y[2 * i], y[2 * i + 1]);
+            return;
+        }
+        uint64_t o1[4], o2[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o1[i] = sub2(mul2(y1[i], c2[i]), mul2(y2[i], s2[i]));
+            o2[i] = add2(mul2(y2[i], c2[i]), mul2(y1[i], s2[i]));
+        }
+        if (half != D / 2) { /* places behind the rotated ones stay, whatever their values */
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float4 v;
-                unpack2f(y[2 * i], v.x, v.y), unpack2f(y[2 * i + 1], v.z, v.w);
-                mine[i] = v;
-            }
-            __syncwarp();
-            const float *head = reinterpret_cast<const float *>(mixed[warp]) + lane / L * D;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = e0 + 2 * i;
-                const int f = e < a.half ? e + a.half : e < 2 * a.half ? e - a.half : e;
-                const int f1 = e + 1 < a.half ? e + 1 + a.half : e + 1 < 2 * a.half ? e + 1 - a.half : e + 1;
-                p[i] = pack2f(head[f], head[f1]);
+                const bool first = P == kRuns ? partners : 8 * l + 2 * i < half;
+                const bool second = P == kRuns ? partners : 8 * l + 2 * i + 1 < half;
+                float f[2], y[2];
+                unpack2f(o1[i], f[0], f[1]), unpack2f(y1[i], y[0], y[1]);
+                o1[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
+                unpack2f(o2[i], f[0], f[1]), unpack2f(y2[i], y[0], y[1]);
+                o2[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float u, v, pu, pv;
-            unpack2f(p[i], pu, pv);
-            if (e0 + 2 * i >= 2 * a.half) /* nothing that is not finite comes by here */
-                pu = pv = 0.f;
-            /* three roundings, as they stand in the definition: no fma */
-            unpack2f(add2(mul2(y[i], c2[i]), mul2(pack2f(pu, pv), s2[i])), u, v);
-            const __nv_bfloat162 b = __floats2bfloat162_rn(u, v);
-            o[i] = *reinterpret_cast<const uint32_t *>(&b);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (P == kBeside) {
+                float a0, a1, b0, b1;
+                unpack2f(o1[i], a0, a1), unpack2f(o2[i], b0, b1);
+                o[2 * i] = round2(a0, b0), o[2 * i + 1] = round2(a1, b1);
+            } else {
+                o[i] = round2(o1[i]), o[4 + i] = round2(o2[i]);
+            }
         }
     };
 
-    const int slot = APPEND ? g.slots[t] : -1;
-    for (int r = r0; r < r1; r += N) {
+    const int slot = APPEND && s1 > k0 ? g.slots[t] : -1;
+    const bool cached = APPEND && slot >= 0 && slot < g.c.pages * g.c.page_size;
+    for (int s = s0; s < s1; ++s) {
         uint32_t next[8], o[8];
-        load(r + N, next); /* zeros past the last */
-        const int row = r + lane / L;
-        const bool key = row >= keys && row < values;
-        if (!APPEND || r < values) {
-            turned(x, row < keys ? a.q_norm : key ? a.k_norm : nullptr, o);
-            if (row < r1) {
-                if (row < keys)
-                    put16<VEC>(a.q_out + t * a.qo_tok + row * a.qo_head + e0, o);
-                else if (key && (!APPEND || a.k_out))
-                    put16<VEC>(a.k_out + t * a.ko_tok + (row - keys) * a.ko_head + e0, o);
+        load(s + 1, next);
+        const bool query = s < k0, value = APPEND && s >= v0;
+        const int row = (s - (query ? 0 : value ? v0 : k0)) * N + in;
+        const bool live = row < (query ? a.heads : a.kv_heads);
+        if (value) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] = x[i];
+        } else {
+            turned(x, query ? a.q_norm : a.k_norm, o);
+            __nv_bfloat16 *out = query ? a.q_out + t * a.qo_tok + row * a.qo_head : a.k_out + t * a.ko_tok + row * a.ko_head;
+            if (live && (query || !APPEND || a.k_out)) {
+                put8<VEC>(out + ea, o);
+                put8<VEC>(out + eb, o + 4);
             }
         }
-        if constexpr (APPEND) {
-            if (r + N > keys) { /* the whole warp */
-                if (row >= values) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        o[i] = x[i];
+        if (APPEND && !query) {
+            if constexpr (kMoves) {
+                if (!value) { /* 16 neighbours a lane */
+                    uint8_t *head = mixed[warp] + in * kRow;
+                    __syncwarp();
+                    *reinterpret_cast<uint4 *>(head + 2 * ea) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4 *>(head + 2 * eb) = make_uint4(o[4], o[5], o[6], o[7]);
+                    __syncwarp();
+                    const uint4 u = *reinterpret_cast<const uint4 *>(head + 32 * l), v = *reinterpret_cast<const uint4 *>(head + 32 * l + 16);
+                    o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w, o[4] = v.x, o[5] = v.y, o[6] = v.z, o[7] = v.w;
                 }
-                uint32_t meta;
-                const uint2 code = quantise16(o, meta);
-                if (row >= keys && row < r1 && slot >= 0 && slot < g.c.pages * g.c.page_size) {
-                    const int page = slot >> g.page_log2, at = slot & (g.c.page_size - 1);
-                    const int h = key ? row - keys : row - values;
-                    const int64_t place = (((int64_t)page * g.c.kv_heads + h) << g.page_log2) + at;
-                    uint8_t *codes = key ? g.c.k_code : g.c.v_code;
-                    uint16_t *metas = key ? g.c.k_meta : g.c.v_meta;
-                    *reinterpret_cast<uint2 *>(codes + place * (D / 2) + kv4_unit<D>(e0 / 64, at) + e0 % 64 / 2) = code;
-                    if (e0 % 64 == 0)
-                        reinterpret_cast<uint32_t *>(metas)[place * (D / 64) + e0 / 64] = meta;
-                }
+            }
+            uint32_t meta;
+            const uint2 code = quantise16(o, meta);
+            if (live && cached) {
+                const int page = slot >> g.page_log2, at = slot & (g.c.page_size - 1), e0 = 16 * l;
+                const int64_t place = (((int64_t)page * g.c.kv_heads + row) << g.page_log2) + at;
+                uint8_t *codes = value ? g.c.v_code : g.c.k_code;
+                uint16_t *metas = value ? g.c.v_meta : g.c.k_meta;
+                *reinterpret_cast<uint2 *>(codes + place * (D / 2) + kv4_unit<D>(e0 / 64, at) + e0 % 64 / 2) = code;
+                if (e0 % 64 == 0)
+                    reinterpret_cast<uint32_t *>(metas)[place * (D / 64) + e0 / 64] = meta;
             }
         }
 #pragma unroll
@@ -241,27 +295,36 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
     }
 }
 
+template <int D, Pairing P>
+auto kernel_of(bool append, bool vec)
+{
+    return append ? (vec ? rope_kernel<D, P, true, true> : rope_kernel<D, P, false, true>)
+                  : (vec ? rope_kernel<D, P, true, false> : rope_kernel<D, P, false, false>);
+}
+template <int D>
+auto kernel_of(const GlintRope &a, bool append, bool vec)
+{
+    return a.interleaved       ? kernel_of<D, kBeside>(append, vec)
+           : a.half % 8 == 0 ? kernel_of<D, kRuns>(append, vec)
+                               : kernel_of<D, kAny>(append, vec);
+}
+
 int launch(Args &g, bool append, bool vec, cudaStream_t st)
 {
     const GlintRope &a = g.a;
     const int n = 32 / (a.head_dim / 16); /* heads a step */
-    g.rows = a.heads + a.kv_heads + (append ? a.kv_heads : 0);
-    /* as many parts of a token as give every SM two warps of each scheduler, while there is a step for each */
-    const int steps = (g.rows + n - 1) / n;
-    const int64_t want = (8LL * sm_count() + a.tokens - 1) / a.tokens;
-    g.chunk = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps)) * n;
-    g.chunks = (g.rows + g.chunk - 1) / g.chunk;
+    g.q_steps = (a.heads + n - 1) / n, g.k_steps = (a.kv_heads + n - 1) / n;
+    g.steps = g.q_steps + (append ? 2 : 1) * g.k_steps;
+    /* as many parts of a token as give every SM eight warps, while there is a step for each */
+    const int64_t want = std::min<int64_t>((8LL * sm_count() + a.tokens - 1) / a.tokens, g.steps);
+    g.chunk = (int)((g.steps + want - 1) / want);
+    g.chunks = (g.steps + g.chunk - 1) / g.chunk;
     g.warps = (int64_t)a.tokens * g.chunks;
     const int64_t grid = (g.warps + kWarps - 1) / kWarps;
     if (grid > INT32_MAX)
         return kBadArg;
-    const auto kernel = [&](auto d) {
-        constexpr int D = decltype(d)::value;
-        return append ? (vec ? rope_kernel<D, true, true> : rope_kernel<D, false, true>)
-                      : (vec ? rope_kernel<D, true, false> : rope_kernel<D, false, false>);
-    };
-    const auto k = a.head_dim == 128 ? kernel(std::integral_constant<int, 128>()) : kernel(std::integral_constant<int, 64>());
-    k<<<(unsigned)grid, kWarps * 32, 0, st>>>(g);
+    const auto kernel = a.head_dim == 128 ? kernel_of<128>(a, append, vec) : kernel_of<64>(a, append, vec);
+    kernel<<<(unsigned)grid, kWarps * 32, 0, st>>>(g);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
