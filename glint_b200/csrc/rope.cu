@@ -29,7 +29,7 @@
 namespace glint {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 /* where a value's partner is: R / 2 places on, in whole runs of 8 or not; beside it */
 enum Pairing : int { kRuns, kAny, kBeside };
 
@@ -90,7 +90,7 @@ __device__ __forceinline__ uint32_t round2(uint64_t v)
 }
 
 template <int D, Pairing P, bool VEC, bool APPEND>
-__global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
+__global__ void __launch_bounds__(kWarps * 32, APPEND ? 5 : 6) rope_kernel(const Args g)
 {
     constexpr int L = D / 16, N = 32 / L; /* lanes a head, heads a step */
     constexpr bool kMoves = APPEND && P == kRuns; /* values go to the lanes that quantise them */
@@ -110,20 +110,35 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
     const int ea = P != kRuns ? 16 * l : partners ? 8 * l : 2 * half + 16 * (l - half / 8);
     const int eb = partners ? ea + half : ea + 8;
 
-    const __nv_bfloat16 *const q = a.q + t * a.q_tok, *const k = a.k + t * a.k_tok, *const v = APPEND ? g.v + t * g.v_tok : nullptr;
     const int k0 = g.q_steps, v0 = g.q_steps + g.k_steps; /* first steps of k and v */
-    auto load = [&](int s, uint32_t (&x)[8]) {
-        const bool query = s < k0, value = APPEND && s >= v0;
-        const int row = (s - (query ? 0 : value ? v0 : k0)) * N + in;
-        const __nv_bfloat16 *p = (query ? q : value ? v : k) + row * (query ? a.q_head : value ? g.v_head : a.k_head);
-        if (s < s1 && row < (query ? a.heads : a.kv_heads)) {
-            get8<VEC>(p + (value ? 16 * l : ea), x);
-            get8<VEC>(p + (value ? 16 * l + 8 : eb), x + 4);
+    /* a step's heads: this lane's one of them, which lies `by` behind that of the step before of the same kind */
+    struct Heads {
+        const __nv_bfloat16 *p;
+        int64_t by;
+        int left; /* heads of its kind from this lane's on; none: <= 0 */
+    };
+    auto heads_at = [&](int s) {
+        const int row = (s - (s < k0 ? 0 : !APPEND || s < v0 ? k0 : v0)) * N + in;
+        if (s < k0)
+            return Heads{a.q + t * a.q_tok + row * a.q_head, N * a.q_head, a.heads - row};
+        if (!APPEND || s < v0)
+            return Heads{a.k + t * a.k_tok + row * a.k_head, N * a.k_head, a.kv_heads - row};
+        return Heads{g.v + t * g.v_tok + row * g.v_head, N * g.v_head, a.kv_heads - row};
+    };
+    Heads from = heads_at(s0);
+    auto load = [&](int s, uint32_t (&x)[8]) { /* of `from`, the heads of step s, which moves on */
+        if (from.left > 0 && s < s1) {
+            const bool value = APPEND && s >= v0;
+            get8<VEC>(from.p + (value ? 16 * l : ea), x);
+            get8<VEC>(from.p + (value ? 16 * l + 8 : eb), x + 4);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 x[i] = 0u;
         }
+        from.p += from.by, from.left -= N;
+        if (s + 1 == k0 || (APPEND && s + 1 == v0))
+            from = heads_at(s + 1);
     };
     uint32_t x[8];
     load(s0, x);
@@ -171,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
 #pragma unroll
             for (int off = 1; off < L; off *= 2)
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
-            const float r = (float)(1. / sqrt(sum * (1. / D) + a.eps));
+            const float r = (float)rsqrt(sum * (1. / D) + a.eps);
             const uint64_t r2 = pack2f(r, r);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -247,11 +262,18 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
 
     const int slot = APPEND && s1 > k0 ? g.slots[t] : -1;
     const bool cached = APPEND && slot >= 0 && slot < g.c.pages * g.c.page_size;
+    __nv_bfloat16 *out = nullptr; /* where this step's heads go */
+    int64_t by = 0;
+    int row = 0; /* this lane's head of its kind */
     for (int s = s0; s < s1; ++s) {
         uint32_t next[8], o[8];
         load(s + 1, next);
         const bool query = s < k0, value = APPEND && s >= v0;
-        const int row = (s - (query ? 0 : value ? v0 : k0)) * N + in;
+        if (s == s0 || s == k0 || (APPEND && s == v0)) {
+            row = (s - (query ? 0 : value ? v0 : k0)) * N + in;
+            by = N * (query ? a.qo_head : a.ko_head);
+            out = query ? a.q_out + t * a.qo_tok + row * a.qo_head : a.k_out + t * a.ko_tok + row * a.ko_head;
+        }
         const bool live = row < (query ? a.heads : a.kv_heads);
         if (value) {
 #pragma unroll
@@ -259,11 +281,11 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
                 o[i] = x[i];
         } else {
             turned(x, query ? a.q_norm : a.k_norm, o);
-            __nv_bfloat16 *out = query ? a.q_out + t * a.qo_tok + row * a.qo_head : a.k_out + t * a.ko_tok + row * a.ko_head;
             if (live && (query || !APPEND || a.k_out)) {
                 put8<VEC>(out + ea, o);
                 put8<VEC>(out + eb, o + 4);
             }
+            out += by;
         }
         if (APPEND && !query) {
             if constexpr (kMoves) {
@@ -292,6 +314,7 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const Args g)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             x[i] = next[i];
+        row += N;
     }
 }
 
