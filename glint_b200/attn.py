@@ -267,12 +267,11 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
     return freq.float().to(device), scale
 
 
-def _heads_apart(t: torch.Tensor, name: str) -> None:
-    """No two heads of an output lie on one another."""
+def _heads_apart(t: torch.Tensor) -> bool:
+    """No two heads of [tokens, heads, head_dim] lie on one another."""
     (T, H, D), (st, sh, _) = t.shape, t.stride()
-    if T and H and not ((sh >= D or H == 1) and (st >= (H - 1) * sh + D or T == 1) or
-                        (st >= D or T == 1) and (sh >= (T - 1) * st + D or H == 1)):
-        raise ValueError(f"the heads of {name} overlap one another")
+    return not T or not H or (sh >= D or H == 1) and (st >= (H - 1) * sh + D or T == 1) or \
+        (st >= D or T == 1) and (sh >= (T - 1) * st + D or H == 1)
 
 
 def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -292,9 +291,24 @@ def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return ea <= off and off + eb <= sa
 
 
-def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, others, keys):
-    """The checks that rope and rope_append share; (struct, stream, q_out, k_out).  others: further
-    inputs (name, tensor) of q's type; keys: k_out is wanted whether it was given or not."""
+def _outputs_apart(q, k, q_out, k_out, more) -> None:
+    """Outputs that the caller gave lie in their own input's place or touch no input, nor one another."""
+    for o, name, own in ((q_out, "q_out", q), (k_out, "k_out", k)):
+        if o is None:
+            continue
+        if not _heads_apart(o):
+            raise ValueError(f"the heads of {name} overlap one another")
+        for x in (q, k, *more):
+            if x is not None and not (x is own and x.data_ptr() == o.data_ptr() and x.stride() == o.stride()) and \
+                    not _rows_apart(o, x):
+                raise ValueError(f"{name} must be {name[0]} itself or apart from q, k and v, which it may overlap")
+    if k_out is not None and q_out is not None and not _rows_apart(q_out, k_out):
+        raise ValueError("q_out and k_out must be apart")
+
+
+def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, more, keys):
+    """The checks that rope and rope_append share; (struct, stream, q_out, k_out).  more: further
+    inputs of q's type; keys: k_out is wanted whether it was given or not."""
     _want(q, "q", torch.bfloat16, (None, None, None), dense=False)
     T, H, D = q.shape
     _head_dim(D)
@@ -317,27 +331,16 @@ def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_
             _want16(w, name)
     if not (eps > 0 and math.isfinite(eps) and math.isfinite(scale)):
         raise ValueError(f"eps must be above 0 and scale finite, not {eps} and {scale}")
-    given = q_out is not None or k_out is not None
+    if q_out is not None or k_out is not None:
+        for o, shape, name in ((q_out, (T, H, D), "q_out"), (k_out, (T, Hk, D), "k_out")):
+            if o is not None:
+                _want(o, name, torch.bfloat16, shape, dense=False)
+        _outputs_apart(q, k, q_out, k_out, more)
     if q_out is None:
         q_out = _empty(q, (T, H, D), torch.bfloat16, stream)
-    else:
-        _want(q_out, "q_out", torch.bfloat16, (T, H, D), dense=False)
-    if k_out is None:
-        if keys and k is not None:
-            k_out = _empty(q, (T, Hk, D), torch.bfloat16, stream)
-    else:
-        _want(k_out, "k_out", torch.bfloat16, (T, Hk, D), dense=False)
+    if k_out is None and keys and k is not None:
+        k_out = _empty(q, (T, Hk, D), torch.bfloat16, stream)
     raw = _raw(q, stream, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
-    if given:
-        outs = [(n, o) for n, o in (("q_out", q_out), ("k_out", k_out)) if o is not None]
-        for n, o in outs:
-            _heads_apart(o, n)
-            for m, x in [("q", q), ("k", k)] + others:
-                itself = m == n[0] and x is not None and x.data_ptr() == o.data_ptr() and x.stride() == o.stride()
-                if x is not None and not itself and not _rows_apart(o, x):
-                    raise ValueError(f"{n} must be {n[0]} itself or apart from q, k and v: it may overlap {m}")
-        if len(outs) == 2 and not _rows_apart(q_out, k_out):
-            raise ValueError("q_out and k_out must be apart")
     qs, os = q.stride(), q_out.stride()
     ks = (0, 0) if k is None else k.stride()
     kos = (0, 0) if k_out is None else k_out.stride()
@@ -361,7 +364,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, in
     multiplied by these first.  q_out and k_out may be q and k themselves (any other overlap is
     refused); left out, they are new and contiguous."""
     a, raw, q_out, k_out = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
-                                 [], True)
+                                 (), True)
     _check(_c().rope(a, raw), "glint_rope_stream")
     return q_out, k_out
 
@@ -438,6 +441,7 @@ class KV4Cache:
             raise ValueError("the cache's tensors must be on one device")
         self.k_code, self.k_meta, self.v_code, self.v_meta = k_code, k_meta, v_code, v_meta
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, 2 * half
+        self.device = k_code.get_device()
         self._c = _pack_cache(k_code.data_ptr(), k_meta.data_ptr(), v_code.data_ptr(), v_meta.data_ptr(), pages,
                               kv_heads, page_size, 2 * half)
 
@@ -476,8 +480,9 @@ def rope_append(cache: KV4Cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     _want(v, "v", torch.bfloat16, k.shape, dense=False)
     _want(slots, "slots", torch.int32, k.shape[:1])
     a, raw, q_out, _ = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
-                             [("v", v)], False)
-    _raw(q, stream, v, slots, cache.k_code)
+                             (v,), False)
+    if slots.get_device() != cache.device or v.get_device() != cache.device or q.get_device() != cache.device:
+        raise ValueError("q, k, v, slots and the cache must be on one device")
     vs = v.stride()
     _check(_c().rope_append(cache._c, a, v.data_ptr(), vs[0], vs[1], slots.data_ptr(), raw), "glint_kv4_rope_append_stream")
     return q_out

@@ -7,6 +7,8 @@ fallback: a missing library or a non-CUDA tensor raises.
 from __future__ import annotations
 
 import ctypes
+import struct
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -166,15 +168,34 @@ class GlintHtileGated(ctypes.Structure):
                [(n, ctypes.c_int) for n in ("M", "F", "K", "blocksize", "mode", "act")]
 
 
-def _gated_lib():
-    L = lib()
-    if not getattr(L, "_gated_bound", False):
-        L.glint_htile_gated_work_bytes.argtypes = [ctypes.POINTER(GlintHtileGated)]
-        L.glint_htile_gated_work_bytes.restype = ctypes.c_int64
-        L.glint_htile_gated_stream.argtypes = [ctypes.POINTER(GlintHtileGated), ctypes.c_void_p]
-        L.glint_htile_gated_stream.restype = ctypes.c_int
-        L._gated_bound = True
-    return L
+_pack_gated_args = struct.Struct("6P6i").pack
+
+
+class _GatedCalls:
+    """The entry points taking the struct as packed bytes, as attn.py has them."""
+
+    def __init__(self):
+        L = lib()
+        self.run = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)(("glint_htile_gated_stream", L))
+        self.work = ctypes.CFUNCTYPE(ctypes.c_int64, ctypes.c_char_p)(("glint_htile_gated_work_bytes", L))
+
+
+_gated: Optional[_GatedCalls] = None
+
+
+def _gated_calls() -> _GatedCalls:
+    global _gated
+    if _gated is None:
+        _gated = _GatedCalls()
+    return _gated
+
+
+# sizes grow with the current device's SMs: `dev` is part of what they are kept by; `place`: the operands'
+# addresses modulo 16
+@lru_cache(maxsize=256)
+def _gated_work(dev: int, place: int, M: int, F: int, K: int, blocksize: int, mode: int) -> int:
+    at = 16 + place
+    return _gated_calls().work(_pack_gated_args(at, at, at, at, at, 0, M, F, K, blocksize, mode, 0))
 
 
 def pack_gated(gate: Sequence[torch.Tensor], up: Sequence[torch.Tensor], F: int, K: int, blocksize: int = 64):
@@ -214,6 +235,7 @@ def htile_gated(x: torch.Tensor, hole: torch.Tensor, plug: torch.Tensor, absmax:
             hole.numel() < n_packed(n) or plug.numel() < n_packed(n) or absmax.numel() < n_absmax(n, blocksize):
         raise ValueError(f"hole and plug must be uint8 planes and absmax the float32 scales of a [{2 * F}, {K}] weight")
     dev = x.get_device()
+    hp, pp, ap, xp = hole.data_ptr(), plug.data_ptr(), absmax.data_ptr(), x.data_ptr()
     if out is not None:
         _cuda(out, "out")
         if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, F):
@@ -221,23 +243,24 @@ def htile_gated(x: torch.Tensor, hole: torch.Tensor, plug: torch.Tensor, absmax:
         for t in (x, hole, plug, absmax):
             if out.data_ptr() < t.data_ptr() + t.numel() * t.element_size() and t.data_ptr() < out.data_ptr() + 2 * M * F:
                 raise ValueError("out overlaps an input")
-    if dev != torch.cuda.current_device() or any(t.get_device() != dev for t in (hole, plug, absmax, out) if t is not None):
+    if hole.get_device() != dev or plug.get_device() != dev or absmax.get_device() != dev or \
+            (out is not None and out.get_device() != dev) or dev != torch.cuda.current_device():
         raise ValueError("all tensors must be on the current device")
-    L, s = _gated_lib(), stream if stream is not None else torch.cuda.current_stream()
 
     def memory(shape, dtype):  # of the stream that writes it
         if stream is None:
-            return torch.empty(shape, dtype=dtype, device=x.device)
+            return x.new_empty(shape, dtype=dtype)
         with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=x.device)
-    out = out if out is not None else memory((M, F), torch.bfloat16)
-    a = GlintHtileGated(hole.data_ptr(), plug.data_ptr(), absmax.data_ptr(), x.data_ptr(), out.data_ptr(), None, M, F, K,
-                        blocksize, _MODES[mode], _ACTS[act])
-    need = L.glint_htile_gated_work_bytes(ctypes.byref(a))
+            return x.new_empty(shape, dtype=dtype)
+    if out is None:
+        out = memory((M, F), torch.bfloat16)
+    mode = _MODES[mode]
+    need = _gated_work(dev, (hp | pp | ap | xp) & 15, M, F, K, blocksize, mode)
     work = memory((need,), torch.uint8) if need > 0 else None
-    if work is not None:
-        a.work = work.data_ptr()
-    _check(L.glint_htile_gated_stream(ctypes.byref(a), s.cuda_stream), "glint_htile_gated_stream")
+    rc = _gated_calls().run(_pack_gated_args(hp, pp, ap, xp, out.data_ptr(), work.data_ptr() if need > 0 else 0, M, F, K,
+                                             blocksize, mode, _ACTS[act]),
+                            torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
+    _check(rc, "glint_htile_gated_stream")
     return out
 
 

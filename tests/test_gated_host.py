@@ -11,7 +11,11 @@ torch = pytest.importorskip("torch")
 def lib():
     from glint_b200 import build, device
     build.build()
-    return device._gated_lib()
+    L = device.lib()
+    L.glint_htile_gated_work_bytes.argtypes = [ctypes.POINTER(device.GlintHtileGated)]
+    L.glint_htile_gated_work_bytes.restype = ctypes.c_int64
+    L.glint_htile_gated_stream.argtypes = [ctypes.POINTER(device.GlintHtileGated), ctypes.c_void_p]
+    return L
 
 
 def call(**kw):
