@@ -701,9 +701,11 @@ int64_t glint_htile_gated_work_bytes(const GlintHtileGated *a)
 {
     if (gated_check(a) != kOk)
         return kBadArg;
-    if (a->M <= kGatedStreamM || a->F == 0 || a->K == 0 || a->mode == GLINT_HTILE_PRECISE || !gated_streams(a))
+    if (a->M == 0 || a->F == 0 || a->K == 0 || !gated_streams(a))
         return 0;
-    return htile_gemm_gated_work(a->M, 2 * a->F, a->K);
+    if (a->M <= kGatedStreamM)
+        return htile_decode_gated_work(a->M, 2 * a->F, a->K);
+    return a->mode == GLINT_HTILE_PRECISE ? 0 : htile_gemm_gated_work(a->M, 2 * a->F, a->K);
 }
 int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
 {
@@ -723,7 +725,7 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
     if (!gated_streams(a))
         return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, mode, a->act, stream);
     if (a->M <= kGatedStreamM)
-        return htile_decode_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, mode, a->act, stream);
+        return htile_decode_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->work, a->M, N, a->K, mode, a->act, stream);
     return htile_gemm_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->work, a->M, N, a->K, mode, a->act, stream);
 }
 

@@ -109,9 +109,10 @@ int htile_decode_gather_launch(const uint8_t *hole, const uint8_t *plug, const f
 
 /* h[M, N / 2] BF16 = act(y[:, 2i]) * y[:, 2i + 1], y as of htile_launch (N even; gated.cuh):
  * M <= 32 and any M of the TMA kernels' shapes (bs == 64, K % 256 == 0, 16-byte alignment), and
- * all others.  work: htile_gemm_gated_work() bytes, fast mode only. */
+ * all others.  work: htile_decode_gated_work() and, in fast mode, htile_gemm_gated_work() bytes. */
+int64_t htile_decode_gated_work(int M, int N, int K);
 int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
-                              void *h, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
+                              void *h, void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
 int64_t htile_gemm_gated_work(int M, int N, int K);
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
                             void *h, void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);

@@ -98,9 +98,10 @@ __device__ __forceinline__ uint32_t split_pair(float c)
  * store covers a quarter of one entry's 128-byte row of 32 replicas, so a warp's
  * store fills four whole rows (four wavefronts, no bank conflicts; one thread per
  * entry writing its own row would put all 32 lanes on the same four banks). */
+template <int WARPS>
 __device__ __forceinline__ void build_pair_lut(uint32_t *lut)
 {
-    for (int i = (int)threadIdx.x; i < 256 * 8; i += kConsumers * 32) {
+    for (int i = (int)threadIdx.x; i < 256 * 8; i += WARPS * 32) {
         const int e = i >> 3;
         const uint32_t v = split_pair(g_cells[e >> 4][e & 15]);
         reinterpret_cast<uint4 *>(lut + e * 64)[i & 7] = make_uint4(v, v, v, v);
@@ -117,6 +118,7 @@ struct DecodeArgs {
     int64_t units;      /* row blocks * KU */
     int max_parts;
     GatherArgs ga;
+    int act; /* kOutGated: of the gate rows */
 };
 
 /* first unit of CTA c under the even split of `units` over `ctas` */
@@ -315,7 +317,26 @@ __device__ __forceinline__ void tile_block_at(uint32_t st, uint32_t pt, const Bl
     tile_math<MT, SPLIT>(E, O, sc, xb, lut_base, lane4, acc);
 }
 
-template <int MT, bool SPLIT, bool BF16OUT>
+/* A 16-row tile's sums as gated outputs: rows 2i and 2i + 1 (gate and up; `n` of the tile's first row is even)
+ * are with two lanes, that differ in the bit of g which is a row's parity.  Of two activation rows each
+ * keeps one: the gate's lane takes up of the first for gate of the second.  put(n, col, value): row pair
+ * n / 2 and activation row. */
+template <int MT, int ROWB, class Put>
+__device__ __forceinline__ void gated_outputs(const float (&acc)[MT][4], int pg, int t, int act, Put put)
+{
+    const bool up = pg & 1;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float keep = up ? acc[mt][2 * h + 1] : acc[mt][2 * h], give = up ? acc[mt][2 * h] : acc[mt][2 * h + 1];
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, give, ROWB == 128 ? 16 : 4);
+            put(pg + 8 * h, mt * 8 + 2 * t + (up ? 1 : 0), up ? gated_value(got, keep, act) : gated_value(keep, got, act));
+        }
+    }
+}
+
+template <int MT, bool SPLIT, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     htile_decode_kernel(const __grid_constant__ CUtensorMap hmap, const __grid_constant__ CUtensorMap pmap,
                         const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap xmap,
@@ -408,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     /* codebook as BF16 hi/lo pairs, one replica per lane (first 128 B of each 256-B
      * entry row); the consumer warps then meet on named barrier 1 (the producer is
      * not in it) */
-    build_pair_lut(lut);
+    build_pair_lut<kConsumers>(lut);
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
     /* y, the workspace and its flags are touched only after the previous kernel
      * in the stream is complete (no-op without programmatic dependent launch) */
@@ -439,85 +460,129 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto put_y = [&](int n, int col, float v) {
             if (n < a.N && col < a.M) {
                 if (a.ga.world > 0)
-                    gather_store<BF16OUT>(a.ga, col, n, v);
-                else if (BF16OUT)
+                    gather_store<OUT == kOutBF16>(a.ga, col, n, v);
+                else if (OUT == kOutBF16)
                     static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * a.N + n] = __float2bfloat16_rn(v);
                 else
                     static_cast<float *>(a.y)[(int64_t)col * a.N + n] = v;
             }
         };
+        auto put_gated = [&] {
+            gated_outputs<MT, kKU / 2>(acc, pg, t, a.act, [&](int row, int col, float v) {
+                const int n = rb * kRows + r0 + row;
+                if (n < a.N && col < a.M)
+                    static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] = __float2bfloat16_rn(v);
+            });
+        };
         if (k0 == 0 && k1 == a.KU) {
+            if constexpr (OUT == kOutGated) {
+                put_gated();
+            } else {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    put_y(rb * kRows + r0 + pg + (q >> 1) * 8, mt * 8 + 2 * t + (q & 1), acc[mt][q]);
+                    for (int q = 0; q < 4; ++q)
+                        put_y(rb * kRows + r0 + pg + (q >> 1) * 8, mt * 8 + 2 * t + (q & 1), acc[mt][q]);
+            }
             return;
         }
         const int64_t first = cta_of((int64_t)rb * a.KU, a.units, ctas);
         const int part = (int)(blockIdx.x - first);
         const int parts = (int)(cta_of((int64_t)rb * a.KU + a.KU - 1, a.units, ctas) - first + 1);
         const float *wsp = a.ws + ((int64_t)rb * a.max_parts) * kRows * MP;
-        int *flg = a.flags + ((int64_t)rb * a.max_parts) * kConsumers + warp;
-        if (part != 0) {
+        if constexpr (OUT == kOutGated) {
+            /* No part waits for another: all are stored, and the last to be counted in adds them, in part
+             * order.  The counts are zero at the start, by the launch. */
+            float *mine = const_cast<float *>(wsp) + ((int64_t)part * kRows + r0 + pg) * MP + 2 * t;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    __stcg(const_cast<float *>(wsp) + ((int64_t)part * kRows + r0 + pg + (q >> 1) * 8) * MP + mt * 8 +
-                               2 * t + (q & 1),
-                           acc[mt][q]);
+                    __stcg(mine + (q >> 1) * 8 * MP + mt * 8 + (q & 1), acc[mt][q]);
+            __threadfence();
             __syncwarp();
+            int done = 0;
             if (lane == 0)
-                asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(flg + part * kConsumers) : "memory");
-            return;
-        }
-        /* lane l waits for the flag of part l (and l + 32, ...): the waits overlap */
-        bool ok = true;
-        for (int pp = (int)lane; pp < parts && ok; pp += 32) {
-            if (pp == 0)
-                continue;
-            int *f = flg + pp * kConsumers;
-            const long long t0 = clock64();
-            uint32_t v = 0;
-            while (true) {
-                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
-                if (v)
-                    break;
-                if (clock64() - t0 > kWaitCycles) {
-                    atomicOr(&g_decode_error, kErrTimeout);
-                    ok = false;
-                    break;
-                }
-                __nanosleep(64);
+                done = atomicAdd(a.flags + (int64_t)rb * kConsumers + warp, 1);
+            if (__shfl_sync(0xFFFFFFFFu, done, 0) != parts - 1)
+                return;
+            __threadfence();
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    acc[mt][q] = 0.f;
+            for (int pp = 0; pp < parts; ++pp) {
+                const float *src = wsp + ((int64_t)pp * kRows + r0 + pg) * MP + 2 * t;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        acc[mt][q] += __ldcg(src + (q >> 1) * 8 * MP + mt * 8 + (q & 1));
             }
-            *f = 0; /* consumed: zero for the next call */
-        }
-        if (!__all_sync(0xFFFFFFFFu, ok))
-            return;
-        /* the parts' sums in part (k) order; loads issued eight at a time so their
-         * L2 latencies overlap */
+            put_gated();
+        } else {
+            int *flg = a.flags + ((int64_t)rb * a.max_parts) * kConsumers + warp;
+            if (part != 0) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = r0 + pg + (q >> 1) * 8, col = mt * 8 + 2 * t + (q & 1);
-                const float *src = wsp + (int64_t)row * MP + col;
-                const int64_t step = (int64_t)kRows * MP;
-                float v = acc[mt][q];
-                int pp = 1;
-                for (; pp + 8 <= parts; pp += 8) {
-                    float w8[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        w8[j] = __ldcg(src + (pp + j) * step);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        v += w8[j];
+                    for (int q = 0; q < 4; ++q)
+                        __stcg(const_cast<float *>(wsp) + ((int64_t)part * kRows + r0 + pg + (q >> 1) * 8) * MP + mt * 8 +
+                                   2 * t + (q & 1),
+                               acc[mt][q]);
+                __syncwarp();
+                if (lane == 0)
+                    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(flg + part * kConsumers) : "memory");
+                return;
+            }
+            /* lane l waits for the flag of part l (and l + 32, ...): the waits overlap */
+            bool ok = true;
+            for (int pp = (int)lane; pp < parts && ok; pp += 32) {
+                if (pp == 0)
+                    continue;
+                int *f = flg + pp * kConsumers;
+                const long long t0 = clock64();
+                uint32_t v = 0;
+                while (true) {
+                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
+                    if (v)
+                        break;
+                    if (clock64() - t0 > kWaitCycles) {
+                        atomicOr(&g_decode_error, kErrTimeout);
+                        ok = false;
+                        break;
+                    }
+                    __nanosleep(64);
                 }
-                for (; pp < parts; ++pp)
-                    v += __ldcg(src + pp * step);
-                put_y(rb * kRows + row, col, v);
+                *f = 0; /* consumed: zero for the next call */
+            }
+            if (!__all_sync(0xFFFFFFFFu, ok))
+                return;
+            /* the parts' sums in part (k) order; loads issued eight at a time so their
+             * L2 latencies overlap */
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = r0 + pg + (q >> 1) * 8, col = mt * 8 + 2 * t + (q & 1);
+                    const float *src = wsp + (int64_t)row * MP + col;
+                    const int64_t step = (int64_t)kRows * MP;
+                    float v = acc[mt][q];
+                    int pp = 1;
+                    for (; pp + 8 <= parts; pp += 8) {
+                        float w8[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            w8[j] = __ldcg(src + (pp + j) * step);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            v += w8[j];
+                    }
+                    for (; pp < parts; ++pp)
+                        v += __ldcg(src + pp * step);
+                    put_y(rb * kRows + row, col, v);
+                }
             }
         }
     };
@@ -593,11 +658,36 @@ constexpr int kTailWarps = 4;
 constexpr int kTailX = 5 * 1024; /* offset of the activation boxes */
 template <int MT>
 constexpr int r_tail_bytes() { return MT <= 2 ? kTailX + r_xsub<MT>() + 3 * 32 * 4 * MT * 4 : 0; }
-template <int MT>
+/* Consumer warps and what goes with them.  16, of up to 112 registers each, so that x of 32 rows fits beside the
+ * codes; of a gated projection 28 of 64 for up to 8 rows and 20 of 96 for up to 16: more warps to hide the
+ * lookups' latency behind, and longer row blocks, so that 194 rows a CTA (2 x 14336 on 148 SMs) are 13
+ * tiles in one block in place of 14 in two, 132 or 149 rows 9 or 10 in one in place of 10 in two.  One
+ * row: 2 x 14336 x 4096 34.2 -> 32.9 us, 2 x 9728 x 2560 18.9 -> 15.7, 2 x 11008 x 4096 27.8 -> 24.1; sixteen: 41.5
+ * -> 41.2, 22.2 -> 18.0, 33.0 -> 27.7. */
+constexpr int kMany = 28, kSome = 20;
+template <int MT, int C>
+struct RowCfg {
+    static constexpr int kThreads = (C + 1) * 32;
+    static constexpr int kBlockMax = kRowBlockMax, kRing = r_ring<MT>(), kScratchWarps = MT <= 2 ? 14 : 7;
+    static constexpr int kTail = r_tail_bytes<MT>();
+};
+template <>
+struct RowCfg<1, kMany> {
+    static constexpr int kThreads = (kMany + 1) * 32;
+    static constexpr int kBlockMax = 208, kRing = 2 * (2 * kBlockMax * 128 + 4096 + r_xsub<1>()), kScratchWarps = 21;
+    static constexpr int kTail = 0;
+};
+template <>
+struct RowCfg<2, kSome> {
+    static constexpr int kThreads = (kSome + 1) * 32;
+    static constexpr int kBlockMax = 160, kRing = r_ring<2>(), kScratchWarps = 15;
+    static constexpr int kTail = 0;
+};
+template <int MT, int C>
 constexpr int r_smem_bytes()
 {
-    return kLutBytes + 1024 + r_ring<MT>() + r_tail_bytes<MT>() + r_scratch_floats<MT>() * 4 +
-           8 * (2 * kRMaxStages + 3) + 64;
+    using F = RowCfg<MT, C>;
+    return kLutBytes + 1024 + F::kRing + F::kTail + F::kScratchWarps * 32 * 4 * MT * 4 + 8 * (2 * kRMaxStages + 3) + 64;
 }
 
 struct RowArgs {
@@ -632,21 +722,22 @@ struct RowArgs {
     int act; /* kOutGated: of the gate rows */
 };
 
-template <int MT, bool SPLIT, int OUT, int NB>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int MT, bool SPLIT, int OUT, int NB, int C>
+__global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
     htile_rows_kernel(const __grid_constant__ CUtensorMap hmap, const __grid_constant__ CUtensorMap pmap,
                       const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap xmap,
                       const __grid_constant__ CUtensorMap hmap16, const __grid_constant__ CUtensorMap pmap16,
                       const __grid_constant__ CUtensorMap amap16, const RowArgs a)
 {
-    static_assert(r_smem_bytes<MT>() <= 232448, "shared memory");
+    using F = RowCfg<MT, C>;
+    static_assert(r_smem_bytes<MT, C>() <= 232448, "shared memory");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint32_t *lut = reinterpret_cast<uint32_t *>(smem_raw);
     uint8_t *ring = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw + kLutBytes) + 1023) & ~uintptr_t(1023));
-    uint8_t *tail = ring + r_ring<MT>(); /* 1 KB aligned: the ring is a multiple of 1 KB */
-    float *scratch = reinterpret_cast<float *>(tail + r_tail_bytes<MT>());
-    uint64_t *full = reinterpret_cast<uint64_t *>(scratch + r_scratch_floats<MT>());
+    uint8_t *tail = ring + F::kRing; /* 1 KB aligned: the ring is a multiple of 1 KB */
+    float *scratch = reinterpret_cast<float *>(tail + F::kTail);
+    uint64_t *full = reinterpret_cast<uint64_t *>(scratch + F::kScratchWarps * 32 * 4 * MT);
     uint64_t *empty = full + kRMaxStages;
     uint64_t *cmb_full = empty + kRMaxStages; /* a row block's KH-1 partials per tile are in scratch */
     uint64_t *cmb_empty = cmb_full + 1;       /* the tile owners have read them */
@@ -669,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *cta_done = 0u;
         mbar_init_fence();
     }
-    if (threadIdx.x == kConsumers * 32) {
+    if (threadIdx.x == C * 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&hmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&pmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&amap) : "memory");
@@ -682,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_begin = blockIdx.x * a.R, n_end = min(a.N, n_begin + a.R);
     const int units = a.nb * a.KU;
 
-    if (warp == kConsumers) {
+    if (warp == C) {
         if (lane == 0) {
             /* the unit's activations: blocks [4 UB ku, 4 UB (ku + 1)) of every row */
             auto load_x = [&](int ku, int s) {
@@ -738,8 +829,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
-    build_pair_lut(lut);
-    asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+    build_pair_lut<C>(lut);
+    asm volatile("bar.sync 1, %0;" ::"n"(C * 32) : "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = (int)(lane >> 2), t = (int)(lane & 3), pg = frag_row<128>(g);
     const uint32_t lut_base = saddr(lut), lane4 = lane * 4u;
@@ -908,37 +999,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int nb0 = n_begin + blk * a.RB;
         if constexpr (OUT == kOutGated) {
-            /* Rows 2i and 2i + 1 (gate and up; nb0 is even) are with lanes g and g + 4, g < 4.  Of
-             * its two activation rows each of the pair keeps one: the lower lane takes up of
-             * the first for gate of the second, and both have what one output needs. */
-            const bool up = g >= 4;
+            gated_outputs<MT, 128>(acc, pg, t, a.act, [&](int row, int col, float v) {
+                const int n = nb0 + r0 + row; /* nb0 is even */
+                if (r0 + row < a.RB && n < n_end && col < a.M)
+                    static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] = __float2bfloat16_rn(v);
+            });
+        } else {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float keep = up ? acc[mt][2 * h + 1] : acc[mt][2 * h], give = up ? acc[mt][2 * h] : acc[mt][2 * h + 1];
-                    const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 16);
-                    const int row = r0 + pg + 8 * h, col = mt * 8 + 2 * t + (up ? 1 : 0), n = nb0 + row;
-                    if (row < a.RB && n < n_end && col < a.M)
-                        static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] =
-                            __float2bfloat16_rn(up ? gated_value(got, keep, a.act) : gated_value(keep, got, a.act));
-                }
-            }
-            continue;
-        }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = r0 + pg + (q >> 1) * 8, col = mt * 8 + 2 * t + (q & 1);
-                const int n = nb0 + row;
-                if (row < a.RB && n < n_end && col < a.M) {
-                    if (a.ga.world > 0) {
-                        gather_store<OUT == kOutBF16>(a.ga, col, n, acc[mt][q]);
-                    } else if (OUT == kOutBF16) {
-                        static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * a.N + n] = __float2bfloat16_rn(acc[mt][q]);
-                    } else {
-                        static_cast<float *>(a.y)[(int64_t)col * a.N + n] = acc[mt][q];
+                for (int q = 0; q < 4; ++q) {
+                    const int row = r0 + pg + (q >> 1) * 8, col = mt * 8 + 2 * t + (q & 1);
+                    const int n = nb0 + row;
+                    if (row < a.RB && n < n_end && col < a.M) {
+                        if (a.ga.world > 0) {
+                            gather_store<OUT == kOutBF16>(a.ga, col, n, acc[mt][q]);
+                        } else if (OUT == kOutBF16) {
+                            static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * a.N + n] = __float2bfloat16_rn(acc[mt][q]);
+                        } else {
+                            static_cast<float *>(a.y)[(int64_t)col * a.N + n] = acc[mt][q];
+                        }
                     }
                 }
             }
@@ -1033,10 +1113,10 @@ struct Maps {
  * waits (griddepcontrol.wait) before reading activations or touching y and its
  * workspace.  `pdl` is off for the fixed-scratch entry, whose flags are reset
  * by a memset just before the launch. */
-template <int MT, bool SPLIT, bool BF16OUT>
+template <int MT, bool SPLIT, int OUT>
 int launch_t(const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool pdl)
 {
-    auto kern = htile_decode_kernel<MT, SPLIT, BF16OUT>;
+    auto kern = htile_decode_kernel<MT, SPLIT, OUT>;
     if (!ensure_smem((const void *)kern, smem_bytes<MT>()))
         return kLaunch;
     cudaLaunchConfig_t cfg = {};
@@ -1056,26 +1136,26 @@ int launch_t(const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool
     return kOk;
 }
 
-template <bool SPLIT, bool BF16OUT>
+template <bool SPLIT, int OUT>
 int launch_mt(int MT, const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool pdl)
 {
     if (MT == 1)
-        return launch_t<1, SPLIT, BF16OUT>(m, a, grid, st, pdl);
+        return launch_t<1, SPLIT, OUT>(m, a, grid, st, pdl);
     if (MT == 2)
-        return launch_t<2, SPLIT, BF16OUT>(m, a, grid, st, pdl);
-    return launch_t<4, SPLIT, BF16OUT>(m, a, grid, st, pdl);
+        return launch_t<2, SPLIT, OUT>(m, a, grid, st, pdl);
+    return launch_t<4, SPLIT, OUT>(m, a, grid, st, pdl);
 }
 
-template <int MT, bool SPLIT, int OUT, int NB>
+template <int MT, bool SPLIT, int OUT, int NB, int C>
 int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
-    auto kern = htile_rows_kernel<MT, SPLIT, OUT, NB>;
-    if (!ensure_smem((const void *)kern, r_smem_bytes<MT>()))
+    auto kern = htile_rows_kernel<MT, SPLIT, OUT, NB, C>;
+    if (!ensure_smem((const void *)kern, r_smem_bytes<MT, C>()))
         return kLaunch;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = r_smem_bytes<MT>();
+    cfg.blockDim = dim3(RowCfg<MT, C>::kThreads);
+    cfg.dynamicSmemBytes = r_smem_bytes<MT, C>();
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1088,14 +1168,14 @@ int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, b
     }
     return kOk;
 }
-template <int MT, bool SPLIT, int OUT>
+template <int MT, bool SPLIT, int OUT, int C = kConsumers>
 int launch_rows_t(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
     const int nb = 4 * a.UB / a.KH;
     if (nb == 2)
-        return launch_rows_nb<MT, SPLIT, OUT, 2>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, SPLIT, OUT, 2, C>(m, a, grid, st, pdl);
     if (nb == 1)
-        return launch_rows_nb<MT, SPLIT, OUT, 1>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, SPLIT, OUT, 1, C>(m, a, grid, st, pdl);
     return kLaunch;
 }
 
@@ -1105,34 +1185,35 @@ constexpr int align1k(int v) { return (v + 1023) & ~1023; }
  * Units take as many 256-k slices (UB = 4, 2, 1) as keep >= 3 ring stages, the
  * consumer warps' plan valid and K whole; row blocks of more than 4 tiles take
  * one (their requests are large already, and the shared tail needs UB = 1). */
-bool plan_rows(RowArgs &a, int R, int MT, bool pairs = false)
+template <int MT, int C = kConsumers>
+bool plan_rows(RowArgs &a, int R, bool pairs = false)
 {
+    using F = RowCfg<MT, C>;
     const int M = a.M, K = a.K;
     a.R = R;
-    a.nb = (a.R + kRowBlockMax - 1) / kRowBlockMax;
+    a.nb = (a.R + F::kBlockMax - 1) / F::kBlockMax;
     a.RB = (a.R + a.nb - 1) / a.nb;
     if (pairs) /* rows 2i and 2i + 1 in one block */
         a.RB += a.RB & 1;
     a.T = (a.RB + 15) / 16;
     a.xrows = std::min(M, 8 * MT);
-    const int ring = MT == 1 ? r_ring<1>() : MT == 2 ? r_ring<2>() : r_ring<4>();
-    const int scratch_warps = MT <= 2 ? 14 : 7;
+    constexpr int ring = F::kRing, scratch_warps = F::kScratchWarps;
     for (int ub = 4; ub >= 1; ub >>= 1) {
         if (ub > 1 && (a.T > 4 || K % (256 * ub) != 0))
             continue;
         /* warps per tile: as many consumer warps as the 16 allow, two blocks per warp
-         * and unit where that still fills them (MT 4: one, for registers) */
+         * and unit where that still fills them (MT 4 and many warps: one, for registers) */
         const int blocks = 4 * ub;
-        int nbk = MT <= 2 ? 2 : 1, kh = blocks / nbk;
-        while ((a.T * kh > kConsumers || a.T * (kh - 1) > scratch_warps) && nbk < blocks) {
+        int nbk = C == kConsumers && MT <= 2 ? 2 : 1, kh = blocks / nbk;
+        while ((a.T * kh > C || a.T * (kh - 1) > scratch_warps) && nbk < blocks) {
             nbk *= 2;
             kh = blocks / nbk;
         }
-        if (a.T * kh < kConsumers / 2 && nbk > 1 && a.T * kh * 2 <= kConsumers && a.T * (kh * 2 - 1) <= scratch_warps) {
+        if (a.T * kh < C / 2 && nbk > 1 && a.T * kh * 2 <= C && a.T * (kh * 2 - 1) <= scratch_warps) {
             nbk /= 2;
             kh = blocks / nbk;
         }
-        if (a.T * kh > kConsumers || a.T * (kh - 1) > scratch_warps || nbk > 2)
+        if (a.T * kh > C || a.T * (kh - 1) > scratch_warps || nbk > 2)
             continue;
         const int pt = align1k(ub * a.RB * 128), at = align1k(ub * a.RB * 16), xt = align1k(4 * ub * a.xrows * 128);
         const int stage = 2 * pt + at + xt;
@@ -1168,7 +1249,8 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
     const int tiles = (N + 15) / 16, base = tiles / sms, extra = tiles - base * sms;
     if (tail && !gt && MT <= 2 && base >= 1 && extra > 0 && (int64_t)extra * (K / 256) <= sms) {
         RowArgs t = a;
-        if (plan_rows(t, base * 16, MT) && t.UB == 1 && t.T * t.KH + kTailWarps <= kConsumers) {
+        if ((MT == 1 ? plan_rows<1>(t, base * 16) : plan_rows<2>(t, base * 16)) && t.UB == 1 &&
+            t.T * t.KH + kTailWarps <= kConsumers) {
             Scratch S;
             t.tail_units = extra * t.KU;
             if (get_scratch(st, (size_t)t.tail_units * 32 * 4 * MT, (size_t)extra, S)) {
@@ -1186,7 +1268,12 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
         int R = (N + g0 - 1) / g0;
         if (gated) /* whole pairs, and no less than the tile of rows that is read from shared memory */
             R = std::max(16, R + (R & 1));
-        if (!plan_rows(a, R, MT, gated))
+        const bool planned = MT == 4              ? plan_rows<4>(a, R, gated)
+                             : MT == 2 && gated     ? plan_rows<2, kSome>(a, R, true)
+                             : MT == 2              ? plan_rows<2>(a, R)
+                             : yk == kOutGated ? plan_rows<1, kMany>(a, R, true)
+                                                  : plan_rows<1>(a, R);
+        if (!planned)
             return kLaunch;
         grid = (N + a.R - 1) / a.R;
     }
@@ -1214,10 +1301,17 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
         maps.h16 = maps.h, maps.p16 = maps.p, maps.am16 = maps.am; /* not read */
     }
     const bool bf = yk == kOutBF16, pr = mode == kPrecise;
+    if (gated) {
+        if (MT == 4)
+            return pr ? launch_rows_t<4, true, kOutGated>(maps, a, grid, st, pdl)
+                      : launch_rows_t<4, false, kOutGated>(maps, a, grid, st, pdl);
+        if (MT == 2)
+            return pr ? launch_rows_t<2, true, kOutGated, kSome>(maps, a, grid, st, pdl)
+                      : launch_rows_t<2, false, kOutGated, kSome>(maps, a, grid, st, pdl);
+        return pr ? launch_rows_t<1, true, kOutGated, kMany>(maps, a, grid, st, pdl)
+                  : launch_rows_t<1, false, kOutGated, kMany>(maps, a, grid, st, pdl);
+    }
 #define GLINT_ROWS_CASE(mt)                                                                                            \
-    if (MT == mt && gated)                                                                                             \
-        return pr ? launch_rows_t<mt, true, kOutGated>(maps, a, grid, st, pdl)                                         \
-                  : launch_rows_t<mt, false, kOutGated>(maps, a, grid, st, pdl);                                       \
     if (MT == mt)                                                                                                      \
         return pr ? (bf ? launch_rows_t<mt, true, kOutBF16>(maps, a, grid, st, pdl)                                     \
                         : launch_rows_t<mt, true, kOutF32>(maps, a, grid, st, pdl))                                     \
@@ -1298,8 +1392,10 @@ int decode_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am
         a.ga = *gt;
     const bool bf = yk == kOutBF16;
     if (mode == kPrecise)
-        return bf ? launch_mt<true, true>(MT, maps, a, grid, st, true) : launch_mt<true, false>(MT, maps, a, grid, st, true);
-    return bf ? launch_mt<false, true>(MT, maps, a, grid, st, true) : launch_mt<false, false>(MT, maps, a, grid, st, true);
+        return bf ? launch_mt<true, kOutBF16>(MT, maps, a, grid, st, true)
+                  : launch_mt<true, kOutF32>(MT, maps, a, grid, st, true);
+    return bf ? launch_mt<false, kOutBF16>(MT, maps, a, grid, st, true)
+              : launch_mt<false, kOutF32>(MT, maps, a, grid, st, true);
 }
 
 /* ---- fixed-scratch variant ---------------------------------------------------
@@ -1389,12 +1485,72 @@ int htile_decode_launch(const uint8_t *hole, const uint8_t *plug, const float *a
     return decode_launch_impl(hole, plug, am, x, y, yk, M, N, K, mode, st, nullptr);
 }
 
-/* act(gate) * up of rows 2i and 2i + 1: always the row-owned kernel, whose sums never leave their
- * CTA (no workspace, at any N) */
-int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
-                              int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+namespace {
+/* stream-K's shares and its workspace: bytes of partial sums, and the counts behind them */
+struct GatedPlan {
+    DecodeArgs a{};
+    int MT, grid;
+    size_t sums, counts;
+    GatedPlan(int M, int N, int K) : MT(M <= 8 ? 1 : (M <= 16 ? 2 : 4))
+    {
+        a.M = M, a.N = N, a.K = K, a.KU = K / (MT <= 2 ? ku_of<1>() : ku_of<4>());
+        const int64_t rbs = (N + kRows - 1) / kRows;
+        a.units = rbs * a.KU;
+        grid = (int)std::min<int64_t>(a.units, sm_count());
+        /* parts per row block: at most ceil(KU / units_per_cta) + 1 */
+        const int64_t per_cta = std::max<int64_t>(1, a.units / grid);
+        a.max_parts = (int)std::min<int64_t>(grid, (a.KU + per_cta - 1) / per_cta + 1);
+        sums = (size_t)rbs * a.max_parts * kRows * 8 * MT * sizeof(float);
+        counts = (size_t)rbs * kConsumers * sizeof(int);
+    }
+};
+/* Counts to zero before the kernel that counts: as a kernel and not as a memset, so that the next one's
+ * weights stream while this one still waits for the last (9 rows, 2 x 18944 x 3584: 46.8 us with the
+ * memset, 43.2 with this). */
+__global__ void zero_counts_kernel(int *counts, int n)
 {
-    return launch_rows(hole, plug, am, x, h, kOutGated, M, N, K, mode, st, true, nullptr, false, act);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+        counts[i] = 0;
+}
+} // namespace
+
+/* act(gate) * up of rows 2i and 2i + 1 for M <= 32, by the kernels that htile_decode_launch takes at these sizes.
+ * The row-owned one keeps sums in its CTAs; stream-K's are the caller's: work of
+ * htile_decode_gated_work() bytes, the counts zeroed here, call by call.  (70B-shaped, 2 x 28672 x
+ * 8192, 16 rows: row-owned 148 us, four blocks of 7 tiles for 24.2 tiles a CTA; stream-K 126.) */
+int64_t htile_decode_gated_work(int M, int N, int K)
+{
+    if (rows_supported(N, K) || N < 16)
+        return 0;
+    const GatedPlan p(M, N, K);
+    return (int64_t)(p.sums + p.counts);
+}
+int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
+                              void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+{
+    if (rows_supported(N, K) || N < 16)
+        return launch_rows(hole, plug, am, x, h, kOutGated, M, N, K, mode, st, true, nullptr, false, act);
+    GatedPlan p(M, N, K);
+    Maps maps;
+    if (!decode_maps(maps, hole, plug, am, x, M, N, K, p.MT))
+        return kLaunch;
+    p.a.x = x, p.a.y = h, p.a.act = act;
+    p.a.ws = static_cast<float *>(work);
+    p.a.flags = reinterpret_cast<int *>(static_cast<unsigned char *>(work) + p.sums);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1), cfg.blockDim = dim3(256), cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, zero_counts_kernel, p.a.flags, (int)(p.counts / sizeof(int))) != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunch;
+    }
+    return mode == kPrecise ? launch_mt<true, kOutGated>(p.MT, maps, p.a, p.grid, st, true)
+                            : launch_mt<false, kOutGated>(p.MT, maps, p.a, p.grid, st, true);
 }
 
 bool htile_gather_supported(int M, int N) { return M >= 1 && M <= 32 && N >= 1; }
@@ -1490,8 +1646,10 @@ int htile_decode_launch_noalloc(const uint8_t *hole, const uint8_t *plug, const 
         return kLaunch;
     const bool bf = yk == kOutBF16;
     if (mode == kPrecise)
-        return bf ? launch_mt<true, true>(MT, maps, a, grid, st, false) : launch_mt<true, false>(MT, maps, a, grid, st, false);
-    return bf ? launch_mt<false, true>(MT, maps, a, grid, st, false) : launch_mt<false, false>(MT, maps, a, grid, st, false);
+        return bf ? launch_mt<true, kOutBF16>(MT, maps, a, grid, st, false)
+                  : launch_mt<true, kOutF32>(MT, maps, a, grid, st, false);
+    return bf ? launch_mt<false, kOutBF16>(MT, maps, a, grid, st, false)
+              : launch_mt<false, kOutF32>(MT, maps, a, grid, st, false);
 }
 
 /* This file's kernel error word (bounded waits that ran out); clear resets it. */

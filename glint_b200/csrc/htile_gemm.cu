@@ -1763,7 +1763,8 @@ int64_t htile_gemm_gated_work(int M, int N, int K)
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
     const int pairs = gemm_plan(a);
-    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int)) : 0;
+    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int))
+               : 0;
 }
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
                             void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)

@@ -228,34 +228,34 @@ __global__ void __launch_bounds__(kWarps * 32, APPEND ? 5 : 6) rope_kernel(const
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 o[i] = round2(y[2 * i], y[2 * i + 1]);
-            return;
-        }
-        uint64_t o1[4], o2[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            o1[i] = sub2(mul2(y1[i], c2[i]), mul2(y2[i], s2[i]));
-            o2[i] = add2(mul2(y2[i], c2[i]), mul2(y1[i], s2[i]));
-        }
-        if (half != D / 2) { /* places behind the rotated ones stay, whatever their values */
+        } else {
+            uint64_t o1[4], o2[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool first = P == kRuns ? partners : 8 * l + 2 * i < half;
-                const bool second = P == kRuns ? partners : 8 * l + 2 * i + 1 < half;
-                float f[2], y[2];
-                unpack2f(o1[i], f[0], f[1]), unpack2f(y1[i], y[0], y[1]);
-                o1[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
-                unpack2f(o2[i], f[0], f[1]), unpack2f(y2[i], y[0], y[1]);
-                o2[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
+                o1[i] = sub2(mul2(y1[i], c2[i]), mul2(y2[i], s2[i]));
+                o2[i] = add2(mul2(y2[i], c2[i]), mul2(y1[i], s2[i]));
             }
-        }
+            if (half != D / 2) { /* places behind the rotated ones stay, whatever their values */
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (P == kBeside) {
-                float a0, a1, b0, b1;
-                unpack2f(o1[i], a0, a1), unpack2f(o2[i], b0, b1);
-                o[2 * i] = round2(a0, b0), o[2 * i + 1] = round2(a1, b1);
-            } else {
-                o[i] = round2(o1[i]), o[4 + i] = round2(o2[i]);
+                for (int i = 0; i < 4; ++i) {
+                    const bool first = P == kRuns ? partners : 8 * l + 2 * i < half;
+                    const bool second = P == kRuns ? partners : 8 * l + 2 * i + 1 < half;
+                    float f[2], y[2];
+                    unpack2f(o1[i], f[0], f[1]), unpack2f(y1[i], y[0], y[1]);
+                    o1[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
+                    unpack2f(o2[i], f[0], f[1]), unpack2f(y2[i], y[0], y[1]);
+                    o2[i] = pack2f(first ? f[0] : y[0], second ? f[1] : y[1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (P == kBeside) {
+                    float a0, a1, b0, b1;
+                    unpack2f(o1[i], a0, a1), unpack2f(o2[i], b0, b1);
+                    o[2 * i] = round2(a0, b0), o[2 * i + 1] = round2(a1, b1);
+                } else {
+                    o[i] = round2(o1[i]), o[4 + i] = round2(o2[i]);
+                }
             }
         }
     };
@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kWarps * 32, APPEND ? 5 : 6) rope_kernel(const
                     *reinterpret_cast<uint4 *>(head + 2 * ea) = make_uint4(o[0], o[1], o[2], o[3]);
                     *reinterpret_cast<uint4 *>(head + 2 * eb) = make_uint4(o[4], o[5], o[6], o[7]);
                     __syncwarp();
-                    const uint4 u = *reinterpret_cast<const uint4 *>(head + 32 * l), v = *reinterpret_cast<const uint4 *>(head + 32 * l + 16);
+                    const uint4 u = *reinterpret_cast<const uint4 *>(head + 32 * l);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(head + 32 * l + 16);
                     o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w, o[4] = v.x, o[5] = v.y, o[6] = v.z, o[7] = v.w;
                 }
             }

@@ -134,14 +134,15 @@ def test_shapes(M, K, F, mode, name):
 
 @pytest.mark.parametrize("mode", ["fast", "precise"])
 @pytest.mark.parametrize("M,K,F", [(1, 4096, 14336), (5, 2048, 6911), (16, 1024, 28672), (31, 512, 18001), (32, 16384, 500),
-                                   (511, 1024, 14336), (300, 512, 9473), (1030, 256, 10000)])
+                                   (511, 1024, 14336), (300, 512, 9473), (1030, 256, 10000), (16, 10240, 6000), (2, 8192, 4999),
+                                   (9, 2560, 9728), (7, 5120, 3000), (8, 3584, 2222), (13, 33280, 50)])
 def test_wide_layers(M, K, F, mode):
     """More rows than two blocks a CTA; tiles shared between CTA pairs (511, 300 and 1030 rows)."""
     check(M, K, F, mode=mode)
 
 
 @pytest.mark.parametrize("mode", ["fast", "precise"])
-@pytest.mark.parametrize("M,K,F,bs", [(1, 64, 5, 64), (4, 192, 33, 64), (40, 320, 9, 64), (3, 512, 10, 128), (9, 96, 6, 32), (2, 34, 3, 17),
+@pytest.mark.parametrize("M,K,F,bs", [(1, 64, 5, 64), (4, 192, 33, 64), (12, 448, 700, 64), (16, 2880, 1111, 64), (20, 2880, 50, 64), (40, 320, 9, 64), (3, 512, 10, 128), (9, 96, 6, 32), (2, 34, 3, 17),
                                       (11, 33, 4, 16), (1, 1, 1, 1), (65, 640, 1000, 64)])
 def test_any_shape(M, K, F, bs, mode):
     check(M, K, F, bs=bs, mode=mode, name="gelu_tanh")
