@@ -43,6 +43,7 @@ struct Args {
     int q_steps, k_steps;     /* of a token's heads; v, with the cache, takes as many as k */
     int steps, chunk, chunks; /* in all; of them a warp takes; such parts a token */
     int64_t warps;            /* tokens * chunks */
+    uint64_t none;            /* -0 twice, see product2() */
 };
 
 /* 8 values as BF16 pairs, by loads that may follow a store to the same place */
@@ -77,6 +78,9 @@ __device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b)
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+/* a b, rounded, that no sum behind it takes into an fma (of mul.rn.f32x2 the assembler makes one): none is -0
+ * twice, from the host, so that no compiler knows it */
+__device__ __forceinline__ uint64_t product2(uint64_t a, uint64_t b, uint64_t none) { return fma2(a, b, none); }
 __device__ __forceinline__ uint32_t round2(float lo, float hi)
 {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
@@ -162,6 +166,7 @@ __global__ void __launch_bounds__(kWarps * 32, APPEND ? 5 : 6) rope_kernel(const
         }
     }
 
+    const uint64_t none = g.none;
     /* the lane's values of a head, normed with its weights (NULL: not) and turned, as BF16 pairs */
     auto turned = [&](const uint32_t (&x)[8], const float *weight, uint32_t (&o)[8]) {
         /* first and second values of pairs 2 i, 2 i + 1 */
@@ -232,8 +237,8 @@ __global__ void __launch_bounds__(kWarps * 32, APPEND ? 5 : 6) rope_kernel(const
             uint64_t o1[4], o2[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                o1[i] = sub2(mul2(y1[i], c2[i]), mul2(y2[i], s2[i]));
-                o2[i] = add2(mul2(y2[i], c2[i]), mul2(y1[i], s2[i]));
+                o1[i] = sub2(product2(y1[i], c2[i], none), product2(y2[i], s2[i], none));
+                o2[i] = add2(product2(y2[i], c2[i], none), product2(y1[i], s2[i], none));
             }
             if (half != D / 2) { /* places behind the rotated ones stay, whatever their values */
 #pragma unroll
@@ -344,6 +349,7 @@ int launch(Args &g, bool append, bool vec, cudaStream_t st)
     g.chunk = (int)((g.steps + want - 1) / want);
     g.chunks = (g.steps + g.chunk - 1) / g.chunk;
     g.warps = (int64_t)a.tokens * g.chunks;
+    g.none = 0x8000000080000000u;
     const int64_t grid = (g.warps + kWarps - 1) / kWarps;
     if (grid > INT32_MAX)
         return kBadArg;
