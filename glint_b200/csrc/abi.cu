@@ -676,59 +676,6 @@ int glint_htile_stream(const uint8_t *d_hole, const uint8_t *d_plug, const float
                         blocksize, mode == GLINT_HTILE_FAST ? kFast : kPrecise, stream);
 }
 
-namespace {
-/* kOk, or what glint_htile_gated_stream returns for these arguments before it looks at work */
-int gated_check(const GlintHtileGated *a)
-{
-    if (!a || a->M < 0 || a->F < 0 || a->K < 0 || a->F > INT32_MAX / 2 ||
-        (a->mode != GLINT_HTILE_PRECISE && a->mode != GLINT_HTILE_FAST) ||
-        (a->act != GLINT_ACT_SILU && a->act != GLINT_ACT_GELU_TANH))
-        return kBadArg;
-    if (a->blocksize <= 0)
-        return kBadBlocksize;
-    return kOk;
-}
-/* the shapes that the kernels on TMA take, at any M */
-bool gated_streams(const GlintHtileGated *a)
-{
-    return htile_decode_supported(a->hole, a->plug, a->absmax, a->x, std::min(a->M, 32), 2 * a->F, a->K, a->blocksize);
-}
-/* rows up to which the streaming kernel is taken */
-constexpr int kGatedStreamM = 32;
-} // namespace
-
-int64_t glint_htile_gated_work_bytes(const GlintHtileGated *a)
-{
-    if (gated_check(a) != kOk)
-        return kBadArg;
-    if (a->M == 0 || a->F == 0 || a->K == 0 || !gated_streams(a))
-        return 0;
-    if (a->M <= kGatedStreamM)
-        return htile_decode_gated_work(a->M, 2 * a->F, a->K);
-    return a->mode == GLINT_HTILE_PRECISE ? 0 : htile_gemm_gated_work(a->M, 2 * a->F, a->K);
-}
-int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
-{
-    const int rc = gated_check(a);
-    if (rc != kOk)
-        return rc;
-    if (a->M == 0 || a->F == 0)
-        return kOk;
-    if (!a->h || (a->K && (!a->hole || !a->plug || !a->absmax || !a->x)))
-        return kBadArg;
-    if (a->K == 0)
-        return cudaMemsetAsync(a->h, 0, (size_t)a->M * a->F * 2, stream) == cudaSuccess ? kOk : kLaunch;
-    if (glint_htile_gated_work_bytes(a) > 0 && (!a->work || !aligned_to(a->work, 16)))
-        return kBadArg;
-    const HtileMode mode = a->mode == GLINT_HTILE_FAST ? kFast : kPrecise;
-    const int N = 2 * a->F;
-    if (!gated_streams(a))
-        return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, mode, a->act, stream);
-    if (a->M <= kGatedStreamM)
-        return htile_decode_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->work, a->M, N, a->K, mode, a->act, stream);
-    return htile_gemm_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->work, a->M, N, a->K, mode, a->act, stream);
-}
-
 int glint_htile_gather_stream(const uint8_t *d_hole, const uint8_t *d_plug, const float *d_absmax,
                               const __nv_bfloat16 *d_x, void *const *d_y_ranks, unsigned int *const *d_flag_ranks,
                               int world, int rank, int y_dtype, int M, int N, int K, int ld_y, int n0,

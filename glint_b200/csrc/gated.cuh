@@ -7,6 +7,14 @@
 
 namespace glint {
 
+/* What the H-TILE kernels' gated epilogues take.  Against activations in FP16 (see htile_gated.cu) a product's sums
+ * are of x[m] / x_scale[m] and, where weights carry their absmax into the tensor cores, of W[n] * row_scale[n]. */
+struct GatedEpilogue {
+    int act;
+    const float *x_scale;   /* [M] powers of two */
+    const float *row_scale; /* [N] powers of two */
+};
+
 /* act(g) u, act(g) = g / (1 + exp(-z)): z = g (silu), or 2 sqrt(2 / pi) (g + 0.044715 g^3), which
  * makes it g (1 + tanh(z / 2)) / 2.  The fast exponential is within 2^-17 of its value
  * wherever act(g) is not 0 in BF16 and the division within 2^-22, far inside the result's

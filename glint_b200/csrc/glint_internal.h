@@ -107,17 +107,21 @@ int htile_decode_gather_launch(const uint8_t *hole, const uint8_t *plug, const f
                                int world, int rank, OutKind y_kind, int M, int N, int K, int ldy, int n0,
                                HtileMode mode, cudaStream_t stream);
 
-/* h[M, N / 2] BF16 = act(y[:, 2i]) * y[:, 2i + 1], y as of htile_launch (N even; gated.cuh):
- * M <= 32 and any M of the TMA kernels' shapes (bs == 64, K % 256 == 0, 16-byte alignment), and
- * all others.  work: htile_decode_gated_work() and, in fast mode, htile_gemm_gated_work() bytes. */
-int64_t htile_decode_gated_work(int M, int N, int K);
+/* h[M, N / 2] BF16 = act(y[:, 2i]) * y[:, 2i + 1], y as of htile_launch (N even; gated.cuh, htile_gated.cu): M <= 32
+ * and any M of the TMA kernels' shapes (bs == 64, K % 256 == 0, 16-byte alignment), and all others.  The first
+ * two take x as it is in precise mode and in FP16 (htile_gated.cu) in fast mode; .._work(): the bytes of
+ * `sums` that they need for tiles split among CTAs, and how many `counts`, zero at the start. */
+struct GatedEpilogue;
+int64_t htile_decode_gated_work(int M, int N, int K, int64_t *counts);
 int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
-                              void *h, void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
-int64_t htile_gemm_gated_work(int M, int N, int K);
+                              void *h, float *sums, int *counts, int M, int N, int K, HtileMode mode, GatedEpilogue ep,
+                              cudaStream_t stream);
+int64_t htile_gemm_gated_work(int M, int N, int K, int64_t *counts);
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
-                            void *h, void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t stream);
+                            void *h, float *sums, int *counts, int M, int N, int K, HtileMode mode, GatedEpilogue ep,
+                            cudaStream_t stream);
 int htile_gemv_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
-                            void *h, int M, int N, int K, int blocksize, HtileMode mode, int act, cudaStream_t stream);
+                            void *h, int M, int N, int K, int blocksize, int act, cudaStream_t stream);
 
 /* K-major layout, parent-only decode GEMV and activation-selected plug correction
  * (kmajor.cu): n % 8 == 0, K % 64 == 0, K <= kKmMaxK, blocksize 64, 16-byte

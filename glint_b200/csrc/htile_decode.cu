@@ -41,6 +41,8 @@
 #include <mutex>
 #include <unordered_map>
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "gated.cuh"
 #include "gather.cuh"
@@ -79,6 +81,17 @@ constexpr int n_slots() { return ku_of<MT>() == 256 ? 2 : 3; } /* as many as fit
 template <int MT>
 constexpr int smem_bytes() { return kLutBytes + 1024 + n_slots<MT>() * slot_bytes<MT>() + 2 * 8 * n_slots<MT>() + 64; }
 
+/* How a weight meets the tensor cores: one BF16 value, the pair (hi, lo), or, against activations in FP16 (gated
+ * projections, htile_gated.cu), one FP16 value. */
+enum Arith : int { kHi = 0, kHiLo = 1, kHalf = 2 };
+
+__device__ __forceinline__ void mma_f16_16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+                 "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_bf16_16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
@@ -98,12 +111,13 @@ __device__ __forceinline__ uint32_t split_pair(float c)
  * store covers a quarter of one entry's 128-byte row of 32 replicas, so a warp's
  * store fills four whole rows (four wavefronts, no bank conflicts; one thread per
  * entry writing its own row would put all 32 lanes on the same four banks). */
-template <int WARPS>
-__device__ __forceinline__ void build_pair_lut(uint32_t *lut)
+template <int WARPS, int ARITH>
+__device__ __forceinline__ void build_lut(uint32_t *lut)
 {
     for (int i = (int)threadIdx.x; i < 256 * 8; i += WARPS * 32) {
         const int e = i >> 3;
-        const uint32_t v = split_pair(g_cells[e >> 4][e & 15]);
+        const float cell = g_cells[e >> 4][e & 15];
+        const uint32_t v = ARITH == kHalf ? (uint32_t)__half_as_ushort(__float2half_rn(cell)) : split_pair(cell);
         reinterpret_cast<uint4 *>(lut + e * 64)[i & 7] = make_uint4(v, v, v, v);
     }
 }
@@ -118,7 +132,7 @@ struct DecodeArgs {
     int64_t units;      /* row blocks * KU */
     int max_parts;
     GatherArgs ga;
-    int act; /* kOutGated: of the gate rows */
+    GatedEpilogue ep; /* kOutGated */
 };
 
 /* first unit of CTA c under the even split of `units` over `ctas` */
@@ -149,7 +163,7 @@ __device__ __forceinline__ int frag_row(int g)
 
 /* Arithmetic of one 64-k block (see tile_block): codes -> codebook -> MMAs -> the
  * block's sums scaled by its absmax and added to acc. */
-template <int MT, bool SPLIT>
+template <int MT, int ARITH>
 __device__ __forceinline__ void tile_math(const uint32_t (&E)[2][2], const uint32_t (&O)[2][2], const float (&sc)[2],
                                           const uint4 (&xb)[MT][2], uint32_t lut_base, uint32_t lane4,
                                           float (&acc)[MT][4])
@@ -178,9 +192,12 @@ __device__ __forceinline__ void tile_math(const uint32_t (&E)[2][2], const uint3
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t xw[4] = {xb[mt][wd].x, xb[mt][wd].y, xb[mt][wd].z, xb[mt][wd].w};
-            mma_bf16_16816(part[st & 1][mt], ahi, xw[(st & 1) * 2], xw[(st & 1) * 2 + 1]);
+            if (ARITH == kHalf)
+                mma_f16_16816(part[st & 1][mt], ahi, xw[(st & 1) * 2], xw[(st & 1) * 2 + 1]);
+            else
+                mma_bf16_16816(part[st & 1][mt], ahi, xw[(st & 1) * 2], xw[(st & 1) * 2 + 1]);
         }
-        if (SPLIT) {
+        if (ARITH == kHiLo) {
             const uint32_t alo[4] = {__byte_perm(e[0][0], e[0][1], 0x7632), __byte_perm(e[1][0], e[1][1], 0x7632),
                                      __byte_perm(e[0][2], e[0][3], 0x7632), __byte_perm(e[1][2], e[1][3], 0x7632)};
 #pragma unroll
@@ -212,7 +229,7 @@ __device__ __forceinline__ void tile_math(const uint32_t (&E)[2][2], const uint3
  * whatever the k order; hi (and lo in precise mode) BF16 halves of the codebook.
  * Lanes whose activation row mt*8+g is >= M (rows the TMA box fills with zeros)
  * take zeros without reading shared memory. */
-template <int MT, bool SPLIT, int ROWB>
+template <int MT, int ARITH, int ROWB>
 __device__ __forceinline__ void tile_block(uint32_t hole, uint32_t plug, uint32_t am, uint32_t am_col, uint32_t xbox,
                                            uint32_t xph, int c, int r0, int ro, int g, int t, uint32_t lut_base,
                                            uint32_t lane4, int M, float (&acc)[MT][4])
@@ -245,7 +262,7 @@ __device__ __forceinline__ void tile_block(uint32_t hole, uint32_t plug, uint32_
         xb[mt][0] = lds128_if(rowb + (((uint32_t)(2 * t) ^ ph) << 4), live);
         xb[mt][1] = lds128_if(rowb + (((uint32_t)(2 * t + 1) ^ ph) << 4), live);
     }
-    tile_math<MT, SPLIT>(E, O, sc, xb, lut_base, lane4, acc);
+    tile_math<MT, ARITH>(E, O, sc, xb, lut_base, lane4, acc);
 }
 
 /* Shared-memory byte offsets, within a ring stage, of one lane's operands of one 64-k
@@ -290,7 +307,7 @@ __device__ __forceinline__ BlockOffs<MT> block_offs(int c, int r0, int ro, int g
 
 /* tile_block with the operands at precomputed offsets from the stage base `st`
  * (plug tile at st + pt). */
-template <int MT, bool SPLIT>
+template <int MT, int ARITH>
 __device__ __forceinline__ void tile_block_at(uint32_t st, uint32_t pt, const BlockOffs<MT> &o, uint32_t lut_base,
                                               uint32_t lane4, float (&acc)[MT][4])
 {
@@ -314,15 +331,15 @@ __device__ __forceinline__ void tile_block_at(uint32_t st, uint32_t pt, const Bl
         xb[mt][0] = lds128_if(st + o.x0[mt], live);
         xb[mt][1] = lds128_if(st + o.x1[mt], live);
     }
-    tile_math<MT, SPLIT>(E, O, sc, xb, lut_base, lane4, acc);
+    tile_math<MT, ARITH>(E, O, sc, xb, lut_base, lane4, acc);
 }
 
 /* A 16-row tile's sums as gated outputs: rows 2i and 2i + 1 (gate and up; `n` of the tile's first row is even)
  * are with two lanes, that differ in the bit of g which is a row's parity.  Of two activation rows each
  * keeps one: the gate's lane takes up of the first for gate of the second.  put(n, col, value): row pair
  * n / 2 and activation row. */
-template <int MT, int ROWB, class Put>
-__device__ __forceinline__ void gated_outputs(const float (&acc)[MT][4], int pg, int t, int act, Put put)
+template <int MT, int ROWB, int ARITH, class Put>
+__device__ __forceinline__ void gated_outputs(const float (&acc)[MT][4], int pg, int t, const GatedEpilogue &ep, int M, Put put)
 {
     const bool up = pg & 1;
 #pragma unroll
@@ -331,12 +348,14 @@ __device__ __forceinline__ void gated_outputs(const float (&acc)[MT][4], int pg,
         for (int h = 0; h < 2; ++h) {
             const float keep = up ? acc[mt][2 * h + 1] : acc[mt][2 * h], give = up ? acc[mt][2 * h] : acc[mt][2 * h + 1];
             const float got = __shfl_xor_sync(0xFFFFFFFFu, give, ROWB == 128 ? 16 : 4);
-            put(pg + 8 * h, mt * 8 + 2 * t + (up ? 1 : 0), up ? gated_value(got, keep, act) : gated_value(keep, got, act));
+            const int col = mt * 8 + 2 * t + (up ? 1 : 0);
+            const float by = ARITH == kHalf ? ep.x_scale[min(col, M - 1)] : 1.f;
+            put(pg + 8 * h, col, gated_value(by * (up ? got : keep), by * (up ? keep : got), ep.act));
         }
     }
 }
 
-template <int MT, bool SPLIT, int OUT>
+template <int MT, int ARITH, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     htile_decode_kernel(const __grid_constant__ CUtensorMap hmap, const __grid_constant__ CUtensorMap pmap,
                         const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap xmap,
@@ -429,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     /* codebook as BF16 hi/lo pairs, one replica per lane (first 128 B of each 256-B
      * entry row); the consumer warps then meet on named barrier 1 (the producer is
      * not in it) */
-    build_pair_lut<kConsumers>(lut);
+    build_lut<kConsumers, ARITH>(lut);
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
     /* y, the workspace and its flags are touched only after the previous kernel
      * in the stream is complete (no-op without programmatic dependent launch) */
@@ -468,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         };
         auto put_gated = [&] {
-            gated_outputs<MT, kKU / 2>(acc, pg, t, a.act, [&](int row, int col, float v) {
+            gated_outputs<MT, kKU / 2, ARITH>(acc, pg, t, a.ep, a.M, [&](int row, int col, float v) {
                 const int n = rb * kRows + r0 + row;
                 if (n < a.N && col < a.M)
                     static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] = __float2bfloat16_rn(v);
@@ -611,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t am_col = kKU == 256 ? 0u : (uint32_t)(ku & 1) * 2;
 #pragma unroll
         for (int c = 0; c < kKU / 64; ++c)
-            tile_block<MT, SPLIT, kKU / 2>(slot, slot + kPlaneTile, slot + 2 * kPlaneTile, am_col + c,
+            tile_block<MT, ARITH, kKU / 2>(slot, slot + kPlaneTile, slot + 2 * kPlaneTile, am_col + c,
                                            xs + (uint32_t)c * (8 * MT * 128), 0u, c, r0, 0, g, t, lut_base, lane4, a.M,
                                            acc);
         __syncwarp();
@@ -719,10 +738,10 @@ struct RowArgs {
     uint32_t tail_tx;
     float *tail_ws;
     int *tail_cnt;
-    int act; /* kOutGated: of the gate rows */
+    GatedEpilogue ep; /* kOutGated */
 };
 
-template <int MT, bool SPLIT, int OUT, int NB, int C>
+template <int MT, int ARITH, int OUT, int NB, int C>
 __global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
     htile_rows_kernel(const __grid_constant__ CUtensorMap hmap, const __grid_constant__ CUtensorMap pmap,
                       const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap xmap,
@@ -829,7 +848,7 @@ __global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
         return;
     }
 
-    build_pair_lut<C>(lut);
+    build_lut<C, ARITH>(lut);
     asm volatile("bar.sync 1, %0;" ::"n"(C * 32) : "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = (int)(lane >> 2), t = (int)(lane & 3), pg = frag_row<128>(g);
@@ -850,7 +869,7 @@ __global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
             const bool ok = lane == 0 ? mbar_wait_suspend_bounded(tail_full, 0u, &g_decode_error) : true;
             const uint32_t ts = saddr(tail);
             if (__shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0))
-                tile_block<MT, SPLIT, 128>(ts, ts + 2048, ts + 4096, (uint32_t)j,
+                tile_block<MT, ARITH, 128>(ts, ts + 2048, ts + 4096, (uint32_t)j,
                                            ts + (uint32_t)(kTailX + j * a.xrows * 128), (uint32_t)(j * a.xrows) & 7u, j,
                                            0, 0, g, t, lut_base, lane4, a.M, acc);
             float4 *part = reinterpret_cast<float4 *>(tail + kTailX + r_xsub<MT>());
@@ -954,7 +973,7 @@ __global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
             const uint32_t st = saddr(ring + s * stage_bytes);
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                tile_block_at<MT, SPLIT>(st, (uint32_t)a.pt, offs[j], lut_base, lane4, acc);
+                tile_block_at<MT, ARITH>(st, (uint32_t)a.pt, offs[j], lut_base, lane4, acc);
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(&empty[s]);
@@ -999,7 +1018,7 @@ __global__ void __launch_bounds__(RowCfg<MT, C>::kThreads, 1)
         }
         const int nb0 = n_begin + blk * a.RB;
         if constexpr (OUT == kOutGated) {
-            gated_outputs<MT, 128>(acc, pg, t, a.act, [&](int row, int col, float v) {
+            gated_outputs<MT, 128, ARITH>(acc, pg, t, a.ep, a.M, [&](int row, int col, float v) {
                 const int n = nb0 + r0 + row; /* nb0 is even */
                 if (r0 + row < a.RB && n < n_end && col < a.M)
                     static_cast<__nv_bfloat16 *>(a.y)[(int64_t)col * (a.N / 2) + n / 2] = __float2bfloat16_rn(v);
@@ -1113,10 +1132,10 @@ struct Maps {
  * waits (griddepcontrol.wait) before reading activations or touching y and its
  * workspace.  `pdl` is off for the fixed-scratch entry, whose flags are reset
  * by a memset just before the launch. */
-template <int MT, bool SPLIT, int OUT>
+template <int MT, int ARITH, int OUT>
 int launch_t(const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool pdl)
 {
-    auto kern = htile_decode_kernel<MT, SPLIT, OUT>;
+    auto kern = htile_decode_kernel<MT, ARITH, OUT>;
     if (!ensure_smem((const void *)kern, smem_bytes<MT>()))
         return kLaunch;
     cudaLaunchConfig_t cfg = {};
@@ -1136,20 +1155,20 @@ int launch_t(const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool
     return kOk;
 }
 
-template <bool SPLIT, int OUT>
+template <int ARITH, int OUT>
 int launch_mt(int MT, const Maps &m, const DecodeArgs &a, int grid, cudaStream_t st, bool pdl)
 {
     if (MT == 1)
-        return launch_t<1, SPLIT, OUT>(m, a, grid, st, pdl);
+        return launch_t<1, ARITH, OUT>(m, a, grid, st, pdl);
     if (MT == 2)
-        return launch_t<2, SPLIT, OUT>(m, a, grid, st, pdl);
-    return launch_t<4, SPLIT, OUT>(m, a, grid, st, pdl);
+        return launch_t<2, ARITH, OUT>(m, a, grid, st, pdl);
+    return launch_t<4, ARITH, OUT>(m, a, grid, st, pdl);
 }
 
-template <int MT, bool SPLIT, int OUT, int NB, int C>
+template <int MT, int ARITH, int OUT, int NB, int C>
 int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
-    auto kern = htile_rows_kernel<MT, SPLIT, OUT, NB, C>;
+    auto kern = htile_rows_kernel<MT, ARITH, OUT, NB, C>;
     if (!ensure_smem((const void *)kern, r_smem_bytes<MT, C>()))
         return kLaunch;
     cudaLaunchConfig_t cfg = {};
@@ -1168,14 +1187,14 @@ int launch_rows_nb(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, b
     }
     return kOk;
 }
-template <int MT, bool SPLIT, int OUT, int C = kConsumers>
+template <int MT, int ARITH, int OUT, int C = kConsumers>
 int launch_rows_t(const Maps &m, const RowArgs &a, int grid, cudaStream_t st, bool pdl)
 {
     const int nb = 4 * a.UB / a.KH;
     if (nb == 2)
-        return launch_rows_nb<MT, SPLIT, OUT, 2, C>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, ARITH, OUT, 2, C>(m, a, grid, st, pdl);
     if (nb == 1)
-        return launch_rows_nb<MT, SPLIT, OUT, 1, C>(m, a, grid, st, pdl);
+        return launch_rows_nb<MT, ARITH, OUT, 1, C>(m, a, grid, st, pdl);
     return kLaunch;
 }
 
@@ -1236,12 +1255,12 @@ bool plan_rows(RowArgs &a, int R, bool pairs = false)
  * leave most SMs a mostly empty last tile. */
 int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
                 OutKind yk, int M, int N, int K, HtileMode mode, cudaStream_t st, bool pdl,
-                const GatherArgs *gt = nullptr, bool tail = false, int act = 0)
+                const GatherArgs *gt = nullptr, bool tail = false, GatedEpilogue ep = {})
 {
     const int MT = M <= 8 ? 1 : (M <= 16 ? 2 : 4);
     const int sms = sm_count();
     RowArgs a{};
-    a.y = y, a.M = M, a.N = N, a.K = K, a.act = act;
+    a.y = y, a.M = M, a.N = N, a.K = K, a.ep = ep;
     const bool gated = yk == kOutGated;
     if (gt)
         a.ga = *gt;
@@ -1303,20 +1322,20 @@ int launch_rows(const uint8_t *hole, const uint8_t *plug, const float *am, const
     const bool bf = yk == kOutBF16, pr = mode == kPrecise;
     if (gated) {
         if (MT == 4)
-            return pr ? launch_rows_t<4, true, kOutGated>(maps, a, grid, st, pdl)
-                      : launch_rows_t<4, false, kOutGated>(maps, a, grid, st, pdl);
+            return pr ? launch_rows_t<4, kHiLo, kOutGated>(maps, a, grid, st, pdl)
+                      : launch_rows_t<4, kHalf, kOutGated>(maps, a, grid, st, pdl);
         if (MT == 2)
-            return pr ? launch_rows_t<2, true, kOutGated, kSome>(maps, a, grid, st, pdl)
-                      : launch_rows_t<2, false, kOutGated, kSome>(maps, a, grid, st, pdl);
-        return pr ? launch_rows_t<1, true, kOutGated, kMany>(maps, a, grid, st, pdl)
-                  : launch_rows_t<1, false, kOutGated, kMany>(maps, a, grid, st, pdl);
+            return pr ? launch_rows_t<2, kHiLo, kOutGated, kSome>(maps, a, grid, st, pdl)
+                      : launch_rows_t<2, kHalf, kOutGated, kSome>(maps, a, grid, st, pdl);
+        return pr ? launch_rows_t<1, kHiLo, kOutGated, kMany>(maps, a, grid, st, pdl)
+                  : launch_rows_t<1, kHalf, kOutGated, kMany>(maps, a, grid, st, pdl);
     }
 #define GLINT_ROWS_CASE(mt)                                                                                            \
     if (MT == mt)                                                                                                      \
-        return pr ? (bf ? launch_rows_t<mt, true, kOutBF16>(maps, a, grid, st, pdl)                                     \
-                        : launch_rows_t<mt, true, kOutF32>(maps, a, grid, st, pdl))                                     \
-                  : (bf ? launch_rows_t<mt, false, kOutBF16>(maps, a, grid, st, pdl)                                    \
-                        : launch_rows_t<mt, false, kOutF32>(maps, a, grid, st, pdl));
+        return pr ? (bf ? launch_rows_t<mt, kHiLo, kOutBF16>(maps, a, grid, st, pdl)                                    \
+                        : launch_rows_t<mt, kHiLo, kOutF32>(maps, a, grid, st, pdl))                                     \
+                  : (bf ? launch_rows_t<mt, kHi, kOutBF16>(maps, a, grid, st, pdl)                                    \
+                        : launch_rows_t<mt, kHi, kOutF32>(maps, a, grid, st, pdl));
     GLINT_ROWS_CASE(1)
     GLINT_ROWS_CASE(2)
     GLINT_ROWS_CASE(4)
@@ -1392,10 +1411,10 @@ int decode_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am
         a.ga = *gt;
     const bool bf = yk == kOutBF16;
     if (mode == kPrecise)
-        return bf ? launch_mt<true, kOutBF16>(MT, maps, a, grid, st, true)
-                  : launch_mt<true, kOutF32>(MT, maps, a, grid, st, true);
-    return bf ? launch_mt<false, kOutBF16>(MT, maps, a, grid, st, true)
-              : launch_mt<false, kOutF32>(MT, maps, a, grid, st, true);
+        return bf ? launch_mt<kHiLo, kOutBF16>(MT, maps, a, grid, st, true)
+                  : launch_mt<kHiLo, kOutF32>(MT, maps, a, grid, st, true);
+    return bf ? launch_mt<kHi, kOutBF16>(MT, maps, a, grid, st, true)
+              : launch_mt<kHi, kOutF32>(MT, maps, a, grid, st, true);
 }
 
 /* ---- fixed-scratch variant ---------------------------------------------------
@@ -1504,53 +1523,33 @@ struct GatedPlan {
         counts = (size_t)rbs * kConsumers * sizeof(int);
     }
 };
-/* Counts to zero before the kernel that counts: as a kernel and not as a memset, so that the next one's
- * weights stream while this one still waits for the last (9 rows, 2 x 18944 x 3584: 46.8 us with the
- * memset, 43.2 with this). */
-__global__ void zero_counts_kernel(int *counts, int n)
-{
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-        counts[i] = 0;
-}
 } // namespace
 
 /* act(gate) * up of rows 2i and 2i + 1 for M <= 32, by the kernels that htile_decode_launch takes at these sizes.
- * The row-owned one keeps sums in its CTAs; stream-K's are the caller's: work of
- * htile_decode_gated_work() bytes, the counts zeroed here, call by call.  (70B-shaped, 2 x 28672 x
- * 8192, 16 rows: row-owned 148 us, four blocks of 7 tiles for 24.2 tiles a CTA; stream-K 126.) */
-int64_t htile_decode_gated_work(int M, int N, int K)
+ * The row-owned one keeps sums in its CTAs; stream-K's are the caller's, and the counts behind them are
+ * zero when the kernel starts.  (70B-shaped, 2 x 28672 x 8192, 16 rows: row-owned 148 us, four blocks of 7
+ * tiles for 24.2 tiles a CTA; stream-K 127.) */
+int64_t htile_decode_gated_work(int M, int N, int K, int64_t *counts)
 {
+    *counts = 0;
     if (rows_supported(N, K) || N < 16)
         return 0;
     const GatedPlan p(M, N, K);
-    return (int64_t)(p.sums + p.counts);
+    *counts = (int64_t)(p.counts / sizeof(int));
+    return (int64_t)p.sums;
 }
 int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
-                              void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+                              float *sums, int *counts, int M, int N, int K, HtileMode mode, GatedEpilogue ep, cudaStream_t st)
 {
     if (rows_supported(N, K) || N < 16)
-        return launch_rows(hole, plug, am, x, h, kOutGated, M, N, K, mode, st, true, nullptr, false, act);
+        return launch_rows(hole, plug, am, x, h, kOutGated, M, N, K, mode, st, true, nullptr, false, ep);
     GatedPlan p(M, N, K);
     Maps maps;
     if (!decode_maps(maps, hole, plug, am, x, M, N, K, p.MT))
         return kLaunch;
-    p.a.x = x, p.a.y = h, p.a.act = act;
-    p.a.ws = static_cast<float *>(work);
-    p.a.flags = reinterpret_cast<int *>(static_cast<unsigned char *>(work) + p.sums);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1), cfg.blockDim = dim3(256), cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, zero_counts_kernel, p.a.flags, (int)(p.counts / sizeof(int))) != cudaSuccess) {
-        cudaGetLastError();
-        return kLaunch;
-    }
-    return mode == kPrecise ? launch_mt<true, kOutGated>(p.MT, maps, p.a, p.grid, st, true)
-                            : launch_mt<false, kOutGated>(p.MT, maps, p.a, p.grid, st, true);
+    p.a.x = x, p.a.y = h, p.a.ep = ep, p.a.ws = sums, p.a.flags = counts;
+    return mode == kPrecise ? launch_mt<kHiLo, kOutGated>(p.MT, maps, p.a, p.grid, st, true)
+                            : launch_mt<kHalf, kOutGated>(p.MT, maps, p.a, p.grid, st, true);
 }
 
 bool htile_gather_supported(int M, int N) { return M >= 1 && M <= 32 && N >= 1; }
@@ -1646,10 +1645,10 @@ int htile_decode_launch_noalloc(const uint8_t *hole, const uint8_t *plug, const 
         return kLaunch;
     const bool bf = yk == kOutBF16;
     if (mode == kPrecise)
-        return bf ? launch_mt<true, kOutBF16>(MT, maps, a, grid, st, false)
-                  : launch_mt<true, kOutF32>(MT, maps, a, grid, st, false);
-    return bf ? launch_mt<false, kOutBF16>(MT, maps, a, grid, st, false)
-              : launch_mt<false, kOutF32>(MT, maps, a, grid, st, false);
+        return bf ? launch_mt<kHiLo, kOutBF16>(MT, maps, a, grid, st, false)
+                  : launch_mt<kHiLo, kOutF32>(MT, maps, a, grid, st, false);
+    return bf ? launch_mt<kHi, kOutBF16>(MT, maps, a, grid, st, false)
+              : launch_mt<kHi, kOutF32>(MT, maps, a, grid, st, false);
 }
 
 /* This file's kernel error word (bounded waits that ran out); clear resets it. */

@@ -1,0 +1,220 @@
+/* The gated feed-forward projection's entry point: which kernel takes a call, and the pass over x before it.
+ *
+ * In fast mode weights and activations meet the tensor cores in FP16: a weight's rounding to one BF16 value (2^-9
+ * of it) would show in h as much as h's own rounding does (error against 64 bits 0.0027 of h's norm, where
+ * BF16 outputs alone are 0.0017 off), to one FP16 value (2^-12) it does not (0.0017), at the same rate.
+ * FP16's range is what that takes care of: each row of x is multiplied by the power of two that brings its
+ * largest finite value into [2^14, 2^15), exactly: every BF16 value down to 2^-29 of the largest keeps all its bits,
+ * and what lies below is off by 2^-40 of the largest at most.  Where weights carry their absmax into the
+ * products (more than 32 rows), so is each row of W by the one that brings its largest absmax into (1/2, 1].
+ * The epilogues divide by both, again exactly.  The pass is one small kernel (a row of x a CTA; 8191 x 4096: 25 us
+ * of the call's 2.1 ms), and the next kernel's weights stream beside it.
+ */
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "gated.cuh"
+#include "glint_internal.h"
+
+namespace glint {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kHeld = 4; /* 16 bytes a thread that stay in registers: K up to 8192 */
+/* up to so many rows the decode kernels: 32 rows of 2 x 14336 x 4096 take them 59 us, the tcgen05 product 85 */
+constexpr int kDecodeM = 32;
+
+struct PrepArgs {
+    const __nv_bfloat16 *x;
+    __half *x16;
+    float *x_scale;
+    const float *absmax;
+    float *row_scale;
+    int *counts;
+    int M, N, K;
+    int x_ctas, row_ctas, n_counts;
+};
+
+/* largest finite |value| of two BF16, as its bits */
+__device__ __forceinline__ uint32_t top2(uint32_t w, uint32_t top)
+{
+    const uint32_t lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
+    top = lo < 0x7F80u ? max(top, lo) : top;
+    return hi < 0x7F80u ? max(top, hi) : top;
+}
+/* 2^k, k in [-126, 127] */
+__device__ __forceinline__ float power(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+
+__global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)
+{
+    /* the next kernel's weights may stream; it waits for this one before it reads what is written here */
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int cta = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (cta < a.x_ctas) {
+        __shared__ uint32_t tops[kThreads / 32];
+        const uint4 *x = reinterpret_cast<const uint4 *>(a.x + (int64_t)cta * a.K);
+        uint4 *out = reinterpret_cast<uint4 *>(a.x16 + (int64_t)cta * a.K);
+        const int n = a.K / 8;
+        uint4 held[kHeld];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            held[j] = i < n ? x[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            top = top2(held[j].x, top2(held[j].y, top2(held[j].z, top2(held[j].w, top))));
+        for (int i = threadIdx.x + kHeld * kThreads; i < n; i += kThreads) {
+            const uint4 w = x[i];
+            top = top2(w.x, top2(w.y, top2(w.z, top2(w.w, top))));
+        }
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+        if (lane == 0)
+            tops[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i)
+            top = max(top, tops[i]);
+        const int k = min(126, 14 - ((int)(top >> 7) - 127)); /* >= -113 */
+        const float by = power(k);
+        auto pair = [&](uint32_t w) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xFFFF0000u) * by);
+            return *reinterpret_cast<const uint32_t *>(&h);
+        };
+        auto put = [&](int i, uint4 w) { out[i] = make_uint4(pair(w.x), pair(w.y), pair(w.z), pair(w.w)); };
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            if (i < n)
+                put(i, held[j]);
+        }
+        for (int i = threadIdx.x + kHeld * kThreads; i < n; i += kThreads)
+            put(i, x[i]);
+        if (threadIdx.x == 0)
+            a.x_scale[cta] = power(-k);
+    } else if (cta < a.x_ctas + a.row_ctas) {
+        /* a warp a row of W: its largest finite absmax */
+        const int n = (cta - a.x_ctas) * (kThreads / 32) + warp, blocks = a.K / 64;
+        if (n >= a.N)
+            return;
+        uint32_t top = 0;
+        for (int i = lane; i < blocks; i += 32) {
+            const uint32_t v = __float_as_uint(a.absmax[(int64_t)n * blocks + i]) & 0x7FFFFFFFu;
+            top = v < 0x7F800000u ? max(top, v) : top;
+        }
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+        if (lane == 0) /* in [-126, 126], so that its inverse is a normal number too */
+            a.row_scale[n] = power(max(-126, min(126, -((int)(top >> 23) - 127) - 1)));
+    } else {
+        for (int i = threadIdx.x; i < a.n_counts; i += kThreads)
+            a.counts[i] = 0;
+    }
+}
+
+/* kOk, or what glint_htile_gated_stream returns for these arguments before it looks at pointers */
+int check(const GlintHtileGated *a)
+{
+    if (!a || a->M < 0 || a->F < 0 || a->K < 0 || a->F > INT32_MAX / 2 ||
+        (a->mode != GLINT_HTILE_PRECISE && a->mode != GLINT_HTILE_FAST) ||
+        (a->act != GLINT_ACT_SILU && a->act != GLINT_ACT_GELU_TANH))
+        return kBadArg;
+    if (a->blocksize <= 0)
+        return kBadBlocksize;
+    return kOk;
+}
+/* the shapes that the kernels on TMA take, at any M */
+bool streams(const GlintHtileGated &a)
+{
+    return htile_decode_supported(a.hole, a.plug, a.absmax, a.x, std::min(a.M, 32), 2 * a.F, a.K, a.blocksize);
+}
+
+/* what lies where in the workspace */
+struct Layout {
+    bool half = false; /* x in FP16 */
+    int64_t x16 = 0, x_scale = 0, row_scale = 0, sums = 0, counts = 0, n_counts = 0, bytes = 0;
+    explicit Layout(const GlintHtileGated &a)
+    {
+        const int N = 2 * a.F;
+        const bool decode = a.M <= kDecodeM;
+        half = a.mode == GLINT_HTILE_FAST;
+        auto take = [&](int64_t n) {
+            const int64_t at = bytes;
+            bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        if (half) {
+            x16 = take((int64_t)a.M * a.K * 2);
+            x_scale = take(((int64_t)a.M + 255) / 256 * 256 * 4); /* whole tiles of rows are read */
+            if (!decode)
+                row_scale = take((int64_t)N * 4);
+        }
+        const int64_t s = decode ? htile_decode_gated_work(a.M, N, a.K, &n_counts)
+                          : half ? htile_gemm_gated_work(a.M, N, a.K, &n_counts)
+                                 : 0;
+        sums = take(s), counts = take(n_counts * (int64_t)sizeof(int));
+    }
+};
+
+} // namespace
+} // namespace glint
+
+using namespace glint;
+
+int64_t glint_htile_gated_work_bytes(const GlintHtileGated *a)
+{
+    if (check(a) != kOk)
+        return kBadArg;
+    if (a->M == 0 || a->F == 0 || a->K == 0 || !streams(*a))
+        return 0;
+    return Layout(*a).bytes;
+}
+
+int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
+{
+    const int rc = check(a);
+    if (rc != kOk)
+        return rc;
+    if (a->M == 0 || a->F == 0)
+        return kOk;
+    if (!a->h || (a->K && (!a->hole || !a->plug || !a->absmax || !a->x)))
+        return kBadArg;
+    if (a->K == 0)
+        return cudaMemsetAsync(a->h, 0, (size_t)a->M * a->F * 2, stream) == cudaSuccess ? kOk : kLaunch;
+    const int N = 2 * a->F;
+    if (!streams(*a))
+        return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, a->act, stream);
+    const Layout at(*a);
+    if (at.bytes > 0 && (!a->work || !aligned_to(a->work, 16)))
+        return kBadArg;
+    char *work = static_cast<char *>(a->work);
+    const bool decode = a->M <= kDecodeM;
+    float *x_scale = reinterpret_cast<float *>(work + at.x_scale), *row_scale = reinterpret_cast<float *>(work + at.row_scale);
+    int *counts = reinterpret_cast<int *>(work + at.counts);
+    if (at.half || at.n_counts) {
+        PrepArgs p{a->x, reinterpret_cast<__half *>(work + at.x16), x_scale, a->absmax, row_scale, counts, a->M, N, a->K, 0, 0,
+                   (int)at.n_counts};
+        if (at.half)
+            p.x_ctas = a->M, p.row_ctas = decode ? 0 : (N + kThreads / 32 - 1) / (kThreads / 32);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.x_ctas + p.row_ctas + (at.n_counts ? 1 : 0)), cfg.blockDim = dim3(kThreads), cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr, cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, gated_prep_kernel, p) != cudaSuccess) {
+            cudaGetLastError();
+            return kLaunch;
+        }
+    }
+    const HtileMode mode = at.half ? kFast : kPrecise;
+    /* FP16 in BF16's place: the kernels know by the mode */
+    const glint_bf16_t *x = at.half ? reinterpret_cast<const glint_bf16_t *>(work + at.x16) : a->x;
+    const GatedEpilogue ep{a->act, at.half ? x_scale : nullptr, at.half && !decode ? row_scale : nullptr};
+    float *sums = reinterpret_cast<float *>(work + at.sums);
+    return decode ? htile_decode_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream)
+                  : htile_gemm_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream);
+}

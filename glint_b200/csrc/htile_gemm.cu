@@ -48,6 +48,8 @@
 #include <mutex>
 #include <unordered_map>
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "gated.cuh"
 #include "gather.cuh"
@@ -254,9 +256,10 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t sa)
     return (uint64_t)((sa >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-/* instruction descriptor: f32 accumulate, BF16 A and B, both K-major, M=256 (pair), N=256 */
+/* instruction descriptor: f32 accumulate, BF16 or FP16 A and B, both K-major, M=256 (pair), N=256 */
+template <bool F16>
 constexpr uint32_t kIdesc =
-    (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BMX >> 3) << 17) | ((uint32_t)((2 * BN) >> 4) << 24);
+    (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BMX >> 3) << 17) | ((uint32_t)((2 * BN) >> 4) << 24);
 
 __device__ __forceinline__ uint64_t pack2f(float lo, float hi)
 {
@@ -285,7 +288,7 @@ struct GemmArgs {
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
     GatherArgs ga; /* world > 0: y[m, n] goes to every rank's y at [m, ga.n0 + n] (row stride ga.ldy) */
-    int act;       /* gated kernel: of the gate rows */
+    GatedEpilogue ep; /* gated kernel */
 };
 
 /* Work split (stream-K for the first S tiles, then data-parallel rounds): the
@@ -344,19 +347,27 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
     }
 }
 /* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of 16
- * rows.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
+ * rows from m on.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
  * second.  o: 8 outputs, of rows 2i + (n & 1), as BF16 pairs. */
-__device__ __forceinline__ void gated16(const uint32_t (&v)[16], bool up, int act, uint32_t (&o)[4])
+__device__ __forceinline__ void gated16(const uint32_t (&v)[16], bool up, const GatedEpilogue &ep, float row, int m,
+                                        uint32_t (&o)[4])
 {
+    /* what sums of this lane's column (`row`) and of the pair's other one are of their values, with x's part in it */
+    const float mine = row, theirs = __shfl_xor_sync(0xFFFFFFFFu, row, 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float h[2];
+        float4 x = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (ep.x_scale)
+            x = __ldg(reinterpret_cast<const float4 *>(ep.x_scale + m + 4 * i));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t a = v[4 * i + 2 * j], b = v[4 * i + 2 * j + 1];
             const float keep = __uint_as_float(up ? b : a), give = __uint_as_float(up ? a : b);
             const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
-            h[j] = gated_value(up ? got : keep, up ? keep : got, act);
+            const float by = j ? (up ? x.w : x.z) : (up ? x.y : x.x);
+            const float a1 = by * mine * keep, b1 = by * theirs * got;
+            h[j] = gated_value(up ? b1 : a1, up ? a1 : b1, ep.act);
         }
         const __nv_bfloat162 b2 = __floats2bfloat162_rn(h[0], h[1]);
         o[i] = *reinterpret_cast<const uint32_t *>(&b2);
@@ -556,7 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                     const uint32_t wa = tmem + kWCol + (uint32_t)ws.i * (BK / 2);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk)
-                        umma_pair_ts_bf16(tmem + kAccCol, wa + kk * 8, sw128_desc(xs + kk * 32), kIdesc,
+                        umma_pair_ts_bf16(tmem + kAccCol, wa + kk * 8, sw128_desc(xs + kk * 32), kIdesc<GATED>,
                                           (ks > k0 || kk > 0) ? 1u : 0u);
                     umma_commit_pair(&step_done[ws.i]);
                 }
@@ -586,6 +597,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                 ws.i -= WSLOTS, ws.ph ^= 1u;
         };
         for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
+            [[maybe_unused]] float row_scale = 1.f;
+            if constexpr (GATED)
+                row_scale = __ldg(args.ep.row_scale + min((T / args.mtiles) * (2 * BN) + (int)rank * BN + r, args.N - 1));
             for (int ks = ga * PSTEPS + group; ks < gb * PSTEPS && alive; ks += C::kGroups, onward()) {
                 const int j = ks & (PSTEPS - 1);
                 if (j == group && !warp_wait(&p_full[st.i], st.ph, alive))
@@ -611,7 +625,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                 if (!warp_wait(&step_done[ws.i], ws.ph ^ 1u, alive))
                     break;
                 tc_fence_after();
-                const uint64_t sc2 = pack2f(sc, sc);
+                const uint64_t sc2 = GATED ? pack2f(sc * row_scale, sc * row_scale) : pack2f(sc, sc);
                 uint32_t o[kWpt / 2];
 #pragma unroll
                 for (int wq = 0; wq < kWpt / 8; ++wq) {
@@ -626,8 +640,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                         float v0, v1;
                         asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pack2f(c0, c1)), "l"(sc2));
                         asm("mov.b64 {%0, %1}, %2;" : "=f"(v0), "=f"(v1) : "l"(d));
-                        __nv_bfloat162 h2 = __floats2bfloat162_rn(v0, v1);
-                        o[wq * 4 + b] = *reinterpret_cast<uint32_t *>(&h2);
+                        if constexpr (GATED) {
+                            __half2 h2 = __floats2half2_rn(v0, v1);
+                            o[wq * 4 + b] = *reinterpret_cast<uint32_t *>(&h2);
+                        } else {
+                            __nv_bfloat162 h2 = __floats2bfloat162_rn(v0, v1);
+                            o[wq * 4 + b] = *reinterpret_cast<uint32_t *>(&h2);
+                        }
                     }
                 }
                 tmem_st(tw + (uint32_t)ws.i * (BK / 2), o);
@@ -655,6 +674,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             const int m0 = (T % args.mtiles) * BMX, n0 = (T / args.mtiles) * (2 * BN);
             const int n = n0 + (int)rank * BN + q * 32 + (int)lane;
             const int mlim = min(BMX, args.M - m0);
+            [[maybe_unused]] float row_back = 1.f; /* 1 / row_scale[n], a power of two */
+            if constexpr (GATED)
+                row_back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
             const bool whole = ga == 0 && gb == G;
             if (whole) {
                 [[maybe_unused]] uint32_t o[2 * C::kChunks][4];
@@ -666,7 +688,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                         uint32_t v[16];
                         tmem_ld16(tb + c0 * 32 + c * 16, v);
                         tmem_ld_wait(v);
-                        gated16(v, n & 1, args.act, o[c]);
+                        gated16(v, n & 1, args.ep, row_back, m0 + c0 * 32 + c * 16, o[c]);
                     }
                 } else {
 #pragma unroll 1
@@ -760,7 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             u[j] = __float_as_uint(acc[j]);
-                        gated16(u, n & 1, args.act, o);
+                        gated16(u, n & 1, args.ep, row_back, m0 + c * 32 + h * 16, o);
                         store_gated(args.y, args.N, o, m0 + c * 32 + h * 16, mlim - c * 32 - h * 16, n);
                     } else {
 #pragma unroll
@@ -828,7 +850,7 @@ struct PreciseArgs {
     int M, N, K;
     int y_bf16;
     int mtiles, tiles;
-    int act; /* gated kernel: of the gate rows */
+    GatedEpilogue ep; /* gated kernel */
 };
 
 __device__ __forceinline__ uint32_t split_hilo(float c)
@@ -1092,7 +1114,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
 #pragma unroll
                     for (int jj = 0; jj < 16; ++jj)
                         v[jj] = __float_as_uint(run[h * 16 + jj]);
-                    gated16(v, n & 1, args.act, o);
+                    gated16(v, n & 1, args.ep, 1.f, m0 + h * 16, o);
                     store_gated(args.y, args.N, o, m0 + h * 16, jl - h * 16, n);
                 }
                 continue;
@@ -1708,7 +1730,7 @@ int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, 
 
 template <bool GATED>
 int precise_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *y,
-                        bool y_bf16, int M, int N, int K, int act, cudaStream_t st)
+                        bool y_bf16, int M, int N, int K, GatedEpilogue ep, cudaStream_t st)
 {
     Maps maps;
     if (!encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, PBMH,
@@ -1722,7 +1744,7 @@ int precise_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *a
     if (!ensure_smem((const void *)htile_gemm_precise_kernel<GATED>, PSmemBytes))
         return kLaunch;
     PreciseArgs a{};
-    a.y = y, a.am = am, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0, a.act = act;
+    a.y = y, a.am = am, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0, a.ep = ep;
     a.mtiles = (M + PBMX - 1) / PBMX;
     a.tiles = a.mtiles * ((N + 2 * BN - 1) / (2 * BN));
     const int pairs = std::max(1, std::min(a.tiles, max_pairs(1)));
@@ -1753,36 +1775,31 @@ int htile_gemm_gather_launch(const uint8_t *hole, const uint8_t *plug, const flo
 int htile_gemm_precise_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x,
                               void *y, bool y_bf16, int M, int N, int K, cudaStream_t st)
 {
-    return precise_launch_impl<false>(hole, plug, am, x, y, y_bf16, M, N, K, 0, st);
+    return precise_launch_impl<false>(hole, plug, am, x, y, y_bf16, M, N, K, GatedEpilogue{}, st);
 }
 
-/* act(gate) * up of rows 2i and 2i + 1 at any M.  Split tiles' sums and counters are the
- * caller's: work of htile_gemm_gated_work() bytes, the counters zeroed here, call by call. */
-int64_t htile_gemm_gated_work(int M, int N, int K)
+/* act(gate) * up of rows 2i and 2i + 1 at any M.  Split tiles' sums are the caller's, and the counts behind them
+ * are zero when the kernel starts. */
+int64_t htile_gemm_gated_work(int M, int N, int K, int64_t *counts)
 {
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
     const int pairs = gemm_plan(a);
-    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float) + (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int))
-               : 0;
+    *counts = (int64_t)a.S * 2 * GemmCfg<true>::kEpiWarps;
+    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float)) : 0;
 }
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
-                            void *work, int M, int N, int K, HtileMode mode, int act, cudaStream_t st)
+                            float *sums, int *counts, int M, int N, int K, HtileMode mode, GatedEpilogue ep, cudaStream_t st)
 {
     if (mode == kPrecise)
-        return precise_launch_impl<true>(hole, plug, am, x, h, true, M, N, K, act, st);
+        return precise_launch_impl<true>(hole, plug, am, x, h, true, M, N, K, ep, st);
     Maps maps;
     if (!gemm_maps(maps, hole, plug, am, x, M, N, K) || !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
         return kLaunch;
     GemmArgs a{};
-    a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.act = act;
+    a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep;
     const int pairs = gemm_plan(a);
-    if (a.S) {
-        a.ws = static_cast<float *>(work);
-        a.counters = reinterpret_cast<int *>(a.ws + part_floats(pairs));
-        if (cudaMemsetAsync(a.counters, 0, (size_t)a.S * 2 * GemmCfg<true>::kEpiWarps * sizeof(int), st) != cudaSuccess)
-            return kLaunch;
-    }
+    a.ws = sums, a.counters = counts;
     htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }

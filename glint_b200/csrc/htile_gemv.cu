@@ -365,13 +365,13 @@ unsigned generic_grid(int64_t items)
 
 } // namespace
 
-/* act(gate) * up of rows 2i and 2i + 1 for the shapes that the TMA kernels do not take */
+/* act(gate) * up of rows 2i and 2i + 1 for the shapes that the TMA kernels do not take, with both halves of
+ * each cell in either mode */
 int htile_gemv_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
-                            int M, int N, int K, int bs, HtileMode mode, int act, cudaStream_t st)
+                            int M, int N, int K, int bs, int act, cudaStream_t st)
 {
     if (gemv_supported(hole, plug, am, x, N, K, bs))
-        return mode == kPrecise ? launch_gemv_slices<true, kOutGated>(hole, plug, am, x, h, M, N, K, bs, act, st)
-                                : launch_gemv_slices<false, kOutGated>(hole, plug, am, x, h, M, N, K, bs, act, st);
+        return launch_gemv_slices<true, kOutGated>(hole, plug, am, x, h, M, N, K, bs, act, st);
     htile_generic_gated_kernel<<<generic_grid((int64_t)(N / 2) * ((M + 7) / 8)), 256, 0, st>>>(
         hole, plug, am, x, static_cast<__nv_bfloat16 *>(h), M, N / 2, K, bs, act);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
