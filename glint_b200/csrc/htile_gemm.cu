@@ -288,6 +288,7 @@ struct GemmArgs {
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
     GatherArgs ga; /* world > 0: y[m, n] goes to every rank's y at [m, ga.n0 + n] (row stride ga.ldy) */
+    int join;         /* gated: split tiles are added by gated_join_kernel, not by their last contributor */
     GatedEpilogue ep; /* gated kernel */
 };
 
@@ -734,6 +735,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                 mbar_arrive_remote(accempty0); /* accumulator free: the rest works from memory */
             __threadfence();
             __syncwarp();
+            if (GATED && args.join)
+                continue;
             int *cnt = args.counters + ((size_t)T * 2 + rank) * C::kEpiWarps + c0 / C::kChunks * 4 + q;
             const int pf = pair_of(args, T * G, npairs), pl = pair_of(args, (T + 1) * G - 1, npairs);
             int prev = 0;
@@ -804,6 +807,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
+}
+
+/* The split tiles of a gated product with few tiles: a warp takes 32 columns (weight rows) and 16 activation rows of
+ * one tile, adds the contributors' sums in K order and stores the outputs.  The last contributor does not do it there,
+ * because two SMs alone would read all partial sums of a tile: 1771 x 5888 x 2 x 204 (14 tiles on 74 pairs) 53 us that
+ * way, 38 with this kernel, 62 with K uncut. */
+constexpr int kJoinRows = 16;
+__global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int npairs)
+{
+    const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint32_t lane = lane_id();
+    const int part = w % (BMX / kJoinRows), q = w / (BMX / kJoinRows) % 4, rank = w / (BMX / kJoinRows * 4) % 2;
+    const int T = w / (BMX / kJoinRows * 8);
+    if (T >= a.S)
+        return;
+    const int pf = pair_of(a, T * a.G, npairs), pl = pair_of(a, (T + 1) * a.G - 1, npairs);
+    const int m0 = (T % a.mtiles) * BMX + part * kJoinRows, n = (T / a.mtiles) * (2 * BN) + rank * BN + q * 32 + (int)lane;
+    if (pf == pl || m0 >= a.M) /* a tile of one pair is stored; whole warps leave */
+        return;
+    float acc[kJoinRows];
+#pragma unroll
+    for (int j = 0; j < kJoinRows; ++j)
+        acc[j] = 0.f;
+    auto at = [&](int p) {
+        const int slot = unit_begin(a, p, npairs) >= T * a.G ? 0 : 1;
+        return a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
+    };
+    for (int p = pf; p <= pl; ++p) {
+        const float *src = at(p);
+#pragma unroll
+        for (int j = 0; j < kJoinRows; ++j)
+            acc[j] += __ldcg(src + j * 32);
+    }
+    const float back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(a.ep.row_scale + min(n, a.N - 1))));
+    uint32_t v[16], o[4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        v[j] = __float_as_uint(acc[j]);
+    gated16(v, n & 1, a.ep, back, m0, o);
+    store_gated(a.y, a.N, o, m0, a.M - m0, n);
 }
 
 /* ---- precise mode (the reference's f32-class accuracy) on tcgen05 ----------------
@@ -1679,12 +1722,20 @@ namespace {
  * two rounds, the tiles beyond one round (e.g. 512 x 14336: 112 tiles on 74 pairs,
  * 86.8 -> 76.9 us; sharing all tiles instead cost more in split-tile sums than it
  * saved). */
-int gemm_plan(GemmArgs &a)
+int gemm_plan(GemmArgs &a, bool gated = false)
 {
     a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
     a.G = a.K / (PSTEPS * BK);
     const int tiles = a.mtiles * a.ntiles;
     const int maxp = max_pairs();
+    if (gated && tiles * 2 <= maxp) {
+        /* No tile for half of the pairs: K is cut for all tiles, down to one group a pair, and gated_join_kernel adds.
+         * Uncut and cut: 98 x 6656 x 2 x 174 (2 tiles) 63 and 30 us; 64 x 4096 x 2 x 4096 (32 tiles) 45 and 36;
+         * 40 x 1024 x 2 x 2000 (16 tiles, 4 groups) 21.5 and 20.2.  Above half, 250 x 4096 x 2 x 6912 (54 tiles)
+         * 48 and 56, 200 x 2048 x 2 x 5000 (40 tiles) 31 and 34. */
+        a.tiles = a.S = tiles, a.R = 0, a.U = tiles * a.G, a.join = 1;
+        return std::min(maxp, a.U);
+    }
     const int rounds = (tiles + maxp - 1) / maxp;
     const bool idle = (double)(rounds * maxp - tiles) > 0.02 * rounds * maxp;
     const bool split1 = tiles > maxp && tiles < 2 * maxp && idle;
@@ -1784,8 +1835,8 @@ int64_t htile_gemm_gated_work(int M, int N, int K, int64_t *counts)
 {
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
-    const int pairs = gemm_plan(a);
-    *counts = (int64_t)a.S * 2 * GemmCfg<true>::kEpiWarps;
+    const int pairs = gemm_plan(a, true);
+    *counts = a.join ? 0 : (int64_t)a.S * 2 * GemmCfg<true>::kEpiWarps;
     return a.S ? (int64_t)(part_floats(pairs) * sizeof(float)) : 0;
 }
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
@@ -1798,9 +1849,11 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
         return kLaunch;
     GemmArgs a{};
     a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep;
-    const int pairs = gemm_plan(a);
+    const int pairs = gemm_plan(a, true);
     a.ws = sums, a.counters = counts;
     htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
+    if (a.join)
+        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a, pairs);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
