@@ -1,21 +1,24 @@
-"""A decoder's attention layer served from GLINT planes and a 4-bit cache.
+"""A decoder's layer served from GLINT planes and a 4-bit cache.
 
     python examples/attention_layer.py [--budget 512] [--steps 64]
 
 What runs, all of it on this library's kernels: the q|k|v linear (device.htile) on packed
-prompts, attention over them (attn_prompt), their keys and values into a paged 4-bit
-cache (kv4_append); the cache's weights seeded by the last tokens of each prompt
-(kv4_attn with several rows) and the cache cut to a budget (kv4_evict); then tokens one
-at a time: q|k|v, append, attention with running weights, eviction every few steps,
-and the o linear.  Random weights; sizes of one Llama-3-8B layer.  Rotary embedding and
-the rest of a model are the caller's: `rope(q, k, positions)` is applied to the views.
+prompts, their queries and keys rotated and keys and values put into a paged 4-bit
+cache (rope_append), attention over them (attn_prompt); the cache's weights seeded by
+the last tokens of each prompt (kv4_attn with several rows) and the cache cut to a budget
+(kv4_evict); then tokens one at a time: q|k|v, rotation and append, attention with
+running weights, eviction every few steps, and the o linear.  After attention the
+feed-forward: gate and up with their activation in one product (device.htile_gated), and
+the down linear.  Random weights; sizes of one Llama-3-8B layer.  A rotary embedding of
+another kind is the caller's: `rope(q, k, positions)` is applied to the views, and the
+keys are appended as it gives them (kv4_append).
 """
 from __future__ import annotations
 
 import argparse
 import sys
 from pathlib import Path
-from typing import Callable, List, Optional
+from typing import Callable, List, Optional, Tuple
 
 import torch
 
@@ -31,12 +34,15 @@ class AttentionLayer:
     [hidden, heads * head_dim] weights.  Each sequence may hold `capacity` slots; beyond
     `budget` (plus `slack`, so that eviction runs once in `slack` steps) the slots of
     least weight go, the `recent` newest tokens excepted.  A call that would take a sequence
-    past its slots raises ValueError."""
+    past its slots raises ValueError.  freqs: what attn.rope_freqs returns, for queries and
+    keys rotated by their positions; or rope, a function of the caller's; or neither."""
 
     def __init__(self, wqkv, wo, hidden: int, heads: int, kv_heads: int, head_dim: int, seqs: int, capacity: int,
                  budget: int, recent: int, slack: int = 16, window: int = 8, page_size: int = 64,
-                 rope: Optional[Callable] = None):
-        self.wqkv, self.wo, self.hidden, self.heads, self.rope = wqkv, wo, hidden, heads, rope
+                 rope: Optional[Callable] = None, freqs: Optional[Tuple[torch.Tensor, float]] = None):
+        if rope and freqs:
+            raise ValueError("rope or freqs, not both")
+        self.wqkv, self.wo, self.hidden, self.heads, self.rope, self.freqs = wqkv, wo, hidden, heads, rope, freqs
         self.kv_heads, self.head_dim, self.budget, self.recent = kv_heads, head_dim, budget, recent
         self.slack, self.window = slack, window
         per = -(-capacity // page_size)
@@ -50,12 +56,20 @@ class AttentionLayer:
         self.pos = [torch.zeros(seqs, kv_heads, per * page_size, dtype=torch.int32, device="cuda") for _ in range(2)]
         self.longest = 0  # an upper bound of lens, kept on the host
 
-    def _qkv(self, x: torch.Tensor, positions: torch.Tensor):
+    def _qkv(self, x: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor):
+        """q, k (both rotated) and v of x's tokens, and k and v in the cache."""
         n = (self.heads + 2 * self.kv_heads) * self.head_dim
         y = device.htile(x, *self.wqkv, n, mode="fast", out_dtype=torch.bfloat16)
         y = y.view(x.shape[0], self.heads + 2 * self.kv_heads, self.head_dim)
         q, k, v = y.split([self.heads, self.kv_heads, self.kv_heads], 1)  # views: no copy
-        return (*self.rope(q, k, positions), v) if self.rope else (q, k, v)
+        if self.freqs:  # in place, in y
+            inv_freq, scale = self.freqs
+            attn.rope_append(self.cache, q, k, v, positions.to(torch.int32), inv_freq, slots, scale=scale, q_out=q, k_out=k)
+        else:
+            if self.rope:
+                q, k = self.rope(q, k, positions)
+            attn.kv4_append(self.cache, k, v, slots)
+        return q, k, v
 
     def _o(self, o: torch.Tensor) -> torch.Tensor:
         o = o.reshape(-1, self.heads * self.head_dim)
@@ -80,9 +94,8 @@ class AttentionLayer:
         ends[1:] = n.cumsum(0)
         seq = torch.arange(len(lens), device="cuda").repeat_interleave(n)
         at = torch.arange(x.shape[0], device="cuda") - ends[seq]
-        q, k, v = self._qkv(x, at)
+        q, k, v = self._qkv(x, at, self._slots(seq, at))
         o, _ = attn.attn_prompt(q, k, v, ends)
-        attn.kv4_append(self.cache, k, v, self._slots(seq, at))
         self.lens.copy_(n)
         self.seen.copy_(n)
         self.longest = max(lens)
@@ -102,9 +115,8 @@ class AttentionLayer:
         if seqs != self.table.shape[0]:
             raise ValueError(f"a token of each of {self.table.shape[0]} sequences, not {seqs}")
         self._room(self.longest + 1)
-        q, k, v = self._qkv(x, self.seen)
         seq = torch.arange(seqs, device="cuda")
-        attn.kv4_append(self.cache, k, v, self._slots(seq, self.lens))
+        q, _, _ = self._qkv(x, self.seen, self._slots(seq, self.lens))
         self.pos[0][seq, :, self.lens.long()] = self.seen[:, None]
         self.lens += 1
         self.seen += 1
@@ -124,6 +136,37 @@ class AttentionLayer:
         self.longest = self.budget
 
 
+class FeedForward:
+    """down(act(gate(x)) * up(x)); gate, up: planes of [ff, hidden] weights, down: of [hidden, ff]."""
+
+    def __init__(self, gate, up, down, hidden: int, ff: int, act: str = "silu"):
+        self.gated, self.down = device.pack_gated(gate, up, ff, hidden), down  # laid out once
+        self.hidden, self.ff, self.act = hidden, ff, act
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        h = device.htile_gated(x, *self.gated, self.ff, mode="fast", act=self.act)
+        return device.htile(h, *self.down, self.hidden, mode="fast", out_dtype=torch.bfloat16)
+
+
+class DecoderLayer:
+    """x + attention(norm(x)), then x + feed_forward(norm(x))."""
+
+    def __init__(self, attention: AttentionLayer, feed_forward: FeedForward, eps: float = 1e-5):
+        self.attention, self.feed_forward, self.eps = attention, feed_forward, eps
+        self.norms = [torch.ones(attention.hidden, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+
+    def _norm(self, x: torch.Tensor, i: int) -> torch.Tensor:
+        return torch.nn.functional.rms_norm(x, x.shape[-1:], self.norms[i], self.eps)
+
+    def prompt(self, x: torch.Tensor, lens: List[int]) -> torch.Tensor:
+        x = x + self.attention.prompt(self._norm(x, 0), lens)
+        return x + self.feed_forward(self._norm(x, 1))
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        x = x + self.attention.step(self._norm(x, 0))
+        return x + self.feed_forward(self._norm(x, 1))
+
+
 def random_planes(n: int, k: int, g: torch.Generator):
     w = (torch.randn(n, k, device="cuda", generator=g) * k ** -0.5).bfloat16()
     return device.encode(w)
@@ -134,13 +177,16 @@ def main() -> None:
     p.add_argument("--budget", type=int, default=512)
     p.add_argument("--steps", type=int, default=64)
     args = p.parse_args()
-    hidden, heads, kv, dim = 4096, 32, 8, 128
+    hidden, heads, kv, dim, ff = 4096, 32, 8, 128, 14336
     lens = [700, 1, 33, 1500, 260]
     g = torch.Generator(device="cuda").manual_seed(0)
-    layer = AttentionLayer(random_planes((heads + 2 * kv) * dim, hidden, g), random_planes(hidden, heads * dim, g),
-                           hidden, heads, kv, dim, len(lens), max(lens) + args.steps, args.budget, args.budget // 8)
+    attention = AttentionLayer(random_planes((heads + 2 * kv) * dim, hidden, g), random_planes(hidden, heads * dim, g),
+                               hidden, heads, kv, dim, len(lens), max(lens) + args.steps, args.budget, args.budget // 8,
+                               freqs=attn.rope_freqs(dim, 500000.0))
+    layer = DecoderLayer(attention, FeedForward(random_planes(ff, hidden, g), random_planes(ff, hidden, g),
+                                                random_planes(hidden, ff, g), hidden, ff))
     y = layer.prompt(torch.randn(sum(lens), hidden, device="cuda", generator=g).bfloat16(), lens)
-    print(f"prompts of {lens} tokens -> {tuple(y.shape)}; slots held {layer.lens.tolist()}")
+    print(f"prompts of {lens} tokens -> {tuple(y.shape)}; slots held {attention.lens.tolist()}")
     x = torch.randn(len(lens), hidden, device="cuda", generator=g).bfloat16()
     begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     begin.record()
@@ -150,7 +196,7 @@ def main() -> None:
     end.synchronize()
     bits = 4 + 32 / attn.BLOCK
     print(f"{args.steps} steps, {begin.elapsed_time(end) / args.steps * 1e3:.0f} us each; slots held "
-          f"{layer.lens.tolist()} of {layer.seen.tolist()} tokens seen, {bits} bits a value; "
+          f"{attention.lens.tolist()} of {attention.seen.tolist()} tokens seen, {bits} bits a value; "
           f"output finite: {bool(x.isfinite().all())}")
 
 
