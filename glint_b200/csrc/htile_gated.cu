@@ -17,6 +17,7 @@
 #include "common.cuh"
 #include "gated.cuh"
 #include "glint_internal.h"
+#include "ptx.cuh"
 
 namespace glint {
 namespace {
@@ -46,6 +47,18 @@ __device__ __forceinline__ uint32_t top2(uint32_t w, uint32_t top)
 }
 /* 2^k, k in [-126, 127] */
 __device__ __forceinline__ float power(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+
+__device__ __forceinline__ uint32_t finite_bits(float v)
+{
+    const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+    return b < 0x7F800000u ? b : 0u;
+}
+/* the power of two that brings a row of W whose largest absmax has these bits into (1/2, 1]; in [2^-126, 2^126], so
+ * that its inverse is a normal number too */
+__device__ __forceinline__ float row_power(uint32_t top)
+{
+    return power(max(-126, min(126, -((int)(top >> 23) - 127) - 1)));
+}
 
 __global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)
 {
@@ -102,16 +115,72 @@ __global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)
         if (n >= a.N)
             return;
         uint32_t top = 0;
-        for (int i = lane; i < blocks; i += 32) {
-            const uint32_t v = __float_as_uint(a.absmax[(int64_t)n * blocks + i]) & 0x7FFFFFFFu;
-            top = v < 0x7F800000u ? max(top, v) : top;
-        }
+        for (int i = lane; i < blocks; i += 32)
+            top = max(top, finite_bits(a.absmax[(int64_t)n * blocks + i]));
         top = __reduce_max_sync(0xFFFFFFFFu, top);
-        if (lane == 0) /* in [-126, 126], so that its inverse is a normal number too */
-            a.row_scale[n] = power(max(-126, min(126, -((int)(top >> 23) - 127) - 1)));
+        if (lane == 0)
+            a.row_scale[n] = row_power(top);
     } else {
         for (int i = threadIdx.x; i < a.n_counts; i += kThreads)
             a.counts[i] = 0;
+    }
+}
+
+/* W in FP16, its rows multiplied by their powers of two, for calls of many rows: a warp a row of W, which first takes
+ * the row's largest absmax; the codebook lies in shared memory once for each lane, so a lookup meets no conflict and
+ * its address is one byte permute. */
+constexpr int kExpandThreads = 512, kExpandCtas = 3 /* an SM */, kExpandAtOnce = 4, kLutBytes = 256 * 256;
+__global__ void __launch_bounds__(kExpandThreads, kExpandCtas)
+    gated_expand_kernel(const uint8_t *hole, const uint8_t *plug, const float *absmax, uint4 *out, float *row_scale, int N, int K)
+{
+    extern __shared__ __align__(16) float lut[];
+    for (int i = threadIdx.x; i < 256 * 32; i += kExpandThreads)
+        lut[(i >> 5) * 64 + (i & 31)] = (&g_cells[0][0])[i >> 5];
+    __syncthreads();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, blocks = K / 64, words = K / 8;
+    const uint32_t base = saddr(lut), lane4 = (uint32_t)lane * 4u;
+    for (int n = blockIdx.x * (kExpandThreads / 32) + warp; n < N; n += gridDim.x * (kExpandThreads / 32)) {
+        const uint32_t *H = reinterpret_cast<const uint32_t *>(hole) + (int64_t)n * words;
+        const uint32_t *P = reinterpret_cast<const uint32_t *>(plug) + (int64_t)n * words;
+        const float *am = absmax + (int64_t)n * blocks;
+        uint4 *o = out + (int64_t)n * words;
+        uint32_t h[kExpandAtOnce], p[kExpandAtOnce];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kExpandAtOnce; ++j) {
+                const int i = min(i0 + j * 32, words - 1);
+                h[j] = __ldcs(H + i), p[j] = __ldcs(P + i);
+            }
+        };
+        load(lane);
+        uint32_t top = 0;
+        for (int i = lane; i < blocks; i += 32)
+            top = max(top, finite_bits(__ldg(am + i)));
+        const float scale = row_power(__reduce_max_sync(0xFFFFFFFFu, top));
+        if (lane == 0)
+            row_scale[n] = scale;
+        for (int i0 = lane; i0 < words; i0 += kExpandAtOnce * 32) {
+            if (i0 != lane)
+                load(i0);
+#pragma unroll
+            for (int j = 0; j < kExpandAtOnce; ++j) {
+                const int i = i0 + j * 32;
+                if (i >= words)
+                    break;
+                const float s = __ldg(am + i / 8) * scale;
+                const uint32_t E = ((h[j] << 4) & 0xF0F0F0F0u) | (p[j] & 0x0F0F0F0Fu);
+                const uint32_t O = (h[j] & 0xF0F0F0F0u) | ((p[j] >> 4) & 0x0F0F0F0Fu);
+                uint32_t w[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float c0 = __uint_as_float(lds32(base + __byte_perm(E, lane4, 0x5504u | (b << 4))));
+                    const float c1 = __uint_as_float(lds32(base + __byte_perm(O, lane4, 0x5504u | (b << 4))));
+                    const __half2 v = __floats2half2_rn(c0 * s, c1 * s);
+                    w[b] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+                o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
     }
 }
 
@@ -135,12 +204,14 @@ bool streams(const GlintHtileGated &a)
 /* what lies where in the workspace */
 struct Layout {
     bool half = false; /* x in FP16 */
-    int64_t x16 = 0, x_scale = 0, row_scale = 0, sums = 0, counts = 0, n_counts = 0, bytes = 0;
+    bool wide = false; /* W in FP16 */
+    int64_t x16 = 0, w16 = 0, x_scale = 0, row_scale = 0, sums = 0, counts = 0, n_counts = 0, bytes = 0;
     explicit Layout(const GlintHtileGated &a)
     {
         const int N = 2 * a.F;
         const bool decode = a.M <= kDecodeM;
         half = a.mode == GLINT_HTILE_FAST;
+        wide = half && htile_gated_wide_takes(a.M, N, a.K);
         auto take = [&](int64_t n) {
             const int64_t at = bytes;
             bytes += (n + 255) / 256 * 256;
@@ -151,8 +222,11 @@ struct Layout {
             x_scale = take(((int64_t)a.M + 255) / 256 * 256 * 4); /* whole tiles of rows are read */
             if (!decode)
                 row_scale = take((int64_t)N * 4);
+            if (wide)
+                w16 = take((int64_t)N * a.K * 2);
         }
         const int64_t s = decode ? htile_decode_gated_work(a.M, N, a.K, &n_counts)
+                          : wide ? htile_gated_wide_work(a.M, N, a.K)
                           : half ? htile_gemm_gated_work(a.M, N, a.K, &n_counts)
                                  : 0;
         sums = take(s), counts = take(n_counts * (int64_t)sizeof(int));
@@ -198,7 +272,7 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
         PrepArgs p{a->x, reinterpret_cast<__half *>(work + at.x16), x_scale, a->absmax, row_scale, counts, a->M, N, a->K, 0, 0,
                    (int)at.n_counts};
         if (at.half)
-            p.x_ctas = a->M, p.row_ctas = decode ? 0 : (N + kThreads / 32 - 1) / (kThreads / 32);
+            p.x_ctas = a->M, p.row_ctas = decode || at.wide ? 0 : (N + kThreads / 32 - 1) / (kThreads / 32);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(p.x_ctas + p.row_ctas + (at.n_counts ? 1 : 0)), cfg.blockDim = dim3(kThreads), cfg.stream = stream;
         cudaLaunchAttribute attr[1];
@@ -215,6 +289,16 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
     const glint_bf16_t *x = at.half ? reinterpret_cast<const glint_bf16_t *>(work + at.x16) : a->x;
     const GatedEpilogue ep{a->act, at.half ? x_scale : nullptr, at.half && !decode ? row_scale : nullptr};
     float *sums = reinterpret_cast<float *>(work + at.sums);
+    if (at.wide) {
+        if (!ensure_smem((const void *)gated_expand_kernel, kLutBytes))
+            return kLaunch;
+        const int ctas = std::min(kExpandCtas * sm_count(), (N + kExpandThreads / 32 - 1) / (kExpandThreads / 32));
+        gated_expand_kernel<<<ctas, kExpandThreads, kLutBytes, stream>>>(a->hole, a->plug, a->absmax,
+                                                                         reinterpret_cast<uint4 *>(work + at.w16), row_scale, N, a->K);
+        if (cudaGetLastError() != cudaSuccess)
+            return kLaunch;
+        return htile_gated_wide_launch(work + at.w16, x, a->h, sums, a->M, N, a->K, ep, stream);
+    }
     return decode ? htile_decode_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream)
                   : htile_gemm_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream);
 }

@@ -182,6 +182,13 @@ __device__ __forceinline__ void umma_pair_ts_bf16(uint32_t d, uint32_t a, uint64
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
                  "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
+/* the same with A from shared memory */
+__device__ __forceinline__ void umma_pair_ss_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
 /* arrive on the mbarrier at `cluster_addr` once this thread's UMMAs are done */
 __device__ __forceinline__ void umma_commit_to(uint32_t cluster_addr)
 {
@@ -288,6 +295,7 @@ struct GemmArgs {
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
     GatherArgs ga; /* world > 0: y[m, n] goes to every rank's y at [m, ga.n0 + n] (row stride ga.ldy) */
+    int group;        /* gated: tiles of so many rows' tiles in turn, see tile_at */
     int join;         /* gated: split tiles are added by gated_join_kernel, not by their last contributor */
     GatedEpilogue ep; /* gated kernel */
 };
@@ -327,6 +335,15 @@ struct Segments {
 struct Maps {
     CUtensorMap x, h, p, am;
 };
+
+/* First row and column of tile T where tiles run through `group` row tiles at a time, all columns of them: what runs
+ * at once then shares its weights and its activations (group = mtiles: all rows first). */
+__device__ __forceinline__ void tile_at(const GemmArgs &a, int T, int &m0, int &n0)
+{
+    const int g = T / (a.group * a.ntiles), first = g * a.group, in = T - first * a.ntiles;
+    const int rows = min(a.group, a.mtiles - first);
+    m0 = (first + in % rows) * BMX, n0 = in / rows * (2 * BN);
+}
 
 /* rows m0 .. m0+jl-1 of a row-major y (row stride `step`) at column n from 32
  * accumulator values (f32 bits) */
@@ -823,7 +840,9 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int n
     if (T >= a.S)
         return;
     const int pf = pair_of(a, T * a.G, npairs), pl = pair_of(a, (T + 1) * a.G - 1, npairs);
-    const int m0 = (T % a.mtiles) * BMX + part * kJoinRows, n = (T / a.mtiles) * (2 * BN) + rank * BN + q * 32 + (int)lane;
+    int m0, n;
+    tile_at(a, T, m0, n);
+    m0 += part * kJoinRows, n += rank * BN + q * 32 + (int)lane;
     if (pf == pl || m0 >= a.M) /* a tile of one pair is stored; whole warps leave */
         return;
     float acc[kJoinRows];
@@ -847,6 +866,177 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int n
         v[j] = __float_as_uint(acc[j]);
     gated16(v, n & 1, a.ep, back, m0, o);
     store_gated(a.y, a.N, o, m0, a.M - m0, n);
+}
+
+/* ---- gated product of many rows, weights expanded before ------------------------- */
+constexpr int WDSTAGES = 6;                    /* shared-memory ring: 128 activation rows and 128 weight rows of a K step */
+constexpr int kWideStage = 2 * kStageX;        /* 32 KB */
+constexpr int kWideEpi0 = 2, kWideEpiWarps = 8; /* two warps a quadrant, half of the columns each */
+constexpr int kWideThreads = (kWideEpi0 + kWideEpiWarps) * 32;
+constexpr int kWideSmem = 1024 + WDSTAGES * kWideStage + 256;
+
+constexpr int kWideGroup = 8; /* row tiles that run at once */
+
+struct WideMaps {
+    CUtensorMap x, w;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
+    gated_wide_kernel(const __grid_constant__ WideMaps maps, const GemmArgs args)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(ring + WDSTAGES * kWideStage); /* leader: both CTAs' tiles landed */
+    uint64_t *empty = full + WDSTAGES;    /* read by the pair's UMMAs */
+    uint64_t *acc_full = empty + WDSTAGES; /* [2] */
+    uint64_t *acc_empty = acc_full + 2;   /* [2] leader: both CTAs' epilogues drained */
+    uint64_t *mma_done = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const uint32_t lane = lane_id();
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    const int G = args.G;
+    const int ub = unit_begin(args, pair, npairs), ue = unit_begin(args, pair + 1, npairs);
+    const Segments seg0{0, ub, ue};
+    int T, ga, gb;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < WDSTAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&acc_full[s], 1);
+            mbar_init(&acc_empty[s], 2 * kWideEpiWarps);
+        }
+        mbar_init(mma_done, 1);
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(tmem_slot)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync(); /* both CTAs' barriers initialised and TMEM allocated */
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool alive = true;
+
+    if (warp == 0) {
+        /* ---- producer (both CTAs): this CTA's activation and weight rows */
+        if (lane == 0) {
+            Ring st;
+            int64_t issued = 0;
+            for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
+                int m0, n0;
+                tile_at(args, T, m0, n0);
+                m0 += (int)rank * BMH, n0 += (int)rank * BN;
+                for (int ks = ga * PSTEPS; ks < gb * PSTEPS; ++ks, st.next<WDSTAGES>()) {
+                    if (!wait_or_fail(&empty[st.i], st.ph ^ 1u, alive))
+                        break;
+                    if (leader)
+                        mbar_expect_tx(&full[st.i], 2 * kWideStage);
+                    const uint32_t fb = peer_addr(saddr(&full[st.i]), 0);
+                    uint8_t *sb = ring + st.i * kWideStage;
+                    tma_load_2d_pair(sb, &maps.x, fb, ks * BK, m0);
+                    tma_load_2d_pair(sb + kStageX, &maps.w, fb, ks * BK, n0);
+                    ++issued;
+                }
+            }
+            if (!alive && leader) {
+                /* let the loads already issued land before the CTA exits */
+                bool drain = true;
+                for (int64_t j = issued > WDSTAGES ? issued - WDSTAGES : 0; j < issued && drain; ++j)
+                    drain = mbar_wait_bounded(&full[(int)(j % WDSTAGES)], (uint32_t)(j / WDSTAGES) & 1u, &g_glint_kernel_error);
+            }
+        }
+    } else if (warp == 1) {
+        /* ---- UMMA issuer (leader CTA only) */
+        if (leader && lane == 0) {
+            Ring st, acc;
+            for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb); acc.next<2>()) {
+                /* the first use of each accumulator waits on parity 1: returns at once */
+                if (!wait_or_fail(&acc_empty[acc.i], acc.ph ^ 1u, alive))
+                    break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(acc.i * BMX);
+                const int k0 = ga * PSTEPS;
+                for (int ks = k0; ks < gb * PSTEPS; ++ks, st.next<WDSTAGES>()) {
+                    if (!wait_or_fail(&full[st.i], st.ph, alive))
+                        break;
+                    tc_fence_after();
+                    const uint32_t xs = saddr(ring + st.i * kWideStage);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; ++kk)
+                        umma_pair_ss_f16(d, sw128_desc(xs + kStageX + kk * 32), sw128_desc(xs + kk * 32), kIdesc<true>,
+                                         (ks > k0 || kk > 0) ? 1u : 0u);
+                    umma_commit_pair(&empty[st.i]);
+                }
+                if (alive)
+                    umma_commit_pair(&acc_full[acc.i]);
+            }
+            /* all UMMAs issued by this thread have completed before TMEM is released */
+            umma_commit_to(peer_addr(saddr(mma_done), 0));
+            mbar_wait_bounded(mma_done, 0, &g_glint_kernel_error);
+        }
+        __syncwarp();
+    } else {
+        /* ---- epilogue: warp w reads TMEM lanes 32*(w%4), weight rows n, of half of the columns, activation rows m */
+        const int q = warp & 3, c0 = (warp - kWideEpi0) / 4 * (BMX / 2);
+        const uint32_t ae0 = peer_addr(saddr(&acc_empty[0]), 0);
+        const uint32_t tb = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
+        Ring acc;
+        for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb); acc.next<2>()) {
+            int m0, n;
+            tile_at(args, T, m0, n);
+            m0 += c0, n += (int)rank * BN + q * 32 + (int)lane;
+            const int mlim = args.M - m0;
+            /* 1 / row_scale[n], a power of two */
+            const float back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
+            if (!warp_wait(&acc_full[acc.i], acc.ph, alive))
+                break;
+            tc_fence_after();
+            const uint32_t ta = tb + (uint32_t)(acc.i * BMX);
+            if (ga == 0 && gb == G) {
+#pragma unroll 1
+                for (int c = 0; c < BMX / 2 && c < mlim; c += 16) {
+                    uint32_t v[16], o[4];
+                    tmem_ld16(ta + c, v);
+                    tmem_ld_wait(v);
+                    gated16(v, n & 1, args.ep, back, m0 + c, o);
+                    store_gated(args.y, args.N, o, m0 + c, mlim - c, n);
+                }
+            } else { /* gated_join_kernel adds; slot 0: the first segment of this pair's range, slot 1: its last */
+                const int slot = ub >= T * G ? 0 : 1;
+                float *mine = args.ws + ((((size_t)pair * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + c0 * 32 + lane;
+#pragma unroll 1
+                for (int c = 0; c < BMX / 2 && c < mlim; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(ta + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        __stcg(mine + (c + j) * 32, __uint_as_float(v[j]));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive_remote(ae0 + (uint32_t)acc.i * 8u);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); /* the peer no longer reads this CTA's TMEM or shared memory */
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
 }
 
 /* ---- precise mode (the reference's f32-class accuracy) on tcgen05 ----------------
@@ -1725,7 +1915,7 @@ namespace {
 int gemm_plan(GemmArgs &a, bool gated = false)
 {
     a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
-    a.G = a.K / (PSTEPS * BK);
+    a.G = a.K / (PSTEPS * BK), a.group = a.mtiles;
     const int tiles = a.mtiles * a.ntiles;
     const int maxp = max_pairs();
     if (gated && tiles * 2 <= maxp) {
@@ -1745,6 +1935,18 @@ int gemm_plan(GemmArgs &a, bool gated = false)
     a.R = split ? (split1 ? 1 : tiles / pairs - 1) : (tiles + pairs - 1) / pairs;
     a.S = split ? tiles - a.R * pairs : 0;
     a.U = a.S * a.G;
+    return pairs;
+}
+/* the same for gated_wide_kernel: the tiles beyond whole rounds are cut, if more than 2% of the time would be idle */
+int wide_plan(GemmArgs &a)
+{
+    a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
+    a.G = a.K / (PSTEPS * BK), a.group = std::min(a.mtiles, kWideGroup);
+    a.tiles = a.mtiles * a.ntiles;
+    const int pairs = std::min(a.tiles, max_pairs()), left = a.tiles % pairs;
+    const bool cut = left && (pairs - left) * 50 > a.tiles;
+    a.S = cut ? left : 0, a.U = a.S * a.G, a.join = cut;
+    a.R = cut ? a.tiles / pairs : (a.tiles + pairs - 1) / pairs;
     return pairs;
 }
 size_t part_floats(int pairs) { return (size_t)pairs * 2 * 2 * 4 * kPartFloats; }
@@ -1852,6 +2054,37 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     const int pairs = gemm_plan(a, true);
     a.ws = sums, a.counters = counts;
     htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
+    if (a.join)
+        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a, pairs);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
+}
+
+/* The same from expanded weights: w FP16 [N, K], the rows multiplied by ep.row_scale. */
+bool htile_gated_wide_takes(int M, int N, int K)
+{
+    return M >= 1024 && (int64_t)((M + BMX - 1) / BMX) * ((N + 2 * BN - 1) / (2 * BN)) >= max_pairs();
+}
+int64_t htile_gated_wide_work(int M, int N, int K)
+{
+    GemmArgs a{};
+    a.M = M, a.N = N, a.K = K;
+    const int pairs = wide_plan(a);
+    return a.S ? (int64_t)(part_floats(pairs) * sizeof(float)) : 0;
+}
+int htile_gated_wide_launch(const void *w, const void *x, void *h, float *sums, int M, int N, int K, GatedEpilogue ep,
+                            cudaStream_t st)
+{
+    WideMaps maps;
+    if (!encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, BMH,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, w, (uint64_t)K, (uint64_t)N, (uint64_t)K * 2, BK, BN,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !ensure_smem((const void *)gated_wide_kernel, kWideSmem))
+        return kLaunch;
+    GemmArgs a{};
+    a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep, a.ws = sums;
+    const int pairs = wide_plan(a);
+    gated_wide_kernel<<<2 * pairs, kWideThreads, kWideSmem, st>>>(maps, a);
     if (a.join)
         gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a, pairs);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
