@@ -364,16 +364,17 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
                 *yp = __uint_as_float(v[j]);
     }
 }
-/* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of 16
+/* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of R
  * rows from m on.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
- * second.  o: 8 outputs, of rows 2i + (n & 1), as BF16 pairs. */
-__device__ __forceinline__ void gated16(const uint32_t (&v)[16], bool up, const GatedEpilogue &ep, float row, int m,
-                                        uint32_t (&o)[4])
+ * second.  o: R / 2 outputs, of rows 2i + (n & 1), as BF16 pairs. */
+template <int R>
+__device__ __forceinline__ void gated_outputs(const uint32_t (&v)[R], bool up, const GatedEpilogue &ep, float row, int m,
+                                              uint32_t (&o)[R / 4])
 {
     /* what sums of this lane's column (`row`) and of the pair's other one are of their values, with x's part in it */
     const float mine = row, theirs = __shfl_xor_sync(0xFFFFFFFFu, row, 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R / 4; ++i) {
         float h[2];
         float4 x = make_float4(1.f, 1.f, 1.f, 1.f);
         if (ep.x_scale)
@@ -392,14 +393,15 @@ __device__ __forceinline__ void gated16(const uint32_t (&v)[16], bool up, const 
     }
 }
 /* them into column n / 2 of h [.., n_cols / 2], rows m0 .. m0+jl-1 */
-__device__ __forceinline__ void store_gated(void *h, int n_cols, const uint32_t (&o)[4], int m0, int jl, int n)
+template <int R4>
+__device__ __forceinline__ void store_gated(void *h, int n_cols, const uint32_t (&o)[R4], int m0, int jl, int n)
 {
     if (n >= n_cols)
         return;
     const size_t ld = (size_t)(n_cols / 2);
     __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(h) + (size_t)(m0 + (n & 1)) * ld + n / 2;
 #pragma unroll
-    for (int j = 0; j < 8; ++j, p += 2 * ld)
+    for (int j = 0; j < 2 * R4; ++j, p += 2 * ld)
         if (2 * j + (n & 1) < jl)
             *p = __ushort_as_bfloat16((unsigned short)(o[j / 2] >> (16 * (j & 1))));
 }
@@ -706,7 +708,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                         uint32_t v[16];
                         tmem_ld16(tb + c0 * 32 + c * 16, v);
                         tmem_ld_wait(v);
-                        gated16(v, n & 1, args.ep, row_back, m0 + c0 * 32 + c * 16, o[c]);
+                        gated_outputs(v, n & 1, args.ep, row_back, m0 + c0 * 32 + c * 16, o[c]);
                     }
                 } else {
 #pragma unroll 1
@@ -802,7 +804,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             u[j] = __float_as_uint(acc[j]);
-                        gated16(u, n & 1, args.ep, row_back, m0 + c * 32 + h * 16, o);
+                        gated_outputs(u, n & 1, args.ep, row_back, m0 + c * 32 + h * 16, o);
                         store_gated(args.y, args.N, o, m0 + c * 32 + h * 16, mlim - c * 32 - h * 16, n);
                     } else {
 #pragma unroll
@@ -826,11 +828,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
     }
 }
 
-/* The split tiles of a gated product with few tiles: a warp takes 32 columns (weight rows) and 16 activation rows of
- * one tile, adds the contributors' sums in K order and stores the outputs.  The last contributor does not do it there,
- * because two SMs alone would read all partial sums of a tile: 1771 x 5888 x 2 x 204 (14 tiles on 74 pairs) 53 us that
- * way, 38 with this kernel, 62 with K uncut. */
-constexpr int kJoinRows = 16;
+/* The split tiles of a gated product: a warp takes 32 columns (weight rows) and 4 activation rows of one tile, adds
+ * the contributors' sums in K order, four at a time, and stores the outputs.  The last contributor does not do it in
+ * the product's kernel, because two SMs alone would read all partial sums of a tile: 1771 x 5888 x 2 x 204 (14
+ * tiles on 74 pairs) 53 us that way, JOIN with this kernel, 62 with K uncut. */
+constexpr int kJoinRows = 4, kJoinAtOnce = 4;
 __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int npairs)
 {
     const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -849,22 +851,30 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int n
 #pragma unroll
     for (int j = 0; j < kJoinRows; ++j)
         acc[j] = 0.f;
-    auto at = [&](int p) {
-        const int slot = unit_begin(a, p, npairs) >= T * a.G ? 0 : 1;
-        return a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
-    };
-    for (int p = pf; p <= pl; ++p) {
-        const float *src = at(p);
+    for (int p0 = pf; p0 <= pl; p0 += kJoinAtOnce) {
+        float v[kJoinAtOnce][kJoinRows];
 #pragma unroll
-        for (int j = 0; j < kJoinRows; ++j)
-            acc[j] += __ldcg(src + j * 32);
+        for (int b = 0; b < kJoinAtOnce; ++b) {
+            const int p = min(p0 + b, pl), slot = unit_begin(a, p, npairs) >= T * a.G ? 0 : 1;
+            const float *src = a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < kJoinRows; ++j)
+                v[b][j] = __ldcg(src + j * 32);
+        }
+#pragma unroll
+        for (int b = 0; b < kJoinAtOnce; ++b)
+            if (p0 + b <= pl) {
+#pragma unroll
+                for (int j = 0; j < kJoinRows; ++j)
+                    acc[j] += v[b][j];
+            }
     }
     const float back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(a.ep.row_scale + min(n, a.N - 1))));
-    uint32_t v[16], o[4];
+    uint32_t v[kJoinRows], o[kJoinRows / 4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < kJoinRows; ++j)
         v[j] = __float_as_uint(acc[j]);
-    gated16(v, n & 1, a.ep, back, m0, o);
+    gated_outputs(v, n & 1, a.ep, back, m0, o);
     store_gated(a.y, a.N, o, m0, a.M - m0, n);
 }
 
@@ -1008,7 +1018,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
                     uint32_t v[16], o[4];
                     tmem_ld16(ta + c, v);
                     tmem_ld_wait(v);
-                    gated16(v, n & 1, args.ep, back, m0 + c, o);
+                    gated_outputs(v, n & 1, args.ep, back, m0 + c, o);
                     store_gated(args.y, args.N, o, m0 + c, mlim - c, n);
                 }
             } else { /* gated_join_kernel adds; slot 0: the first segment of this pair's range, slot 1: its last */
@@ -1347,7 +1357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
 #pragma unroll
                     for (int jj = 0; jj < 16; ++jj)
                         v[jj] = __float_as_uint(run[h * 16 + jj]);
-                    gated16(v, n & 1, args.ep, 1.f, m0 + h * 16, o);
+                    gated_outputs(v, n & 1, args.ep, 1.f, m0 + h * 16, o);
                     store_gated(args.y, args.N, o, m0 + h * 16, jl - h * 16, n);
                 }
                 continue;
