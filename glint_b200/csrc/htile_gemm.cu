@@ -291,6 +291,7 @@ struct GemmArgs {
     int S;        /* tiles 0 .. S-1 are cut into units shared evenly by the pairs */
     int R;        /* whole-tile rounds after that: pair p takes tiles S + p + r P, r < R */
     int U;        /* units of the shared part: S x G */
+    int P;        /* pairs that share them, a unit or more each */
     int tiles;
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
@@ -301,17 +302,15 @@ struct GemmArgs {
 };
 
 /* Work split (stream-K for the first S tiles, then data-parallel rounds): the
- * units (tile, K group) of tiles 0 .. S-1 are cut into P equal ranges, pair p
+ * units (tile, K group) of tiles 0 .. S-1 are cut into P equal ranges, none empty
+ * (a tile's contributors are the pairs from its first unit's to its last's), pair p
  * owning [unit_begin(p), unit_begin(p + 1)); the remaining R * P tiles go
  * whole, round-robin.  S = tiles mod P + P with two or more rounds, or tiles - P
  * between one and two (R = 1 there), so every pair ends at the same time, a shared
  * tile has at most a few contributors, and their sums are done while whole tiles
  * run. */
-__device__ __forceinline__ int unit_begin(const GemmArgs &a, int p, int P) { return (int)((int64_t)p * a.U / P); }
-__device__ __forceinline__ int pair_of(const GemmArgs &a, int u, int P)
-{
-    return (int)(((int64_t)(u + 1) * P - 1) / a.U);
-}
+__device__ __forceinline__ int unit_begin(const GemmArgs &a, int p) { return (int)((int64_t)min(p, a.P) * a.U / a.P); }
+__device__ __forceinline__ int pair_of(const GemmArgs &a, int u) { return (int)(((int64_t)(u + 1) * a.P - 1) / a.U); }
 /* Segments of one pair's work in order: tile T, K groups [ga, gb). */
 struct Segments {
     int r = 0, u = 0, ue = 0;
@@ -482,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
     const bool leader = rank == 0;
     const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
     const int G = args.G;
-    const int ub = unit_begin(args, pair, npairs), ue = unit_begin(args, pair + 1, npairs);
+    const int ub = unit_begin(args, pair), ue = unit_begin(args, pair + 1);
     const Segments seg0{0, ub, ue};
     int T, ga, gb;
 
@@ -757,7 +756,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             if (GATED && args.join)
                 continue;
             int *cnt = args.counters + ((size_t)T * 2 + rank) * C::kEpiWarps + c0 / C::kChunks * 4 + q;
-            const int pf = pair_of(args, T * G, npairs), pl = pair_of(args, (T + 1) * G - 1, npairs);
+            const int pf = pair_of(args, T * G), pl = pair_of(args, (T + 1) * G - 1);
             int prev = 0;
             if (lane == 0)
                 prev = atomicAdd(cnt, 1);
@@ -784,7 +783,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
 #pragma unroll
                         for (int b = 0; b < C::kAtOnce; ++b) {
                             const int pq = min(p0 + b, pl);
-                            const int sq = unit_begin(args, pq, npairs) >= T * G ? 0 : 1;
+                            const int sq = unit_begin(args, pq) >= T * G ? 0 : 1;
                             const float *src = args.ws + ((((size_t)pq * 2 + sq) * 2 + rank) * 4 + q) * kPartFloats +
                                                c * 1024 + h * 512 + lane;
 #pragma unroll
@@ -833,7 +832,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
  * the product's kernel, because two SMs alone would read all partial sums of a tile: 1771 x 5888 x 2 x 204 (14
  * tiles on 74 pairs) 53 us that way, JOIN with this kernel, 62 with K uncut. */
 constexpr int kJoinRows = 4, kJoinAtOnce = 4;
-__global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int npairs)
+__global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a)
 {
     const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
     const uint32_t lane = lane_id();
@@ -841,7 +840,7 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int n
     const int T = w / (BMX / kJoinRows * 8);
     if (T >= a.S)
         return;
-    const int pf = pair_of(a, T * a.G, npairs), pl = pair_of(a, (T + 1) * a.G - 1, npairs);
+    const int pf = pair_of(a, T * a.G), pl = pair_of(a, (T + 1) * a.G - 1);
     int m0, n;
     tile_at(a, T, m0, n);
     m0 += part * kJoinRows, n += rank * BN + q * 32 + (int)lane;
@@ -855,7 +854,7 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a, int n
         float v[kJoinAtOnce][kJoinRows];
 #pragma unroll
         for (int b = 0; b < kJoinAtOnce; ++b) {
-            const int p = min(p0 + b, pl), slot = unit_begin(a, p, npairs) >= T * a.G ? 0 : 1;
+            const int p = min(p0 + b, pl), slot = unit_begin(a, p) >= T * a.G ? 0 : 1;
             const float *src = a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
 #pragma unroll
             for (int j = 0; j < kJoinRows; ++j)
@@ -909,7 +908,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
     const bool leader = rank == 0;
     const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
     const int G = args.G;
-    const int ub = unit_begin(args, pair, npairs), ue = unit_begin(args, pair + 1, npairs);
+    const int ub = unit_begin(args, pair), ue = unit_begin(args, pair + 1);
     const Segments seg0{0, ub, ue};
     int T, ga, gb;
 
@@ -1934,7 +1933,7 @@ int gemm_plan(GemmArgs &a, bool gated = false)
          * 40 x 1024 x 2 x 2000 (16 tiles, 4 groups) 21.5 and 20.2.  Above half, 250 x 4096 x 2 x 6912 (54 tiles)
          * 48 and 56, 200 x 2048 x 2 x 5000 (40 tiles) 31 and 34. */
         a.tiles = a.S = tiles, a.R = 0, a.U = tiles * a.G, a.join = 1;
-        return std::min(maxp, a.U);
+        return a.P = std::min(maxp, a.U);
     }
     const int rounds = (tiles + maxp - 1) / maxp;
     const bool idle = (double)(rounds * maxp - tiles) > 0.02 * rounds * maxp;
@@ -1944,7 +1943,7 @@ int gemm_plan(GemmArgs &a, bool gated = false)
     a.tiles = tiles;
     a.R = split ? (split1 ? 1 : tiles / pairs - 1) : (tiles + pairs - 1) / pairs;
     a.S = split ? tiles - a.R * pairs : 0;
-    a.U = a.S * a.G;
+    a.U = a.S * a.G, a.P = std::max(1, std::min(pairs, a.U));
     return pairs;
 }
 /* the same for gated_wide_kernel: the tiles beyond whole rounds are cut, if more than 2% of the time would be idle */
@@ -1955,7 +1954,7 @@ int wide_plan(GemmArgs &a)
     a.tiles = a.mtiles * a.ntiles;
     const int pairs = std::min(a.tiles, max_pairs()), left = a.tiles % pairs;
     const bool cut = left && (pairs - left) * 50 > a.tiles;
-    a.S = cut ? left : 0, a.U = a.S * a.G, a.join = cut;
+    a.S = cut ? left : 0, a.U = a.S * a.G, a.P = std::max(1, std::min(pairs, a.U)), a.join = cut;
     a.R = cut ? a.tiles / pairs : (a.tiles + pairs - 1) / pairs;
     return pairs;
 }
@@ -2065,7 +2064,7 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     a.ws = sums, a.counters = counts;
     htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
     if (a.join)
-        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a, pairs);
+        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
@@ -2096,7 +2095,7 @@ int htile_gated_wide_launch(const void *w, const void *x, void *h, float *sums, 
     const int pairs = wide_plan(a);
     gated_wide_kernel<<<2 * pairs, kWideThreads, kWideSmem, st>>>(maps, a);
     if (a.join)
-        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a, pairs);
+        gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
