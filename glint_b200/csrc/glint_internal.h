@@ -120,7 +120,7 @@ int64_t htile_gemm_gated_work(int M, int N, int K, int64_t *counts);
 int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,
                             void *h, float *sums, int *counts, int M, int N, int K, HtileMode mode, GatedEpilogue ep,
                             cudaStream_t stream);
-bool htile_gated_wide_takes(int M, int N, int K);
+bool htile_gated_wide_takes(int M, int N);
 int64_t htile_gated_wide_work(int M, int N, int K);
 int htile_gated_wide_launch(const void *w, const void *x, void *h, float *sums, int M, int N, int K, GatedEpilogue ep,
                             cudaStream_t st);

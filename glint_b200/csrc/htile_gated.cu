@@ -36,6 +36,7 @@ struct PrepArgs {
     int *counts;
     int M, N, K;
     int x_ctas, row_ctas, n_counts;
+    int expands; /* gated_expand_kernel follows */
 };
 
 /* largest finite |value| of two BF16, as its bits */
@@ -62,9 +63,13 @@ __device__ __forceinline__ float row_power(uint32_t top)
 
 __global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)
 {
-    /* the next kernel's weights may stream; it waits for this one before it reads what is written here */
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    /* The next kernel may start.  One that reads what is written here waits for this one, its weights stream
+     * meanwhile; gated_expand_kernel writes what kernels before this one may still read. */
+    if (!a.expands)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.expands)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int cta = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     if (cta < a.x_ctas) {
         __shared__ uint32_t tops[kThreads / 32];
@@ -182,6 +187,7 @@ __global__ void __launch_bounds__(kExpandThreads, kExpandCtas)
             }
         }
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory"); /* whoever follows this kernel follows gated_prep_kernel too */
 }
 
 /* kOk, or what glint_htile_gated_stream returns for these arguments before it looks at pointers */
@@ -211,7 +217,7 @@ struct Layout {
         const int N = 2 * a.F;
         const bool decode = a.M <= kDecodeM;
         half = a.mode == GLINT_HTILE_FAST;
-        wide = half && htile_gated_wide_takes(a.M, N, a.K);
+        wide = half && htile_gated_wide_takes(a.M, N);
         auto take = [&](int64_t n) {
             const int64_t at = bytes;
             bytes += (n + 255) / 256 * 256;
@@ -232,6 +238,22 @@ struct Layout {
         sums = take(s), counts = take(n_counts * (int64_t)sizeof(int));
     }
 };
+
+/* a kernel that may start while the one before it runs */
+template <typename... P, typename... A>
+bool launch_early(void (*kernel)(P...), int ctas, int threads, int smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess)
+        return true;
+    cudaGetLastError();
+    return false;
+}
 
 } // namespace
 } // namespace glint
@@ -270,19 +292,11 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
     int *counts = reinterpret_cast<int *>(work + at.counts);
     if (at.half || at.n_counts) {
         PrepArgs p{a->x, reinterpret_cast<__half *>(work + at.x16), x_scale, a->absmax, row_scale, counts, a->M, N, a->K, 0, 0,
-                   (int)at.n_counts};
+                   (int)at.n_counts, at.wide};
         if (at.half)
             p.x_ctas = a->M, p.row_ctas = decode || at.wide ? 0 : (N + kThreads / 32 - 1) / (kThreads / 32);
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(p.x_ctas + p.row_ctas + (at.n_counts ? 1 : 0)), cfg.blockDim = dim3(kThreads), cfg.stream = stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr, cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, gated_prep_kernel, p) != cudaSuccess) {
-            cudaGetLastError();
+        if (!launch_early(gated_prep_kernel, p.x_ctas + p.row_ctas + (at.n_counts ? 1 : 0), kThreads, 0, stream, p))
             return kLaunch;
-        }
     }
     const HtileMode mode = at.half ? kFast : kPrecise;
     /* FP16 in BF16's place: the kernels know by the mode */
@@ -293,9 +307,8 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
         if (!ensure_smem((const void *)gated_expand_kernel, kLutBytes))
             return kLaunch;
         const int ctas = std::min(kExpandCtas * sm_count(), (N + kExpandThreads / 32 - 1) / (kExpandThreads / 32));
-        gated_expand_kernel<<<ctas, kExpandThreads, kLutBytes, stream>>>(a->hole, a->plug, a->absmax,
-                                                                         reinterpret_cast<uint4 *>(work + at.w16), row_scale, N, a->K);
-        if (cudaGetLastError() != cudaSuccess)
+        if (!launch_early(gated_expand_kernel, ctas, kExpandThreads, kLutBytes, stream, a->hole, a->plug, a->absmax,
+                          reinterpret_cast<uint4 *>(work + at.w16), row_scale, N, a->K))
             return kLaunch;
         return htile_gated_wide_launch(work + at.w16, x, a->h, sums, a->M, N, a->K, ep, stream);
     }

@@ -877,7 +877,14 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a)
     store_gated(a.y, a.N, o, m0, a.M - m0, n);
 }
 
-/* ---- gated product of many rows, weights expanded before ------------------------- */
+/* ---- gated product of many rows, weights expanded before -------------------------
+ * The kernel above looks a weight up once for each tile of 256 activation rows, and its dequantisers, not its tensor
+ * cores, set its pace (950 TFLOP/s).  With many row tiles all weights are looked up once (gated_expand_kernel, FP16, each
+ * row times its power of two: the same operands) and this kernel multiplies: the same pairs and tiles, both operands
+ * from shared memory, 32 KB a K step and CTA in a ring of six, and two accumulators, so that a tile's epilogue runs
+ * beside the next one's products.  2048 x 4096 x 2 x 14336: 299 us, 1609 TFLOP/s, 0.99 of the library's BF16 product in
+ * a burst; with the expansion (64 us, 5.6 TB/s), x's pass (10, beside it) and the sums of cut tiles (8) 393.  A ring of
+ * five takes 2% longer; tiles in groups of 8 row tiles within 2% of 4, 16 and 32. */
 constexpr int WDSTAGES = 6;                    /* shared-memory ring: 128 activation rows and 128 weight rows of a K step */
 constexpr int kWideStage = 2 * kStageX;        /* 32 KB */
 constexpr int kWideEpi0 = 2, kWideEpiWarps = 8; /* two warps a quadrant, half of the columns each */
@@ -2068,10 +2075,13 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
 
-/* The same from expanded weights: w FP16 [N, K], the rows multiplied by ep.row_scale. */
-bool htile_gated_wide_takes(int M, int N, int K)
+/* The same from expanded weights: w FP16 [N, K], the rows multiplied by ep.row_scale.  It takes the calls whose row
+ * tiles would have every weight looked up four times or more, unless there are fewer tiles than pairs: with the
+ * expansion, from planes and so, at 4096 x 2 x 14336: 768 rows 200 and 203 us, 900 rows 262 and 231, 2048 rows 483
+ * and 393, 8191 rows 2246 and 1515. */
+bool htile_gated_wide_takes(int M, int N)
 {
-    return M >= 1024 && (int64_t)((M + BMX - 1) / BMX) * ((N + 2 * BN - 1) / (2 * BN)) >= max_pairs();
+    return M > 3 * BMX && (int64_t)((M + BMX - 1) / BMX) * ((N + 2 * BN - 1) / (2 * BN)) >= max_pairs();
 }
 int64_t htile_gated_wide_work(int M, int N, int K)
 {

@@ -138,9 +138,11 @@ def test_shapes(M, K, F, mode, name):
 @pytest.mark.parametrize("M,K,F", [(1, 4096, 14336), (5, 2048, 6911), (16, 1024, 28672), (31, 512, 18001), (32, 16384, 500),
                                    (511, 1024, 14336), (300, 512, 9473), (1030, 256, 10000), (16, 10240, 6000), (2, 8192, 4999),
                                    (9, 2560, 9728), (7, 5120, 3000), (8, 3584, 2222), (13, 33280, 50),
-                                   (98, 6656, 174), (1771, 5888, 204), (33, 33280, 3), (640, 4096, 1535), (65, 1792, 129)])
+                                   (98, 6656, 174), (1771, 5888, 204), (33, 33280, 3), (640, 4096, 1535), (65, 1792, 129),
+                                   (769, 256, 4700), (2311, 768, 1021), (2817, 2304, 1537), (1025, 512, 9345), (5000, 256, 650)])
 def test_wide_layers(M, K, F, mode):
-    """More rows than two blocks a CTA; tiles shared between CTA pairs (511, 300 and 1030 rows)."""
+    """More rows than two blocks a CTA; tiles shared between CTA pairs (511 and 300 rows); weights expanded first, with
+    whole tiles alone and with a cut rest (769 rows and more)."""
     check(M, K, F, mode=mode)
 
 
