@@ -36,6 +36,13 @@
  *               column = activation row) to y.
  * Weights reach the MMA as RN_bf16(cell * absmax) (relative error <= 2^-9 per
  * weight), i.e. the GLINT_HTILE_FAST arithmetic.
+ * The gated product (GATED) is the same kernel on FP16 values: weights RN_f16(cell * absmax * the row's power of two),
+ * warps 2-17 dequantisers in two groups that take K steps in turn, warps 18-25 epilogue, warp 26 plane producer.  It
+ * starts while the pass over x runs (griddepcontrol).  A K step takes 0.48 us with 64 rows, 0.57 with 256, where the
+ * tensor cores need 0.27 to 0.38 as the clock goes: lookups and UMMAs a quarter each 0.32, either alone 0.41 (so both
+ * bound it, through the issue slots and tensor memory that they share, and behind them the planes' way from HBM); no
+ * lookup table's cost alone (without its reads 1.5 us of 77), no longer rings, nor publishing a step's weights
+ * one step later (2 us more).
  *
  * Every mbarrier wait is bounded (about one second of clock64 time) and suspends
  * the warp between polls; when a wait runs out the kernel records an error in
@@ -75,7 +82,8 @@ constexpr int kDeq0 = 2;                 /* first dequantiser warp */
 constexpr int kStepWarps = 8;             /* dequantisers of a K step */
 constexpr int kWpt = BK * 4 / kStepWarps; /* 32 weights per dequantiser thread and K step */
 /* Warps of the product alone and with a gated epilogue, whose accumulator is busy longer
- * (an exchange, an exponential and a division for each output): two warps a quadrant there. */
+ * (an exchange, an exponential and a division for each output): two warps a quadrant there, and two groups of
+ * dequantisers, that take K steps in turn (511 x 4096 x 2 x 14336 in a cold loop: one group 130 us, two 126). */
 template <bool GATED>
 struct GemmCfg {
     static constexpr int kGroups = GATED ? 2 : 1; /* of dequantisers, that take K steps in turn */
@@ -83,7 +91,6 @@ struct GemmCfg {
     static constexpr int kEpi0 = kDeq0 + kDeqWarps;
     static constexpr int kPlaneWarp = kEpi0 + kEpiWarps; /* plane producer */
     static constexpr int kThreads = (kPlaneWarp + 1) * 32;
-    static constexpr int kChunks = BMX / 32 / (kEpiWarps / 4); /* of 32 columns, an epilogue warp's */
     static constexpr int kAtOnce = GATED ? 2 : 4; /* contributors of a split tile loaded before they are added */
 };
 constexpr int kPartFloats = 8 * 32 * 32;            /* one epilogue warp's share of a partial tile */
@@ -171,6 +178,9 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *m
                  "l"(map), "r"(bar_cluster), "r"(x), "r"(y)
                  : "memory");
 }
+
+/* the kernel before this one is done (launched early: see htile_gemm_gated_launch) */
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -296,6 +306,7 @@ struct GemmArgs {
     float *ws;    /* partial tiles of split tiles: [pair][slot 2][rank 2][quadrant 4][kPartFloats] */
     int *counters; /* per tile, rank and quadrant: contributors done (reset by the last) */
     GatherArgs ga; /* world > 0: y[m, n] goes to every rank's y at [m, ga.n0 + n] (row stride ga.ldy) */
+    int half;         /* gated: activation rows that a CTA holds, BMH or, in a product of few rows, fewer */
     int group;        /* gated: tiles of so many rows' tiles in turn, see tile_at */
     int join;         /* gated: split tiles are added by gated_join_kernel, not by their last contributor */
     GatedEpilogue ep; /* gated kernel */
@@ -365,31 +376,38 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
 }
 /* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of R
  * rows from m on.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
- * second.  o: R / 2 outputs, of rows 2i + (n & 1), as BF16 pairs. */
-template <int R>
-__device__ __forceinline__ void gated_outputs(const uint32_t (&v)[R], bool up, const GatedEpilogue &ep, float row, int m,
-                                              uint32_t (&o)[R / 4])
+ * second.  o: R / 2 outputs, of rows 2i + (n & 1), as BF16 pairs.  What the sums are to be multiplied by: x_scale of
+ * their row and `row` of their column. */
+template <int ACT, int R>
+__device__ __forceinline__ void gated_outputs_of(const uint32_t (&v)[R], bool up, const float *x_scale, float row, int m,
+                                                 uint32_t (&o)[R / 4])
 {
-    /* what sums of this lane's column (`row`) and of the pair's other one are of their values, with x's part in it */
-    const float mine = row, theirs = __shfl_xor_sync(0xFFFFFFFFu, row, 1);
+    const float other = __shfl_xor_sync(0xFFFFFFFFu, row, 1), by_g = up ? other : row, by_u = up ? row : other;
 #pragma unroll
     for (int i = 0; i < R / 4; ++i) {
-        float h[2];
         float4 x = make_float4(1.f, 1.f, 1.f, 1.f);
-        if (ep.x_scale)
-            x = __ldg(reinterpret_cast<const float4 *>(ep.x_scale + m + 4 * i));
+        if (x_scale)
+            x = __ldg(reinterpret_cast<const float4 *>(x_scale + m + 4 * i));
+        float h[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t a = v[4 * i + 2 * j], b = v[4 * i + 2 * j + 1];
-            const float keep = __uint_as_float(up ? b : a), give = __uint_as_float(up ? a : b);
-            const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
+            const float a = __uint_as_float(v[4 * i + 2 * j]), b = __uint_as_float(v[4 * i + 2 * j + 1]);
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, up ? a : b, 1);
             const float by = j ? (up ? x.w : x.z) : (up ? x.y : x.x);
-            const float a1 = by * mine * keep, b1 = by * theirs * got;
-            h[j] = gated_value(up ? b1 : a1, up ? a1 : b1, ep.act);
+            h[j] = gated_value(by * by_g * (up ? got : a), by * by_u * (up ? b : got), ACT);
         }
         const __nv_bfloat162 b2 = __floats2bfloat162_rn(h[0], h[1]);
         o[i] = *reinterpret_cast<const uint32_t *>(&b2);
     }
+}
+template <int R>
+__device__ __forceinline__ void gated_outputs(const uint32_t (&v)[R], bool up, const GatedEpilogue &ep, float row, int m,
+                                              uint32_t (&o)[R / 4])
+{
+    if (ep.act == GLINT_ACT_GELU_TANH)
+        gated_outputs_of<GLINT_ACT_GELU_TANH>(v, up, ep.x_scale, row, m, o);
+    else
+        gated_outputs_of<GLINT_ACT_SILU>(v, up, ep.x_scale, row, m, o);
 }
 /* them into column n / 2 of h [.., n_cols / 2], rows m0 .. m0+jl-1 */
 template <int R4>
@@ -399,10 +417,17 @@ __device__ __forceinline__ void store_gated(void *h, int n_cols, const uint32_t 
         return;
     const size_t ld = (size_t)(n_cols / 2);
     __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(h) + (size_t)(m0 + (n & 1)) * ld + n / 2;
+    auto put = [&](int j) { *p = __ushort_as_bfloat16((unsigned short)(o[j / 2] >> (16 * (j & 1)))); };
+    if (jl >= 4 * R4) {
 #pragma unroll
-    for (int j = 0; j < 2 * R4; ++j, p += 2 * ld)
-        if (2 * j + (n & 1) < jl)
-            *p = __ushort_as_bfloat16((unsigned short)(o[j / 2] >> (16 * (j & 1))));
+        for (int j = 0; j < 2 * R4; ++j, p += 2 * ld)
+            put(j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2 * R4; ++j, p += 2 * ld)
+            if (2 * j + (n & 1) < jl)
+                put(j);
+    }
 }
 /* y rows m0 .. m0+jl-1 at column n: this call's y; in a gathered call this
  * rank's y and, with `peers`, every other rank's (over NVLink, starting with the
@@ -480,7 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
-    const int G = args.G;
+    const int G = args.G, half = GATED ? args.half : BMH;
     const int ub = unit_begin(args, pair), ue = unit_begin(args, pair + 1);
     const Segments seg0{0, ub, ue};
     int T, ga, gb;
@@ -518,11 +543,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
 
     if (warp == 0) {
         /* ---- activation producer (both CTAs): this CTA's half of the x tile */
+        if constexpr (GATED)
+            griddep_wait();
         if (lane == 0) {
             Ring st, back; /* back: the step XSTAGES before, whose tile the next one replaces */
             int64_t issued = 0;
             for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
-                const int mr = (T % args.mtiles) * BMX + (int)rank * BMH;
+                const int mr = (T % args.mtiles) * BMX + (int)rank * half;
                 for (int ks = ga * PSTEPS; ks < gb * PSTEPS && alive; ++ks, st.next<XSTAGES>()) {
                     if (issued >= XSTAGES) {
                         if (!wait_or_fail(&step_done[back.i], back.ph, alive))
@@ -530,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                         back.next<WSLOTS>();
                     }
                     if (leader)
-                        mbar_expect_tx(&x_full[st.i], 2 * kStageX);
+                        mbar_expect_tx(&x_full[st.i], 2 * half * BK * 2);
                     tma_load_2d_pair(xring + st.i * kStageX, &maps.x, peer_addr(saddr(&x_full[st.i]), 0), ks * BK, mr);
                     ++issued;
                 }
@@ -573,6 +600,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         if (leader && lane == 0) {
             Ring st, ws;
             int t = 0;
+            const uint32_t idesc = kIdesc<GATED> - (GATED ? (uint32_t)((BMH - half) * 2 >> 3) << 17 : 0u);
             for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb); ++t) {
                 if (t >= 1 && !wait_or_fail(acc_empty, (uint32_t)(t - 1) & 1u, alive))
                     break;
@@ -586,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                     const uint32_t wa = tmem + kWCol + (uint32_t)ws.i * (BK / 2);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk)
-                        umma_pair_ts_bf16(tmem + kAccCol, wa + kk * 8, sw128_desc(xs + kk * 32), kIdesc<GATED>,
+                        umma_pair_ts_bf16(tmem + kAccCol, wa + kk * 8, sw128_desc(xs + kk * 32), idesc,
                                           (ks > k0 || kk > 0) ? 1u : 0u);
                     umma_commit_pair(&step_done[ws.i]);
                 }
@@ -615,6 +643,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             if ((ws.i += C::kGroups) >= WSLOTS)
                 ws.i -= WSLOTS, ws.ph ^= 1u;
         };
+        if constexpr (GATED)
+            griddep_wait();
         for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
             [[maybe_unused]] float row_scale = 1.f;
             if constexpr (GATED)
@@ -682,39 +712,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
          * contributor stores its f32 partial (L2 only) and counts itself in; the
          * last one adds all partials in K order, so y does not depend on which
          * pair finished last. */
-        const int q = warp & 3, c0 = GATED ? (warp - C::kEpi0) / 4 * C::kChunks : 0, c1 = c0 + C::kChunks;
+        /* its chunks of 32 columns: all, or every second one of a gated tile */
+        const int q = warp & 3, c0 = GATED ? (warp - C::kEpi0) / 4 : 0, cs = C::kEpiWarps / 4;
         const uint32_t accempty0 = peer_addr(saddr(acc_empty), 0);
         const uint32_t tb = tmem + ((uint32_t)(q * 32) << 16) + kAccCol;
         int t = 0;
+        if constexpr (GATED)
+            griddep_wait();
         for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb); ++t) {
-            if (!warp_wait(acc_full, (uint32_t)t & 1u, alive))
-                break;
-            tc_fence_after();
             const int m0 = (T % args.mtiles) * BMX, n0 = (T / args.mtiles) * (2 * BN);
             const int n = n0 + (int)rank * BN + q * 32 + (int)lane;
             const int mlim = min(BMX, args.M - m0);
             [[maybe_unused]] float row_back = 1.f; /* 1 / row_scale[n], a power of two */
-            if constexpr (GATED)
+            if constexpr (GATED) {
                 row_back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
+                /* the tile's x_scale into L1 while the products run */
+                asm volatile("" ::"f"(__ldg(args.ep.x_scale + m0 + (lane & 7) * 32)));
+            }
+            if (!warp_wait(acc_full, (uint32_t)t & 1u, alive))
+                break;
+            tc_fence_after();
             const bool whole = ga == 0 && gb == G;
             if (whole) {
-                [[maybe_unused]] uint32_t o[2 * C::kChunks][4];
-                if constexpr (GATED) {
-                    /* the outputs stay in registers until the accumulator is released: their stores
-                     * run beside the next tile's products */
-#pragma unroll
-                    for (int c = 0; c < 2 * C::kChunks; ++c) {
-                        uint32_t v[16];
-                        tmem_ld16(tb + c0 * 32 + c * 16, v);
-                        tmem_ld_wait(v);
-                        gated_outputs(v, n & 1, args.ep, row_back, m0 + c0 * 32 + c * 16, o[c]);
-                    }
-                } else {
 #pragma unroll 1
-                    for (int c = 0; c < BMX / 32 && c * 32 < mlim; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(tb + c * 32, v);
-                        tmem_ld_wait();
+                for (int c = c0; c < BMX / 32 && c * 32 < mlim; c += cs) {
+                    uint32_t v[32];
+                    tmem_ld32(tb + c * 32, v);
+                    tmem_ld_wait();
+                    if constexpr (GATED) {
+                        uint32_t o[8];
+                        gated_outputs(v, n & 1, args.ep, row_back, m0 + c * 32, o);
+                        store_gated(args.y, args.N, o, m0 + c * 32, mlim - c * 32, n);
+                    } else {
                         store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, false);
                     }
                 }
@@ -722,11 +751,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_remote(accempty0);
-                if constexpr (GATED) {
-#pragma unroll
-                    for (int c = 0; c < 2 * C::kChunks; ++c)
-                        store_gated(args.y, args.N, o[c], m0 + c0 * 32 + c * 16, mlim - c0 * 32 - c * 16, n);
-                }
                 if (!GATED && args.ga.world > 1 && n < args.N) {
                     if (args.y_bf16)
                         copy_rows_to_peers<__nv_bfloat16>(args.ga, m0, mlim, args.ga.n0 + n);
@@ -739,7 +763,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             const int slot = ub >= T * G ? 0 : 1;
             float *mine = args.ws + ((((size_t)pair * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats;
 #pragma unroll 1
-            for (int c = c0; c < c1; ++c) {
+            for (int c = c0; c < BMX / 32 && (!GATED || c * 32 < mlim); c += cs) {
                 uint32_t v[32];
                 tmem_ld32(tb + c * 32, v);
                 tmem_ld_wait();
@@ -755,7 +779,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             __syncwarp();
             if (GATED && args.join)
                 continue;
-            int *cnt = args.counters + ((size_t)T * 2 + rank) * C::kEpiWarps + c0 / C::kChunks * 4 + q;
+            int *cnt = args.counters + ((size_t)T * 2 + rank) * C::kEpiWarps + (GATED ? c0 * 4 : 0) + q;
             const int pf = pair_of(args, T * G), pl = pair_of(args, (T + 1) * G - 1);
             int prev = 0;
             if (lane == 0)
@@ -769,7 +793,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             if (lane == 0)
                 *cnt = 0;
 #pragma unroll 1
-            for (int c = c0; c < c1 && c * 32 < mlim; ++c) {
+            for (int c = c0; c < BMX / 32 && c * 32 < mlim; c += cs) {
                 uint32_t v[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -1932,6 +1956,7 @@ int gemm_plan(GemmArgs &a, bool gated = false)
 {
     a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
     a.G = a.K / (PSTEPS * BK), a.group = a.mtiles;
+    a.half = !gated || a.M > 128 ? BMH : a.M > 64 ? 64 : 32;
     const int tiles = a.mtiles * a.ntiles;
     const int maxp = max_pairs();
     if (gated && tiles * 2 <= maxp) {
@@ -1968,9 +1993,9 @@ int wide_plan(GemmArgs &a)
 size_t part_floats(int pairs) { return (size_t)pairs * 2 * 2 * 4 * kPartFloats; }
 
 bool gemm_maps(Maps &maps, const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, int M,
-               int N, int K)
+               int N, int K, int half)
 {
-    return encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, BMH,
+    return encode_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, BK, half,
                       CU_TENSOR_MAP_SWIZZLE_128B) &&
            encode_map(&maps.h, CU_TENSOR_MAP_DATA_TYPE_UINT8, hole, (uint64_t)K / 2, (uint64_t)N, (uint64_t)K / 2,
                       PSTEPS * BK / 2, BN, CU_TENSOR_MAP_SWIZZLE_128B) &&
@@ -1984,7 +2009,7 @@ int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, 
                      bool y_bf16, int M, int N, int K, cudaStream_t st, const GatherArgs *ga)
 {
     Maps maps;
-    if (!gemm_maps(maps, hole, plug, am, x, M, N, K) || !ensure_smem((const void *)htile_gemm_kernel<false>, kSmemBytes))
+    if (!gemm_maps(maps, hole, plug, am, x, M, N, K, BMH) || !ensure_smem((const void *)htile_gemm_kernel<false>, kSmemBytes))
         return kLaunch;
     GemmArgs a{};
     a.y = y, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0;
@@ -2062,14 +2087,24 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
 {
     if (mode == kPrecise)
         return precise_launch_impl<true>(hole, plug, am, x, h, true, M, N, K, ep, st);
-    Maps maps;
-    if (!gemm_maps(maps, hole, plug, am, x, M, N, K) || !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
-        return kLaunch;
     GemmArgs a{};
     a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep;
     const int pairs = gemm_plan(a, true);
+    Maps maps;
+    if (!gemm_maps(maps, hole, plug, am, x, M, N, K, a.half) || !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
+        return kLaunch;
     a.ws = sums, a.counters = counts;
-    htile_gemm_kernel<true><<<2 * pairs, GemmCfg<true>::kThreads, kSmemBytes, st>>>(maps, a);
+    /* codebook, tensor memory and the first planes while gated_prep_kernel runs */
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(2 * pairs), cfg.blockDim = dim3(GemmCfg<true>::kThreads), cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, htile_gemm_kernel<true>, maps, a) != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunch;
+    }
     if (a.join)
         gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
