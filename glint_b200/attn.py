@@ -309,19 +309,26 @@ def _outputs_apart(q, k, q_out, k_out, more) -> None:
 def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, more, keys):
     """The checks that rope and rope_append share; (struct, stream, q_out, k_out).  more: further
     inputs of q's type; keys: k_out is wanted whether it was given or not."""
-    _want(q, "q", torch.bfloat16, (None, None, None), dense=False)
+    # a check that holds costs half of _want's call: what does not pass here is named there
+    if q.dtype is not torch.bfloat16 or not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+        _want(q, "q", torch.bfloat16, (None, None, None), dense=False)
     T, H, D = q.shape
     _head_dim(D)
     if H < 1:
         raise ValueError("q must have a head or more")
     Hk = 0
     if k is not None:
-        _want(k, "k", torch.bfloat16, (T, None, D), dense=False)
-        Hk = k.shape[1]
+        shape = k.shape
+        if k.dtype is not torch.bfloat16 or not k.is_cuda or len(shape) != 3 or shape[0] != T or shape[2] != D or \
+                k.stride(2) != 1:
+            _want(k, "k", torch.bfloat16, (T, None, D), dense=False)
+        Hk = shape[1]
     elif k_norm is not None or k_out is not None:
         raise ValueError("k_norm and k_out need k")
-    _want(positions, "positions", torch.int32, (T,))
-    _want(inv_freq, "inv_freq", torch.float32, (None,))
+    if positions.dtype is not torch.int32 or not positions.is_cuda or positions.shape != (T,) or not positions.is_contiguous():
+        _want(positions, "positions", torch.int32, (T,))
+    if inv_freq.dtype is not torch.float32 or not inv_freq.is_cuda or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        _want(inv_freq, "inv_freq", torch.float32, (None,))
     half = inv_freq.shape[0]
     if half > D // 2:
         raise ValueError(f"inv_freq must have {D // 2} frequencies or fewer, not {half}")
@@ -340,7 +347,13 @@ def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_
         q_out = _empty(q, (T, H, D), torch.bfloat16, stream)
     if k_out is None and keys and k is not None:
         k_out = _empty(q, (T, Hk, D), torch.bfloat16, stream)
-    raw = _raw(q, stream, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
+    dev = q.get_device()
+    if stream is None and q_norm is None and k_norm is None and (k is None or k.get_device() == dev) and \
+            positions.get_device() == dev and inv_freq.get_device() == dev and q_out.get_device() == dev and \
+            (k_out is None or k_out.get_device() == dev) and dev == torch.cuda.current_device():
+        raw = torch._C._cuda_getCurrentRawStream(dev)
+    else:
+        raw = _raw(q, stream, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
     qs, os = q.stride(), q_out.stride()
     ks = (0, 0) if k is None else k.stride()
     kos = (0, 0) if k_out is None else k_out.stride()
@@ -476,9 +489,13 @@ def rope_append(cache: KV4Cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     returned) and the same bytes in the cache.  The rotated keys go to the cache alone unless k_out is given (k
     itself, or a tensor of k's shape), as a prompt's attention wants them.  A token whose slot is
     negative is rotated and not cached."""
-    _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
-    _want(v, "v", torch.bfloat16, k.shape, dense=False)
-    _want(slots, "slots", torch.int32, k.shape[:1])
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != cache.kv_heads or shape[2] != cache.head_dim:
+        _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
+    if v.dtype is not torch.bfloat16 or not v.is_cuda or v.shape != shape or v.stride(2) != 1:
+        _want(v, "v", torch.bfloat16, shape, dense=False)
+    if slots.dtype is not torch.int32 or not slots.is_cuda or slots.shape != shape[:1] or not slots.is_contiguous():
+        _want(slots, "slots", torch.int32, shape[:1])
     a, raw, q_out, _ = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
                              (v,), False)
     if slots.get_device() != cache.device or v.get_device() != cache.device or q.get_device() != cache.device:

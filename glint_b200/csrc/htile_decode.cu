@@ -682,7 +682,7 @@ constexpr int r_tail_bytes() { return MT <= 2 ? kTailX + r_xsub<MT>() + 3 * 32 *
  * lookups' latency behind, and longer row blocks, so that 194 rows a CTA (2 x 14336 on 148 SMs) are 13
  * tiles in one block in place of 14 in two, 132 or 149 rows 9 or 10 in one in place of 10 in two.  One
  * row: 2 x 14336 x 4096 34.2 -> 32.9 us, 2 x 9728 x 2560 18.9 -> 15.7, 2 x 11008 x 4096 27.8 -> 24.1; sixteen: 41.5
- * -> 41.2, 22.2 -> 18.0, 33.0 -> 27.7. */
+ * -> 41.2, 22.2 -> 18.0, 33.0 -> 27.7 (BF16 operands; the pass that makes x FP16 adds 2.8). */
 constexpr int kMany = 28, kSome = 20;
 template <int MT, int C>
 struct RowCfg {

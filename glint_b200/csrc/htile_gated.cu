@@ -7,8 +7,15 @@
  * largest finite value into [2^14, 2^15), exactly: every BF16 value down to 2^-29 of the largest keeps all its bits,
  * and what lies below is off by 2^-40 of the largest at most.  Where weights carry their absmax into the
  * products (more than 32 rows), so is each row of W by the one that brings its largest absmax into (1/2, 1].
- * The epilogues divide by both, again exactly.  The pass is one small kernel (a row of x a CTA; 8191 x 4096: 25 us
- * of the call's 2.1 ms), and the next kernel's weights stream beside it.
+ * The epilogues divide by both, again exactly.  The pass is one small kernel (a row of x a CTA; 2.8 us for a token,
+ * 25 for 8191 x 4096), beside which the next kernel's weights stream or are expanded.
+ *
+ * Three ways, at 4096 x 2 x 14336 (us; memory's floor 19.5, the tensor cores' 0.145 a row in a burst):
+ *   1 to 32 rows    the decode kernels, lookups straight into mma.sync: 35.9 for a row, 62.7 for 32 (the second 65.6
+ *                   for 33)
+ *   from there      the tcgen05 product from planes: 66 for 64 rows, 81 for 256, 135 for 511
+ *   from 769 rows, unless there are fewer tiles than CTA pairs, weights expanded first: 231 for 900 (the second
+ *                   262), 391 for 2048 (483), 1330 to 1515 for 8191, as the clock goes (2246)
  */
 #include <cuda_fp16.h>
 
@@ -24,8 +31,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kHeld = 4; /* 16 bytes a thread that stay in registers: K up to 8192 */
-/* up to so many rows the decode kernels: 32 rows of 2 x 14336 x 4096 take them 59 us, the tcgen05 product 85 */
-constexpr int kDecodeM = 32;
+constexpr int kDecodeM = 32; /* rows that the decode kernels take */
 
 struct PrepArgs {
     const __nv_bfloat16 *x;
@@ -133,10 +139,12 @@ __global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)
 
 /* W in FP16, its rows multiplied by their powers of two, for calls of many rows: a warp a row of W, which first takes
  * the row's largest absmax; the codebook lies in shared memory once for each lane, so a lookup meets no conflict and
- * its address is one byte permute. */
+ * its address is one byte permute.  Memory bounds it: 2 x 14336 x 4096 64 us, 5.6 TB/s; two or eight loads of a plane
+ * under way in place of four, or two CTAs of 768 threads, 63 to 67. */
 constexpr int kExpandThreads = 512, kExpandCtas = 3 /* an SM */, kExpandAtOnce = 4, kLutBytes = 256 * 256;
 __global__ void __launch_bounds__(kExpandThreads, kExpandCtas)
-    gated_expand_kernel(const uint8_t *hole, const uint8_t *plug, const float *absmax, uint4 *out, float *row_scale, int N, int K)
+    gated_expand_kernel(const uint8_t *hole, const uint8_t *plug, const float *absmax, uint4 *out, float *row_scale, int N,
+                        int K)
 {
     extern __shared__ __align__(16) float lut[];
     for (int i = threadIdx.x; i < 256 * 32; i += kExpandThreads)
@@ -282,13 +290,15 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
         return cudaMemsetAsync(a->h, 0, (size_t)a->M * a->F * 2, stream) == cudaSuccess ? kOk : kLaunch;
     const int N = 2 * a->F;
     if (!streams(*a))
-        return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, a->act, stream);
+        return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, a->act,
+                                       stream);
     const Layout at(*a);
     if (at.bytes > 0 && (!a->work || !aligned_to(a->work, 16)))
         return kBadArg;
     char *work = static_cast<char *>(a->work);
     const bool decode = a->M <= kDecodeM;
-    float *x_scale = reinterpret_cast<float *>(work + at.x_scale), *row_scale = reinterpret_cast<float *>(work + at.row_scale);
+    float *x_scale = reinterpret_cast<float *>(work + at.x_scale);
+    float *row_scale = reinterpret_cast<float *>(work + at.row_scale);
     int *counts = reinterpret_cast<int *>(work + at.counts);
     if (at.half || at.n_counts) {
         PrepArgs p{a->x, reinterpret_cast<__half *>(work + at.x16), x_scale, a->absmax, row_scale, counts, a->M, N, a->K, 0, 0,
@@ -312,6 +322,6 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
             return kLaunch;
         return htile_gated_wide_launch(work + at.w16, x, a->h, sums, a->M, N, a->K, ep, stream);
     }
-    return decode ? htile_decode_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream)
-                  : htile_gemm_gated_launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream);
+    const auto launch = decode ? htile_decode_gated_launch : htile_gemm_gated_launch;
+    return launch(a->hole, a->plug, a->absmax, x, a->h, sums, counts, a->M, N, a->K, mode, ep, stream);
 }

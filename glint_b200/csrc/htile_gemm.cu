@@ -854,7 +854,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
 /* The split tiles of a gated product: a warp takes 32 columns (weight rows) and 4 activation rows of one tile, adds
  * the contributors' sums in K order, four at a time, and stores the outputs.  The last contributor does not do it in
  * the product's kernel, because two SMs alone would read all partial sums of a tile: 1771 x 5888 x 2 x 204 (14
- * tiles on 74 pairs) 53 us that way, JOIN with this kernel, 62 with K uncut. */
+ * tiles on 74 pairs) 53 us that way, 38 with this kernel, 10 of them its own, 62 with K uncut. */
 constexpr int kJoinRows = 4, kJoinAtOnce = 4;
 __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a)
 {
@@ -879,7 +879,8 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a)
 #pragma unroll
         for (int b = 0; b < kJoinAtOnce; ++b) {
             const int p = min(p0 + b, pl), slot = unit_begin(a, p) >= T * a.G ? 0 : 1;
-            const float *src = a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
+            const float *src =
+                a.ws + ((((size_t)p * 2 + slot) * 2 + rank) * 4 + q) * kPartFloats + part * kJoinRows * 32 + lane;
 #pragma unroll
             for (int j = 0; j < kJoinRows; ++j)
                 v[b][j] = __ldcg(src + j * 32);
@@ -1037,7 +1038,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
             m0 += c0, n += (int)rank * BN + q * 32 + (int)lane;
             const int mlim = args.M - m0;
             /* 1 / row_scale[n], a power of two */
-            const float back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
+            const float back =
+                __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
             if (!warp_wait(&acc_full[acc.i], acc.ph, alive))
                 break;
             tc_fence_after();
@@ -2091,7 +2093,8 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep;
     const int pairs = gemm_plan(a, true);
     Maps maps;
-    if (!gemm_maps(maps, hole, plug, am, x, M, N, K, a.half) || !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
+    if (!gemm_maps(maps, hole, plug, am, x, M, N, K, a.half) ||
+        !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
         return kLaunch;
     a.ws = sums, a.counters = counts;
     /* codebook, tensor memory and the first planes while gated_prep_kernel runs */

@@ -17,6 +17,12 @@
  * The mean is summed in 64 bits and products and sums are rounded one by one, as they stand
  * above: the result depends on no order, and what is then rounded to BF16 and to 4 bits is
  * the same whichever of the entry points computes it.
+ *
+ * Bytes bound it: q and k read and written once, v read, codes written.  32768 tokens, 32 / 8 heads of 128,
+ * norms: 124 us, 5.4 TB/s where a copy reaches 6.4 (its floor 105); 16383 tokens into the cache 89 us of 61, the
+ * quantisation's shuffles and conversions in the way; few tokens are launch and latency: 1 token 2.6 us, 513
+ * 4.7, 7 into the cache 3.6.  CTAs of 4 warps, 6 an SM (5 with the cache): of 8 warps 127 to 150 us for the 124, more
+ * CTAs with fewer registers 154.
  */
 #include <cuda_runtime.h>
 #include <stdint.h>
