@@ -488,7 +488,7 @@ def rope_append(cache: KV4Cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     """rope(q, k, ...), then kv4_append(cache, the rotated k, v, slots), in one pass: the same q_out (which is
     returned) and the same bytes in the cache.  The rotated keys go to the cache alone unless k_out is given (k
     itself, or a tensor of k's shape), as a prompt's attention wants them.  A token whose slot is
-    negative is rotated and not cached."""
+    negative is rotated and not cached; no slot twice in one call."""
     shape = k.shape
     if len(shape) != 3 or shape[1] != cache.kv_heads or shape[2] != cache.head_dim:
         _want(k, "k", torch.bfloat16, (None, cache.kv_heads, cache.head_dim), dense=False)
