@@ -306,6 +306,9 @@ def _outputs_apart(q, k, q_out, k_out, more) -> None:
         raise ValueError("q_out and k_out must be apart")
 
 
+_DENSE = torch.contiguous_format
+
+
 def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, more, keys):
     """The checks that rope and rope_append share; (struct, stream, q_out, k_out).  more: further
     inputs of q's type; keys: k_out is wanted whether it was given or not."""
@@ -325,7 +328,8 @@ def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_
         Hk = shape[1]
     elif k_norm is not None or k_out is not None:
         raise ValueError("k_norm and k_out need k")
-    if positions.dtype is not torch.int32 or not positions.is_cuda or positions.shape != (T,) or not positions.is_contiguous():
+    if positions.dtype is not torch.int32 or not positions.is_cuda or positions.shape != (T,) or \
+            not positions.is_contiguous():
         _want(positions, "positions", torch.int32, (T,))
     if inv_freq.dtype is not torch.float32 or not inv_freq.is_cuda or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         _want(inv_freq, "inv_freq", torch.float32, (None,))
@@ -344,9 +348,11 @@ def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_
                 _want(o, name, torch.bfloat16, shape, dense=False)
         _outputs_apart(q, k, q_out, k_out, more)
     if q_out is None:
-        q_out = _empty(q, (T, H, D), torch.bfloat16, stream)
+        q_out = torch.empty_like(q, memory_format=_DENSE) if stream is None else \
+            _empty(q, (T, H, D), torch.bfloat16, stream)
     if k_out is None and keys and k is not None:
-        k_out = _empty(q, (T, Hk, D), torch.bfloat16, stream)
+        k_out = torch.empty_like(k, memory_format=_DENSE) if stream is None else \
+            _empty(q, (T, Hk, D), torch.bfloat16, stream)
     dev = q.get_device()
     if stream is None and q_norm is None and k_norm is None and (k is None or k.get_device() == dev) and \
             positions.get_device() == dev and inv_freq.get_device() == dev and q_out.get_device() == dev and \
