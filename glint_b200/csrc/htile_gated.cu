@@ -1,12 +1,13 @@
 /* The gated feed-forward projection's entry point: which kernel takes a call, and the pass over x before it.
  *
- * In fast mode weights and activations meet the tensor cores in FP16: a weight's rounding to one BF16 value (2^-9
+ * In fast mode weights and activations meet the tensor cores in FP16: a weight's rounding to one BF16 value (2^-8
  * of it) would show in h as much as h's own rounding does (error against 64 bits 0.0027 of h's norm, where
- * BF16 outputs alone are 0.0017 off), to one FP16 value (2^-12) it does not (0.0017), at the same rate.
+ * BF16 outputs alone are 0.0017 off), to one FP16 value (2^-11) it does not (0.0017), at the same rate.
  * FP16's range is what that takes care of: each row of x is multiplied by the power of two that brings its
  * largest finite value into [2^14, 2^15), exactly: every BF16 value down to 2^-29 of the largest keeps all its bits,
- * and what lies below is off by 2^-40 of the largest at most.  Where weights carry their absmax into the
- * products (more than 32 rows), so is each row of W by the one that brings its largest absmax into (1/2, 1].
+ * and what lies below is off by 2^-39 of the largest at most.  Where weights carry their absmax into the
+ * products (more than 32 rows), so is each row of W by the one that brings its largest absmax into [2^14, 2^15) (no cell
+ * is above 1; the sums of 2^30 at most stay far inside f32).
  * The epilogues divide by both, again exactly.  The pass is one small kernel (a row of x a CTA; 2.8 us for a token,
  * 25 for 8191 x 4096), beside which the next kernel's weights stream or are expanded.
  *
@@ -62,11 +63,11 @@ __device__ __forceinline__ uint32_t finite_bits(float v)
     const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
     return b < 0x7F800000u ? b : 0u;
 }
-/* the power of two that brings a row of W whose largest absmax has these bits into (1/2, 1]; in [2^-126, 2^126], so
+/* the power of two that brings a row of W whose largest absmax has these bits into [2^14, 2^15); up to 2^126, so
  * that its inverse is a normal number too */
 __device__ __forceinline__ float row_power(uint32_t top)
 {
-    return power(max(-126, min(126, -((int)(top >> 23) - 127) - 1)));
+    return power(min(126, 14 - ((int)(top >> 23) - 127)));
 }
 
 __global__ void __launch_bounds__(kThreads) gated_prep_kernel(const PrepArgs a)

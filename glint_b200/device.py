@@ -220,7 +220,7 @@ def htile_gated(x: torch.Tensor, hole: torch.Tensor, plug: torch.Tensor, absmax:
                 blocksize: int = 64, mode="precise", act: str = "silu", out=None, stream=None) -> torch.Tensor:
     """h[M, F] = act(x @ Wg^T) * (x @ Wu^T) in BF16, the planes those of the [2 F, K] weight with Wg's and
     Wu's rows in turn (pack_gated).  act: "silu" or "gelu_tanh"; mode: "precise" as htile's, or "fast", weights
-    and x as one FP16 value each (2^-12 of a weight); both products in f32 up to the activation.  Its workspace
+    and x as one FP16 value each (2^-11 of a weight); both products in f32 up to the activation.  Its workspace
     (glint_htile_gated_work_bytes) is of x's size and, fast from 769 rows on, 4 F K bytes more for as long."""
     for t, nm in ((x, "x"), (hole, "hole"), (plug, "plug"), (absmax, "absmax")):
         _cuda(t, nm)

@@ -62,11 +62,12 @@ int glint_htile_stream(
  *   GLINT_ACT_SILU       act(g) = g / (1 + exp(-g))
  *   GLINT_ACT_GELU_TANH  act(g) = g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2
  * x BF16 [M, K], h BF16 [M, F], row-major; h overlaps nothing else.  mode: GLINT_HTILE_PRECISE as above, or
- * GLINT_HTILE_FAST, weights and x as one FP16 value each (relative error <= 2^-12 per weight; rows are
+ * GLINT_HTILE_FAST, weights and x as one FP16 value each (relative error <= 2^-11 per weight; rows are
  * brought into FP16's range by powers of two, so x keeps its BF16 bits down to 2^-29 of a row's largest
- * finite value).  Any M, F, K, blocksize and pointer alignment is accepted; blocksize 64, K % 256 == 0 and
- * 16-byte aligned pointers take the streaming and tensor-core kernels, others kernels that do the same in
- * either mode, with BF16 halves (blocksize and K multiples of 64) or in f32.
+ * finite value, and weights their 11 bits down to 2^-29 of a row's largest absmax).  Any M, F, K, blocksize
+ * and pointer alignment is accepted; blocksize 64, K % 256 == 0 and 16-byte aligned pointers take the
+ * streaming and tensor-core kernels, others kernels that do the same in either mode, with BF16 halves
+ * (blocksize and K multiples of 64) or in f32.
  * work: glint_htile_gated_work_bytes() of 16-byte aligned device memory (by sizes, mode, alignment and the
  * current device; 0: NULL will do), the call's own until it completes, of any content; -1
  * for arguments that the call itself refuses.  In fast mode that is x again and, from 769 rows on, 4 F K bytes for

@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_gated import D, check, gen, gpu, kernel_error, planes  # noqa: E402,F401
+from test_gpu_gated import D, act, check, gen, gpu, kernel_error, planes, weights, within  # noqa: E402,F401
 
 WAYS = [(800, 512, 2400), (1100, 256, 2000), (90, 1024, 130)]  # expanded: with a cut rest, without; few tiles
 
@@ -97,3 +97,23 @@ def test_streams_and_graphs(M, K, F):
         torch.cuda.synchronize()
         assert all(torch.equal(o.view(torch.int16), b.view(torch.int16)) for two, b in zip(outs, want) for o in two)
     assert kernel_error() == 0
+
+
+@pytest.mark.parametrize("M,K,F", WAYS + [(20, 512, 300), (300, 512, 1000)])
+def test_blocks_of_other_sizes(M, K, F):
+    """Blocks of a row whose absmax differ by up to 2^24: each weight keeps its FP16 rounding, 2^-11 of itself."""
+    g = gen(M + 1)
+    hole, plug, am = planes(2 * F, K, 64, g)
+    am = torch.exp2(-24 * torch.rand(am.shape, device="cuda", generator=g))
+    # activations that lift the small blocks to the others' height, so that their errors would show
+    x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+    am.view(2 * F, -1)[:, 1:] = am.view(2 * F, -1)[:, 1:] * 2.0 ** -10
+    x[:, 64:] *= 2.0 ** 10
+    h = D().htile_gated(x, hole, plug, am, F, mode="fast")
+    w = weights(hole, plug, am, 2 * F, K, 64, "f32")
+    y, s = x.double() @ w.T, x.double().abs() @ w.abs().T
+    off = (2.0 ** -11 + (K / 16 + 8) * 2.0 ** -22) * s
+    gate, up, dg, du = y[:, 0::2], y[:, 1::2], off[:, 0::2], off[:, 1::2]
+    a = act(gate, "silu")
+    bound = 1.13 * dg * (up.abs() + du) + a.abs() * du + (2.0 ** -8 + 2.0 ** -16) * (a * up).abs() + 1e-36 * (1 + up.abs())
+    within(h, a * up, bound)
