@@ -201,6 +201,19 @@ def _head_dim(d: int) -> None:
         raise ValueError(f"head_dim must be 64 or 128, not {d}")
 
 
+# of a model's rope_scaling: what each rope_type reads, and what changes nothing (the original length alone only
+# says when to stretch, short_factor and long_factor are what `factors` was taken from)
+_ROPE_KEYS = {
+    "default": {"original_max_position_embeddings"},
+    "linear": {"factor", "original_max_position_embeddings"},
+    "llama3": {"factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor", "mscale",
+             "mscale_all_dim", "truncate"},
+    "longrope": {"factors", "factor", "original_max_position_embeddings", "attention_factor", "short_factor", "long_factor"},
+}
+_ROPE_INERT = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "finetuned"}
+
+
 def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
                device="cuda") -> Tuple[torch.Tensor, float]:
     """(inv_freq [rotary_dim / 2] f32, scale) for rope: base ** (-2 i / rotary_dim), stretched for contexts
@@ -212,18 +225,30 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
     llama3    wavelengths over original_max_position_embeddings / low_freq_factor divided by `factor`,
               those under .. / high_freq_factor kept, between them a ramp over their turns
     yarn      frequencies of fewer than beta_slow (1) turns in the original length divided by `factor`,
-              those of more than beta_fast (32) kept, between them a ramp over their numbers; scale
-              attention_factor, or 0.1 ln(factor) + 1
+              those of more than beta_fast (32) kept, between them a ramp over their numbers, whose ends
+              are whole numbers unless truncate is False; scale attention_factor, or with mscale
+              and mscale_all_dim m(mscale) / m(mscale_all_dim), or m(1), m(s) = 0.1 s ln(factor) + 1
     longrope  each divided by its own of `factors` (a model's short_factor or long_factor); scale
-              attention_factor, or with `factor` sqrt(1 + ln(factor) / ln(original length))"""
+              attention_factor, or with `factor` sqrt(1 + ln(factor) / ln(original length)), or 1
+
+    rotary_dim is the part of a head that is rotated, partial_rotary_factor included; rope_theta, where
+    `scaling` has it, must be `base`.  A key that the kind does not read and that could change the
+    result raises ValueError; keys whose value is None count as absent."""
     if rotary_dim < 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even, not {rotary_dim}")
     if not base > 0:
         raise ValueError(f"base must be above 0, not {base}")
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
     freq = base ** (-2 * i / max(rotary_dim, 1))
-    scaling = dict(scaling or {})
+    scaling = {key: v for key, v in (scaling or {}).items() if v is not None}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _ROPE_KEYS:
+        raise ValueError(f"rope_type must be default, linear, llama3, yarn or longrope, not {kind!r}")
+    unread = sorted(set(scaling) - _ROPE_KEYS[kind] - _ROPE_INERT)
+    if unread:
+        raise ValueError(f"rope_type {kind!r} does not read {', '.join(map(repr, unread))}")
+    if scaling.get("rope_theta", base) != base:
+        raise ValueError(f"base is {base}, but 'rope_theta' {scaling['rope_theta']}")
 
     def of(key, *default):
         v = scaling.get(key)
@@ -249,11 +274,19 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
 
         def number(turns):  # of the frequency that makes so many turns
             return rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
-        low = max(math.floor(number(of("beta_fast", 32.0))), 0)
-        high = min(math.ceil(number(of("beta_slow", 1.0))), rotary_dim - 1)
+        low, high = number(of("beta_fast", 32.0)), number(of("beta_slow", 1.0))
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         keep = 1 - ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq * (keep + (1 - keep) / factor)
-        scale = of("attention_factor", 0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
+
+        def magnitude(by):
+            return 0.1 * by * math.log(factor) + 1 if factor > 1 else 1.0
+        if ("mscale" in scaling) != ("mscale_all_dim" in scaling):
+            raise ValueError("'mscale' and 'mscale_all_dim' go together")
+        scale = of("attention_factor", magnitude(of("mscale", 1.0)) / magnitude(of("mscale_all_dim"))
+                   if "mscale_all_dim" in scaling else magnitude(1.0))
     elif kind == "longrope":
         factors = torch.tensor(scaling.get("factors") or [], dtype=torch.float64)
         if factors.shape != freq.shape or not bool((factors > 0).all()):
@@ -262,8 +295,6 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
         by = of("factor", 1.0)
         scale = of("attention_factor", math.sqrt(1 + math.log(by) / math.log(of("original_max_position_embeddings")))
                    if by > 1 else 1.0)
-    elif kind != "default":
-        raise ValueError(f"rope_type must be default, linear, llama3, yarn or longrope, not {kind!r}")
     return freq.float().to(device), scale
 
 
