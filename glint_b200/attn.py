@@ -324,13 +324,14 @@ def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _outputs_apart(q, k, q_out, k_out, more) -> None:
     """Outputs that the caller gave lie in their own input's place or touch no input, nor one another."""
-    for o, name, own in ((q_out, "q_out", q), (k_out, "k_out", k)):
+    inputs = (q, k, *more)
+    for own, (o, name) in enumerate(((q_out, "q_out"), (k_out, "k_out"))):
         if o is None:
             continue
         if not _heads_apart(o):
             raise ValueError(f"the heads of {name} overlap one another")
-        for x in (q, k, *more):
-            if x is not None and not (x is own and x.data_ptr() == o.data_ptr() and x.stride() == o.stride()) and \
+        for i, x in enumerate(inputs):  # by place: one tensor may be both q and k
+            if x is not None and not (i == own and x.data_ptr() == o.data_ptr() and x.stride() == o.stride()) and \
                     not _rows_apart(o, x):
                 raise ValueError(f"{name} must be {name[0]} itself or apart from q, k and v, which it may overlap")
     if k_out is not None and q_out is not None and not _rows_apart(q_out, k_out):
