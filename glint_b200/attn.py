@@ -307,7 +307,7 @@ def _heads_apart(t: torch.Tensor) -> bool:
 
 def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Two [tokens, heads, head_dim] tensors of one type surely share no element: their spans do
-    not meet, or they are different heads of one buffer's tokens."""
+    not meet, or they are different heads of one buffer's tokens, beside one another or in turn."""
     (T, Ha, D), (sa, ha, _) = a.shape, a.stride()
     (Tb, Hb, _), (sb, hb, _) = b.shape, b.stride()
     if not (T and Ha and Tb and Hb):
@@ -316,9 +316,17 @@ def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     pa, pb = a.data_ptr(), b.data_ptr()
     if pa + ((T - 1) * sa + ea) * size <= pb or pb + ((Tb - 1) * sb + eb) * size <= pa:
         return True
-    if sa != sb or (pb - pa) % size:
+    if (pb - pa) % size:
         return False
-    off = (pb - pa) // size % sa if sa else 0
+    off = (pb - pa) // size
+    # in turn: of every `turn` places a has the first D and b those from off % turn on
+    turn = ha if Ha > 1 else hb if Hb > 1 else 0
+    if turn and (Ha == 1 or ha == turn) and (Hb == 1 or hb == turn) and (T == 1 or sa % turn == 0) and \
+            (Tb == 1 or sb % turn == 0) and D <= off % turn <= turn - D:
+        return True
+    if sa != sb:
+        return False
+    off = off % sa if sa else 0
     return ea <= off and off + eb <= sa
 
 

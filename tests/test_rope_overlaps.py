@@ -20,3 +20,44 @@ def test_one_tensor_as_queries_and_keys():
     apart(t, t, None, other, ())
     apart(t, other, t, other, ())
     apart(t, None, t, None, ())
+
+
+def places(t):
+    base = t.storage_offset()
+    T, H, D = t.shape
+    return {base + i * t.stride(0) + h * t.stride(1) + d for i in range(T) for h in range(H) for d in range(D)}
+
+
+def test_heads_in_turn():
+    """A fused buffer with each head's query, key and value side by side: they share nothing, and are taken in place."""
+    from glint_b200 import attn
+    for T, H in ((5, 4), (1, 4), (5, 1), (1, 1)):
+        y = torch.zeros(T, H, 3, 64, dtype=torch.bfloat16)
+        q, k, v = (y[:, :, i] for i in range(3))
+        apart(q, k, q, k, (v,))
+        apart(q, k, q, None, (v,))
+        apart(q, k, v, None, ())
+        with pytest.raises(ValueError):
+            apart(q, k, k, None, (v,))
+        with pytest.raises(ValueError):
+            apart(q, k, q, v, (v,))
+    # groups of two queries and a key: the first queries of the groups beside the keys
+    y = torch.zeros(5, 4, 3, 64, dtype=torch.bfloat16)
+    assert attn._rows_apart(y[:, :, 0], y[:, :, 2]) and attn._rows_apart(y[:, ::2, 0], y[:, 1::2, 0])
+    assert not attn._rows_apart(y[:, :, 0], y[:, ::2, 0]) and not attn._rows_apart(y[:, 0], y[:, :, 0])
+
+
+def test_every_answer_apart_is_right():
+    from glint_b200 import attn
+    store = torch.zeros(400, dtype=torch.int16)
+    views = [store.as_strided((T, H, 4), (st, sh, 1), off) for T in (1, 2, 3) for H in (1, 2, 3)
+             for st, sh in ((24, 8), (24, 12), (12, 24), (8, 8), (20, 8), (16, 8), (0, 8), (8, 0), (36, 12), (4, 12), (7, 12))
+             for off in (0, 1, 4, 8, 12, 20, 33)]
+    where = [places(v) for v in views]
+    said = 0
+    for a, pa in zip(views, where):
+        for b, pb in zip(views, where):
+            if attn._rows_apart(a, b):
+                said += 1
+                assert not pa & pb, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert said > 10000
