@@ -347,6 +347,7 @@ def _outputs_apart(q, k, q_out, k_out, more) -> None:
 
 
 _DENSE = torch.contiguous_format
+_LEAST_EPS = 2.0 ** -250  # below, a head of zeros would have an infinite 1 / sqrt(eps) in f32
 
 
 def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream, more, keys):
@@ -380,8 +381,8 @@ def _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_
         if w is not None:
             _want(w, name, torch.float32, (D,))
             _want16(w, name)
-    if not (eps > 0 and math.isfinite(eps) and math.isfinite(scale)):
-        raise ValueError(f"eps must be above 0 and scale finite, not {eps} and {scale}")
+    if not (eps >= _LEAST_EPS and math.isfinite(eps) and math.isfinite(scale)):
+        raise ValueError(f"eps must be 2^-250 or more and scale finite, not {eps} and {scale}")
     if q_out is not None or k_out is not None:
         for o, shape, name in ((q_out, (T, H, D), "q_out"), (k_out, (T, Hk, D), "k_out")):
             if o is not None:

@@ -36,6 +36,7 @@ namespace glint {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr double kLeastEps = 0x1p-250; /* r of a head of zeros is a number in f32 */
 /* where a value's partner is: R / 2 places on, in whole runs of 8 or not; beside it */
 enum Pairing : int { kRuns, kAny, kBeside };
 
@@ -371,7 +372,8 @@ int check(const GlintRope *a, bool keys)
         return kBadArg;
     if (a->head_dim != 64 && a->head_dim != 128)
         return kUnsupported;
-    if (a->tokens < 0 || a->heads < 1 || a->kv_heads < 0 || a->half < 0 || a->half > a->head_dim / 2 || !(a->eps > 0.) ||
+    if (a->tokens < 0 || a->heads < 1 || a->kv_heads < 0 || a->half < 0 || a->half > a->head_dim / 2 ||
+        !(a->eps >= kLeastEps) ||
         (int64_t)a->heads + 2 * (int64_t)a->kv_heads > INT32_MAX / 4)
         return kBadArg;
     if (a->tokens == 0)

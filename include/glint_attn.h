@@ -38,7 +38,7 @@ extern "C" {
  *       interleaved; places from 2 half on are y.  0 <= half <= head_dim / 2.
  * Angles and r are computed in 64 bits and rounded to f32, products and sums of y, c and s
  * are rounded to f32 one by one and o once to BF16.  positions device int32, inv_freq
- * device f32; scale and eps in 64 bits, eps > 0.  q_out may be q itself (the same strides),
+ * device f32; scale and eps in 64 bits, eps >= 2^-250.  q_out may be q itself (the same strides),
  * k_out k; otherwise outputs overlap no input.  16-byte aligned tensors with
  * strides that are multiples of 8 are read and written 16 bytes at a time. */
 typedef struct GlintRope {

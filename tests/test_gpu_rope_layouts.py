@@ -44,3 +44,14 @@ def test_one_tensor_as_queries_and_keys():
     assert torch.equal(bits(t), bits(kept))
     a, b = A().rope(t, t, at, freqs(32))
     assert torch.equal(bits(a), bits(b))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_heads_of_zeros_with_the_least_eps(dim):
+    x = torch.zeros(3, 4, dim, dtype=torch.bfloat16, device="cuda")
+    at, w = torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(dim, device="cuda")
+    for eps in (2.0 ** -250, 1e-30):
+        q, k = A().rope(x, x, at, freqs(dim // 2), q_norm=w, k_norm=w, eps=eps)
+        assert bool((q == 0).all()) and bool((k == 0).all())
+    with pytest.raises(ValueError, match="eps"):
+        A().rope(x, x, at, freqs(dim // 2), q_norm=w, eps=1e-80)
