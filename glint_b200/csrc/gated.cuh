@@ -8,7 +8,9 @@
 namespace glint {
 
 /* What the H-TILE kernels' gated epilogues take.  Against activations in FP16 (see htile_gated.cu) a product's sums
- * are of x[m] / x_scale[m] and, where weights carry their absmax into the tensor cores, of W[n] * row_scale[n]. */
+ * are of x[m] / x_scale[m] and, where weights carry their absmax into the tensor cores, of W[n] * row_scale[n].  Both
+ * are written by the kernel before, beside which the products may already run: behind griddepcontrol.wait they are read by
+ * plain loads, never as data that stays the same for the kernel's whole life (__ldg, a const __restrict__ pointer). */
 struct GatedEpilogue {
     int act;
     const float *x_scale;   /* [M] powers of two */

@@ -387,7 +387,7 @@ __device__ __forceinline__ void gated_outputs_of(const uint32_t (&v)[R], bool up
     for (int i = 0; i < R / 4; ++i) {
         float4 x = make_float4(1.f, 1.f, 1.f, 1.f);
         if (x_scale)
-            x = __ldg(reinterpret_cast<const float4 *>(x_scale + m + 4 * i));
+            x = *reinterpret_cast<const float4 *>(x_scale + m + 4 * i);
         float h[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -648,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
         for (Segments sg = seg0; alive && sg.next(args, pair, npairs, T, ga, gb);) {
             [[maybe_unused]] float row_scale = 1.f;
             if constexpr (GATED)
-                row_scale = __ldg(args.ep.row_scale + min((T / args.mtiles) * (2 * BN) + (int)rank * BN + r, args.N - 1));
+                row_scale = args.ep.row_scale[min((T / args.mtiles) * (2 * BN) + (int)rank * BN + r, args.N - 1)];
             for (int ks = ga * PSTEPS + group; ks < gb * PSTEPS && alive; ks += C::kGroups, onward()) {
                 const int j = ks & (PSTEPS - 1);
                 if (j == group && !warp_wait(&p_full[st.i], st.ph, alive))
@@ -725,9 +725,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             const int mlim = min(BMX, args.M - m0);
             [[maybe_unused]] float row_back = 1.f; /* 1 / row_scale[n], a power of two */
             if constexpr (GATED) {
-                row_back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
+                row_back = __uint_as_float((254u << 23) - __float_as_uint(args.ep.row_scale[min(n, args.N - 1)]));
                 /* the tile's x_scale into L1 while the products run */
-                asm volatile("" ::"f"(__ldg(args.ep.x_scale + m0 + (lane & 7) * 32)));
+                asm volatile("" ::"f"(args.ep.x_scale[m0 + (lane & 7) * 32]));
             }
             if (!warp_wait(acc_full, (uint32_t)t & 1u, alive))
                 break;
@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const GemmArgs a)
                     acc[j] += v[b][j];
             }
     }
-    const float back = __uint_as_float((254u << 23) - __float_as_uint(__ldg(a.ep.row_scale + min(n, a.N - 1))));
+    const float back = __uint_as_float((254u << 23) - __float_as_uint(a.ep.row_scale[min(n, a.N - 1)]));
     uint32_t v[kJoinRows], o[kJoinRows / 4];
 #pragma unroll
     for (int j = 0; j < kJoinRows; ++j)
@@ -1039,7 +1039,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
             const int mlim = args.M - m0;
             /* 1 / row_scale[n], a power of two */
             const float back =
-                __uint_as_float((254u << 23) - __float_as_uint(__ldg(args.ep.row_scale + min(n, args.N - 1))));
+                __uint_as_float((254u << 23) - __float_as_uint(args.ep.row_scale[min(n, args.N - 1)]));
             if (!warp_wait(&acc_full[acc.i], acc.ph, alive))
                 break;
             tc_fence_after();
