@@ -253,14 +253,25 @@ struct Ring {
             i = 0, ph ^= 1u;
     }
 };
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-/* the loads into r have arrived: its values are this statement's, so no use moves ahead of it */
+/* The loads into r have arrived: its values are this statement's, so no use moves ahead of it.  (A wait that
+ * names no register orders memory alone, not arithmetic on what an earlier asm statement gave.) */
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16])
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
                    "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :
                  : "memory");
 }
@@ -738,7 +749,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
                 for (int c = c0; c < BMX / 32 && c * 32 < mlim; c += cs) {
                     uint32_t v[32];
                     tmem_ld32(tb + c * 32, v);
-                    tmem_ld_wait();
+                    tmem_ld_wait(v);
                     if constexpr (GATED) {
                         uint32_t o[8];
                         gated_outputs(v, n & 1, args.ep, row_back, m0 + c * 32, o);
@@ -766,7 +777,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             for (int c = c0; c < BMX / 32 && (!GATED || c * 32 < mlim); c += cs) {
                 uint32_t v[32];
                 tmem_ld32(tb + c * 32, v);
-                tmem_ld_wait();
+                tmem_ld_wait(v);
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     __stcg(mine + (c * 32 + j) * 32 + lane, __uint_as_float(v[j]));
@@ -1060,7 +1071,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
                 for (int c = 0; c < BMX / 2 && c < mlim; c += 32) {
                     uint32_t v[32];
                     tmem_ld32(ta + c, v);
-                    tmem_ld_wait();
+                    tmem_ld_wait(v);
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         __stcg(mine + (c + j) * 32, __uint_as_float(v[j]));
@@ -1369,7 +1380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PThreads, 1)
                 for (int h = 0; h < 2; ++h) {
                     uint32_t v[16];
                     tmem_ld16(tb + (uint32_t)b * PBMX + (uint32_t)h * 16u, v);
-                    tmem_ld_wait();
+                    tmem_ld_wait(v);
 #pragma unroll
                     for (int jj = 0; jj < 16; ++jj)
                         run[h * 16 + jj] = fmaf(s, __uint_as_float(v[jj]), run[h * 16 + jj]);
@@ -1761,7 +1772,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Cfg<PLUG>::kThread
                     const uint64_t sw2 = pack2u(__float_as_uint(wsf), __float_as_uint(wsf));
                     uint32_t v[IEpiCols];
                     tmem_ld32(tb + (uint32_t)(b * C::kSlotCols + term * IBMX), v);
-                    tmem_ld_wait();
+                    tmem_ld_wait(v);
                     if (term == (PLUG ? 1 : 0)) {
                         tc_fence_before();
                         __syncwarp();

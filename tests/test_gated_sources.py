@@ -22,3 +22,22 @@ def test_scales_are_not_read_as_constant():
                 at += 1
             assert not re.search(r"x_scale|row_scale", text[m.end():at]), f"{path.name}: {text[m.start():at]}"
         assert not re.search(r"__restrict__\s+(x_scale|row_scale)", text), path.name
+
+
+def test_waits_for_tensor_memory_name_the_registers():
+    """A wait for tcgen05.ld that names no register lets arithmetic on the loaded values move ahead of it."""
+    text = source("htile_gemm.cu")
+    calls = re.findall(r"(tmem_ld16|tmem_ld32|tmem_ld_wait)\s*\(([^;{]*)\)\s*;", text)
+    assert len([c for c in calls if c[0] == "tmem_ld_wait"]) >= 6
+    waiting = None
+    for name, args in calls:
+        last = args.split(",")[-1].strip()
+        if name == "tmem_ld_wait":
+            assert waiting and last == waiting, (name, args, waiting)
+            waiting = None
+        else:
+            assert waiting is None, (name, args)
+            waiting = last
+    assert waiting is None
+    for m in re.finditer(r"tcgen05\.wait::ld[^;]*;\"\s*:([^:]*):", text):
+        assert '"+r"' in m.group(1), m.group(0)
