@@ -110,7 +110,8 @@ int htile_decode_gather_launch(const uint8_t *hole, const uint8_t *plug, const f
 /* h[M, N / 2] BF16 = act(y[:, 2i]) * y[:, 2i + 1], y as of htile_launch (N even; gated.cuh, htile_gated.cu): M <= 32
  * and any M of the TMA kernels' shapes (bs == 64, K % 256 == 0, 16-byte alignment), and all others.  The first
  * two take x as it is in precise mode and in FP16 (htile_gated.cu) in fast mode; .._work(): the bytes of
- * `sums` that they need for tiles split among CTAs, and how many `counts`, zero at the start. */
+ * `sums` that they need for tiles split among CTAs (-1 where the device does not tell how many fit), and how many
+ * `counts`, zero at the start. */
 struct GatedEpilogue;
 int64_t htile_decode_gated_work(int M, int N, int K, int64_t *counts);
 int htile_decode_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *absmax, const __nv_bfloat16 *x,

@@ -222,7 +222,7 @@ bool streams(const GlintHtileGated &a)
 struct Layout {
     bool half = false; /* x in FP16 */
     bool wide = false; /* W in FP16 */
-    int64_t x16 = 0, w16 = 0, x_scale = 0, row_scale = 0, sums = 0, counts = 0, n_counts = 0, bytes = 0;
+    int64_t x16 = 0, w16 = 0, x_scale = 0, row_scale = 0, sums = 0, counts = 0, n_counts = 0, bytes = 0; /* -1: unknown */
     explicit Layout(const GlintHtileGated &a)
     {
         const int N = 2 * a.F;
@@ -246,6 +246,10 @@ struct Layout {
                           : wide ? htile_gated_wide_work(a.M, N, a.K)
                           : half ? htile_gemm_gated_work(a.M, N, a.K, &n_counts)
                                  : 0;
+        if (s < 0) {
+            bytes = -1;
+            return;
+        }
         sums = take(s), counts = take(n_counts * (int64_t)sizeof(int));
     }
 };
@@ -296,6 +300,8 @@ int glint_htile_gated_stream(const GlintHtileGated *a, cudaStream_t stream)
         return htile_gemv_gated_launch(a->hole, a->plug, a->absmax, a->x, a->h, a->M, N, a->K, a->blocksize, a->act,
                                        stream);
     const Layout at(*a);
+    if (at.bytes < 0)
+        return kLaunch;
     if (at.bytes > 0 && (!a->work || !aligned_to(a->work, 16)))
         return kBadArg;
     char *work = static_cast<char *>(a->work);

@@ -1925,14 +1925,24 @@ bool gemm_scratch(cudaStream_t st, size_t ws_floats, size_t n_counters, float **
     return true;
 }
 
-/* CTA pairs of `kernel` that fit on the device at once (one pair per two SMs at
- * most); cached per device and kernel kind (0 fast, 1 precise, 2 int8) */
-int max_pairs(int kind = 0)
+/* CTA pairs of a kernel that fit on the device at once (one pair per two SMs at most), kept per device;
+ * 0, not kept, where the device does not tell: a number in its place could differ between a workspace's query and the
+ * call.  The kernel's limit of dynamic shared memory is raised before the query, which finds no room for a pair otherwise. */
+enum PairKernel : int { kPairsFast, kPairsPrecise, kPairsInt8, kPairsGated, kPairsWide, kPairKernels };
+int max_pairs(PairKernel kind)
 {
-    static int cached[64][3] = {};
+    static int cached[64][kPairKernels] = {};
+    struct {
+        const void *kernel;
+        int threads, smem;
+    } const of[kPairKernels] = {{(const void *)htile_gemm_kernel<false>, GemmCfg<false>::kThreads, kSmemBytes},
+                                {(const void *)htile_gemm_precise_kernel<false>, PThreads, PSmemBytes},
+                                {(const void *)int8_tc_kernel<false>, I8Cfg<false>::kThreads, I8Cfg<false>::kSmem},
+                                {(const void *)htile_gemm_kernel<true>, GemmCfg<true>::kThreads, kSmemBytes},
+                                {(const void *)gated_wide_kernel, kWideThreads, kWideSmem}};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return std::max(1, sm_count() / 2);
+        return 0;
     if (cached[dev][kind] > 0)
         return cached[dev][kind];
     int n = 0;
@@ -1941,19 +1951,16 @@ int max_pairs(int kind = 0)
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2 * std::max(1, sm_count() / 2));
-    cfg.blockDim = dim3(kind == 2 ? I8Cfg<false>::kThreads : kind ? PThreads : GemmCfg<false>::kThreads);
-    cfg.dynamicSmemBytes = kind == 2 ? I8Cfg<false>::kSmem : kind ? PSmemBytes : kSmemBytes;
+    cfg.blockDim = dim3(of[kind].threads);
+    cfg.dynamicSmemBytes = of[kind].smem;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const void *kern = kind == 2   ? (const void *)int8_tc_kernel<false>
-                       : kind == 1 ? (const void *)htile_gemm_precise_kernel<false>
-                                   : (const void *)htile_gemm_kernel<false>;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    if (!ensure_smem(of[kind].kernel, of[kind].smem) ||
+        cudaOccupancyMaxActiveClusters(&n, of[kind].kernel, &cfg) != cudaSuccess || n <= 0) {
         cudaGetLastError();
-        n = std::max(1, sm_count() / 2);
+        return 0;
     }
-    cached[dev][kind] = n;
-    return n;
+    return cached[dev][kind] = n;
 }
 } // namespace
 
@@ -1964,14 +1971,16 @@ namespace {
  * after which whole rounds follow (their sums overlap whole tiles); between one and
  * two rounds, the tiles beyond one round (e.g. 512 x 14336: 112 tiles on 74 pairs,
  * 86.8 -> 76.9 us; sharing all tiles instead cost more in split-tile sums than it
- * saved). */
+ * saved).  Returns the pairs, or 0 (see max_pairs()). */
 int gemm_plan(GemmArgs &a, bool gated = false)
 {
     a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
     a.G = a.K / (PSTEPS * BK), a.group = a.mtiles;
     a.half = !gated || a.M > 128 ? BMH : a.M > 64 ? 64 : 32;
     const int tiles = a.mtiles * a.ntiles;
-    const int maxp = max_pairs();
+    const int maxp = max_pairs(gated ? kPairsGated : kPairsFast);
+    if (!maxp)
+        return 0;
     if (gated && tiles * 2 <= maxp) {
         /* No tile for half of the pairs: K is cut for all tiles, down to one group a pair, and gated_join_kernel adds.
          * Uncut and cut: 98 x 6656 x 2 x 174 (2 tiles) 63 and 30 us; 64 x 4096 x 2 x 4096 (32 tiles) 45 and 36;
@@ -1997,7 +2006,10 @@ int wide_plan(GemmArgs &a)
     a.mtiles = (a.M + BMX - 1) / BMX, a.ntiles = (a.N + 2 * BN - 1) / (2 * BN);
     a.G = a.K / (PSTEPS * BK), a.group = std::min(a.mtiles, kWideGroup);
     a.tiles = a.mtiles * a.ntiles;
-    const int pairs = std::min(a.tiles, max_pairs()), left = a.tiles % pairs;
+    const int pairs = std::min(a.tiles, max_pairs(kPairsWide));
+    if (!pairs)
+        return 0;
+    const int left = a.tiles % pairs;
     const bool cut = left && (pairs - left) * 50 > a.tiles;
     a.S = cut ? left : 0, a.U = a.S * a.G, a.P = std::max(1, std::min(pairs, a.U)), a.join = cut;
     a.R = cut ? a.tiles / pairs : (a.tiles + pairs - 1) / pairs;
@@ -2029,7 +2041,7 @@ int gemm_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *am, 
     if (ga)
         a.ga = *ga;
     const int pairs = gemm_plan(a);
-    if (!gemm_scratch(st, part_floats(pairs), (size_t)a.tiles * 8, &a.ws, &a.counters))
+    if (!pairs || !gemm_scratch(st, part_floats(pairs), (size_t)a.tiles * 8, &a.ws, &a.counters))
         return kLaunch;
     htile_gemm_kernel<false><<<2 * pairs, GemmCfg<false>::kThreads, kSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
@@ -2054,7 +2066,7 @@ int precise_launch_impl(const uint8_t *hole, const uint8_t *plug, const float *a
     a.y = y, a.am = am, a.M = M, a.N = N, a.K = K, a.y_bf16 = y_bf16 ? 1 : 0, a.ep = ep;
     a.mtiles = (M + PBMX - 1) / PBMX;
     a.tiles = a.mtiles * ((N + 2 * BN - 1) / (2 * BN));
-    const int pairs = std::max(1, std::min(a.tiles, max_pairs(1)));
+    const int pairs = std::max(1, std::min(a.tiles, max_pairs(kPairsPrecise)));
     htile_gemm_precise_kernel<GATED><<<2 * pairs, PThreads, PSmemBytes, st>>>(maps, a);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunch;
 }
@@ -2092,6 +2104,8 @@ int64_t htile_gemm_gated_work(int M, int N, int K, int64_t *counts)
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
     const int pairs = gemm_plan(a, true);
+    if (!pairs)
+        return -1;
     *counts = a.join ? 0 : (int64_t)a.S * 2 * GemmCfg<true>::kEpiWarps;
     return a.S ? (int64_t)(part_floats(pairs) * sizeof(float)) : 0;
 }
@@ -2104,7 +2118,7 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
     a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep;
     const int pairs = gemm_plan(a, true);
     Maps maps;
-    if (!gemm_maps(maps, hole, plug, am, x, M, N, K, a.half) ||
+    if (!pairs || !gemm_maps(maps, hole, plug, am, x, M, N, K, a.half) ||
         !ensure_smem((const void *)htile_gemm_kernel<true>, kSmemBytes))
         return kLaunch;
     a.ws = sums, a.counters = counts;
@@ -2130,13 +2144,15 @@ int htile_gemm_gated_launch(const uint8_t *hole, const uint8_t *plug, const floa
  * and 393, 8191 rows 2246 and 1515. */
 bool htile_gated_wide_takes(int M, int N)
 {
-    return M > 3 * BMX && (int64_t)((M + BMX - 1) / BMX) * ((N + 2 * BN - 1) / (2 * BN)) >= max_pairs();
+    return M > 3 * BMX && (int64_t)((M + BMX - 1) / BMX) * ((N + 2 * BN - 1) / (2 * BN)) >= max_pairs(kPairsWide);
 }
 int64_t htile_gated_wide_work(int M, int N, int K)
 {
     GemmArgs a{};
     a.M = M, a.N = N, a.K = K;
     const int pairs = wide_plan(a);
+    if (!pairs)
+        return -1;
     return a.S ? (int64_t)(part_floats(pairs) * sizeof(float)) : 0;
 }
 int htile_gated_wide_launch(const void *w, const void *x, void *h, float *sums, int M, int N, int K, GatedEpilogue ep,
@@ -2152,6 +2168,8 @@ int htile_gated_wide_launch(const void *w, const void *x, void *h, float *sums, 
     GemmArgs a{};
     a.y = h, a.M = M, a.N = N, a.K = K, a.y_bf16 = 1, a.ep = ep, a.ws = sums;
     const int pairs = wide_plan(a);
+    if (!pairs)
+        return kLaunch;
     gated_wide_kernel<<<2 * pairs, kWideThreads, kWideSmem, st>>>(maps, a);
     if (a.join)
         gated_join_kernel<<<a.S * (BMX / kJoinRows), 256, 0, st>>>(a);
@@ -2192,7 +2210,7 @@ cudaError_t int8_tc_gemm_launch(const int8_t *xq, const float *sx, const int8_t 
     a.sx = sx, a.sw = sw, a.ps = psc, a.y = y, a.M = M, a.N = N, a.K = K, a.accumulate = accumulate;
     a.mtiles = (M + IBMX - 1) / IBMX;
     a.tiles = a.mtiles * ((N + 2 * BN - 1) / (2 * BN));
-    const int pairs = std::max(1, std::min(a.tiles, max_pairs(2)));
+    const int pairs = std::max(1, std::min(a.tiles, max_pairs(kPairsInt8)));
     return pq4 ? int8_tc_launch_t<true>(maps, a, pairs, st) : int8_tc_launch_t<false>(maps, a, pairs, st);
 }
 

@@ -195,7 +195,10 @@ def _gated_calls() -> _GatedCalls:
 @lru_cache(maxsize=256)
 def _gated_work(dev: int, place: int, M: int, F: int, K: int, blocksize: int, mode: int) -> int:
     at = 16 + place
-    return _gated_calls().work(_pack_gated_args(at, at, at, at, at, 0, M, F, K, blocksize, mode, 0))
+    need = _gated_calls().work(_pack_gated_args(at, at, at, at, at, 0, M, F, K, blocksize, mode, 0))
+    if need < 0:  # raised, so that it is not kept
+        raise RuntimeError("glint_htile_gated_work_bytes: arguments refused, or the device does not answer")
+    return need
 
 
 def pack_gated(gate: Sequence[torch.Tensor], up: Sequence[torch.Tensor], F: int, K: int, blocksize: int = 64):

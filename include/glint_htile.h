@@ -70,7 +70,7 @@ int glint_htile_stream(
  * (blocksize and K multiples of 64) or in f32.
  * work: glint_htile_gated_work_bytes() of 16-byte aligned device memory (by sizes, mode, alignment and the
  * current device; 0: NULL will do), the call's own until it completes, of any content; -1
- * for arguments that the call itself refuses.  In fast mode that is x again and, from 769 rows on, 4 F K bytes for
+ * for arguments that the call itself refuses, or where the device does not answer.  In fast mode that is x again and, from 769 rows on, 4 F K bytes for
  * the weight in FP16 (235 MB for 2 x 14336 x 4096); sums of shared tiles take up to 39 MB besides. */
 #define GLINT_ACT_SILU 0
 #define GLINT_ACT_GELU_TANH 1

@@ -41,3 +41,17 @@ def test_waits_for_tensor_memory_name_the_registers():
     assert waiting is None
     for m in re.finditer(r"tcgen05\.wait::ld[^;]*;\"\s*:([^:]*):", text):
         assert '"+r"' in m.group(1), m.group(0)
+
+
+def test_pairs_are_counted_behind_the_kernels_own_limit():
+    """max_pairs(): a kernel's shared memory limit is raised before the device is asked how many fit, each kernel is
+    asked about itself, and a guess is not kept for the calls that follow."""
+    text = source("htile_gemm.cu")
+    body = text[text.index("int max_pairs("):]
+    body = body[:body.index("\n}\n")]
+    assert body.index("ensure_smem(") < body.index("cudaOccupancyMaxActiveClusters(")
+    kept = [line for line in body.splitlines() if re.search(r"cached\[dev\]\[kind\]\s*=[^=]", line)]
+    assert len(kept) == 1 and body.index(kept[0]) > body.rindex("cudaGetLastError()")
+    for kernel in ("htile_gemm_kernel<false>", "htile_gemm_kernel<true>", "gated_wide_kernel", "htile_gemm_precise_kernel<false>",
+                   "int8_tc_kernel<false>"):
+        assert kernel in body, kernel
