@@ -747,14 +747,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<GATED>::kThr
             if (whole) {
 #pragma unroll 1
                 for (int c = c0; c < BMX / 32 && c * 32 < mlim; c += cs) {
-                    uint32_t v[32];
-                    tmem_ld32(tb + c * 32, v);
-                    tmem_ld_wait(v);
                     if constexpr (GATED) {
-                        uint32_t o[8];
-                        gated_outputs(v, n & 1, args.ep, row_back, m0 + c * 32, o);
-                        store_gated(args.y, args.N, o, m0 + c * 32, mlim - c * 32, n);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t v[16], o[4];
+                            tmem_ld16(tb + c * 32 + h * 16, v);
+                            tmem_ld_wait(v);
+                            gated_outputs(v, n & 1, args.ep, row_back, m0 + c * 32 + h * 16, o);
+                            store_gated(args.y, args.N, o, m0 + c * 32 + h * 16, mlim - c * 32 - h * 16, n);
+                        }
                     } else {
+                        uint32_t v[32];
+                        tmem_ld32(tb + c * 32, v);
+                        tmem_ld_wait(v);
                         store_y(args, v, m0 + c * 32, min(32, mlim - c * 32), n, false);
                     }
                 }
