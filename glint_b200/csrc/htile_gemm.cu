@@ -387,8 +387,9 @@ __device__ __forceinline__ void store_rows(void *y, bool y_bf16, size_t step, co
 }
 /* Outputs of a gated product: pairs of lanes hold the columns n (even: gate) and n + 1 (up) of R
  * rows from m on.  Of two rows each lane of a pair keeps one: the even lane takes up of the first for gate of the
- * second.  o: R / 2 outputs, of rows 2i + (n & 1), as BF16 pairs.  What the sums are to be multiplied by: x_scale of
- * their row and `row` of their column. */
+ * second.  o: R / 2 outputs, of rows 2i + (n & 1), as BF16 pairs.  What the sums are to be multiplied by: `row` of
+ * their column, then x_scale of their row, one after the other: the two powers' own product may be past f32's range
+ * where the sum times either is not. */
 template <int ACT, int R>
 __device__ __forceinline__ void gated_outputs_of(const uint32_t (&v)[R], bool up, const float *x_scale, float row, int m,
                                                  uint32_t (&o)[R / 4])
@@ -405,7 +406,7 @@ __device__ __forceinline__ void gated_outputs_of(const uint32_t (&v)[R], bool up
             const float a = __uint_as_float(v[4 * i + 2 * j]), b = __uint_as_float(v[4 * i + 2 * j + 1]);
             const float got = __shfl_xor_sync(0xFFFFFFFFu, up ? a : b, 1);
             const float by = j ? (up ? x.w : x.z) : (up ? x.y : x.x);
-            h[j] = gated_value(by * by_g * (up ? got : a), by * by_u * (up ? b : got), ACT);
+            h[j] = gated_value(by_g * (up ? got : a) * by, by_u * (up ? b : got) * by, ACT);
         }
         const __nv_bfloat162 b2 = __floats2bfloat162_rn(h[0], h[1]);
         o[i] = *reinterpret_cast<const uint32_t *>(&b2);

@@ -64,7 +64,8 @@ int glint_htile_stream(
  * x BF16 [M, K], h BF16 [M, F], row-major; h overlaps nothing else.  mode: GLINT_HTILE_PRECISE as above, or
  * GLINT_HTILE_FAST, weights and x as one FP16 value each (relative error <= 2^-11 per weight; rows are
  * brought into FP16's range by powers of two, so x keeps its BF16 bits down to 2^-29 of a row's largest
- * finite value, and weights their 11 bits down to 2^-29 of a row's largest absmax).  Any M, F, K, blocksize
+ * finite value, and weights their 11 bits down to 2^-29 of a row's largest absmax; a row's largest absmax
+ * is below 2^90, for its sums to stay inside f32).  Any M, F, K, blocksize
  * and pointer alignment is accepted; blocksize 64, K % 256 == 0 and 16-byte aligned pointers take the
  * streaming and tensor-core kernels, others kernels that do the same in either mode, with BF16 halves
  * (blocksize and K multiples of 64) or in f32.
