@@ -7,7 +7,8 @@
  * largest finite value into [2^14, 2^15), exactly: every BF16 value down to 2^-29 of the largest keeps all its bits,
  * and what lies below is off by 2^-39 of the largest at most.  Where weights carry their absmax into the
  * products (more than 32 rows), so is each row of W by the one that brings its largest absmax into [2^14, 2^15) (no cell
- * is above 1; the sums of 2^30 at most stay far inside f32).
+ * is above 1; products of 2^30 at most, whose sums stay far inside f32): every weight down to 2^-28 of its row's largest
+ * absmax keeps its 11 bits, and what lies below is off by 2^-39 of that at most.
  * The epilogues divide by both, again exactly.  The pass is one small kernel (a row of x a CTA; 2.8 us for a token,
  * 25 for 8191 x 4096), beside which the next kernel's weights stream or are expanded.
  *

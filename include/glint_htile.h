@@ -64,15 +64,18 @@ int glint_htile_stream(
  * x BF16 [M, K], h BF16 [M, F], row-major; h overlaps nothing else.  mode: GLINT_HTILE_PRECISE as above, or
  * GLINT_HTILE_FAST, weights and x as one FP16 value each (relative error <= 2^-11 per weight; rows are
  * brought into FP16's range by powers of two, so x keeps its BF16 bits down to 2^-29 of a row's largest
- * finite value, and weights their 11 bits down to 2^-29 of a row's largest absmax; a row's largest absmax
- * is below 2^90, for its sums to stay inside f32).  Any M, F, K, blocksize
+ * finite value, and weights, with more than 32 rows of x, their 11 bits down to 2^-28 of their row's largest
+ * absmax, below which they are off by 2^-39 of that at most; a row's largest absmax is below 2^90, for its
+ * sums to stay inside f32).  Any M, F, K, blocksize
  * and pointer alignment is accepted; blocksize 64, K % 256 == 0 and 16-byte aligned pointers take the
  * streaming and tensor-core kernels, others kernels that do the same in either mode, with BF16 halves
  * (blocksize and K multiples of 64) or in f32.
  * work: glint_htile_gated_work_bytes() of 16-byte aligned device memory (by sizes, mode, alignment and the
  * current device; 0: NULL will do), the call's own until it completes, of any content; -1
- * for arguments that the call itself refuses, or where the device does not answer.  In fast mode that is x again and, from 769 rows on, 4 F K bytes for
- * the weight in FP16 (235 MB for 2 x 14336 x 4096); sums of shared tiles take up to 39 MB besides. */
+ * for arguments that the call itself refuses, or where the device does not answer.  In fast mode that is x
+ * again and, from 769 rows on, 4 F K bytes for the weight in FP16 (235 MB for 2 x 14336 x 4096).  Sums of shared
+ * tiles take up to 39 MB besides with more than 32 rows; with fewer, in either mode, up to 10 MB for K above 8192 or
+ * up to 780 F bytes for 2 F above 224 rows an SM (66 MB for 2 x 128256). */
 #define GLINT_ACT_SILU 0
 #define GLINT_ACT_GELU_TANH 1
 typedef struct GlintHtileGated {

@@ -48,3 +48,21 @@ def test_order_of_first_calls():
             got.setdefault(part, []).append([line for line in lines[at[part] + 1:end] if line])
     for part, (a, b) in got.items():
         assert a == b and len(a) == 4, part
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("M,K,F", [(1, 4096, 14336), (32, 4096, 128256), (9, 8192, 28672), (32, 12544, 384), (32, 33280, 50), (16, 256, 18001),
+                                   (33, 4096, 14336), (511, 4096, 14336), (98, 6656, 174), (900, 4096, 14336), (2311, 768, 1021)])
+def test_workspace_is_as_large_as_documented(M, K, F, mode):
+    from glint_b200 import device
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    need = device._gated_work.__wrapped__(0, 0, M, F, K, 64, mode)
+    copies = 2 * M * K + 8 * F + 1024 if mode else 0  # x in FP16, scales of its rows
+    if mode and M > 32:
+        copies += 8 * F
+    if mode and M > 768 and need > 4 * F * K:
+        copies += 4 * F * K
+    sums = 780 * F if 2 * F > 224 * sms else 10e6
+    if M > 32:
+        sums = 39e6 if mode else 0
+    assert need <= copies + sums + 64 * 1024, (need, copies, sums)

@@ -8,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_gated import D, gen, gpu, kernel_error, kind_of, planes, within  # noqa: E402,F401
+from test_gpu_gated import D, cells, gen, gpu, kernel_error, kind_of, planes, weights, within  # noqa: E402,F401
 from test_gpu_gated_tails import multiplied  # noqa: E402
 
 WAYS = [(3, 512, 300), (20, 256, 70), (40, 512, 100), (300, 512, 9473), (300, 256, 1000), (800, 256, 2400)]
@@ -48,3 +48,34 @@ def test_large_values_that_meet_no_weight(M, K, F):
         h = D().htile_gated(x, hole, plug, am, F, mode="fast", act=name)
         assert bool((h == 0).all())
     assert kernel_error() == 0
+
+
+@pytest.mark.parametrize("e", [0, 9, 27])
+@pytest.mark.parametrize("M,K,F", WAYS)
+def test_weights_of_small_blocks_keep_their_bits(M, K, F, e):
+    """The only x that is not 0 meets a block whose absmax is 2^-e of the row's largest, twice, so that the two products
+    of each gate all but cancel: what FP16 made of the two weights, 2^-11 of each at most, stands beside a small g.  The
+    sums' own error is (K / 16 + 8) 2^-22 of S = sum |w x| at most (see test_gpu_gated)."""
+    g = gen(M + e)
+    hole, plug, am = planes(2 * F, K, 64, g)
+    am = am.view(2 * F, -1)
+    am[:, 0] = 1.0
+    am[:, 1] = 2.0 ** -e * torch.rand(2 * F, device="cuda", generator=g).add(1)
+    c = cells()
+    one, two = (int((c - v).abs().argmin()) for v in (0.9 + 0.01 * e / 9, 0.6))
+    for col, code in ((64, one), (65, two)):  # a byte: the even column in the low nibble
+        for plane, v in ((hole, code >> 4), (plug, code & 15)):
+            byte = plane.view(2 * F, K // 2)[::2, col // 2]
+            byte.copy_(byte & (0x0F if col % 2 else 0xF0) | (v << 4 if col % 2 else v))
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    by = 2.0 ** e * 2.0 ** (torch.arange(M, device="cuda") % 4)
+    x[:, 64], x[:, 65] = by, -(c[one] / c[two] * by).bfloat16()
+    h = D().htile_gated(x, hole, plug, am.reshape(-1), F, mode="fast")
+    torch.cuda.synchronize()
+    w = weights(hole, plug, am.reshape(-1), 2 * F, K, 64, "f32")
+    y, s = x.double() @ w.T, x.double().abs() @ w.abs().T
+    off = (2.0 ** -11 + (K / 16 + 8) * 2.0 ** -22) * s
+    gate, up, dg, du = y[:, 0::2], y[:, 1::2], off[:, 0::2], off[:, 1::2]
+    assert bool((gate.abs() < 2.0 ** -7 * s[:, 0::2]).all())
+    a = gate * torch.sigmoid(gate)
+    within(h, a * up, 1.13 * dg * (up.abs() + du) + a.abs() * du + (2.0 ** -8 + 2.0 ** -16) * (a * up).abs())
