@@ -75,7 +75,11 @@ int glint_htile_stream(
  * for arguments that the call itself refuses, or where the device does not answer.  In fast mode that is x
  * again and, from 769 rows on, 4 F K bytes for the weight in FP16 (235 MB for 2 x 14336 x 4096).  Sums of shared
  * tiles take up to 39 MB besides with more than 32 rows; with fewer, in either mode, up to 10 MB for K above 8192 or
- * up to 780 F bytes for 2 F above 224 rows an SM (66 MB for 2 x 128256). */
+ * up to 780 F bytes for 2 F above 224 rows an SM (66 MB for 2 x 128256).
+ * Planes and absmax (not x, nor what h and work replace) may be read while the kernel before the call is still
+ * running, if that one lets its successors start early (griddepcontrol.launch_dependents): a kernel that does so
+ * must not be the one that writes them.  No kernel of this library that does writes any; glint_htile_stream asks the same
+ * for up to 32 rows. */
 #define GLINT_ACT_SILU 0
 #define GLINT_ACT_GELU_TANH 1
 typedef struct GlintHtileGated {

@@ -55,3 +55,10 @@ def test_pairs_are_counted_behind_the_kernels_own_limit():
     for kernel in ("htile_gemm_kernel<false>", "htile_gemm_kernel<true>", "gated_wide_kernel", "htile_gemm_precise_kernel<false>",
                    "int8_tc_kernel<false>"):
         assert kernel in body, kernel
+
+
+def test_writers_of_planes_let_nobody_start_early():
+    """htile (to 32 rows) and htile_gated read planes before the kernel ahead of them is done if that one lets its
+    successors start early; what writes planes, scales or K-major copies of them does not."""
+    early = {path.name for path in CSRC.glob("*.cu*") if "griddepcontrol.launch_dependents" in source(path.name)}
+    assert early == {"attn_prompt.cu", "htile_decode.cu", "htile_gated.cu", "kv4_attn.cu"}  # none of which writes any
