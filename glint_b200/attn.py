@@ -271,6 +271,8 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
         freq = freq * (keep + (1 - keep) / of("factor"))
     elif kind == "yarn":
         factor, length = of("factor"), of("original_max_position_embeddings")
+        if base == 1:
+            raise ValueError("rope_type 'yarn' needs a base other than 1")
 
         def number(turns):  # of the frequency that makes so many turns
             return rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -288,13 +290,16 @@ def rope_freqs(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] =
         scale = of("attention_factor", magnitude(of("mscale", 1.0)) / magnitude(of("mscale_all_dim"))
                    if "mscale_all_dim" in scaling else magnitude(1.0))
     elif kind == "longrope":
-        factors = torch.tensor(scaling.get("factors") or [], dtype=torch.float64)
+        factors = torch.as_tensor(scaling.get("factors", []), dtype=torch.float64, device="cpu")
         if factors.shape != freq.shape or not bool((factors > 0).all()):
             raise ValueError(f"'factors' must be {rotary_dim // 2} numbers above 0")
         freq = freq / factors
-        by = of("factor", 1.0)
-        scale = of("attention_factor", math.sqrt(1 + math.log(by) / math.log(of("original_max_position_embeddings")))
-                   if by > 1 else 1.0)
+        by, scale = of("factor", 1.0), of("attention_factor", 1.0)
+        if by > 1 and "attention_factor" not in scaling:
+            length = of("original_max_position_embeddings")
+            if length == 1:
+                raise ValueError("'original_max_position_embeddings' must be above 1")
+            scale = math.sqrt(1 + math.log(by) / math.log(length))
     return freq.float().to(device), scale
 
 

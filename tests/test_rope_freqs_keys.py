@@ -95,3 +95,22 @@ def test_keys_that_change_nothing(kind):
     assert freqs(64, 1e4, {**GOOD[kind], **more}) == want
     with pytest.raises(ValueError, match="rope_theta"):
         freqs(64, 1e4, {**GOOD[kind], "rope_theta": 500000.0})
+
+
+def test_factors_in_a_tensor():
+    factors = [1 + i / 8 for i in range(32)]
+    want = freqs(64, 1e4, dict(rope_type="longrope", factors=factors, factor=4.0, **LENGTH))
+    for f in (torch.tensor(factors), torch.tensor(factors, dtype=torch.float64), tuple(factors)):
+        assert freqs(64, 1e4, dict(rope_type="longrope", factors=f, factor=4.0, **LENGTH)) == want
+    assert freqs(64, 1e4, dict(rope_type="longrope", factors=factors))[1] == 1.0
+    assert freqs(64, 1e4, dict(rope_type="longrope", factors=factors, factor=4.0, attention_factor=1.5))[1] == 1.5
+
+
+def test_sizes_without_a_logarithm():
+    for base, scaling in ((1.0, dict(rope_type="yarn", factor=4.0, **LENGTH)),
+                          (1e4, dict(rope_type="longrope", factors=[1.0] * 32, factor=4.0, original_max_position_embeddings=1))):
+        with pytest.raises(ValueError):
+            freqs(64, base, scaling)
+    for scaling in (dict(rope_type="longrope"), dict(rope_type="longrope", factors=torch.ones(31)), dict(rope_type="longrope", factors=[])):
+        with pytest.raises(ValueError, match="factors"):
+            freqs(64, 1e4, scaling)
