@@ -312,27 +312,29 @@ def _heads_apart(t: torch.Tensor) -> bool:
 
 def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Two [tokens, heads, head_dim] tensors of one type surely share no element: their spans do
-    not meet, or they are different heads of one buffer's tokens, beside one another or in turn."""
-    (T, Ha, D), (sa, ha, _) = a.shape, a.stride()
+    not meet, or they are different heads of one buffer, beside one another or in turn, with either axis the outer one."""
+    (Ta, Ha, D), (sa, ha, _) = a.shape, a.stride()
     (Tb, Hb, _), (sb, hb, _) = b.shape, b.stride()
-    if not (T and Ha and Tb and Hb):
+    if not (Ta and Ha and Tb and Hb):
         return True
-    ea, eb, size = (Ha - 1) * ha + D, (Hb - 1) * hb + D, a.element_size()
-    pa, pb = a.data_ptr(), b.data_ptr()
-    if pa + ((T - 1) * sa + ea) * size <= pb or pb + ((Tb - 1) * sb + eb) * size <= pa:
+    size, pa, pb = a.element_size(), a.data_ptr(), b.data_ptr()
+    if pa + ((Ta - 1) * sa + (Ha - 1) * ha + D) * size <= pb or pb + ((Tb - 1) * sb + (Hb - 1) * hb + D) * size <= pa:
         return True
     if (pb - pa) % size:
         return False
     off = (pb - pa) // size
-    # in turn: of every `turn` places a has the first D and b those from off % turn on
-    turn = ha if Ha > 1 else hb if Hb > 1 else 0
-    if turn and (Ha == 1 or ha == turn) and (Hb == 1 or hb == turn) and (T == 1 or sa % turn == 0) and \
-            (Tb == 1 or sb % turn == 0) and D <= off % turn <= turn - D:
-        return True
-    if sa != sb:
-        return False
-    off = off % sa if sa else 0
-    return ea <= off and off + eb <= sa
+    # counts and strides of the outer and the inner axis of each
+    for na, sa, ma, ra, nb, sb, mb, rb in ((Ta, sa, Ha, ha, Tb, sb, Hb, hb), (Ha, ha, Ta, sa, Hb, hb, Tb, sb)):
+        # beside: of every s places a's inner axis takes the first, b's others
+        s = sa if na > 1 else sb if nb > 1 else 0
+        if s and (na == 1 or sa == s) and (nb == 1 or sb == s) and (ma - 1) * ra + D <= off % s <= s - (mb - 1) * rb - D:
+            return True
+        # in turn: of every r places a has the first D and b those from off % r on
+        r = ra if ma > 1 else rb if mb > 1 else 0
+        if r and (ma == 1 or ra == r) and (mb == 1 or rb == r) and (na == 1 or sa % r == 0) and (nb == 1 or sb % r == 0) and \
+                D <= off % r <= r - D:
+            return True
+    return False
 
 
 def _outputs_apart(q, k, q_out, k_out, more) -> None:

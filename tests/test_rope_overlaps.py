@@ -61,3 +61,18 @@ def test_every_answer_apart_is_right():
                 said += 1
                 assert not pa & pb, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
     assert said > 10000
+
+
+def test_heads_outermost():
+    """[heads, 3, tokens, head_dim] and [heads, tokens, 3, head_dim] buffers, seen as [tokens, heads, head_dim]."""
+    for T, H in ((5, 4), (1, 4), (5, 1)):
+        for y in (torch.zeros(H, 3, T, 64, dtype=torch.bfloat16).permute(2, 0, 1, 3),
+                  torch.zeros(H, T, 3, 64, dtype=torch.bfloat16).permute(1, 0, 2, 3)):
+            q, k, v = (y[:, :, i] for i in range(3))
+            apart(q, k, q, k, (v,))
+            for bad in (k, v):
+                with pytest.raises(ValueError):
+                    apart(q, k, bad, None, (v,))
+        y = torch.zeros(2 * H, T, 64, dtype=torch.bfloat16).transpose(0, 1)
+        apart(y[:, ::2], y[:, 1::2], y[:, ::2], y[:, 1::2], ())
+        apart(y[:, :H], y[:, H:], y[:, :H], y[:, H:], ())
