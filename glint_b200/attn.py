@@ -428,8 +428,8 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, in
     inv_freq [half] f32 (rope_freqs): 2 * half <= head_dim values of a head are rotated, the pairs (i, i +
     half), or (2i, 2i + 1) with interleaved, by position * inv_freq[i]; the others stay.  scale multiplies cos
     and sin.  q_norm, k_norm [head_dim] f32: each head is divided by sqrt(mean of squares + eps) and
-    multiplied by these first.  q_out and k_out may be q and k themselves (any other overlap is
-    refused); left out, they are new and contiguous."""
+    multiplied by these first.  q_out may be q itself and k_out k (any other overlap
+    with an input or one another is refused); left out, they are new and contiguous."""
     a, raw, q_out, k_out = _rope(q, k, positions, inv_freq, interleaved, scale, q_norm, k_norm, eps, q_out, k_out, stream,
                                  (), True)
     _check(_c().rope(a, raw), "glint_rope_stream")

@@ -13,11 +13,13 @@
  * 25 for 8191 x 4096), beside which the next kernel's weights stream or are expanded.
  *
  * Three ways, at 4096 x 2 x 14336 (us; memory's floor 19.5, the tensor cores' 0.145 a row in a burst):
- *   1 to 32 rows    the decode kernels, lookups straight into mma.sync: 35.9 for a row, 62.7 for 32 (the second 65.6
+ *   1 to 32 rows    the decode kernels, lookups straight into mma.sync: 35.9 for a row, 63.3 for 32 (the second 67.5
  *                   for 33)
- *   from there      the tcgen05 product from planes: 66 for 64 rows, 81 for 256, 135 for 511
- *   from 769 rows, unless there are fewer tiles than CTA pairs, weights expanded first: 231 for 900 (the second
- *                   262), 391 for 2048 (483), 1330 to 1515 for 8191, as the clock goes (2246)
+ *   from there      the tcgen05 product from planes: 68 for 64 rows, 81 for 256, 135 for 511
+ *   from 769 rows, unless there are fewer tiles than CTA pairs, weights expanded first: 226 to 231 for 900 (the
+ *                   second 262), 381 to 391 for 2048 (483), 1330 to 1515 for 8191, as the clock goes (2246)
+ * Precise mode takes the first two ways with x as it is: 37.4 us for a row (the pass is not there), 78.5 for 32, 126
+ * for 64, 421 for 511, 5745 for 8191.
  */
 #include <cuda_fp16.h>
 

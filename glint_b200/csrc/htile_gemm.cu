@@ -1990,7 +1990,7 @@ int gemm_plan(GemmArgs &a, bool gated = false)
     if (gated && tiles * 2 <= maxp) {
         /* No tile for half of the pairs: K is cut for all tiles, down to one group a pair, and gated_join_kernel adds.
          * Uncut and cut: 98 x 6656 x 2 x 174 (2 tiles) 63 and 30 us; 64 x 4096 x 2 x 4096 (32 tiles) 45 and 36;
-         * 40 x 1024 x 2 x 2000 (16 tiles, 4 groups) 21.5 and 20.2.  Above half, 250 x 4096 x 2 x 6912 (54 tiles)
+         * 40 x 1024 x 2 x 2000 (16 tiles, 4 groups) 21.5 and 20.2 (cut and started early: 20, 32 and 16).  Above half, 250 x 4096 x 2 x 6912 (54 tiles)
          * 48 and 56, 200 x 2048 x 2 x 5000 (40 tiles) 31 and 34. */
         a.tiles = a.S = tiles, a.R = 0, a.U = tiles * a.G, a.join = 1;
         return a.P = std::min(maxp, a.U);

@@ -366,7 +366,8 @@ unsigned generic_grid(int64_t items)
 } // namespace
 
 /* act(gate) * up of rows 2i and 2i + 1 for the shapes that the TMA kernels do not take, with both halves of
- * each cell in either mode */
+ * each cell in either mode.  Every 32 rows of x read and look up all weights again: 2880 x 2 x 2880 16 us for a row, 32 for
+ * 32, 502 for 511; blocks of 32 or odd addresses, an output a warp, 4096 x 2 x 14336 569 us for a row. */
 int htile_gemv_gated_launch(const uint8_t *hole, const uint8_t *plug, const float *am, const __nv_bfloat16 *x, void *h,
                             int M, int N, int K, int bs, int act, cudaStream_t st)
 {

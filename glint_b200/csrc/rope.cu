@@ -21,7 +21,8 @@
  * Bytes bound it: q and k read and written once, v read, codes written.  32768 tokens, 32 / 8 heads of 128,
  * norms: 124 us, 5.4 TB/s where a copy reaches 6.4 (its floor 105); 16383 tokens into the cache 89 us of 61, the
  * quantisation's shuffles and conversions in the way; few tokens are launch and latency: 1 token 2.6 us, 513
- * 4.7, 7 into the cache 3.6.  CTAs of 4 warps, 6 an SM (5 with the cache): of 8 warps 127 to 150 us for the 124, more
+ * 4.7, 7 into the cache 3.6.  Partners that are no runs of 8, through shared memory: 32768 tokens (no norms, 122 us with
+ * runs) 261 us; operands at odd addresses, value by value, 302, both 638, side by side 940.  CTAs of 4 warps, 6 an SM (5 with the cache): of 8 warps 127 to 150 us for the 124, more
  * CTAs with fewer registers 154.
  */
 #include <cuda_runtime.h>
